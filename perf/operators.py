@@ -15,11 +15,11 @@ TYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
 def listed():
     return [
         # eight rows of a small decoder fork in the middle of a page: launches
-        dict(name="pages_fork_small", kind="pages", layers=4, pages=64, page=16, heads=4, dim=64, copies=8, times=4, rows=16, columns=8, entries=64, dtype="bf16"),
+        dict(name="pages_fork_small", kind="pages", layers=4, pages=64, page=16, heads=4, dim=64, copies=8, times=4, rows=16, columns=8, changed=8, dtype="bf16"),
         # a batch of rollouts forks: every sample gets a last page of its own in sixteen layers of the dense 8 B configuration
-        dict(name="pages_fork_rollouts", kind="pages", layers=16, pages=256, page=64, heads=8, dim=128, copies=112, times=7, rows=128, columns=64, entries=4000, dtype="bf16"),
+        dict(name="pages_fork_rollouts", kind="pages", layers=16, pages=256, page=64, heads=8, dim=128, copies=112, times=7, rows=128, columns=64, changed=112, dtype="bf16"),
         # the server's default pages of 16 tokens moved to the front of their pool, and the tables that named them
-        dict(name="pages_compact", kind="pages", layers=24, pages=4096, page=16, heads=2, dim=64, copies=1500, times=1, rows=256, columns=64, entries=1500, dtype="bf16"),
+        dict(name="pages_compact", kind="pages", layers=24, pages=4096, page=16, heads=2, dim=64, copies=1500, times=1, rows=256, columns=64, changed=100, dtype="bf16"),
         # four samples of one prompt, a decoder of width 1024: latency
         dict(name="prefix_small", kind="prefix", rows=4, groups=1, shared=448, shared_to=448, apart=1, apart_to=60, heads=8, kv=4, dim=128, page=64, window=0, softcap=0.0, sinks=False,
              resting=0, dtype="bf16"),
@@ -61,7 +61,7 @@ def draw(rng):
         copies = _log(rng, 1, pages // 3)
         rows, columns = _log(rng, 1, 256), _log(rng, 1, 128)
         return dict(kind=kind, layers=layers, pages=pages, page=page, heads=heads, dim=dim, copies=copies, times=rng.choice((1, 1, 3, 8)), rows=rows, columns=columns,
-                    entries=rng.randint(0, min(rows * columns, 4000)), dtype=dtype)
+                    changed=rng.randint(0, min(rows, 8000 // columns)), dtype=dtype)
     if kind == "prefix":
         plain = rng.random() < 0.75
         rows = _log(rng, 1, 128 if plain else 32)
@@ -108,9 +108,12 @@ def _prepare_pages(case, seed):
     # a page is copied `times` times; what is written is written once, and not read
     src = order[n:][torch.arange(n) // case["times"]]
     table = torch.randint(case["pages"], (case["rows"], case["columns"]), generator=g, device=DEV, dtype=torch.int32)
-    places = torch.randperm(case["rows"] * case["columns"], generator=h)[:case["entries"]]
-    entries = torch.stack([places // case["columns"], places % case["columns"], torch.randint(case["pages"], (len(places),), generator=h)], 1)
-    return dict(kind="pages", k=k, v=v, table=table, copies=torch.stack([src, order[:n]], 1).tolist(), entries=entries.tolist())
+    # pieces of rows' tables: (row, first column, pages)
+    each = (case["columns"] + 1) // 2
+    named = torch.randint(case["pages"], (case["changed"], each), generator=h).tolist()
+    first = torch.randint(case["columns"] - each + 1, (case["changed"],), generator=h).tolist()
+    tables = list(zip(torch.randperm(case["rows"], generator=h).tolist(), first, named))
+    return dict(kind="pages", k=k, v=v, table=table, src=src.tolist(), dst=order[:n].tolist(), tables=tables)
 
 
 def _prepare_prefix(case, seed):
@@ -173,14 +176,14 @@ def _run_pages(s):
     k, v, table = s["k"], s["v"], s["table"]
     if own:
         from dew_b200.ops import pages
-        pages.move_pages([k, v], s["copies"], table, s["entries"])
+        pages.move_pages([k, v], s["src"], s["dst"], table, s["tables"])
     else:
-        src, dst = torch.tensor(s["copies"], device=DEV).unbind(1)
+        src, dst = torch.tensor([s["src"], s["dst"]], device=DEV)
         k[:, dst] = k[:, src]
         v[:, dst] = v[:, src]
-        if s["entries"]:
-            row, column, page = torch.tensor(s["entries"], device=DEV).unbind(1)
-            table[row, column] = page.int()
+        if s["tables"]:
+            row, first, pages = (torch.tensor(x, device=DEV) for x in zip(*s["tables"]))
+            table[row[:, None], first[:, None] + torch.arange(pages.shape[1], device=DEV)] = pages.int()
     return {"k": k, "v": v, "table": table}
 
 
@@ -226,7 +229,7 @@ def _run_adapters(s):
 def work(case):
     if case["kind"] == "pages":
         size = case["layers"] * case["page"] * case["heads"] * case["dim"] * (4 if case["dtype"] == "fp32" else 2)
-        return {"bytes": 2 * size * (-(-case["copies"] // case["times"]) + case["copies"]) + 4 * case["entries"], "flops": 0}
+        return {"bytes": 2 * size * (-(-case["copies"] // case["times"]) + case["copies"]) + 4 * case["changed"] * ((case["columns"] + 1) // 2), "flops": 0}
     size = 4 if case["dtype"] == "fp32" else 2
     if case["kind"] == "prefix":
         sizes, shared, apart = _lengths(case)
@@ -247,11 +250,12 @@ def exact(case, seed):
     s = prepare(case, seed)
     if case["kind"] == "pages":
         comes_from = torch.arange(case["pages"])
-        for src, dst in s["copies"]:
+        for src, dst in zip(s["src"], s["dst"]):
             comes_from[dst] = src
         table = s["table"].clone().cpu()
-        for row, column, page in s["entries"]:
-            table[row, column] = page
+        for row, first, pages in s["tables"]:
+            for i, page in enumerate(pages):
+                table[row, first + i] = page
         return {"k": s["k"].double().index_select(1, comes_from.to(DEV)), "v": s["v"].double().index_select(1, comes_from.to(DEV)), "table": table}
     if case["kind"] == "prefix":
         return _exact_prefix(s)
