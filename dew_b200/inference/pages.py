@@ -30,6 +30,14 @@ class Seat:
     reused_tokens: int          # prompt tokens already present in re-used pages (need no prefill)
 
 
+@dataclass
+class Fork:
+    """Pages of a row that begins with another row's tokens: whole pages are shared, ``src`` (that row's last, partly filled page) is to be copied to ``dst``."""
+    pages: List[int]
+    src: List[int]
+    dst: List[int]
+
+
 class HostTier:
     """Evicted prefix pages kept in pinned host memory: when the device pool takes back a cached page, its keys and values (every
     layer's) are copied to a host slot under the page's chain hash; a later prompt with that prefix copies them back into a fresh
@@ -161,6 +169,62 @@ class PageLedger:
             self.refs[p] = 1
         pages.extend(added)
         return added
+
+    def fork(self, pages: Sequence[int], tokens: int, total_tokens: int) -> Fork:
+        """Pages for a row of ``total_tokens`` that begins with the ``tokens`` a row of ``pages`` holds.  What both write from here on is theirs alone: a page that those tokens
+        do not fill is copied."""
+        whole, rest = divmod(tokens, self.page_size)
+        if tokens < 0 or total_tokens < tokens or len(pages) * self.page_size < tokens:
+            raise ValueError(f"a row of {len(pages)} pages cannot be forked at {tokens} of {total_tokens} tokens")
+        need = (total_tokens + self.page_size - 1) // self.page_size - whole
+        if need > self.available():
+            raise OutOfPages(f"need {need} pages, {self.available()} available")
+        shared = list(pages[:whole])
+        if any(p not in self.refs for p in pages[:whole + (rest > 0)]):
+            raise ValueError("a row can be forked while its pages are its own: these have been given back")
+        for p in shared:
+            self.refs[p] += 1
+        own = [self._take() for _ in range(need)]
+        for p in own:
+            self.refs[p] = 1
+        return Fork(shared + own, [pages[whole]] if rest else [], own[:1] if rest else [])
+
+    def truncate(self, pages: List[int], tokens: int) -> List[int]:
+        """Give back the pages of a row (in place) that its first ``tokens`` do not need; returns them."""
+        keep = (max(0, tokens) + self.page_size - 1) // self.page_size
+        dropped = pages[keep:]
+        del pages[keep:]
+        self.release(dropped)
+        return dropped
+
+    def compact(self) -> Dict[int, int]:
+        """Rename the pages in use (and the cached ones) so that they are the pool's first, and return ``{old: new}`` of those that move.  The caller copies their contents and
+        puts the new names into its rows' lists and tables."""
+        held = sorted(set(self.refs) | set(self.idle))
+        holes = iter(sorted(set(range(len(held))) - set(held)))
+        moved = {p: next(holes) for p in held if p >= len(held)}
+        if moved:
+            name = lambda p: moved.get(p, p)
+            self.refs = {name(p): n for p, n in self.refs.items()}
+            self.name_of = {name(p): h for p, h in self.name_of.items()}
+            self.page_of = {h: name(p) for h, p in self.page_of.items()}
+            self.idle = OrderedDict((name(p), None) for p in self.idle)
+        self.free = list(range(self.pages - 1, len(held) - 1, -1))
+        return moved
+
+    def resize(self, pages: int) -> None:
+        """Another number of pages.  Those in use have to be among the first ``pages`` (``compact``)."""
+        if any(p >= pages for p in (*self.refs, *self.idle)):
+            raise ValueError(f"pages past {pages} are in use")
+        self.pages = pages
+        self.free = [p for p in range(pages - 1, -1, -1) if p not in self.refs and p not in self.idle]
+
+    def evict(self, most: int) -> None:
+        """Give up cached pages, the least recently released first, until at most ``most`` pages are held."""
+        while self.idle and len(self.refs) + len(self.idle) > most:
+            kept, self.free = self.free, []
+            kept.append(self._take())                            # (of the cached pages: the free ones are out of sight)
+            self.free = kept
 
     def publish(self, prompt: Sequence[int], pages: Sequence[int]) -> None:
         """After a prompt's prefill: name its full pages so later requests can re-use them."""

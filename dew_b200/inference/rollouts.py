@@ -43,6 +43,12 @@ class RolloutServer:
     def submit(self, prompt: Sequence[int], max_new_tokens: int, *, key: int = 0, sampling: Optional[Sampling] = None) -> "Future[Draw]":
         raise NotImplementedError
 
+    def submit_group(self, prompt: Sequence[int], n: int, max_new_tokens: int, *, keys: Optional[Sequence[int]] = None,
+                     sampling: Optional[Sampling] = None) -> "List[Future[Draw]]":
+        """``n`` draws of one prompt, as a group-relative objective wants them."""
+        keys = list(range(n)) if keys is None else list(keys)
+        return [self.submit(prompt, max_new_tokens, key=k, sampling=sampling) for k in keys]
+
     def load(self, variables: Any, version: int) -> None:
         raise NotImplementedError
 
@@ -83,6 +89,17 @@ class NativeRolloutServer(RolloutServer):
             self._lock.notify_all()
         return fut
 
+    def submit_group(self, prompt, n, max_new_tokens, *, keys=None, sampling=None):
+        """The prompt is read once and the draws fork from it (``Server.submit_group``)."""
+        keys = list(range(n)) if keys is None else [int(k) for k in keys]
+        if n < 1 or len(keys) != n or not len(prompt):
+            raise ValueError(f"{n} draws with {len(keys)} keys of a prompt of {len(prompt)} tokens")
+        with self._lock:
+            futures = [self.submit(prompt, max_new_tokens, key=k, sampling=sampling) for k in keys]
+            tickets = [entry[0] for entry in self._incoming[-n:]]
+            tickets[0].waiting = tickets[1:]
+        return futures
+
     def load(self, variables, version: int) -> None:
         """Queue a weight swap; it is applied between two server steps.  Versions must not go backwards."""
         with self._lock:
@@ -113,9 +130,11 @@ class NativeRolloutServer(RolloutServer):
                 if load is not None:
                     self.server.reload(load[0])
                     resident = load[1]
+                forked = {id(w) for ticket, _, _ in incoming for w in ticket.waiting}
                 for ticket, fut, version in incoming:
                     ticket.submitted = self.server.clock()
-                    self.server.queue.append(ticket)
+                    if id(ticket) not in forked:
+                        self.server.queue.append(ticket)
                     self._live.append((ticket, fut, version))
                 if self.server.busy:
                     self.server.step()

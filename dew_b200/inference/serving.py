@@ -36,6 +36,7 @@ class Ticket:
     done: bool = False
     terminated: bool = False
     error: Optional[BaseException] = None
+    waiting: List["Ticket"] = field(default_factory=list, repr=False)      # samples of the same prompt that fork from this one's row when it has been read
 
     def result(self) -> List[int]:
         if self.error is not None:
@@ -116,6 +117,42 @@ class Server:
         self.queue.append(t)
         return t
 
+    def submit_group(self, prompt, n: int, max_new_tokens: int, keys: Optional[Sequence[int]] = None, sampling: Optional[Sampling] = None, on_token=None) -> List[Ticket]:
+        """``n`` samples of one prompt, which is read once: the other rows fork from the first when it has been (whole pages are shared, a last page that is partly filled is
+        copied).  What finds no slot or pages then is seated like any other request.  ``keys``: a key for each, 0 .. n - 1 by default."""
+        keys = list(range(n)) if keys is None else [int(k) for k in keys]
+        if n < 1 or len(keys) != n:
+            raise ValueError(f"{n} samples with {len(keys)} keys")
+        first = self.submit(prompt, max_new_tokens, keys[0], sampling, on_token)
+        if not first.prompt:
+            self.queue.pop()
+            raise ValueError("a group of samples needs a prompt of one token or more")
+        first.waiting = [Ticket(first.prompt, max_new_tokens, k, sampling, on_token, submitted=first.submitted) for k in keys[1:]]
+        return [first, *first.waiting]
+
+    def compact(self) -> int:
+        """Move the pages in use to the front of the pool; returns how many moved.  Between two steps."""
+        moved = self.ledger.compact()
+        if moved:
+            tables = []
+            for slot, r in enumerate(self.rows):
+                if r is not None and any(p in moved for p in r.pages):
+                    r.pages = [moved.get(p, p) for p in r.pages]
+                    tables.append((slot, 0, r.pages))
+            self.store.move_pages(list(moved), list(moved.values()), tables)
+        return len(moved)
+
+    def resize(self, pages: int) -> None:
+        """A pool of another number of pages: what rollouts give back to training between rounds, and take again.  Cached pages are given up where they do not fit; pages in use
+        have to.  Between two steps; the decode step is captured again."""
+        if pages < len(self.ledger.refs):
+            raise OutOfPages(f"{len(self.ledger.refs)} pages are in use, {pages} are left")
+        self.ledger.evict(pages)
+        self.compact()
+        self._graph = None
+        self.store.resize(pages)
+        self.ledger.resize(pages)
+
     @property
     def occupancy(self) -> int:
         return sum(r is not None for r in self.rows)
@@ -129,11 +166,10 @@ class Server:
         return self.occupancy > 0 or bool(self.queue) or self._pending is not None
 
     def fail(self, exc: BaseException) -> None:
-        for r in self.rows:
-            if r is not None:
-                r.ticket.error, r.ticket.done = exc, True
-        for t in self.queue:
-            t.error, t.done = exc, True
+        for t in [r.ticket for r in self.rows if r is not None] + list(self.queue):
+            for each in (t, *t.waiting):
+                each.error, each.done = exc, True
+            t.waiting = []
         self.queue.clear()
         self.rows = [None] * self.slots
 
@@ -234,6 +270,34 @@ class Server:
                     tok = self._draw(last_logits[i][None], r, 0)
                     self.last_tokens[s] = tok
                     r.pending_first = True
+                    if r.ticket.waiting:
+                        self._fork(s, r, last_logits[i][None])
+
+    def _fork(self, slot: int, row: _Row, logits: torch.Tensor) -> None:
+        """The samples that wait for ``row``'s prompt take free slots with its pages; each draws its first token from the same ``logits``."""
+        waiting, row.ticket.waiting = row.ticket.waiting, []
+        src, dst, tables, children = [], [], [], []
+        for child in (s for s in range(self.slots) if self.rows[s] is None):
+            if not waiting:
+                break
+            t = waiting[0]
+            try:
+                fork = self.ledger.fork(row.pages, len(t.prompt), len(t.prompt) + t.max_new_tokens)
+            except OutOfPages:
+                break
+            waiting.pop(0)
+            src += fork.src
+            dst += fork.dst
+            tables.append((child, 0, fork.pages))
+            children.append(child)
+            self.rows[child] = _Row(t, fork.pages, prefilled=len(t.prompt), pending_first=True)
+        self.queue.extendleft(reversed(waiting))
+        if not children:
+            return
+        self.store.move_pages(src, dst, tables)
+        self.store.fork_rows([slot] * len(children), children)
+        for child in children:
+            self.last_tokens[child] = self._draw(logits, self.rows[child], 0)
 
     def _draw(self, logits: torch.Tensor, row: _Row, step: int) -> torch.Tensor:
         s = row.ticket.sampling or self.sampling

@@ -23,6 +23,7 @@ from ..ops import latent as M
 from ..ops import library as L
 from ..ops import paged as P
 from ..ops import rotary, token_mix
+from ..ops.pages import move_pages
 
 LIMITS = {"int8": 127.0, "float8_e4m3fn": 448.0}
 KINDS = {None: 0, "int8": 1, "float8_e4m3fn": 2}
@@ -346,6 +347,56 @@ class KVStore:
         buf = self.latent(layer, width)
         rows = self._rows(self.rows if self.row_ids is None else self.row_ids.numel())
         return buf[rows, :length]
+
+    # ------------------------------------------------------------------ pages that move
+    def pools(self) -> List[torch.Tensor]:
+        """Every tensor that a page has a share of, as ``[layers, pages, ...]`` without the spare page."""
+        if self.slots is None:
+            found = [self.k, self.v] + ([self.k_scale, self.v_scale] if self.kind else [])
+        else:
+            found = list({t.data_ptr(): t[None] for i, s in enumerate(self.slots) if s.source is None for t in (self.k[i], self.v[i]) if t is not None}.values())
+        return [t[:, :self.pages] for t in found]
+
+    def move_pages(self, src: Sequence[int], dst: Sequence[int], tables: Sequence[Tuple[int, int, Sequence[int]]] = ()) -> None:
+        """Copy pages ``src`` to ``dst`` in every layer, and write the pieces ``(row, first column, pages)`` of the page table, in one launch (``ops.pages``)."""
+        pools = self.pools()
+        if pools:
+            move_pages(pools, src, dst, self.page_table, tables)
+
+    def resize(self, pages: int) -> None:
+        """Pools of another number of pages (a graph that was captured over the old ones has to be captured again).  What the first pages hold stays; what the table names past
+        the end, the caller has moved (``move_pages``) or does not need."""
+        if pages < 1:
+            raise ValueError(f"a cache of {pages} pages")
+        kept = min(pages, self.pages)
+
+        def sized(t: torch.Tensor, axis: int) -> torch.Tensor:
+            shape = list(t.shape)
+            shape[axis] = pages + 1
+            new = t.new_ones(shape) if t is self.k_scale or t is self.v_scale else t.new_zeros(shape)
+            new.narrow(axis, 0, kept).copy_(t.narrow(axis, 0, kept))
+            return new
+        if self.slots is None:
+            for name in ("k", "v", "k_scale", "v_scale"):
+                if getattr(self, name) is not None:
+                    setattr(self, name, sized(getattr(self, name), 1))
+        else:
+            # (layers that read another's keys and values, and latent rows, name one pool several times)
+            for old in [t for pools in (self.k, self.v) for t in pools if t is not None]:
+                if not any(old is t for pools in (self.k, self.v) for t in pools):
+                    continue
+                new = sized(old, 0)
+                self.k, self.v = ([new if t is old else t for t in pools] for pools in (self.k, self.v))
+        self.pages = pages
+
+    def fork_rows(self, parents: Sequence[int], children: Sequence[int]) -> None:
+        """Give rows ``children`` what rows ``parents`` keep beside their pages (recurrent states, latents): the same list of parents may name a row several times."""
+        for row in (*parents, *children):
+            if not 0 <= row < self.rows:
+                raise ValueError(f"row {row} of a cache of {self.rows}")
+        kept = [t[None] for t in self.kept_states()] + [t[None] for t in self.__dict__.get("_latent", {}).values()]
+        if kept and len(children):
+            move_pages(kept, parents, children)
 
     # ------------------------------------------------------------------ addressing
     def select(self, row_ids: Optional[torch.Tensor]) -> "KVStore":

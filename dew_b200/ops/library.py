@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+from contextlib import contextmanager
 from pathlib import Path
 from typing import Dict, Optional
 
@@ -160,6 +161,24 @@ def ensure_device(t: torch.Tensor) -> None:
     if getattr(_TLS, "device", None) != idx:
         check(load().dewb_set_device(ctypes.c_int(idx)), "set_device")
         _TLS.device = idx
+
+
+@contextmanager
+def on_device_of(t: torch.Tensor):
+    """``t``'s device current, for torch and for the library, while a launch is issued; yields its current stream.  (``use_cuda`` alone is enough where the caller has made the
+    device current.)"""
+    idx = t.get_device()
+    if idx == torch._C._cuda_getDevice():
+        ensure_device(t)
+        yield torch._C._cuda_getCurrentRawStream(idx)
+        return
+    with torch.cuda.device(idx):
+        _TLS.device = None
+        ensure_device(t)
+        try:
+            yield torch._C._cuda_getCurrentRawStream(idx)
+        finally:
+            _TLS.device = None
 
 
 def stream() -> int:
