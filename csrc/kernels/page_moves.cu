@@ -93,14 +93,13 @@ __global__ void __launch_bounds__(THREADS) move_pages_kernel(const __grid_consta
   }
 }
 
-// One launch: copies [c0, c1) of the pools [p0, p1) and the entries [e0, e1) of the table, counted through the spans' pages.
+// One launch: copies [c0, c1) of the pools [p0, p1), and the next `entries` of the table: `pages`, in span s from its `done`-th entry on and in those behind it.
 template <int N>
-int launch(const Pool* pools, int p0, int p1, const int* src, const int* dst, int c0, int c1, int* table, const int* at, const int* begin, const int* pages, int s0, int s1,
-           int e0, int e1, cudaStream_t stream) {
+int launch(const Pool* pools, int p0, int p1, const int* src, const int* dst, int c0, int c1, int* table, int columns, const int* row, const int* first, const int* length,
+           const int* pages, int s, int done, int entries, cudaStream_t stream) {
   Moves<N> m;
   m.pools = p1 - p0;
   m.copies = c1 - c0;
-  m.spans = s1 - s0;
   m.table = table;
   long long blocks = 0;
   for (int i = 0; i < m.pools; ++i) {
@@ -114,11 +113,21 @@ int launch(const Pool* pools, int p0, int p1, const int* src, const int* dst, in
   int* to = m.data;
   for (int c = c0; c < c1; ++c) *to++ = src[c];
   for (int c = c0; c < c1; ++c) *to++ = dst[c];
-  for (int s = s0; s < s1; ++s) *to++ = at[s] + (begin[s] < e0 ? e0 - begin[s] : 0);
-  for (int s = s0; s < s1; ++s) *to++ = begin[s] < e0 ? 0 : begin[s] - e0;
-  *to++ = e1 - e0;
-  for (int e = e0; e < e1; ++e) *to++ = pages[e];
-  blocks += (e1 - e0 + THREADS - 1) / THREADS;
+  m.spans = 0;
+  for (int e = 0, i = s, d = done; e < entries; ++i, d = 0)
+    if (length[i] > d) {
+      *to++ = row[i] * columns + first[i] + d;
+      e += length[i] - d;
+      ++m.spans;
+    }
+  for (int e = 0, i = s, d = done; e < entries; ++i, d = 0)
+    if (length[i] > d) {
+      *to++ = e;
+      e += length[i] - d;
+    }
+  *to++ = entries;
+  for (int e = 0; e < entries; ++e) *to++ = pages[e];
+  blocks += (entries + THREADS - 1) / THREADS;
   if (blocks == 0) return 0;
   move_pages_kernel<N><<<static_cast<int>(blocks), THREADS, 0, stream>>>(m);
   return static_cast<int>(cudaGetLastError());
@@ -136,8 +145,9 @@ int by_from(const void* a, const void* b) {
 }  // namespace
 
 // What is wrong with the copies and spans: 0 nothing, -11 a page outside the pool, -12 a page written twice, -13 a page read and written, -14 an entry outside the table,
-// -15 no memory to look, -16 an entry written twice.  Host only.  `begin` has spans + 1 places in `pages`.
-extern "C" int dewb_check_moves(const int* src, const int* dst, int copies, int pages_in_pool, const int* at, const int* begin, const int* pages, int spans, long long entries) {
+// -15 no memory to look, -16 an entry written twice.  Host only.  Span s writes length[s] entries of row[s] from column first[s] on.
+extern "C" int dewb_check_moves(const int* src, const int* dst, int copies, int pages_in_pool, const int* row, const int* first, const int* length, const int* pages, int spans,
+                                int rows, int columns) {
   if (copies < 0 || spans < 0 || pages_in_pool < 0) return -3;
   unsigned char* seen = static_cast<unsigned char*>(std::calloc(pages_in_pool > 0 ? pages_in_pool : 1, 1));
   if (seen == nullptr) return -15;
@@ -150,69 +160,73 @@ extern "C" int dewb_check_moves(const int* src, const int* dst, int copies, int 
   for (int i = 0; i < copies && rc == 0; ++i)
     if (seen[src[i]]) rc = -13;
   std::free(seen);
+  long long n = 0;
   for (int s = 0; s < spans && rc == 0; ++s) {
-    if (begin[s + 1] < begin[s] || at[s] < 0 || static_cast<long long>(at[s]) + (begin[s + 1] - begin[s]) > entries) rc = -14;
-    for (int e = begin[s]; e < begin[s + 1] && rc == 0; ++e)
-      if (pages[e] < 0 || pages[e] >= pages_in_pool) rc = -11;
+    if (length[s] < 0 || row[s] < 0 || row[s] >= rows || first[s] < 0 || first[s] > columns - length[s]) { rc = -14; break; }
+    for (int e = 0; e < length[s] && rc == 0; ++e)
+      if (pages[n + e] < 0 || pages[n + e] >= pages_in_pool) rc = -11;
+    n += length[s];
   }
   if (rc != 0 || spans < 2) return rc;
+  if (n > 0x7fffffffll) return -3;
   Ends* ends = static_cast<Ends*>(std::malloc(sizeof(Ends) * spans));
   if (ends == nullptr) return -15;
-  int n = 0;
+  int used = 0;
   bool sorted = true;
   for (int s = 0; s < spans; ++s) {
-    if (begin[s + 1] == begin[s]) continue;
-    ends[n] = {at[s], static_cast<long long>(at[s]) + (begin[s + 1] - begin[s])};
-    sorted = sorted && (n == 0 || ends[n - 1].from <= ends[n].from);
-    ++n;
+    if (length[s] == 0) continue;
+    const long long at = static_cast<long long>(row[s]) * columns + first[s];
+    ends[used] = {at, at + length[s]};
+    sorted = sorted && (used == 0 || ends[used - 1].from <= at);
+    ++used;
   }
-  if (!sorted) std::qsort(ends, n, sizeof(Ends), by_from);
-  for (int i = 1; i < n && rc == 0; ++i)
+  if (!sorted) std::qsort(ends, used, sizeof(Ends), by_from);
+  for (int i = 1; i < used && rc == 0; ++i)
     if (ends[i].from < ends[i - 1].to) rc = -16;
   std::free(ends);
   return rc;
 }
 
-// `pools`: layers x pages_in_pool pages of page_bytes each, one behind another within a layer; `table`: int32 [entries].  All lists are the host's and are read before this
-// returns.  One launch for up to 32 pools and what fits the parameters, more where there is more.  `launches` counts them.
-extern "C" int dewb_move_pages(const void* pools_ptr, int pools, int pages_in_pool, const int* src, const int* dst, int copies, int* table, long long entries, const int* at,
-                               const int* begin, const int* pages, int spans, int* launches, void* stream_ptr) {
+// `pools`: layers x pages_in_pool pages of page_bytes each, one behind another within a layer; `table`: int32 [rows, columns].  All lists are the host's and are read before
+// this returns.  One launch for up to 32 pools and what fits the parameters, more where there is more.  `launches` counts them.
+extern "C" int dewb_move_pages(const void* pools_ptr, int pools, int pages_in_pool, const int* src, const int* dst, int copies, int* table, int rows, int columns, const int* row,
+                               const int* first, const int* length, const int* pages, int spans, int* launches, void* stream_ptr) {
   using namespace dewb::pagemoves;
   *launches = 0;
   const Pool* pool = static_cast<const Pool*>(pools_ptr);
-  int rc = dewb_check_moves(src, dst, copies, pages_in_pool, at, begin, pages, spans, entries);
+  int rc = static_cast<long long>(rows) * columns > 0x7fffffffll ? -3 : dewb_check_moves(src, dst, copies, pages_in_pool, row, first, length, pages, spans, rows, columns);
   if (rc != 0) return rc;
   for (int i = 0; i < pools; ++i)
     if (pool[i].layers < 0 || pool[i].page_bytes < 0) return -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  // the table's entries go with the first launch that has room for them: spans [s, ...) and entries [e, ...) are still to be written
-  const int last = spans > 0 ? begin[spans] : 0;
-  int s = 0, e = 0, p = 0, c = 0;
+  // the table's entries go with the first launch that has room for them: span s, of which `done` entries are written, comes next, and its pages begin at `named`
+  int s = 0, done = 0, p = 0, c = 0;
+  long long named = 0;
   bool copying = copies > 0 && pools > 0;
-  while (copying || e < last) {
+  while (s < spans && length[s] == 0) ++s;
+  while (copying || s < spans) {
     int p1 = p, c1 = c, room = MANY - 1;
     if (copying) {
       p1 = pools - p < MOST_POOLS ? pools : p + MOST_POOLS;
       c1 = copies - c < room / 2 ? copies : c + room / 2;
       room -= 2 * (c1 - c);
     }
-    int s1 = s, e1 = e;
-    while (s1 < spans && e1 < last && room > 2) {
-      room -= 2;
-      const int end = begin[s1 + 1], take = end - e1 < room ? end - e1 : room;
-      room -= take;
-      e1 += take;
-      if (e1 < end) { ++s1; break; }
-      ++s1;
+    const int s0 = s, done0 = done;
+    const long long named0 = named;
+    while (s < spans && room > 2) {
+      const int take = length[s] - done < room - 2 ? length[s] - done : room - 2;
+      room -= 2 + take;
+      done += take;
+      named += take;
+      if (done < length[s]) break;
+      done = 0;
+      do ++s; while (s < spans && length[s] == 0);
     }
-    const int used = 2 * (c1 - c) + 2 * (s1 - s) + 1 + (e1 - e);
-    rc = used <= FEW ? launch<FEW>(pool, p, p1, src, dst, c, c1, table, at, begin, pages, s, s1, e, e1, stream)
-                     : launch<MANY>(pool, p, p1, src, dst, c, c1, table, at, begin, pages, s, s1, e, e1, stream);
+    const bool few = MANY - room <= FEW;
+    rc = few ? launch<FEW>(pool, p, p1, src, dst, c, c1, table, columns, row, first, length, pages + named0, s0, done0, static_cast<int>(named - named0), stream)
+             : launch<MANY>(pool, p, p1, src, dst, c, c1, table, columns, row, first, length, pages + named0, s0, done0, static_cast<int>(named - named0), stream);
     if (rc != 0) return rc;
     ++*launches;
-    if (s1 > s && e1 < begin[s1]) --s1;                        // the last span goes on in the next launch
-    s = s1;
-    e = e1;
     if (copying) {
       c = c1;
       if (c == copies) {

@@ -80,6 +80,8 @@ _SIGNATURES = {
     "dewb_colsum_bf16": "ppp" + "lil" + "p",
     "dewb_ada_slab": "ii",
     "dewb_ada_bwd": "pppppp" + "l" + "ppppp" + "iiii" + "p",
+    "dewb_move_pages": "pii" + "ppi" + "pii" + "ppppi" + "pp",
+    "dewb_check_moves": "ppii" + "ppppi" + "ii",
     "dewb_rope_append": "pppp" + "iiiii" + "ppp" + "ii" + "p",
     "dewb_paged_decode_persist": "ppp" + "l" + "pppppppp" + "iiiiiii" + "f" + "iii" + "f" + "pp" + "l" + "i" + "pp",
 }

@@ -3,7 +3,8 @@ compaction of the pool does to the device.  The page numbers are the host's, who
 from __future__ import annotations
 
 import ctypes
-from array import array
+import struct
+from itertools import chain
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -43,16 +44,15 @@ def _check(src: Sequence[int], dst: Sequence[int], pages: int, table: Optional[t
 def _pool(t: torch.Tensor, pages: int, device) -> _Pool:
     if t.dim() < 2 or t.shape[1] != pages or t.device != device:
         raise ValueError(f"move_pages: pools of one device and [layers, {pages}, ...], got {tuple(t.shape)} on {t.device}")
-    size = 1
-    for i in range(t.dim() - 1, 0, -1):
-        if t.shape[i] != 1 and t.stride(i) != size:
+    shape, strides, size, by = t.shape, t.stride(), 1, t.element_size()
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and strides[i] != size:
             raise ValueError("move_pages: the pages of a layer have to be one piece of memory, one behind another")
-        size *= t.shape[i]
-    by = t.element_size()
+        size *= shape[i]
     size //= max(1, pages)
     if size * by >= 1 << 31:
         raise ValueError("move_pages: pages of 2 GB and more are not built")
-    return _Pool(t.data_ptr(), t.stride(0) * by, t.shape[0], size * by)
+    return _Pool(t.data_ptr(), strides[0] * by, shape[0], size * by)
 
 
 def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], table: Optional[torch.Tensor] = None, tables: Sequence[Span] = ()) -> None:
@@ -68,7 +68,7 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     if tables and (table is None or table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.device != pools[0].device):
         raise ValueError("move_pages: the table is int32 [rows, columns] in one piece on the pools' device")
     pages = pools[0].shape[1] if pools[0].dim() > 1 else 0
-    made = [_pool(t, pages, pools[0].device) for t in pools]
+    made = (_Pool * len(pools))(*(_pool(t, pages, pools[0].device) for t in pools))
     if not L.use_cuda(pools[0]):
         _check(src, dst, pages, table, tables)
         if len(src):
@@ -79,21 +79,22 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
             if len(ps):
                 table[row, first:first + len(ps)] = torch.tensor(list(ps), dtype=torch.int32, device=table.device)
         return
-    columns = table.shape[1] if tables else 0
-    at, begin, named = array("i"), array("i", [0]), array("i")
-    for row, first, ps in tables:
-        if not (0 <= row < table.shape[0] and 0 <= first <= columns - len(ps)):
-            _refuse(-14)
-        at.append(row * columns + first)
-        named.extend(ps)
-        begin.append(len(named))
-    s, d = array("i", src), array("i", dst)
+    spans = [] if not tables else list(zip(*tables))
+    named = list(chain.from_iterable(spans[2])) if tables else []
+    lengths = list(map(len, spans[2])) if tables else []
+    try:
+        # (the quickest way from lists to integers; the bytes are held until the call is over)
+        numbers = struct.pack(f"{2 * len(src) + 3 * len(tables) + len(named)}i", *src, *dst, *(spans[0] if tables else ()), *(spans[1] if tables else ()), *lengths, *named)
+    except struct.error as e:
+        raise ValueError(f"move_pages: {e}") from None
+    n, spans_n = len(src), len(tables)
+    start = ctypes.cast(ctypes.c_char_p(numbers), ctypes.c_void_p).value
+    part = lambda i: start + 4 * i
     launches = ctypes.c_int(0)
-    where = lambda a: ctypes.c_void_p(a.buffer_info()[0])
     with L.on_device_of(pools[0]) as stream:
-        rc = L.load().dewb_move_pages((_Pool * len(made))(*made), ctypes.c_int(len(made)), ctypes.c_int(pages), where(s), where(d), ctypes.c_int(len(s)), L.ptr(table if tables else None),
-                                      ctypes.c_longlong(table.numel() if tables else 0), where(at), where(begin), where(named), ctypes.c_int(len(at)),
-                                      ctypes.byref(launches), ctypes.c_void_p(stream))
+        rc = L.load().dewb_move_pages(ctypes.addressof(made), len(pools), pages, part(0), part(n), n, L.at(table if tables else None), table.shape[0] if tables else 0,
+                                      table.shape[1] if tables else 0, part(2 * n), part(2 * n + spans_n), part(2 * n + 2 * spans_n), part(2 * n + 3 * spans_n), spans_n,
+                                      ctypes.addressof(launches), stream)
     _refuse(rc)
     L.check(rc, "move_pages")
     L.count_launches(launches.value)

@@ -1,6 +1,6 @@
 """Pages that move: copies and table pieces, the ledger's forks and compaction, samples that fork from one prompt."""
+import ctypes
 import random
-from ctypes import c_int, c_longlong, c_void_p
 
 import pytest
 import torch
@@ -58,21 +58,17 @@ def _native(src, dst, pages, columns, rows, tables):
     """What the launcher's own look at the lists says (host code: it runs without a GPU)."""
     if not L.exists():
         pytest.skip("the library is not built")
-    ints = lambda x: (c_int * max(1, len(x)))(*x)
-    at, begin, named = [], [0], []
-    for row, first, ps in tables:
-        at.append(row * columns + first)
-        named += ps
-        begin.append(len(named))
-    return L.load().dewb_check_moves(ints(src), ints(dst), c_int(len(src)), c_int(pages), ints(at), ints(begin), ints(named), c_int(len(at)), c_longlong(rows * columns))
+    ints = lambda x: (ctypes.c_int * max(1, len(x)))(*x)
+    at = lambda x: ctypes.addressof(x)
+    lists = [ints(x) for x in (src, dst, [t[0] for t in tables], [t[1] for t in tables], [len(t[2]) for t in tables], [p for t in tables for p in t[2]])]
+    return L.load().dewb_check_moves(at(lists[0]), at(lists[1]), len(src), pages, *map(at, lists[2:]), len(tables), rows, columns)
 
 
 def test_the_launchers_look():
     assert _native([5, 5, 0], [1, 2, 8], 9, 4, 3, [(2, 1, [7, 8]), (0, 0, [3]), (1, 4, []), (1, 0, [1])]) == 0
     assert _native([], [], 9, 4, 3, []) == 0
     codes = [_native(src, dst, 9, 4, 3, tables) for src, dst, tables in REFUSED]
-    # (a row before the table's first, or a column before a row's, is refused in front of the launcher)
-    assert codes == [-11, -11, -12, -13, -13, -14, -14, 0, -14, -11, -11, -16]
+    assert codes == [-11, -11, -12, -13, -13, -14, -14, -14, -14, -11, -11, -16]
 
 
 def test_a_fork_shares_whole_pages_and_copies_the_last():
