@@ -82,6 +82,7 @@ _SIGNATURES = {
     "dewb_ada_bwd": "pppppp" + "l" + "ppppp" + "iiii" + "p",
     "dewb_move_pages": "pii" + "ppi" + "pii" + "ppppi" + "pp",
     "dewb_check_moves": "ppii" + "ppppi" + "ii",
+    "dewb_shared_decode": "pl" + "pppp" + "ppppp" + "p" + "pppp" + "iiiiiiiiii" + "ff" + "ii" + "pp",
     "dewb_rope_append": "pppp" + "iiiii" + "ppp" + "ii" + "p",
     "dewb_paged_decode_persist": "ppp" + "l" + "pppppppp" + "iiiiiii" + "f" + "iii" + "f" + "pp" + "l" + "i" + "pp",
 }

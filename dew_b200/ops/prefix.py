@@ -1,0 +1,132 @@
+"""A decode step of rows that share prefixes (``csrc/kernels/shared_prefix.cu``): the keys and values of a group's shared pages are read once for all of its rows, not once a row."""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
+
+import torch
+
+from . import library as L
+
+
+class Shared(NamedTuple):
+    """Which rows of a batch share a prefix, as int32 tensors on the device (their values may change under a captured step): group ``g`` is rows ``order[first[g]:first[g + 1]]``,
+    whose tables name the same pages for their first ``tokens[g]`` keys.  ``order`` holds every row once; a row that shares nothing is a group of its own."""
+    order: torch.Tensor        # [rows]
+    first: torch.Tensor        # [groups + 1]
+    tokens: torch.Tensor       # [groups]
+
+
+def group_rows(tables: Sequence[Optional[Sequence[int]]], page_size: int, least: int = 1) -> Tuple[List[int], List[int], List[int]]:
+    """``order, first, tokens`` of ``Shared`` for rows of these pages (None: an empty row), as lists of as many groups as rows: rows whose first pages are the same make a group,
+    which shares the pages that all of it begins with.  Fewer than ``least`` tokens are not worth a group."""
+    families: Dict[object, List[int]] = {}
+    for r, pages in enumerate(tables):
+        families.setdefault(pages[0] if pages else ("alone", r), []).append(r)
+    order, first, tokens = [], [0], []
+    for rows in families.values():
+        common = 0
+        if len(rows) > 1:
+            for column in zip(*(tables[r] for r in rows)):
+                if any(p != column[0] for p in column):
+                    break
+                common += 1
+        pieces = [rows] if common * page_size >= max(1, least) else [[r] for r in rows]
+        for piece in pieces:
+            order += piece
+            first.append(len(order))
+            tokens.append(common * page_size if len(piece) > 1 else 0)
+    empty = len(order) - len(tokens)
+    return order, first + [len(order)] * empty, tokens + [0] * empty
+
+
+def shared_decode_reference(q, k, v, table, lengths, scale, window=None, softcap=0.0, sinks=None, k_scale=None, v_scale=None) -> torch.Tensor:
+    """Every row by its own table, in fp32: what sharing does not change."""
+    R, H, D = q.shape
+    page, G = k.shape[1:3]
+    n = max(int(lengths.max()), 1) if R else 1
+    key = torch.arange(n, device=q.device)
+    slots = (table.long()[:, key // page] * page + key % page).clamp(0, k.shape[0] * page - 1)
+    seen = key < lengths[:, None]
+    if window:
+        seen = seen & (key >= lengths[:, None] - window)
+
+    def rows(t, by):
+        t = t.reshape(-1, G, D)[slots].float()
+        t = t if by is None else t * by.reshape(-1, G)[slots][..., None]
+        return torch.where(seen[..., None, None], t, torch.zeros_like(t))           # (what a row does not see may be anything)
+    kr, vr = rows(k, k_scale), rows(v, v_scale)
+    s = torch.einsum("rghd,rngd->rghn", q.float().reshape(R, G, H // G, D), kr) * scale
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+    s = s.masked_fill(~seen[:, None, None], -math.inf)
+    if sinks is not None:
+        s = torch.cat([s, sinks.float().view(1, G, H // G, 1).expand(R, -1, -1, 1)], -1)
+    p = torch.nan_to_num(torch.softmax(s, -1)) if sinks is None else torch.softmax(s, -1)[..., :-1]
+    return torch.einsum("rghn,rngd->rghd", p, vr).reshape(R, H, D).to(q.dtype)
+
+
+_POOLS = {torch.int8: 1, torch.float8_e4m3fn: 2}
+
+
+def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_scale, v_scale) -> None:
+    if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or q.shape[2] != k.shape[3] or k.shape[2] == 0 or q.shape[1] % k.shape[2]:
+        raise ValueError(f"shared_decode: queries [rows, heads, dim] and pools [pages, page, kv heads, dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != v.dtype or (k.dtype != q.dtype and k.dtype not in _POOLS):
+        raise TypeError(f"shared_decode: bf16 or fp32 queries and pools of their type, int8 or float8_e4m3fn, got {q.dtype}, {k.dtype}, {v.dtype}")
+    R, H, D = q.shape
+    scales = (k_scale, v_scale) if k.dtype in _POOLS else ()
+    if (k_scale is None) == bool(scales) or (v_scale is None) == bool(scales):
+        raise ValueError("shared_decode: scales belong to int8 and float8 pools")
+    if not 0 < D <= 256:
+        raise ValueError(f"shared_decode: heads of up to 256, got {D}")
+    if shared.order.shape != (R,) or shared.tokens.dim() != 1 or shared.first.shape != (shared.tokens.shape[0] + 1,) or (R and not len(shared.tokens)):
+        raise ValueError(f"shared_decode: order [rows], first [groups + 1] and tokens [groups] for {R} rows, got {[tuple(t.shape) for t in shared]}")
+    if table.dim() != 2 or table.shape[0] != R or lengths.shape != (R,):
+        raise ValueError(f"shared_decode: a table [rows, columns] and lengths [rows] for {R} rows, got {tuple(table.shape)}, {tuple(lengths.shape)}")
+    if any(t.dtype != torch.int32 or not t.is_contiguous() for t in (table, lengths, *shared)):
+        raise TypeError("shared_decode: table, lengths, order, first and tokens are int32 in one piece")
+    if any(s.shape != k.shape[:3] or s.dtype != torch.float32 or not s.is_contiguous() for s in scales):
+        raise ValueError("shared_decode: fp32 scales [pages, page, kv heads]")
+    if sinks is not None and (sinks.shape != (H,) or sinks.dtype != torch.float32 or not sinks.is_contiguous()):
+        raise ValueError("shared_decode: fp32 sinks, one a head")
+    if (window is not None and window < 1) or softcap < 0:
+        raise ValueError(f"shared_decode: a window of 1 or more and a cap of 0 or more, got {window}, {softcap}")
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("shared_decode: pools in one piece")
+    if any(t is not None and t.device != q.device for t in (k, v, table, lengths, *shared, sinks, k_scale, v_scale)):
+        raise ValueError("shared_decode: tensors of one device")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, sinks)):
+        raise NotImplementedError("shared_decode has no gradient: it is a step of generation")
+
+
+def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, shared: Shared, scale: float, *,
+                  window: Optional[int] = None, softcap: float = 0.0, sinks: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                  v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query token of every row, ``q [rows, heads, dim]`` (a view with other rows between will do), against the first ``lengths[r]`` keys of its pages -> ``[rows, heads,
+    dim]``; rows of length 0 give zeros.  Pools ``[pages, page, kv heads, dim]``, ``table [rows, columns]``.  A ``window`` leaves a row its last keys, ``softcap`` and ``sinks`` are
+    those of ``ops.attention``.  ``shared`` says what is read once for several rows; it does not change what is computed.
+
+    Page numbers, lengths and rows that lie outside their tensors are reported by the status word (``library.check_status``) and read nothing."""
+    _check(q, k, v, table, lengths, shared, window, softcap, sinks, k_scale, v_scale)
+    R, H, D = q.shape
+    if R == 0:
+        return q.new_empty(q.shape)
+    if not L.use_cuda(q):
+        return shared_decode_reference(q, k, v, table, lengths, scale, window, softcap, sinks, k_scale, v_scale)
+    if q.stride(2) != 1 or (H > 1 and q.stride(1) != D):
+        q = q.contiguous()
+    out = torch.empty(R, H, D, dtype=q.dtype, device=q.device)
+    pages, page, G, _ = k.shape
+    splits = max(1, min(32, -(-table.shape[1] * page // 512)))
+    parts = torch.empty(2 * splits * R * H * (D + 2), dtype=torch.float32, device=q.device)
+    at = parts.data_ptr()
+    one = 2 * splits * R * H * 4
+    with L.on_device_of(q) as stream:
+        L.check(L.load().dewb_shared_decode(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), L.at(k_scale), L.at(v_scale), table.data_ptr(), lengths.data_ptr(),
+                                            shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + one, at + 2 * one, out.data_ptr(),
+                                            R, H, G, D, page, table.shape[1], pages, len(shared.tokens), splits, window or 0, scale, softcap,
+                                            int(q.dtype == torch.float32), _POOLS.get(k.dtype, 0), L.status(q.device).data_ptr(), stream), "shared_decode")
+    L.count_launches(2)
+    return out
