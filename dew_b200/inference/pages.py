@@ -121,12 +121,13 @@ class PageLedger:
             return page
         raise OutOfPages("the KV page pool is exhausted")
 
-    def seat(self, prompt: Sequence[int], total_tokens: int) -> Seat:
-        """Pages for a row that will hold ``total_tokens`` (prompt + generation budget), re-using cached prefix pages."""
+    def seat(self, prompt: Sequence[int], total_tokens: int, salt: bytes = b"") -> Seat:
+        """Pages for a row that will hold ``total_tokens`` (prompt + generation budget), re-using cached prefix pages (of rows with the same ``salt``: what beside the tokens
+        their contents depend on)."""
         need = (total_tokens + self.page_size - 1) // self.page_size
         pages: List[int] = []
         reused = 0
-        prev = b""
+        prev = salt
         full_prompt_pages = len(prompt) // self.page_size
         if self.prefix_cache:
             for i in range(full_prompt_pages):
@@ -226,11 +227,11 @@ class PageLedger:
             kept.append(self._take())                            # (of the cached pages: the free ones are out of sight)
             self.free = kept
 
-    def publish(self, prompt: Sequence[int], pages: Sequence[int]) -> None:
+    def publish(self, prompt: Sequence[int], pages: Sequence[int], salt: bytes = b"") -> None:
         """After a prompt's prefill: name its full pages so later requests can re-use them."""
         if not self.prefix_cache:
             return
-        prev = b""
+        prev = salt
         for i in range(len(prompt) // self.page_size):
             name = chain_hash(prev, prompt[i * self.page_size:(i + 1) * self.page_size])
             page = pages[i]

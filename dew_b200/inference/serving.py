@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import time
 from collections import deque
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 from typing import Any, Callable, Deque, Dict, List, Optional, Sequence
 
@@ -19,6 +20,9 @@ from ..nn.kv_cache import KVCache
 from ..sampling.text import Sampling, make_cache, transform_logits
 from ..utils import keys as K
 from .pages import HostTier, OutOfPages, PageLedger
+
+
+SHARED_LEAST = 64        # fewest tokens that rows have to begin with together
 
 
 @dataclass
@@ -36,6 +40,9 @@ class Ticket:
     done: bool = False
     terminated: bool = False
     error: Optional[BaseException] = None
+    adapter: Optional[str] = None
+    adapter_slot: int = -1
+    salt: bytes = b""                                                       # what beside the prompt its pages depend on
     waiting: List["Ticket"] = field(default_factory=list, repr=False)      # samples of the same prompt that fork from this one's row when it has been read
 
     def result(self) -> List[int]:
@@ -57,7 +64,9 @@ class Server:
     def __init__(self, model, variables=None, *, slots: int, capacity: int, kv_cache: Optional[KVCache] = None,
                  chunk: Optional[int] = None, prefix_cache: bool = True, decode_steps: int = 1, sampling: Optional[Sampling] = None,
                  tokenizer=None, prefill_budget: Optional[int] = None, cuda_graph: bool = False, clock: Callable[[], float] = time.perf_counter,
-                 host_pages: int = 0):
+                 host_pages: int = 0, shared_prefix: bool = False, adapters=None):
+        """``shared_prefix``: decode steps read the pages that several rows begin with once for all of them.  ``adapters``: an ``nn.lora.AdapterBank`` over ``model``, whose
+        adapters requests name."""
         self.model, self.variables, self.tokenizer = model, variables, tokenizer
         self.slots, self.capacity = slots, capacity
         limit = getattr(getattr(model, "config", None), "max_seq_len", None)
@@ -85,6 +94,9 @@ class Server:
         self.queue: Deque[Ticket] = deque()
         self.device = p.device
         self.clock = clock
+        self.shared_prefix, self._shared_rows = bool(shared_prefix), None
+        self.adapters = adapters
+        self._row_adapters = None if adapters is None else torch.full((slots,), -1, dtype=torch.int32, device=self.device)
         self.last_tokens = torch.zeros(slots, dtype=torch.long, device=self.device)      # device-resident draws
         self._pending: Optional[tuple] = None                                            # (tokens on host (async), rows snapshot, event)
         self.cuda_graph = cuda_graph and self.device.type == "cuda"
@@ -102,32 +114,52 @@ class Server:
     # ------------------------------------------------------------------ construction / API
     @classmethod
     def from_task(cls, task, *, slots: int, capacity: int, admission=None, kv_cache=None, chunk=None, prefix_cache=None,
-                  host_pages: int = 0, decode_steps: int = 1, cuda_graph: bool = False) -> "Server":
+                  host_pages: int = 0, decode_steps: int = 1, cuda_graph: bool = False, shared_prefix: bool = False, adapters=None) -> "Server":
         return cls(task.model, task.variables, slots=slots, capacity=capacity, kv_cache=kv_cache if kv_cache is not None else task.kv_cache,
                    chunk=chunk, prefix_cache=True if prefix_cache is None else bool(prefix_cache), decode_steps=decode_steps, host_pages=host_pages,
-                   sampling=task.sampling, tokenizer=task.tokenizer, cuda_graph=cuda_graph)
+                   sampling=task.sampling, tokenizer=task.tokenizer, cuda_graph=cuda_graph, shared_prefix=shared_prefix, adapters=adapters)
 
-    def submit(self, prompt, max_new_tokens: int, key: int = 0, sampling: Optional[Sampling] = None, on_token=None) -> Ticket:
+    def submit(self, prompt, max_new_tokens: int, key: int = 0, sampling: Optional[Sampling] = None, on_token=None, adapter: Optional[str] = None) -> Ticket:
         if isinstance(prompt, str):
             prompt = self.tokenizer.encode(prompt)
         prompt = [int(t) for t in prompt]
         if len(prompt) + max_new_tokens > self.capacity:
             raise ValueError(f"prompt of {len(prompt)} tokens + {max_new_tokens} new exceeds the row capacity {self.capacity}")
         t = Ticket(prompt, max_new_tokens, key, sampling, on_token, submitted=self.clock())
+        self._hold(t, adapter)
         self.queue.append(t)
         return t
 
-    def submit_group(self, prompt, n: int, max_new_tokens: int, keys: Optional[Sequence[int]] = None, sampling: Optional[Sampling] = None, on_token=None) -> List[Ticket]:
+    def _hold(self, ticket: Ticket, adapter: Optional[str]) -> None:
+        """The request's adapter stays as it is until ``_let_go``."""
+        if adapter is None:
+            return
+        if self.adapters is None:
+            raise ValueError(f"adapter {adapter!r}: the server was made without a bank of adapters")
+        ticket.adapter, ticket.adapter_slot = adapter, self.adapters.acquire(adapter)
+        ticket.salt = f"{adapter}/{self.adapters.version[adapter]}/".encode()        # (keys and values depend on it: no other adapter's pages will do)
+
+    def _let_go(self, ticket: Ticket) -> None:
+        if ticket.adapter is not None:
+            self.adapters.release(ticket.adapter)
+            ticket.adapter = None
+
+    def _with_adapters(self, ids):
+        return nullcontext() if self.adapters is None else self.adapters.using(ids)
+
+    def submit_group(self, prompt, n: int, max_new_tokens: int, keys: Optional[Sequence[int]] = None, sampling: Optional[Sampling] = None, on_token=None,
+                     adapter: Optional[str] = None) -> List[Ticket]:
         """``n`` samples of one prompt, which is read once: the other rows fork from the first when it has been (whole pages are shared, a last page that is partly filled is
         copied).  What finds no slot or pages then is seated like any other request.  ``keys``: a key for each, 0 .. n - 1 by default."""
         keys = list(range(n)) if keys is None else [int(k) for k in keys]
         if n < 1 or len(keys) != n:
             raise ValueError(f"{n} samples with {len(keys)} keys")
-        first = self.submit(prompt, max_new_tokens, keys[0], sampling, on_token)
-        if not first.prompt:
-            self.queue.pop()
+        if not len(prompt):
             raise ValueError("a group of samples needs a prompt of one token or more")
+        first = self.submit(prompt, max_new_tokens, keys[0], sampling, on_token, adapter)
         first.waiting = [Ticket(first.prompt, max_new_tokens, k, sampling, on_token, submitted=first.submitted) for k in keys[1:]]
+        for t in first.waiting:
+            self._hold(t, adapter)
         return [first, *first.waiting]
 
     def compact(self) -> int:
@@ -169,6 +201,7 @@ class Server:
         for t in [r.ticket for r in self.rows if r is not None] + list(self.queue):
             for each in (t, *t.waiting):
                 each.error, each.done = exc, True
+                self._let_go(each)
             t.waiting = []
         self.queue.clear()
         self.rows = [None] * self.slots
@@ -207,13 +240,15 @@ class Server:
                 continue
             t = self.queue[0]
             try:
-                seat = self.ledger.seat(t.prompt, len(t.prompt) + t.max_new_tokens)
+                seat = self.ledger.seat(t.prompt, len(t.prompt) + t.max_new_tokens, t.salt)
             except OutOfPages:
                 break
             self.queue.popleft()
             table = self.store.page_table[slot]
             table[: len(seat.pages)] = torch.tensor(seat.pages, dtype=torch.int32, device=self.device)
             self.rows[slot] = _Row(t, seat.pages, prefilled=seat.reused_tokens)
+            if self._row_adapters is not None:
+                self._row_adapters[slot] = t.adapter_slot
 
     def _prefill(self) -> None:
         """Chunked prefill: every row still reading its prompt advances by up to ``chunk`` tokens; rows are batched and
@@ -252,7 +287,7 @@ class Server:
             ids, pos = ids_h.to(self.device, non_blocking=True), pos_h.to(self.device, non_blocking=True)
             slots = torch.tensor([s for s, _ in members], device=self.device)
             self.store.chunk_span = (start, start + longest)
-            with torch.no_grad():
+            with torch.no_grad(), self._with_adapters(None if self.adapters is None else self._row_adapters[slots]):
                 # the head runs only on each row's last position (the only logits a prefill chunk can need)
                 if hasattr(self.model, "logits"):
                     hidden = self._call(ids, positions=pos, cache=self.store.select(slots), return_hidden=True)
@@ -266,7 +301,7 @@ class Server:
             for i, (s, r) in enumerate(members):
                 r.prefilled += last[i] + 1
                 if r.prefilled >= len(r.ticket.prompt):
-                    self.ledger.publish(r.ticket.prompt, r.pages)
+                    self.ledger.publish(r.ticket.prompt, r.pages, r.ticket.salt)
                     tok = self._draw(last_logits[i][None], r, 0)
                     self.last_tokens[s] = tok
                     r.pending_first = True
@@ -291,6 +326,8 @@ class Server:
             tables.append((child, 0, fork.pages))
             children.append(child)
             self.rows[child] = _Row(t, fork.pages, prefilled=len(t.prompt), pending_first=True)
+            if self._row_adapters is not None:
+                self._row_adapters[child] = t.adapter_slot
         self.queue.extendleft(reversed(waiting))
         if not children:
             return
@@ -320,7 +357,7 @@ class Server:
         """Device work of one decode step, on static buffers (``last_tokens``, ``_in_pos``, ``_prev``) so that it can be
         captured once into a CUDA graph and replayed."""
         self._prev.copy_(self.last_tokens)
-        with torch.no_grad():
+        with torch.no_grad(), self._with_adapters(self._row_adapters):
             hidden = self._call(self.last_tokens[:, None], positions=self._in_pos[:, None], cache=self.store.select(None),
                                 return_hidden=True)[:, 0]
             if greedy:
@@ -365,6 +402,7 @@ class Server:
             e.record()
             self._ring_events[self._ring_at] = e
         if any_live:
+            self._share_prefixes()
             if self.cuda_graph and greedy:
                 if self._graph is None:
                     kept = [(t, t.clone()) for t in self.store.kept_states()]
@@ -400,6 +438,16 @@ class Server:
             r.generated += 1
         return True
 
+    def _share_prefixes(self) -> None:
+        """Tell the cache which rows begin with the same pages, where that has changed."""
+        if not self.shared_prefix:
+            return
+        tables = [None if r is None else r.pages for r in self.rows]
+        known = [None if t is None else tuple(t) for t in tables]
+        if known != self._shared_rows:
+            self._shared_rows = known
+            self.store.share(tables, SHARED_LEAST)
+
     def _queue_settle(self, host, snapshot, ev) -> None:
         self._later = getattr(self, "_later", deque())
         self._later.append((host, snapshot, ev))
@@ -431,6 +479,7 @@ class Server:
                 if (samp.eos_token_ids and tok in samp.eos_token_ids) or len(t.tokens) >= t.max_new_tokens:
                     t.terminated = bool(samp.eos_token_ids and tok in samp.eos_token_ids)
                     t.done, t.finished_time = True, now
+                    self._let_go(t)
                     if self.rows[s] is r:
                         self.ledger.release(r.pages)
                         self.rows[s] = None

@@ -22,7 +22,7 @@ from .. import ops
 from ..ops import latent as M
 from ..ops import library as L
 from ..ops import paged as P
-from ..ops import rotary, token_mix
+from ..ops import prefix, rotary, token_mix
 from ..ops.pages import move_pages
 
 LIMITS = {"int8": 127.0, "float8_e4m3fn": 448.0}
@@ -190,6 +190,7 @@ class KVStore:
         self._scratch = None
         self.chunk_span: Optional[Tuple[int, int]] = None      # (first position, one past the last) of the prefill chunk in flight, when the caller knows
         self.together = True         # whether every row of that chunk starts at its first position
+        self.shared: Optional[prefix.Shared] = None            # rows that share a prefix, of decode steps over all rows
 
     # ------------------------------------------------------------------ layers that differ (CacheSlot)
     @property
@@ -274,6 +275,9 @@ class KVStore:
         R, D, H, G = packed.shape[0], packed.shape[-1], heads.q, heads.kv
         out = torch.empty(R, H, D, dtype=packed.dtype, device=packed.device)
         factors = visible.gain is not None or visible.sigmoid is not None
+        if self._shares(packed[:, 0]) and not factors and not visible.keep and not visible.chunk:
+            return prefix.shared_decode(packed[:, 0, :H], self.k[slot], self.v[slot], c.table, c.lengths, self.shared, scale, window=visible.window, softcap=visible.softcap,
+                                        sinks=visible.sinks)
         if D == 128 and self.page_size % 64 == 0 and H // G <= 8 and hasattr(lib, "dewb_paged_decode_persist") and (R <= 1024 or not factors):
             self._fused_decode(lib, slot, packed, packed.shape[2] * D, c.lengths, R, H, D, visible.window, visible.sinks, out, scale=scale, kv_heads=G, table=c.table,
                                visible=visible)
@@ -388,6 +392,27 @@ class KVStore:
                 new = sized(old, 0)
                 self.k, self.v = ([new if t is old else t for t in pools] for pools in (self.k, self.v))
         self.pages = pages
+
+    def share(self, tables: Optional[Sequence[Optional[Sequence[int]]]], least: int = 1) -> None:
+        """Rows whose pages (``tables``, one list a row, None for an empty one) begin with the same ones read those once in the decode steps to come (``ops.prefix``), from
+        ``least`` shared tokens on; None: every row reads its own again.  The step may be captured: a later call changes what it reads."""
+        if tables is None:
+            self.shared = None
+            return
+        if len(tables) != self.rows:
+            raise ValueError(f"{len(tables)} tables for a cache of {self.rows} rows")
+        order, first, tokens = prefix.group_rows(tables, self.page_size, least)
+        now = torch.tensor(order + first + tokens, dtype=torch.int32)
+        kept = self.__dict__.get("_groups")
+        if kept is None:
+            kept = self._groups = torch.empty(3 * self.rows + 1, dtype=torch.int32, device=self.device)
+        kept.copy_(now)
+        self.shared = prefix.Shared(kept[:self.rows], kept[self.rows:2 * self.rows + 1], kept[2 * self.rows + 1:])
+
+    def _shares(self, q: torch.Tensor) -> bool:
+        """Whether a decode step with queries ``[rows, heads, dim]`` goes by what the rows share."""
+        return (self.shared is not None and self.row_ids is None and q.shape[0] == self.rows and q.shape[-1] <= 256 and q.dtype in (torch.bfloat16, torch.float32)
+                and (self.kind != 0 or q.dtype == self.dtype) and not (q.requires_grad and torch.is_grad_enabled()))
 
     def fork_rows(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Give rows ``children`` what rows ``parents`` keep beside their pages (recurrent states, latents): the same list of parents may name a row several times."""
@@ -553,8 +578,11 @@ class KVStore:
         at = lambda t: 0 if t is None else t.data_ptr()
         L.check(lib.dewb_rope_append(at(qkv), at(cos), at(sin), at(pos32), R, Hq, self.kv_heads, D, cos.shape[0] if cos is not None else 0, at(self.k[layer]),
                                      at(self.v[layer]), at(self.page_table), self.page_size, self.max_pages, L.stream()), "rope_append")
-        out = torch.empty((R, Hq, D), dtype=qkv.dtype, device=qkv.device)
         sinks32 = None if sinks is None else sinks.detach().float().contiguous()      # referenced until the launch is enqueued
+        if self._shares(qkv):
+            L.count_launches(1)
+            return prefix.shared_decode(qkv[:, :Hq], self.k[layer], self.v[layer], self.page_table, lens32, self.shared, 1.0 / math.sqrt(D), window=window, sinks=sinks32)
+        out = torch.empty((R, Hq, D), dtype=qkv.dtype, device=qkv.device)
         self._fused_decode(lib, layer, qkv, H * D, lens32, R, Hq, D, window, sinks32, out)
         L.count_launches(1)
         return out
@@ -580,6 +608,10 @@ class KVStore:
         """``q [R, Hq, D]`` against each row's first ``lengths[r]`` cached tokens -> ``[R, Hq, D]``."""
         R, Hq, D = q.shape
         scale = scale if scale is not None else 1.0 / math.sqrt(D)
+        if self._shares(q):
+            return prefix.shared_decode(q, self.k[layer], self.v[layer], self.page_table, lengths.to(torch.int32).contiguous(), self.shared, scale, window=window, softcap=softcap,
+                                        sinks=None if sinks is None else sinks.detach().float().contiguous(), k_scale=self.k_scale[layer] if self.kind else None,
+                                        v_scale=self.v_scale[layer] if self.kind else None)
         if (L.use_cuda(q) and q.dtype == torch.bfloat16 and self.row_ids is None and R == self.rows and not softcap
                 and Hq // self.kv_heads <= 8 and D in (64, 128, 256)):
             lib = L.load()

@@ -10,6 +10,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
+from ..ops import adapters
 from .layers import Linear, declare
 
 
@@ -254,3 +255,143 @@ def from_peft_state(state: Mapping[str, torch.Tensor]) -> Dict[str, torch.Tensor
             if k.endswith(src):
                 out[k[:-len(src)] + dst] = v
     return out
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Serving: adapters of many requests beside one copy of the weights
+
+
+class AdaptedLinear(nn.Module):
+    """A ``Linear`` beside which every token may have an adapter of its own, as ``bank.using`` says; without it, the ``Linear``."""
+
+    def __init__(self, base: Linear, bank: "AdapterBank"):
+        super().__init__()
+        self.base = base
+        self._of = (bank,)                                 # (not a module of this one)
+        w = base.weight
+        self.register_buffer("a", torch.zeros(bank.slots, bank.rank, base.in_features, dtype=w.dtype, device=w.device), persistent=False)
+        self.register_buffer("b", torch.zeros(bank.slots, base.out_features, bank.rank, dtype=w.dtype, device=w.device), persistent=False)
+        self.register_buffer("scale", torch.zeros(bank.slots, dtype=torch.float32, device=w.device), persistent=False)
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    @property
+    def bias(self):
+        return self.base.bias
+
+    @property
+    def in_features(self):
+        return self.base.in_features
+
+    @property
+    def out_features(self):
+        return self.base.out_features
+
+    def forward(self, x):
+        y = self.base(x)
+        ids = self._of[0].ids_for(x.shape[:-1])
+        return y if ids is None else adapters.add_adapters(y, x, adapters.Bank(self.a, self.b, self.scale), ids)
+
+
+class AdapterBank:
+    """Room for ``slots`` adapters of rank up to ``rank`` beside the ``targets`` of ``model`` (regexes over the attribute names of its ``Linear`` layers, which are replaced).
+    ``load`` takes what ``lora_state`` (or ``from_peft_state``) gives; ``using`` says which adapter each row of the calls inside it has.  For generation: the adapters take no
+    gradient."""
+
+    def __init__(self, model: nn.Module, targets: Iterable[str] = ("qkv_proj", "o_proj"), slots: int = 8, rank: int = 16):
+        if slots < 1 or rank < 1:
+            raise ValueError(f"a bank of {slots} adapters of rank {rank}")
+        self.slots, self.rank = slots, rank
+        pats = [re.compile(t) for t in targets]
+        self.layers: Dict[str, AdaptedLinear] = {}
+        for path, module in list(model.named_modules()):
+            for name, child in list(module.named_children()):
+                if type(child) is Linear and any(p.search(name) for p in pats):
+                    layer = AdaptedLinear(child, self)
+                    setattr(module, name, layer)
+                    self.layers[f"{path}.{name}" if path else name] = layer
+        if not self.layers:
+            raise ValueError(f"no Linear matches {list(targets)}")
+        self.names: Dict[str, int] = {}                    # adapter -> slot
+        self.version: Dict[str, int] = {}                  # how often something was loaded under that name
+        self.holds: Dict[str, int] = {}                    # requests in flight
+        self._ids: Optional[torch.Tensor] = None
+        self._wide: Dict[Tuple[int, ...], torch.Tensor] = {}
+
+    def load(self, name: str, state: Mapping[str, torch.Tensor], alpha: float, rs: bool = False) -> int:
+        """Put an adapter under ``name`` (in place of one that is not in use); returns its slot.  Its scale is ``alpha / rank``, or ``alpha / sqrt(rank)`` with ``rs``, by each
+        layer's own rank; layers that it does not name are left as the model has them."""
+        found = {}
+        for key, t in state.items():
+            path, _, part = key.rpartition(".")
+            if part not in ("lora_a", "lora_b") or path not in self.layers:
+                raise KeyError(f"adapter {name!r}: {key} belongs to no layer of the bank (their parts are lora_a and lora_b; a layer's magnitude cannot be served beside it)")
+            found.setdefault(path, {})[part] = t
+        for path, parts in found.items():
+            layer, a, b = self.layers[path], parts.get("lora_a"), parts.get("lora_b")
+            if a is None or b is None or a.dim() != 2 or b.shape != (layer.out_features, a.shape[0]) or a.shape[1] != layer.in_features or not 0 < a.shape[0] <= self.rank:
+                raise ValueError(f"adapter {name!r}, {path}: lora_a [rank, {layer.in_features}] and lora_b [{layer.out_features}, rank] of rank up to {self.rank}")
+        self._free(name)
+        slot = self.names.get(name)
+        if slot is None:
+            taken = set(self.names.values())
+            slot = next((i for i in range(self.slots) if i not in taken), None)
+            if slot is None:
+                raise RuntimeError(f"the bank's {self.slots} slots are taken: {sorted(self.names)}")
+        with torch.no_grad():
+            for path, layer in self.layers.items():
+                parts = found.get(path)
+                layer.a[slot].zero_()
+                layer.b[slot].zero_()
+                layer.scale[slot] = 0.0
+                if parts is not None:
+                    r = parts["lora_a"].shape[0]
+                    layer.a[slot, :r] = parts["lora_a"].to(layer.a)
+                    layer.b[slot, :, :r] = parts["lora_b"].to(layer.b)
+                    layer.scale[slot] = alpha / (math.sqrt(r) if rs else r)
+        self.names[name] = slot
+        self.version[name] = self.version.get(name, 0) + 1
+        return slot
+
+    def remove(self, name: str) -> None:
+        self._free(name)
+        del self.names[name]
+
+    def _free(self, name: str) -> None:
+        if self.holds.get(name):
+            raise RuntimeError(f"adapter {name!r} is in use by {self.holds[name]} requests")
+
+    def acquire(self, name: str) -> int:
+        """The adapter's slot, held for a request until ``release``."""
+        if name not in self.names:
+            raise KeyError(f"no adapter {name!r}; loaded: {sorted(self.names)}")
+        self.holds[name] = self.holds.get(name, 0) + 1
+        return self.names[name]
+
+    def release(self, name: str) -> None:
+        self.holds[name] -= 1
+
+    @contextmanager
+    def using(self, ids: Optional[torch.Tensor]):
+        """Rows' adapters (int32 ``[rows]`` on the model's device, below 0: none) for the calls inside.  The tensor is read when they run: a captured call follows its values."""
+        if ids is not None and (ids.dtype != torch.int32 or ids.dim() != 1):
+            raise TypeError(f"one int32 id a row, got {ids.dtype} {tuple(ids.shape)}")
+        before = self._ids, self._wide
+        self._ids, self._wide = ids, {}
+        try:
+            yield self
+        finally:
+            self._ids, self._wide = before
+
+    def ids_for(self, shape) -> Optional[torch.Tensor]:
+        """The ids of tokens ``[rows, ...]``."""
+        if self._ids is None:
+            return None
+        shape = tuple(shape)
+        if shape not in self._wide:
+            if not shape or shape[0] != self._ids.shape[0]:
+                raise ValueError(f"adapters of {self._ids.shape[0]} rows in a call of {shape}")
+            self._wide[shape] = self._ids.view(-1, *(1,) * (len(shape) - 1)).expand(shape).contiguous()
+        return self._wide[shape]
