@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
     const long long to_part = (static_cast<long long>(blockIdx.z) * a.rows + row) * a.heads + head0 + x % heads;
     // a row that rests is in the tile, and sees none of it
     const bool rests = a.lengths[row] <= 0;
-    if (lane == 0) { a.part_m[to_part] = rests ? -INFINITY : m[i]; a.part_l[to_part] = l[i]; }
+    if (lane == 0) { a.part_m[to_part] = rests ? -INFINITY : m[i]; a.part_l[to_part] = rests ? 0.f : l[i]; }
 #pragma unroll
     for (int c = 0; c < MOST_D / 32; ++c)
       if (c * 32 + lane < D) a.part_acc[to_part * D + c * 32 + lane] = acc[i][c];
@@ -215,7 +215,9 @@ __global__ void __launch_bounds__(64) join_parts_kernel(const __grid_constant__ 
   float sum = sink > -INFINITY ? exp2f(sink - top) : 0.f;
   for (int p = 0; p < 2 * a.splits; ++p) {
     const float m = a.part_m[p * step + one];
-    if (m > -INFINITY) sum += a.part_l[p * step + one] * exp2f(m - top);
+    const float l = a.part_l[p * step + one];
+    if (m > -INFINITY) sum += l * exp2f(m - top);
+    else if (l != l) sum = l;                            // (no score that is a number)
   }
   for (int d = threadIdx.x; d < a.D; d += 64) {
     float x = 0.f;
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(64) join_parts_kernel(const __grid_constant__ 
       const float m = a.part_m[p * step + one];
       if (m > -INFINITY) x += a.part_acc[(p * step + one) * a.D + d] * exp2f(m - top);
     }
-    put(static_cast<TQ*>(a.out) + one * a.D + d, sum > 0.f ? x / sum : 0.f);
+    put(static_cast<TQ*>(a.out) + one * a.D + d, sum > 0.f || sum != sum ? x / sum : 0.f);
   }
 }
 

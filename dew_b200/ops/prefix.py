@@ -1,4 +1,5 @@
-"""A decode step of rows that share prefixes (``csrc/kernels/shared_prefix.cu``): the keys and values of a group's shared pages are read once for all of its rows, not once a row."""
+"""A decode step of rows that share prefixes (``csrc/kernels/shared_prefix_sm100.cu``; ``shared_prefix.cu`` for types and
+widths that it does not take): the keys and values of a group's shared pages are read once for all of its rows, not once a row."""
 from __future__ import annotations
 
 import ctypes
@@ -67,6 +68,28 @@ def shared_decode_reference(q, k, v, table, lengths, scale, window=None, softcap
     return torch.einsum("rghn,rngd->rghd", p, vr).reshape(R, H, D).to(q.dtype)
 
 
+LEAST_TILES = 4          # 64-key tiles that a CTA of the tensor cores' kernel takes at least
+MOST_ROWS = 512          # rows, and groups, that its lists hold
+_CTAS: Dict[Tuple[int, int], int] = {}
+
+
+def _ctas(lib, device, D: int) -> int:
+    key = (device.index or 0, D)
+    if key not in _CTAS:
+        _CTAS[key] = lib.dewb_shared_mma_ctas(ctypes.c_int(D))
+    return _CTAS[key]
+
+
+def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: int, groups: int) -> bool:
+    """Whether the call is one of ``shared_prefix_sm100.cu``'s: bf16 throughout, heads of 64, 128 or 256, pages of whole sixteens of tokens, 16-byte rows, tables whose tiles
+    can be counted in 32 bits."""
+    R, H, D = q.shape
+    pages, page, G, _ = k.shape
+    return (q.dtype == k.dtype == torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
+            and (2 * R * -(-H // G // 128) + groups) * G * (columns * page // 64 + 2) < 1 << 30
+            and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
+
+
 _POOLS = {torch.int8: 1, torch.float8_e4m3fn: 2}
 
 
@@ -119,14 +142,29 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
         q = q.contiguous()
     out = torch.empty(R, H, D, dtype=q.dtype, device=q.device)
     pages, page, G, _ = k.shape
+    groups, err, fp32 = len(shared.tokens), L.status(q.device).data_ptr(), torch.float32
+    if on_tensor_cores(q, k, v, table.shape[1], groups):
+        with L.on_device_of(q) as stream:
+            lib = L.load()
+            ctas = _ctas(lib, q.device, D)
+            rows = 2 * R * H + 256 * ctas
+            # one piece of scratch a call: sums, maxima and sums of weights, the plan
+            scratch = torch.empty(rows * (D + 2) + 2 * (R + groups) + 4, dtype=fp32, device=q.device)
+            at = scratch.data_ptr()
+            L.check(lib.dewb_shared_decode_mma(q.data_ptr(), q.stride(0) if R > 1 else H * D, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(),
+                                               shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + 4 * rows * D, at + 4 * rows * (D + 2), out.data_ptr(),
+                                               R, H, G, D, page, table.shape[1], pages, groups, window or 0, LEAST_TILES, ctas, scale, softcap, err, stream),
+                    "shared_decode_mma")
+        L.count_launches(2)
+        return out
     splits = max(1, min(32, -(-table.shape[1] * page // 512)))
-    parts = torch.empty(2 * splits * R * H * (D + 2), dtype=torch.float32, device=q.device)
+    parts = torch.empty(2 * splits * R * H * (D + 2), dtype=fp32, device=q.device)
     at = parts.data_ptr()
     one = 2 * splits * R * H * 4
     with L.on_device_of(q) as stream:
         L.check(L.load().dewb_shared_decode(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), L.at(k_scale), L.at(v_scale), table.data_ptr(), lengths.data_ptr(),
                                             shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + one, at + 2 * one, out.data_ptr(),
-                                            R, H, G, D, page, table.shape[1], pages, len(shared.tokens), splits, window or 0, scale, softcap,
-                                            int(q.dtype == torch.float32), _POOLS.get(k.dtype, 0), L.status(q.device).data_ptr(), stream), "shared_decode")
+                                            R, H, G, D, page, table.shape[1], pages, groups, splits, window or 0, scale, softcap,
+                                            int(q.dtype == fp32), _POOLS.get(k.dtype, 0), err, stream), "shared_decode")
     L.count_launches(2)
     return out
