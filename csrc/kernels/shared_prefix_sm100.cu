@@ -1,23 +1,31 @@
 // A decode step of rows that share prefixes, on the tensor cores: bf16 queries and pools, heads of 64, 128 or 256, pages of a multiple of 16 tokens.
 //
-// The work is lists of 64-key tiles.  A group's shared keys (shared_range.cuh) make a list for each key head and each 128 of the group's (row, head) queries on it; a row's own
-// keys make one for each key head.  All lists stand behind one another in one sequence, which the CTAs share evenly: a list may begin in one CTA and end in another.  Every
-// list is the same work to the kernel: up to 128 queries, a page table's row, a range of keys.
+// The work is lists: up to some number of queries (row, head) against a range of keys of one key head.  A group's shared keys (shared_range.cuh) make a list for each key head,
+// a row's own keys another.  There are two kinds, and all lists of a kind stand behind one another in one sequence of tiles that the CTAs share evenly: a list may begin in one
+// CTA and end in another.
 //
-//   warps 0..3  softmax: a thread a query; also fetch the queries, and write results
-//   warp 4      TMA: keys and values, a 64-key tile a slot of one ring, in the order of their use, across lists
-//   warp 5      tensor cores: S = Q K^T of a tile into one of two score buffers, O += P V with P over its scores
+// TALL lists (a group of more than 32 queries on a key head, 128 of them a list): queries are the rows of the products.  Per 64 keys  S = Q K^T  (one of two score buffers in
+// tensor memory),  a thread a query makes the weights P over its scores,  O += P V  with P read from tensor memory.
 //
-// A query tile is 128 rows tall however few queries a list has (four, of a row's own keys): the products of 64 keys then take 256 cycles, while an SM's share of the memory
-// rate brings those 64 keys and values in 1400 (heads of 128).  What a row of a list does is the business of its lane of tensor memory alone, so lanes without a query hold
-// anything.  Two CTAs an SM (one at heads of 256): a tile's chain from scores to products is longer than its products, and the other CTA's lie beside it.
+// WIDE lists (up to 32 queries: a row's own keys, a small group): keys are the rows, so that few queries make small products and every thread has work.  Per 128 keys
+// S^T = K Q^T (16 or 32 columns),  a thread a key makes its weights for all queries,  P^T goes to shared memory,  O^T += V^T P^T (a lane a column of the head).  All queries'
+// weights are relative to one maximum a query, which the threads agree on anew only where a score has passed it by 2^8 (one vote a tile); sums of weights stay with the
+// threads until the list ends.
+//
+//   warps 0..3  softmax, results;  tall lists' queries
+//   warp 4      TMA: keys and values; wide lists' queries, and what the list is about, a list ahead
+//   warp 5      tensor cores
+//
+// Two CTAs an SM (one at heads of 256), whose chains lie beside one another: an SM's share of the memory rate brings 64 keys and values of a head of 128 in 1400 cycles.
+// With four queries as rows of a 128-row product, a wide list's tile took one warp 2300 cycles of scores (four of its lanes had any) and a list of one tile 7100, mostly chain:
+// 128 rows in 16 groups of 1000 to 2048 shared tokens 181 us, 128 rows behind 8192 shared tokens 121.
 //
 // No score needs a mask but at the ends of a list's keys, where it is the same for all queries.  Values there are put to zero in shared memory, since a weight of zero does
 // not cancel what is not a number.
 //
 // A list that is a row's whole attention is finished here.  Otherwise (m, l, sum) of a list, or of the piece of it that a CTA had, goes to scratch, and a second kernel joins
-// a query's pieces:  o = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i.  Scratch is bounded by queries and CTAs, whatever the keys' number: a CTA holds at most two lists
-// in part (its first and its last), the others' queries have a place of their own.  Nothing is counted with atomics: the same call gives the same bits.
+// a query's pieces:  o = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i.  Scratch is bounded by queries and CTAs, whatever the keys' number: of each kind a CTA holds at most
+// two lists in part (its first and its last), the others' queries have a place of their own.  Nothing is counted with atomics: the same call gives the same bits.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -29,39 +37,73 @@
 namespace dewb {
 namespace sharedmma {
 
-constexpr int BM = 128, BN = 64;                  // queries of a list, keys of a tile
+constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys of a tile
+constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
 constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
-constexpr int MOST_ROWS = 512;
-constexpr float RESCALE = 8.f;                    // how far (log2) a row's maximum may grow before O is rescaled
+constexpr int MOST_ROWS = 448;
+constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t FULL = 0xffffffffu;
 
 template <int D>
 struct Cfg {
   static constexpr int SUB = D / 64;              // 64-column pieces of a row
-  static constexpr int Q_BYTES = BM * D * 2;
-  static constexpr int SLOT = BN * D * 2;
-  static constexpr int RING = D == 64 ? 8 : 4;
+  static constexpr int Q_BYTES = BM * D * 2;      // tall: the queries.  wide: two lists' queries and two tiles' weights
+  static constexpr int SLOT = BN * D * 2, RING = D == 64 ? 8 : 4;              // tall: keys or values of a tile
+  static constexpr int W_TILE = WK * D * 2, W_SLOTS = RING / 4;                // wide: the same memory, half for keys and half for values
+  static constexpr int W_Q = WN * D * 2, W_P = WN * WK * 2;
   static constexpr int CTAS = D == 256 ? 1 : 2;   // an SM
+  static constexpr int HALVES = D == 256 ? 2 : 1; // wide: 128-column pieces of a head
   static constexpr int TM_O = 2 * BN, TM_COLS = D == 256 ? 512 : 256;
+  static constexpr int TM_WO = 2 * WN;
+  static constexpr int EXTRA = 2 * W_Q + 2 * W_P > Q_BYTES ? 2 * W_Q + 2 * W_P - Q_BYTES : 0;      // (where that is more)
+};
+
+struct Ranges {                                   // the keys of a list, [a0, a1) and [b0, b1), and its tiles of N
+  int a0, a1, b0, b1;
+  template <int N> __device__ __forceinline__ int a_tiles() const { return a1 > a0 ? (a1 + N - 1) / N - a0 / N : 0; }
+  template <int N> __device__ __forceinline__ int b_first() const { return a1 > a0 ? max(b0 / N, (a1 + N - 1) / N) : b0 / N; }
+  template <int N> __device__ __forceinline__ int tiles() const { return a_tiles<N>() + (b1 > b0 ? max(0, (b1 + N - 1) / N - b_first<N>()) : 0); }
+  template <int N> __device__ __forceinline__ int tile(int i) const { const int n = a_tiles<N>(); return i < n ? a0 / N + i : b_first<N>() + i - n; }
+  __device__ __forceinline__ bool sees(int key) const { return (key >= a0 && key < a1) || (key >= b0 && key < b1); }
+  __device__ __forceinline__ bool meets(int key, int n) const { return (key < a1 && key + n > a0 && a1 > a0) || (key < b1 && key + n > b0 && b1 > b0); }
+};
+
+// A list, or the piece of it that a CTA has.
+struct Item {
+  Ranges keys;
+  int index, list, lists;                         // group or place, and which of its lists
+  bool shared;                                    // of a group
+  int start, units;                               // the whole list's first unit and tiles
+  int from, tiles;                                // of its tiles
+  int place, each, hk, head0, n;                  // first query counted through the places, query heads a row, key head, first query head, queries
+  int row;                                        // whose table
 };
 
 struct Bars {
-  uint64_t full[8], empty[8], q_full, s_full[2], p_full[2], done;
+  uint64_t full[8], empty[8], tall_full, s_full[2], p_full[2], done;           // tall lists
+  uint64_t wk_full[2], wk_empty[2], wv_full[2], wv_empty[2], wq_full[2], wq_empty[2], ws_full[2], wp_full[2], w_done;      // wide lists
   uint32_t tmem;
   int abort_flag, poisoned;
 };
 
 // what a CTA knows of all lists
 struct Lists {
-  int prefix_units, per_cta;
-  int first[MOST_ROWS + 1];                       // groups: first place
+  int tall_units, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;
+  short first[MOST_ROWS + 2];                     // groups: first place
+  short row[MOST_ROWS], group[MOST_ROWS];         // places (row -1: none)
+  short through[MOST_ROWS];                       // groups: a row that holds something
   int lo[MOST_ROWS], hi[MOST_ROWS];               // groups: shared keys (hi 0: none)
-  int at[MOST_ROWS + 1];                          // groups: first unit
+  int tall[MOST_ROWS + 1], wide[MOST_ROWS + 1];   // groups: units of either kind before
   int own[MOST_ROWS + 1];                         // places: own tiles before
   int len[MOST_ROWS];                             // places
-  short row[MOST_ROWS], group[MOST_ROWS];         // places (-1: none)
-  short through[MOST_ROWS];                       // groups: a row that holds something
+  union {
+    Item now[4];                                  // tall: the list at hand of each softmax warp (its registers are for a row of scores)
+    struct {
+      Item item[2];                               // wide: beside the lists' queries
+      float most[4][WN], sums[4][WN];             // the softmax's warps tell one another
+    };
+  };
 };
 
 struct Args {
@@ -70,25 +112,12 @@ struct Args {
   const int *table, *lengths, *order, *first, *tokens;
   const float* sinks;
   __nv_bfloat16* out;
-  float* acc;                                     // [2 rows heads + 2 ctas 128][D]
+  float* acc;                                     // [2 rows heads + ctas (2 128 + 2 32)][D]
   float2* ml;                                     // [the same]: maximum (log2), sum
-  int* plan;                                      // for the second kernel: see write_plan
+  int4* plan;                                     // [rows][2], for the second kernel: see write_plan
   int rows, heads, kv_heads, page_size, box, max_pages, pages, groups, window, least;
   float scale_log2, cap_log2;
   int* err;
-};
-
-struct Ranges {                                   // the keys of a list, [a0, a1) and [b0, b1), and its tiles
-  int a0, a1, b0, b1;
-  __device__ __forceinline__ int a_tiles() const { return a1 > a0 ? (a1 + BN - 1) / BN - a0 / BN : 0; }
-  __device__ __forceinline__ int b_first() const { return a1 > a0 ? max(b0 / BN, (a1 + BN - 1) / BN) : b0 / BN; }
-  __device__ __forceinline__ int tiles() const { return a_tiles() + (b1 > b0 ? max(0, (b1 + BN - 1) / BN - b_first()) : 0); }
-  __device__ __forceinline__ int tile(int i) const { const int n = a_tiles(); return i < n ? a0 / BN + i : b_first() + i - n; }
-  __device__ __forceinline__ bool sees(int key) const { return (key >= a0 && key < a1) || (key >= b0 && key < b1); }
-  __device__ __forceinline__ bool whole(int tile) const {
-    const int x = tile * BN, y = x + BN;
-    return (x >= a0 && y <= a1) || (x >= b0 && y <= b1);
-  }
 };
 
 __device__ __forceinline__ Ranges own_ranges(int len, int window, int lo, int hi) {
@@ -98,16 +127,8 @@ __device__ __forceinline__ Ranges own_ranges(int len, int window, int lo, int hi
   return Ranges{first, max(first, lo), hi, max(hi, len)};
 }
 
-struct Item {
-  int place, hk, head0, n;                        // first place, key head, first query head, queries
-  int each;                                       // query heads a row
-  int row;                                        // whose table
-  int from, tiles;                                // of the list's tiles
-  int slot;                                       // scratch: >= 0 a CTA's place for a piece, -1 the queries' own places of lists of groups, -2 of rows, -3 finished here
-  Ranges keys;
-};
-
-__device__ __forceinline__ int last_at_most(const int* x, int n, int v) {      // largest i in [0, n) with x[i] <= v (x[0] <= v)
+template <typename T>
+__device__ __forceinline__ int last_at_most(const T* x, int n, int v) {        // largest i in [0, n) with x[i] <= v (x[0] <= v)
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -116,48 +137,87 @@ __device__ __forceinline__ int last_at_most(const int* x, int n, int v) {      /
   return lo;
 }
 
-// The piece that begins at unit u and ends with its list or before `end`.
-__device__ __forceinline__ Item locate(const Lists& s, const Args& a, int u, int end) {
-  const int ratio = a.heads / a.kv_heads, chunks = (ratio + BM - 1) / BM;
-  Item w;
-  int start, units;
-  if (u < s.prefix_units) {
-    const int g = last_at_most(s.at, a.groups, u);
-    const int queries = (s.first[g + 1] - s.first[g]) * ratio, tall = (queries + BM - 1) / BM;
-    w.keys = Ranges{s.lo[g], s.hi[g], 0, 0};
-    units = w.keys.tiles();
-    const int list = (u - s.at[g]) / units;
-    start = s.at[g] + list * units;
-    w.hk = list / tall;
-    const int m0 = (list - w.hk * tall) * BM;
-    w.place = s.first[g] * ratio + m0;            // (counted in queries)
+__device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * (a.heads / a.kv_heads); }
+
+// index, shared, list and start are known: the rest, for the piece from unit u on; `same`: of the group or place of the list before.
+template <bool TALL>
+__device__ __forceinline__ void fill(Item& w, const Lists& s, const Args& a, int u, int end, bool same) {
+  const int ratio = a.heads / a.kv_heads;
+  if (TALL || w.shared) {
+    const int queries = group_queries(s, a, w.index), pieces = TALL ? (queries + BM - 1) / BM : 1;
+    if (!same) {
+      w.keys = Ranges{s.lo[w.index], s.hi[w.index], 0, 0};
+      w.lists = a.kv_heads * pieces;
+      w.row = s.through[w.index];
+    }
+    w.hk = TALL ? w.list / pieces : w.list;
+    const int m0 = TALL ? (w.list - w.hk * pieces) * BM : 0;
+    w.place = s.first[w.index] * ratio + m0;
     w.each = ratio;
     w.head0 = w.hk * ratio;
-    w.n = min(BM, queries - m0);
-    w.row = s.through[g];
-    w.slot = -1;
+    w.n = min(TALL ? BM : WN, queries - m0);
   } else {
-    const int lists = a.kv_heads * chunks, v = u - s.prefix_units;
-    const int i = last_at_most(s.own, a.rows, v / lists);
-    units = s.own[i + 1] - s.own[i];
-    start = s.prefix_units + s.own[i] * lists;
-    const int list = (u - start) / units;
-    start += list * units;
-    w.hk = list / chunks;
-    const int c = list - w.hk * chunks;
-    w.n = min(BM, ratio - c * BM);
-    w.each = w.n;
-    w.place = i * w.n;
-    w.head0 = w.hk * ratio + c * BM;
-    w.row = s.row[i];
-    const int g = s.group[i];
-    w.keys = own_ranges(s.len[i], a.window, s.lo[g], s.hi[g]);
-    w.slot = s.hi[g] == 0 ? -3 : -2;
+    const int chunks = (ratio + WN - 1) / WN;
+    if (!same) {
+      const int g = s.group[w.index];
+      w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g]);
+      w.lists = a.kv_heads * chunks;
+      w.row = s.row[w.index];
+    }
+    w.hk = chunks == 1 ? w.list : w.list / chunks;
+    const int c = w.list - w.hk * chunks;
+    w.n = w.each = min(WN, ratio - c * WN);
+    w.place = w.index * w.n;
+    w.head0 = w.hk * ratio + c * WN;
   }
-  w.from = u - start;
-  w.tiles = min(end, start + units) - u;
-  if (w.tiles < units) w.slot = 2 * blockIdx.x + (w.from == 0 ? 1 : 0);
+  w.from = u - w.start;
+  w.tiles = min(end, w.start + w.units) - u;
+}
+
+// The piece that begins at unit u and ends with its list or before `end`.
+template <bool TALL>
+__device__ __forceinline__ Item locate(const Lists& s, const Args& a, int u, int end) {
+  Item w;
+  w.shared = TALL || u < s.wide_shared_units;
+  if (w.shared) {
+    const int* at = TALL ? s.tall : s.wide;
+    w.index = last_at_most(at, a.groups, u);
+    w.start = at[w.index];
+    w.units = Ranges{s.lo[w.index], s.hi[w.index], 0, 0}.tiles<TALL ? BN : WK>();
+  } else {
+    const int lists = a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
+    w.index = last_at_most(s.own, a.rows, (u - s.wide_shared_units) / lists);
+    w.start = s.wide_shared_units + s.own[w.index] * lists;
+    w.units = s.own[w.index + 1] - s.own[w.index];
+  }
+  w.list = (u - w.start) / w.units;
+  w.start += w.list * w.units;
+  fill<TALL>(w, s, a, u, end, false);
   return w;
+}
+
+// The list behind w's, which is in this CTA to its end; u: its first unit, before `end`.
+template <bool TALL>
+__device__ __forceinline__ void advance(Item& w, const Lists& s, const Args& a, int u, int end) {
+  w.start = u;
+  if (++w.list < w.lists) {
+    fill<TALL>(w, s, a, u, end, true);
+    return;
+  }
+  w.list = 0;
+  if (!TALL && w.shared && u >= s.wide_shared_units) {
+    w.shared = false;
+    w.index = -1;
+  }
+  if (TALL || w.shared) {
+    const int* at = TALL ? s.tall : s.wide;
+    do ++w.index; while (at[w.index + 1] <= u);
+    w.units = Ranges{s.lo[w.index], s.hi[w.index], 0, 0}.tiles<TALL ? BN : WK>();
+  } else {
+    do ++w.index; while (s.own[w.index + 1] == s.own[w.index]);
+    w.units = s.own[w.index + 1] - s.own[w.index];
+  }
+  fill<TALL>(w, s, a, u, end, false);
 }
 
 // the row and head of a list's query
@@ -168,26 +228,48 @@ __device__ __forceinline__ void query(const Lists& s, const Item& w, int i, int&
   head = w.head0 + x - place * w.each;
 }
 
-// What the second kernel needs: units a CTA, units of groups, places' tiles, groups and lengths, groups' first units and tiles.
-__device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int tid) {
-  int* p = a.plan;
-  if (tid == 0) { p[0] = s.per_cta; p[1] = s.prefix_units; }
-  p += 2;
-  for (int i = tid; i <= a.rows; i += THREADS) p[i] = s.own[i];
-  p += a.rows + 1;
-  for (int i = tid; i < a.rows; i += THREADS) p[i] = s.group[i];
-  p += a.rows;
-  for (int g = tid; g <= a.groups; g += THREADS) p[g] = s.at[g];
-  p += a.groups + 1;
-  for (int g = tid; g < a.groups; g += THREADS) p[g] = Ranges{s.lo[g], s.hi[g], 0, 0}.tiles();
+// Queries [.][D] to their rows (128-byte swizzle) of 64-column pieces `part` bytes apart, by `threads` threads.
+template <int D, int EACH>
+__device__ __forceinline__ void fetch_queries(uint8_t* to, int part, const Lists& s, const Args& a, const Item& w, int t, int threads) {
+  constexpr int PIECES = D / 8;
+  for (int i0 = t; i0 < w.n * PIECES; i0 += threads * EACH) {
+    uint4 v[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = i0 + e * threads, x = i / PIECES;
+      if (i >= w.n * PIECES) break;
+      int row, head;
+      query(s, w, x, row, head);
+      v[e] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.q + row * a.q_stride + static_cast<long long>(head) * D) + i % PIECES);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = i0 + e * threads, x = i / PIECES, c = i % PIECES;
+      if (i >= w.n * PIECES) break;
+      *reinterpret_cast<uint4*>(to + (c >> 3) * part + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[e];
+    }
+  }
+  fence_proxy_async();
+  __syncwarp();
 }
 
-// Running sums of n numbers f(i) into x[0..n] by one warp.
-template <typename F>
-__device__ __forceinline__ void running_sums(int* x, int n, int lane, F f) {
+// What the second kernel needs of a place: its group's first unit and tiles (of either kind), its own; its group's first place and queries a key head (0: wide), units a CTA.
+__device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int tid) {
+  const int lists = a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
+  for (int i = tid; i < a.rows; i += THREADS) {
+    const int g = s.group[i], queries = group_queries(s, a, g);
+    const Ranges both{s.lo[g], s.hi[g], 0, 0};
+    const bool tall = queries > WN;
+    a.plan[2 * i] = make_int4(tall ? s.tall[g] : s.wide[g], tall ? both.tiles<BN>() : both.tiles<WK>(), s.wide_shared_units + s.own[i] * lists, s.own[i + 1] - s.own[i]);
+    a.plan[2 * i + 1] = make_int4(s.first[g], tall ? queries : 0, s.tall_per_cta, s.wide_per_cta);
+  }
+}
+
+// x[i + 1], 0 <= i < n, to their running sums; x[0] = 0.  One warp.
+__device__ __forceinline__ void running_sums(int* x, int n, int lane) {
   const int per = (n + 31) / 32, i0 = min(n, lane * per), i1 = min(n, i0 + per);
   int sum = 0;
-  for (int i = i0; i < i1; ++i) sum += f(i);
+  for (int i = i0; i < i1; ++i) sum += x[i + 1];
   int to = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -196,35 +278,46 @@ __device__ __forceinline__ void running_sums(int* x, int n, int lane, F f) {
   }
   int run = to - sum;
   if (lane == 0) x[0] = 0;
-  for (int i = i0; i < i1; ++i) { run += f(i); x[i + 1] = run; }
+  for (int i = i0; i < i1; ++i) { run += x[i + 1]; x[i + 1] = run; }
 }
 
 __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int warp, int lane) {
-  const int most = a.max_pages * a.page_size, ratio = a.heads / a.kv_heads;
-  int* live = s.at;                               // (until the units are known)
+  constexpr int EACH = (MOST_ROWS + THREADS - 1) / THREADS;
+  const int most = a.max_pages * a.page_size;
+  int* live = s.own;                              // (until the places' tiles are known)
+  // rows and lengths are on their way while the groups are looked at
+  int row_of[EACH], len_of[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = e * THREADS + tid;
+    row_of[e] = i < a.rows ? a.order[i] : 0;
+  }
   for (int g = tid; g <= a.groups; g += THREADS) {
-    s.first[g] = min(max(a.first[g], 0), a.rows);
+    s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
     if (g == a.groups) break;
     s.lo[g] = 0;
     s.hi[g] = min(max(a.tokens[g], 0), most);
     live[g] = 0;
     s.through[g] = -1;
   }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) len_of[e] = row_of[e] >= 0 && row_of[e] < a.rows ? a.lengths[row_of[e]] : 0;
   __syncthreads();
-  for (int i0 = warp * 32; i0 < a.rows; i0 += THREADS) {
-    const int i = i0 + lane;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = e * THREADS + tid;
+    if (e * THREADS + warp * 32 >= a.rows) break;
     int g = -1, row = -1, len = 0;
     if (i < a.rows) {
       g = last_at_most(s.first, a.groups, i);
-      row = a.order[i];
+      row = row_of[e];
       bool bad = row < 0 || row >= a.rows;
       if (i < s.first[g] || i >= s.first[g + 1]) { g = -1; bad = true; }
       if (bad) {
         row = -1;
       } else {
-        const int n = a.lengths[row];
-        bad = n > most;
-        len = min(max(n, 0), most);
+        bad = len_of[e] > most;
+        len = min(max(len_of[e], 0), most);
       }
       if (bad && blockIdx.x == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
       s.row[i] = static_cast<short>(row);
@@ -245,23 +338,203 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     }
   }
   __syncthreads();
-  for (int g = tid; g < a.groups; g += THREADS)
+  for (int g = tid; g < a.groups; g += THREADS) {
     if (live[g] < 2 || s.lo[g] >= s.hi[g]) s.lo[g] = s.hi[g] = 0;
+    const int queries = group_queries(s, a, g);
+    const Ranges both{s.lo[g], s.hi[g], 0, 0};
+    s.tall[g + 1] = s.hi[g] == 0 || queries <= WN ? 0 : a.kv_heads * ((queries + BM - 1) / BM) * both.tiles<BN>();
+    s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * both.tiles<WK>();
+  }
+  __syncthreads();
+  for (int i = tid; i < a.rows; i += THREADS) s.own[i + 1] = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles<WK>();
+  if (warp == 1) running_sums(s.tall, a.groups, lane);
+  if (warp == 2) running_sums(s.wide, a.groups, lane);
   __syncthreads();
   if (warp == 0) {
-    running_sums(s.own, a.rows, lane, [&](int i) { return own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles(); });
-  } else if (warp == 1) {
-    running_sums(s.at, a.groups, lane, [&](int g) {
-      return s.hi[g] == 0 ? 0 : a.kv_heads * (((s.first[g + 1] - s.first[g]) * ratio + BM - 1) / BM) * Ranges{s.lo[g], s.hi[g], 0, 0}.tiles();
-    });
+    running_sums(s.own, a.rows, lane);
+    __syncwarp();
+    if (lane == 0) {
+      const int ctas = static_cast<int>(gridDim.x);
+      s.tall_units = s.tall[a.groups];
+      s.wide_shared_units = s.wide[a.groups];
+      s.wide_units = s.wide_shared_units + s.own[a.rows] * a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
+      s.tall_per_cta = max(2 * a.least, (s.tall_units + ctas - 1) / ctas);
+      s.wide_per_cta = max(a.least, (s.wide_units + ctas - 1) / ctas);
+    }
   }
   __syncthreads();
-  if (tid == 0) {
-    const int units = s.at[a.groups] + s.own[a.rows] * a.kv_heads * ((ratio + BM - 1) / BM);
-    s.prefix_units = s.at[a.groups];
-    s.per_cta = max(a.least, (units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+}
+
+// ---------------------------------------------------------------------------------------------------------- wide lists' softmax
+__device__ __forceinline__ bool any_of_128(bool p) {       // whether p holds for any of the softmax's threads
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(p)) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+template <int NC>
+__device__ __forceinline__ void load_columns(uint32_t at, float (&x)[NC]) {
+  if constexpr (NC == 32) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(at, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(v[i]);
+  } else {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(at, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < NC; ++i) x[i] = __uint_as_float(v[i]);
   }
-  __syncthreads();
+}
+
+struct Wide {                                     // what a list's softmax works with
+  uint32_t t_s, t_o;                              // tensor memory, this warp's lanes
+  uint8_t *weights, *values;                      // shared memory
+  Bars* bars;
+  volatile int* abort_flag;
+  int tid, warp, lane;
+};
+
+// One wide list of up to NC queries, whose first tile is the CTA's t-th: false after a wait that ran out.  (All warps pass all barriers, whatever went wrong: waits that
+// follow one that ran out return at once.)
+template <int D, int NC>
+__device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Args& a, const Item& w, int& t) {
+  using C = Cfg<D>;
+  Bars* bars = x.bars;
+  const int tid = x.tid, lane = x.lane, warp = x.warp, tiles = w.tiles, n = w.n;
+  constexpr int PART = NC < 16 ? NC : 16;         // queries at a time where more would not fit the registers
+  bool ok = true;
+  float m[NC], l[NC];                             // (l: of this thread's keys)
+#pragma unroll
+  for (int q = 0; q < NC; ++q) { m[q] = -INFINITY; l[q] = 0.f; }
+  for (int j = 0; j < tiles; ++j, ++t) {
+    const int b = t & 1;
+    if (!mbar_wait_warp(&bars->ws_full[b], (t >> 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_TMEM_FULL)); ok = false; }
+    tc_fence_after();
+    const bool seen = w.keys.sees(w.keys.tile<WK>(w.from + j) * WK + tid);
+    float s[NC];
+    load_columns<NC>(x.t_s + b * WN, s);
+    bool past = false;
+#pragma unroll
+    for (int q = 0; q < NC; ++q) {
+      s[q] *= a.scale_log2;
+      // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), in the log2 domain
+      if (a.cap_log2 > 0.f) s[q] = fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + fast_exp2(s[q] * (2.f * LOG2E / a.cap_log2))), a.cap_log2);
+      s[q] = seen ? s[q] : -INFINITY;
+      past = past || (q < n && s[q] > m[q] + RESCALE);
+    }
+    if (any_of_128(past)) {
+#pragma unroll
+      for (int q = 0; q < NC; ++q) {
+        float top = s[q];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+        if (lane == q) lists.most[warp][q] = top;
+      }
+      sync_128();
+      // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
+      if (j > 0 && !mbar_wait_warp(&bars->w_done, (t - 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < NC; c += PART) {
+        float by[PART];
+#pragma unroll
+        for (int i = 0; i < PART; ++i) {
+          const int q = c + i;
+          const float now = fmaxf(m[q], fmaxf(fmaxf(lists.most[0][q], lists.most[1][q]), fmaxf(lists.most[2][q], lists.most[3][q])));
+          by[i] = m[q] > -INFINITY && q < n ? fast_exp2(m[q] - now) : 1.f;
+          m[q] = now;
+          l[q] *= by[i];
+        }
+        if (j == 0) continue;
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(x.t_o + h * WN + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < PART; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by[i]);
+          tmem_st_32x32b_x16(x.t_o + h * WN + c, v);
+        }
+      }
+      tmem_st_wait();
+    }
+    // weights: query q's row of 128 keys in two 64-key pieces (128-byte swizzle)
+    uint8_t* to = x.weights + b * C::W_P + (tid >> 6) * (WN * 128) + (tid & 7) * 2;
+#pragma unroll
+    for (int q = 0; q < NC; ++q) {
+      const float p = fast_exp2(s[q] - (m[q] == -INFINITY ? 0.f : m[q]));
+      l[q] += p;
+      *reinterpret_cast<__nv_bfloat16*>(to + q * 128 + ((((tid >> 3) & 7) ^ (q & 7)) << 4)) = __float2bfloat16(p);
+    }
+    if (__ballot_sync(FULL, !seen) != 0) {        // values that nobody sees, to zero (each thread its key's)
+      const int slot = t % C::W_SLOTS;
+      if (!mbar_wait_warp(&bars->wv_full[slot], (t / C::W_SLOTS) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; }
+      if (!seen) {
+#pragma unroll
+        for (int p = 0; p < C::SUB; ++p)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(x.values + slot * C::W_TILE + p * (WK * 128) + tid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->wp_full[b]);
+  }
+  // where the results go (lane q: query q's), and the sums of weights
+  const bool entire = tiles == w.units;
+  const bool last = entire && !w.shared && lists.hi[lists.group[w.index]] == 0;
+  int row = -1, head = 0;
+  if (lane < n) query(lists, w, lane, row, head);
+  const long long one = static_cast<long long>(row) * a.heads + head, all = static_cast<long long>(a.rows) * a.heads;
+  long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * 2 * BM + (2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
+  if (row < 0) at = -1;
+#pragma unroll
+  for (int q = 0; q < NC; ++q) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l[q] += __shfl_xor_sync(FULL, l[q], o);
+    if (lane == q) lists.sums[warp][q] = l[q];
+  }
+  sync_128();
+  if (!mbar_wait_warp(&bars->w_done, (t - 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
+  tc_fence_after();
+#pragma unroll
+  for (int c = 0; c < NC; c += PART) {
+    float by[PART];                               // what the results are multiplied with
+#pragma unroll
+    for (int i = 0; i < PART; ++i) {
+      const int q = c + i;
+      const float sum = (lists.sums[0][q] + lists.sums[1][q]) + (lists.sums[2][q] + lists.sums[3][q]);
+      by[i] = 1.f;
+      if (last) {
+        const float sink = a.sinks != nullptr && q < n ? a.sinks[w.head0 + q] * LOG2E : -INFINITY;
+        const float top = fmaxf(m[q], sink), own = m[q] > -INFINITY ? fast_exp2(m[q] - top) : 0.f;
+        const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - top) : 0.f);
+        by[i] = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
+      } else if (tid == q && at >= 0) {
+        a.ml[at] = make_float2(m[q], sum);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < C::HALVES; ++h) {
+      float o[PART];
+      load_columns<PART>(x.t_o + h * WN + c, o);
+#pragma unroll
+      for (int i = 0; i < PART; ++i) {
+        const long long to = __shfl_sync(FULL, at, c + i);
+        if (c + i < n && to >= 0 && tid < D) {
+          if (last) a.out[to * D + h * 128 + tid] = __float2bfloat16(o[i] * by[i]);
+          else a.acc[to * D + h * 128 + tid] = o[i];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  return ok;
 }
 
 template <int D>
@@ -273,16 +546,22 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (threadIdx.x == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
     return;
   }
-  uint8_t *sQ = smem, *ring = smem + C::Q_BYTES;
+  uint8_t *sQ = smem, *ring = smem + C::Q_BYTES + C::EXTRA;
   Bars* bars = reinterpret_cast<Bars*>(ring + C::RING * C::SLOT);
   Lists& lists = *reinterpret_cast<Lists*>(bars + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     bars->poisoned = *reinterpret_cast<volatile int*>(a.err);
     for (int i = 0; i < C::RING; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars->s_full[i], 1); mbar_init(&bars->p_full[i], 4); }
-    mbar_init(&bars->q_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1); mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->wk_full[i], 1); mbar_init(&bars->wk_empty[i], 1); mbar_init(&bars->wv_full[i], 1); mbar_init(&bars->wv_empty[i], 1);
+      mbar_init(&bars->wq_full[i], 1); mbar_init(&bars->wq_empty[i], 5);       // (the products' end, and the softmax's four warps)
+      mbar_init(&bars->ws_full[i], 1); mbar_init(&bars->wp_full[i], 4);
+    }
+    mbar_init(&bars->tall_full, 4);
     mbar_init(&bars->done, 1);
+    mbar_init(&bars->w_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -290,84 +569,104 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   __syncthreads();
   if (bars->poisoned != 0) return;
   if (warp == MMA_WARP) { tmem_alloc(&bars->tmem, C::TM_COLS); tmem_relinquish(); }
+  if (warp == TMA_WARP && lane == 0) { tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
   make_lists(lists, a, tid, warp, lane);
-  if (blockIdx.x == 0) write_plan(lists, a, tid);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   volatile int* abort_flag = &bars->abort_flag;
-  const int chunks = (a.heads / a.kv_heads + BM - 1) / BM;
-  const int units = lists.prefix_units + lists.own[a.rows] * a.kv_heads * chunks;
-  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(blockIdx.x) * lists.per_cta)), u1 = min(units, u0 + lists.per_cta);
+  auto share = [&](int units, int per, int cta, int& u0, int& u1) {
+    u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(cta) * per));
+    u1 = min(units, u0 + per);
+  };
+  int u0, u1, v0, v1;
+  share(lists.tall_units, lists.tall_per_cta, blockIdx.x, u0, u1);
+  share(lists.wide_units, lists.wide_per_cta, blockIdx.x, v0, v1);
+  bool ok = true;
+  // pool row of the box of `box` tokens that holds `key`, by the table of a row
+  auto pool_row = [&](const int* table, int key) -> int {
+    const int page = table[key / a.page_size];
+    if (page < 0 || page >= a.pages) {            // past the pool's end: zeros
+      atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+      return a.pages * a.page_size;
+    }
+    return page * a.page_size + key % a.page_size;
+  };
 
-  if (warp == TMA_WARP) {
-    // ------------------------------------------------------------------ TMA: a list's K0 K1 V0 K2 V1 ... V(n-1); a lane a box of rows
-    if (lane == 0) { tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
+  // ------------------------------------------------------------------------------------------------------ tall lists
+  if (const int total = u1 - u0; total == 0) {
+  } else if (warp == TMA_WARP) {
+    // K(0) K(1) V(0) K(2) V(1) ... V(total - 1); a lane a box of rows
     int slot = 0;
     uint32_t phase = 1;
-    bool ok = true;
     const int boxes = BN / a.box;
-    for (int u = u0; u < u1 && ok;) {
-      const Item w = locate(lists, a, u, u1);
-      u += w.tiles;
-      const int* table = a.table + static_cast<long long>(w.row) * a.max_pages;
-      int row0 = 0, row1 = 0;                     // pool rows of this lane's box of the last two tiles asked for (even, odd)
-      unsigned some0 = 0, some1 = 0;              // lanes whose box holds a key of the list
-      auto fetch = [&](const CUtensorMap* map, int row, unsigned lanes) -> bool {
-        if (!mbar_wait_warp(&bars->empty[slot], phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); return false; }
-        if (lane == 0) mbar_expect_tx(&bars->full[slot], static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
-        __syncwarp();
-        if (lanes >> lane & 1) {
-          uint8_t* to = ring + slot * C::SLOT + lane * a.box * 128;
+    int pool_row0 = 0, pool_row1 = 0, hk0 = 0, hk1 = 0;   // of the last even and odd tile whose keys were asked for
+    unsigned lanes0 = 0, lanes1 = 0;
+    auto fetch = [&](const CUtensorMap* map, int row, unsigned lanes, int hk) -> bool {
+      if (!mbar_wait_warp(&bars->empty[slot], phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); return false; }
+      if (lane == 0) mbar_expect_tx(&bars->full[slot], static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
+      __syncwarp();
+      if (lanes >> lane & 1) {
+        uint8_t* to = ring + slot * C::SLOT + lane * a.box * 128;
 #pragma unroll
-          for (int t = 0; t < C::SUB; ++t) tma_load_2d(to + t * (BN * 128), map, &bars->full[slot], w.hk * D + t * 64, row);
-        }
-        __syncwarp();
-        if (++slot == C::RING) { slot = 0; phase ^= 1; }
-        return true;
-      };
-      auto keys = [&](int j) -> bool {
-        const int key0 = w.keys.tile(w.from + j) * BN + lane * a.box;
-        bool any = false;
-        int row = 0;
-        if (lane < boxes) {
-          any = (key0 < w.keys.a1 && key0 + a.box > w.keys.a0 && w.keys.a1 > w.keys.a0) || (key0 < w.keys.b1 && key0 + a.box > w.keys.b0 && w.keys.b1 > w.keys.b0);
-          if (any) {
-            int page = table[key0 / a.page_size];
-            if (page < 0 || page >= a.pages) {    // past the pool's end: zeros
-              atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
-              row = a.pages * a.page_size;
-            } else {
-              row = page * a.page_size + key0 % a.page_size;
-            }
-          }
-        }
-        const unsigned some = __ballot_sync(FULL, any);
-        if (j & 1) { row1 = row; some1 = some; } else { row0 = row; some0 = some; }
-        return fetch(&tk, row, some);
-      };
-      ok = keys(0) && (w.tiles < 2 || keys(1));
-      for (int j = 0; ok && j < w.tiles; ++j) {
-        ok = fetch(&tv, j & 1 ? row1 : row0, j & 1 ? some1 : some0);
-        if (ok && j + 2 < w.tiles) ok = keys(j + 2);
+        for (int p = 0; p < C::SUB; ++p) tma_load_2d(to + p * (BN * 128), map, &bars->full[slot], hk * D + p * 64, row);
       }
+      __syncwarp();
+      if (++slot == C::RING) { slot = 0; phase ^= 1; }
+      return true;
+    };
+    Item w = locate<true>(lists, a, u0, u1);
+    int u = u0, j = 0;                            // the next tile whose keys are asked for: tile j of w's piece, unit u
+    auto keys = [&](int t) -> bool {
+      if (j == w.tiles) {
+        advance<true>(w, lists, a, u, u1);
+        j = 0;
+      }
+      const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
+      const bool any = lane < boxes && w.keys.meets(key, a.box);
+      const int row = any ? pool_row(a.table + static_cast<long long>(w.row) * a.max_pages, key) : 0;
+      const unsigned lanes = __ballot_sync(FULL, any);
+      if (t & 1) { pool_row1 = row; lanes1 = lanes; hk1 = w.hk; } else { pool_row0 = row; lanes0 = lanes; hk0 = w.hk; }
+      ++j;
+      ++u;
+      return fetch(&tk, row, lanes, w.hk);
+    };
+    ok = keys(0) && (total < 2 || keys(1));
+    for (int t = 0; ok && t < total; ++t) {
+      ok = t & 1 ? fetch(&tv, pool_row1, lanes1, hk1) : fetch(&tv, pool_row0, lanes0, hk0);
+      if (ok && t + 2 < total) ok = keys(t + 2);
     }
   } else if (warp == MMA_WARP) {
-    // ------------------------------------------------------------------ tensor cores (the warp waits together, one lane issues)
+    // over the tiles of all lists: S(0) S(1) PV(0) S(2) PV(1) ... (the warp waits together, one lane issues)
     constexpr uint32_t idesc_qk = make_idesc(BM, BN, 1, 1, 0, 0);
     constexpr uint32_t idesc_pv = make_idesc(BM, D, 1, 1, 0, 1);
     int slot = 0;
-    uint32_t phase = 0, q_phase = 0, p_phase = 0;  // (p_phase: a bit for each buffer)
-    bool ok = true;
-    const uint32_t qa = smem_u32(sQ);
+    uint32_t phase = 0, p_phase = 0;              // (p_phase: a bit for each buffer)
     auto take = [&](int& at) -> bool {
       at = slot;
       if (!mbar_wait_warp(&bars->full[slot], phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); return false; }
       if (++slot == C::RING) { slot = 0; phase ^= 1; }
       return true;
     };
-    auto scores = [&](int b) -> bool {
+    Item w = locate<true>(lists, a, u0, u1);
+    int u = u0, j = 0;                            // as for the keys
+    uint32_t tall_phase = 0, fresh = 0;           // (fresh: a bit for each buffer, whether its tile is its list's first)
+    const uint32_t qa = smem_u32(sQ);
+    auto scores = [&](int t) -> bool {
+      const int b = t & 1;
+      if (j == w.tiles) {
+        advance<true>(w, lists, a, u, u1);
+        j = 0;
+      }
+      fresh &= ~(1u << b);
+      if (j == 0) {
+        if (!mbar_wait_warp(&bars->tall_full, tall_phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); return false; }
+        tall_phase ^= 1;
+        fresh |= 1u << b;
+      }
+      ++j;
+      ++u;
       int at;
       if (!take(at)) return false;
       tc_fence_after();
@@ -383,68 +682,55 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       __syncwarp();
       return true;
     };
-    for (int u = u0; u < u1 && ok;) {
-      const Item w = locate(lists, a, u, u1);
-      u += w.tiles;
-      ok = mbar_wait_warp(&bars->q_full, q_phase, abort_flag);
-      if (!ok) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); break; }
-      q_phase ^= 1;
-      ok = scores(0) && (w.tiles < 2 || scores(1));
-      for (int j = 0; ok && j < w.tiles; ++j) {
-        const int b = j & 1;
-        int at;
-        ok = take(at);
-        if (!ok) break;
-        if (!mbar_wait_warp(&bars->p_full[b], p_phase >> b & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
-        p_phase ^= 1u << b;
-        tc_fence_after();
-        const uint32_t va = smem_u32(ring + at * C::SLOT);
-        if (elect_one()) {
+    ok = scores(0) && (total < 2 || scores(1));
+    for (int t = 0; ok && t < total; ++t) {
+      const int b = t & 1;
+      int at;
+      ok = take(at);
+      if (!ok) break;
+      if (!mbar_wait_warp(&bars->p_full[b], p_phase >> b & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+      p_phase ^= 1u << b;
+      tc_fence_after();
+      const uint32_t va = smem_u32(ring + at * C::SLOT);
+      const uint32_t add = fresh >> b & 1 ? 0u : 1u;
+      if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 || j > 0 ? 1u : 0u);
-          umma_commit(&bars->done);
-          umma_commit(&bars->empty[at]);
-        }
-        __syncwarp();
-        if (j + 2 < w.tiles) ok = scores(b);
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 ? 1u : add);
+        umma_commit(&bars->done);
+        umma_commit(&bars->empty[at]);
       }
+      __syncwarp();
+      if (t + 2 < total) ok = scores(t + 2);
     }
   } else {
-    // ------------------------------------------------------------------ softmax, queries, results
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t t_s = tmem + lane_addr, t_o = tmem + lane_addr + C::TM_O;
-    uint32_t s_phase = 0;                          // (a bit for each buffer)
-    int taken = 0, products = 0;                  // slots of the ring, and products with values, before this list
-    bool ok = true;
+    uint32_t s_phase = 0;                         // (a bit for each buffer)
     auto queries = [&](const Item& w) {
-      constexpr int PIECES = D / 8;
-      for (int i = tid; i < w.n * PIECES; i += BM) {
-        const int x = i / PIECES, c = i - x * PIECES;
-        int row, head;
-        query(lists, w, x, row, head);
-        const uint4 v = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.q + row * a.q_stride + static_cast<long long>(head) * D) + c);
-        *reinterpret_cast<uint4*>(sQ + (c >> 3) * (BM * 128) + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v;
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->q_full);
+      fetch_queries<D, 4>(sQ, BM * 128, lists, a, w, tid, BM);
+      if (lane == 0) mbar_arrive(&bars->tall_full);
     };
-    Item w;
-    if (u0 < u1) {
-      w = locate(lists, a, u0, u1);
-      queries(w);
+    const Item& w = lists.now[warp];
+    {
+      const Item first = locate<true>(lists, a, u0, u1);
+      if (lane == 0) lists.now[warp] = first;
+      queries(first);
+      __syncwarp();
     }
-    for (int u = u0; u < u1 && ok;) {
+    for (int t = 0; t < total && ok;) {
       const bool active = warp * 32 < w.n, mine = tid < w.n;
+      const int tiles = w.tiles;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < w.tiles; ++j) {
-        const int b = j & 1;
+      for (int j = 0; j < tiles; ++j, ++t) {
+        const int b = t & 1;
         if (!mbar_wait_warp(&bars->s_full[b], s_phase >> b & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_TMEM_FULL)); ok = false; break; }
         s_phase ^= 1u << b;
         tc_fence_after();
-        const int tile = w.keys.tile(w.from + j);
-        const bool whole = w.keys.whole(tile);
+        // which of the tile's keys the list sees
+        const int key0 = w.keys.tile<BN>(w.from + j) * BN;
+        const uint32_t sees[2] = {__ballot_sync(FULL, w.keys.sees(key0 + lane)), __ballot_sync(FULL, w.keys.sees(key0 + 32 + lane))};
+        const bool whole = (sees[0] & sees[1]) == FULL;
         if (active) {
           float s[BN];
           {
@@ -463,7 +749,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
           if (!whole) {
 #pragma unroll
-            for (int x = 0; x < BN; ++x) s[x] = w.keys.sees(tile * BN + x) ? s[x] : -INFINITY;
+            for (int x = 0; x < BN; ++x) s[x] = sees[x >> 5] >> (x & 31) & 1 ? s[x] : -INFINITY;
           }
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -477,7 +763,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (need) { m = m_new; l *= by; }
             if (j > 0) {
               // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
-              if (!mbar_wait_warp(&bars->done, (products + j - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+              if (!mbar_wait_warp(&bars->done, (t - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
               tc_fence_after();
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
@@ -491,7 +777,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
           }
           const float base = m == -INFINITY ? 0.f : m;
-          float sum[2] = {0.f, 0.f};
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[16];
@@ -499,21 +785,25 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             for (int x = 0; x < 16; ++x) {
               const float p0 = fast_exp2(s[c * 32 + 2 * x] - base), p1 = fast_exp2(s[c * 32 + 2 * x + 1] - base);
               pk[x] = pack_bf16(p0, p1);
-              sum[0] += p0;
-              sum[1] += p1;
+              sum[2 * c] += p0;
+              sum[2 * c + 1] += p1;
             }
             tmem_st_32x32b_x16(t_s + b * BN + c * 16, pk);
           }
-          l += sum[0] + sum[1];
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_st_wait();
         }
         if (!whole) {
-          // values that nobody sees, to zero: they stand in the slot that the j-th value tile of the list has
-          const int at = taken + (j + 1 < w.tiles ? 2 + 2 * j : 2 * w.tiles - 1), slot = at % C::RING;
+          // values that nobody sees, to zero, in the slot that the t-th value tile has
+          const int at = t + 1 < total ? 2 + 2 * t : 2 * total - 1, slot = at % C::RING;
           if (!mbar_wait_warp(&bars->full[slot], (at / C::RING) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; break; }
-          for (int i = tid; i < BN * C::SUB * 8; i += BM) {
-            const int x = (i >> 3) % BN;
-            if (!w.keys.sees(tile * BN + x)) *reinterpret_cast<uint4*>(ring + slot * C::SLOT + i * 16) = make_uint4(0, 0, 0, 0);
+          const int x = tid >> 1;                 // a key's values by two threads
+          if (!((x < 32 ? sees[0] : sees[1]) >> (x & 31) & 1)) {
+#pragma unroll
+            for (int p = 0; p < C::SUB; ++p)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<uint4*>(ring + slot * C::SLOT + p * (BN * 128) + x * 128 + ((tid & 1) * 4 + c) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
         }
@@ -522,50 +812,156 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (lane == 0) mbar_arrive(&bars->p_full[b]);
       }
       if (!ok) break;
-      taken += 2 * w.tiles;
-      products += w.tiles;
-      u += w.tiles;
-      // all of this list's scores are made: the next one's queries may take their place
-      const Item now = w;
-      if (u < u1) {
-        w = locate(lists, a, u, u1);
-        queries(w);
+      // where the result goes (a piece of a list in a place of the CTA's)
+      float* to = nullptr;
+      if (mine) {
+        int row, head;
+        query(lists, w, tid, row, head);
+        const long long at = tiles == w.units ? static_cast<long long>(row) * a.heads + head
+                                              : 2ll * a.rows * a.heads + static_cast<long long>(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * BM + tid;
+        if (row >= 0) {
+          a.ml[at] = make_float2(m, l);
+          to = a.acc + at * D;
+        }
       }
-      if (!mbar_wait_warp(&bars->done, (products - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+      // all of this list's scores are made, and those of the lists before: the next one's queries may take their place
+      if (t < total) {
+        Item next = w;
+        advance<true>(next, lists, a, u0 + t, u1);
+        __syncwarp();
+        if (lane == 0) lists.now[warp] = next;
+        queries(next);
+        __syncwarp();
+      }
+      if (!mbar_wait_warp(&bars->done, (t - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
       tc_fence_after();
       if (active) {
-        int row = -1, head = 0;
-        if (mine) query(lists, now, tid, row, head);
-        const long long one = static_cast<long long>(row) * a.heads + head, all = static_cast<long long>(a.rows) * a.heads;
-        const bool last = now.slot == -3;
-        const long long at = now.slot >= 0 ? 2 * all + static_cast<long long>(now.slot) * BM + tid : now.slot == -1 ? one : all + one;
-        float by = 1.f;
-        if (last) {
-          const float sink = a.sinks != nullptr && row >= 0 ? a.sinks[head] * LOG2E : -INFINITY;
-          const float top = fmaxf(m, sink), own = m > -INFINITY ? fast_exp2(m - top) : 0.f;
-          const float total = l * own + (sink > -INFINITY ? fast_exp2(sink - top) : 0.f);
-          by = total > 0.f || total != total ? own / total : 0.f;
-        } else if (row >= 0) {
-          a.ml[at] = make_float2(m, l);
-        }
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t v[32];
           tmem_ld_32x32b_x32(t_o + c * 32, v);
           tmem_ld_wait();
-          if (row >= 0) {
-            if (last) {
-              store_row_32<false>(a.out + one * D + c * 32, v, by);
-            } else {
-              store_row_32<false>(a.acc + at * D + c * 32, v, 1.f);
-            }
-          }
+          if (to != nullptr) store_row_32<false>(to + c * 32, v, 1.f);
           __syncwarp();
         }
       }
       tc_fence_before();
     }
   }
+
+  // ------------------------------------------------------------------------------------------------------ wide lists, in the same memory
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (*abort_flag != 0) ok = false;
+  uint8_t *w_keys = ring, *w_values = ring + C::W_SLOTS * C::W_TILE, *w_weights = sQ + 2 * C::W_Q;
+  if (const int total = v1 - v0; total == 0 || !ok) {
+  } else if (warp == TMA_WARP) {
+    // K(0) V(0) K(1) V(1) ...
+    const int boxes = WK / a.box;
+    auto fetch = [&](const CUtensorMap* map, uint8_t* to, uint64_t* full, uint64_t* empty, int t, int row, unsigned lanes, int hk) -> bool {
+      const int slot = t % C::W_SLOTS;
+      if (!mbar_wait_warp(&empty[slot], ((t / C::W_SLOTS) & 1) ^ 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); return false; }
+      if (lane == 0) mbar_expect_tx(&full[slot], static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
+      __syncwarp();
+      if (lanes >> lane & 1) {
+#pragma unroll
+        for (int p = 0; p < C::SUB; ++p) tma_load_2d(to + slot * C::W_TILE + lane * a.box * 128 + p * (WK * 128), map, &full[slot], hk * D + p * 64, row);
+      }
+      __syncwarp();
+      return true;
+    };
+    Item w = locate<false>(lists, a, v0, v1);
+    for (int t = 0, list = 0, j = 0; ok && t < total; ++t, ++j) {
+      const bool begins = j == w.tiles || t == 0;
+      if (j == w.tiles) {
+        advance<false>(w, lists, a, v0 + t, v1);
+        j = 0;
+      }
+      const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
+      const bool any = lane < boxes && w.keys.meets(key, a.box);
+      const int row = any ? pool_row(a.table + static_cast<long long>(w.row) * a.max_pages, key) : 0;
+      const unsigned lanes = __ballot_sync(FULL, any);
+      ok = fetch(&tk, w_keys, bars->wk_full, bars->wk_empty, t, row, lanes, w.hk);
+      if (ok && begins) {
+        const int q = list & 1;
+        ok = mbar_wait_warp(&bars->wq_empty[q], ((list >> 1) & 1) ^ 1, abort_flag);
+        if (!ok) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); break; }
+        if (lane == 0) lists.item[q] = w;
+        fetch_queries<D, 4>(sQ + q * C::W_Q, WN * 128, lists, a, w, lane, 32);
+        if (lane == 0) mbar_arrive(&bars->wq_full[q]);
+        ++list;
+      }
+      ok = ok && fetch(&tv, w_values, bars->wv_full, bars->wv_empty, t, row, lanes, w.hk);
+    }
+  } else if (warp == MMA_WARP) {
+    // S(0) S(1) PV(0) S(2) PV(1) ...
+    constexpr uint32_t idesc_s[2] = {make_idesc(WK, 16, 1, 1, 0, 0), make_idesc(WK, 32, 1, 1, 0, 0)};
+    constexpr uint32_t idesc_o[2] = {make_idesc(128, 16, 1, 1, 1, 0), make_idesc(128, 32, 1, 1, 1, 0)};
+    int list = -1, j = 0, tiles = 0;
+    bool more = false;                            // than 16 queries
+    uint32_t flags = 0;                           // bits b: whether the tile in buffer b is its list's first, 2 + b: whether its list has more than 16 queries
+    auto scores = [&](int t) -> bool {
+      const int b = t & 1, slot = t % C::W_SLOTS;
+      if (j == tiles) {
+        ++list;
+        if (!mbar_wait_warp(&bars->wq_full[list & 1], (list >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); return false; }
+        tiles = lists.item[list & 1].tiles;
+        more = lists.item[list & 1].n > 16;
+        j = 0;
+      }
+      flags = (flags & ~(5u << b)) | ((j == 0 ? 1u : 0u) | (more ? 4u : 0u)) << b;
+      ++j;
+      if (!mbar_wait_warp(&bars->wk_full[slot], (t / C::W_SLOTS) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); return false; }
+      tc_fence_after();
+      const uint32_t ka = smem_u32(w_keys + slot * C::W_TILE), qa = smem_u32(sQ + (list & 1) * C::W_Q), idesc = more ? idesc_s[1] : idesc_s[0];
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16_ss(tmem + b * WN, make_sdesc_sw128(ka + (kk >> 2) * (WK * 128) + (kk & 3) * 32, 16, 1024),
+                       make_sdesc_sw128(qa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+        umma_commit(&bars->ws_full[b]);
+        umma_commit(&bars->wk_empty[slot]);
+        if (j == tiles) umma_commit(&bars->wq_empty[list & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    ok = scores(0);
+    for (int t = 0; ok && t < total; ++t) {
+      if (t + 1 < total && !scores(t + 1)) { ok = false; break; }
+      const int b = t & 1, slot = t % C::W_SLOTS;
+      if (!mbar_wait_warp(&bars->wv_full[slot], (t / C::W_SLOTS) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; break; }
+      if (!mbar_wait_warp(&bars->wp_full[b], (t >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+      tc_fence_after();
+      const uint32_t va = smem_u32(w_values + slot * C::W_TILE), pa = smem_u32(w_weights + b * C::W_P);
+      const uint32_t idesc = flags >> (2 + b) & 1 ? idesc_o[1] : idesc_o[0], add = flags >> b & 1 ? 0u : 1u;
+      if (elect_one()) {
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+          for (int kk = 0; kk < WK / 16; ++kk)    // (a head of 64 fills half of the rows: the others are of whatever follows)
+            umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
+                         make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
+        umma_commit(&bars->w_done);
+        umma_commit(&bars->wv_empty[slot]);
+      }
+      __syncwarp();
+    }
+  } else {
+    const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+    const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, bars, abort_flag, tid, warp, lane};
+    for (int t = 0, list = 0; t < total; ++list) {
+      const int q = list & 1;
+      if (!mbar_wait_warp(&bars->wq_full[q], (list >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
+      if (any_of_128(!ok)) break;                 // (all warps or none)
+      const Item& w = lists.item[q];               // (not a copy: the registers are for scores)
+      ok = w.n <= 8 ? wide_list<D, 8>(x, lists, a, w, t) : w.n <= 16 ? wide_list<D, 16>(x, lists, a, w, t) : wide_list<D, 32>(x, lists, a, w, t);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->wq_empty[q]);
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1) write_plan(lists, a, tid);
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) {
@@ -577,42 +973,36 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 
 // A CTA a (place, key head), a warp a query: the pieces of its group's list and of its row's.
 template <int D>
-__global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a, int ctas) {
   const int place = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ratio = a.heads / a.kv_heads, chunks = (ratio + BM - 1) / BM;
-  const int* p = a.plan;
-  const int per = p[0], prefix_units = p[1];
-  p += 2;
-  const int own0 = p[place], own_tiles = p[place + 1] - own0;
-  p += a.rows + 1;
-  const int g = p[place];
-  p += a.rows;
-  const int at = p[g];
-  p += a.groups + 1;
-  const int tiles = p[g];
+  const int ratio = a.heads / a.kv_heads, chunks = (ratio + WN - 1) / WN;
   const int row = a.order[place];
+  const int4 lists = a.plan[2 * place], group = a.plan[2 * place + 1];
   if (row < 0 || row >= a.rows) return;
-  const bool rests = a.lengths[row] <= 0;
-  const int begin = max(0, a.first[g]), queries = (min(a.rows, a.first[g + 1]) - begin) * ratio, tall = (queries + BM - 1) / BM;
-  const long long all = static_cast<long long>(a.rows) * a.heads;
+  const bool rests = a.lengths[row] <= 0, tall = group.y > 0;
+  const int pieces = (group.y + BM - 1) / BM;
+  const long long all = static_cast<long long>(a.rows) * a.heads, wide0 = 2 * all + static_cast<long long>(ctas) * 2 * BM;
   constexpr int EACH = D / 32;
   for (int h = warp; h < ratio; h += 4) {
     const int head = hk * ratio + h;
     const long long one = static_cast<long long>(row) * a.heads + head;
-    // the two lists: first unit, tiles, lane
-    const int x = (place - begin) * ratio + h, c = h / BM;
-    const int start[2] = {at + (hk * tall + x / BM) * tiles, prefix_units + own0 * a.kv_heads * chunks + (hk * chunks + c) * own_tiles};
-    const int n[2] = {rests ? 0 : tiles, rests ? 0 : own_tiles}, in[2] = {x % BM, h - c * BM};
-    if (n[0] == 0 && n[1] > 0 && start[1] / per == (start[1] + n[1] - 1) / per) continue;      // finished
+    // the two lists: units a CTA, first unit, tiles, where a CTA's pieces are and how tall, lane
+    const int x = (place - group.x) * ratio + h, c = h / WN;
+    const int per[2] = {tall ? group.z : group.w, group.w};
+    const int start[2] = {lists.x + (tall ? hk * pieces + x / BM : hk) * lists.y, lists.z + (hk * chunks + c) * lists.w};
+    const int n[2] = {rests ? 0 : lists.y, rests ? 0 : lists.w};
+    const long long at[2] = {tall ? 2 * all + x % BM : wide0 + x, wide0 + h - c * WN};
+    const int step[2] = {tall ? BM : WN, WN};
+    if (n[0] == 0 && n[1] > 0 && start[1] / per[1] == (start[1] + n[1] - 1) / per[1]) continue;      // finished
     float top = a.sinks != nullptr ? a.sinks[head] * LOG2E : -INFINITY, sum = top > -INFINITY ? 1.f : 0.f, o[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) o[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (n[k] == 0) continue;
-      const int c0 = start[k] / per, c1 = (start[k] + n[k] - 1) / per;
+      const int c0 = start[k] / per[k], c1 = (start[k] + n[k] - 1) / per[k];
       for (int cta = c0; cta <= c1; ++cta) {
-        const long long from = c0 == c1 ? k * all + one : 2 * all + (2ll * cta + (cta == c0 ? 1 : 0)) * BM + in[k];
+        const long long from = c0 == c1 ? k * all + one : at[k] + (2ll * cta + (cta == c0 ? 1 : 0)) * step[k];
         const float2 ml = a.ml[from];
         float v[EACH];
 #pragma unroll
@@ -648,34 +1038,35 @@ int multiprocessors() {
 template <int D>
 int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas, cudaStream_t stream) {
   using C = Cfg<D>;
-  constexpr int SMEM = C::Q_BYTES + C::RING * C::SLOT + static_cast<int>(sizeof(Bars) + sizeof(Lists));
+  constexpr int SMEM = C::Q_BYTES + C::EXTRA + C::RING * C::SLOT + static_cast<int>(sizeof(Bars) + sizeof(Lists));
   static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "over an SM's shared memory");
   cudaError_t e = cudaFuncSetAttribute(shared_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
   if (e != cudaSuccess) return static_cast<int>(e);
   shared_mma_kernel<D><<<ctas, THREADS, SMEM, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
-  join_pieces_kernel<D><<<dim3(a.rows, a.kv_heads), 128, 0, stream>>>(a);
+  join_pieces_kernel<D><<<dim3(a.rows, a.kv_heads), 128, 0, stream>>>(a, ctas);
   return static_cast<int>(cudaGetLastError());
 }
 
 }  // namespace sharedmma
 }  // namespace dewb
 
-// CTAs of the first kernel on the current device (two pieces of 128 queries each are kept in scratch).
+// CTAs of the first kernel on the current device.
 extern "C" int dewb_shared_mma_ctas(int D) { return dewb::sharedmma::multiprocessors() * (D == 256 ? 1 : 2); }
 
-// As dewb_shared_decode, on the tensor cores: bf16, D 64, 128 or 256, page_size a multiple of 16, up to 512 rows and as many groups, everything 16-byte aligned and q_stride a
-// multiple of 8.  acc: (2 rows heads + 256 ctas) D floats; ml: as many pairs; plan: 2 rows + 2 groups + 4 integers.  A CTA takes at least `least` tiles.  Two launches.
+// As dewb_shared_decode, on the tensor cores: bf16, D 64, 128 or 256, page_size a multiple of 16, up to 448 rows and as many groups, everything 16-byte aligned and q_stride a
+// multiple of 8.  acc: (2 rows heads + 320 ctas) D floats; ml: as many pairs; plan: 8 rows integers on a 16-byte boundary.  A CTA takes at least `least` tiles of 128 keys.  Two launches.
 extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const void* k, const void* v, const int* table, const int* lengths, const int* order, const int* first,
-                                      const int* tokens, const float* sinks, float* acc, void* ml, int* plan, void* out, int rows, int heads, int kv_heads, int D, int page_size,
+                                      const int* tokens, const float* sinks, float* acc, void* ml, void* plan, void* out, int rows, int heads, int kv_heads, int D, int page_size,
                                       int max_pages, int pages, int groups, int window, int least, int ctas, float scale, float cap, int* err, void* stream_ptr) {
   using namespace dewb::sharedmma;
   if (rows <= 0) return 0;
-  const long long most = static_cast<long long>(max_pages) * page_size, chunks = heads > 0 && kv_heads > 0 ? (heads / kv_heads + BM - 1) / BM : 1;
+  const long long most = static_cast<long long>(max_pages) * page_size, chunks = heads > 0 && kv_heads > 0 ? (heads / kv_heads + WN - 1) / WN : 1;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || page_size % 16 != 0 || max_pages <= 0 || pages <= 0 || groups <= 0 || groups > MOST_ROWS ||
       rows > MOST_ROWS || window < 0 || least < 1 || ctas < 1 || most > 0x3fffffffll || static_cast<long long>(pages) * page_size > 0x7fffff00ll || kv_heads > 65535 ||
       (2ll * rows * chunks + groups) * kv_heads * ((most + BN - 1) / BN + 1) > 0x3fffffffll || q_stride % 8 != 0 ||
-      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc)) & 15))
+      ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc) |
+        reinterpret_cast<uintptr_t>(plan)) & 15))
     return -3;
   const int box = page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16;
   CUtensorMap tk, tv;
@@ -684,7 +1075,7 @@ extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const v
   if ((r = dewb::make_tmap_2d(&tk, k, tall, cols, cols, box, 64, 2, true))) return 1000 + r;
   if ((r = dewb::make_tmap_2d(&tv, v, tall, cols, cols, box, 64, 2, true))) return 2000 + r;
   const Args a{reinterpret_cast<const __nv_bfloat16*>(q), q_stride, table, lengths, order, first, tokens, sinks, reinterpret_cast<__nv_bfloat16*>(out), acc,
-               reinterpret_cast<float2*>(ml), plan, rows, heads, kv_heads, page_size, box, max_pages, pages, groups, window, least, scale * LOG2E, cap * LOG2E, err};
+               reinterpret_cast<float2*>(ml), reinterpret_cast<int4*>(plan), rows, heads, kv_heads, page_size, box, max_pages, pages, groups, window, least, scale * LOG2E, cap * LOG2E, err};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   if (D == 64) return launch<64>(tk, tv, a, ctas, stream);
   if (D == 128) return launch<128>(tk, tv, a, ctas, stream);

@@ -68,8 +68,8 @@ def shared_decode_reference(q, k, v, table, lengths, scale, window=None, softcap
     return torch.einsum("rghn,rngd->rghd", p, vr).reshape(R, H, D).to(q.dtype)
 
 
-LEAST_TILES = 4          # 64-key tiles that a CTA of the tensor cores' kernel takes at least
-MOST_ROWS = 512          # rows, and groups, that its lists hold
+LEAST_TILES = 2          # 128-key tiles that a CTA of the tensor cores' kernel takes at least
+MOST_ROWS = 448          # rows, and groups, that its lists hold
 _CTAS: Dict[Tuple[int, int], int] = {}
 
 
@@ -86,7 +86,7 @@ def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: 
     R, H, D = q.shape
     pages, page, G, _ = k.shape
     return (q.dtype == k.dtype == torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
-            and (2 * R * -(-H // G // 128) + groups) * G * (columns * page // 64 + 2) < 1 << 30
+            and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 2) < 1 << 30
             and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
 
 
@@ -147,9 +147,9 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
         with L.on_device_of(q) as stream:
             lib = L.load()
             ctas = _ctas(lib, q.device, D)
-            rows = 2 * R * H + 256 * ctas
+            rows = 2 * R * H + 320 * ctas
             # one piece of scratch a call: sums, maxima and sums of weights, the plan
-            scratch = torch.empty(rows * (D + 2) + 2 * (R + groups) + 4, dtype=fp32, device=q.device)
+            scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
             at = scratch.data_ptr()
             L.check(lib.dewb_shared_decode_mma(q.data_ptr(), q.stride(0) if R > 1 else H * D, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(),
                                                shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + 4 * rows * D, at + 4 * rows * (D + 2), out.data_ptr(),
