@@ -1,8 +1,8 @@
 // A decode step of rows that share prefixes, on the tensor cores: bf16 queries and pools, heads of 64, 128 or 256, pages of a multiple of 16 tokens.
 //
 // The work is lists: up to some number of queries (row, head) against a range of keys of one key head.  A group's shared keys (shared_range.cuh) make a list for each key head,
-// a row's own keys another.  There are two kinds, and all lists of a kind stand behind one another in one sequence of tiles that the CTAs share evenly: a list may begin in one
-// CTA and end in another.
+// a row's own keys another.  There are two kinds, each with CTAs of its own (as many as its share of the work, dealt over the SMs).  All lists of a kind stand behind one
+// another in one sequence of tiles that its CTAs share evenly: a list may begin in one CTA and end in another.
 //
 // TALL lists (a group of more than 32 queries on a key head, 128 of them a list): queries are the rows of the products.  Per 64 keys  S = Q K^T  (one of two score buffers in
 // tensor memory),  a thread a query makes the weights P over its scores,  O += P V  with P read from tensor memory.
@@ -13,7 +13,7 @@
 // threads until the list ends.
 //
 //   warps 0..3  softmax, results;  tall lists' queries
-//   warp 4      TMA: keys and values; wide lists' queries, and what the list is about, a list ahead
+//   warp 4      TMA: keys and values; finds out what the next list is about, and fetches wide lists' queries
 //   warp 5      tensor cores
 //
 // Two CTAs an SM (one at heads of 256), whose chains lie beside one another: an SM's share of the memory rate brings 64 keys and values of a head of 128 in 1400 cycles.
@@ -26,6 +26,7 @@
 // A list that is a row's whole attention is finished here.  Otherwise (m, l, sum) of a list, or of the piece of it that a CTA had, goes to scratch, and a second kernel joins
 // a query's pieces:  o = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i.  Scratch is bounded by queries and CTAs, whatever the keys' number: of each kind a CTA holds at most
 // two lists in part (its first and its last), the others' queries have a place of their own.  Nothing is counted with atomics: the same call gives the same bits.
+#include <cstddef>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -41,6 +42,7 @@ constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys o
 constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
 constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
 constexpr int MOST_ROWS = 448;
+constexpr int TALL_COST = 1, WIDE_COST = 2;        // of a tile, where CTAs are dealt
 constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t FULL = 0xffffffffu;
@@ -80,16 +82,17 @@ struct Item {
   int row;                                        // whose table
 };
 
-struct Bars {
-  uint64_t full[8], empty[8], tall_full, s_full[2], p_full[2], done;           // tall lists
-  uint64_t wk_full[2], wk_empty[2], wv_full[2], wv_empty[2], wq_full[2], wq_empty[2], ws_full[2], wp_full[2], w_done;      // wide lists
+struct alignas(16) Bars {
+  uint64_t list_full[2], list_empty[2];           // what a list is about (wide: and its queries)
+  uint64_t full[8], empty[8];                     // slots of the ring.  wide: [0, 2) keys, [2, 4) values
+  uint64_t q_full, s_full[2], p_full[2], done;
   uint32_t tmem;
   int abort_flag, poisoned;
 };
 
 // what a CTA knows of all lists
 struct Lists {
-  int tall_units, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;
+  int tall_units, tall_ctas, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;
   short first[MOST_ROWS + 2];                     // groups: first place
   short row[MOST_ROWS], group[MOST_ROWS];         // places (row -1: none)
   short through[MOST_ROWS];                       // groups: a row that holds something
@@ -97,13 +100,10 @@ struct Lists {
   int tall[MOST_ROWS + 1], wide[MOST_ROWS + 1];   // groups: units of either kind before
   int own[MOST_ROWS + 1];                         // places: own tiles before
   int len[MOST_ROWS];                             // places
-  union {
-    Item now[4];                                  // tall: the list at hand of each softmax warp (its registers are for a row of scores)
-    struct {
-      Item item[2];                               // wide: beside the lists' queries
-      float most[4][WN], sums[4][WN];             // the softmax's warps tell one another
-    };
-  };
+  Item item[2];                                   // the list at hand and the next one
+  float most[4][WN];                              // wide: largest scores, by warp
+  alignas(16) float top[4][WN], by[4][WN];        // (read four at a time) each warp's copy of the maxima in use, and what sums made with older ones are multiplied with
+  float sums[WN];                                 // of weights, and then what results are multiplied with
 };
 
 struct Args {
@@ -115,7 +115,7 @@ struct Args {
   float* acc;                                     // [2 rows heads + ctas (2 128 + 2 32)][D]
   float2* ml;                                     // [the same]: maximum (log2), sum
   int4* plan;                                     // [rows][2], for the second kernel: see write_plan
-  int rows, heads, kv_heads, page_size, box, max_pages, pages, groups, window, least;
+  int rows, heads, kv_heads, ratio, chunks, page_size, box, max_pages, pages, groups, window, least;      // (ratio: heads a key head; chunks of 32 of those)
   float scale_log2, cap_log2;
   int* err;
 };
@@ -130,6 +130,7 @@ __device__ __forceinline__ Ranges own_ranges(int len, int window, int lo, int hi
 template <typename T>
 __device__ __forceinline__ int last_at_most(const T* x, int n, int v) {        // largest i in [0, n) with x[i] <= v (x[0] <= v)
   int lo = 0, hi = n;
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (x[mid] <= v) lo = mid; else hi = mid;
@@ -137,116 +138,106 @@ __device__ __forceinline__ int last_at_most(const T* x, int n, int v) {        /
   return lo;
 }
 
-__device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * (a.heads / a.kv_heads); }
+// A wait that does not end at once, out of line: many places wait, and each launch reads its code anew.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait(bar, parity, abort_flag); }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code, int lane) {
+  if (__all_sync(FULL, mbar_try_wait(bar, parity))) return true;
+  if (__all_sync(FULL, wait_on(bar, parity, abort_flag))) return true;
+  if (lane == 0) atomicCAS(err, 0, code);
+  return false;
+}
 
-// index, shared, list and start are known: the rest, for the piece from unit u on; `same`: of the group or place of the list before.
+__device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * a.ratio; }
+
+// The list that unit u is of, up to `end`; unless `begins`, w is the one before.  One thread.
 template <bool TALL>
-__device__ __forceinline__ void fill(Item& w, const Lists& s, const Args& a, int u, int end, bool same) {
-  const int ratio = a.heads / a.kv_heads;
-  if (TALL || w.shared) {
-    const int queries = group_queries(s, a, w.index), pieces = TALL ? (queries + BM - 1) / BM : 1;
-    if (!same) {
-      w.keys = Ranges{s.lo[w.index], s.hi[w.index], 0, 0};
-      w.lists = a.kv_heads * pieces;
-      w.row = s.through[w.index];
-    }
-    w.hk = TALL ? w.list / pieces : w.list;
-    const int m0 = TALL ? (w.list - w.hk * pieces) * BM : 0;
-    w.place = s.first[w.index] * ratio + m0;
-    w.each = ratio;
-    w.head0 = w.hk * ratio;
-    w.n = min(TALL ? BM : WN, queries - m0);
+__device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, int u, int end, bool begins) {
+  const int* at = TALL ? s.tall : s.wide;
+  bool same = false;
+  if (begins) {
+    w.shared = TALL || u < s.wide_shared_units;
+    w.index = w.shared ? last_at_most(at, a.groups, u) : last_at_most(s.own, a.rows, (u - s.wide_shared_units) / (a.kv_heads * a.chunks));
+  } else if (++w.list < w.lists) {
+    same = true;
+    w.start = u;
   } else {
-    const int chunks = (ratio + WN - 1) / WN;
-    if (!same) {
+    if (!TALL && w.shared && u >= s.wide_shared_units) {
+      w.shared = false;
+      w.index = -1;
+    }
+    if (w.shared) {
+#pragma unroll 1
+      do ++w.index; while (at[w.index + 1] <= u);
+    } else {
+#pragma unroll 1
+      do ++w.index; while (s.own[w.index + 1] == s.own[w.index]);
+    }
+  }
+  if (!same) {
+    if (w.shared) {
+      w.keys = Ranges{s.lo[w.index], s.hi[w.index], 0, 0};
+      w.lists = a.kv_heads * (TALL ? (group_queries(s, a, w.index) + BM - 1) / BM : 1);
+      w.row = s.through[w.index];
+      w.start = at[w.index];
+      w.units = w.keys.tiles<TALL ? BN : WK>();
+    } else {
       const int g = s.group[w.index];
       w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g]);
-      w.lists = a.kv_heads * chunks;
+      w.lists = a.kv_heads * a.chunks;
       w.row = s.row[w.index];
+      w.start = s.wide_shared_units + s.own[w.index] * w.lists;
+      w.units = s.own[w.index + 1] - s.own[w.index];
     }
-    w.hk = chunks == 1 ? w.list : w.list / chunks;
-    const int c = w.list - w.hk * chunks;
-    w.n = w.each = min(WN, ratio - c * WN);
+    w.list = begins ? (u - w.start) / w.units : 0;
+    w.start += w.list * w.units;
+  }
+  if (w.shared) {
+    const int queries = group_queries(s, a, w.index), pieces = TALL ? (queries + BM - 1) / BM : 1;
+    w.hk = TALL ? w.list / pieces : w.list;
+    const int m0 = TALL ? (w.list - w.hk * pieces) * BM : 0;
+    w.place = s.first[w.index] * a.ratio + m0;
+    w.each = a.ratio;
+    w.head0 = w.hk * a.ratio;
+    w.n = min(TALL ? BM : WN, queries - m0);
+  } else {
+    w.hk = a.chunks == 1 ? w.list : w.list / a.chunks;
+    const int c = w.list - w.hk * a.chunks;
+    w.n = w.each = min(WN, a.ratio - c * WN);
     w.place = w.index * w.n;
-    w.head0 = w.hk * ratio + c * WN;
+    w.head0 = w.hk * a.ratio + c * WN;
   }
   w.from = u - w.start;
   w.tiles = min(end, w.start + w.units) - u;
 }
 
-// The piece that begins at unit u and ends with its list or before `end`.
-template <bool TALL>
-__device__ __forceinline__ Item locate(const Lists& s, const Args& a, int u, int end) {
-  Item w;
-  w.shared = TALL || u < s.wide_shared_units;
-  if (w.shared) {
-    const int* at = TALL ? s.tall : s.wide;
-    w.index = last_at_most(at, a.groups, u);
-    w.start = at[w.index];
-    w.units = Ranges{s.lo[w.index], s.hi[w.index], 0, 0}.tiles<TALL ? BN : WK>();
-  } else {
-    const int lists = a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
-    w.index = last_at_most(s.own, a.rows, (u - s.wide_shared_units) / lists);
-    w.start = s.wide_shared_units + s.own[w.index] * lists;
-    w.units = s.own[w.index + 1] - s.own[w.index];
-  }
-  w.list = (u - w.start) / w.units;
-  w.start += w.list * w.units;
-  fill<TALL>(w, s, a, u, end, false);
-  return w;
+// row * heads + head of a list's query i, -1 for none
+__device__ __forceinline__ int query(const Lists& s, const Args& a, const Item& w, int i) {
+  if (i >= w.n) return -1;
+  const int x = w.place + i, place = x / w.each, row = s.row[place];
+  return row < 0 ? -1 : row * a.heads + w.head0 + x - place * w.each;
 }
 
-// The list behind w's, which is in this CTA to its end; u: its first unit, before `end`.
-template <bool TALL>
-__device__ __forceinline__ void advance(Item& w, const Lists& s, const Args& a, int u, int end) {
-  w.start = u;
-  if (++w.list < w.lists) {
-    fill<TALL>(w, s, a, u, end, true);
-    return;
-  }
-  w.list = 0;
-  if (!TALL && w.shared && u >= s.wide_shared_units) {
-    w.shared = false;
-    w.index = -1;
-  }
-  if (TALL || w.shared) {
-    const int* at = TALL ? s.tall : s.wide;
-    do ++w.index; while (at[w.index + 1] <= u);
-    w.units = Ranges{s.lo[w.index], s.hi[w.index], 0, 0}.tiles<TALL ? BN : WK>();
-  } else {
-    do ++w.index; while (s.own[w.index + 1] == s.own[w.index]);
-    w.units = s.own[w.index + 1] - s.own[w.index];
-  }
-  fill<TALL>(w, s, a, u, end, false);
-}
-
-// the row and head of a list's query
-__device__ __forceinline__ void query(const Lists& s, const Item& w, int i, int& row, int& head) {
-  const int x = w.place + i;
-  const int place = x / w.each;
-  row = s.row[place];
-  head = w.head0 + x - place * w.each;
-}
-
-// Queries [.][D] to their rows (128-byte swizzle) of 64-column pieces `part` bytes apart, by `threads` threads.
-template <int D, int EACH>
-__device__ __forceinline__ void fetch_queries(uint8_t* to, int part, const Lists& s, const Args& a, const Item& w, int t, int threads) {
-  constexpr int PIECES = D / 8;
-  for (int i0 = t; i0 < w.n * PIECES; i0 += threads * EACH) {
+// A warp's up to 32 queries (lane i holds query()'s answer for number i) to rows of 128 bytes (128-byte swizzle), 64-column pieces `apart` bytes apart; `to`: the first's row,
+// on a 1024-byte boundary.
+template <int D>
+__device__ __forceinline__ void fetch_queries(uint8_t* to, int apart, const Args& a, int mine, int n, int lane) {
+  constexpr int PIECES = D / 8, ROWS = 32 / PIECES, EACH = 4;
+  const int row = mine / a.heads;
+  const long long from = mine < 0 ? -1 : row * a.q_stride + static_cast<long long>(mine - row * a.heads) * D;
+  const int c = lane % PIECES;
+#pragma unroll 1
+  for (int x0 = 0; x0 < n; x0 += ROWS * EACH) {
     uint4 v[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int i = i0 + e * threads, x = i / PIECES;
-      if (i >= w.n * PIECES) break;
-      int row, head;
-      query(s, w, x, row, head);
-      v[e] = row < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.q + row * a.q_stride + static_cast<long long>(head) * D) + i % PIECES);
+      const int x = x0 + e * ROWS + lane / PIECES;
+      const long long at = __shfl_sync(FULL, from, x & 31);
+      v[e] = x < n && at >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + at) + c) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-      const int i = i0 + e * threads, x = i / PIECES, c = i % PIECES;
-      if (i >= w.n * PIECES) break;
-      *reinterpret_cast<uint4*>(to + (c >> 3) * part + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[e];
+      const int x = x0 + e * ROWS + lane / PIECES;
+      if (x < n) *reinterpret_cast<uint4*>(to + (c >> 3) * apart + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[e];
     }
   }
   fence_proxy_async();
@@ -255,7 +246,8 @@ __device__ __forceinline__ void fetch_queries(uint8_t* to, int part, const Lists
 
 // What the second kernel needs of a place: its group's first unit and tiles (of either kind), its own; its group's first place and queries a key head (0: wide), units a CTA.
 __device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int tid) {
-  const int lists = a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
+  const int lists = a.kv_heads * a.chunks;
+#pragma unroll 1
   for (int i = tid; i < a.rows; i += THREADS) {
     const int g = s.group[i], queries = group_queries(s, a, g);
     const Ranges both{s.lo[g], s.hi[g], 0, 0};
@@ -269,6 +261,7 @@ __device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int ti
 __device__ __forceinline__ void running_sums(int* x, int n, int lane) {
   const int per = (n + 31) / 32, i0 = min(n, lane * per), i1 = min(n, i0 + per);
   int sum = 0;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) sum += x[i + 1];
   int to = sum;
 #pragma unroll
@@ -278,6 +271,7 @@ __device__ __forceinline__ void running_sums(int* x, int n, int lane) {
   }
   int run = to - sum;
   if (lane == 0) x[0] = 0;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) { run += x[i + 1]; x[i + 1] = run; }
 }
 
@@ -286,12 +280,10 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
   const int most = a.max_pages * a.page_size;
   int* live = s.own;                              // (until the places' tiles are known)
   // rows and lengths are on their way while the groups are looked at
-  int row_of[EACH], len_of[EACH];
+  int row_of[EACH];
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    const int i = e * THREADS + tid;
-    row_of[e] = i < a.rows ? a.order[i] : 0;
-  }
+  for (int e = 0; e < EACH; ++e) row_of[e] = e * THREADS + tid < a.rows ? a.order[e * THREADS + tid] : -1;
+#pragma unroll 1
   for (int g = tid; g <= a.groups; g += THREADS) {
     s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
     if (g == a.groups) break;
@@ -301,33 +293,36 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     s.through[g] = -1;
   }
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) len_of[e] = row_of[e] >= 0 && row_of[e] < a.rows ? a.lengths[row_of[e]] : 0;
-  __syncthreads();
-#pragma unroll
   for (int e = 0; e < EACH; ++e) {
     const int i = e * THREADS + tid;
-    if (e * THREADS + warp * 32 >= a.rows) break;
+    if (i >= a.rows) break;
+    const bool bad = row_of[e] < 0 || row_of[e] >= a.rows;
+    s.row[i] = static_cast<short>(bad ? -1 : row_of[e]);
+    s.len[i] = bad ? -1 : a.lengths[row_of[e]];
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i0 = warp * 32; i0 < a.rows; i0 += THREADS) {
+    const int i = i0 + lane;
     int g = -1, row = -1, len = 0;
     if (i < a.rows) {
       g = last_at_most(s.first, a.groups, i);
-      row = row_of[e];
-      bool bad = row < 0 || row >= a.rows;
-      if (i < s.first[g] || i >= s.first[g + 1]) { g = -1; bad = true; }
-      if (bad) {
-        row = -1;
-      } else {
-        bad = len_of[e] > most;
-        len = min(max(len_of[e], 0), most);
+      row = s.row[i];
+      len = s.len[i];
+      bool bad = row < 0 || len > most;
+      if (i < s.first[g] || i >= s.first[g + 1]) {
+        g = -1;
+        bad = true;
       }
+      len = g < 0 ? 0 : min(max(len, 0), most);
+      if (g < 0) s.row[i] = -1;
       if (bad && blockIdx.x == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
-      s.row[i] = static_cast<short>(row);
       s.group[i] = static_cast<short>(max(g, 0));
       s.len[i] = len;
     }
     // groups are neighbouring places: lanes of one group answer together
-    const bool holds = len > 0 && g >= 0;
-    const unsigned same = __match_any_sync(FULL, holds ? g : -1);
-    if (holds) {
+    const unsigned same = __match_any_sync(FULL, len > 0 ? g : -1);
+    if (len > 0) {
       const int lo = __reduce_max_sync(same, row_first(len, a.window)), hi = __reduce_min_sync(same, len);
       if (lane == __ffs(same) - 1) {
         atomicMax(&s.lo[g], lo);
@@ -338,6 +333,7 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     }
   }
   __syncthreads();
+#pragma unroll 1
   for (int g = tid; g < a.groups; g += THREADS) {
     if (live[g] < 2 || s.lo[g] >= s.hi[g]) s.lo[g] = s.hi[g] = 0;
     const int queries = group_queries(s, a, g);
@@ -346,21 +342,24 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * both.tiles<WK>();
   }
   __syncthreads();
+#pragma unroll 1
   for (int i = tid; i < a.rows; i += THREADS) s.own[i + 1] = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles<WK>();
-  if (warp == 1) running_sums(s.tall, a.groups, lane);
-  if (warp == 2) running_sums(s.wide, a.groups, lane);
   __syncthreads();
-  if (warp == 0) {
-    running_sums(s.own, a.rows, lane);
-    __syncwarp();
-    if (lane == 0) {
-      const int ctas = static_cast<int>(gridDim.x);
-      s.tall_units = s.tall[a.groups];
-      s.wide_shared_units = s.wide[a.groups];
-      s.wide_units = s.wide_shared_units + s.own[a.rows] * a.kv_heads * ((a.heads / a.kv_heads + WN - 1) / WN);
-      s.tall_per_cta = max(2 * a.least, (s.tall_units + ctas - 1) / ctas);
-      s.wide_per_cta = max(a.least, (s.wide_units + ctas - 1) / ctas);
-    }
+  if (warp < 3) running_sums(warp == 0 ? s.tall : warp == 1 ? s.wide : s.own, warp < 2 ? a.groups : a.rows, lane);
+  __syncthreads();
+  if (tid == 0) {
+    const int ctas = static_cast<int>(gridDim.x);
+    s.tall_units = s.tall[a.groups];
+    s.wide_shared_units = s.wide[a.groups];
+    s.wide_units = s.wide_shared_units + s.own[a.rows] * a.kv_heads * a.chunks;
+    // CTAs for either kind by their work
+    const long long tall = static_cast<long long>(s.tall_units) * TALL_COST, wide = static_cast<long long>(s.wide_units) * WIDE_COST;
+    int k = tall == 0 ? 0 : wide == 0 ? ctas : static_cast<int>((tall * ctas + (tall + wide) / 2) / (tall + wide));
+    if (tall > 0 && wide > 0) k = min(max(k, 1), ctas - 1);
+    s.tall_ctas = min(k, (s.tall_units + 2 * a.least - 1) / (2 * a.least));
+    s.tall_per_cta = s.tall_ctas == 0 ? 1 : (s.tall_units + s.tall_ctas - 1) / s.tall_ctas;
+    const int rest = max(1, ctas - s.tall_ctas);
+    s.wide_per_cta = max(a.least, (s.wide_units + rest - 1) / rest);
   }
   __syncthreads();
 }
@@ -373,6 +372,23 @@ __device__ __forceinline__ bool any_of_128(bool p) {       // whether p holds fo
 }
 __device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 
+// largest of a warp's values
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void tmem_ld_x4(uint32_t at, float (&x)[4]) {
+  uint32_t v[4];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at) : "memory");
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+}
+__device__ __forceinline__ void tmem_st_x4(uint32_t at, const float (&x)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(__float_as_uint(x[0])), "r"(__float_as_uint(x[1])), "r"(__float_as_uint(x[2])),
+               "r"(__float_as_uint(x[3])) : "memory");
+}
 template <int NC>
 __device__ __forceinline__ void load_columns(uint32_t at, float (&x)[NC]) {
   if constexpr (NC == 32) {
@@ -395,86 +411,95 @@ struct Wide {                                     // what a list's softmax works
   uint8_t *weights, *values;                      // shared memory
   Bars* bars;
   volatile int* abort_flag;
-  int tid, warp, lane;
+  int tid, warp, lane, cta;                       // (cta: among those of wide lists)
 };
 
 // One wide list of up to NC queries, whose first tile is the CTA's t-th: false after a wait that ran out.  (All warps pass all barriers, whatever went wrong: waits that
 // follow one that ran out return at once.)
+//
+// What runs once a list is written as loops: straight code comes from L2 at some 250 cycles a 128-byte line when a launch first runs it, and all CTAs of a launch are at
+// the same line.  (Unrolled over 32 queries, a launch's first maxima took 25000 cycles, and first results 6000.)
 template <int D, int NC>
 __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Args& a, const Item& w, int& t) {
   using C = Cfg<D>;
   Bars* bars = x.bars;
   const int tid = x.tid, lane = x.lane, warp = x.warp, tiles = w.tiles, n = w.n;
-  constexpr int PART = NC < 16 ? NC : 16;         // queries at a time where more would not fit the registers
+  float *top = lists.top[warp], *by = lists.by[warp];
   bool ok = true;
-  float m[NC], l[NC];                             // (l: of this thread's keys)
+  float l[NC];                                    // sums of this thread's keys' weights
 #pragma unroll
-  for (int q = 0; q < NC; ++q) { m[q] = -INFINITY; l[q] = 0.f; }
+  for (int q = 0; q < NC; ++q) l[q] = 0.f;
+  __syncwarp();
+  if (lane < NC) top[lane] = -INFINITY;
+  __syncwarp();
+#pragma unroll 1
   for (int j = 0; j < tiles; ++j, ++t) {
     const int b = t & 1;
-    if (!mbar_wait_warp(&bars->ws_full[b], (t >> 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_TMEM_FULL)); ok = false; }
+    ok = wait(&bars->s_full[b], (t >> 1) & 1, x.abort_flag, a.err, ERR_WAIT_TMEM_FULL, lane) && ok;
     tc_fence_after();
     const bool seen = w.keys.sees(w.keys.tile<WK>(w.from + j) * WK + tid);
     float s[NC];
     load_columns<NC>(x.t_s + b * WN, s);
+#pragma unroll
+    for (int q = 0; q < NC; ++q) s[q] *= a.scale_log2;
+    if (a.cap_log2 > 0.f) {
+      // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), in the log2 domain
+      const float twice = 2.f * LOG2E / a.cap_log2;
+#pragma unroll
+      for (int q = 0; q < NC; ++q) s[q] = fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + fast_exp2(s[q] * twice)), a.cap_log2);
+    }
     bool past = false;
 #pragma unroll
-    for (int q = 0; q < NC; ++q) {
-      s[q] *= a.scale_log2;
-      // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), in the log2 domain
-      if (a.cap_log2 > 0.f) s[q] = fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + fast_exp2(s[q] * (2.f * LOG2E / a.cap_log2))), a.cap_log2);
-      s[q] = seen ? s[q] : -INFINITY;
-      past = past || (q < n && s[q] > m[q] + RESCALE);
+    for (int q = 0; q < NC; q += 4) {
+      const float4 m = *reinterpret_cast<const float4*>(top + q);
+      past = past || (q < n && s[q] > m.x + RESCALE) || (q + 1 < n && s[q + 1] > m.y + RESCALE) || (q + 2 < n && s[q + 2] > m.z + RESCALE) || (q + 3 < n && s[q + 3] > m.w + RESCALE);
     }
-    if (any_of_128(past)) {
+    if (any_of_128(past && seen)) {
+      float mine = -INFINITY;
 #pragma unroll
       for (int q = 0; q < NC; ++q) {
-        float top = s[q];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-        if (lane == q) lists.most[warp][q] = top;
+        const float most = warp_max(seen ? s[q] : -INFINITY);
+        mine = lane == q ? most : mine;
       }
+      lists.most[warp][lane] = mine;
       sync_128();
-      // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
-      if (j > 0 && !mbar_wait_warp(&bars->w_done, (t - 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < NC; c += PART) {
-        float by[PART];
-#pragma unroll
-        for (int i = 0; i < PART; ++i) {
-          const int q = c + i;
-          const float now = fmaxf(m[q], fmaxf(fmaxf(lists.most[0][q], lists.most[1][q]), fmaxf(lists.most[2][q], lists.most[3][q])));
-          by[i] = m[q] > -INFINITY && q < n ? fast_exp2(m[q] - now) : 1.f;
-          m[q] = now;
-          l[q] *= by[i];
-        }
-        if (j == 0) continue;
-#pragma unroll
-        for (int h = 0; h < C::HALVES; ++h) {
-          uint32_t v[16];
-          tmem_ld_32x32b_x16(x.t_o + h * WN + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < PART; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * by[i]);
-          tmem_st_32x32b_x16(x.t_o + h * WN + c, v);
-        }
+      if (lane < NC) {
+        const float was = top[lane], now = fmaxf(was, fmaxf(fmaxf(lists.most[0][lane], lists.most[1][lane]), fmaxf(lists.most[2][lane], lists.most[3][lane])));
+        by[lane] = was > -INFINITY && lane < n ? fast_exp2(was - now) : 1.f;
+        top[lane] = now;
       }
-      tmem_st_wait();
+      __syncwarp();
+      if (j > 0) {
+#pragma unroll
+        for (int q = 0; q < NC; ++q) l[q] *= by[q];
+        // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
+        ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < C::HALVES * WN; c += 4) {
+          if ((c & (WN - 1)) >= n) continue;
+          float o[4];
+          tmem_ld_x4(x.t_o + c, o);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] *= by[(c & (WN - 1)) + i];
+          tmem_st_x4(x.t_o + c, o);
+        }
+        tmem_st_wait();
+      }
     }
     // weights: query q's row of 128 keys in two 64-key pieces (128-byte swizzle)
     uint8_t* to = x.weights + b * C::W_P + (tid >> 6) * (WN * 128) + (tid & 7) * 2;
 #pragma unroll
     for (int q = 0; q < NC; ++q) {
-      const float p = fast_exp2(s[q] - (m[q] == -INFINITY ? 0.f : m[q]));
+      const float m = top[q], p = seen ? fast_exp2(s[q] - (m == -INFINITY ? 0.f : m)) : 0.f;
       l[q] += p;
       *reinterpret_cast<__nv_bfloat16*>(to + q * 128 + ((((tid >> 3) & 7) ^ (q & 7)) << 4)) = __float2bfloat16(p);
     }
     if (__ballot_sync(FULL, !seen) != 0) {        // values that nobody sees, to zero (each thread its key's)
       const int slot = t % C::W_SLOTS;
-      if (!mbar_wait_warp(&bars->wv_full[slot], (t / C::W_SLOTS) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; }
+      ok = wait(&bars->full[2 + slot], (t / C::W_SLOTS) & 1, x.abort_flag, a.err, ERR_WAIT_FULL, lane) && ok;
       if (!seen) {
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < C::SUB; ++p)
 #pragma unroll
           for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(x.values + slot * C::W_TILE + p * (WK * 128) + tid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
@@ -483,56 +508,60 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
     fence_proxy_async();
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->wp_full[b]);
+    if (lane == 0) mbar_arrive(&bars->p_full[b]);
   }
-  // where the results go (lane q: query q's), and the sums of weights
+  // where the results go (lane q: query q's)
   const bool entire = tiles == w.units;
   const bool last = entire && !w.shared && lists.hi[lists.group[w.index]] == 0;
-  int row = -1, head = 0;
-  if (lane < n) query(lists, w, lane, row, head);
-  const long long one = static_cast<long long>(row) * a.heads + head, all = static_cast<long long>(a.rows) * a.heads;
-  long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * 2 * BM + (2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
-  if (row < 0) at = -1;
+  const int one = query(lists, a, w, lane);
+  const long long all = static_cast<long long>(a.rows) * a.heads;
+  long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * 2 * BM + (2 * x.cta + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
+  if (one < 0) at = -1;
+  ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
+  tc_fence_after();
+  // sums over the threads, through the weights' memory (all products with them are done): four threads a query, each every fourth thread's
+  float* part = reinterpret_cast<float*>(x.weights);
 #pragma unroll
-  for (int q = 0; q < NC; ++q) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l[q] += __shfl_xor_sync(FULL, l[q], o);
-    if (lane == q) lists.sums[warp][q] = l[q];
+  for (int q = 0; q < NC; ++q) part[q * WK + tid] = l[q];
+  sync_128();
+  {
+    const int q = tid >> 2;
+    float sum = 0.f;
+    if (q < n)
+#pragma unroll 4
+      for (int i = tid & 3; i < WK; i += 4) sum += part[q * WK + ((i + q * 4) & (WK - 1))];
+    sum += __shfl_xor_sync(FULL, sum, 1);
+    sum += __shfl_xor_sync(FULL, sum, 2);
+    if ((tid & 3) == 0) {
+      float scale = sum;
+      if (last && q < n) {
+        const float m = top[q], sink = a.sinks != nullptr ? a.sinks[w.head0 + q] * LOG2E : -INFINITY;
+        const float both = fmaxf(m, sink), own = m > -INFINITY ? fast_exp2(m - both) : 0.f;
+        const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - both) : 0.f);
+        scale = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
+      }
+      lists.sums[q] = scale;
+    }
   }
   sync_128();
-  if (!mbar_wait_warp(&bars->w_done, (t - 1) & 1, x.abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
-  tc_fence_after();
+  if (!last && warp == 0 && at >= 0) a.ml[at] = make_float2(top[lane], lists.sums[lane]);
+#pragma unroll 1
+  for (int c = 0; c < C::HALVES * WN; c += 4) {
+    const int q = c & (WN - 1);
+    if (q >= n) continue;
+    float o[4];
+    tmem_ld_x4(x.t_o + c, o);
 #pragma unroll
-  for (int c = 0; c < NC; c += PART) {
-    float by[PART];                               // what the results are multiplied with
-#pragma unroll
-    for (int i = 0; i < PART; ++i) {
-      const int q = c + i;
-      const float sum = (lists.sums[0][q] + lists.sums[1][q]) + (lists.sums[2][q] + lists.sums[3][q]);
-      by[i] = 1.f;
-      if (last) {
-        const float sink = a.sinks != nullptr && q < n ? a.sinks[w.head0 + q] * LOG2E : -INFINITY;
-        const float top = fmaxf(m[q], sink), own = m[q] > -INFINITY ? fast_exp2(m[q] - top) : 0.f;
-        const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - top) : 0.f);
-        by[i] = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
-      } else if (tid == q && at >= 0) {
-        a.ml[at] = make_float2(m[q], sum);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < C::HALVES; ++h) {
-      float o[PART];
-      load_columns<PART>(x.t_o + h * WN + c, o);
-#pragma unroll
-      for (int i = 0; i < PART; ++i) {
-        const long long to = __shfl_sync(FULL, at, c + i);
-        if (c + i < n && to >= 0 && tid < D) {
-          if (last) a.out[to * D + h * 128 + tid] = __float2bfloat16(o[i] * by[i]);
-          else a.acc[to * D + h * 128 + tid] = o[i];
-        }
+    for (int i = 0; i < 4; ++i) {
+      const long long to = __shfl_sync(FULL, at, q + i);
+      if (q + i < n && to >= 0 && tid < D) {
+        const long long place = to * D + (c / WN) * 128 + tid;
+        if (last) a.out[place] = __float2bfloat16(o[i] * lists.sums[q + i]);
+        else a.acc[place] = o[i];
       }
     }
   }
+  sync_128();                                     // (the weights' memory and the sums are the next list's)
   tc_fence_before();
   return ok;
 }
@@ -550,18 +579,18 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   Bars* bars = reinterpret_cast<Bars*>(ring + C::RING * C::SLOT);
   Lists& lists = *reinterpret_cast<Lists*>(bars + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t *w_keys = ring, *w_values = ring + C::W_SLOTS * C::W_TILE, *w_weights = sQ + 2 * C::W_Q;
   if (tid == 0) {
     bars->poisoned = *reinterpret_cast<volatile int*>(a.err);
     for (int i = 0; i < C::RING; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->s_full[i], 1); mbar_init(&bars->p_full[i], 4);
-      mbar_init(&bars->wk_full[i], 1); mbar_init(&bars->wk_empty[i], 1); mbar_init(&bars->wv_full[i], 1); mbar_init(&bars->wv_empty[i], 1);
-      mbar_init(&bars->wq_full[i], 1); mbar_init(&bars->wq_empty[i], 5);       // (the products' end, and the softmax's four warps)
-      mbar_init(&bars->ws_full[i], 1); mbar_init(&bars->wp_full[i], 4);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->list_full[i], 1);
+      mbar_init(&bars->list_empty[i], 5);         // (the tensor cores' warp, and the softmax's four)
     }
-    mbar_init(&bars->tall_full, 4);
+    mbar_init(&bars->q_full, 4);
     mbar_init(&bars->done, 1);
-    mbar_init(&bars->w_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -576,156 +605,174 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   volatile int* abort_flag = &bars->abort_flag;
-  auto share = [&](int units, int per, int cta, int& u0, int& u1) {
-    u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(cta) * per));
-    u1 = min(units, u0 + per);
-  };
-  int u0, u1, v0, v1;
-  share(lists.tall_units, lists.tall_per_cta, blockIdx.x, u0, u1);
-  share(lists.wide_units, lists.wide_per_cta, blockIdx.x, v0, v1);
+  // this CTA's kind, number among those of its kind, and units
+  const int before = static_cast<int>(static_cast<long long>(blockIdx.x) * lists.tall_ctas / gridDim.x);
+  const bool tall = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * lists.tall_ctas / gridDim.x) > before;
+  const int cta = tall ? before : static_cast<int>(blockIdx.x) - before;
+  const int units = tall ? lists.tall_units : lists.wide_units, per = tall ? lists.tall_per_cta : lists.wide_per_cta;
+  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(cta) * per)), u1 = min(units, u0 + per);
+  const int total = u1 - u0;                      // its tiles; t counts them
   bool ok = true;
-  // pool row of the box of `box` tokens that holds `key`, by the table of a row
-  auto pool_row = [&](const int* table, int key) -> int {
-    const int page = table[key / a.page_size];
+  // pool row of the box of tokens that holds `key`, by a row's table
+  auto pool_row = [&](int row, int key) -> int {
+    const int page = a.table[static_cast<long long>(row) * a.max_pages + key / a.page_size];
     if (page < 0 || page >= a.pages) {            // past the pool's end: zeros
       atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
       return a.pages * a.page_size;
     }
     return page * a.page_size + key % a.page_size;
   };
-
-  // ------------------------------------------------------------------------------------------------------ tall lists
-  if (const int total = u1 - u0; total == 0) {
-  } else if (warp == TMA_WARP) {
-    // K(0) K(1) V(0) K(2) V(1) ... V(total - 1); a lane a box of rows
-    int slot = 0;
-    uint32_t phase = 1;
-    const int boxes = BN / a.box;
-    int pool_row0 = 0, pool_row1 = 0, hk0 = 0, hk1 = 0;   // of the last even and odd tile whose keys were asked for
-    unsigned lanes0 = 0, lanes1 = 0;
-    auto fetch = [&](const CUtensorMap* map, int row, unsigned lanes, int hk) -> bool {
-      if (!mbar_wait_warp(&bars->empty[slot], phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); return false; }
-      if (lane == 0) mbar_expect_tx(&bars->full[slot], static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
-      __syncwarp();
-      if (lanes >> lane & 1) {
-        uint8_t* to = ring + slot * C::SLOT + lane * a.box * 128;
+  // the TMA warp: boxes of rows of one tile, a lane a box, to `to`
+  auto load = [&](const CUtensorMap* map, uint8_t* to, int keys, uint64_t* full, int row, unsigned lanes, int hk) {
+    if (lane == 0) mbar_expect_tx(full, static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
+    __syncwarp();
+    if (lanes >> lane & 1) {
 #pragma unroll
-        for (int p = 0; p < C::SUB; ++p) tma_load_2d(to + p * (BN * 128), map, &bars->full[slot], hk * D + p * 64, row);
-      }
-      __syncwarp();
-      if (++slot == C::RING) { slot = 0; phase ^= 1; }
-      return true;
-    };
-    Item w = locate<true>(lists, a, u0, u1);
-    int u = u0, j = 0;                            // the next tile whose keys are asked for: tile j of w's piece, unit u
-    auto keys = [&](int t) -> bool {
-      if (j == w.tiles) {
-        advance<true>(w, lists, a, u, u1);
-        j = 0;
-      }
-      const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
-      const bool any = lane < boxes && w.keys.meets(key, a.box);
-      const int row = any ? pool_row(a.table + static_cast<long long>(w.row) * a.max_pages, key) : 0;
-      const unsigned lanes = __ballot_sync(FULL, any);
-      if (t & 1) { pool_row1 = row; lanes1 = lanes; hk1 = w.hk; } else { pool_row0 = row; lanes0 = lanes; hk0 = w.hk; }
-      ++j;
-      ++u;
-      return fetch(&tk, row, lanes, w.hk);
-    };
-    ok = keys(0) && (total < 2 || keys(1));
-    for (int t = 0; ok && t < total; ++t) {
-      ok = t & 1 ? fetch(&tv, pool_row1, lanes1, hk1) : fetch(&tv, pool_row0, lanes0, hk0);
-      if (ok && t + 2 < total) ok = keys(t + 2);
+      for (int p = 0; p < C::SUB; ++p) tma_load_2d(to + lane * a.box * 128 + p * (keys * 128), map, full, hk * D + p * 64, row);
     }
-  } else if (warp == MMA_WARP) {
+    __syncwarp();
+  };
+
+  if (total == 0) {
+    // (fewer tiles than CTAs)
+  } else if (tall && warp == TMA_WARP) {
+    // K(0) K(1) V(0) K(2) V(1) ... V(total - 1)
+    int slot = 0, list = -1, j = 0, tiles = 0;
+    uint32_t phase = 1;
+    int row0 = 0, row1 = 0, hk0 = 0, hk1 = 0;     // of the last even and odd tile whose keys were asked for
+    unsigned lanes0 = 0, lanes1 = 0;
+#pragma unroll 1
+    for (int t = 0; ok && t < total + 2; ++t) {
+#pragma unroll 1
+      for (int what = 0; what < 2 && ok; ++what) {                 // the values of tile t - 2, the keys of tile t
+        if (what == 0 ? t < 2 : t >= total) continue;
+        if (what == 1) {
+          if (j == tiles) {
+            ++list;
+            ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+            if (!ok) break;
+            if (lane == 0) {
+              if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
+              next_list<true>(lists.item[list & 1], lists, a, u0 + t, u1, list == 0);
+              mbar_arrive(&bars->list_full[list & 1]);
+            }
+            __syncwarp();
+            tiles = lists.item[list & 1].tiles;
+            j = 0;
+          }
+          const Item& w = lists.item[list & 1];
+          const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
+          const bool any = lane * a.box < BN && w.keys.meets(key, a.box);
+          const int row = any ? pool_row(w.row, key) : 0;
+          const unsigned lanes = __ballot_sync(FULL, any);
+          if (t & 1) { row1 = row; lanes1 = lanes; hk1 = w.hk; } else { row0 = row; lanes0 = lanes; hk0 = w.hk; }
+          ++j;
+        }
+        ok = wait(&bars->empty[slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        if (!ok) break;
+        load(what == 1 ? &tk : &tv, ring + slot * C::SLOT, BN, &bars->full[slot], t & 1 ? row1 : row0, t & 1 ? lanes1 : lanes0, t & 1 ? hk1 : hk0);
+        if (++slot == C::RING) { slot = 0; phase ^= 1; }
+      }
+    }
+  } else if (tall && warp == MMA_WARP) {
     // over the tiles of all lists: S(0) S(1) PV(0) S(2) PV(1) ... (the warp waits together, one lane issues)
     constexpr uint32_t idesc_qk = make_idesc(BM, BN, 1, 1, 0, 0);
     constexpr uint32_t idesc_pv = make_idesc(BM, D, 1, 1, 0, 1);
-    int slot = 0;
-    uint32_t phase = 0, p_phase = 0;              // (p_phase: a bit for each buffer)
-    auto take = [&](int& at) -> bool {
-      at = slot;
-      if (!mbar_wait_warp(&bars->full[slot], phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); return false; }
-      if (++slot == C::RING) { slot = 0; phase ^= 1; }
-      return true;
-    };
-    Item w = locate<true>(lists, a, u0, u1);
-    int u = u0, j = 0;                            // as for the keys
-    uint32_t tall_phase = 0, fresh = 0;           // (fresh: a bit for each buffer, whether its tile is its list's first)
+    int slot = 0, list = -1, j = 0, tiles = 0;
+    uint32_t phase = 0, fresh = 0;                // (fresh: a bit for each buffer, whether its tile is its list's first)
     const uint32_t qa = smem_u32(sQ);
-    auto scores = [&](int t) -> bool {
+#pragma unroll 1
+    for (int t = 0; ok && t < total + 2; ++t) {
       const int b = t & 1;
-      if (j == w.tiles) {
-        advance<true>(w, lists, a, u, u1);
-        j = 0;
+      if (t >= 2) {                               // PV(t - 2)
+        ok = wait(&bars->full[slot], phase, abort_flag, a.err, ERR_WAIT_FULL, lane) && wait(&bars->p_full[b], ((t - 2) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_u32(ring + slot * C::SLOT);
+        const uint32_t add = fresh >> b & 1 ? 0u : 1u;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 ? 1u : add);
+          umma_commit(&bars->done);
+          umma_commit(&bars->empty[slot]);
+        }
+        __syncwarp();
+        if (++slot == C::RING) { slot = 0; phase ^= 1; }
       }
+      if (t >= total) continue;
       fresh &= ~(1u << b);
-      if (j == 0) {
-        if (!mbar_wait_warp(&bars->tall_full, tall_phase, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); return false; }
-        tall_phase ^= 1;
+      if (j == tiles) {
+        ++list;
+        ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        if (!ok) break;
+        tiles = lists.item[list & 1].tiles;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
+        ok = wait(&bars->q_full, list & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        j = 0;
         fresh |= 1u << b;
       }
       ++j;
-      ++u;
-      int at;
-      if (!take(at)) return false;
+      ok = ok && wait(&bars->full[slot], phase, abort_flag, a.err, ERR_WAIT_FULL, lane);
+      if (!ok) break;
       tc_fence_after();
-      const uint32_t ka = smem_u32(ring + at * C::SLOT);
+      const uint32_t ka = smem_u32(ring + slot * C::SLOT);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           umma_bf16_ss(tmem + b * BN, make_sdesc_sw128(qa + (kk >> 2) * (BM * 128) + (kk & 3) * 32, 16, 1024),
                        make_sdesc_sw128(ka + (kk >> 2) * (BN * 128) + (kk & 3) * 32, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
         umma_commit(&bars->s_full[b]);
-        umma_commit(&bars->empty[at]);
+        umma_commit(&bars->empty[slot]);
       }
       __syncwarp();
-      return true;
-    };
-    ok = scores(0) && (total < 2 || scores(1));
-    for (int t = 0; ok && t < total; ++t) {
-      const int b = t & 1;
-      int at;
-      ok = take(at);
-      if (!ok) break;
-      if (!mbar_wait_warp(&bars->p_full[b], p_phase >> b & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
-      p_phase ^= 1u << b;
-      tc_fence_after();
-      const uint32_t va = smem_u32(ring + at * C::SLOT);
-      const uint32_t add = fresh >> b & 1 ? 0u : 1u;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 ? 1u : add);
-        umma_commit(&bars->done);
-        umma_commit(&bars->empty[at]);
-      }
-      __syncwarp();
-      if (t + 2 < total) ok = scores(t + 2);
+      if (++slot == C::RING) { slot = 0; phase ^= 1; }
     }
-  } else {
+  } else if (tall) {
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t t_s = tmem + lane_addr, t_o = tmem + lane_addr + C::TM_O;
-    uint32_t s_phase = 0;                         // (a bit for each buffer)
-    auto queries = [&](const Item& w) {
-      fetch_queries<D, 4>(sQ, BM * 128, lists, a, w, tid, BM);
-      if (lane == 0) mbar_arrive(&bars->tall_full);
-    };
-    const Item& w = lists.now[warp];
-    {
-      const Item first = locate<true>(lists, a, u0, u1);
-      if (lane == 0) lists.now[warp] = first;
-      queries(first);
-      __syncwarp();
-    }
-    for (int t = 0; t < total && ok;) {
-      const bool active = warp * 32 < w.n, mine = tid < w.n;
+    float* to = nullptr;                          // where the last list's result goes
+    bool active = false;
+#pragma unroll 1
+    for (int t = 0, list = 0;; ++list) {
+      const Item& w = lists.item[list & 1];
+      int one = -1;
+      if (t < total) {
+        // all scores of the lists before are made: the next one's queries may take the place of theirs
+        ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        if (!ok) break;
+        one = query(lists, a, w, tid);
+        fetch_queries<D>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
+        if (lane == 0) mbar_arrive(&bars->q_full);
+      }
+      if (list > 0) {
+        ok = wait(&bars->done, (t - 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        if (!ok) break;
+        tc_fence_after();
+        if (active) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(t_o + c * 32, v);
+            tmem_ld_wait();
+            if (to != nullptr) store_row_32<false>(to + c * 32, v, 1.f);
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+      }
+      if (t >= total) break;
       const int tiles = w.tiles;
+      const bool mine = tid < w.n;
+      active = warp * 32 < w.n;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < tiles; ++j, ++t) {
+#pragma unroll 1
+    #pragma unroll 1
+  for (int j = 0; j < tiles; ++j, ++t) {
         const int b = t & 1;
-        if (!mbar_wait_warp(&bars->s_full[b], s_phase >> b & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_TMEM_FULL)); ok = false; break; }
-        s_phase ^= 1u << b;
+        ok = wait(&bars->s_full[b], (t >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL, lane);
+        if (!ok) break;
         tc_fence_after();
         // which of the tile's keys the list sees
         const int key0 = w.keys.tile<BN>(w.from + j) * BN;
@@ -763,7 +810,8 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (need) { m = m_new; l *= by; }
             if (j > 0) {
               // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
-              if (!mbar_wait_warp(&bars->done, (t - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+              ok = wait(&bars->done, (t - 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+              if (!ok) break;
               tc_fence_after();
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
@@ -796,10 +844,11 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (!whole) {
           // values that nobody sees, to zero, in the slot that the t-th value tile has
           const int at = t + 1 < total ? 2 + 2 * t : 2 * total - 1, slot = at % C::RING;
-          if (!mbar_wait_warp(&bars->full[slot], (at / C::RING) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; break; }
+          ok = wait(&bars->full[slot], (at / C::RING) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
+          if (!ok) break;
           const int x = tid >> 1;                 // a key's values by two threads
           if (!((x < 32 ? sees[0] : sees[1]) >> (x & 31) & 1)) {
-#pragma unroll
+#pragma unroll 1
             for (int p = 0; p < C::SUB; ++p)
 #pragma unroll
               for (int c = 0; c < 4; ++c)
@@ -812,87 +861,51 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (lane == 0) mbar_arrive(&bars->p_full[b]);
       }
       if (!ok) break;
-      // where the result goes (a piece of a list in a place of the CTA's)
-      float* to = nullptr;
-      if (mine) {
-        int row, head;
-        query(lists, w, tid, row, head);
-        const long long at = tiles == w.units ? static_cast<long long>(row) * a.heads + head
-                                              : 2ll * a.rows * a.heads + static_cast<long long>(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * BM + tid;
-        if (row >= 0) {
-          a.ml[at] = make_float2(m, l);
-          to = a.acc + at * D;
-        }
+      // (a piece of a list goes to a place of the CTA's)
+      to = nullptr;
+      if (one >= 0) {
+        const long long at = tiles == w.units ? one : 2ll * a.rows * a.heads + static_cast<long long>(2 * cta + (w.from == 0 ? 1 : 0)) * BM + tid;
+        a.ml[at] = make_float2(m, l);
+        to = a.acc + at * D;
       }
-      // all of this list's scores are made, and those of the lists before: the next one's queries may take their place
-      if (t < total) {
-        Item next = w;
-        advance<true>(next, lists, a, u0 + t, u1);
-        __syncwarp();
-        if (lane == 0) lists.now[warp] = next;
-        queries(next);
-        __syncwarp();
-      }
-      if (!mbar_wait_warp(&bars->done, (t - 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
-      tc_fence_after();
-      if (active) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t_o + c * 32, v);
-          tmem_ld_wait();
-          if (to != nullptr) store_row_32<false>(to + c * 32, v, 1.f);
-          __syncwarp();
-        }
-      }
-      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
     }
-  }
-
-  // ------------------------------------------------------------------------------------------------------ wide lists, in the same memory
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (*abort_flag != 0) ok = false;
-  uint8_t *w_keys = ring, *w_values = ring + C::W_SLOTS * C::W_TILE, *w_weights = sQ + 2 * C::W_Q;
-  if (const int total = v1 - v0; total == 0 || !ok) {
   } else if (warp == TMA_WARP) {
     // K(0) V(0) K(1) V(1) ...
-    const int boxes = WK / a.box;
-    auto fetch = [&](const CUtensorMap* map, uint8_t* to, uint64_t* full, uint64_t* empty, int t, int row, unsigned lanes, int hk) -> bool {
+    int list = -1, j = 0, tiles = 0;
+#pragma unroll 1
+    for (int t = 0; ok && t < total; ++t, ++j) {
+      const bool begins = j == tiles;
       const int slot = t % C::W_SLOTS;
-      if (!mbar_wait_warp(&empty[slot], ((t / C::W_SLOTS) & 1) ^ 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); return false; }
-      if (lane == 0) mbar_expect_tx(&full[slot], static_cast<uint32_t>(__popc(lanes)) * a.box * D * 2);
-      __syncwarp();
-      if (lanes >> lane & 1) {
-#pragma unroll
-        for (int p = 0; p < C::SUB; ++p) tma_load_2d(to + slot * C::W_TILE + lane * a.box * 128 + p * (WK * 128), map, &full[slot], hk * D + p * 64, row);
-      }
-      __syncwarp();
-      return true;
-    };
-    Item w = locate<false>(lists, a, v0, v1);
-    for (int t = 0, list = 0, j = 0; ok && t < total; ++t, ++j) {
-      const bool begins = j == w.tiles || t == 0;
-      if (j == w.tiles) {
-        advance<false>(w, lists, a, v0 + t, v1);
+      const uint32_t phase = ((t / C::W_SLOTS) & 1) ^ 1;
+      if (begins) {
+        ++list;
+        ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        if (!ok) break;
+        if (lane == 0) {
+          if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
+          next_list<false>(lists.item[list & 1], lists, a, u0 + t, u1, list == 0);
+        }
+        __syncwarp();
+        tiles = lists.item[list & 1].tiles;
         j = 0;
       }
+      const Item& w = lists.item[list & 1];
       const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
-      const bool any = lane < boxes && w.keys.meets(key, a.box);
-      const int row = any ? pool_row(a.table + static_cast<long long>(w.row) * a.max_pages, key) : 0;
+      const bool any = lane * a.box < WK && w.keys.meets(key, a.box);
+      const int row = any ? pool_row(w.row, key) : 0;
       const unsigned lanes = __ballot_sync(FULL, any);
-      ok = fetch(&tk, w_keys, bars->wk_full, bars->wk_empty, t, row, lanes, w.hk);
-      if (ok && begins) {
-        const int q = list & 1;
-        ok = mbar_wait_warp(&bars->wq_empty[q], ((list >> 1) & 1) ^ 1, abort_flag);
-        if (!ok) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_EMPTY)); break; }
-        if (lane == 0) lists.item[q] = w;
-        fetch_queries<D, 4>(sQ + q * C::W_Q, WN * 128, lists, a, w, lane, 32);
-        if (lane == 0) mbar_arrive(&bars->wq_full[q]);
-        ++list;
+#pragma unroll 1
+      for (int what = 0; what < 2 && ok; ++what) {                 // keys, values
+        ok = wait(&bars->empty[2 * what + slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        if (!ok) break;
+        load(what == 0 ? &tk : &tv, (what == 0 ? w_keys : w_values) + slot * C::W_TILE, WK, &bars->full[2 * what + slot], row, lanes, w.hk);
+        if (what == 0 && begins) {
+          fetch_queries<D>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
+          if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
+        }
       }
-      ok = ok && fetch(&tv, w_values, bars->wv_full, bars->wv_empty, t, row, lanes, w.hk);
     }
   } else if (warp == MMA_WARP) {
     // S(0) S(1) PV(0) S(2) PV(1) ...
@@ -901,38 +914,40 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     int list = -1, j = 0, tiles = 0;
     bool more = false;                            // than 16 queries
     uint32_t flags = 0;                           // bits b: whether the tile in buffer b is its list's first, 2 + b: whether its list has more than 16 queries
-    auto scores = [&](int t) -> bool {
-      const int b = t & 1, slot = t % C::W_SLOTS;
-      if (j == tiles) {
-        ++list;
-        if (!mbar_wait_warp(&bars->wq_full[list & 1], (list >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); return false; }
-        tiles = lists.item[list & 1].tiles;
-        more = lists.item[list & 1].n > 16;
-        j = 0;
-      }
-      flags = (flags & ~(5u << b)) | ((j == 0 ? 1u : 0u) | (more ? 4u : 0u)) << b;
-      ++j;
-      if (!mbar_wait_warp(&bars->wk_full[slot], (t / C::W_SLOTS) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); return false; }
-      tc_fence_after();
-      const uint32_t ka = smem_u32(w_keys + slot * C::W_TILE), qa = smem_u32(sQ + (list & 1) * C::W_Q), idesc = more ? idesc_s[1] : idesc_s[0];
-      if (elect_one()) {
+#pragma unroll 1
+    for (int t = 0; ok && t <= total; ++t) {
+      if (t < total) {                            // S(t)
+        const int b = t & 1, slot = t % C::W_SLOTS;
+        if (j == tiles) {
+          ++list;
+          ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+          if (!ok) break;
+          tiles = lists.item[list & 1].tiles;
+          more = lists.item[list & 1].n > 16;
+          j = 0;
+        }
+        flags = (flags & ~(5u << b)) | ((j == 0 ? 1u : 0u) | (more ? 4u : 0u)) << b;
+        ++j;
+        ok = wait(&bars->full[slot], (t / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ka = smem_u32(w_keys + slot * C::W_TILE), qa = smem_u32(sQ + (list & 1) * C::W_Q), idesc = more ? idesc_s[1] : idesc_s[0];
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma_bf16_ss(tmem + b * WN, make_sdesc_sw128(ka + (kk >> 2) * (WK * 128) + (kk & 3) * 32, 16, 1024),
-                       make_sdesc_sw128(qa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-        umma_commit(&bars->ws_full[b]);
-        umma_commit(&bars->wk_empty[slot]);
-        if (j == tiles) umma_commit(&bars->wq_empty[list & 1]);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16_ss(tmem + b * WN, make_sdesc_sw128(ka + (kk >> 2) * (WK * 128) + (kk & 3) * 32, 16, 1024),
+                         make_sdesc_sw128(qa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+          umma_commit(&bars->s_full[b]);
+          umma_commit(&bars->empty[slot]);
+          if (j == tiles) umma_commit(&bars->list_empty[list & 1]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      return true;
-    };
-    ok = scores(0);
-    for (int t = 0; ok && t < total; ++t) {
-      if (t + 1 < total && !scores(t + 1)) { ok = false; break; }
-      const int b = t & 1, slot = t % C::W_SLOTS;
-      if (!mbar_wait_warp(&bars->wv_full[slot], (t / C::W_SLOTS) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_FULL)); ok = false; break; }
-      if (!mbar_wait_warp(&bars->wp_full[b], (t >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; break; }
+      if (t == 0) continue;
+      const int b = (t - 1) & 1, slot = (t - 1) % C::W_SLOTS;      // PV(t - 1)
+      ok = wait(&bars->full[2 + slot], ((t - 1) / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) &&
+           wait(&bars->p_full[b], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+      if (!ok) break;
       tc_fence_after();
       const uint32_t va = smem_u32(w_values + slot * C::W_TILE), pa = smem_u32(w_weights + b * C::W_P);
       const uint32_t idesc = flags >> (2 + b) & 1 ? idesc_o[1] : idesc_o[0], add = flags >> b & 1 ? 0u : 1u;
@@ -943,22 +958,23 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           for (int kk = 0; kk < WK / 16; ++kk)    // (a head of 64 fills half of the rows: the others are of whatever follows)
             umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
                          make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
-        umma_commit(&bars->w_done);
-        umma_commit(&bars->wv_empty[slot]);
+        umma_commit(&bars->done);
+        umma_commit(&bars->empty[2 + slot]);
       }
       __syncwarp();
     }
   } else {
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
-    const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, bars, abort_flag, tid, warp, lane};
+    const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, bars, abort_flag, tid, warp, lane, cta};
+#pragma unroll 1
     for (int t = 0, list = 0; t < total; ++list) {
       const int q = list & 1;
-      if (!mbar_wait_warp(&bars->wq_full[q], (list >> 1) & 1, abort_flag)) { if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_WAIT_OTHER)); ok = false; }
+      ok = wait(&bars->list_full[q], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
       if (any_of_128(!ok)) break;                 // (all warps or none)
-      const Item& w = lists.item[q];               // (not a copy: the registers are for scores)
+      const Item& w = lists.item[q];              // (not a copy: the registers are for scores)
       ok = w.n <= 8 ? wide_list<D, 8>(x, lists, a, w, t) : w.n <= 16 ? wide_list<D, 16>(x, lists, a, w, t) : wide_list<D, 32>(x, lists, a, w, t);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->wq_empty[q]);
+      if (lane == 0) mbar_arrive(&bars->list_empty[q]);
     }
   }
   if (blockIdx.x == gridDim.x - 1) write_plan(lists, a, tid);
@@ -975,7 +991,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 template <int D>
 __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a, int ctas) {
   const int place = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ratio = a.heads / a.kv_heads, chunks = (ratio + WN - 1) / WN;
+  const int ratio = a.ratio, chunks = a.chunks;
   const int row = a.order[place];
   const int4 lists = a.plan[2 * place], group = a.plan[2 * place + 1];
   if (row < 0 || row >= a.rows) return;
@@ -1038,6 +1054,7 @@ int multiprocessors() {
 template <int D>
 int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas, cudaStream_t stream) {
   using C = Cfg<D>;
+  static_assert(sizeof(Bars) % 16 == 0 && alignof(Lists) == 16 && offsetof(Lists, top) % 16 == 0, "the maxima are read four at a time");
   constexpr int SMEM = C::Q_BYTES + C::EXTRA + C::RING * C::SLOT + static_cast<int>(sizeof(Bars) + sizeof(Lists));
   static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "over an SM's shared memory");
   cudaError_t e = cudaFuncSetAttribute(shared_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
@@ -1075,7 +1092,7 @@ extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const v
   if ((r = dewb::make_tmap_2d(&tk, k, tall, cols, cols, box, 64, 2, true))) return 1000 + r;
   if ((r = dewb::make_tmap_2d(&tv, v, tall, cols, cols, box, 64, 2, true))) return 2000 + r;
   const Args a{reinterpret_cast<const __nv_bfloat16*>(q), q_stride, table, lengths, order, first, tokens, sinks, reinterpret_cast<__nv_bfloat16*>(out), acc,
-               reinterpret_cast<float2*>(ml), reinterpret_cast<int4*>(plan), rows, heads, kv_heads, page_size, box, max_pages, pages, groups, window, least, scale * LOG2E, cap * LOG2E, err};
+               reinterpret_cast<float2*>(ml), reinterpret_cast<int4*>(plan), rows, heads, kv_heads, heads / kv_heads, static_cast<int>(chunks), page_size, box, max_pages, pages, groups, window, least, scale * LOG2E, cap * LOG2E, err};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   if (D == 64) return launch<64>(tk, tv, a, ctas, stream);
   if (D == 128) return launch<128>(tk, tv, a, ctas, stream);
