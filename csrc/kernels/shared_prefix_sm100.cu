@@ -2,7 +2,8 @@
 //
 // The work is lists: up to some number of queries (row, head) against a range of keys of one key head.  A group's shared keys (shared_range.cuh) make a list for each key head,
 // a row's own keys another.  There are two kinds, each with CTAs of its own (as many as its share of the work, dealt over the SMs).  All lists of a kind stand behind one
-// another in one sequence of tiles that its CTAs share evenly: a list may begin in one CTA and end in another.
+// another in one sequence that its CTAs share evenly, tile by tile: a list may begin in one CTA and end in another.  In front of each list there is room in the sequence for
+// what beginning and ending one costs, so that CTAs with many short lists get fewer tiles.
 //
 // TALL lists (a group of more than 32 queries on a key head, 128 of them a list): queries are the rows of the products.  Per 64 keys  S = Q K^T  (one of two score buffers in
 // tensor memory),  a thread a query makes the weights P over its scores,  O += P V  with P read from tensor memory.
@@ -42,7 +43,8 @@ constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys o
 constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
 constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
 constexpr int MOST_ROWS = 448;
-constexpr int TALL_COST = 1, WIDE_COST = 2;        // of a tile, where CTAs are dealt
+constexpr int TALL_GAP = 2, WIDE_GAP = 1;         // tiles that a list takes as long as beyond its own
+constexpr int TALL_COST = 1, WIDE_COST = 2;       // of a tile, where CTAs are dealt
 constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t FULL = 0xffffffffu;
@@ -51,7 +53,7 @@ template <int D>
 struct Cfg {
   static constexpr int SUB = D / 64;              // 64-column pieces of a row
   static constexpr int Q_BYTES = BM * D * 2;      // tall: the queries.  wide: two lists' queries and two tiles' weights
-  static constexpr int SLOT = BN * D * 2, RING = D == 64 ? 8 : 4;              // tall: keys or values of a tile
+  static constexpr int SLOT = BN * D * 2, RING = D == 64 ? 8 : 4, HALF = RING / 2;                // tall: a tile's keys (first half) or values
   static constexpr int W_TILE = WK * D * 2, W_SLOTS = RING / 4;                // wide: the same memory, half for keys and half for values
   static constexpr int W_Q = WN * D * 2, W_P = WN * WK * 2;
   static constexpr int CTAS = D == 256 ? 1 : 2;   // an SM
@@ -76,15 +78,15 @@ struct Item {
   Ranges keys;
   int index, list, lists;                         // group or place, and which of its lists
   bool shared;                                    // of a group
-  int start, units;                               // the whole list's first unit and tiles
-  int from, tiles;                                // of its tiles
+  int start, units;                               // the whole list's first tile, in the sequence, and its tiles
+  int from, tiles;                                // of its tiles (tiles 0: the CTA's lists are over)
   int place, each, hk, head0, n;                  // first query counted through the places, query heads a row, key head, first query head, queries
   int row;                                        // whose table
 };
 
 struct alignas(16) Bars {
   uint64_t list_full[2], list_empty[2];           // what a list is about (wide: and its queries)
-  uint64_t full[8], empty[8];                     // slots of the ring.  wide: [0, 2) keys, [2, 4) values
+  uint64_t full[8], empty[8];                     // slots of the ring: [0, 4) keys, [4, 8) values
   uint64_t q_full, s_full[2], p_full[2], done;
   uint32_t tmem;
   int abort_flag, poisoned;
@@ -92,7 +94,7 @@ struct alignas(16) Bars {
 
 // what a CTA knows of all lists
 struct Lists {
-  int tall_units, tall_ctas, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;
+  int tall_units, tall_ctas, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;      // (units: tiles and the room in front of lists)
   short first[MOST_ROWS + 2];                     // groups: first place
   short row[MOST_ROWS], group[MOST_ROWS];         // places (row -1: none)
   short through[MOST_ROWS];                       // groups: a row that holds something
@@ -103,7 +105,7 @@ struct Lists {
   Item item[2];                                   // the list at hand and the next one
   float most[4][WN];                              // wide: largest scores, by warp
   alignas(16) float top[4][WN], by[4][WN];        // (read four at a time) each warp's copy of the maxima in use, and what sums made with older ones are multiplied with
-  float sums[WN];                                 // of weights, and then what results are multiplied with
+  float sums[4][WN];                              // of weights, by warp
 };
 
 struct Args {
@@ -149,28 +151,36 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 
 __device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * a.ratio; }
 
-// The list that unit u is of, up to `end`; unless `begins`, w is the one before.  One thread.
+// The CTA's first list, from unit u on, or (!begins) the one behind w's; up to `end`.  One thread.
 template <bool TALL>
 __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, int u, int end, bool begins) {
+  constexpr int GAP = TALL ? TALL_GAP : WIDE_GAP;
   const int* at = TALL ? s.tall : s.wide;
   bool same = false;
   if (begins) {
+    w.tiles = 0;
+    if (u >= end) return;
     w.shared = TALL || u < s.wide_shared_units;
     w.index = w.shared ? last_at_most(at, a.groups, u) : last_at_most(s.own, a.rows, (u - s.wide_shared_units) / (a.kv_heads * a.chunks));
-  } else if (++w.list < w.lists) {
-    same = true;
-    w.start = u;
   } else {
-    if (!TALL && w.shared && u >= s.wide_shared_units) {
-      w.shared = false;
-      w.index = -1;
-    }
-    if (w.shared) {
-#pragma unroll 1
-      do ++w.index; while (at[w.index + 1] <= u);
+    u = w.start + w.units;                         // (the room in front of the next list)
+    w.tiles = 0;
+    if (u + GAP >= end) return;
+    if (++w.list < w.lists) {
+      same = true;
+      w.start = u + GAP;
     } else {
+      if (!TALL && w.shared && u >= s.wide_shared_units) {
+        w.shared = false;
+        w.index = -1;
+      }
+      if (w.shared) {
 #pragma unroll 1
-      do ++w.index; while (s.own[w.index + 1] == s.own[w.index]);
+        do ++w.index; while (at[w.index + 1] <= u);
+      } else {
+#pragma unroll 1
+        do ++w.index; while (s.own[w.index + 1] == s.own[w.index]);
+      }
     }
   }
   if (!same) {
@@ -178,18 +188,18 @@ __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, i
       w.keys = Ranges{s.lo[w.index], s.hi[w.index], 0, 0};
       w.lists = a.kv_heads * (TALL ? (group_queries(s, a, w.index) + BM - 1) / BM : 1);
       w.row = s.through[w.index];
-      w.start = at[w.index];
+      w.start = at[w.index] + GAP;
       w.units = w.keys.tiles<TALL ? BN : WK>();
     } else {
       const int g = s.group[w.index];
       w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g]);
       w.lists = a.kv_heads * a.chunks;
       w.row = s.row[w.index];
-      w.start = s.wide_shared_units + s.own[w.index] * w.lists;
-      w.units = s.own[w.index + 1] - s.own[w.index];
+      w.start = s.wide_shared_units + s.own[w.index] * w.lists + GAP;
+      w.units = s.own[w.index + 1] - s.own[w.index] - GAP;
     }
-    w.list = begins ? (u - w.start) / w.units : 0;
-    w.start += w.list * w.units;
+    w.list = begins ? (u + GAP - w.start) / (w.units + GAP) : 0;
+    w.start += w.list * (w.units + GAP);
   }
   if (w.shared) {
     const int queries = group_queries(s, a, w.index), pieces = TALL ? (queries + BM - 1) / BM : 1;
@@ -206,8 +216,8 @@ __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, i
     w.place = w.index * w.n;
     w.head0 = w.hk * a.ratio + c * WN;
   }
-  w.from = u - w.start;
-  w.tiles = min(end, w.start + w.units) - u;
+  w.from = max(u - w.start, 0);
+  w.tiles = max(min(end, w.start + w.units) - max(u, w.start), 0);
 }
 
 // row * heads + head of a list's query i, -1 for none
@@ -252,7 +262,7 @@ __device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int ti
     const int g = s.group[i], queries = group_queries(s, a, g);
     const Ranges both{s.lo[g], s.hi[g], 0, 0};
     const bool tall = queries > WN;
-    a.plan[2 * i] = make_int4(tall ? s.tall[g] : s.wide[g], tall ? both.tiles<BN>() : both.tiles<WK>(), s.wide_shared_units + s.own[i] * lists, s.own[i + 1] - s.own[i]);
+    a.plan[2 * i] = make_int4(tall ? s.tall[g] : s.wide[g], tall ? both.tiles<BN>() : both.tiles<WK>(), s.wide_shared_units + s.own[i] * lists, max(s.own[i + 1] - s.own[i] - WIDE_GAP, 0));
     a.plan[2 * i + 1] = make_int4(s.first[g], tall ? queries : 0, s.tall_per_cta, s.wide_per_cta);
   }
 }
@@ -275,7 +285,8 @@ __device__ __forceinline__ void running_sums(int* x, int n, int lane) {
   for (int i = i0; i < i1; ++i) { run += x[i + 1]; x[i + 1] = run; }
 }
 
-__device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int warp, int lane) {
+// false: an earlier launch reported an error (read here, beside what else is on its way)
+__device__ __forceinline__ bool make_lists(Lists& s, Bars* bars, const Args& a, int tid, int warp, int lane) {
   constexpr int EACH = (MOST_ROWS + THREADS - 1) / THREADS;
   const int most = a.max_pages * a.page_size;
   int* live = s.own;                              // (until the places' tiles are known)
@@ -283,6 +294,7 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
   int row_of[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) row_of[e] = e * THREADS + tid < a.rows ? a.order[e * THREADS + tid] : -1;
+  if (tid == THREADS - 1) bars->poisoned = *reinterpret_cast<volatile int*>(a.err);
 #pragma unroll 1
   for (int g = tid; g <= a.groups; g += THREADS) {
     s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
@@ -301,6 +313,7 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     s.len[i] = bad ? -1 : a.lengths[row_of[e]];
   }
   __syncthreads();
+  if (bars->poisoned != 0) return false;
 #pragma unroll 1
   for (int i0 = warp * 32; i0 < a.rows; i0 += THREADS) {
     const int i = i0 + lane;
@@ -338,12 +351,15 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     if (live[g] < 2 || s.lo[g] >= s.hi[g]) s.lo[g] = s.hi[g] = 0;
     const int queries = group_queries(s, a, g);
     const Ranges both{s.lo[g], s.hi[g], 0, 0};
-    s.tall[g + 1] = s.hi[g] == 0 || queries <= WN ? 0 : a.kv_heads * ((queries + BM - 1) / BM) * both.tiles<BN>();
-    s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * both.tiles<WK>();
+    s.tall[g + 1] = s.hi[g] == 0 || queries <= WN ? 0 : a.kv_heads * ((queries + BM - 1) / BM) * (both.tiles<BN>() + TALL_GAP);
+    s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * (both.tiles<WK>() + WIDE_GAP);
   }
   __syncthreads();
 #pragma unroll 1
-  for (int i = tid; i < a.rows; i += THREADS) s.own[i + 1] = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles<WK>();
+  for (int i = tid; i < a.rows; i += THREADS) {
+    const int n = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles<WK>();
+    s.own[i + 1] = n == 0 ? 0 : n + WIDE_GAP;
+  }
   __syncthreads();
   if (warp < 3) running_sums(warp == 0 ? s.tall : warp == 1 ? s.wide : s.own, warp < 2 ? a.groups : a.rows, lane);
   __syncthreads();
@@ -356,12 +372,14 @@ __device__ __forceinline__ void make_lists(Lists& s, const Args& a, int tid, int
     const long long tall = static_cast<long long>(s.tall_units) * TALL_COST, wide = static_cast<long long>(s.wide_units) * WIDE_COST;
     int k = tall == 0 ? 0 : wide == 0 ? ctas : static_cast<int>((tall * ctas + (tall + wide) / 2) / (tall + wide));
     if (tall > 0 && wide > 0) k = min(max(k, 1), ctas - 1);
-    s.tall_ctas = min(k, (s.tall_units + 2 * a.least - 1) / (2 * a.least));
+    const int least = a.least + WIDE_GAP;
+    s.tall_ctas = min(k, (s.tall_units + 2 * least - 1) / (2 * least));
     s.tall_per_cta = s.tall_ctas == 0 ? 1 : (s.tall_units + s.tall_ctas - 1) / s.tall_ctas;
     const int rest = max(1, ctas - s.tall_ctas);
-    s.wide_per_cta = max(a.least, (s.wide_units + rest - 1) / rest);
+    s.wide_per_cta = max(least, (s.wide_units + rest - 1) / rest);
   }
   __syncthreads();
+  return true;
 }
 
 // ---------------------------------------------------------------------------------------------------------- wide lists' softmax
@@ -435,9 +453,9 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
 #pragma unroll 1
   for (int j = 0; j < tiles; ++j, ++t) {
     const int b = t & 1;
+    const bool seen = w.keys.sees(w.keys.tile<WK>(w.from + j) * WK + tid);
     ok = wait(&bars->s_full[b], (t >> 1) & 1, x.abort_flag, a.err, ERR_WAIT_TMEM_FULL, lane) && ok;
     tc_fence_after();
-    const bool seen = w.keys.sees(w.keys.tile<WK>(w.from + j) * WK + tid);
     float s[NC];
     load_columns<NC>(x.t_s + b * WN, s);
 #pragma unroll
@@ -454,7 +472,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
       const float4 m = *reinterpret_cast<const float4*>(top + q);
       past = past || (q < n && s[q] > m.x + RESCALE) || (q + 1 < n && s[q + 1] > m.y + RESCALE) || (q + 2 < n && s[q + 2] > m.z + RESCALE) || (q + 3 < n && s[q + 3] > m.w + RESCALE);
     }
-    if (any_of_128(past && seen)) {
+    if (j == 0 || any_of_128(past && seen)) {
       float mine = -INFINITY;
 #pragma unroll
       for (int q = 0; q < NC; ++q) {
@@ -497,7 +515,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
     }
     if (__ballot_sync(FULL, !seen) != 0) {        // values that nobody sees, to zero (each thread its key's)
       const int slot = t % C::W_SLOTS;
-      ok = wait(&bars->full[2 + slot], (t / C::W_SLOTS) & 1, x.abort_flag, a.err, ERR_WAIT_FULL, lane) && ok;
+      ok = wait(&bars->full[4 + slot], (t / C::W_SLOTS) & 1, x.abort_flag, a.err, ERR_WAIT_FULL, lane) && ok;
       if (!seen) {
 #pragma unroll 1
         for (int p = 0; p < C::SUB; ++p)
@@ -517,34 +535,35 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
   const long long all = static_cast<long long>(a.rows) * a.heads;
   long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * 2 * BM + (2 * x.cta + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
   if (one < 0) at = -1;
-  ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
-  tc_fence_after();
-  // sums over the threads, through the weights' memory (all products with them are done): four threads a query, each every fourth thread's
-  float* part = reinterpret_cast<float*>(x.weights);
+  // sums over a warp: each exchange halves the queries that a lane is about, until lane i has query i % NC's
 #pragma unroll
-  for (int q = 0; q < NC; ++q) part[q * WK + tid] = l[q];
-  sync_128();
-  {
-    const int q = tid >> 2;
-    float sum = 0.f;
-    if (q < n)
-#pragma unroll 4
-      for (int i = tid & 3; i < WK; i += 4) sum += part[q * WK + ((i + q * 4) & (WK - 1))];
-    sum += __shfl_xor_sync(FULL, sum, 1);
-    sum += __shfl_xor_sync(FULL, sum, 2);
-    if ((tid & 3) == 0) {
-      float scale = sum;
-      if (last && q < n) {
-        const float m = top[q], sink = a.sinks != nullptr ? a.sinks[w.head0 + q] * LOG2E : -INFINITY;
-        const float both = fmaxf(m, sink), own = m > -INFINITY ? fast_exp2(m - both) : 0.f;
-        const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - both) : 0.f);
-        scale = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
-      }
-      lists.sums[q] = scale;
+  for (int h = NC / 2; h > 0; h >>= 1) {
+    const bool upper = lane & h;
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float other = __shfl_xor_sync(FULL, upper ? l[i] : l[i + h], h);
+      l[i] = (upper ? l[i + h] : l[i]) + other;
     }
   }
+#pragma unroll
+  for (int h = NC; h < 32; h <<= 1) l[0] += __shfl_xor_sync(FULL, l[0], h);
+  lists.sums[warp][lane] = l[0];
   sync_128();
-  if (!last && warp == 0 && at >= 0) a.ml[at] = make_float2(top[lane], lists.sums[lane]);
+  float scale = 1.f;                              // lane q: what query q's result is multiplied with
+  if (lane < n) {
+    const float m = top[lane], sum = (lists.sums[0][lane] + lists.sums[1][lane]) + (lists.sums[2][lane] + lists.sums[3][lane]);
+    if (last) {
+      const float sink = a.sinks != nullptr ? a.sinks[w.head0 + lane] * LOG2E : -INFINITY;
+      const float both = fmaxf(m, sink), own = m > -INFINITY ? fast_exp2(m - both) : 0.f;
+      const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - both) : 0.f);
+      scale = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
+    } else if (warp == 0 && at >= 0) {
+      a.ml[at] = make_float2(m, sum);
+    }
+  }
+  __syncwarp();
+  ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
+  tc_fence_after();
 #pragma unroll 1
   for (int c = 0; c < C::HALVES * WN; c += 4) {
     const int q = c & (WN - 1);
@@ -554,14 +573,14 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const long long to = __shfl_sync(FULL, at, q + i);
+      const float by = __shfl_sync(FULL, scale, q + i);
       if (q + i < n && to >= 0 && tid < D) {
         const long long place = to * D + (c / WN) * 128 + tid;
-        if (last) a.out[place] = __float2bfloat16(o[i] * lists.sums[q + i]);
+        if (last) a.out[place] = __float2bfloat16(o[i] * by);
         else a.acc[place] = o[i];
       }
     }
   }
-  sync_128();                                     // (the weights' memory and the sums are the next list's)
   tc_fence_before();
   return ok;
 }
@@ -581,8 +600,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t *w_keys = ring, *w_values = ring + C::W_SLOTS * C::W_TILE, *w_weights = sQ + 2 * C::W_Q;
   if (tid == 0) {
-    bars->poisoned = *reinterpret_cast<volatile int*>(a.err);
-    for (int i = 0; i < C::RING; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
+    for (int i = 0; i < 8; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], 4);
@@ -595,11 +613,14 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     fence_barrier_init();
     fence_proxy_async();
   }
-  __syncthreads();
-  if (bars->poisoned != 0) return;
-  if (warp == MMA_WARP) { tmem_alloc(&bars->tmem, C::TM_COLS); tmem_relinquish(); }
+  griddep_launch();                               // (the second kernel's CTAs come as these end; they wait for all of this grid)
   if (warp == TMA_WARP && lane == 0) { tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
-  make_lists(lists, a, tid, warp, lane);
+  if (!make_lists(lists, bars, a, tid, warp, lane)) {
+    if (blockIdx.x == gridDim.x - 1)              // (the second kernel finds that there is nothing)
+      for (int i = tid; i < 2 * a.rows; i += THREADS) a.plan[i] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  if (warp == MMA_WARP) { tmem_alloc(&bars->tmem, C::TM_COLS); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -611,7 +632,6 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   const int cta = tall ? before : static_cast<int>(blockIdx.x) - before;
   const int units = tall ? lists.tall_units : lists.wide_units, per = tall ? lists.tall_per_cta : lists.wide_per_cta;
   const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(cta) * per)), u1 = min(units, u0 + per);
-  const int total = u1 - u0;                      // its tiles; t counts them
   bool ok = true;
   // pool row of the box of tokens that holds `key`, by a row's table
   auto pool_row = [&](int row, int key) -> int {
@@ -633,12 +653,9 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     __syncwarp();
   };
 
-  if (total == 0) {
-    // (fewer tiles than CTAs)
-  } else if (tall && warp == TMA_WARP) {
-    // K(0) K(1) V(0) K(2) V(1) ... V(total - 1)
-    int slot = 0, list = -1, j = 0, tiles = 0;
-    uint32_t phase = 1;
+  if (tall && warp == TMA_WARP) {
+    // K(0) K(1) V(0) K(2) V(1) ...  (t counts the CTA's tiles, over all lists)
+    int list = -1, j = 0, tiles = 0, total = 0x3fffffff;
     int row0 = 0, row1 = 0, hk0 = 0, hk1 = 0;     // of the last even and odd tile whose keys were asked for
     unsigned lanes0 = 0, lanes1 = 0;
 #pragma unroll 1
@@ -653,12 +670,13 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (!ok) break;
             if (lane == 0) {
               if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
-              next_list<true>(lists.item[list & 1], lists, a, u0 + t, u1, list == 0);
+              next_list<true>(lists.item[list & 1], lists, a, u0, u1, list == 0);
               mbar_arrive(&bars->list_full[list & 1]);
             }
             __syncwarp();
             tiles = lists.item[list & 1].tiles;
             j = 0;
+            if (tiles == 0) { total = t; continue; }
           }
           const Item& w = lists.item[list & 1];
           const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
@@ -668,37 +686,37 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           if (t & 1) { row1 = row; lanes1 = lanes; hk1 = w.hk; } else { row0 = row; lanes0 = lanes; hk0 = w.hk; }
           ++j;
         }
-        ok = wait(&bars->empty[slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        const int at = what == 1 ? t : t - 2, slot = at % C::HALF, bar = 4 * (1 - what) + slot;
+        ok = wait(&bars->empty[bar], ((at / C::HALF) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
         if (!ok) break;
-        load(what == 1 ? &tk : &tv, ring + slot * C::SLOT, BN, &bars->full[slot], t & 1 ? row1 : row0, t & 1 ? lanes1 : lanes0, t & 1 ? hk1 : hk0);
-        if (++slot == C::RING) { slot = 0; phase ^= 1; }
+        load(what == 1 ? &tk : &tv, ring + (slot + (what == 1 ? 0 : C::HALF)) * C::SLOT, BN, &bars->full[bar], t & 1 ? row1 : row0, t & 1 ? lanes1 : lanes0, t & 1 ? hk1 : hk0);
       }
     }
   } else if (tall && warp == MMA_WARP) {
     // over the tiles of all lists: S(0) S(1) PV(0) S(2) PV(1) ... (the warp waits together, one lane issues)
     constexpr uint32_t idesc_qk = make_idesc(BM, BN, 1, 1, 0, 0);
     constexpr uint32_t idesc_pv = make_idesc(BM, D, 1, 1, 0, 1);
-    int slot = 0, list = -1, j = 0, tiles = 0;
-    uint32_t phase = 0, fresh = 0;                // (fresh: a bit for each buffer, whether its tile is its list's first)
+    int list = -1, j = 0, tiles = 0, total = 0x3fffffff;
+    uint32_t fresh = 0;                           // (fresh: a bit for each buffer, whether its tile is its list's first)
     const uint32_t qa = smem_u32(sQ);
 #pragma unroll 1
     for (int t = 0; ok && t < total + 2; ++t) {
       const int b = t & 1;
       if (t >= 2) {                               // PV(t - 2)
-        ok = wait(&bars->full[slot], phase, abort_flag, a.err, ERR_WAIT_FULL, lane) && wait(&bars->p_full[b], ((t - 2) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        const int slot = (t - 2) % C::HALF;
+        ok = wait(&bars->full[4 + slot], ((t - 2) / C::HALF) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) && wait(&bars->p_full[b], ((t - 2) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t va = smem_u32(ring + slot * C::SLOT);
+        const uint32_t va = smem_u32(ring + (C::HALF + slot) * C::SLOT);
         const uint32_t add = fresh >> b & 1 ? 0u : 1u;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
             umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 ? 1u : add);
           umma_commit(&bars->done);
-          umma_commit(&bars->empty[slot]);
+          umma_commit(&bars->empty[4 + slot]);
         }
         __syncwarp();
-        if (++slot == C::RING) { slot = 0; phase ^= 1; }
       }
       if (t >= total) continue;
       fresh &= ~(1u << b);
@@ -707,6 +725,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
         tiles = lists.item[list & 1].tiles;
+        if (tiles == 0) { total = t; continue; }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
         ok = wait(&bars->q_full, list & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
@@ -714,7 +733,8 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         fresh |= 1u << b;
       }
       ++j;
-      ok = ok && wait(&bars->full[slot], phase, abort_flag, a.err, ERR_WAIT_FULL, lane);
+      const int slot = t % C::HALF;
+      ok = ok && wait(&bars->full[slot], (t / C::HALF) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
       if (!ok) break;
       tc_fence_after();
       const uint32_t ka = smem_u32(ring + slot * C::SLOT);
@@ -727,21 +747,24 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         umma_commit(&bars->empty[slot]);
       }
       __syncwarp();
-      if (++slot == C::RING) { slot = 0; phase ^= 1; }
     }
   } else if (tall) {
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t t_s = tmem + lane_addr, t_o = tmem + lane_addr + C::TM_O;
+    // scores take their scale with the maximum's subtraction, where that orders them and nothing comes between
+    const bool plain = a.cap_log2 <= 0.f && a.scale_log2 > 0.f;
+    const float factor = plain ? a.scale_log2 : 1.f;
     float* to = nullptr;                          // where the last list's result goes
     bool active = false;
 #pragma unroll 1
     for (int t = 0, list = 0;; ++list) {
+      // all scores of the lists before are made: the next one's queries may take the place of theirs
       const Item& w = lists.item[list & 1];
+      ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+      if (!ok) break;
+      const int tiles = w.tiles;
       int one = -1;
-      if (t < total) {
-        // all scores of the lists before are made: the next one's queries may take the place of theirs
-        ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
-        if (!ok) break;
+      if (tiles > 0) {
         one = query(lists, a, w, tid);
         fetch_queries<D>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
         if (lane == 0) mbar_arrive(&bars->q_full);
@@ -762,22 +785,20 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         tc_fence_before();
       }
-      if (t >= total) break;
-      const int tiles = w.tiles;
+      if (tiles == 0) break;
       const bool mine = tid < w.n;
       active = warp * 32 < w.n;
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-    #pragma unroll 1
-  for (int j = 0; j < tiles; ++j, ++t) {
+      for (int j = 0; j < tiles; ++j, ++t) {
         const int b = t & 1;
-        ok = wait(&bars->s_full[b], (t >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL, lane);
-        if (!ok) break;
-        tc_fence_after();
         // which of the tile's keys the list sees
         const int key0 = w.keys.tile<BN>(w.from + j) * BN;
         const uint32_t sees[2] = {__ballot_sync(FULL, w.keys.sees(key0 + lane)), __ballot_sync(FULL, w.keys.sees(key0 + 32 + lane))};
         const bool whole = (sees[0] & sees[1]) == FULL;
+        ok = wait(&bars->s_full[b], (t >> 1) & 1, abort_flag, a.err, ERR_WAIT_TMEM_FULL, lane);
+        if (!ok) break;
+        tc_fence_after();
         if (active) {
           float s[BN];
           {
@@ -786,13 +807,17 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             tmem_ld_32x32b_x32(t_s + b * BN + 32, v[1]);
             tmem_ld_wait();
 #pragma unroll
-            for (int x = 0; x < BN; ++x) s[x] = __uint_as_float(v[x >> 5][x & 31]) * a.scale_log2;
+            for (int x = 0; x < BN; ++x) s[x] = __uint_as_float(v[x >> 5][x & 31]);
           }
-          if (a.cap_log2 > 0.f) {
-            // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), in the log2 domain
-            const float twice = 2.f * LOG2E / a.cap_log2;
+          if (!plain) {
 #pragma unroll
-            for (int x = 0; x < BN; ++x) s[x] = fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + fast_exp2(s[x] * twice)), a.cap_log2);
+            for (int x = 0; x < BN; ++x) s[x] *= a.scale_log2;
+            if (a.cap_log2 > 0.f) {
+              // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), in the log2 domain
+              const float twice = 2.f * LOG2E / a.cap_log2;
+#pragma unroll
+              for (int x = 0; x < BN; ++x) s[x] = fmaf(-2.f * a.cap_log2, __fdividef(1.f, 1.f + fast_exp2(s[x] * twice)), a.cap_log2);
+            }
           }
           if (!whole) {
 #pragma unroll
@@ -800,10 +825,10 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int x = 4; x < BN; x += 4)
+          for (int x = 4; x < BN; x += 8)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], s[x + q]);
-          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            for (int q = 0; q < 4; ++q) mx[q] = x + 4 + q < BN ? fmaxf(fmaxf(mx[q], s[x + q]), s[x + 4 + q]) : fmaxf(mx[q], s[x + q]);
+          const float m_new = fmaxf(m, factor * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           const bool need = mine && (m_new - m > RESCALE || (m == -INFINITY && m_new > -INFINITY));
           if (__any_sync(FULL, need)) {
             const float by = need && m > -INFINITY ? fast_exp2(m - m_new) : 1.f;
@@ -813,7 +838,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               ok = wait(&bars->done, (t - 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
               if (!ok) break;
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[16];
                 tmem_ld_32x32b_x16(t_o + c * 16, v);
@@ -825,26 +850,31 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             }
           }
           const float base = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t times = pair_of(factor, factor), less = pair_of(-base, -base);
+          uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-              const float p0 = fast_exp2(s[c * 32 + 2 * x] - base), p1 = fast_exp2(s[c * 32 + 2 * x + 1] - base);
+              float p0, p1;
+              unpair(fma2(pair_of(s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]), times, less), p0, p1);
+              p0 = fast_exp2(p0);
+              p1 = fast_exp2(p1);
               pk[x] = pack_bf16(p0, p1);
-              sum[2 * c] += p0;
-              sum[2 * c + 1] += p1;
+              if (x & 1) sum1 = add2(sum1, pair_of(p0, p1)); else sum0 = add2(sum0, pair_of(p0, p1));
             }
             tmem_st_32x32b_x16(t_s + b * BN + c * 16, pk);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          float p0, p1;
+          unpair(add2(sum0, sum1), p0, p1);
+          l += p0 + p1;
           tmem_st_wait();
         }
         if (!whole) {
           // values that nobody sees, to zero, in the slot that the t-th value tile has
-          const int at = t + 1 < total ? 2 + 2 * t : 2 * total - 1, slot = at % C::RING;
-          ok = wait(&bars->full[slot], (at / C::RING) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
+          const int slot = t % C::HALF;
+          ok = wait(&bars->full[4 + slot], (t / C::HALF) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
           if (!ok) break;
           const int x = tid >> 1;                 // a key's values by two threads
           if (!((x < 32 ? sees[0] : sees[1]) >> (x & 31) & 1)) {
@@ -852,7 +882,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             for (int p = 0; p < C::SUB; ++p)
 #pragma unroll
               for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<uint4*>(ring + slot * C::SLOT + p * (BN * 128) + x * 128 + ((tid & 1) * 4 + c) * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(ring + (C::HALF + slot) * C::SLOT + p * (BN * 128) + x * 128 + ((tid & 1) * 4 + c) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
         }
@@ -875,7 +905,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     // K(0) V(0) K(1) V(1) ...
     int list = -1, j = 0, tiles = 0;
 #pragma unroll 1
-    for (int t = 0; ok && t < total; ++t, ++j) {
+    for (int t = 0; ok; ++t, ++j) {
       const bool begins = j == tiles;
       const int slot = t % C::W_SLOTS;
       const uint32_t phase = ((t / C::W_SLOTS) & 1) ^ 1;
@@ -885,11 +915,15 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (!ok) break;
         if (lane == 0) {
           if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
-          next_list<false>(lists.item[list & 1], lists, a, u0 + t, u1, list == 0);
+          next_list<false>(lists.item[list & 1], lists, a, u0, u1, list == 0);
         }
         __syncwarp();
         tiles = lists.item[list & 1].tiles;
         j = 0;
+        if (tiles == 0) {
+          if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
+          break;
+        }
       }
       const Item& w = lists.item[list & 1];
       const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
@@ -898,9 +932,9 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       const unsigned lanes = __ballot_sync(FULL, any);
 #pragma unroll 1
       for (int what = 0; what < 2 && ok; ++what) {                 // keys, values
-        ok = wait(&bars->empty[2 * what + slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        ok = wait(&bars->empty[4 * what + slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
         if (!ok) break;
-        load(what == 0 ? &tk : &tv, (what == 0 ? w_keys : w_values) + slot * C::W_TILE, WK, &bars->full[2 * what + slot], row, lanes, w.hk);
+        load(what == 0 ? &tk : &tv, (what == 0 ? w_keys : w_values) + slot * C::W_TILE, WK, &bars->full[4 * what + slot], row, lanes, w.hk);
         if (what == 0 && begins) {
           fetch_queries<D>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
           if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
@@ -911,21 +945,22 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     // S(0) S(1) PV(0) S(2) PV(1) ...
     constexpr uint32_t idesc_s[2] = {make_idesc(WK, 16, 1, 1, 0, 0), make_idesc(WK, 32, 1, 1, 0, 0)};
     constexpr uint32_t idesc_o[2] = {make_idesc(128, 16, 1, 1, 1, 0), make_idesc(128, 32, 1, 1, 1, 0)};
-    int list = -1, j = 0, tiles = 0;
+    int list = -1, j = 0, tiles = 0, total = 0x3fffffff;
     bool more = false;                            // than 16 queries
     uint32_t flags = 0;                           // bits b: whether the tile in buffer b is its list's first, 2 + b: whether its list has more than 16 queries
 #pragma unroll 1
     for (int t = 0; ok && t <= total; ++t) {
+      if (j == tiles && t < total) {
+        ++list;
+        ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        if (!ok) break;
+        tiles = lists.item[list & 1].tiles;
+        more = lists.item[list & 1].n > 16;
+        j = 0;
+        if (tiles == 0) total = t;
+      }
       if (t < total) {                            // S(t)
         const int b = t & 1, slot = t % C::W_SLOTS;
-        if (j == tiles) {
-          ++list;
-          ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
-          if (!ok) break;
-          tiles = lists.item[list & 1].tiles;
-          more = lists.item[list & 1].n > 16;
-          j = 0;
-        }
         flags = (flags & ~(5u << b)) | ((j == 0 ? 1u : 0u) | (more ? 4u : 0u)) << b;
         ++j;
         ok = wait(&bars->full[slot], (t / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
@@ -945,7 +980,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
       if (t == 0) continue;
       const int b = (t - 1) & 1, slot = (t - 1) % C::W_SLOTS;      // PV(t - 1)
-      ok = wait(&bars->full[2 + slot], ((t - 1) / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) &&
+      ok = wait(&bars->full[4 + slot], ((t - 1) / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) &&
            wait(&bars->p_full[b], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
       if (!ok) break;
       tc_fence_after();
@@ -959,7 +994,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
                          make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
         umma_commit(&bars->done);
-        umma_commit(&bars->empty[2 + slot]);
+        umma_commit(&bars->empty[4 + slot]);
       }
       __syncwarp();
     }
@@ -967,11 +1002,12 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, bars, abort_flag, tid, warp, lane, cta};
 #pragma unroll 1
-    for (int t = 0, list = 0; t < total; ++list) {
+    for (int t = 0, list = 0;; ++list) {
       const int q = list & 1;
       ok = wait(&bars->list_full[q], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
       if (any_of_128(!ok)) break;                 // (all warps or none)
       const Item& w = lists.item[q];              // (not a copy: the registers are for scores)
+      if (w.tiles == 0) break;
       ok = w.n <= 8 ? wide_list<D, 8>(x, lists, a, w, t) : w.n <= 16 ? wide_list<D, 16>(x, lists, a, w, t) : wide_list<D, 32>(x, lists, a, w, t);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->list_empty[q]);
@@ -987,56 +1023,84 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   }
 }
 
-// A CTA a (place, key head), a warp a query: the pieces of its group's list and of its row's.
+// A CTA a (place, key head), a warp a query: the pieces of its group's list and of its row's.  Bound by latency: what does not come from the first kernel is read before it ends.
 template <int D>
 __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a, int ctas) {
+  constexpr int EACH = D / 32;                    // a lane's neighbouring columns
   const int place = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ratio = a.ratio, chunks = a.chunks;
   const int row = a.order[place];
-  const int4 lists = a.plan[2 * place], group = a.plan[2 * place + 1];
-  if (row < 0 || row >= a.rows) return;
-  const bool rests = a.lengths[row] <= 0, tall = group.y > 0;
-  const int pieces = (group.y + BM - 1) / BM;
+  const bool there = row >= 0 && row < a.rows, rests = !there || a.lengths[row] <= 0;
   const long long all = static_cast<long long>(a.rows) * a.heads, wide0 = 2 * all + static_cast<long long>(ctas) * 2 * BM;
-  constexpr int EACH = D / 32;
-  for (int h = warp; h < ratio; h += 4) {
-    const int head = hk * ratio + h;
+  float sink = a.sinks != nullptr && warp < a.ratio ? a.sinks[hk * a.ratio + warp] * LOG2E : -INFINITY;
+  griddep_wait();
+  if (!there) return;
+  const int4 lists = a.plan[2 * place], group = a.plan[2 * place + 1];
+  const bool tall = group.y > 0;
+#pragma unroll 1
+  for (int h = warp; h < a.ratio; h += 4) {
+    const int head = hk * a.ratio + h;
     const long long one = static_cast<long long>(row) * a.heads + head;
-    // the two lists: units a CTA, first unit, tiles, where a CTA's pieces are and how tall, lane
-    const int x = (place - group.x) * ratio + h, c = h / WN;
-    const int per[2] = {tall ? group.z : group.w, group.w};
-    const int start[2] = {lists.x + (tall ? hk * pieces + x / BM : hk) * lists.y, lists.z + (hk * chunks + c) * lists.w};
-    const int n[2] = {rests ? 0 : lists.y, rests ? 0 : lists.w};
-    const long long at[2] = {tall ? 2 * all + x % BM : wide0 + x, wide0 + h - c * WN};
-    const int step[2] = {tall ? BM : WN, WN};
-    if (n[0] == 0 && n[1] > 0 && start[1] / per[1] == (start[1] + n[1] - 1) / per[1]) continue;      // finished
-    float top = a.sinks != nullptr ? a.sinks[head] * LOG2E : -INFINITY, sum = top > -INFINITY ? 1.f : 0.f, o[EACH];
+    if (h > warp && a.sinks != nullptr) sink = a.sinks[head] * LOG2E;
+    float top = sink, sum = top > -INFINITY ? 1.f : 0.f, o[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) o[i] = 0.f;
-#pragma unroll
+    bool finished = false;
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-      if (n[k] == 0) continue;
-      const int c0 = start[k] / per[k], c1 = (start[k] + n[k] - 1) / per[k];
+      const int n = rests ? 0 : k == 0 ? lists.y : lists.w;
+      if (n == 0) continue;
+      // the list's first tile in its sequence, units a CTA, the queries' places in a CTA's piece
+      int start, per, step;
+      long long at;
+      if (k == 0) {
+        const int x = (place - group.x) * a.ratio + h, pieces = (group.y + BM - 1) / BM;
+        start = lists.x + (tall ? (hk * pieces + x / BM) * (n + TALL_GAP) + TALL_GAP : hk * (n + WIDE_GAP) + WIDE_GAP);
+        per = tall ? group.z : group.w;
+        step = tall ? BM : WN;
+        at = tall ? 2 * all + x % BM : wide0 + x;
+      } else {
+        const int c = h / WN;
+        start = lists.z + (hk * a.chunks + c) * (n + WIDE_GAP) + WIDE_GAP;
+        per = group.w;
+        step = WN;
+        at = wide0 + h - c * WN;
+      }
+      const int c0 = start / per, c1 = (start + n - 1) / per;
+      finished = k == 1 && lists.y == 0 && c0 == c1;
+      if (finished) break;
+#pragma unroll 2
       for (int cta = c0; cta <= c1; ++cta) {
-        const long long from = c0 == c1 ? k * all + one : at[k] + (2ll * cta + (cta == c0 ? 1 : 0)) * step[k];
+        const long long from = c0 == c1 ? k * all + one : at + (2ll * cta + (cta == c0 ? 1 : 0)) * step;
         const float2 ml = a.ml[from];
         float v[EACH];
+        const float* p = a.acc + from * D + lane * EACH;
+        if constexpr (EACH == 2) {
+          const float2 x = *reinterpret_cast<const float2*>(p);
+          v[0] = x.x; v[1] = x.y;
+        } else {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) v[i] = a.acc[from * D + i * 32 + lane];
-        if (ml.x == -INFINITY) {                   // (nothing but scores of minus infinity, or none that is a number)
-          if (ml.y != ml.y) sum = ml.y;
-          continue;
+          for (int i = 0; i < EACH; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p + i);
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+          }
         }
-        const float m = fmaxf(top, ml.x), was = top > -INFINITY ? fast_exp2(top - m) : 0.f, is = fast_exp2(ml.x - m);
-        sum = sum * was + ml.y * is;
+        // (nothing but scores of minus infinity: nothing to add, unless none was a number)
+        const float m = fmaxf(top, ml.x), was = top > -INFINITY ? fast_exp2(top - m) : 0.f, is = ml.x > -INFINITY ? fast_exp2(ml.x - m) : 0.f;
+        sum = ml.y != ml.y ? ml.y : sum * was + ml.y * is;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) o[i] = o[i] * was + v[i] * is;
+        for (int i = 0; i < EACH; ++i) o[i] = o[i] * was + (is > 0.f ? v[i] * is : 0.f);
         top = m;
       }
     }
+    if (finished) continue;
     const float by = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    uint32_t w[EACH / 2];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) a.out[one * D + i * 32 + lane] = __float2bfloat16(o[i] * by);
+    for (int i = 0; i < EACH; i += 2) w[i / 2] = pack_bf16(o[i] * by, o[i + 1] * by);
+    __nv_bfloat16* to = a.out + one * D + lane * EACH;
+    if constexpr (EACH == 2) *reinterpret_cast<uint32_t*>(to) = w[0];
+    else if constexpr (EACH == 4) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -1061,8 +1125,16 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas
   if (e != cudaSuccess) return static_cast<int>(e);
   shared_mma_kernel<D><<<ctas, THREADS, SMEM, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
-  join_pieces_kernel<D><<<dim3(a.rows, a.kv_heads), 128, 0, stream>>>(a, ctas);
-  return static_cast<int>(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows, a.kv_heads);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, join_pieces_kernel<D>, a, ctas));
 }
 
 }  // namespace sharedmma
@@ -1081,7 +1153,7 @@ extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const v
   const long long most = static_cast<long long>(max_pages) * page_size, chunks = heads > 0 && kv_heads > 0 ? (heads / kv_heads + WN - 1) / WN : 1;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || page_size % 16 != 0 || max_pages <= 0 || pages <= 0 || groups <= 0 || groups > MOST_ROWS ||
       rows > MOST_ROWS || window < 0 || least < 1 || ctas < 1 || most > 0x3fffffffll || static_cast<long long>(pages) * page_size > 0x7fffff00ll || kv_heads > 65535 ||
-      (2ll * rows * chunks + groups) * kv_heads * ((most + BN - 1) / BN + 1) > 0x3fffffffll || q_stride % 8 != 0 ||
+      (2ll * rows * chunks + groups) * kv_heads * ((most + BN - 1) / BN + 1 + TALL_GAP) > 0x3fffffffll || q_stride % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc) |
         reinterpret_cast<uintptr_t>(plan)) & 15))
     return -3;
