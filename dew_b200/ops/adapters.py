@@ -15,6 +15,18 @@ class Bank(NamedTuple):
     scale: torch.Tensor
 
 
+SCANNED = 512            # tokens whose ids every CTA looks through; more are grouped by a kernel of their own
+
+
+def on_tensor_cores(x: torch.Tensor, n: int, rank: int) -> bool:
+    return x.dtype == torch.bfloat16 and n <= 4096 and rank <= 512
+
+
+def _splits(tiles: int, rank: int, width: int) -> int:
+    """Parts of the width that are summed apart: enough CTAs for the SMs, each with 128 columns a warp at least."""
+    return max(1, min(16, width // 512, 592 // max(1, tiles * -(-rank // 64))))
+
+
 def _check(x, bank: Bank, ids, out: int, weight_device) -> None:
     a, b, scale = bank
     if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or scale.shape != a.shape[:1]:
@@ -58,11 +70,24 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
     ids = ids.contiguous()
     n, rank, width = bank.a.shape
     tokens, out = x2.shape[0], y.shape[-1]
-    splits = max(1, min(16, width // 256, 592 // tokens))
-    low = torch.empty(splits * tokens * rank, dtype=torch.float32, device=x.device)
+    err = L.status(x.device).data_ptr()
     with L.on_device_of(x) as stream:
+        if on_tensor_cores(x, n, rank):
+            # one piece of scratch a call: the rank's values by parts of the width, the tokens by adapter, their tiles
+            grouped = tokens > SCANNED
+            splits = _splits(tokens // 64 + 1 if grouped else min(tokens, n), rank, width)
+            values = -(-splits * tokens * rank // 4) * 4
+            scratch = torch.empty(values + (-(-tokens // 4) * 4 + 4 * (tokens // 64 + min(n, tokens) + 2) if grouped else 0), dtype=torch.float32, device=x.device)
+            at = scratch.data_ptr()
+            order = at + 4 * values if grouped else 0
+            L.check(L.load().dewb_add_adapters_mma(x2.data_ptr(), x2.stride(0), bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), ids.data_ptr(), order,
+                                                   order + -(-tokens // 4) * 16 if grouped else 0, at, y.data_ptr(), tokens, n, rank, width, out, splits, err, stream), "add_adapters_mma")
+            L.count_launches(3 if grouped else 2)
+            return y
+        splits = max(1, min(16, width // 256, 592 // tokens))
+        low = torch.empty(splits * tokens * rank, dtype=torch.float32, device=x.device)
         L.check(L.load().dewb_add_adapters(x2.data_ptr(), x2.stride(0), bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), ids.data_ptr(), low.data_ptr(), y.data_ptr(),
-                                           tokens, n, rank, width, out, splits, int(x.dtype == torch.float32), L.status(x.device).data_ptr(), stream), "add_adapters")
+                                           tokens, n, rank, width, out, splits, int(x.dtype == torch.float32), err, stream), "add_adapters")
     L.count_launches(2)
     return y
 

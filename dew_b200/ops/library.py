@@ -84,6 +84,7 @@ _SIGNATURES = {
     "dewb_check_moves": "ppii" + "ppppi" + "ii",
     "dewb_shared_decode": "pl" + "pppp" + "ppppp" + "p" + "pppp" + "iiiiiiiiii" + "ff" + "ii" + "pp",
     "dewb_shared_decode_mma": "pl" + "pp" + "ppppp" + "p" + "pppp" + "iiiiiiiiiii" + "ff" + "pp",
+    "dewb_add_adapters_mma": "pl" + "pppp" + "pppp" + "iiiiii" + "pp",
     "dewb_add_adapters": "pl" + "pppp" + "pp" + "iiiiiii" + "pp",
     "dewb_rope_append": "pppp" + "iiiii" + "ppp" + "ii" + "p",
     "dewb_paged_decode_persist": "ppp" + "l" + "pppppppp" + "iiiiiii" + "f" + "iii" + "f" + "pp" + "l" + "i" + "pp",
