@@ -1,16 +1,18 @@
 // Low-rank adapters of many requests beside one projection:  y_t += s_i B_i (A_i x_t),  i the adapter of token t (below 0: none).
 //
-// Two kernels: shares of A_i x in fp32 (the width is split over CTAs), then B_i times their sum, added to y.  An adapter's tokens are worked on together, up to 16 (steps of
-// generation) or 64 (prompts) of them as the rows of products on the tensor cores, so that its A and B come from memory once for all of them.
+// An adapter's tokens are worked on together, so that its A and B come from memory once for all of them.
 //
-//   rows of a tile   up to 512 tokens: each CTA looks through the ids itself.  CTA t goes on if token t is the first, 17th, 33rd ... of its adapter.  More tokens: a kernel of one
-//                    CTA counts them and writes the tiles down (8192 tokens: 5 us, where looking through them all in each CTA would take longer than the products).
-//   operands         go from memory to registers as the products take them.  A lane of m16n8k16 holds two pairs of neighbouring elements of a row; which elements of the
-//                    sum they are does not matter as long as both operands agree.  So a lane takes eight in a row (16 bytes), four lanes 32, and calls them two products' worth.
-//   results          the columns of four n8 blocks are dealt so that a lane's eight are neighbours: y is read and written 16 bytes at a time.
+// STEPS OF GENERATION, up to 512 tokens: one kernel.  A cluster of eight CTAs takes up to 16 tokens of an adapter: each makes the products with A over an eighth of the width, they
+// add them up through one another's shared memory, and each multiplies with an eighth of B's rows.  Cluster t goes on if token t is the first, 17th, 33rd ... of its adapter, which
+// it finds out by looking through the ids.  Operands go from memory to registers as the warp-level products take them (16 rows are too few for the others): a lane of m16n8k16 holds
+// two pairs of neighbouring elements of a row, and which elements of the sum they are does not matter as long as both operands agree.  So a lane takes eight in a row (16 bytes),
+// four lanes 32, and calls them two products' worth.  B and y are on their way while A's products are added up.  The columns of four n8 blocks are dealt so that a lane's eight
+// are neighbours: y is read and written 16 bytes at a time.  Bound by latency (ids, operands, one cluster barrier, results) and, with many adapters, by reading A and B.
 //
-// Bound by memory: A and B once an adapter in a step of generation; x and twice y for prompts.  The values between the two are rounded to bf16 for the second product, after their
-// sum and scale in fp32: what an adapter adds is off by at most half a step of each rank's share.
+// PROMPTS: three kernels.  One CTA counts the tokens of each adapter and writes down tiles of up to 128.  Then 128 x 64 x width products, tokens gathered by 16-byte copies, the
+// width in parts; then a CTA a tile and 1024 columns of y: the parts' sum times the scale, rounded to bf16, times B on the tensor cores, added to y.  Bound by x and twice y.
+//
+// The values between the two products are rounded to bf16 after their sum and scale in fp32: what an adapter adds is off by at most half a step of each rank's share.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -80,9 +82,8 @@ __global__ void __launch_bounds__(128) expand_kernel(const __grid_constant__ Arg
 // ---------------------------------------------------------------------------------------------------------- bf16
 using bf16 = __nv_bfloat16;
 constexpr int SCANNED = 512;     // tokens whose ids each CTA looks through
-constexpr int RB = 64;           // rank's values a CTA makes
-constexpr int COLS = 256;        // y's columns a CTA adds to
-constexpr int MOST_ADAPTERS = 4096;
+constexpr int MOST_ADAPTERS = 4096, MOST_RANK = 512;
+constexpr uint32_t FULL = 0xffffffffu;
 
 struct Tile { int adapter, begin, count, pad; };
 
@@ -90,9 +91,9 @@ struct Mma {
   const bf16 *x, *a, *b;
   const float* scale;
   const int* ids;
-  const int *order, *tiles_n;    // the tokens by adapter, and (behind) their tiles; null: look through the ids
+  const int *order, *tiles_n;    // prompts: the tokens by adapter, and their tiles
   const Tile* tiles;
-  float* low;                    // [splits, tokens, rank]
+  float* low;                    // prompts: [splits, tokens, rank]
   bf16* y;
   long long x_stride;
   int tokens, adapters, rank, width, out, splits;
@@ -103,7 +104,7 @@ struct Mma {
 // Eight elements of a row, the first `n` of which exist.
 __device__ __forceinline__ uint4 load8(const bf16* p, int n, bool wide) {
   if (n <= 0) return make_uint4(0, 0, 0, 0);
-  if (wide) return __ldg(reinterpret_cast<const uint4*>(p));         // (n is 8: sizes are multiples of 8 then)
+  if (wide && n >= 8) return __ldg(reinterpret_cast<const uint4*>(p));
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -112,234 +113,528 @@ __device__ __forceinline__ uint4 load8(const bf16* p, int n, bool wide) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-// The CTA's tile: its adapter, and its tokens in rows[0, MT) (-1 behind the last).  False: nothing to do.  All threads.
-template <int MT>
-__device__ __forceinline__ bool find_tile(const Mma& m, int* rows, int& adapter) {
-  __shared__ int found;
-  const int lane = threadIdx.x & 31;
-  if (m.order != nullptr) {
-    if (static_cast<int>(blockIdx.x) >= *m.tiles_n) return false;
-    const Tile t = m.tiles[blockIdx.x];
-    for (int i = threadIdx.x; i < MT; i += blockDim.x) rows[i] = i < t.count ? m.order[t.begin + i] : -1;
-    adapter = t.adapter;
-    __syncthreads();
-    return true;
+__device__ __forceinline__ void store8(bf16* p, const uint32_t (&w)[4], int n, bool wide) {
+  if (wide && n >= 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = __ushort_as_bfloat16(static_cast<unsigned short>(w[e >> 1] >> (e & 1) * 16));
   }
-  if (threadIdx.x < 32) {
-    const int t0 = blockIdx.x, mine = m.ids[t0];
-    bool go = mine >= 0 && mine < m.adapters;
-    if (mine >= m.adapters && lane == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
-    int before = 0, n = 0;
-    if (go) {
-#pragma unroll 4
-      for (int i0 = 0; i0 < m.tokens; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned same = __ballot_sync(0xffffffffu, i < m.tokens && m.ids[i] == mine);
-        const unsigned earlier = t0 >= i0 + 32 ? 0xffffffffu : t0 <= i0 ? 0u : (1u << (t0 - i0)) - 1;
-        before += __popc(same & earlier);
-        const unsigned mine_on = same & ~earlier;
-        const int at = n + __popc(mine_on & ((1u << lane) - 1));
-        if ((mine_on >> lane & 1) && at < MT) rows[at] = i;
-        n += __popc(mine_on);
-      }
-      go = before % MT == 0;
-      for (int i = lane; i < MT; i += 32) if (i >= n) rows[i] = -1;
-    }
-    if (lane == 0) found = go ? mine : -1;
-  }
-  __syncthreads();
-  adapter = found;
-  return adapter >= 0;
 }
 
-// grid (tile, part of the width, 64 of the rank's values): the warps take every WARPS-th 32 of the width.
-template <int M16, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) shrink_mma_kernel(const __grid_constant__ Mma m) {
-  constexpr int MT = 16 * M16;
-  __shared__ int rows[MT];
-  extern __shared__ float sums[];                // [WARPS / 2][MT][RB]
-  int adapter;
-  griddep_launch();
-  if (m.order != nullptr) griddep_wait();        // (the tiles are the kernel's before this)
-  if (!find_tile<MT>(m, rows, adapter)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.y, r0 = blockIdx.z * RB, blocks = min(RB / 8, (m.rank - r0 + 7) / 8);
-  const int per = ((m.width + m.splits - 1) / m.splits + 31) / 32 * 32, from = split * per, to = min(m.width, from + per);
-  const bf16* xr[2 * M16];
-#pragma unroll
-  for (int i = 0; i < 2 * M16; ++i) {
-    const int row = rows[i * 8 + g];
-    xr[i] = row < 0 ? nullptr : m.x + row * m.x_stride;
-  }
-  const bf16* ar = m.a + (static_cast<long long>(adapter) * m.rank + r0 + g) * m.width;
-  float acc[M16][RB / 8][4];
-#pragma unroll
-  for (int i = 0; i < M16; ++i)
-#pragma unroll
-    for (int n = 0; n < RB / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
-#pragma unroll 2
-  for (int k0 = from + warp * 32; k0 < to; k0 += WARPS * 32) {
-    const int k = k0 + c * 8, left = to - k;
-    uint4 xv[2 * M16];
-#pragma unroll
-    for (int i = 0; i < 2 * M16; ++i) xv[i] = xr[i] == nullptr ? make_uint4(0, 0, 0, 0) : load8(xr[i] + k, left, m.wide_x);
-#pragma unroll
-    for (int n = 0; n < RB / 8; ++n) {
-      if (n >= blocks) break;
-      const uint4 av = r0 + n * 8 + g < m.rank ? load8(ar + static_cast<long long>(n) * 8 * m.width + k, left, m.wide_x) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < M16; ++i) {
-        const uint32_t one[4] = {xv[2 * i].x, xv[2 * i + 1].x, xv[2 * i].y, xv[2 * i + 1].y}, two[4] = {xv[2 * i].z, xv[2 * i + 1].z, xv[2 * i].w, xv[2 * i + 1].w};
-        mma16::mma(acc[i][n], one, av.x, av.y);
-        mma16::mma(acc[i][n], two, av.z, av.w);
-      }
-    }
-  }
-  // the warps' sums, halving their number: the upper half writes, the lower half adds
-#pragma unroll
-  for (int half = WARPS / 2; half > 0; half >>= 1) {
-    if (warp >= half && warp < 2 * half) {
-      float* to_sum = sums + (warp - half) * MT * RB;
-#pragma unroll
-      for (int i = 0; i < M16; ++i)
-#pragma unroll
-        for (int n = 0; n < RB / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) to_sum[((i * (RB / 8) + n) * 4 + e) * 32 + lane] = acc[i][n][e];
-    }
-    __syncthreads();
-    if (warp < half) {
-      const float* add = sums + warp * MT * RB;
-#pragma unroll
-      for (int i = 0; i < M16; ++i)
-#pragma unroll
-        for (int n = 0; n < RB / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][n][e] += add[((i * (RB / 8) + n) * 4 + e) * 32 + lane];
-    }
-    __syncthreads();
-  }
-  if (warp != 0) return;
-#pragma unroll
-  for (int i = 0; i < M16; ++i)
-#pragma unroll
-    for (int n = 0; n < RB / 8; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int row = rows[i * 16 + g + (e >> 1) * 8], r = r0 + n * 8 + 2 * c + (e & 1);
-        if (row >= 0 && r < m.rank) m.low[(static_cast<long long>(split) * m.tokens + row) * m.rank + r] = acc[i][n][e];
-      }
+// ---------------------------------------------------------------------------------------------------------- steps of generation
+constexpr int CLUSTER = 8, STEP_WARPS = 4, STEP_THREADS = STEP_WARPS * 32, MT = 16;
+constexpr int RB = 64;           // rank's values at a time
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// grid (tile, COLS columns of y): a warp takes every fourth 32 columns.
-template <int M16>
-__global__ void __launch_bounds__(128) expand_mma_kernel(const __grid_constant__ Mma m) {
-  constexpr int MT = 16 * M16;
+// grid (CLUSTER, tokens)
+__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __grid_constant__ Mma m) {
+  extern __shared__ __align__(16) float sums[];  // [wide / 8][16][8]: this CTA's share of the rank's values; then as bf16 [16][wide + 8]; in front, the warps' shares
+  __shared__ unsigned same[SCANNED / 32];
   __shared__ int rows[MT];
-  extern __shared__ uint4 low16[];               // [MT][rank in whole 32s] bf16, + 8 a row (bank spacing)
-  bf16* low = reinterpret_cast<bf16*>(low16);
-  int adapter;
-  if (m.order != nullptr) griddep_wait();
-  if (!find_tile<MT>(m, rows, adapter)) return;
-  if (m.order == nullptr) griddep_wait();        // (the ids are older than the kernel before this, which makes the rank's values)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int wide = (m.rank + 31) / 32 * 32, pitch = wide + 8;
-  const float by = m.scale[adapter];
-  for (int i = threadIdx.x; i < MT * wide; i += 128) {
-    const int t = i / wide, r = i - t * wide, row = rows[t];
-    float s = 0.f;
-    if (row >= 0 && r < m.rank)
-      for (int k = 0; k < m.splits; ++k) s += m.low[(static_cast<long long>(k) * m.tokens + row) * m.rank + r];
-    low[t * pitch + r] = __float2bfloat16(s * by);
-  }
-  __syncthreads();
-  int row[2 * M16];
-#pragma unroll
-  for (int i = 0; i < 2 * M16; ++i) row[i] = rows[i * 8 + g];
-  const bf16* b = m.b + static_cast<long long>(adapter) * m.out * m.rank;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int part = cluster_ctarank(), t0 = blockIdx.y;
+  // the tokens of this one's adapter
+  const int mine = m.ids[t0];
 #pragma unroll 1
-  for (int n0 = blockIdx.y * COLS + warp * 32; n0 < min(m.out, (static_cast<int>(blockIdx.y) + 1) * COLS); n0 += 128) {
-    float acc[M16][4][4];
+  for (int i0 = warp * 32; i0 < m.tokens; i0 += STEP_THREADS) {
+    const unsigned w = __ballot_sync(FULL, i0 + lane < m.tokens && m.ids[i0 + lane] == mine);
+    if (lane == 0) same[i0 >> 5] = w;
+  }
+  if (mine >= m.adapters && tid == 0 && part == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+  if (tid < MT) rows[tid] = -1;
+  __syncthreads();
+  if (mine < 0 || mine >= m.adapters) return;
+  int before = 0;
+#pragma unroll 1
+  for (int w = 0; w < t0 >> 5; ++w) before += __popc(same[w]);
+  before += __popc(same[t0 >> 5] & ((1u << (t0 & 31)) - 1));
+  if (before % MT != 0) return;                  // (all CTAs of a cluster, or none)
+#pragma unroll 1
+  for (int i = tid; i < m.tokens; i += STEP_THREADS) {
+    if (i < t0 || !(same[i >> 5] >> (i & 31) & 1)) continue;
+    int rank_of = __popc(same[i >> 5] & ((1u << (i & 31)) - 1)) - before;
+#pragma unroll 1
+    for (int w = 0; w < i >> 5; ++w) rank_of += __popc(same[w]);
+    if (rank_of < MT) rows[rank_of] = i;
+  }
+  __syncthreads();
+  const int row0 = rows[g], row1 = rows[g + 8];
+  const int wide = (m.rank + 31) / 32 * 32;
+  float* share = sums + STEP_WARPS * MT * RB;    // [MT][wide]
+  // ---- x A^T over an eighth of the width
+  {
+    const int per = ((m.width + CLUSTER - 1) / CLUSTER + 31) / 32 * 32, from = part * per, to = min(m.width, from + per);
+    const bf16 *x0 = m.x + max(row0, 0) * m.x_stride, *x1 = m.x + max(row1, 0) * m.x_stride;
+#pragma unroll 1
+    for (int r0 = 0; r0 < wide; r0 += RB) {
+      const bf16* ar = m.a + (static_cast<long long>(mine) * m.rank + r0 + g) * m.width;
+      const int blocks = min(RB / 8, (m.rank - r0 + 7) / 8);
+      float acc[RB / 8][4];
 #pragma unroll
-    for (int i = 0; i < M16; ++i)
+      for (int n = 0; n < RB / 8; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-    // y is on its way meanwhile: this lane's eight columns of each row
-    const int col = n0 + c * 8, left = m.out - col;
-    uint4 old[2 * M16];
-#pragma unroll
-    for (int i = 0; i < 2 * M16; ++i) {
-      const bf16* p = m.y + static_cast<long long>(max(row[i], 0)) * m.out + col;
-      old[i] = row[i] < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(p) : load8(p, left, false);
-    }
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll 2
-    for (int k0 = 0; k0 < m.rank; k0 += 32) {
-      const int k = k0 + c * 8;
-      uint4 bv[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + (g >> 1) * 8 + j * 2 + (g & 1);           // block j's column g
-        bv[j] = n < m.out ? load8(b + static_cast<long long>(n) * m.rank + k, m.rank - k, m.wide_b) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < M16; ++i) {
-        const uint4 lo = *reinterpret_cast<const uint4*>(low + (i * 16 + g) * pitch + k), hi = *reinterpret_cast<const uint4*>(low + (i * 16 + 8 + g) * pitch + k);
+      for (int k0 = from + warp * 32; k0 < to; k0 += STEP_WARPS * 32) {
+        const int k = k0 + c * 8, left = to - k;
+        const uint4 lo = row0 < 0 ? make_uint4(0, 0, 0, 0) : load8(x0 + k, left, m.wide_x), hi = row1 < 0 ? make_uint4(0, 0, 0, 0) : load8(x1 + k, left, m.wide_x);
         const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
+        uint4 av[RB / 8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16::mma(acc[i][j], one, bv[j].x, bv[j].y);
-          mma16::mma(acc[i][j], two, bv[j].z, bv[j].w);
+        for (int n = 0; n < RB / 8; ++n)
+          av[n] = n < blocks && r0 + n * 8 + g < m.rank ? load8(ar + static_cast<long long>(n) * 8 * m.width + k, left, m.wide_x) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < RB / 8; ++n) {
+          if (n >= blocks) break;
+          mma16::mma(acc[n], one, av[n].x, av[n].y);
+          mma16::mma(acc[n], two, av[n].z, av[n].w);
         }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 2 * M16; ++i) {
-      if (row[i] < 0 || left <= 0) continue;
+      for (int n = 0; n < RB / 8; ++n)
+        if (n < blocks) *reinterpret_cast<float4*>(sums + ((warp * (RB / 8) + n) * 32 + lane) * 4) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+      __syncthreads();
+      // the warps' shares: value e of lane l in block n is row l / 4 + 8 (e / 2), column 8 n + 2 (l % 4) + e % 2
+#pragma unroll 1
+      for (int i = tid; i < blocks * 32; i += STEP_THREADS) {
+        const int n = i >> 5, l = i & 31;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; ++w) {
+          const float4 u = *reinterpret_cast<const float4*>(sums + ((w * (RB / 8) + n) * 32 + l) * 4);
+          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        }
+        float* to_share = share + (l >> 2) * wide + r0 + n * 8 + 2 * (l & 3);
+        to_share[0] = v.x; to_share[1] = v.y; to_share[8 * wide] = v.z; to_share[8 * wide + 1] = v.w;
+      }
+      __syncthreads();
+    }
+  }
+  cluster_arrive();
+  // ---- meanwhile, this warp's first columns of B and y are fetched
+  const int per = ((m.out + CLUSTER - 1) / CLUSTER + 31) / 32 * 32, n_end = min(m.out, (part + 1) * per);
+  const bf16* b = m.b + static_cast<long long>(mine) * m.out * m.rank;
+  uint4 bv[4], old[2];
+  auto fetch_b = [&](int n0, int k) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + (g >> 1) * 8 + j * 2 + (g & 1);             // block j's column g
+      bv[j] = n < n_end ? load8(b + static_cast<long long>(n) * m.rank + k, m.rank - k, m.wide_b) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto fetch_y = [&](int n0) {
+    const int col = n0 + c * 8, left = m.out - col;
+    old[0] = row0 < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(m.y + static_cast<long long>(row0) * m.out + col)
+                                                                        : load8(m.y + static_cast<long long>(row0) * m.out + col, left, false);
+    old[1] = row1 < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(m.y + static_cast<long long>(row1) * m.out + col)
+                                                                        : load8(m.y + static_cast<long long>(row1) * m.out + col, left, false);
+  };
+  int n0 = part * per + warp * 32;
+  if (n0 < n_end) {
+    fetch_b(n0, c * 8);
+    fetch_y(n0);
+  }
+  const float by = m.scale[mine];
+  cluster_wait();
+  // ---- the CTAs' shares, their sum times the scale to bf16 (behind the shares)
+  const int pitch = wide + 8;
+  bf16* low = reinterpret_cast<bf16*>(share + MT * wide);
+  {
+    const uint32_t at = smem_u32(share);
+#pragma unroll 1
+    for (int i = tid; i < MT * wide; i += STEP_THREADS) {
+      const int t = i / wide, r = i - t * wide;
+      float v = 0.f;
+#pragma unroll
+      for (int p = 0; p < CLUSTER; ++p) v += ld_cluster(map_to_cta(at + i * 4, p));
+      low[t * pitch + r] = __float2bfloat16(r < m.rank ? v * by : 0.f);
+    }
+  }
+  cluster_arrive();                              // (its share is read by others until here)
+  __syncthreads();
+#pragma unroll 1
+  for (; n0 < n_end; n0 += STEP_THREADS) {
+    float acc[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+#pragma unroll 1
+    for (int k0 = 0; k0 < m.rank; k0 += 32) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(low + g * pitch + k0 + c * 8), hi = *reinterpret_cast<const uint4*>(low + (8 + g) * pitch + k0 + c * 8);
+      const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        mma16::mma(acc[j], one, bv[j].x, bv[j].y);
+        mma16::mma(acc[j], two, bv[j].z, bv[j].w);
+      }
+      const bool same_columns = k0 + 32 < m.rank;
+      if (same_columns || n0 + STEP_THREADS < n_end) fetch_b(same_columns ? n0 : n0 + STEP_THREADS, (same_columns ? k0 + 32 : 0) + c * 8);
+    }
+    const int col = n0 + c * 8, left = m.out - col;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = i == 0 ? row0 : row1;
       const uint32_t was[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
       uint32_t now[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(was[j]) + acc[i / 2][j][2 * (i & 1)], bf16_hi(was[j]) + acc[i / 2][j][2 * (i & 1) + 1]);
-      bf16* p = m.y + static_cast<long long>(row[i]) * m.out + col;
-      if (m.wide_y && left >= 8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(now[0], now[1], now[2], now[3]);
-      } else {
+      for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(was[j]) + acc[j][2 * i], bf16_hi(was[j]) + acc[j][2 * i + 1]);
+      if (row >= 0 && left > 0) store8(m.y + static_cast<long long>(row) * m.out + col, now, left, m.wide_y);
+    }
+    if (n0 + STEP_THREADS < n_end) fetch_y(n0 + STEP_THREADS);
+  }
+  cluster_wait();                                // (no CTA's memory goes while another reads it)
+}
+
+// ---------------------------------------------------------------------------------------------------------- prompts
+constexpr int TALL = 128;        // tokens a tile
+constexpr int KB = 64;           // columns of an operand's slot (128 bytes)
+constexpr int MAKE_STAGES = 4, AHEAD = 3;
+constexpr int X_SLOT = TALL * KB * 2, A_SLOT = RB * KB * 2, MAKE_SMEM = MAKE_STAGES * (X_SLOT + A_SLOT) + 1024;
+constexpr int ADD_COLS = 1024, ADD_N = 128, ADD_STAGES = 3, B_SLOT = ADD_N * KB * 2;
+
+// 16 bytes (8 elements, the first n of which exist) to shared memory, as zeros where there are none
+__device__ __forceinline__ void copy8(uint32_t to, const bf16* p, int n, bool wide) {
+  if (wide) {
+    const int bytes = max(0, min(n, 8)) * 2;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(bytes) : "memory");
+  } else {
+    const uint4 v = load8(p, n, false);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  }
+}
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+struct alignas(16) Bars {
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2];
+  uint32_t tmem;
+  int abort_flag, poisoned;
+  int rows[TALL];
+};
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code, int lane) {
+  if (mbar_wait_warp(bar, parity, abort_flag)) return true;
+  if (lane == 0) atomicCAS(err, 0, code);
+  return false;
+}
+
+// grid (tile, part of the width, 64 of the rank's values); warps 0..3 fetch and write, warp 4 issues products
+__global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ Mma m) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ Bars bars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < MAKE_STAGES; ++i) { mbar_init(&bars.full[i], 4); mbar_init(&bars.empty[i], 1); }
+    mbar_init(&bars.acc_full[0], 1);
+    bars.abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+    bars.poisoned = *reinterpret_cast<volatile int*>(m.err);
+  }
+  griddep_launch();
+  griddep_wait();                                // (the tiles are the kernel's before this)
+  __syncthreads();
+  if (bars.poisoned != 0 || static_cast<int>(blockIdx.x) >= *m.tiles_n) return;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+    return;
+  }
+  const Tile tile = m.tiles[blockIdx.x];
+  if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
+  if (warp == 4) { tmem_alloc(&bars.tmem, 64); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int split = blockIdx.y, r0 = blockIdx.z * RB, ranks = min(RB, m.rank - r0), n16 = (ranks + 15) / 16;
+  const int per = ((m.width + m.splits - 1) / m.splits + KB - 1) / KB * KB, from = split * per, to = min(m.width, from + per);
+  const int steps = max(0, (to - from + KB - 1) / KB);
+  uint8_t *sx = smem, *sa = smem + MAKE_STAGES * X_SLOT;
+  if (warp < 4) {
+    const int c = tid & 7;
+    const bf16* xr[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = bars.rows[(tid >> 3) + 16 * e];
+      xr[e] = row < 0 ? nullptr : m.x + row * m.x_stride + c * 8;
+    }
+    const bf16* ar = m.a + (static_cast<long long>(tile.adapter) * m.rank + r0 + (tid >> 3)) * m.width + c * 8;
+    bool ok = true;
+#pragma unroll 1
+    for (int s = 0; s < steps + AHEAD; ++s) {
+      if (s < steps) {
+        const int slot = s % MAKE_STAGES;
+        ok = ok && wait(&bars.empty[slot], ((s / MAKE_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+        const int k = from + s * KB, left = to - k - c * 8;
+        const uint32_t xs = smem_u32(sx + slot * X_SLOT) + (tid >> 3) * 128 + ((c ^ ((tid >> 3) & 7)) << 4);
+        const uint32_t as = smem_u32(sa + slot * A_SLOT) + (tid >> 3) * 128 + ((c ^ ((tid >> 3) & 7)) << 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < left) p[e] = __ushort_as_bfloat16(static_cast<unsigned short>(now[e >> 1] >> (e & 1) * 16));
+          if (xr[e] != nullptr) copy8(xs + e * 2048, left > 0 ? xr[e] + k : xr[e], left, m.wide_x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((tid >> 3) + 16 * e < ranks) copy8(as + e * 2048, left > 0 ? ar + static_cast<long long>(e) * 16 * m.width + k : m.a, left, m.wide_x);
+      }
+      copies_end_group();
+      if (s >= AHEAD) {
+        copies_wait<AHEAD>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.full[(s - AHEAD) % MAKE_STAGES]);
       }
     }
+    if (steps > 0) ok = wait(&bars.acc_full[0], 0, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane) && ok;
+    tc_fence_after();
+    const int row = bars.rows[tid];
+    float* low = m.low + (static_cast<long long>(split) * m.tokens + max(row, 0)) * m.rank + r0;
+#pragma unroll 1
+    for (int c16 = 0; c16 < n16; ++c16) {
+      uint32_t v[16];
+      tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c16 * 16, v);
+      tmem_ld_wait();
+      if (row >= 0) {
+        if (steps == 0)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0;
+        if (m.rank % 4 == 0 && c16 * 16 + 16 <= ranks) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint4*>(low + c16 * 16 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (c16 * 16 + i < ranks) low[c16 * 16 + i] = __uint_as_float(v[i]);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    const uint32_t idesc = make_idesc(TALL, 16, 1, 1, 0, 0) + (static_cast<uint32_t>((n16 - 1) * 16 >> 3) << 17);
+    bool ok = true;
+#pragma unroll 1
+    for (int s = 0; s < steps && ok; ++s) {
+      const int slot = s % MAKE_STAGES;
+      ok = wait(&bars.full[slot], (s / MAKE_STAGES) & 1, abort_flag, m.err, ERR_WAIT_FULL, lane);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t xa = smem_u32(sx + slot * X_SLOT), aa = smem_u32(sa + slot * A_SLOT);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; ++kk)
+          umma_bf16_ss(tmem, make_sdesc_sw128(xa + kk * 32, 16, 1024), make_sdesc_sw128(aa + kk * 32, 16, 1024), idesc, s > 0 || kk > 0 ? 1u : 0u);
+        umma_commit(&bars.empty[slot]);
+        if (s == steps - 1) umma_commit(&bars.acc_full[0]);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 64);
   }
 }
 
-// One CTA: the tokens by adapter, and tiles of up to `tall` of them.  (Where a token stands among its adapter's does not change its result.)
-__global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restrict__ ids, int tokens, int adapters, int tall, int* __restrict__ order, int* __restrict__ tiles_n,
+// grid (tile, ADD_COLS columns of y); warps 0..3 add to y, 4..7 fetch B, 8 issues products of 128 tokens and 128 columns
+__global__ void __launch_bounds__(288, 2) add_columns_kernel(const __grid_constant__ Mma m) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ Bars bars;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < ADD_STAGES; ++i) { mbar_init(&bars.full[i], 4); mbar_init(&bars.empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4); }
+    bars.abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+    bars.poisoned = *reinterpret_cast<volatile int*>(m.err);
+  }
+  griddep_wait();
+  __syncthreads();
+  if (bars.poisoned != 0 || static_cast<int>(blockIdx.x) >= *m.tiles_n) return;
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+    return;
+  }
+  const Tile tile = m.tiles[blockIdx.x];
+  const int kblocks = (m.rank + KB - 1) / KB;
+  if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
+  if (warp == 8) { tmem_alloc(&bars.tmem, 2 * ADD_N); tmem_relinquish(); }
+  uint8_t *sl = smem, *sb = smem + kblocks * X_SLOT;
+  __syncthreads();
+  {
+    // the rank's values: the parts' sum, times the scale, eight a thread
+    const float by = m.scale[tile.adapter];
+#pragma unroll 1
+    for (int i = tid; i < TALL * kblocks * 8; i += 288) {
+      const int t = i / (kblocks * 8), k = i - t * kblocks * 8, row = bars.rows[t], n = m.rank - k * 8;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (row >= 0 && n > 0) {
+#pragma unroll 2
+        for (int p = 0; p < m.splits; ++p) {
+          const float* from = m.low + (static_cast<long long>(p) * m.tokens + row) * m.rank + k * 8;
+          if (m.rank % 4 == 0 && n >= 8) {
+            const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
+            f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w; f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (e < n) f[e] += from[e];
+          }
+        }
+      }
+      *reinterpret_cast<uint4*>(sl + (k >> 3) * X_SLOT + t * 128 + (((k & 7) ^ (t & 7)) << 4)) =
+          make_uint4(pack_bf16(f[0] * by, f[1] * by), pack_bf16(f[2] * by, f[3] * by), pack_bf16(f[4] * by, f[5] * by), pack_bf16(f[6] * by, f[7] * by));
+    }
+  }
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  volatile int* abort_flag = &bars.abort_flag;
+  const int c0 = blockIdx.y * ADD_COLS, c1 = min(m.out, c0 + ADD_COLS), n_tiles = (c1 - c0 + ADD_N - 1) / ADD_N, steps = n_tiles * kblocks;
+  bool ok = true;
+  if (warp >= 4 && warp < 8) {
+    const int p = tid - 128, c = p & 7;
+    const bf16* b = m.b + static_cast<long long>(tile.adapter) * m.out * m.rank;
+#pragma unroll 1
+    for (int s = 0; s < steps + ADD_STAGES - 1; ++s) {
+      if (s < steps) {
+        const int slot = s % ADD_STAGES, nt = s / kblocks, kb = s - nt * kblocks;
+        ok = ok && wait(&bars.empty[slot], ((s / ADD_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+        const int k = kb * KB + c * 8, left = m.rank - k;
+        const uint32_t bs = smem_u32(sb + slot * B_SLOT) + (p >> 3) * 128 + ((c ^ ((p >> 3) & 7)) << 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = c0 + nt * ADD_N + (p >> 3) + 16 * e;
+          const bool there = n < c1 && left > 0;
+          copy8(bs + e * 2048, there ? b + static_cast<long long>(n) * m.rank + k : m.b, there ? left : 0, m.wide_b);
+        }
+      }
+      copies_end_group();
+      if (s >= ADD_STAGES - 1) {
+        copies_wait<ADD_STAGES - 1>();
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.full[(s - (ADD_STAGES - 1)) % ADD_STAGES]);
+      }
+    }
+  } else if (warp == 8) {
+    constexpr uint32_t idesc = make_idesc(TALL, ADD_N, 1, 1, 0, 0);
+#pragma unroll 1
+    for (int s = 0; s < steps && ok; ++s) {
+      const int slot = s % ADD_STAGES, nt = s / kblocks, kb = s - nt * kblocks, buf = nt & 1;
+      if (kb == 0) ok = wait(&bars.acc_empty[buf], ((nt >> 1) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_TMEM_EMPTY, lane);
+      ok = ok && wait(&bars.full[slot], (s / ADD_STAGES) & 1, abort_flag, m.err, ERR_WAIT_FULL, lane);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t la = smem_u32(sl + kb * X_SLOT), ba = smem_u32(sb + slot * B_SLOT);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; ++kk)
+          umma_bf16_ss(tmem + buf * ADD_N, make_sdesc_sw128(la + kk * 32, 16, 1024), make_sdesc_sw128(ba + kk * 32, 16, 1024), idesc, kb > 0 || kk > 0 ? 1u : 0u);
+        umma_commit(&bars.empty[slot]);
+        if (kb == kblocks - 1) umma_commit(&bars.acc_full[buf]);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int row = bars.rows[tid];
+    bf16* y = m.y + static_cast<long long>(max(row, 0)) * m.out;
+    // y a step of 32 columns ahead of the sums
+    uint4 old[4];
+    auto fetch = [&](int col) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = col + i * 8, left = c1 - at;
+        old[i] = row < 0 || left <= 0 ? make_uint4(0, 0, 0, 0) : m.wide_y ? *reinterpret_cast<const uint4*>(y + at) : load8(y + at, left, false);
+      }
+    };
+    fetch(c0);
+#pragma unroll 1
+    for (int nt = 0; nt < n_tiles && ok; ++nt) {
+      const int buf = nt & 1;
+      ok = wait(&bars.acc_full[buf], (nt >> 1) & 1, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < ADD_N / 32; ++c) {
+        const int col = c0 + nt * ADD_N + c * 32;
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + buf * ADD_N + c * 32, v);
+        uint4 was[4] = {old[0], old[1], old[2], old[3]};
+        fetch(col + 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w[4] = {was[i].x, was[i].y, was[i].z, was[i].w};
+          uint32_t now[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(w[j]) + __uint_as_float(v[i * 8 + 2 * j]), bf16_hi(w[j]) + __uint_as_float(v[i * 8 + 2 * j + 1]));
+          const int left = c1 - (col + i * 8);
+          if (row >= 0 && left > 0) store8(y + col + i * 8, now, left, m.wide_y);
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.acc_empty[buf]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * ADD_N);
+  }
+}
+
+// One CTA: the tokens by adapter, and tiles of up to TALL of them.  (Where a token stands among its adapter's does not change its result.)
+__global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restrict__ ids, int tokens, int adapters, int* __restrict__ order, int* __restrict__ tiles_n,
                                                             Tile* __restrict__ tiles, int* __restrict__ err) {
   extern __shared__ int at[];                    // [adapters]: counts, then where the next token goes
   __shared__ int totals[32][2], carry[2];
+  constexpr int HELD = 8;                        // ids that a thread keeps
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_launch();
+  int held[HELD];
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) held[e] = e * 1024 + tid < tokens ? ids[e * 1024 + tid] : -1;
   for (int i = tid; i < adapters; i += 1024) at[i] = 0;
   if (tid == 0) carry[0] = carry[1] = 0;
   __syncthreads();
-  for (int i0 = 0; i0 < tokens; i0 += 1024) {
-    const int i = i0 + tid, id = i < tokens ? ids[i] : -1;
+  auto each = [&](auto take) {
+#pragma unroll
+    for (int e = 0; e < HELD; ++e)
+      if (e * 1024 < tokens) take(e * 1024 + tid, held[e]);
+#pragma unroll 1
+    for (int i0 = HELD * 1024; i0 < tokens; i0 += 1024) take(i0 + tid, i0 + tid < tokens ? ids[i0 + tid] : -1);
+  };
+  each([&](int, int id) {
     const bool there = id >= 0 && id < adapters;
     if (id >= adapters) atomicCAS(err, 0, static_cast<int>(ERR_BAD_ARG));
-    const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1);
+    const unsigned same = __match_any_sync(FULL, there ? id : -1);
     if (there && lane == __ffs(same) - 1) atomicAdd(&at[id], __popc(same));
-  }
+  });
   __syncthreads();
   for (int i0 = 0; i0 < adapters; i0 += 1024) {
-    const int i = i0 + tid, n = i < adapters ? at[i] : 0, t = (n + tall - 1) / tall;
+    const int i = i0 + tid, n = i < adapters ? at[i] : 0, t = (n + TALL - 1) / TALL;
     int sn = n, st = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int vn = __shfl_up_sync(0xffffffffu, sn, o), vt = __shfl_up_sync(0xffffffffu, st, o);
+      const int vn = __shfl_up_sync(FULL, sn, o), vt = __shfl_up_sync(FULL, st, o);
       if (lane >= o) { sn += vn; st += vt; }
     }
     if (lane == 31) { totals[warp][0] = sn; totals[warp][1] = st; }
@@ -350,24 +645,25 @@ __global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restric
     if (tid == 1023) { carry[0] = bn + sn; carry[1] = bt + st; }
     if (i < adapters) {
       at[i] = bn + sn - n;
-      for (int j = 0; j < t; ++j) tiles[bt + st - t + j] = Tile{i, bn + sn - n + j * tall, min(tall, n - j * tall), 0};
+      for (int j = 0; j < t; ++j) tiles[bt + st - t + j] = Tile{i, bn + sn - n + j * TALL, min(TALL, n - j * TALL), 0};
     }
     __syncthreads();
   }
   if (tid == 0) *tiles_n = carry[1];
-  for (int i0 = 0; i0 < tokens; i0 += 1024) {
-    const int i = i0 + tid, id = i < tokens ? ids[i] : -1;
+  each([&](int i, int id) {
     const bool there = id >= 0 && id < adapters;
-    const unsigned same = __match_any_sync(0xffffffffu, there ? id : -1);
+    const unsigned same = __match_any_sync(FULL, there ? id : -1);
     int base = 0;
     if (there && lane == __ffs(same) - 1) base = atomicAdd(&at[id], __popc(same));
-    base = __shfl_sync(0xffffffffu, base, __ffs(same) - 1);
+    base = __shfl_sync(FULL, base, __ffs(same) - 1);
     if (there) order[base + __popc(same & ((1u << lane) - 1))] = i;
-  }
+  });
 }
 
 template <typename K>
 int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const Mma& m) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -379,24 +675,6 @@ int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream
   cfg.attrs = &early;
   cfg.numAttrs = 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, m));
-}
-
-template <int M16, int WARPS>
-int launch_mma(const Mma& m, int tiles, cudaStream_t stream) {
-  constexpr int MT = 16 * M16;
-  constexpr int sums = WARPS / 2 * MT * RB * 4;
-  const int low = MT * ((m.rank + 31) / 32 * 32 + 8) * 2;
-  cudaError_t e;
-  if ((e = cudaFuncSetAttribute(shrink_mma_kernel<M16, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, sums)) != cudaSuccess) return static_cast<int>(e);
-  if ((e = cudaFuncSetAttribute(expand_mma_kernel<M16>, cudaFuncAttributeMaxDynamicSharedMemorySize, low)) != cudaSuccess) return static_cast<int>(e);
-  const dim3 first(tiles, m.splits, (m.rank + RB - 1) / RB), second(tiles, (m.out + COLS - 1) / COLS);
-  if (m.order != nullptr) {
-    if (int rc = launch_early(shrink_mma_kernel<M16, WARPS>, first, WARPS * 32, sums, stream, m)) return rc;
-  } else {
-    shrink_mma_kernel<M16, WARPS><<<first, WARPS * 32, sums, stream>>>(m);
-    if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
-  }
-  return launch_early(expand_mma_kernel<M16>, second, 128, low, stream, m);
 }
 
 }  // namespace adapters
@@ -422,23 +700,31 @@ extern "C" int dewb_add_adapters(const void* x, long long x_stride, const void* 
   return static_cast<int>(cudaGetLastError());
 }
 
-// The same on the tensor cores: bf16, rank up to 512, up to 4096 adapters, any widths.  Up to 512 tokens: two launches; more: three, and order (tokens integers), then tiles (one
-// integer on a 16-byte boundary, 12 bytes unused, then 16 bytes for each of tokens / 64 + min(adapters, tokens) + 1).
+// The same on the tensor cores: bf16, rank up to 512, up to 4096 adapters, any widths.  Up to 512 tokens: one launch, no scratch.  More: three, and scratch: low (splits x tokens x
+// rank floats), order (tokens integers), tiles (4 integers, then 4 for each of tokens / 128 + min(adapters, tokens) + 1, on a 16-byte boundary).
 extern "C" int dewb_add_adapters_mma(const void* x, long long x_stride, const void* a, const void* b, const float* scale, const int* ids, int* order, void* tiles, float* low, void* y,
                                      int tokens, int adapters, int rank, int width, int out, int splits, int* err, void* stream_ptr) {
   using namespace dewb::adapters;
   if (tokens <= 0 || out <= 0) return 0;
-  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > 512 || width <= 0 || splits < 1 || splits > 65535 || out > 65535 * COLS || (tokens > SCANNED && order == nullptr)) return -3;
+  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > MOST_RANK || width <= 0 || splits < 1 || splits > 65535 || out > 65535 * ADD_COLS) return -3;
   auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   int* n = static_cast<int*>(tiles);
-  Mma m{static_cast<const bf16*>(x), static_cast<const bf16*>(a), static_cast<const bf16*>(b), scale, ids, nullptr, n, reinterpret_cast<const Tile*>(n + 4), low, static_cast<bf16*>(y),
-        x_stride, tokens, adapters, rank, width, out, splits,
-        width % 8 == 0 && x_stride % 8 == 0 && whole(x) && whole(a), rank % 8 == 0 && whole(b), out % 8 == 0 && whole(y), err};
+  const Mma m{static_cast<const bf16*>(x), static_cast<const bf16*>(a), static_cast<const bf16*>(b), scale, ids, order, n, n == nullptr ? nullptr : reinterpret_cast<const Tile*>(n + 4), low,
+              static_cast<bf16*>(y), x_stride, tokens, adapters, rank, width, out, splits,
+              width % 8 == 0 && x_stride % 8 == 0 && whole(x) && whole(a), rank % 8 == 0 && whole(b), out % 8 == 0 && whole(y), err};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  if (tokens <= SCANNED) return launch_mma<1, 4>(m, tokens, stream);
-  group_tokens_kernel<<<1, 1024, adapters * 4, stream>>>(ids, tokens, adapters, 64, order, n, reinterpret_cast<Tile*>(n + 4), err);
+  if (tokens <= SCANNED) {
+    const int wide = (rank + 31) / 32 * 32, smem = 4 * (STEP_WARPS * MT * RB + MT * wide) + 2 * MT * (wide + 8);
+    cudaError_t e = cudaFuncSetAttribute(adapters_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    adapters_step_kernel<<<dim3(CLUSTER, tokens), STEP_THREADS, smem, stream>>>(m);
+    return static_cast<int>(cudaGetLastError());
+  }
+  if (order == nullptr || tiles == nullptr || low == nullptr || !whole(tiles) || !whole(low)) return -3;
+  group_tokens_kernel<<<1, 1024, adapters * 4, stream>>>(ids, tokens, adapters, order, n, reinterpret_cast<Tile*>(n + 4), err);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
-  m.order = order;
-  return launch_mma<4, 4>(m, tokens / 64 + (adapters < tokens ? adapters : tokens) + 1, stream);
+  const int most = tokens / TALL + (adapters < tokens ? adapters : tokens) + 1;
+  if (int rc = launch_early(make_low_kernel, dim3(most, splits, (rank + RB - 1) / RB), 160, MAKE_SMEM, stream, m)) return rc;
+  return launch_early(add_columns_kernel, dim3(most, (out + ADD_COLS - 1) / ADD_COLS), 288, (rank + KB - 1) / KB * X_SLOT + ADD_STAGES * B_SLOT, stream, m);
 }

@@ -23,8 +23,8 @@ def on_tensor_cores(x: torch.Tensor, n: int, rank: int) -> bool:
 
 
 def _splits(tiles: int, rank: int, width: int) -> int:
-    """Parts of the width that are summed apart: enough CTAs for the SMs, each with 128 columns a warp at least."""
-    return max(1, min(16, width // 512, 592 // max(1, tiles * -(-rank // 64))))
+    """Parts of a prompt's width that are summed apart: two CTAs an SM, each with four slots' worth of columns at least."""
+    return max(1, min(8, width // 256, 296 // (tiles * -(-rank // 64))))
 
 
 def _check(x, bank: Bank, ids, out: int, weight_device) -> None:
@@ -75,14 +75,16 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
         if on_tensor_cores(x, n, rank):
             # one piece of scratch a call: the rank's values by parts of the width, the tokens by adapter, their tiles
             grouped = tokens > SCANNED
-            splits = _splits(tokens // 64 + 1 if grouped else min(tokens, n), rank, width)
-            values = -(-splits * tokens * rank // 4) * 4
-            scratch = torch.empty(values + (-(-tokens // 4) * 4 + 4 * (tokens // 64 + min(n, tokens) + 2) if grouped else 0), dtype=torch.float32, device=x.device)
-            at = scratch.data_ptr()
-            order = at + 4 * values if grouped else 0
-            L.check(L.load().dewb_add_adapters_mma(x2.data_ptr(), x2.stride(0), bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), ids.data_ptr(), order,
-                                                   order + -(-tokens // 4) * 16 if grouped else 0, at, y.data_ptr(), tokens, n, rank, width, out, splits, err, stream), "add_adapters_mma")
-            L.count_launches(3 if grouped else 2)
+            splits, order, tiles, scratch = 1, 0, 0, None
+            if grouped:
+                splits = _splits(tokens // 128 + 1, rank, width)
+                values, numbers = -(-splits * tokens * rank // 4) * 4, -(-tokens // 4) * 4
+                scratch = torch.empty(values + numbers + 4 * (tokens // 128 + min(n, tokens) + 2), dtype=torch.float32, device=x.device)
+                order = scratch.data_ptr() + 4 * values
+                tiles = order + 4 * numbers
+            L.check(L.load().dewb_add_adapters_mma(x2.data_ptr(), x2.stride(0), bank.a.data_ptr(), bank.b.data_ptr(), bank.scale.data_ptr(), ids.data_ptr(), order, tiles, L.at(scratch),
+                                                   y.data_ptr(), tokens, n, rank, width, out, splits, err, stream), "add_adapters_mma")
+            L.count_launches(3 if grouped else 1)
             return y
         splits = max(1, min(16, width // 256, 592 // tokens))
         low = torch.empty(splits * tokens * rank, dtype=torch.float32, device=x.device)
