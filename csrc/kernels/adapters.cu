@@ -2,15 +2,17 @@
 //
 // An adapter's tokens are worked on together, so that its A and B come from memory once for all of them.
 //
-// STEPS OF GENERATION, up to 512 tokens: one kernel.  A cluster of eight CTAs takes up to 16 tokens of an adapter: each makes the products with A over an eighth of the width, they
-// add them up through one another's shared memory, and each multiplies with an eighth of B's rows.  Cluster t goes on if token t is the first, 17th, 33rd ... of its adapter, which
+// STEPS OF GENERATION, up to 512 tokens: one kernel.  A cluster of eight CTAs (four, from 33 tokens on) takes up to 16 tokens of an adapter: each makes the products with A over its part
+// of the width, they add them up through one another's shared memory, and each multiplies with its part of B's rows.  Cluster t goes on if token t is the first, 17th, 33rd ... of its adapter, which
 // it finds out by looking through the ids.  Operands go from memory to registers as the warp-level products take them (16 rows are too few for the others): a lane of m16n8k16 holds
 // two pairs of neighbouring elements of a row, and which elements of the sum they are does not matter as long as both operands agree.  So a lane takes eight in a row (16 bytes),
 // four lanes 32, and calls them two products' worth.  B and y are on their way while A's products are added up.  The columns of four n8 blocks are dealt so that a lane's eight
 // are neighbours: y is read and written 16 bytes at a time.  Bound by latency (ids, operands, one cluster barrier, results) and, with many adapters, by reading A and B.
 //
 // PROMPTS: three kernels.  One CTA counts the tokens of each adapter and writes down tiles of up to 128.  Then 128 x 64 x width products, tokens gathered by 16-byte copies, the
-// width in parts; then a CTA a tile and 1024 columns of y: the parts' sum times the scale, rounded to bf16, times B on the tensor cores, added to y.  Bound by x and twice y.
+// width in parts; then the
+// pieces of 128 columns of all tiles, shared evenly by as many CTAs as fit the SMs: the parts' sum times the scale, rounded to bf16, times B on the tensor cores, added to y, whose
+// piece has come to shared memory meanwhile and leaves from there (a row's 256 bytes at a time: with 64, from registers, 62 us instead of @@ for 8192 x 4096).  Bound by x and twice y.
 //
 // The values between the two products are rounded to bf16 after their sum and scale in fp32: what an adapter adds is off by at most half a step of each rank's share.
 #include <cstdint>
@@ -19,6 +21,7 @@
 
 #include "../common/mma_bf16.cuh"
 #include "../common/ptx.cuh"
+#include "../common/tmap.h"
 
 namespace dewb {
 namespace adapters {
@@ -124,7 +127,7 @@ __device__ __forceinline__ void store8(bf16* p, const uint32_t (&w)[4], int n, b
 }
 
 // ---------------------------------------------------------------------------------------------------------- steps of generation
-constexpr int CLUSTER = 8, STEP_WARPS = 4, STEP_THREADS = STEP_WARPS * 32, MT = 16;
+constexpr int STEP_WARPS = 4, STEP_THREADS = STEP_WARPS * 32, MT = 16;
 constexpr int RB = 64;           // rank's values at a time
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
@@ -133,13 +136,15 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return v;
 }
 
-// grid (CLUSTER, tokens)
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __grid_constant__ Mma m) {
+// grid (CLUSTER, tokens), clusters of the CTAs of a token
+template <int CLUSTER>
+__global__ void __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __grid_constant__ Mma m) {
   extern __shared__ __align__(16) float sums[];  // [wide / 8][16][8]: this CTA's share of the rank's values; then as bf16 [16][wide + 8]; in front, the warps' shares
   __shared__ unsigned same[SCANNED / 32];
   __shared__ int rows[MT];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int part = cluster_ctarank(), t0 = blockIdx.y;
+  griddep_wait();
   // the tokens of this one's adapter
   const int mine = m.ids[t0];
 #pragma unroll 1
@@ -168,7 +173,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(STEP_THREADS) 
   const int row0 = rows[g], row1 = rows[g + 8];
   const int wide = (m.rank + 31) / 32 * 32;
   float* share = sums + STEP_WARPS * MT * RB;    // [MT][wide]
-  // ---- x A^T over an eighth of the width
+  // ---- x A^T over this CTA's part of the width
   {
     const int per = ((m.width + CLUSTER - 1) / CLUSTER + 31) / 32 * 32, from = part * per, to = min(m.width, from + per);
     const bf16 *x0 = m.x + max(row0, 0) * m.x_stride, *x1 = m.x + max(row1, 0) * m.x_stride;
@@ -296,9 +301,16 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(STEP_THREADS) 
 // ---------------------------------------------------------------------------------------------------------- prompts
 constexpr int TALL = 128;        // tokens a tile
 constexpr int KB = 64;           // columns of an operand's slot (128 bytes)
-constexpr int MAKE_STAGES = 4, AHEAD = 3;
-constexpr int X_SLOT = TALL * KB * 2, A_SLOT = RB * KB * 2, MAKE_SMEM = MAKE_STAGES * (X_SLOT + A_SLOT) + 1024;
-constexpr int ADD_COLS = 1024, ADD_N = 128, ADD_STAGES = 3, B_SLOT = ADD_N * KB * 2;
+constexpr int MAKE_STAGES = 3, AHEAD = 2;
+constexpr int X_SLOT = TALL * KB * 2, A_SLOT = RB * KB * 2, MAKE_SMEM = MAKE_STAGES * (X_SLOT + A_SLOT);
+constexpr int ADD_N = 128, ADD_STAGES = 2, B_SLOT = ADD_N * KB * 2, Y_SLOT = TALL * ADD_N * 2;
+
+// Four rows of 64 columns (128-byte swizzle), each by its number; rows and columns outside the matrix are zeros.
+__device__ __forceinline__ void tma_gather4(void* to, const CUtensorMap* map, uint64_t* bar, int col, int r0, int r1, int r2, int r3) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(to)),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+               : "memory");
+}
 
 // 16 bytes (8 elements, the first n of which exist) to shared memory, as zeros where there are none
 __device__ __forceinline__ void copy8(uint32_t to, const bf16* p, int n, bool wide) {
@@ -315,10 +327,10 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 struct alignas(16) Bars {
-  uint64_t full[4], empty[4], acc_full[2], acc_empty[2];
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], y_full[2], y_done[2], y_free[2];
   uint32_t tmem;
   int abort_flag, poisoned;
-  int rows[TALL];
+  alignas(16) int rows[TALL];      // (read four at a time)
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code, int lane) {
@@ -327,13 +339,22 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   return false;
 }
 
-// grid (tile, part of the width, 64 of the rank's values); warps 0..3 fetch and write, warp 4 issues products
-__global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ Mma m) {
+// a lane's four rows of a tile (the first one's where there are no more: what comes of those goes nowhere)
+__device__ __forceinline__ int4 four_rows(const int* rows, int lane) {
+  const int4 v = *reinterpret_cast<const int4*>(rows + 4 * lane);
+  return make_int4(v.x < 0 ? rows[0] : v.x, v.y < 0 ? rows[0] : v.y, v.z < 0 ? rows[0] : v.z, v.w < 0 ? rows[0] : v.w);
+}
+
+// grid (tile, part of the width, 64 of the rank's values); warps 0..3 write results, warp 4 issues products, warp 5 fetches tokens (a lane four of them) and A.  Without TMA, for
+// rows that do not begin at 16 bytes, warps 0..3 fetch: each step then waits for all of a thread's copies at the fence between them and the products (33 us instead of @@ for
+// 8192 tokens, 4096 wide).
+template <bool TMA>
+__global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, const __grid_constant__ Mma m) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < MAKE_STAGES; ++i) { mbar_init(&bars.full[i], 4); mbar_init(&bars.empty[i], 1); }
+    for (int i = 0; i < MAKE_STAGES; ++i) { mbar_init(&bars.full[i], TMA ? 1 : 4); mbar_init(&bars.empty[i], 1); }
     mbar_init(&bars.acc_full[0], 1);
     bars.abort_flag = 0;
     fence_barrier_init();
@@ -348,6 +369,7 @@ __global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ M
     if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
     return;
   }
+  if (TMA && warp == 5 && lane == 0) { tma_prefetch_desc(&tx); tma_prefetch_desc(&ta); }
   const Tile tile = m.tiles[blockIdx.x];
   if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
   if (warp == 4) { tmem_alloc(&bars.tmem, 64); tmem_relinquish(); }
@@ -360,7 +382,26 @@ __global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ M
   const int per = ((m.width + m.splits - 1) / m.splits + KB - 1) / KB * KB, from = split * per, to = min(m.width, from + per);
   const int steps = max(0, (to - from + KB - 1) / KB);
   uint8_t *sx = smem, *sa = smem + MAKE_STAGES * X_SLOT;
-  if (warp < 4) {
+  if (TMA && warp == 5) {
+    const int4 four = four_rows(bars.rows, lane);
+    const bool there = 4 * lane < tile.count;
+    const uint32_t bytes = (tile.count + 3) / 4 * 512 + A_SLOT;
+    bool ok = true;
+#pragma unroll 1
+    for (int s = 0; s < steps && ok; ++s) {
+      const int slot = s % MAKE_STAGES;
+      ok = wait(&bars.empty[slot], ((s / MAKE_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(&bars.full[slot], bytes);
+        tma_load_2d(sa + slot * A_SLOT, &ta, &bars.full[slot], from + s * KB, tile.adapter * m.rank + r0);
+      }
+      __syncwarp();
+      if (there) tma_gather4(sx + slot * X_SLOT + lane * 512, &tx, &bars.full[slot], from + s * KB, four.x, four.y, four.z, four.w);
+      __syncwarp();
+    }
+  } else if (warp < 4) {
+   if constexpr (!TMA) {
     const int c = tid & 7;
     const bf16* xr[8];
 #pragma unroll
@@ -393,7 +434,8 @@ __global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ M
         if (lane == 0) mbar_arrive(&bars.full[(s - AHEAD) % MAKE_STAGES]);
       }
     }
-    if (steps > 0) ok = wait(&bars.acc_full[0], 0, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane) && ok;
+   }
+    if (steps > 0) wait(&bars.acc_full[0], 0, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane);
     tc_fence_after();
     const int row = bars.rows[tid];
     float* low = m.low + (static_cast<long long>(split) * m.tokens + max(row, 0)) * m.rank + r0;
@@ -418,7 +460,7 @@ __global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ M
       }
       __syncwarp();
     }
-  } else {
+  } else if (warp == 4) {
     const uint32_t idesc = make_idesc(TALL, 16, 1, 1, 0, 0) + (static_cast<uint32_t>((n16 - 1) * 16 >> 3) << 17);
     bool ok = true;
 #pragma unroll 1
@@ -447,14 +489,19 @@ __global__ void __launch_bounds__(160) make_low_kernel(const __grid_constant__ M
   }
 }
 
-// grid (tile, ADD_COLS columns of y); warps 0..3 add to y, 4..7 fetch B, 8 issues products of 128 tokens and 128 columns
-__global__ void __launch_bounds__(288, 2) add_columns_kernel(const __grid_constant__ Mma m) {
+// Pieces of 128 tokens and 128 columns; warps 0..3 add to y in shared memory, 4..7 put it back, 8 issues products, 9 fetches B and y.  Without TMA (rows that do not begin at 16
+// bytes) warps 4..7 fetch too.
+template <bool TMA>
+__global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap ty, const __grid_constant__ Mma m) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < ADD_STAGES; ++i) { mbar_init(&bars.full[i], 4); mbar_init(&bars.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.full[i], TMA ? 1 : 4); mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4);
+      mbar_init(&bars.y_full[i], TMA ? 1 : 4); mbar_init(&bars.y_done[i], 4); mbar_init(&bars.y_free[i], 4);
+    }
     bars.abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -462,142 +509,206 @@ __global__ void __launch_bounds__(288, 2) add_columns_kernel(const __grid_consta
   }
   griddep_wait();
   __syncthreads();
-  if (bars.poisoned != 0 || static_cast<int>(blockIdx.x) >= *m.tiles_n) return;
+  const int kblocks = (m.rank + KB - 1) / KB, n_tiles = (m.out + ADD_N - 1) / ADD_N;
+  const long long units = static_cast<long long>(*m.tiles_n) * n_tiles, each = (units + gridDim.x - 1) / gridDim.x;
+  const long long u0 = min(units, blockIdx.x * each), u1 = min(units, u0 + each);
+  if (bars.poisoned != 0 || u0 >= u1) return;
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
     return;
   }
-  const Tile tile = m.tiles[blockIdx.x];
-  const int kblocks = (m.rank + KB - 1) / KB;
-  if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
+  if (TMA && warp == 9 && lane == 0) { tma_prefetch_desc(&tb); tma_prefetch_desc(&ty); }
   if (warp == 8) { tmem_alloc(&bars.tmem, 2 * ADD_N); tmem_relinquish(); }
-  uint8_t *sl = smem, *sb = smem + kblocks * X_SLOT;
-  __syncthreads();
-  {
-    // the rank's values: the parts' sum, times the scale, eight a thread
-    const float by = m.scale[tile.adapter];
+  uint8_t *sl = smem, *sb = smem + kblocks * X_SLOT, *sy = sb + ADD_STAGES * B_SLOT;
+  volatile int* abort_flag = &bars.abort_flag;
+  bool ok = true;
+  int piece = 0;                                 // of this CTA's, counted over its tiles
 #pragma unroll 1
-    for (int i = tid; i < TALL * kblocks * 8; i += 288) {
-      const int t = i / (kblocks * 8), k = i - t * kblocks * 8, row = bars.rows[t], n = m.rank - k * 8;
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row >= 0 && n > 0) {
-#pragma unroll 2
-        for (int p = 0; p < m.splits; ++p) {
-          const float* from = m.low + (static_cast<long long>(p) * m.tokens + row) * m.rank + k * 8;
-          if (m.rank % 4 == 0 && n >= 8) {
-            const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
-            f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w; f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
-          } else {
+  for (long long u = u0; u < u1;) {
+    const int at = static_cast<int>(u / n_tiles), first = static_cast<int>(u - static_cast<long long>(at) * n_tiles);
+    const int n = static_cast<int>(min(u1 - u, static_cast<long long>(n_tiles - first))), steps = n * kblocks;
+    u += n;
+    const Tile tile = m.tiles[at];
+    __syncthreads();                             // (the tile before is done with)
+    if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
+    __syncthreads();
+    {
+      // the rank's values: the parts' sum, times the scale, eight a thread
+      const float by = m.scale[tile.adapter];
+#pragma unroll 1
+      for (int i = tid; i < TALL * kblocks * 8; i += 320) {
+        const int t = i / (kblocks * 8), k = i - t * kblocks * 8, row = bars.rows[t], left = m.rank - k * 8;
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (row >= 0 && left > 0) {
+#pragma unroll 4
+          for (int p = 0; p < m.splits; ++p) {
+            const float* from = m.low + (static_cast<long long>(p) * m.tokens + row) * m.rank + k * 8;
+            if (m.rank % 4 == 0 && left >= 8) {
+              const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+              f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) if (e < n) f[e] += from[e];
+              for (int e = 0; e < 8; ++e) if (e < left) f[e] += from[e];
+            }
           }
         }
+        *reinterpret_cast<uint4*>(sl + (k >> 3) * X_SLOT + t * 128 + (((k & 7) ^ (t & 7)) << 4)) =
+            make_uint4(pack_bf16(f[0] * by, f[1] * by), pack_bf16(f[2] * by, f[3] * by), pack_bf16(f[4] * by, f[5] * by), pack_bf16(f[6] * by, f[7] * by));
       }
-      *reinterpret_cast<uint4*>(sl + (k >> 3) * X_SLOT + t * 128 + (((k & 7) ^ (t & 7)) << 4)) =
-          make_uint4(pack_bf16(f[0] * by, f[1] * by), pack_bf16(f[2] * by, f[3] * by), pack_bf16(f[4] * by, f[5] * by), pack_bf16(f[6] * by, f[7] * by));
     }
-  }
-  fence_proxy_async();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = bars.tmem;
-  volatile int* abort_flag = &bars.abort_flag;
-  const int c0 = blockIdx.y * ADD_COLS, c1 = min(m.out, c0 + ADD_COLS), n_tiles = (c1 - c0 + ADD_N - 1) / ADD_N, steps = n_tiles * kblocks;
-  bool ok = true;
-  if (warp >= 4 && warp < 8) {
-    const int p = tid - 128, c = p & 7;
-    const bf16* b = m.b + static_cast<long long>(tile.adapter) * m.out * m.rank;
-#pragma unroll 1
-    for (int s = 0; s < steps + ADD_STAGES - 1; ++s) {
-      if (s < steps) {
-        const int slot = s % ADD_STAGES, nt = s / kblocks, kb = s - nt * kblocks;
-        ok = ok && wait(&bars.empty[slot], ((s / ADD_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
-        const int k = kb * KB + c * 8, left = m.rank - k;
-        const uint32_t bs = smem_u32(sb + slot * B_SLOT) + (p >> 3) * 128 + ((c ^ ((p >> 3) & 7)) << 4);
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem;
+    if (warp >= 4 && warp < 8) {
+      const int p = tid - 128, c = p & 7, yc = p & 15;
+      const bf16* b = m.b + static_cast<long long>(tile.adapter) * m.out * m.rank;
+      // put back piece i (of this tile's)
+      auto put_back = [&](int i) {
+        const int buf = (piece + i) & 1, col = (first + i) * ADD_N + yc * 8, left = m.out - col;
+        ok = ok && wait(&bars.y_done[buf], ((piece + i) >> 1) & 1, abort_flag, m.err, ERR_WAIT_OTHER, lane);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int n = c0 + nt * ADD_N + (p >> 3) + 16 * e;
-          const bool there = n < c1 && left > 0;
-          copy8(bs + e * 2048, there ? b + static_cast<long long>(n) * m.rank + k : m.b, there ? left : 0, m.wide_b);
+        for (int e = 0; e < 16; ++e) {
+          const int t = (p >> 4) + 8 * e, row = bars.rows[t];
+          const uint4 v = *reinterpret_cast<const uint4*>(sy + buf * Y_SLOT + (yc >> 3) * (TALL * 128) + t * 128 + (((yc & 7) ^ (t & 7)) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          if (row >= 0 && left > 0 && ok) store8(m.y + static_cast<long long>(row) * m.out + col, w, left, m.wide_y);
+        }
+      };
+      if constexpr (TMA) {
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          put_back(i);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.y_free[(piece + i) & 1]);
+        }
+      } else {
+        // a slot of B a step (64 of the rank), y's piece with a piece's first; told of when the next one is on its way
+#pragma unroll 1
+        for (int step = 0; step <= steps; ++step) {
+          const int i = step / kblocks, kb = step - i * kblocks;
+          if (step < steps) {
+            if (kb == 0) {
+              if (i >= 2) put_back(i - 2);
+              const int buf = (piece + i) & 1, col = (first + i) * ADD_N + yc * 8, left = m.out - col;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int t = (p >> 4) + 8 * e, row = bars.rows[t];
+                if (row >= 0) copy8(smem_u32(sy + buf * Y_SLOT + (yc >> 3) * (TALL * 128) + t * 128 + (((yc & 7) ^ (t & 7)) << 4)), left > 0 ? m.y + static_cast<long long>(row) * m.out + col : m.y, left, m.wide_y);
+              }
+            }
+            const int s = piece * kblocks + step, slot = s % ADD_STAGES, k = kb * KB + c * 8, k_left = m.rank - k;
+            ok = ok && wait(&bars.empty[slot], ((s / ADD_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+            const uint32_t bs = smem_u32(sb + slot * B_SLOT) + (p >> 3) * 128 + ((c ^ ((p >> 3) & 7)) << 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = (first + i) * ADD_N + (p >> 3) + 16 * e;
+              const bool there = row < m.out && k_left > 0;
+              copy8(bs + e * 2048, there ? b + static_cast<long long>(row) * m.rank + k : m.b, there ? k_left : 0, m.wide_b);
+            }
+          }
+          copies_end_group();
+          if (step == 0) continue;
+          copies_wait<1>();
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            const int before = (step - 1) / kblocks;
+            mbar_arrive(&bars.full[(piece * kblocks + step - 1) % ADD_STAGES]);
+            if ((step - 1) % kblocks == 0) mbar_arrive(&bars.y_full[(piece + before) & 1]);
+          }
+        }
+        if (n >= 2) put_back(n - 2);
+        put_back(n - 1);
+      }
+    } else if (warp == 9) {
+      if constexpr (TMA) {
+        const int4 four = four_rows(bars.rows, lane);
+        const bool there = 4 * lane < tile.count;
+#pragma unroll 1
+        for (int step = 0; step < steps && ok; ++step) {
+          const int i = step / kblocks, kb = step - i * kblocks, s = piece * kblocks + step, slot = s % ADD_STAGES, buf = (piece + i) & 1;
+          if (kb == 0) {
+            ok = wait(&bars.y_free[buf], (((piece + i) >> 1) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+            if (!ok) break;
+            fence_proxy_async();                 // (what threads read and wrote there is behind us)
+            if (lane == 0) mbar_expect_tx(&bars.y_full[buf], (tile.count + 3) / 4 * 1024);
+            __syncwarp();
+            if (there) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                tma_gather4(sy + buf * Y_SLOT + h * (TALL * 128) + lane * 512, &ty, &bars.y_full[buf], (first + i) * ADD_N + h * 64, four.x, four.y, four.z, four.w);
+            }
+            __syncwarp();
+          }
+          ok = wait(&bars.empty[slot], ((s / ADD_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(&bars.full[slot], B_SLOT);
+            tma_load_2d(sb + slot * B_SLOT, &tb, &bars.full[slot], kb * KB, tile.adapter * m.out + (first + i) * ADD_N);
+          }
+          __syncwarp();
         }
       }
-      copies_end_group();
-      if (s >= ADD_STAGES - 1) {
-        copies_wait<ADD_STAGES - 1>();
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.full[(s - (ADD_STAGES - 1)) % ADD_STAGES]);
-      }
-    }
-  } else if (warp == 8) {
-    constexpr uint32_t idesc = make_idesc(TALL, ADD_N, 1, 1, 0, 0);
+    } else if (warp == 8) {
+      constexpr uint32_t idesc = make_idesc(TALL, ADD_N, 1, 1, 0, 0);
 #pragma unroll 1
-    for (int s = 0; s < steps && ok; ++s) {
-      const int slot = s % ADD_STAGES, nt = s / kblocks, kb = s - nt * kblocks, buf = nt & 1;
-      if (kb == 0) ok = wait(&bars.acc_empty[buf], ((nt >> 1) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_TMEM_EMPTY, lane);
-      ok = ok && wait(&bars.full[slot], (s / ADD_STAGES) & 1, abort_flag, m.err, ERR_WAIT_FULL, lane);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t la = smem_u32(sl + kb * X_SLOT), ba = smem_u32(sb + slot * B_SLOT);
-      if (elect_one()) {
+      for (int i = 0; i < steps && ok; ++i) {
+        const int s = piece * kblocks + i, slot = s % ADD_STAGES, nt = i / kblocks, kb = i - nt * kblocks, buf = (piece + nt) & 1;
+        if (kb == 0) ok = wait(&bars.acc_empty[buf], (((piece + nt) >> 1) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_TMEM_EMPTY, lane);
+        ok = ok && wait(&bars.full[slot], (s / ADD_STAGES) & 1, abort_flag, m.err, ERR_WAIT_FULL, lane);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t la = smem_u32(sl + kb * X_SLOT), ba = smem_u32(sb + slot * B_SLOT);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < KB / 16; ++kk)
-          umma_bf16_ss(tmem + buf * ADD_N, make_sdesc_sw128(la + kk * 32, 16, 1024), make_sdesc_sw128(ba + kk * 32, 16, 1024), idesc, kb > 0 || kk > 0 ? 1u : 0u);
-        umma_commit(&bars.empty[slot]);
-        if (kb == kblocks - 1) umma_commit(&bars.acc_full[buf]);
-      }
-      __syncwarp();
-    }
-  } else {
-    const int row = bars.rows[tid];
-    bf16* y = m.y + static_cast<long long>(max(row, 0)) * m.out;
-    // y a step of 32 columns ahead of the sums
-    uint4 old[4];
-    auto fetch = [&](int col) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = col + i * 8, left = c1 - at;
-        old[i] = row < 0 || left <= 0 ? make_uint4(0, 0, 0, 0) : m.wide_y ? *reinterpret_cast<const uint4*>(y + at) : load8(y + at, left, false);
-      }
-    };
-    fetch(c0);
-#pragma unroll 1
-    for (int nt = 0; nt < n_tiles && ok; ++nt) {
-      const int buf = nt & 1;
-      ok = wait(&bars.acc_full[buf], (nt >> 1) & 1, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane);
-      if (!ok) break;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < ADD_N / 32; ++c) {
-        const int col = c0 + nt * ADD_N + c * 32;
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + buf * ADD_N + c * 32, v);
-        uint4 was[4] = {old[0], old[1], old[2], old[3]};
-        fetch(col + 32);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w[4] = {was[i].x, was[i].y, was[i].z, was[i].w};
-          uint32_t now[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(w[j]) + __uint_as_float(v[i * 8 + 2 * j]), bf16_hi(w[j]) + __uint_as_float(v[i * 8 + 2 * j + 1]));
-          const int left = c1 - (col + i * 8);
-          if (row >= 0 && left > 0) store8(y + col + i * 8, now, left, m.wide_y);
+          for (int kk = 0; kk < KB / 16; ++kk)
+            umma_bf16_ss(tmem + buf * ADD_N, make_sdesc_sw128(la + kk * 32, 16, 1024), make_sdesc_sw128(ba + kk * 32, 16, 1024), idesc, kb > 0 || kk > 0 ? 1u : 0u);
+          umma_commit(&bars.empty[slot]);
+          if (kb == kblocks - 1) umma_commit(&bars.acc_full[buf]);
         }
         __syncwarp();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.acc_empty[buf]);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int buf = (piece + i) & 1, phase = ((piece + i) >> 1) & 1;
+        ok = ok && wait(&bars.acc_full[buf], phase, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane) && wait(&bars.y_full[buf], phase, abort_flag, m.err, ERR_WAIT_FULL, lane);
+        tc_fence_after();
+        uint8_t* mine = sy + buf * Y_SLOT + tid * 128;
+#pragma unroll
+        for (int c = 0; c < ADD_N / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + buf * ADD_N + c * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4* y = reinterpret_cast<uint4*>(mine + (c >> 1) * (TALL * 128) + ((((c & 1) * 4 + q) ^ (tid & 7)) << 4));
+            const uint4 was = *y;
+            const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+            uint32_t now[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(w[j]) + __uint_as_float(v[q * 8 + 2 * j]), bf16_hi(w[j]) + __uint_as_float(v[q * 8 + 2 * j + 1]));
+            *y = make_uint4(now[0], now[1], now[2], now[3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars.acc_empty[buf]);
+          mbar_arrive(&bars.y_done[buf]);
+        }
+      }
     }
+    piece += n;
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * ADD_N);
+    tmem_dealloc(bars.tmem, 2 * ADD_N);
   }
 }
 
@@ -660,8 +771,19 @@ __global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restric
   });
 }
 
-template <typename K>
-int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const Mma& m) {
+int multiprocessors() {
+  static int n[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (n[dev] == 0) {
+    int v = 0;
+    n[dev] = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+  }
+  return n[dev];
+}
+
+template <typename K, typename... A>
+int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, int cluster, const A&... args) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
@@ -669,12 +791,15 @@ int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, m));
+  cudaLaunchAttribute with[2] = {};
+  with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  with[0].val.programmaticStreamSerializationAllowed = 1;
+  with[1].id = cudaLaunchAttributeClusterDimension;
+  with[1].val.clusterDim.x = cluster;
+  with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
+  cfg.attrs = with;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 }  // namespace adapters
@@ -706,7 +831,7 @@ extern "C" int dewb_add_adapters_mma(const void* x, long long x_stride, const vo
                                      int tokens, int adapters, int rank, int width, int out, int splits, int* err, void* stream_ptr) {
   using namespace dewb::adapters;
   if (tokens <= 0 || out <= 0) return 0;
-  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > MOST_RANK || width <= 0 || splits < 1 || splits > 65535 || out > 65535 * ADD_COLS) return -3;
+  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > MOST_RANK || width <= 0 || splits < 1 || splits > 65535 ) return -3;
   auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   int* n = static_cast<int*>(tiles);
   const Mma m{static_cast<const bf16*>(x), static_cast<const bf16*>(a), static_cast<const bf16*>(b), scale, ids, order, n, n == nullptr ? nullptr : reinterpret_cast<const Tile*>(n + 4), low,
@@ -715,16 +840,32 @@ extern "C" int dewb_add_adapters_mma(const void* x, long long x_stride, const vo
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   if (tokens <= SCANNED) {
     const int wide = (rank + 31) / 32 * 32, smem = 4 * (STEP_WARPS * MT * RB + MT * wide) + 2 * MT * (wide + 8);
-    cudaError_t e = cudaFuncSetAttribute(adapters_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    adapters_step_kernel<<<dim3(CLUSTER, tokens), STEP_THREADS, smem, stream>>>(m);
-    return static_cast<int>(cudaGetLastError());
+    // (128 tokens of 48 adapters of rank 32, 4096 to 6144: clusters of eight 18 us, of four @@; one token, 1024 to 2048: @@)
+    return tokens <= 32 ? launch_early(adapters_step_kernel<8>, dim3(8, tokens), STEP_THREADS, smem, stream, 8, m) : launch_early(adapters_step_kernel<4>, dim3(4, tokens), STEP_THREADS, smem, stream, 4, m);
   }
   if (order == nullptr || tiles == nullptr || low == nullptr || !whole(tiles) || !whole(low)) return -3;
   group_tokens_kernel<<<1, 1024, adapters * 4, stream>>>(ids, tokens, adapters, order, n, reinterpret_cast<Tile*>(n + 4), err);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return static_cast<int>(e);
   const int most = tokens / TALL + (adapters < tokens ? adapters : tokens) + 1;
-  if (int rc = launch_early(make_low_kernel, dim3(most, splits, (rank + RB - 1) / RB), 160, MAKE_SMEM, stream, m)) return rc;
-  return launch_early(add_columns_kernel, dim3(most, (out + ADD_COLS - 1) / ADD_COLS), 288, (rank + KB - 1) / KB * X_SLOT + ADD_STAGES * B_SLOT, stream, m);
+  CUtensorMap t0 = {}, t1 = {};
+  const uint64_t rows = tokens, ranks = static_cast<uint64_t>(adapters) * rank, outs = static_cast<uint64_t>(adapters) * out;
+  int rc;
+  const dim3 first(most, splits, (rank + RB - 1) / RB);
+  if (m.wide_x) {
+    if ((rc = dewb::make_tmap_2d(&t0, x, rows, width, x_stride, 1, KB, 2, true))) return 1000 + rc;
+    if ((rc = dewb::make_tmap_2d(&t1, a, ranks, width, width, RB, KB, 2, true))) return 2000 + rc;
+    rc = launch_early(make_low_kernel<true>, first, 192, MAKE_SMEM, stream, 1, t0, t1, m);
+  } else {
+    rc = launch_early(make_low_kernel<false>, first, 192, MAKE_SMEM, stream, 1, t0, t1, m);
+  }
+  if (rc) return rc;
+  // two CTAs an SM where their memory fits
+  const int smem = (rank + KB - 1) / KB * X_SLOT + ADD_STAGES * B_SLOT + 2 * Y_SLOT, ctas = multiprocessors() * (2 * (smem + 2048) <= 228 * 1024 ? 2 : 1);
+  if (m.wide_b && m.wide_y && outs < 0x7fffff00ull) {
+    if ((rc = dewb::make_tmap_2d(&t0, b, outs, rank, rank, ADD_N, KB, 2, true))) return 3000 + rc;
+    if ((rc = dewb::make_tmap_2d(&t1, y, rows, out, out, 1, KB, 2, true))) return 4000 + rc;
+    return launch_early(add_columns_kernel<true>, dim3(ctas), 320, smem, stream, 1, t0, t1, m);
+  }
+  return launch_early(add_columns_kernel<false>, dim3(ctas), 320, smem, stream, 1, t0, t1, m);
 }

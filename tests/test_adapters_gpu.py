@@ -41,6 +41,22 @@ def test_prompts(tokens, used, runs, without):
     check(batch(tokens, 64, 32, 512, 768, BF16, device=DEV, used=used, runs=runs, without=without))
 
 
+@pytest.mark.parametrize("n, rank, width, out", [(3, 8, 72, 136), (5, 5, 200, 1000), (2, 13, 520, 72), (40, 72, 136, 264), (2, 200, 264, 392), (4, 16, 33, 17), (3, 24, 64, 130), (600, 4, 128, 128)])
+@pytest.mark.parametrize("tokens, runs", [(513, True), (900, False)])
+def test_prompts_of_odd_sizes(n, rank, width, out, tokens, runs):
+    check(batch(tokens, n, rank, width, out, BF16, device=DEV, runs=runs))
+
+
+def test_prompts_of_one_token_each_and_of_one_adapter():
+    a = batch(700, 700, 8, 64, 128, BF16, device=DEV, without=0.0)
+    a["ids"] = torch.randperm(700, device=DEV, dtype=torch.int32)
+    for t in a["bank"]:
+        t.copy_(torch.randn_like(t) * 0.3)
+    check(a)
+    check({**a, "ids": torch.full_like(a["ids"], 5)})
+    check({**a, "ids": torch.where(torch.arange(700, device=DEV) == 650, 3, -1).to(torch.int32)})
+
+
 def test_layouts_bias_and_streams():
     a = batch(96, 5, 16, 256, 384, BF16, device=DEV)
     bias = torch.randn(384, device=DEV).to(BF16)
