@@ -2,19 +2,21 @@
 //
 // An adapter's tokens are worked on together, so that its A and B come from memory once for all of them.
 //
-// STEPS OF GENERATION, up to 512 tokens: one kernel.  A cluster of eight CTAs (four, from 33 tokens on) takes up to 16 tokens of an adapter: each makes the products with A over its part
-// of the width, they add them up through one another's shared memory, and each multiplies with its part of B's rows.  Cluster t goes on if token t is the first, 17th, 33rd ... of its adapter, which
-// it finds out by looking through the ids.  Operands go from memory to registers as the warp-level products take them (16 rows are too few for the others): a lane of m16n8k16 holds
+// STEPS OF GENERATION, up to 512 tokens: one kernel.  A cluster of eight CTAs takes up to 16 tokens of an adapter: each makes the products with A over its part
+// of the width, they add them up through one another's shared memory, and each multiplies with its part of B's rows.  Cluster t takes the t-th such tile in the order of their first
+// tokens, which it finds out by looking through the ids.  Operands go from memory to registers as the warp-level products take them (16 rows are too few for the others): a lane of m16n8k16 holds
 // two pairs of neighbouring elements of a row, and which elements of the sum they are does not matter as long as both operands agree.  So a lane takes eight in a row (16 bytes),
 // four lanes 32, and calls them two products' worth.  B and y are on their way while A's products are added up.  The columns of four n8 blocks are dealt so that a lane's eight
 // are neighbours: y is read and written 16 bytes at a time.  Bound by latency (ids, operands, one cluster barrier, results) and, with many adapters, by reading A and B.
 //
-// PROMPTS: three kernels.  One CTA counts the tokens of each adapter and writes down tiles of up to 128.  Then 128 x 64 x width products, tokens gathered by 16-byte copies, the
-// width in parts; then the
-// pieces of 128 columns of all tiles, shared evenly by as many CTAs as fit the SMs: the parts' sum times the scale, rounded to bf16, times B on the tensor cores, added to y, whose
-// piece has come to shared memory meanwhile and leaves from there (a row's 256 bytes at a time: with 64, from registers, 62 us instead of @@ for 8192 x 4096).  Bound by x and twice y.
+// PROMPTS: three kernels.  One CTA puts the tokens in the order of their adapters and writes down tiles of up to 128.  Then 128 x 64 x width products on the tensor cores; tokens
+// come by TMA, as a block where a tile's are neighbours, else four at a time by their numbers.  A tile's width is shared out over a cluster, whose CTAs add up through one another's
+// shared memory and write the rank's values, times the scale, in bf16 and in the tiles' order: the second product's operand as it stands.  Then pieces of 128 columns of all tiles,
+// shared evenly by as many CTAs as fit the SMs: times B on the tensor cores, added to y, whose piece has come to shared memory meanwhile and leaves from there.
+// Bound by x and twice y, and by the latencies of three kernels.
 //
 // The values between the two products are rounded to bf16 after their sum and scale in fp32: what an adapter adds is off by at most half a step of each rank's share.
+#include <algorithm>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -85,7 +87,8 @@ __global__ void __launch_bounds__(128) expand_kernel(const __grid_constant__ Arg
 // ---------------------------------------------------------------------------------------------------------- bf16
 using bf16 = __nv_bfloat16;
 constexpr int SCANNED = 512;     // tokens whose ids each CTA looks through
-constexpr int MOST_ADAPTERS = 4096, MOST_RANK = 512;
+constexpr int MOST_ADAPTERS = 3500,            // (16 counts each fit a CTA's shared memory)
+              MOST_RANK = 512;
 constexpr uint32_t FULL = 0xffffffffu;
 
 struct Tile { int adapter, begin, count, pad; };
@@ -96,10 +99,10 @@ struct Mma {
   const int* ids;
   const int *order, *tiles_n;    // prompts: the tokens by adapter, and their tiles
   const Tile* tiles;
-  float* low;                    // prompts: [splits, tokens, rank]
+  bf16* low;                     // prompts: [tokens, wide], an adapter's tokens together: the rank's values times the scale, zeros behind them
   bf16* y;
   long long x_stride;
-  int tokens, adapters, rank, width, out, splits;
+  int tokens, adapters, rank, width, out, splits, wide;
   bool wide_x, wide_b, wide_y;   // whether rows of x and a, of b, of y can be taken 16 bytes at a time
   int* err;
 };
@@ -127,47 +130,87 @@ __device__ __forceinline__ void store8(bf16* p, const uint32_t (&w)[4], int n, b
 }
 
 // ---------------------------------------------------------------------------------------------------------- steps of generation
-constexpr int STEP_WARPS = 4, STEP_THREADS = STEP_WARPS * 32, MT = 16;
-constexpr int RB = 64;           // rank's values at a time
+constexpr int CLUSTER = 8, STEP_WARPS = 4, STEP_THREADS = STEP_WARPS * 32, MT = 16;
+constexpr int RB = 64;           // rank's values at a time (steps: 32 where there are no more)
 
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 
-// grid (CLUSTER, tokens), clusters of the CTAs of a token
-template <int CLUSTER>
-__global__ void __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __grid_constant__ Mma m) {
+// grid (CLUSTER, as many tiles as there can be)
+template <int CLUSTER, int RB>
+__global__ void __launch_bounds__(STEP_THREADS, 4) adapters_step_kernel(const __grid_constant__ Mma m) {
   extern __shared__ __align__(16) float sums[];  // [wide / 8][16][8]: this CTA's share of the rank's values; then as bf16 [16][wide + 8]; in front, the warps' shares
-  __shared__ unsigned same[SCANNED / 32];
+  __shared__ unsigned first[SCANNED / 32];
+  __shared__ int adapter_at[2];                  // the tile's adapter, and how many of its tokens come before
   __shared__ int rows[MT];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int part = cluster_ctarank(), t0 = blockIdx.y;
+  const int part = cluster_ctarank(), tile = blockIdx.y;
   griddep_wait();
-  // the tokens of this one's adapter
-  const int mine = m.ids[t0];
-#pragma unroll 1
-  for (int i0 = warp * 32; i0 < m.tokens; i0 += STEP_THREADS) {
-    const unsigned w = __ballot_sync(FULL, i0 + lane < m.tokens && m.ids[i0 + lane] == mine);
-    if (lane == 0) same[i0 >> 5] = w;
+  // which tokens begin a tile: those with no token of their adapter before them, or 16, 32, ... of them.  A warp counts a quarter of the tokens by adapter
+  constexpr int HELD = SCANNED / STEP_THREADS;
+  unsigned short* counts = reinterpret_cast<unsigned short*>(sums);                  // [adapters][STEP_WARPS], those of adapters that occur
+  const int quarter = (m.tokens + STEP_THREADS - 1) / STEP_THREADS * 32, from_token = warp * quarter;
+  int id[HELD], before[HELD];
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    const int i = from_token + e * 32 + lane;
+    id[e] = e * 32 < quarter && i < m.tokens ? m.ids[i] : -1;
+    if (id[e] >= m.adapters) {
+      if (tile == 0 && part == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+      id[e] = -1;
+    }
+    if (id[e] >= 0) *reinterpret_cast<uint2*>(counts + STEP_WARPS * id[e]) = make_uint2(0, 0);
   }
-  if (mine >= m.adapters && tid == 0 && part == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
   if (tid < MT) rows[tid] = -1;
   __syncthreads();
-  if (mine < 0 || mine >= m.adapters) return;
-  int before = 0;
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    if (e * 32 >= quarter) break;
+    const unsigned same = __match_any_sync(FULL, id[e]);
+    const int mine_at = STEP_WARPS * id[e] + warp, so_far = id[e] >= 0 ? counts[mine_at] : 0;
+    before[e] = so_far + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (id[e] >= 0 && lane == __ffs(same) - 1) counts[mine_at] = static_cast<unsigned short>(so_far + __popc(same));
+    __syncwarp();
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    if (e * 32 >= quarter) break;
+    if (id[e] >= 0)
+#pragma unroll
+      for (int w = 0; w < STEP_WARPS - 1; ++w) before[e] += w < warp ? counts[STEP_WARPS * id[e] + w] : 0;
+    const unsigned begin = __ballot_sync(FULL, id[e] >= 0 && before[e] % MT == 0);
+    if (lane == 0) first[from_token / 32 + e] = begin;
+  }
+  __syncthreads();
+  // this cluster's: the tile that begins with the `tile`-th of them
+  const int blocks_of_32 = STEP_WARPS * (quarter / 32);
+  int w32 = 0, left_of = tile;
 #pragma unroll 1
-  for (int w = 0; w < t0 >> 5; ++w) before += __popc(same[w]);
-  before += __popc(same[t0 >> 5] & ((1u << (t0 & 31)) - 1));
-  if (before % MT != 0) return;                  // (all CTAs of a cluster, or none)
+  while (w32 < blocks_of_32 && left_of >= __popc(first[w32])) left_of -= __popc(first[w32++]);
+  if (w32 >= blocks_of_32) return;               // (all CTAs of a cluster, or none)
+  unsigned begin = first[w32];
 #pragma unroll 1
-  for (int i = tid; i < m.tokens; i += STEP_THREADS) {
-    if (i < t0 || !(same[i >> 5] >> (i & 31) & 1)) continue;
-    int rank_of = __popc(same[i >> 5] & ((1u << (i & 31)) - 1)) - before;
-#pragma unroll 1
-    for (int w = 0; w < i >> 5; ++w) rank_of += __popc(same[w]);
-    if (rank_of < MT) rows[rank_of] = i;
+  for (; left_of > 0; --left_of) begin &= begin - 1;
+#pragma unroll
+  for (int e = 0; e < HELD; ++e)
+    if (e * 32 < quarter && from_token + e * 32 + lane == w32 * 32 + __ffs(begin) - 1) { adapter_at[0] = id[e]; adapter_at[1] = before[e]; }
+  __syncthreads();
+  const int mine = adapter_at[0];
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) {
+    const int n = before[e] - adapter_at[1];
+    if (e * 32 < quarter && id[e] == mine && n >= 0 && n < MT) rows[n] = from_token + e * 32 + lane;
   }
   __syncthreads();
   const int row0 = rows[g], row1 = rows[g + 8];
@@ -186,20 +229,29 @@ __global__ void __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __gri
       for (int n = 0; n < RB / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-#pragma unroll 2
-      for (int k0 = from + warp * 32; k0 < to; k0 += STEP_WARPS * 32) {
-        const int k = k0 + c * 8, left = to - k;
-        const uint4 lo = row0 < 0 ? make_uint4(0, 0, 0, 0) : load8(x0 + k, left, m.wide_x), hi = row1 < 0 ? make_uint4(0, 0, 0, 0) : load8(x1 + k, left, m.wide_x);
-        const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
-        uint4 av[RB / 8];
+      // (as many operands on their way as there are registers for: 128 columns of 32 ranks, 64 of 64)
+      constexpr int DEEP = 128 / RB;
+#pragma unroll 1
+      for (int k0 = from + warp * 32; k0 < to; k0 += STEP_WARPS * 32 * DEEP) {
+        uint4 lo[DEEP], hi[DEEP], av[DEEP][RB / 8];
 #pragma unroll
-        for (int n = 0; n < RB / 8; ++n)
-          av[n] = n < blocks && r0 + n * 8 + g < m.rank ? load8(ar + static_cast<long long>(n) * 8 * m.width + k, left, m.wide_x) : make_uint4(0, 0, 0, 0);
+        for (int d = 0; d < DEEP; ++d) {
+          const int k = k0 + d * STEP_WARPS * 32 + c * 8, left = to - k;
+          lo[d] = row0 < 0 ? make_uint4(0, 0, 0, 0) : load8(x0 + k, left, m.wide_x);
+          hi[d] = row1 < 0 ? make_uint4(0, 0, 0, 0) : load8(x1 + k, left, m.wide_x);
 #pragma unroll
-        for (int n = 0; n < RB / 8; ++n) {
-          if (n >= blocks) break;
-          mma16::mma(acc[n], one, av[n].x, av[n].y);
-          mma16::mma(acc[n], two, av[n].z, av[n].w);
+          for (int n = 0; n < RB / 8; ++n)
+            av[d][n] = n < blocks && r0 + n * 8 + g < m.rank ? load8(ar + static_cast<long long>(n) * 8 * m.width + k, left, m.wide_x) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+          const uint32_t one[4] = {lo[d].x, hi[d].x, lo[d].y, hi[d].y}, two[4] = {lo[d].z, hi[d].z, lo[d].w, hi[d].w};
+#pragma unroll
+          for (int n = 0; n < RB / 8; ++n) {
+            if (n >= blocks) break;
+            mma16::mma(acc[n], one, av[d][n].x, av[d][n].y);
+            mma16::mma(acc[n], two, av[d][n].z, av[d][n].w);
+          }
         }
       }
 #pragma unroll
@@ -223,29 +275,31 @@ __global__ void __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __gri
     }
   }
   cluster_arrive();
-  // ---- meanwhile, this warp's first columns of B and y are fetched
-  const int per = ((m.out + CLUSTER - 1) / CLUSTER + 31) / 32 * 32, n_end = min(m.out, (part + 1) * per);
+  // ---- meanwhile, this warp's first columns of B and y are fetched: PIECES of 32 of the rank for 32 columns, in the order of their use
+  constexpr int PIECES = 3;
+  const int per = ((m.out + CLUSTER - 1) / CLUSTER + 31) / 32 * 32, n_end = min(m.out, (part + 1) * per), n_first = part * per + warp * 32;
+  const int kblocks = wide / 32, pieces = n_first < n_end ? (n_end - n_first + STEP_THREADS - 1) / STEP_THREADS * kblocks : 0;
   const bf16* b = m.b + static_cast<long long>(mine) * m.out * m.rank;
-  uint4 bv[4], old[2];
-  auto fetch_b = [&](int n0, int k) {
+  uint4 bv[PIECES][4], old[PIECES][2];
+  auto fetch = [&](int i, uint4 (&bp)[4], uint4 (&yp)[2]) {
+    if (i >= pieces) return;
+    const int nt = i / kblocks, kb = i - nt * kblocks, n0 = n_first + nt * STEP_THREADS, k = kb * 32 + c * 8;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = n0 + (g >> 1) * 8 + j * 2 + (g & 1);             // block j's column g
-      bv[j] = n < n_end ? load8(b + static_cast<long long>(n) * m.rank + k, m.rank - k, m.wide_b) : make_uint4(0, 0, 0, 0);
+      bp[j] = n < n_end ? load8(b + static_cast<long long>(n) * m.rank + k, m.rank - k, m.wide_b) : make_uint4(0, 0, 0, 0);
+    }
+    if (kb != 0) return;
+    const int col = n0 + c * 8, left = m.out - col;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = h == 0 ? row0 : row1;
+      const bf16* p = m.y + static_cast<long long>(max(row, 0)) * m.out + col;
+      yp[h] = row < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(p) : load8(p, left, false);
     }
   };
-  auto fetch_y = [&](int n0) {
-    const int col = n0 + c * 8, left = m.out - col;
-    old[0] = row0 < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(m.y + static_cast<long long>(row0) * m.out + col)
-                                                                        : load8(m.y + static_cast<long long>(row0) * m.out + col, left, false);
-    old[1] = row1 < 0 ? make_uint4(0, 0, 0, 0) : m.wide_y && left >= 8 ? *reinterpret_cast<const uint4*>(m.y + static_cast<long long>(row1) * m.out + col)
-                                                                        : load8(m.y + static_cast<long long>(row1) * m.out + col, left, false);
-  };
-  int n0 = part * per + warp * 32;
-  if (n0 < n_end) {
-    fetch_b(n0, c * 8);
-    fetch_y(n0);
-  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) fetch(i, bv[i], old[i]);
   const float by = m.scale[mine];
   cluster_wait();
   // ---- the CTAs' shares, their sum times the scale to bf16 (behind the shares)
@@ -264,36 +318,39 @@ __global__ void __launch_bounds__(STEP_THREADS) adapters_step_kernel(const __gri
   }
   cluster_arrive();                              // (its share is read by others until here)
   __syncthreads();
+  float acc[4][4];
 #pragma unroll 1
-  for (; n0 < n_end; n0 += STEP_THREADS) {
-    float acc[4][4];
+  for (int i0 = 0; i0 < pieces; i0 += PIECES) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int p = 0; p < PIECES; ++p) {
+      const int i = i0 + p;
+      if (i >= pieces) break;
+      const int nt = i / kblocks, kb = i - nt * kblocks;
+      if (kb == 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-#pragma unroll 1
-    for (int k0 = 0; k0 < m.rank; k0 += 32) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(low + g * pitch + k0 + c * 8), hi = *reinterpret_cast<const uint4*>(low + (8 + g) * pitch + k0 + c * 8);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] = e & 1 ? bf16_hi(word(old[p][e >> 1], j)) : bf16_lo(word(old[p][e >> 1], j));
+      }
+      const uint4 lo = *reinterpret_cast<const uint4*>(low + g * pitch + kb * 32 + c * 8), hi = *reinterpret_cast<const uint4*>(low + (8 + g) * pitch + kb * 32 + c * 8);
       const uint32_t one[4] = {lo.x, hi.x, lo.y, hi.y}, two[4] = {lo.z, hi.z, lo.w, hi.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        mma16::mma(acc[j], one, bv[j].x, bv[j].y);
-        mma16::mma(acc[j], two, bv[j].z, bv[j].w);
+        mma16::mma(acc[j], one, bv[p][j].x, bv[p][j].y);
+        mma16::mma(acc[j], two, bv[p][j].z, bv[p][j].w);
       }
-      const bool same_columns = k0 + 32 < m.rank;
-      if (same_columns || n0 + STEP_THREADS < n_end) fetch_b(same_columns ? n0 : n0 + STEP_THREADS, (same_columns ? k0 + 32 : 0) + c * 8);
-    }
-    const int col = n0 + c * 8, left = m.out - col;
+      fetch(i + PIECES, bv[p], old[p]);
+      if (kb != kblocks - 1) continue;
+      const int col = n_first + nt * STEP_THREADS + c * 8, left = m.out - col;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = i == 0 ? row0 : row1;
-      const uint32_t was[4] = {old[i].x, old[i].y, old[i].z, old[i].w};
-      uint32_t now[4];
+      for (int h = 0; h < 2; ++h) {
+        const int row = h == 0 ? row0 : row1;
+        uint32_t now[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) now[j] = pack_bf16(bf16_lo(was[j]) + acc[j][2 * i], bf16_hi(was[j]) + acc[j][2 * i + 1]);
-      if (row >= 0 && left > 0) store8(m.y + static_cast<long long>(row) * m.out + col, now, left, m.wide_y);
+        for (int j = 0; j < 4; ++j) now[j] = pack_bf16(acc[j][2 * h], acc[j][2 * h + 1]);
+        if (row >= 0 && left > 0) store8(m.y + static_cast<long long>(row) * m.out + col, now, left, m.wide_y);
+      }
     }
-    if (n0 + STEP_THREADS < n_end) fetch_y(n0 + STEP_THREADS);
   }
   cluster_wait();                                // (no CTA's memory goes while another reads it)
 }
@@ -303,6 +360,8 @@ constexpr int TALL = 128;        // tokens a tile
 constexpr int KB = 64;           // columns of an operand's slot (128 bytes)
 constexpr int MAKE_STAGES = 3, AHEAD = 2;
 constexpr int X_SLOT = TALL * KB * 2, A_SLOT = RB * KB * 2, MAKE_SMEM = MAKE_STAGES * (X_SLOT + A_SLOT);
+constexpr int LOW_PITCH = RB + 4;                // floats of a token's row in shared memory
+static_assert(TALL * LOW_PITCH * 4 <= MAKE_SMEM, "the values lie where the operands were");
 constexpr int ADD_N = 128, ADD_STAGES = 2, B_SLOT = ADD_N * KB * 2, Y_SLOT = TALL * ADD_N * 2;
 
 // Four rows of 64 columns (128-byte swizzle), each by its number; rows and columns outside the matrix are zeros.
@@ -327,7 +386,7 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 struct alignas(16) Bars {
-  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], y_full[2], y_done[2], y_free[2];
+  uint64_t full[4], empty[4], acc_full[2], acc_empty[2], y_full[2], y_done[2], y_free[2], low_full;
   uint32_t tmem;
   int abort_flag, poisoned;
   alignas(16) int rows[TALL];      // (read four at a time)
@@ -339,6 +398,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   return false;
 }
 
+// whether a tile's tokens are neighbours (all threads)
+__device__ __forceinline__ bool neighbours(const int* rows, int count, int tid) { return __syncthreads_and(tid >= count || rows[tid] == rows[0] + tid) != 0; }
+
 // a lane's four rows of a tile (the first one's where there are no more: what comes of those goes nowhere)
 __device__ __forceinline__ int4 four_rows(const int* rows, int lane) {
   const int4 v = *reinterpret_cast<const int4*>(rows + 4 * lane);
@@ -346,10 +408,9 @@ __device__ __forceinline__ int4 four_rows(const int* rows, int lane) {
 }
 
 // grid (tile, part of the width, 64 of the rank's values); warps 0..3 write results, warp 4 issues products, warp 5 fetches tokens (a lane four of them) and A.  Without TMA, for
-// rows that do not begin at 16 bytes, warps 0..3 fetch: each step then waits for all of a thread's copies at the fence between them and the products (33 us instead of @@ for
-// 8192 tokens, 4096 wide).
+// rows that do not begin at 16 bytes, warps 0..3 fetch: each step then waits for all of a thread's copies at the fence between them and the products.
 template <bool TMA>
-__global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap ta, const __grid_constant__ Mma m) {
+__global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tx_block, const __grid_constant__ CUtensorMap ta, const __grid_constant__ Mma m) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -359,23 +420,23 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
     bars.abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
-    bars.poisoned = *reinterpret_cast<volatile int*>(m.err);
   }
-  griddep_launch();
   griddep_wait();                                // (the tiles are the kernel's before this)
+  griddep_launch();                              // (and of use to the next one from here on)
   __syncthreads();
-  if (bars.poisoned != 0 || static_cast<int>(blockIdx.x) >= *m.tiles_n) return;
+  if (static_cast<int>(blockIdx.x) >= *m.tiles_n) return;        // (all CTAs of a cluster, or none)
   if ((smem_u32(smem) & 1023u) != 0) {
     if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
     return;
   }
-  if (TMA && warp == 5 && lane == 0) { tma_prefetch_desc(&tx); tma_prefetch_desc(&ta); }
+  if (TMA && warp == 5 && lane == 0) { tma_prefetch_desc(&tx); tma_prefetch_desc(&tx_block); tma_prefetch_desc(&ta); }
   const Tile tile = m.tiles[blockIdx.x];
   if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
   if (warp == 4) { tmem_alloc(&bars.tmem, 64); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const bool block = TMA && neighbours(bars.rows, tile.count, tid);
   const uint32_t tmem = bars.tmem;
   volatile int* abort_flag = &bars.abort_flag;
   const int split = blockIdx.y, r0 = blockIdx.z * RB, ranks = min(RB, m.rank - r0), n16 = (ranks + 15) / 16;
@@ -385,7 +446,7 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
   if (TMA && warp == 5) {
     const int4 four = four_rows(bars.rows, lane);
     const bool there = 4 * lane < tile.count;
-    const uint32_t bytes = (tile.count + 3) / 4 * 512 + A_SLOT;
+    const uint32_t bytes = (block ? X_SLOT : (tile.count + 3) / 4 * 512) + A_SLOT;
     bool ok = true;
 #pragma unroll 1
     for (int s = 0; s < steps && ok; ++s) {
@@ -395,9 +456,10 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
       if (lane == 0) {
         mbar_expect_tx(&bars.full[slot], bytes);
         tma_load_2d(sa + slot * A_SLOT, &ta, &bars.full[slot], from + s * KB, tile.adapter * m.rank + r0);
+        if (block) tma_load_2d(sx + slot * X_SLOT, &tx_block, &bars.full[slot], from + s * KB, bars.rows[0]);
       }
       __syncwarp();
-      if (there) tma_gather4(sx + slot * X_SLOT + lane * 512, &tx, &bars.full[slot], from + s * KB, four.x, four.y, four.z, four.w);
+      if (there && !block) tma_gather4(sx + slot * X_SLOT + lane * 512, &tx, &bars.full[slot], from + s * KB, four.x, four.y, four.z, four.w);
       __syncwarp();
     }
   } else if (warp < 4) {
@@ -437,28 +499,16 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
    }
     if (steps > 0) wait(&bars.acc_full[0], 0, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane);
     tc_fence_after();
-    const int row = bars.rows[tid];
-    float* low = m.low + (static_cast<long long>(split) * m.tokens + max(row, 0)) * m.rank + r0;
+    // this part's values to shared memory, where the operands were
+    float* mine = reinterpret_cast<float*>(smem) + tid * LOW_PITCH;
 #pragma unroll 1
     for (int c16 = 0; c16 < n16; ++c16) {
       uint32_t v[16];
       tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c16 * 16, v);
       tmem_ld_wait();
-      if (row >= 0) {
-        if (steps == 0)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = 0;
-        if (m.rank % 4 == 0 && c16 * 16 + 16 <= ranks) {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<uint4*>(low + c16 * 16 + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c16 * 16 + i < ranks) low[c16 * 16 + i] = __uint_as_float(v[i]);
-        }
-      }
-      __syncwarp();
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<uint4*>(mine + c16 * 16 + i) = steps == 0 ? make_uint4(0, 0, 0, 0) : make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
   } else if (warp == 4) {
     const uint32_t idesc = make_idesc(TALL, 16, 1, 1, 0, 0) + (static_cast<uint32_t>((n16 - 1) * 16 >> 3) << 17);
@@ -487,12 +537,43 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
     tc_fence_after();
     tmem_dealloc(tmem, 64);
   }
+  // ---- each CTA adds up its share of the tokens: eight of the rank's values a thread, times the scale, to bf16
+  cluster_arrive();
+  cluster_wait();
+  const float by = m.scale[tile.adapter];
+  const uint32_t at = smem_u32(smem);
+  const int share = TALL / m.splits, end = min(tile.count, (split + 1) * share), columns = min(RB, m.wide - r0) / 8;
+#pragma unroll 1
+  for (int i = tid; i < share * columns; i += 192) {
+    const int t = split * share + i / columns, k = i % columns * 8;
+    if (t >= end) break;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k < n16 * 16) {
+#pragma unroll 4
+      for (int p = 0; p < m.splits; ++p) {
+        const uint32_t from_cta = map_to_cta(at + (t * LOW_PITCH + k) * 4, p);
+        const float4 u = ld_cluster4(from_cta), v = ld_cluster4(from_cta + 16);
+        f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w; f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = k + e < ranks ? f[e] * by : 0.f;
+    *reinterpret_cast<uint4*>(m.low + static_cast<long long>(tile.begin + t) * m.wide + r0 + k) =
+        make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  }
+  cluster_arrive();                              // (no CTA's memory goes while another reads it)
+  cluster_wait();
 }
 
-// Pieces of 128 tokens and 128 columns; warps 0..3 add to y in shared memory, 4..7 put it back, 8 issues products, 9 fetches B and y.  Without TMA (rows that do not begin at 16
-// bytes) warps 4..7 fetch too.
+// Told of when this thread's copies have come.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+
+// Pieces of 128 tokens and 128 columns; warps 0..3 add to y in shared memory, 4..7 put it back (one thread each half, where a tile is a block), 8 issues products, 9 fetches the
+// rank's values, B and y: a tile of neighbours as a block, else four rows at a time.  (Fetched by the threads that put it back, 16 bytes each: 144 us instead of 90 for 8192 tokens
+// and 8192 columns.)  Without TMA (rows of B or y that do not begin at 16 bytes) warps 4..7 fetch both.
 template <bool TMA>
-__global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap ty, const __grid_constant__ Mma m) {
+__global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_constant__ CUtensorMap tl, const __grid_constant__ CUtensorMap tb, const __grid_constant__ CUtensorMap ty,
+                                                             const __grid_constant__ CUtensorMap ty_block, const __grid_constant__ Mma m) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -500,71 +581,59 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.full[i], TMA ? 1 : 4); mbar_init(&bars.empty[i], 1);
       mbar_init(&bars.acc_full[i], 1); mbar_init(&bars.acc_empty[i], 4);
-      mbar_init(&bars.y_full[i], TMA ? 1 : 4); mbar_init(&bars.y_done[i], 4); mbar_init(&bars.y_free[i], 4);
+      mbar_init(&bars.y_full[i], TMA ? 1 : 128); mbar_init(&bars.y_done[i], 4); mbar_init(&bars.y_free[i], 4);
     }
+    mbar_init(&bars.low_full, 1);
     bars.abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
     bars.poisoned = *reinterpret_cast<volatile int*>(m.err);
   }
-  griddep_wait();
-  __syncthreads();
-  const int kblocks = (m.rank + KB - 1) / KB, n_tiles = (m.out + ADD_N - 1) / ADD_N;
-  const long long units = static_cast<long long>(*m.tiles_n) * n_tiles, each = (units + gridDim.x - 1) / gridDim.x;
+  // (the tiles are complete when this kernel may begin; the rank's values, and y, after the wait)
+  const int kblocks = m.wide / KB, n_tiles = (m.out + ADD_N - 1) / ADD_N;
+  const long long units = static_cast<long long>(__ldcg(m.tiles_n)) * n_tiles, each = (units + gridDim.x - 1) / gridDim.x;
   const long long u0 = min(units, blockIdx.x * each), u1 = min(units, u0 + each);
-  if (bars.poisoned != 0 || u0 >= u1) return;
-  if ((smem_u32(smem) & 1023u) != 0) {
-    if (tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+  __syncthreads();
+  if (bars.poisoned != 0 || u0 >= u1 || (smem_u32(smem) & 1023u) != 0) {
+    if (u0 < u1 && bars.poisoned == 0 && tid == 0) atomicCAS(m.err, 0, static_cast<int>(ERR_BAD_ARG));
+    griddep_wait();
     return;
   }
-  if (TMA && warp == 9 && lane == 0) { tma_prefetch_desc(&tb); tma_prefetch_desc(&ty); }
+  if (warp == 9 && lane == 0) { tma_prefetch_desc(&tl); if (TMA) { tma_prefetch_desc(&tb); tma_prefetch_desc(&ty); tma_prefetch_desc(&ty_block); } }
   if (warp == 8) { tmem_alloc(&bars.tmem, 2 * ADD_N); tmem_relinquish(); }
   uint8_t *sl = smem, *sb = smem + kblocks * X_SLOT, *sy = sb + ADD_STAGES * B_SLOT;
   volatile int* abort_flag = &bars.abort_flag;
   bool ok = true;
-  int piece = 0;                                 // of this CTA's, counted over its tiles
+  int piece = 0, tile_at = 0;                    // of this CTA's, the pieces counted over its tiles
 #pragma unroll 1
-  for (long long u = u0; u < u1;) {
+  for (long long u = u0; u < u1; ++tile_at) {
     const int at = static_cast<int>(u / n_tiles), first = static_cast<int>(u - static_cast<long long>(at) * n_tiles);
     const int n = static_cast<int>(min(u1 - u, static_cast<long long>(n_tiles - first))), steps = n * kblocks;
     u += n;
-    const Tile tile = m.tiles[at];
+    const int4 what = __ldcg(reinterpret_cast<const int4*>(m.tiles + at));
+    const Tile tile{what.x, what.y, what.z, 0};
     __syncthreads();                             // (the tile before is done with)
-    if (tid < TALL) bars.rows[tid] = tid < tile.count ? m.order[tile.begin + tid] : -1;
-    __syncthreads();
-    {
-      // the rank's values: the parts' sum, times the scale, eight a thread
-      const float by = m.scale[tile.adapter];
-#pragma unroll 1
-      for (int i = tid; i < TALL * kblocks * 8; i += 320) {
-        const int t = i / (kblocks * 8), k = i - t * kblocks * 8, row = bars.rows[t], left = m.rank - k * 8;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (row >= 0 && left > 0) {
-#pragma unroll 4
-          for (int p = 0; p < m.splits; ++p) {
-            const float* from = m.low + (static_cast<long long>(p) * m.tokens + row) * m.rank + k * 8;
-            if (m.rank % 4 == 0 && left >= 8) {
-              const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
-              f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) if (e < left) f[e] += from[e];
-            }
-          }
-        }
-        *reinterpret_cast<uint4*>(sl + (k >> 3) * X_SLOT + t * 128 + (((k & 7) ^ (t & 7)) << 4)) =
-            make_uint4(pack_bf16(f[0] * by, f[1] * by), pack_bf16(f[2] * by, f[3] * by), pack_bf16(f[4] * by, f[5] * by), pack_bf16(f[6] * by, f[7] * by));
-      }
-    }
-    fence_proxy_async();
+    if (tid < TALL) bars.rows[tid] = tid < tile.count ? __ldcg(m.order + tile.begin + tid) : -1;
     tc_fence_before();
     __syncthreads();
+    const bool block = TMA && neighbours(bars.rows, tile.count, tid);
     tc_fence_after();
+    if (tile_at == 0) griddep_wait();
     const uint32_t tmem = bars.tmem;
     if (warp >= 4 && warp < 8) {
       const int p = tid - 128, c = p & 7, yc = p & 15;
       const bf16* b = m.b + static_cast<long long>(tile.adapter) * m.out * m.rank;
-      // put back piece i (of this tile's)
+      // y's piece i (of this tile's), 16 bytes of 16 rows a thread: fetched, and put back by the thread that fetched it
+      auto fetch_y = [&](int i) {
+        const int buf = (piece + i) & 1, col = (first + i) * ADD_N + yc * 8, left = m.out - col;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int t = (p >> 4) + 8 * e, row = bars.rows[t];
+          if (row >= 0) copy8(smem_u32(sy + buf * Y_SLOT + (yc >> 3) * (TALL * 128) + t * 128 + (((yc & 7) ^ (t & 7)) << 4)), left > 0 ? m.y + static_cast<long long>(row) * m.out + col : m.y, left, m.wide_y);
+        }
+        if (m.wide_y) copies_arrive(&bars.y_full[buf]);
+        else mbar_arrive(&bars.y_full[buf]);
+      };
       auto put_back = [&](int i) {
         const int buf = (piece + i) & 1, col = (first + i) * ADD_N + yc * 8, left = m.out - col;
         ok = ok && wait(&bars.y_done[buf], ((piece + i) >> 1) & 1, abort_flag, m.err, ERR_WAIT_OTHER, lane);
@@ -579,24 +648,29 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
       if constexpr (TMA) {
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
-          put_back(i);
+          const int buf = (piece + i) & 1, half = warp - 4, col = (first + i) * ADD_N + half * 64;
+          if (block && tile.count == TALL) {
+            ok = ok && wait(&bars.y_done[buf], ((piece + i) >> 1) & 1, abort_flag, m.err, ERR_WAIT_OTHER, lane);
+            if (ok && half < 2 && col < m.out && lane == 0) {
+              tma_store_2d(&ty_block, sy + buf * Y_SLOT + half * (TALL * 128), col, bars.rows[0]);
+              tma_store_commit();
+              tma_store_wait_read<0>();
+            }
+          } else {
+            put_back(i);
+          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars.y_free[(piece + i) & 1]);
+          if (lane == 0) mbar_arrive(&bars.y_free[buf]);
         }
       } else {
-        // a slot of B a step (64 of the rank), y's piece with a piece's first; told of when the next one is on its way
+        // a slot of B a step (64 of the rank); told of when the next one is on its way
 #pragma unroll 1
         for (int step = 0; step <= steps; ++step) {
           const int i = step / kblocks, kb = step - i * kblocks;
           if (step < steps) {
             if (kb == 0) {
               if (i >= 2) put_back(i - 2);
-              const int buf = (piece + i) & 1, col = (first + i) * ADD_N + yc * 8, left = m.out - col;
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int t = (p >> 4) + 8 * e, row = bars.rows[t];
-                if (row >= 0) copy8(smem_u32(sy + buf * Y_SLOT + (yc >> 3) * (TALL * 128) + t * 128 + (((yc & 7) ^ (t & 7)) << 4)), left > 0 ? m.y + static_cast<long long>(row) * m.out + col : m.y, left, m.wide_y);
-              }
+              fetch_y(i);
             }
             const int s = piece * kblocks + step, slot = s % ADD_STAGES, k = kb * KB + c * 8, k_left = m.rank - k;
             ok = ok && wait(&bars.empty[slot], ((s / ADD_STAGES) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
@@ -613,19 +687,22 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
           copies_wait<1>();
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) {
-            const int before = (step - 1) / kblocks;
-            mbar_arrive(&bars.full[(piece * kblocks + step - 1) % ADD_STAGES]);
-            if ((step - 1) % kblocks == 0) mbar_arrive(&bars.y_full[(piece + before) & 1]);
-          }
+          if (lane == 0) mbar_arrive(&bars.full[(piece * kblocks + step - 1) % ADD_STAGES]);
         }
+      }
+      if constexpr (!TMA) {
         if (n >= 2) put_back(n - 2);
         put_back(n - 1);
       }
     } else if (warp == 9) {
+      if (lane == 0) {
+        mbar_expect_tx(&bars.low_full, kblocks * X_SLOT);
+#pragma unroll 1
+        for (int kb = 0; kb < kblocks; ++kb) tma_load_2d(sl + kb * X_SLOT, &tl, &bars.low_full, kb * KB, tile.begin);
+      }
+      __syncwarp();
       if constexpr (TMA) {
         const int4 four = four_rows(bars.rows, lane);
-        const bool there = 4 * lane < tile.count;
 #pragma unroll 1
         for (int step = 0; step < steps && ok; ++step) {
           const int i = step / kblocks, kb = step - i * kblocks, s = piece * kblocks + step, slot = s % ADD_STAGES, buf = (piece + i) & 1;
@@ -633,9 +710,10 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
             ok = wait(&bars.y_free[buf], (((piece + i) >> 1) & 1) ^ 1, abort_flag, m.err, ERR_WAIT_EMPTY, lane);
             if (!ok) break;
             fence_proxy_async();                 // (what threads read and wrote there is behind us)
-            if (lane == 0) mbar_expect_tx(&bars.y_full[buf], (tile.count + 3) / 4 * 1024);
+            if (lane == 0) mbar_expect_tx(&bars.y_full[buf], block ? Y_SLOT : (tile.count + 3) / 4 * 1024);
             __syncwarp();
-            if (there) {
+            if (block && lane < 2) tma_load_2d(sy + buf * Y_SLOT + lane * (TALL * 128), &ty_block, &bars.y_full[buf], (first + i) * ADD_N + lane * 64, bars.rows[0]);
+            if (!block && 4 * lane < tile.count) {
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 tma_gather4(sy + buf * Y_SLOT + h * (TALL * 128) + lane * 512, &ty, &bars.y_full[buf], (first + i) * ADD_N + h * 64, four.x, four.y, four.z, four.w);
@@ -653,6 +731,7 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
       }
     } else if (warp == 8) {
       constexpr uint32_t idesc = make_idesc(TALL, ADD_N, 1, 1, 0, 0);
+      ok = ok && wait(&bars.low_full, tile_at & 1, abort_flag, m.err, ERR_WAIT_FULL, lane);
 #pragma unroll 1
       for (int i = 0; i < steps && ok; ++i) {
         const int s = piece * kblocks + i, slot = s % ADD_STAGES, nt = i / kblocks, kb = i - nt * kblocks, buf = (piece + nt) & 1;
@@ -694,6 +773,7 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
           }
         }
         tc_fence_before();
+        if (TMA && block) fence_proxy_async();   // (a copy takes it from there)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&bars.acc_empty[buf]);
@@ -712,36 +792,50 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
   }
 }
 
-// One CTA: the tokens by adapter, and tiles of up to TALL of them.  (Where a token stands among its adapter's does not change its result.)
-__global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restrict__ ids, int tokens, int adapters, int* __restrict__ order, int* __restrict__ tiles_n,
-                                                            Tile* __restrict__ tiles, int* __restrict__ err) {
-  extern __shared__ int at[];                    // [adapters]: counts, then where the next token goes
-  __shared__ int totals[32][2], carry[2];
-  constexpr int HELD = 8;                        // ids that a thread keeps
+// One CTA: the tokens by adapter, each adapter's in their order (a run of neighbours is fetched as a block then), and tiles of up to TALL of them.  A warp looks through a
+// sixteenth of the tokens, and counts them by adapter for itself.
+constexpr int GROUP_WARPS = 16;
+__global__ void __launch_bounds__(GROUP_WARPS * 32) group_tokens_kernel(const int* __restrict__ ids, int tokens, int adapters, int* __restrict__ order, int* __restrict__ tiles_n,
+                                                                        Tile* __restrict__ tiles, int* __restrict__ err) {
+  extern __shared__ int at[];                    // [GROUP_WARPS][adapters]: counts, then where the next token goes
+  __shared__ int totals[GROUP_WARPS][2], carry[2];
+  constexpr int HELD = 16;                       // ids that a lane keeps
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  griddep_wait();
   griddep_launch();
+  const int per = ((tokens + GROUP_WARPS - 1) / GROUP_WARPS + 31) / 32 * 32, from = warp * per, to = min(tokens, from + per);
   int held[HELD];
 #pragma unroll
-  for (int e = 0; e < HELD; ++e) held[e] = e * 1024 + tid < tokens ? ids[e * 1024 + tid] : -1;
-  for (int i = tid; i < adapters; i += 1024) at[i] = 0;
+  for (int e = 0; e < HELD; ++e) held[e] = from + e * 32 + lane < to ? ids[from + e * 32 + lane] : -1;
+  for (int i = tid; i < GROUP_WARPS * adapters; i += GROUP_WARPS * 32) at[i] = 0;
   if (tid == 0) carry[0] = carry[1] = 0;
   __syncthreads();
+  int* mine = at + warp * adapters;
   auto each = [&](auto take) {
 #pragma unroll
     for (int e = 0; e < HELD; ++e)
-      if (e * 1024 < tokens) take(e * 1024 + tid, held[e]);
+      if (from + e * 32 < to) take(from + e * 32 + lane, held[e]);
 #pragma unroll 1
-    for (int i0 = HELD * 1024; i0 < tokens; i0 += 1024) take(i0 + tid, i0 + tid < tokens ? ids[i0 + tid] : -1);
+    for (int i0 = from + HELD * 32; i0 < to; i0 += 32) take(i0 + lane, i0 + lane < to ? ids[i0 + lane] : -1);
   };
   each([&](int, int id) {
     const bool there = id >= 0 && id < adapters;
     if (id >= adapters) atomicCAS(err, 0, static_cast<int>(ERR_BAD_ARG));
     const unsigned same = __match_any_sync(FULL, there ? id : -1);
-    if (there && lane == __ffs(same) - 1) atomicAdd(&at[id], __popc(same));
+    if (there && lane == __ffs(same) - 1) mine[id] += __popc(same);
+    __syncwarp();
   });
   __syncthreads();
-  for (int i0 = 0; i0 < adapters; i0 += 1024) {
-    const int i = i0 + tid, n = i < adapters ? at[i] : 0, t = (n + TALL - 1) / TALL;
+  for (int i0 = 0; i0 < adapters; i0 += GROUP_WARPS * 32) {
+    const int i = i0 + tid;
+    int n = 0;
+    if (i < adapters)
+      for (int w = 0; w < GROUP_WARPS; ++w) {
+        const int v = at[w * adapters + i];
+        at[w * adapters + i] = n;
+        n += v;
+      }
+    const int t = (n + TALL - 1) / TALL;
     int sn = n, st = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -753,9 +847,9 @@ __global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restric
     int bn = carry[0], bt = carry[1];
     for (int w = 0; w < warp; ++w) { bn += totals[w][0]; bt += totals[w][1]; }
     __syncthreads();
-    if (tid == 1023) { carry[0] = bn + sn; carry[1] = bt + st; }
+    if (tid == GROUP_WARPS * 32 - 1) { carry[0] = bn + sn; carry[1] = bt + st; }
     if (i < adapters) {
-      at[i] = bn + sn - n;
+      for (int w = 0; w < GROUP_WARPS; ++w) at[w * adapters + i] += bn + sn - n;
       for (int j = 0; j < t; ++j) tiles[bt + st - t + j] = Tile{i, bn + sn - n + j * TALL, min(TALL, n - j * TALL), 0};
     }
     __syncthreads();
@@ -764,10 +858,10 @@ __global__ void __launch_bounds__(1024) group_tokens_kernel(const int* __restric
   each([&](int i, int id) {
     const bool there = id >= 0 && id < adapters;
     const unsigned same = __match_any_sync(FULL, there ? id : -1);
-    int base = 0;
-    if (there && lane == __ffs(same) - 1) base = atomicAdd(&at[id], __popc(same));
-    base = __shfl_sync(FULL, base, __ffs(same) - 1);
-    if (there) order[base + __popc(same & ((1u << lane) - 1))] = i;
+    if (there) order[mine[id] + __popc(same & ((1u << lane) - 1))] = i;
+    __syncwarp();
+    if (there && lane == __ffs(same) - 1) mine[id] += __popc(same);
+    __syncwarp();
   });
 }
 
@@ -783,9 +877,11 @@ int multiprocessors() {
 }
 
 template <typename K, typename... A>
-int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, int cluster, const A&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return static_cast<int>(e);
+int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, dim3 cluster, const A&... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -795,10 +891,11 @@ int launch_early(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream
   with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   with[0].val.programmaticStreamSerializationAllowed = 1;
   with[1].id = cudaLaunchAttributeClusterDimension;
-  with[1].val.clusterDim.x = cluster;
-  with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
+  with[1].val.clusterDim.x = cluster.x;
+  with[1].val.clusterDim.y = cluster.y;
+  with[1].val.clusterDim.z = 1;
   cfg.attrs = with;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.numAttrs = cluster.x * cluster.y > 1 ? 2 : 1;
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
@@ -825,47 +922,50 @@ extern "C" int dewb_add_adapters(const void* x, long long x_stride, const void* 
   return static_cast<int>(cudaGetLastError());
 }
 
-// The same on the tensor cores: bf16, rank up to 512, up to 4096 adapters, any widths.  Up to 512 tokens: one launch, no scratch.  More: three, and scratch: low (splits x tokens x
-// rank floats), order (tokens integers), tiles (4 integers, then 4 for each of tokens / 128 + min(adapters, tokens) + 1, on a 16-byte boundary).
-extern "C" int dewb_add_adapters_mma(const void* x, long long x_stride, const void* a, const void* b, const float* scale, const int* ids, int* order, void* tiles, float* low, void* y,
+// The same on the tensor cores: bf16, rank up to 512, up to 3500 adapters, any widths.  Up to 512 tokens: one launch, no scratch.  More: three, and scratch: low (tokens x rank
+// rounded up to 64, bf16), order (tokens integers), tiles (4 integers, then 4 for each of tokens / 128 + min(adapters, tokens) + 1), low and tiles on 16-byte boundaries; splits 1, 2, 4 or 8.
+extern "C" int dewb_add_adapters_mma(const void* x, long long x_stride, const void* a, const void* b, const float* scale, const int* ids, int* order, void* tiles, void* low, void* y,
                                      int tokens, int adapters, int rank, int width, int out, int splits, int* err, void* stream_ptr) {
   using namespace dewb::adapters;
   if (tokens <= 0 || out <= 0) return 0;
-  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > MOST_RANK || width <= 0 || splits < 1 || splits > 65535 ) return -3;
+  if (adapters <= 0 || adapters > MOST_ADAPTERS || rank <= 0 || rank > MOST_RANK || width <= 0 || splits < 1 || splits > 8 || (splits & (splits - 1))) return -3;
   auto whole = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   int* n = static_cast<int*>(tiles);
-  const Mma m{static_cast<const bf16*>(x), static_cast<const bf16*>(a), static_cast<const bf16*>(b), scale, ids, order, n, n == nullptr ? nullptr : reinterpret_cast<const Tile*>(n + 4), low,
-              static_cast<bf16*>(y), x_stride, tokens, adapters, rank, width, out, splits,
+  const int wide = (rank + KB - 1) / KB * KB;
+  const Mma m{static_cast<const bf16*>(x), static_cast<const bf16*>(a), static_cast<const bf16*>(b), scale, ids, order, n, n == nullptr ? nullptr : reinterpret_cast<const Tile*>(n + 4),
+              static_cast<bf16*>(low), static_cast<bf16*>(y), x_stride, tokens, adapters, rank, width, out, splits, wide,
               width % 8 == 0 && x_stride % 8 == 0 && whole(x) && whole(a), rank % 8 == 0 && whole(b), out % 8 == 0 && whole(y), err};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   if (tokens <= SCANNED) {
-    const int wide = (rank + 31) / 32 * 32, smem = 4 * (STEP_WARPS * MT * RB + MT * wide) + 2 * MT * (wide + 8);
-    // (128 tokens of 48 adapters of rank 32, 4096 to 6144: clusters of eight 18 us, of four @@; one token, 1024 to 2048: @@)
-    return tokens <= 32 ? launch_early(adapters_step_kernel<8>, dim3(8, tokens), STEP_THREADS, smem, stream, 8, m) : launch_early(adapters_step_kernel<4>, dim3(4, tokens), STEP_THREADS, smem, stream, 4, m);
+    const int pad = (rank + 31) / 32 * 32, ranks = rank <= 32 ? 32 : 64, smem = std::max(4 * (STEP_WARPS * MT * ranks + MT * pad) + 2 * MT * (pad + 8), 2 * STEP_WARPS * adapters);
+    const dim3 grid(CLUSTER, std::min(tokens, std::min(adapters, tokens) + tokens / MT));
+    return rank <= 32 ? launch_early(adapters_step_kernel<CLUSTER, 32>, grid, STEP_THREADS, smem, stream, dim3(CLUSTER), m)
+                      : launch_early(adapters_step_kernel<CLUSTER, 64>, grid, STEP_THREADS, smem, stream, dim3(CLUSTER), m);
   }
   if (order == nullptr || tiles == nullptr || low == nullptr || !whole(tiles) || !whole(low)) return -3;
-  group_tokens_kernel<<<1, 1024, adapters * 4, stream>>>(ids, tokens, adapters, order, n, reinterpret_cast<Tile*>(n + 4), err);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  const int most = tokens / TALL + (adapters < tokens ? adapters : tokens) + 1;
-  CUtensorMap t0 = {}, t1 = {};
+  int rc = launch_early(group_tokens_kernel, dim3(1), GROUP_WARPS * 32, GROUP_WARPS * adapters * 4, stream, dim3(1), ids, tokens, adapters, order, n, reinterpret_cast<Tile*>(n + 4), err);
+  if (rc) return rc;
+  const int most = tokens / TALL + std::min(adapters, tokens) + 1;
+  CUtensorMap t0 = {}, t1 = {}, t2 = {}, t3 = {};
   const uint64_t rows = tokens, ranks = static_cast<uint64_t>(adapters) * rank, outs = static_cast<uint64_t>(adapters) * out;
-  int rc;
-  const dim3 first(most, splits, (rank + RB - 1) / RB);
+  const dim3 first(most, splits, (rank + RB - 1) / RB), together(1, splits);
   if (m.wide_x) {
     if ((rc = dewb::make_tmap_2d(&t0, x, rows, width, x_stride, 1, KB, 2, true))) return 1000 + rc;
-    if ((rc = dewb::make_tmap_2d(&t1, a, ranks, width, width, RB, KB, 2, true))) return 2000 + rc;
-    rc = launch_early(make_low_kernel<true>, first, 192, MAKE_SMEM, stream, 1, t0, t1, m);
+    if ((rc = dewb::make_tmap_2d(&t1, x, rows, width, x_stride, TALL, KB, 2, true))) return 1000 + rc;
+    if ((rc = dewb::make_tmap_2d(&t2, a, ranks, width, width, RB, KB, 2, true))) return 2000 + rc;
+    rc = launch_early(make_low_kernel<true>, first, 192, MAKE_SMEM, stream, together, t0, t1, t2, m);
   } else {
-    rc = launch_early(make_low_kernel<false>, first, 192, MAKE_SMEM, stream, 1, t0, t1, m);
+    rc = launch_early(make_low_kernel<false>, first, 192, MAKE_SMEM, stream, together, t0, t1, t2, m);
   }
   if (rc) return rc;
   // two CTAs an SM where their memory fits
-  const int smem = (rank + KB - 1) / KB * X_SLOT + ADD_STAGES * B_SLOT + 2 * Y_SLOT, ctas = multiprocessors() * (2 * (smem + 2048) <= 228 * 1024 ? 2 : 1);
+  const int smem = wide / KB * X_SLOT + ADD_STAGES * B_SLOT + 2 * Y_SLOT, ctas = multiprocessors() * (2 * (smem + 2048) <= 228 * 1024 ? 2 : 1);
+  if ((rc = dewb::make_tmap_2d(&t0, low, rows, wide, wide, TALL, KB, 2, true))) return 3000 + rc;
   if (m.wide_b && m.wide_y && outs < 0x7fffff00ull) {
-    if ((rc = dewb::make_tmap_2d(&t0, b, outs, rank, rank, ADD_N, KB, 2, true))) return 3000 + rc;
-    if ((rc = dewb::make_tmap_2d(&t1, y, rows, out, out, 1, KB, 2, true))) return 4000 + rc;
-    return launch_early(add_columns_kernel<true>, dim3(ctas), 320, smem, stream, 1, t0, t1, m);
+    if ((rc = dewb::make_tmap_2d(&t1, b, outs, rank, rank, ADD_N, KB, 2, true))) return 4000 + rc;
+    if ((rc = dewb::make_tmap_2d(&t2, y, rows, out, out, 1, KB, 2, true))) return 5000 + rc;
+    if ((rc = dewb::make_tmap_2d(&t3, y, rows, out, out, TALL, KB, 2, true))) return 5000 + rc;
+    return launch_early(add_columns_kernel<true>, dim3(ctas), 320, smem, stream, dim3(1), t0, t1, t2, t3, m);
   }
-  return launch_early(add_columns_kernel<false>, dim3(ctas), 320, smem, stream, 1, t0, t1, m);
+  return launch_early(add_columns_kernel<false>, dim3(ctas), 320, smem, stream, dim3(1), t0, t1, t2, t3, m);
 }

@@ -1121,8 +1121,14 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas
   static_assert(sizeof(Bars) % 16 == 0 && alignof(Lists) == 16 && offsetof(Lists, top) % 16 == 0, "the maxima are read four at a time");
   constexpr int SMEM = C::Q_BYTES + C::EXTRA + C::RING * C::SLOT + static_cast<int>(sizeof(Bars) + sizeof(Lists));
   static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "over an SM's shared memory");
-  cudaError_t e = cudaFuncSetAttribute(shared_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+  static bool allowed[64] = {};                  // (once for a device)
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev >= 64 || !allowed[dev]) {
+    if ((e = cudaFuncSetAttribute(shared_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) != cudaSuccess) return static_cast<int>(e);
+    if (dev < 64) allowed[dev] = true;
+  }
   shared_mma_kernel<D><<<ctas, THREADS, SMEM, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};

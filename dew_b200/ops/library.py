@@ -187,6 +187,11 @@ def on_device_of(t: torch.Tensor):
             _TLS.device = None
 
 
+def device_is_current(t: torch.Tensor) -> bool:
+    """Whether a launch for ``t`` can be issued as things stand; else it belongs under ``on_device_of``, whose entry and exit take as long as a launch."""
+    return t.get_device() == torch._C._cuda_getDevice()
+
+
 def stream() -> int:
     """The current stream of the current device."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())

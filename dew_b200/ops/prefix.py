@@ -85,7 +85,7 @@ def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: 
     can be counted in 32 bits."""
     R, H, D = q.shape
     pages, page, G, _ = k.shape
-    return (q.dtype == k.dtype == torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
+    return (q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
             and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 2) < 1 << 30
             and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
 
@@ -94,33 +94,46 @@ _POOLS = {torch.int8: 1, torch.float8_e4m3fn: 2}
 
 
 def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_scale, v_scale) -> None:
-    if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape or q.shape[2] != k.shape[3] or k.shape[2] == 0 or q.shape[1] % k.shape[2]:
+    order, first, tokens = shared
+    q_shape, k_shape = q.shape, k.shape
+    if len(q_shape) != 3 or len(k_shape) != 4 or k_shape != v.shape or q_shape[2] != k_shape[3] or k_shape[2] == 0 or q_shape[1] % k_shape[2]:
         raise ValueError(f"shared_decode: queries [rows, heads, dim] and pools [pages, page, kv heads, dim], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if q.dtype not in (torch.bfloat16, torch.float32) or k.dtype != v.dtype or (k.dtype != q.dtype and k.dtype not in _POOLS):
+    own, pool = q.dtype, k.dtype
+    if (own is not torch.bfloat16 and own is not torch.float32) or pool != v.dtype or (pool is not own and pool not in _POOLS):
         raise TypeError(f"shared_decode: bf16 or fp32 queries and pools of their type, int8 or float8_e4m3fn, got {q.dtype}, {k.dtype}, {v.dtype}")
-    R, H, D = q.shape
-    scales = (k_scale, v_scale) if k.dtype in _POOLS else ()
-    if (k_scale is None) == bool(scales) or (v_scale is None) == bool(scales):
+    R, H, D = q_shape
+    scaled = pool is not own
+    if (k_scale is not None) != scaled or (v_scale is not None) != scaled:
         raise ValueError("shared_decode: scales belong to int8 and float8 pools")
     if not 0 < D <= 256:
         raise ValueError(f"shared_decode: heads of up to 256, got {D}")
-    if shared.order.shape != (R,) or shared.tokens.dim() != 1 or shared.first.shape != (shared.tokens.shape[0] + 1,) or (R and not len(shared.tokens)):
+    groups = len(tokens) if tokens.dim() == 1 else -1
+    if groups < (R > 0) or order.shape != (R,) or first.shape != (groups + 1,):
         raise ValueError(f"shared_decode: order [rows], first [groups + 1] and tokens [groups] for {R} rows, got {[tuple(t.shape) for t in shared]}")
-    if table.dim() != 2 or table.shape[0] != R or lengths.shape != (R,):
+    if table.dim() != 2 or len(table) != R or lengths.shape != (R,):
         raise ValueError(f"shared_decode: a table [rows, columns] and lengths [rows] for {R} rows, got {tuple(table.shape)}, {tuple(lengths.shape)}")
-    if any(t.dtype != torch.int32 or not t.is_contiguous() for t in (table, lengths, *shared)):
-        raise TypeError("shared_decode: table, lengths, order, first and tokens are int32 in one piece")
-    if any(s.shape != k.shape[:3] or s.dtype != torch.float32 or not s.is_contiguous() for s in scales):
-        raise ValueError("shared_decode: fp32 scales [pages, page, kv heads]")
-    if sinks is not None and (sinks.shape != (H,) or sinks.dtype != torch.float32 or not sinks.is_contiguous()):
-        raise ValueError("shared_decode: fp32 sinks, one a head")
+    device = q.device
+    apart = k.device != device or v.device != device
+    for t in (table, lengths, order, first, tokens):
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            raise TypeError("shared_decode: table, lengths, order, first and tokens are int32 in one piece")
+        apart = apart or t.device != device
+    if scaled:
+        for t in (k_scale, v_scale):
+            if t.shape != k_shape[:3] or t.dtype is not torch.float32 or not t.is_contiguous():
+                raise ValueError("shared_decode: fp32 scales [pages, page, kv heads]")
+            apart = apart or t.device != device
+    if sinks is not None:
+        if sinks.shape != (H,) or sinks.dtype is not torch.float32 or not sinks.is_contiguous():
+            raise ValueError("shared_decode: fp32 sinks, one a head")
+        apart = apart or sinks.device != device
     if (window is not None and window < 1) or softcap < 0:
         raise ValueError(f"shared_decode: a window of 1 or more and a cap of 0 or more, got {window}, {softcap}")
     if not (k.is_contiguous() and v.is_contiguous()):
         raise ValueError("shared_decode: pools in one piece")
-    if any(t is not None and t.device != q.device for t in (k, v, table, lengths, *shared, sinks, k_scale, v_scale)):
+    if apart:
         raise ValueError("shared_decode: tensors of one device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, sinks)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad)):
         raise NotImplementedError("shared_decode has no gradient: it is a step of generation")
 
 
@@ -138,33 +151,34 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
         return q.new_empty(q.shape)
     if not L.use_cuda(q):
         return shared_decode_reference(q, k, v, table, lengths, scale, window, softcap, sinks, k_scale, v_scale)
-    if q.stride(2) != 1 or (H > 1 and q.stride(1) != D):
+    if not L.device_is_current(q):
+        with L.on_device_of(q):
+            return shared_decode(q, k, v, table, lengths, shared, scale, window=window, softcap=softcap, sinks=sinks, k_scale=k_scale, v_scale=v_scale)
+    strides = q.stride()
+    if strides[2] != 1 or (H > 1 and strides[1] != D):
         q = q.contiguous()
+        strides = q.stride()
     out = torch.empty(R, H, D, dtype=q.dtype, device=q.device)
     pages, page, G, _ = k.shape
-    groups, err, fp32 = len(shared.tokens), L.status(q.device).data_ptr(), torch.float32
-    if on_tensor_cores(q, k, v, table.shape[1], groups):
-        with L.on_device_of(q) as stream:
-            lib = L.load()
-            ctas = _ctas(lib, q.device, D)
-            rows = 2 * R * H + 320 * ctas
-            # one piece of scratch a call: sums, maxima and sums of weights, the plan
-            scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
-            at = scratch.data_ptr()
-            L.check(lib.dewb_shared_decode_mma(q.data_ptr(), q.stride(0) if R > 1 else H * D, k.data_ptr(), v.data_ptr(), table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(),
-                                               shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + 4 * rows * D, at + 4 * rows * (D + 2), out.data_ptr(),
-                                               R, H, G, D, page, table.shape[1], pages, groups, window or 0, LEAST_TILES, ctas, scale, softcap, err, stream),
-                    "shared_decode_mma")
+    columns, groups, fp32, lib = table.shape[1], len(shared.tokens), torch.float32, L.load()
+    numbers = (table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks))
+    err, stream = L.status(q.device).data_ptr(), L.stream()
+    if on_tensor_cores(q, k, v, columns, groups):
+        ctas = _ctas(lib, q.device, D)
+        rows = 2 * R * H + 320 * ctas
+        # one piece of scratch a call: sums, maxima and sums of weights, the plan
+        scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
+        at = scratch.data_ptr()
+        L.check(lib.dewb_shared_decode_mma(q.data_ptr(), strides[0] if R > 1 else H * D, k.data_ptr(), v.data_ptr(), *numbers, at, at + 4 * rows * D, at + 4 * rows * (D + 2),
+                                           out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, ctas, scale, softcap, err, stream), "shared_decode_mma")
         L.count_launches(2)
         return out
-    splits = max(1, min(32, -(-table.shape[1] * page // 512)))
+    splits = max(1, min(32, -(-columns * page // 512)))
     parts = torch.empty(2 * splits * R * H * (D + 2), dtype=fp32, device=q.device)
     at = parts.data_ptr()
     one = 2 * splits * R * H * 4
-    with L.on_device_of(q) as stream:
-        L.check(L.load().dewb_shared_decode(q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), L.at(k_scale), L.at(v_scale), table.data_ptr(), lengths.data_ptr(),
-                                            shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks), at, at + one, at + 2 * one, out.data_ptr(),
-                                            R, H, G, D, page, table.shape[1], pages, groups, splits, window or 0, scale, softcap,
-                                            int(q.dtype == fp32), _POOLS.get(k.dtype, 0), err, stream), "shared_decode")
+    L.check(lib.dewb_shared_decode(q.data_ptr(), strides[0], k.data_ptr(), v.data_ptr(), L.at(k_scale), L.at(v_scale), *numbers, at, at + one, at + 2 * one, out.data_ptr(),
+                                   R, H, G, D, page, columns, pages, groups, splits, window or 0, scale, softcap, int(q.dtype is fp32), _POOLS.get(k.dtype, 0), err, stream),
+            "shared_decode")
     L.count_launches(2)
     return out
