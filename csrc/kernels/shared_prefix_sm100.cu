@@ -41,7 +41,7 @@ namespace sharedmma {
 
 constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys of a tile
 constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
-constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;
+constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;              // of an engine
 constexpr int MOST_ROWS = 448;
 constexpr int TALL_GAP = 2, WIDE_GAP = 1;         // tiles that a list takes as long as beyond its own
 constexpr int TALL_COST = 1, WIDE_COST = 2;       // of a tile, where CTAs are dealt
@@ -56,11 +56,12 @@ struct Cfg {
   static constexpr int SLOT = BN * D * 2, RING = D == 64 ? 8 : 4, HALF = RING / 2;                // tall: a tile's keys (first half) or values
   static constexpr int W_TILE = WK * D * 2, W_SLOTS = RING / 4;                // wide: the same memory, half for keys and half for values
   static constexpr int W_Q = WN * D * 2, W_P = WN * WK * 2;
-  static constexpr int CTAS = D == 256 ? 1 : 2;   // an SM
+  static constexpr int ENGINES = D == 256 ? 1 : 2;                             // a CTA, which has its SM to itself
   static constexpr int HALVES = D == 256 ? 2 : 1; // wide: 128-column pieces of a head
   static constexpr int TM_O = 2 * BN, TM_COLS = D == 256 ? 512 : 256;
   static constexpr int TM_WO = 2 * WN;
   static constexpr int EXTRA = 2 * W_Q + 2 * W_P > Q_BYTES ? 2 * W_Q + 2 * W_P - Q_BYTES : 0;      // (where that is more)
+  static constexpr int ENGINE = Q_BYTES + EXTRA + RING * SLOT;                 // bytes
 };
 
 struct Ranges {                                   // the keys of a list, [a0, a1) and [b0, b1), and its tiles of N
@@ -88,13 +89,21 @@ struct alignas(16) Bars {
   uint64_t list_full[2], list_empty[2];           // what a list is about (wide: and its queries)
   uint64_t full[8], empty[8];                     // slots of the ring: [0, 4) keys, [4, 8) values
   uint64_t q_full, s_full[2], p_full[2], done;
-  uint32_t tmem;
-  int abort_flag, poisoned;
+  int abort_flag;
 };
 
-// what a CTA knows of all lists
+struct alignas(16) Own {                          // an engine's
+  Bars bars;
+  Item item[2];                                   // the list at hand and the next one
+  float most[4][WN];                              // wide: largest scores, by warp
+  alignas(16) float top[4][WN], by[4][WN];        // (read four at a time) each warp's copy of the maxima in use, and what sums made with older ones are multiplied with
+  float sums[4][WN];                              // of weights, by warp
+};
+
+// what a CTA knows of all lists (an engine is an engine of the grid's)
 struct Lists {
-  int tall_units, tall_ctas, tall_per_cta, wide_shared_units, wide_units, wide_per_cta;      // (units: tiles and the room in front of lists)
+  int tall_units, tall_engines, tall_each, wide_shared_units, wide_units, wide_each;         // (units: tiles and the room in front of lists)
+  bool apart;                                     // whether no more engines than CTAs have work
   short first[MOST_ROWS + 2];                     // groups: first place
   short row[MOST_ROWS], group[MOST_ROWS];         // places (row -1: none)
   short through[MOST_ROWS];                       // groups: a row that holds something
@@ -102,10 +111,8 @@ struct Lists {
   int tall[MOST_ROWS + 1], wide[MOST_ROWS + 1];   // groups: units of either kind before
   int own[MOST_ROWS + 1];                         // places: own tiles before
   int len[MOST_ROWS];                             // places
-  Item item[2];                                   // the list at hand and the next one
-  float most[4][WN];                              // wide: largest scores, by warp
-  alignas(16) float top[4][WN], by[4][WN];        // (read four at a time) each warp's copy of the maxima in use, and what sums made with older ones are multiplied with
-  float sums[4][WN];                              // of weights, by warp
+  uint32_t tmem;
+  int poisoned;
 };
 
 struct Args {
@@ -114,7 +121,7 @@ struct Args {
   const int *table, *lengths, *order, *first, *tokens;
   const float* sinks;
   __nv_bfloat16* out;
-  float* acc;                                     // [2 rows heads + ctas (2 128 + 2 32)][D]
+  float* acc;                                     // [2 rows heads + engines (2 128 + 2 32)][D]
   float2* ml;                                     // [the same]: maximum (log2), sum
   int4* plan;                                     // [rows][2], for the second kernel: see write_plan
   int rows, heads, kv_heads, ratio, chunks, page_size, box, max_pages, pages, groups, window, least;      // (ratio: heads a key head; chunks of 32 of those)
@@ -255,15 +262,15 @@ __device__ __forceinline__ void fetch_queries(uint8_t* to, int apart, const Args
 }
 
 // What the second kernel needs of a place: its group's first unit and tiles (of either kind), its own; its group's first place and queries a key head (0: wide), units a CTA.
-__device__ __forceinline__ void write_plan(const Lists& s, const Args& a, int tid) {
+__device__ __forceinline__ void write_plan(const Lists& s, const Args& a) {
   const int lists = a.kv_heads * a.chunks;
 #pragma unroll 1
-  for (int i = tid; i < a.rows; i += THREADS) {
+  for (int i = threadIdx.x; i < a.rows; i += blockDim.x) {
     const int g = s.group[i], queries = group_queries(s, a, g);
     const Ranges both{s.lo[g], s.hi[g], 0, 0};
     const bool tall = queries > WN;
     a.plan[2 * i] = make_int4(tall ? s.tall[g] : s.wide[g], tall ? both.tiles<BN>() : both.tiles<WK>(), s.wide_shared_units + s.own[i] * lists, max(s.own[i + 1] - s.own[i] - WIDE_GAP, 0));
-    a.plan[2 * i + 1] = make_int4(s.first[g], tall ? queries : 0, s.tall_per_cta, s.wide_per_cta);
+    a.plan[2 * i + 1] = make_int4(s.first[g], tall ? queries : 0, s.tall_each, s.wide_each);
   }
 }
 
@@ -285,16 +292,18 @@ __device__ __forceinline__ void running_sums(int* x, int n, int lane) {
   for (int i = i0; i < i1; ++i) { run += x[i + 1]; x[i + 1] = run; }
 }
 
-// false: an earlier launch reported an error (read here, beside what else is on its way)
-__device__ __forceinline__ bool make_lists(Lists& s, Bars* bars, const Args& a, int tid, int warp, int lane) {
+// All of a CTA's threads.  false: an earlier launch reported an error (read here, beside what else is on its way)
+template <int THREADS>
+__device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines) {
   constexpr int EACH = (MOST_ROWS + THREADS - 1) / THREADS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int most = a.max_pages * a.page_size;
   int* live = s.own;                              // (until the places' tiles are known)
   // rows and lengths are on their way while the groups are looked at
   int row_of[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) row_of[e] = e * THREADS + tid < a.rows ? a.order[e * THREADS + tid] : -1;
-  if (tid == THREADS - 1) bars->poisoned = *reinterpret_cast<volatile int*>(a.err);
+  if (tid == THREADS - 1) s.poisoned = *reinterpret_cast<volatile int*>(a.err);
 #pragma unroll 1
   for (int g = tid; g <= a.groups; g += THREADS) {
     s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
@@ -313,7 +322,7 @@ __device__ __forceinline__ bool make_lists(Lists& s, Bars* bars, const Args& a, 
     s.len[i] = bad ? -1 : a.lengths[row_of[e]];
   }
   __syncthreads();
-  if (bars->poisoned != 0) return false;
+  if (s.poisoned != 0) return false;
 #pragma unroll 1
   for (int i0 = warp * 32; i0 < a.rows; i0 += THREADS) {
     const int i = i0 + lane;
@@ -364,31 +373,31 @@ __device__ __forceinline__ bool make_lists(Lists& s, Bars* bars, const Args& a, 
   if (warp < 3) running_sums(warp == 0 ? s.tall : warp == 1 ? s.wide : s.own, warp < 2 ? a.groups : a.rows, lane);
   __syncthreads();
   if (tid == 0) {
-    const int ctas = static_cast<int>(gridDim.x);
     s.tall_units = s.tall[a.groups];
     s.wide_shared_units = s.wide[a.groups];
     s.wide_units = s.wide_shared_units + s.own[a.rows] * a.kv_heads * a.chunks;
-    // CTAs for either kind by their work
+    // engines for either kind by their work
     const long long tall = static_cast<long long>(s.tall_units) * TALL_COST, wide = static_cast<long long>(s.wide_units) * WIDE_COST;
-    int k = tall == 0 ? 0 : wide == 0 ? ctas : static_cast<int>((tall * ctas + (tall + wide) / 2) / (tall + wide));
-    if (tall > 0 && wide > 0) k = min(max(k, 1), ctas - 1);
+    int k = tall == 0 ? 0 : wide == 0 ? engines : static_cast<int>((tall * engines + (tall + wide) / 2) / (tall + wide));
+    if (tall > 0 && wide > 0) k = min(max(k, 1), engines - 1);
     const int least = a.least + WIDE_GAP;
-    s.tall_ctas = min(k, (s.tall_units + 2 * least - 1) / (2 * least));
-    s.tall_per_cta = s.tall_ctas == 0 ? 1 : (s.tall_units + s.tall_ctas - 1) / s.tall_ctas;
-    const int rest = max(1, ctas - s.tall_ctas);
-    s.wide_per_cta = max(least, (s.wide_units + rest - 1) / rest);
+    s.tall_engines = min(k, (s.tall_units + 2 * least - 1) / (2 * least));
+    s.tall_each = s.tall_engines == 0 ? 1 : (s.tall_units + s.tall_engines - 1) / s.tall_engines;
+    const int rest = max(1, engines - s.tall_engines);
+    s.wide_each = max(least, (s.wide_units + rest - 1) / rest);
+    s.apart = s.tall_engines + (s.wide_units + s.wide_each - 1) / s.wide_each <= static_cast<int>(gridDim.x);
   }
   __syncthreads();
   return true;
 }
 
 // ---------------------------------------------------------------------------------------------------------- wide lists' softmax
-__device__ __forceinline__ bool any_of_128(bool p) {       // whether p holds for any of the softmax's threads
+__device__ __forceinline__ bool any_of_128(bool p, int engine) {       // whether p holds for any of an engine's softmax's threads
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(p)) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(static_cast<uint32_t>(p)), "r"(1 + engine) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void sync_128() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void sync_128(int engine) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + engine) : "memory"); }
 
 // largest of a warp's values
 __device__ __forceinline__ float warp_max(float x) {
@@ -427,9 +436,9 @@ __device__ __forceinline__ void load_columns(uint32_t at, float (&x)[NC]) {
 struct Wide {                                     // what a list's softmax works with
   uint32_t t_s, t_o;                              // tensor memory, this warp's lanes
   uint8_t *weights, *values;                      // shared memory
-  Bars* bars;
+  Own* own;
   volatile int* abort_flag;
-  int tid, warp, lane, cta;                       // (cta: among those of wide lists)
+  int tid, warp, lane, engine, at;                // (engine: of the CTA's; at: among those of wide lists)
 };
 
 // One wide list of up to NC queries, whose first tile is the CTA's t-th: false after a wait that ran out.  (All warps pass all barriers, whatever went wrong: waits that
@@ -438,11 +447,12 @@ struct Wide {                                     // what a list's softmax works
 // What runs once a list is written as loops: straight code comes from L2 at some 250 cycles a 128-byte line when a launch first runs it, and all CTAs of a launch are at
 // the same line.  (Unrolled over 32 queries, a launch's first maxima took 25000 cycles, and first results 6000.)
 template <int D, int NC>
-__device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Args& a, const Item& w, int& t) {
+__device__ __forceinline__ bool wide_list(const Wide& x, const Lists& lists, const Args& a, const Item& w, int& t) {
   using C = Cfg<D>;
-  Bars* bars = x.bars;
+  Own& own = *x.own;
+  Bars* bars = &own.bars;
   const int tid = x.tid, lane = x.lane, warp = x.warp, tiles = w.tiles, n = w.n;
-  float *top = lists.top[warp], *by = lists.by[warp];
+  float *top = own.top[warp], *by = own.by[warp];
   bool ok = true;
   float l[NC];                                    // sums of this thread's keys' weights
 #pragma unroll
@@ -472,17 +482,17 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
       const float4 m = *reinterpret_cast<const float4*>(top + q);
       past = past || (q < n && s[q] > m.x + RESCALE) || (q + 1 < n && s[q + 1] > m.y + RESCALE) || (q + 2 < n && s[q + 2] > m.z + RESCALE) || (q + 3 < n && s[q + 3] > m.w + RESCALE);
     }
-    if (j == 0 || any_of_128(past && seen)) {
+    if (j == 0 || any_of_128(past && seen, x.engine)) {
       float mine = -INFINITY;
 #pragma unroll
       for (int q = 0; q < NC; ++q) {
         const float most = warp_max(seen ? s[q] : -INFINITY);
         mine = lane == q ? most : mine;
       }
-      lists.most[warp][lane] = mine;
-      sync_128();
+      own.most[warp][lane] = mine;
+      sync_128(x.engine);
       if (lane < NC) {
-        const float was = top[lane], now = fmaxf(was, fmaxf(fmaxf(lists.most[0][lane], lists.most[1][lane]), fmaxf(lists.most[2][lane], lists.most[3][lane])));
+        const float was = top[lane], now = fmaxf(was, fmaxf(fmaxf(own.most[0][lane], own.most[1][lane]), fmaxf(own.most[2][lane], own.most[3][lane])));
         by[lane] = was > -INFINITY && lane < n ? fast_exp2(was - now) : 1.f;
         top[lane] = now;
       }
@@ -533,7 +543,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
   const bool last = entire && !w.shared && lists.hi[lists.group[w.index]] == 0;
   const int one = query(lists, a, w, lane);
   const long long all = static_cast<long long>(a.rows) * a.heads;
-  long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * 2 * BM + (2 * x.cta + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
+  long long at = last ? one : !entire ? 2 * all + static_cast<long long>(gridDim.x) * (C::ENGINES * 2 * BM) + (2 * x.at + (w.from == 0 ? 1 : 0)) * WN + lane : w.shared ? one : all + one;
   if (one < 0) at = -1;
   // sums over a warp: each exchange halves the queries that a lane is about, until lane i has query i % NC's
 #pragma unroll
@@ -547,16 +557,16 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
   }
 #pragma unroll
   for (int h = NC; h < 32; h <<= 1) l[0] += __shfl_xor_sync(FULL, l[0], h);
-  lists.sums[warp][lane] = l[0];
-  sync_128();
+  own.sums[warp][lane] = l[0];
+  sync_128(x.engine);
   float scale = 1.f;                              // lane q: what query q's result is multiplied with
   if (lane < n) {
-    const float m = top[lane], sum = (lists.sums[0][lane] + lists.sums[1][lane]) + (lists.sums[2][lane] + lists.sums[3][lane]);
+    const float m = top[lane], sum = (own.sums[0][lane] + own.sums[1][lane]) + (own.sums[2][lane] + own.sums[3][lane]);
     if (last) {
       const float sink = a.sinks != nullptr ? a.sinks[w.head0 + lane] * LOG2E : -INFINITY;
-      const float both = fmaxf(m, sink), own = m > -INFINITY ? fast_exp2(m - both) : 0.f;
-      const float total = sum * own + (sink > -INFINITY ? fast_exp2(sink - both) : 0.f);
-      scale = sum != sum ? sum : total > 0.f || total != total ? own / total : 0.f;
+      const float both = fmaxf(m, sink), part = m > -INFINITY ? fast_exp2(m - both) : 0.f;
+      const float total = sum * part + (sink > -INFINITY ? fast_exp2(sink - both) : 0.f);
+      scale = sum != sum ? sum : total > 0.f || total != total ? part / total : 0.f;
     } else if (warp == 0 && at >= 0) {
       a.ml[at] = make_float2(m, sum);
     }
@@ -586,7 +596,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, Lists& lists, const Arg
 }
 
 template <int D>
-__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS)
+__global__ void __launch_bounds__(THREADS * Cfg<D>::ENGINES, 1)
 shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ Args a) {
   using C = Cfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -594,10 +604,13 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     if (threadIdx.x == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
     return;
   }
-  uint8_t *sQ = smem, *ring = smem + C::Q_BYTES + C::EXTRA;
-  Bars* bars = reinterpret_cast<Bars*>(ring + C::RING * C::SLOT);
-  Lists& lists = *reinterpret_cast<Lists*>(bars + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // the softmax's warps of all engines come first: a warp reads the quarter of tensor memory's lanes that its number in the CTA says
+  const int number = threadIdx.x >> 5, lane = threadIdx.x & 31, others = number - 4 * C::ENGINES;
+  const int engine = others < 0 ? number / 4 : others / 2, warp = others < 0 ? number % 4 : 4 + others % 2, tid = warp * 32 + lane;
+  uint8_t *sQ = smem + engine * C::ENGINE, *ring = sQ + C::Q_BYTES + C::EXTRA;
+  Own& own = reinterpret_cast<Own*>(smem + C::ENGINES * C::ENGINE)[engine];
+  Lists& lists = *reinterpret_cast<Lists*>(reinterpret_cast<Own*>(smem + C::ENGINES * C::ENGINE) + C::ENGINES);
+  Bars* bars = &own.bars;
   uint8_t *w_keys = ring, *w_values = ring + C::W_SLOTS * C::W_TILE, *w_weights = sQ + 2 * C::W_Q;
   if (tid == 0) {
     for (int i = 0; i < 8; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
@@ -614,24 +627,26 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     fence_proxy_async();
   }
   griddep_launch();                               // (the second kernel's CTAs come as these end; they wait for all of this grid)
-  if (warp == TMA_WARP && lane == 0) { tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
-  if (!make_lists(lists, bars, a, tid, warp, lane)) {
+  if (warp == TMA_WARP && lane == 0 && engine == 0) { tma_prefetch_desc(&tk); tma_prefetch_desc(&tv); }
+  const int engines = static_cast<int>(gridDim.x) * C::ENGINES;
+  if (!make_lists<THREADS * C::ENGINES>(lists, a, engines)) {
     if (blockIdx.x == gridDim.x - 1)              // (the second kernel finds that there is nothing)
-      for (int i = tid; i < 2 * a.rows; i += THREADS) a.plan[i] = make_int4(0, 0, 0, 0);
+      for (int i = threadIdx.x; i < 2 * a.rows; i += blockDim.x) a.plan[i] = make_int4(0, 0, 0, 0);
     return;
   }
-  if (warp == MMA_WARP) { tmem_alloc(&bars->tmem, C::TM_COLS); tmem_relinquish(); }
+  if (warp == MMA_WARP && engine == 0) { tmem_alloc(&lists.tmem, C::ENGINES * C::TM_COLS); tmem_relinquish(); }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = lists.tmem + engine * C::TM_COLS;
   volatile int* abort_flag = &bars->abort_flag;
-  // this CTA's kind, number among those of its kind, and units
-  const int before = static_cast<int>(static_cast<long long>(blockIdx.x) * lists.tall_ctas / gridDim.x);
-  const bool tall = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * lists.tall_ctas / gridDim.x) > before;
-  const int cta = tall ? before : static_cast<int>(blockIdx.x) - before;
-  const int units = tall ? lists.tall_units : lists.wide_units, per = tall ? lists.tall_per_cta : lists.wide_per_cta;
-  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(cta) * per)), u1 = min(units, u0 + per);
+  // this engine's kind, number among those of its kind, and units.  (A CTA's two are of one kind but in one CTA at most: of two kinds, each pushes the other's code out of the SM's
+  // instruction cache.  Where there are CTAs enough, only one of each has work)
+  const int place = lists.apart ? engine * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * C::ENGINES + engine;
+  const bool tall = place < lists.tall_engines;
+  const int at = tall ? place : place - lists.tall_engines;
+  const int units = tall ? lists.tall_units : lists.wide_units, per = tall ? lists.tall_each : lists.wide_each;
+  const int u0 = static_cast<int>(min(static_cast<long long>(units), static_cast<long long>(at) * per)), u1 = min(units, u0 + per);
   bool ok = true;
   // pool row of the box of tokens that holds `key`, by a row's table
   auto pool_row = [&](int row, int key) -> int {
@@ -669,16 +684,16 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
             if (!ok) break;
             if (lane == 0) {
-              if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
-              next_list<true>(lists.item[list & 1], lists, a, u0, u1, list == 0);
+              if (list > 0) own.item[list & 1] = own.item[(list & 1) ^ 1];
+              next_list<true>(own.item[list & 1], lists, a, u0, u1, list == 0);
               mbar_arrive(&bars->list_full[list & 1]);
             }
             __syncwarp();
-            tiles = lists.item[list & 1].tiles;
+            tiles = own.item[list & 1].tiles;
             j = 0;
             if (tiles == 0) { total = t; continue; }
           }
-          const Item& w = lists.item[list & 1];
+          const Item& w = own.item[list & 1];
           const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
           const bool any = lane * a.box < BN && w.keys.meets(key, a.box);
           const int row = any ? pool_row(w.row, key) : 0;
@@ -686,8 +701,8 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           if (t & 1) { row1 = row; lanes1 = lanes; hk1 = w.hk; } else { row0 = row; lanes0 = lanes; hk0 = w.hk; }
           ++j;
         }
-        const int at = what == 1 ? t : t - 2, slot = at % C::HALF, bar = 4 * (1 - what) + slot;
-        ok = wait(&bars->empty[bar], ((at / C::HALF) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+        const int nth = what == 1 ? t : t - 2, slot = nth % C::HALF, bar = 4 * (1 - what) + slot;
+        ok = wait(&bars->empty[bar], ((nth / C::HALF) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
         if (!ok) break;
         load(what == 1 ? &tk : &tv, ring + (slot + (what == 1 ? 0 : C::HALF)) * C::SLOT, BN, &bars->full[bar], t & 1 ? row1 : row0, t & 1 ? lanes1 : lanes0, t & 1 ? hk1 : hk0);
       }
@@ -724,7 +739,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         ++list;
         ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
-        tiles = lists.item[list & 1].tiles;
+        tiles = own.item[list & 1].tiles;
         if (tiles == 0) { total = t; continue; }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
@@ -759,7 +774,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll 1
     for (int t = 0, list = 0;; ++list) {
       // all scores of the lists before are made: the next one's queries may take the place of theirs
-      const Item& w = lists.item[list & 1];
+      const Item& w = own.item[list & 1];
       ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
       if (!ok) break;
       const int tiles = w.tiles;
@@ -894,9 +909,9 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       // (a piece of a list goes to a place of the CTA's)
       to = nullptr;
       if (one >= 0) {
-        const long long at = tiles == w.units ? one : 2ll * a.rows * a.heads + static_cast<long long>(2 * cta + (w.from == 0 ? 1 : 0)) * BM + tid;
-        a.ml[at] = make_float2(m, l);
-        to = a.acc + at * D;
+        const long long where = tiles == w.units ? one : 2ll * a.rows * a.heads + static_cast<long long>(2 * at + (w.from == 0 ? 1 : 0)) * BM + tid;
+        a.ml[where] = make_float2(m, l);
+        to = a.acc + where * D;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
@@ -914,18 +929,18 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
         if (!ok) break;
         if (lane == 0) {
-          if (list > 0) lists.item[list & 1] = lists.item[(list & 1) ^ 1];
-          next_list<false>(lists.item[list & 1], lists, a, u0, u1, list == 0);
+          if (list > 0) own.item[list & 1] = own.item[(list & 1) ^ 1];
+          next_list<false>(own.item[list & 1], lists, a, u0, u1, list == 0);
         }
         __syncwarp();
-        tiles = lists.item[list & 1].tiles;
+        tiles = own.item[list & 1].tiles;
         j = 0;
         if (tiles == 0) {
           if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
           break;
         }
       }
-      const Item& w = lists.item[list & 1];
+      const Item& w = own.item[list & 1];
       const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
       const bool any = lane * a.box < WK && w.keys.meets(key, a.box);
       const int row = any ? pool_row(w.row, key) : 0;
@@ -954,8 +969,8 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         ++list;
         ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
-        tiles = lists.item[list & 1].tiles;
-        more = lists.item[list & 1].n > 16;
+        tiles = own.item[list & 1].tiles;
+        more = own.item[list & 1].n > 16;
         j = 0;
         if (tiles == 0) total = t;
       }
@@ -1000,37 +1015,37 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
   } else {
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
-    const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, bars, abort_flag, tid, warp, lane, cta};
+    const Wide x{tmem + lane_addr, tmem + lane_addr + C::TM_WO, w_weights, w_values, &own, abort_flag, tid, warp, lane, engine, at};
 #pragma unroll 1
     for (int t = 0, list = 0;; ++list) {
       const int q = list & 1;
       ok = wait(&bars->list_full[q], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
-      if (any_of_128(!ok)) break;                 // (all warps or none)
-      const Item& w = lists.item[q];              // (not a copy: the registers are for scores)
+      if (any_of_128(!ok, engine)) break;                 // (all warps or none)
+      const Item& w = own.item[q];              // (not a copy: the registers are for scores)
       if (w.tiles == 0) break;
       ok = w.n <= 8 ? wide_list<D, 8>(x, lists, a, w, t) : w.n <= 16 ? wide_list<D, 16>(x, lists, a, w, t) : wide_list<D, 32>(x, lists, a, w, t);
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->list_empty[q]);
     }
   }
-  if (blockIdx.x == gridDim.x - 1) write_plan(lists, a, tid);
+  if (blockIdx.x == gridDim.x - 1) write_plan(lists, a);
   tc_fence_before();
   __syncthreads();
-  if (warp == MMA_WARP) {
+  if (warp == MMA_WARP && engine == 0) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::TM_COLS);
+    tmem_dealloc(tmem, C::ENGINES * C::TM_COLS);
   }
 }
 
 // A CTA a (place, key head), a warp a query: the pieces of its group's list and of its row's.  Bound by latency: what does not come from the first kernel is read before it ends.
 template <int D>
-__global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a, int ctas) {
+__global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant__ Args a, int engines) {
   constexpr int EACH = D / 32;                    // a lane's neighbouring columns
   const int place = blockIdx.x, hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row = a.order[place];
   const bool there = row >= 0 && row < a.rows, rests = !there || a.lengths[row] <= 0;
-  const long long all = static_cast<long long>(a.rows) * a.heads, wide0 = 2 * all + static_cast<long long>(ctas) * 2 * BM;
+  const long long all = static_cast<long long>(a.rows) * a.heads, wide0 = 2 * all + static_cast<long long>(engines) * 2 * BM;
   float sink = a.sinks != nullptr && warp < a.ratio ? a.sinks[hk * a.ratio + warp] * LOG2E : -INFINITY;
   griddep_wait();
   if (!there) return;
@@ -1049,7 +1064,7 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant_
     for (int k = 0; k < 2; ++k) {
       const int n = rests ? 0 : k == 0 ? lists.y : lists.w;
       if (n == 0) continue;
-      // the list's first tile in its sequence, units a CTA, the queries' places in a CTA's piece
+      // the list's first tile in its sequence, units an engine, the queries' places in an engine's piece
       int start, per, step;
       long long at;
       if (k == 0) {
@@ -1069,8 +1084,8 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant_
       finished = k == 1 && lists.y == 0 && c0 == c1;
       if (finished) break;
 #pragma unroll 2
-      for (int cta = c0; cta <= c1; ++cta) {
-        const long long from = c0 == c1 ? k * all + one : at + (2ll * cta + (cta == c0 ? 1 : 0)) * step;
+      for (int c = c0; c <= c1; ++c) {
+        const long long from = c0 == c1 ? k * all + one : at + (2ll * c + (c == c0 ? 1 : 0)) * step;
         const float2 ml = a.ml[from];
         float v[EACH];
         const float* p = a.acc + from * D + lane * EACH;
@@ -1115,21 +1130,24 @@ int multiprocessors() {
   return n[dev];
 }
 
+static bool room_allowed[3][64];                  // whether a device has been asked for the first kernel's shared memory
+
 template <int D>
-int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas, cudaStream_t stream) {
+int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int engines, cudaStream_t stream) {
   using C = Cfg<D>;
-  static_assert(sizeof(Bars) % 16 == 0 && alignof(Lists) == 16 && offsetof(Lists, top) % 16 == 0, "the maxima are read four at a time");
-  constexpr int SMEM = C::Q_BYTES + C::EXTRA + C::RING * C::SLOT + static_cast<int>(sizeof(Bars) + sizeof(Lists));
-  static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "over an SM's shared memory");
-  static bool allowed[64] = {};                  // (once for a device)
+  static_assert(sizeof(Own) % 16 == 0 && alignof(Own) == 16 && offsetof(Own, top) % 16 == 0 && C::ENGINE % 1024 == 0, "the maxima are read four at a time");
+  constexpr int SMEM = C::ENGINES * (C::ENGINE + static_cast<int>(sizeof(Own))) + static_cast<int>(sizeof(Lists));
+  static_assert(SMEM <= 227 * 1024, "over an SM's shared memory");
+  if (engines % C::ENGINES != 0) return -3;
+  constexpr int kind = D == 64 ? 0 : D == 128 ? 1 : 2;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev >= 64 || !allowed[dev]) {
+  if (dev >= 64 || !room_allowed[kind][dev]) {
     if ((e = cudaFuncSetAttribute(shared_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) != cudaSuccess) return static_cast<int>(e);
-    if (dev < 64) allowed[dev] = true;
+    if (dev < 64) room_allowed[kind][dev] = true;
   }
-  shared_mma_kernel<D><<<ctas, THREADS, SMEM, stream>>>(tk, tv, a);
+  shared_mma_kernel<D><<<engines / C::ENGINES, THREADS * C::ENGINES, SMEM, stream>>>(tk, tv, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return static_cast<int>(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.rows, a.kv_heads);
@@ -1140,25 +1158,25 @@ int launch(const CUtensorMap& tk, const CUtensorMap& tv, const Args& a, int ctas
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, join_pieces_kernel<D>, a, ctas));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, join_pieces_kernel<D>, a, engines));
 }
 
 }  // namespace sharedmma
 }  // namespace dewb
 
-// CTAs of the first kernel on the current device.
-extern "C" int dewb_shared_mma_ctas(int D) { return dewb::sharedmma::multiprocessors() * (D == 256 ? 1 : 2); }
+// Engines of the first kernel on the current device.
+extern "C" int dewb_shared_mma_engines(int D) { return dewb::sharedmma::multiprocessors() * (D == 256 ? 1 : 2); }
 
 // As dewb_shared_decode, on the tensor cores: bf16, D 64, 128 or 256, page_size a multiple of 16, up to 448 rows and as many groups, everything 16-byte aligned and q_stride a
-// multiple of 8.  acc: (2 rows heads + 320 ctas) D floats; ml: as many pairs; plan: 8 rows integers on a 16-byte boundary.  A CTA takes at least `least` tiles of 128 keys.  Two launches.
+// multiple of 8.  acc: (2 rows heads + 320 engines) D floats; ml: as many pairs; plan: 8 rows integers on a 16-byte boundary.  An engine takes at least `least` tiles of 128 keys; engines: as dewb_shared_mma_engines has it.  Two launches.
 extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const void* k, const void* v, const int* table, const int* lengths, const int* order, const int* first,
                                       const int* tokens, const float* sinks, float* acc, void* ml, void* plan, void* out, int rows, int heads, int kv_heads, int D, int page_size,
-                                      int max_pages, int pages, int groups, int window, int least, int ctas, float scale, float cap, int* err, void* stream_ptr) {
+                                      int max_pages, int pages, int groups, int window, int least, int engines, float scale, float cap, int* err, void* stream_ptr) {
   using namespace dewb::sharedmma;
   if (rows <= 0) return 0;
   const long long most = static_cast<long long>(max_pages) * page_size, chunks = heads > 0 && kv_heads > 0 ? (heads / kv_heads + WN - 1) / WN : 1;
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || page_size <= 0 || page_size % 16 != 0 || max_pages <= 0 || pages <= 0 || groups <= 0 || groups > MOST_ROWS ||
-      rows > MOST_ROWS || window < 0 || least < 1 || ctas < 1 || most > 0x3fffffffll || static_cast<long long>(pages) * page_size > 0x7fffff00ll || kv_heads > 65535 ||
+      rows > MOST_ROWS || window < 0 || least < 1 || engines < 1 || most > 0x3fffffffll || static_cast<long long>(pages) * page_size > 0x7fffff00ll || kv_heads > 65535 ||
       (2ll * rows * chunks + groups) * kv_heads * ((most + BN - 1) / BN + 1 + TALL_GAP) > 0x3fffffffll || q_stride % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(acc) |
         reinterpret_cast<uintptr_t>(plan)) & 15))
@@ -1172,8 +1190,8 @@ extern "C" int dewb_shared_decode_mma(const void* q, long long q_stride, const v
   const Args a{reinterpret_cast<const __nv_bfloat16*>(q), q_stride, table, lengths, order, first, tokens, sinks, reinterpret_cast<__nv_bfloat16*>(out), acc,
                reinterpret_cast<float2*>(ml), reinterpret_cast<int4*>(plan), rows, heads, kv_heads, heads / kv_heads, static_cast<int>(chunks), page_size, box, max_pages, pages, groups, window, least, scale * LOG2E, cap * LOG2E, err};
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  if (D == 64) return launch<64>(tk, tv, a, ctas, stream);
-  if (D == 128) return launch<128>(tk, tv, a, ctas, stream);
-  if (D == 256) return launch<256>(tk, tv, a, ctas, stream);
+  if (D == 64) return launch<64>(tk, tv, a, engines, stream);
+  if (D == 128) return launch<128>(tk, tv, a, engines, stream);
+  if (D == 256) return launch<256>(tk, tv, a, engines, stream);
   return -3;
 }

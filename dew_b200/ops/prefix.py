@@ -68,16 +68,16 @@ def shared_decode_reference(q, k, v, table, lengths, scale, window=None, softcap
     return torch.einsum("rghn,rngd->rghd", p, vr).reshape(R, H, D).to(q.dtype)
 
 
-LEAST_TILES = 2          # 128-key tiles that a CTA of the tensor cores' kernel takes at least
+LEAST_TILES = 2          # 128-key tiles that an engine of the tensor cores' kernel takes at least
 MOST_ROWS = 448          # rows, and groups, that its lists hold
-_CTAS: Dict[Tuple[int, int], int] = {}
+_ENGINES: Dict[Tuple[int, int], int] = {}
 
 
-def _ctas(lib, device, D: int) -> int:
+def _engines(lib, device, D: int) -> int:
     key = (device.index or 0, D)
-    if key not in _CTAS:
-        _CTAS[key] = lib.dewb_shared_mma_ctas(ctypes.c_int(D))
-    return _CTAS[key]
+    if key not in _ENGINES:
+        _ENGINES[key] = lib.dewb_shared_mma_engines(ctypes.c_int(D))
+    return _ENGINES[key]
 
 
 def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: int, groups: int) -> bool:
@@ -164,13 +164,13 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     numbers = (table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks))
     err, stream = L.status(q.device).data_ptr(), L.stream()
     if on_tensor_cores(q, k, v, columns, groups):
-        ctas = _ctas(lib, q.device, D)
-        rows = 2 * R * H + 320 * ctas
+        engines = _engines(lib, q.device, D)
+        rows = 2 * R * H + 320 * engines
         # one piece of scratch a call: sums, maxima and sums of weights, the plan
         scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
         at = scratch.data_ptr()
         L.check(lib.dewb_shared_decode_mma(q.data_ptr(), strides[0] if R > 1 else H * D, k.data_ptr(), v.data_ptr(), *numbers, at, at + 4 * rows * D, at + 4 * rows * (D + 2),
-                                           out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, ctas, scale, softcap, err, stream), "shared_decode_mma")
+                                           out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, engines, scale, softcap, err, stream), "shared_decode_mma")
         L.count_launches(2)
         return out
     splits = max(1, min(32, -(-columns * page // 512)))
