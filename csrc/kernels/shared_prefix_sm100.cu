@@ -236,10 +236,10 @@ __device__ __forceinline__ int query(const Lists& s, const Args& a, const Item& 
 }
 
 // A warp's up to 32 queries (lane i holds query()'s answer for number i) to rows of 128 bytes (128-byte swizzle), 64-column pieces `apart` bytes apart; `to`: the first's row,
-// on a 1024-byte boundary.
-template <int D>
+// on a 1024-byte boundary.  EACH: 16-byte loads of a lane that are on their way at a time.
+template <int D, int EACH>
 __device__ __forceinline__ void fetch_queries(uint8_t* to, int apart, const Args& a, int mine, int n, int lane) {
-  constexpr int PIECES = D / 8, ROWS = 32 / PIECES, EACH = 4;
+  constexpr int PIECES = D / 8, ROWS = 32 / PIECES;
   const int row = mine / a.heads;
   const long long from = mine < 0 ? -1 : row * a.q_stride + static_cast<long long>(mine - row * a.heads) * D;
   const int c = lane % PIECES;
@@ -709,18 +709,20 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
     }
   } else if (tall && warp == MMA_WARP) {
-    // over the tiles of all lists: S(0) S(1) PV(0) S(2) PV(1) ... (the warp waits together, one lane issues)
+    // over the tiles of all lists: S(0) S(1) PV(0) S(2) PV(1) ..., but all of a list's products before the next one's scores, whose queries come when its softmax is done (the warp
+    // waits together, one lane issues)
     constexpr uint32_t idesc_qk = make_idesc(BM, BN, 1, 1, 0, 0);
     constexpr uint32_t idesc_pv = make_idesc(BM, D, 1, 1, 0, 1);
-    int list = -1, j = 0, tiles = 0, total = 0x3fffffff;
-    uint32_t fresh = 0;                           // (fresh: a bit for each buffer, whether its tile is its list's first)
+    int list = -1, j = 0, tiles = 0, pv = 0;
+    uint32_t fresh = 0;                           // (a bit for each buffer, whether its tile is its list's first)
     const uint32_t qa = smem_u32(sQ);
 #pragma unroll 1
-    for (int t = 0; ok && t < total + 2; ++t) {
-      const int b = t & 1;
-      if (t >= 2) {                               // PV(t - 2)
-        const int slot = (t - 2) % C::HALF;
-        ok = wait(&bars->full[4 + slot], ((t - 2) / C::HALF) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) && wait(&bars->p_full[b], ((t - 2) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+    for (int t = 0; ok; ++t) {
+      const bool begins = j == tiles;
+#pragma unroll 1
+      for (; pv < (begins ? t : t - 1); ++pv) {   // PV(pv)
+        const int b = pv & 1, slot = pv % C::HALF;
+        ok = wait(&bars->full[4 + slot], (pv / C::HALF) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) && wait(&bars->p_full[b], (pv >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
         tc_fence_after();
         const uint32_t va = smem_u32(ring + (C::HALF + slot) * C::SLOT);
@@ -734,14 +736,15 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         __syncwarp();
       }
-      if (t >= total) continue;
+      if (!ok) break;
+      const int b = t & 1;
       fresh &= ~(1u << b);
-      if (j == tiles) {
+      if (begins) {
         ++list;
         ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
         tiles = own.item[list & 1].tiles;
-        if (tiles == 0) { total = t; continue; }
+        if (tiles == 0) break;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
         ok = wait(&bars->q_full, list & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
@@ -782,7 +785,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       int one = -1;
       if (tiles > 0) {
         one = query(lists, a, w, tid);
-        fetch_queries<D>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
+        fetch_queries<D, D / 8 < 16 ? D / 8 : 16>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
         if (lane == 0) mbar_arrive(&bars->q_full);
       }
       if (list > 0) {
@@ -918,65 +921,107 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       if (lane == 0) mbar_arrive(&bars->list_empty[list & 1]);
     }
   } else if (warp == TMA_WARP) {
-    // K(0) V(0) K(1) V(1) ...
-    int list = -1, j = 0, tiles = 0;
+    // K(0) V(0) K(1) V(1) ...; a tile's pages are looked up while the values of the one before wait for their slot, unless that would wait for an item's room
+    int list = -1, j = 0, tiles = 0, row = 0, hk = 0;
+    unsigned lanes = 0;
+    bool begins = true, more = true;
 #pragma unroll 1
-    for (int t = 0; ok; ++t, ++j) {
-      const bool begins = j == tiles;
-      const int slot = t % C::W_SLOTS;
+    for (int t = -1; ok && more; ++t) {
+      const int slot = t % C::W_SLOTS, row_v = row, hk_v = hk;
       const uint32_t phase = ((t / C::W_SLOTS) & 1) ^ 1;
-      if (begins) {
-        ++list;
-        ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+      const unsigned lanes_v = lanes;
+      if (t >= 0) {
+        ok = wait(&bars->empty[slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
         if (!ok) break;
-        if (lane == 0) {
-          if (list > 0) own.item[list & 1] = own.item[(list & 1) ^ 1];
-          next_list<false>(own.item[list & 1], lists, a, u0, u1, list == 0);
-        }
-        __syncwarp();
-        tiles = own.item[list & 1].tiles;
-        j = 0;
-        if (tiles == 0) {
+        load(&tk, w_keys + slot * C::W_TILE, WK, &bars->full[slot], row, lanes, hk);
+        if (begins) {
+          const Item& w = own.item[list & 1];
+          fetch_queries<D, 8>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
           if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
-          break;
         }
       }
-      const Item& w = own.item[list & 1];
-      const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
-      const bool any = lane * a.box < WK && w.keys.meets(key, a.box);
-      const int row = any ? pool_row(w.row, key) : 0;
-      const unsigned lanes = __ballot_sync(FULL, any);
+      const int next = list + 1;
+      const bool early = j < tiles || __all_sync(FULL, mbar_try_wait(&bars->list_empty[next & 1], ((next >> 1) & 1) ^ 1));
 #pragma unroll 1
-      for (int what = 0; what < 2 && ok; ++what) {                 // keys, values
-        ok = wait(&bars->empty[4 * what + slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
-        if (!ok) break;
-        load(what == 0 ? &tk : &tv, (what == 0 ? w_keys : w_values) + slot * C::W_TILE, WK, &bars->full[4 * what + slot], row, lanes, w.hk);
-        if (what == 0 && begins) {
-          fetch_queries<D>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
-          if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
+      for (int what = 0; what < 2 && ok; ++what) {
+        if (early != (what == 0)) {               // the values
+          if (t < 0) continue;
+          ok = wait(&bars->empty[4 + slot], phase, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+          if (ok) load(&tv, w_values + slot * C::W_TILE, WK, &bars->full[4 + slot], row_v, lanes_v, hk_v);
+          continue;
         }
+        begins = j == tiles;                      // the next tile
+        if (begins) {
+          list = next;
+          ok = wait(&bars->list_empty[list & 1], ((list >> 1) & 1) ^ 1, abort_flag, a.err, ERR_WAIT_EMPTY, lane);
+          if (!ok) break;
+          if (lane == 0) {
+            if (list > 0) own.item[list & 1] = own.item[(list & 1) ^ 1];
+            next_list<false>(own.item[list & 1], lists, a, u0, u1, list == 0);
+          }
+          __syncwarp();
+          tiles = own.item[list & 1].tiles;
+          j = 0;
+          if (tiles == 0) {
+            more = false;
+            if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
+            continue;
+          }
+        }
+        const Item& w = own.item[list & 1];
+        const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
+        const bool any = lane * a.box < WK && w.keys.meets(key, a.box);
+        row = any ? pool_row(w.row, key) : 0;
+        lanes = __ballot_sync(FULL, any);
+        hk = w.hk;
+        ++j;
       }
     }
   } else if (warp == MMA_WARP) {
-    // S(0) S(1) PV(0) S(2) PV(1) ...
+    // S(0) S(1) PV(0) S(2) PV(1) ..., but a list's last products before the next one's scores
     constexpr uint32_t idesc_s[2] = {make_idesc(WK, 16, 1, 1, 0, 0), make_idesc(WK, 32, 1, 1, 0, 0)};
     constexpr uint32_t idesc_o[2] = {make_idesc(128, 16, 1, 1, 1, 0), make_idesc(128, 32, 1, 1, 1, 0)};
-    int list = -1, j = 0, tiles = 0, total = 0x3fffffff;
-    bool more = false;                            // than 16 queries
+    int list = -1, j = 0, tiles = 0;
+    bool more = false, over = false;              // (more: than 16 queries)
     uint32_t flags = 0;                           // bits b: whether the tile in buffer b is its list's first, 2 + b: whether its list has more than 16 queries
 #pragma unroll 1
-    for (int t = 0; ok && t <= total; ++t) {
-      if (j == tiles && t < total) {
-        ++list;
-        ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
-        if (!ok) break;
-        tiles = own.item[list & 1].tiles;
-        more = own.item[list & 1].n > 16;
-        j = 0;
-        if (tiles == 0) total = t;
-      }
-      if (t < total) {                            // S(t)
-        const int b = t & 1, slot = t % C::W_SLOTS;
+    for (int t = 0; ok && !over; ++t) {
+      const bool begins = j == tiles;
+#pragma unroll 1
+      for (int what = 0; what < 2 && ok; ++what) {
+        if (begins == (what == 0)) {              // PV(t - 1)
+          if (t == 0) continue;
+          const int b = (t - 1) & 1, slot = (t - 1) % C::W_SLOTS;
+          ok = wait(&bars->full[4 + slot], ((t - 1) / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) &&
+               wait(&bars->p_full[b], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = smem_u32(w_values + slot * C::W_TILE), pa = smem_u32(w_weights + b * C::W_P);
+          const uint32_t idesc = flags >> (2 + b) & 1 ? idesc_o[1] : idesc_o[0], add = flags >> b & 1 ? 0u : 1u;
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < C::HALVES; ++h)
+#pragma unroll
+              for (int kk = 0; kk < WK / 16; ++kk)  // (a head of 64 fills half of the rows: the others are of whatever follows)
+                umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
+                             make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
+            umma_commit(&bars->done);
+            umma_commit(&bars->empty[4 + slot]);
+          }
+          __syncwarp();
+          continue;
+        }
+        if (begins) {
+          ++list;
+          ok = wait(&bars->list_full[list & 1], (list >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+          if (!ok) break;
+          tiles = own.item[list & 1].tiles;
+          more = own.item[list & 1].n > 16;
+          j = 0;
+          over = tiles == 0;
+          if (over) break;
+        }
+        const int b = t & 1, slot = t % C::W_SLOTS;                // S(t)
         flags = (flags & ~(5u << b)) | ((j == 0 ? 1u : 0u) | (more ? 4u : 0u)) << b;
         ++j;
         ok = wait(&bars->full[slot], (t / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane);
@@ -994,25 +1039,6 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         }
         __syncwarp();
       }
-      if (t == 0) continue;
-      const int b = (t - 1) & 1, slot = (t - 1) % C::W_SLOTS;      // PV(t - 1)
-      ok = wait(&bars->full[4 + slot], ((t - 1) / C::W_SLOTS) & 1, abort_flag, a.err, ERR_WAIT_FULL, lane) &&
-           wait(&bars->p_full[b], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t va = smem_u32(w_values + slot * C::W_TILE), pa = smem_u32(w_weights + b * C::W_P);
-      const uint32_t idesc = flags >> (2 + b) & 1 ? idesc_o[1] : idesc_o[0], add = flags >> b & 1 ? 0u : 1u;
-      if (elect_one()) {
-#pragma unroll
-        for (int h = 0; h < C::HALVES; ++h)
-#pragma unroll
-          for (int kk = 0; kk < WK / 16; ++kk)    // (a head of 64 fills half of the rows: the others are of whatever follows)
-            umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
-                         make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
-        umma_commit(&bars->done);
-        umma_commit(&bars->empty[4 + slot]);
-      }
-      __syncwarp();
     }
   } else {
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
