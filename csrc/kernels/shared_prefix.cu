@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
   float* sk = sq + QUERIES * D;                          // [KEYS][D + 1]
   float* sv = sk + KEYS * wide;                          // [KEYS][D]
   float* sp = sv + KEYS * D;                             // [QUERIES][KEYS]
-  __shared__ long long stok[KEYS];
+  __shared__ long long stok[2][KEYS];                    // where keys stand in the pools (-1: nowhere), of this tile and the next one
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ratio = a.heads / a.kv_heads, chunks = (ratio + QUERIES - 1) / QUERIES;
   const int at = blockIdx.x, hk = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
@@ -115,34 +115,39 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
     }
   const int* table = a.table + static_cast<long long>(through) * a.max_pages;
   const float scale2 = a.scale * 1.4426950408889634f, cap2 = a.cap * 1.4426950408889634f;
-  for (int k0 = from; k0 < to; k0 += KEYS) {
+  auto look_up = [&](int k0, int b) {                    // (a thread a key)
+    const int x = first + k0 + tid, key = x < gap ? x : x + skip;
+    long long tok = -1;
+    if (k0 + tid < to) {
+      const int page = table[key / a.page_size];
+      if (page >= 0 && page < a.pages) tok = static_cast<long long>(page) * a.page_size + key % a.page_size;
+      else atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+    }
+    stok[b][tid] = tok;
+  };
+  if (tid < KEYS) look_up(from, 0);
+  int b = 0;
+  for (int k0 = from; k0 < to; k0 += KEYS, b ^= 1) {
     __syncthreads();
-    if (tid < KEYS) {
-      const int x = first + k0 + tid, key = x < gap ? x : x + skip;
-      long long tok = -1;
-      if (k0 + tid < to) {
-        const int page = table[key / a.page_size];
-        if (page >= 0 && page < a.pages) tok = static_cast<long long>(page) * a.page_size + key % a.page_size;
-        else atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+    if (tid < KEYS && k0 + KEYS < to) look_up(k0 + KEYS, b ^ 1);
+    // a warp every fourth key, a lane every 32nd column: eight keys' loads are on their way at a time
+    for (int d = lane; d < D; d += 32) {
+      float kx[KEYS / WARPS], vx[KEYS / WARPS];
+#pragma unroll
+      for (int e = 0; e < KEYS / WARPS; ++e) {
+        const long long tok = stok[b][e * WARPS + warp], x = (tok * a.kv_heads + hk) * D + d;
+        kx[e] = tok >= 0 ? as_float(static_cast<const TP*>(a.k)[x]) : 0.f;
+        vx[e] = tok >= 0 ? as_float(static_cast<const TP*>(a.v)[x]) : 0.f;
+        if (SCALED && tok >= 0) { kx[e] *= a.k_scale[tok * a.kv_heads + hk]; vx[e] *= a.v_scale[tok * a.kv_heads + hk]; }
       }
-      stok[tid] = tok;
+#pragma unroll
+      for (int e = 0; e < KEYS / WARPS; ++e) {
+        sk[(e * WARPS + warp) * wide + d] = kx[e];
+        sv[(e * WARPS + warp) * D + d] = vx[e];
+      }
     }
     __syncthreads();
-    for (int i = tid; i < KEYS * D; i += THREADS) {
-      const int j = i / D, d = i - j * D;
-      const long long tok = stok[j];
-      float kx = 0.f, vx = 0.f;
-      if (tok >= 0) {
-        const long long x = (tok * a.kv_heads + hk) * D + d;
-        kx = as_float(static_cast<const TP*>(a.k)[x]);
-        vx = as_float(static_cast<const TP*>(a.v)[x]);
-        if (SCALED) { kx *= a.k_scale[tok * a.kv_heads + hk]; vx *= a.v_scale[tok * a.kv_heads + hk]; }
-      }
-      sk[j * wide + d] = kx;
-      sv[i] = vx;
-    }
-    __syncthreads();
-    const bool seen = stok[lane] >= 0;
+    const bool seen = stok[b][lane] >= 0;
     float s[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) s[i] = 0.f;

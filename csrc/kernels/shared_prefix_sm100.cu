@@ -65,8 +65,8 @@ struct Cfg {
   static constexpr int ENGINE = Q_BYTES + EXTRA + RING * SLOT;                 // bytes
 };
 
-struct Ranges {                                   // the keys of a list, [a0, a1) and [b0, b1), and its tiles of N
-  int a0, a1, b0, b1;
+struct Ranges {                                   // the keys of a list, [a0, a1) and [b0, b1), counted from `base`, and its tiles of N
+  int a0, a1, b0, b1, base;
   template <int N> __device__ __forceinline__ int a_tiles() const { return a1 > a0 ? (a1 + N - 1) / N - a0 / N : 0; }
   template <int N> __device__ __forceinline__ int b_first() const { return a1 > a0 ? max(b0 / N, (a1 + N - 1) / N) : b0 / N; }
   template <int N> __device__ __forceinline__ int tiles() const { return a_tiles<N>() + (b1 > b0 ? max(0, (b1 + N - 1) / N - b_first<N>()) : 0); }
@@ -130,11 +130,16 @@ struct Args {
   int* err;
 };
 
-__device__ __forceinline__ Ranges own_ranges(int len, int window, int lo, int hi) {
-  if (len == 0) return Ranges{0, 0, 0, 0};
+// [a0, a1) and [b0, b1) counted from the box that the first of them begins in (so a row's first own tile is full: 64 rows of 500 keys behind 64 shared ones 62 us instead of 86)
+__device__ __forceinline__ Ranges ranges(int a0, int a1, int b0, int b1, int box) {
+  const int base = (a1 > a0 ? a0 : b0) & -box;     // (boxes are of 16, 32 or 64)
+  return a1 > a0 ? Ranges{a0 - base, a1 - base, b0 - base, b1 - base, base} : Ranges{0, 0, b0 - base, b1 - base, base};
+}
+__device__ __forceinline__ Ranges own_ranges(int len, int window, int lo, int hi, int box) {
+  if (len == 0) return Ranges{0, 0, 0, 0, 0};
   const int first = row_first(len, window);
-  if (hi == 0) return Ranges{first, len, 0, 0};
-  return Ranges{first, max(first, lo), hi, max(hi, len)};
+  if (hi == 0) return ranges(first, len, 0, 0, box);
+  return ranges(first, max(first, lo), hi, max(hi, len), box);
 }
 
 template <typename T>
@@ -193,14 +198,14 @@ __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, i
   }
   if (!same) {
     if (w.shared) {
-      w.keys = Ranges{s.lo[w.index], s.hi[w.index], 0, 0};
+      w.keys = ranges(s.lo[w.index], s.hi[w.index], 0, 0, a.box);
       w.lists = a.kv_heads * (TALL ? (group_queries(s, a, w.index) + BM - 1) / BM : 1);
       w.row = s.through[w.index];
       w.start = at[w.index] + GAP;
       w.units = w.keys.tiles<TALL ? BN : WK>();
     } else {
       const int g = s.group[w.index];
-      w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g]);
+      w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g], a.box);
       w.lists = a.kv_heads * a.chunks;
       w.row = s.row[w.index];
       w.start = s.wide_shared_units + s.own[w.index] * w.lists + GAP;
@@ -268,7 +273,7 @@ __device__ __forceinline__ void write_plan(const Lists& s, const Args& a) {
 #pragma unroll 1
   for (int i = threadIdx.x; i < a.rows; i += blockDim.x) {
     const int g = s.group[i], queries = group_queries(s, a, g);
-    const Ranges both{s.lo[g], s.hi[g], 0, 0};
+    const Ranges both = ranges(s.lo[g], s.hi[g], 0, 0, a.box);
     const bool tall = queries > WN;
     a.plan[2 * i] = make_int4(tall ? s.tall[g] : s.wide[g], tall ? both.tiles<BN>() : both.tiles<WK>(), s.wide_shared_units + s.own[i] * lists, max(s.own[i + 1] - s.own[i] - WIDE_GAP, 0));
     a.plan[2 * i + 1] = make_int4(s.first[g], tall ? queries : 0, s.tall_each, s.wide_each);
@@ -360,14 +365,14 @@ __device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines)
   for (int g = tid; g < a.groups; g += THREADS) {
     if (live[g] < 2 || s.lo[g] >= s.hi[g]) s.lo[g] = s.hi[g] = 0;
     const int queries = group_queries(s, a, g);
-    const Ranges both{s.lo[g], s.hi[g], 0, 0};
+    const Ranges both = ranges(s.lo[g], s.hi[g], 0, 0, a.box);
     s.tall[g + 1] = s.hi[g] == 0 || queries <= WN ? 0 : a.kv_heads * ((queries + BM - 1) / BM) * (both.tiles<BN>() + TALL_GAP);
     s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * (both.tiles<WK>() + WIDE_GAP);
   }
   __syncthreads();
 #pragma unroll 1
   for (int i = tid; i < a.rows; i += THREADS) {
-    const int n = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]]).tiles<WK>();
+    const int n = own_ranges(s.len[i], a.window, s.lo[s.group[i]], s.hi[s.group[i]], a.box).tiles<WK>();
     s.own[i + 1] = n == 0 ? 0 : n + WIDE_GAP;
   }
   __syncthreads();
@@ -697,7 +702,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           const Item& w = own.item[list & 1];
           const int key = w.keys.tile<BN>(w.from + j) * BN + lane * a.box;
           const bool any = lane * a.box < BN && w.keys.meets(key, a.box);
-          const int row = any ? pool_row(w.row, key) : 0;
+          const int row = any ? pool_row(w.row, w.keys.base + key) : 0;
           const unsigned lanes = __ballot_sync(FULL, any);
           if (t & 1) { row1 = row; lanes1 = lanes; hk1 = w.hk; } else { row0 = row; lanes0 = lanes; hk0 = w.hk; }
           ++j;
@@ -971,7 +976,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         const Item& w = own.item[list & 1];
         const int key = w.keys.tile<WK>(w.from + j) * WK + lane * a.box;
         const bool any = lane * a.box < WK && w.keys.meets(key, a.box);
-        row = any ? pool_row(w.row, key) : 0;
+        row = any ? pool_row(w.row, w.keys.base + key) : 0;
         lanes = __ballot_sync(FULL, any);
         hk = w.hk;
         ++j;

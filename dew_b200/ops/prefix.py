@@ -90,6 +90,11 @@ def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: 
             and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
 
 
+def _splits(most: int, lists: int) -> int:
+    """Parts of the keys in the kernel for other types: of 128 keys as long as there are no more than 2048 CTAs (rows times key heads times parts), then of 512."""
+    return max(1, min(32, -(-most // 128), max(-(-most // 512), 2048 // lists)))
+
+
 _POOLS = {torch.int8: 1, torch.float8_e4m3fn: 2}
 
 
@@ -173,7 +178,7 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
                                            out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, engines, scale, softcap, err, stream), "shared_decode_mma")
         L.count_launches(2)
         return out
-    splits = max(1, min(32, -(-columns * page // 512)))
+    splits = _splits(columns * page, R * G)
     parts = torch.empty(2 * splits * R * H * (D + 2), dtype=fp32, device=q.device)
     at = parts.data_ptr()
     one = 2 * splits * R * H * 4
