@@ -275,7 +275,7 @@ class KVStore:
         R, D, H, G = packed.shape[0], packed.shape[-1], heads.q, heads.kv
         out = torch.empty(R, H, D, dtype=packed.dtype, device=packed.device)
         factors = visible.gain is not None or visible.sigmoid is not None
-        if self._shares(packed[:, 0]) and not factors and not visible.keep and not visible.chunk:
+        if self._shares(packed[:, 0], slot) and not factors and not visible.keep and not visible.chunk:
             return prefix.shared_decode(packed[:, 0, :H], self.k[slot], self.v[slot], c.table, c.lengths, self.shared, scale, window=visible.window, softcap=visible.softcap,
                                         sinks=visible.sinks)
         if D == 128 and self.page_size % 64 == 0 and H // G <= 8 and hasattr(lib, "dewb_paged_decode_persist") and (R <= 1024 or not factors):
@@ -409,10 +409,15 @@ class KVStore:
         kept.copy_(now)
         self.shared = prefix.Shared(kept[:self.rows], kept[self.rows:2 * self.rows + 1], kept[2 * self.rows + 1:])
 
-    def _shares(self, q: torch.Tensor) -> bool:
-        """Whether a decode step with queries ``[rows, heads, dim]`` goes by what the rows share."""
-        return (self.shared is not None and self.row_ids is None and q.shape[0] == self.rows and q.shape[-1] <= 256 and q.dtype in (torch.bfloat16, torch.float32)
-                and (self.kind != 0 or q.dtype == self.dtype) and not (q.requires_grad and torch.is_grad_enabled()))
+    def _shares(self, q: torch.Tensor, layer: int) -> bool:
+        """Whether a decode step with queries ``[rows, heads, dim]`` goes by what the rows share: where the tensor cores' kernel takes it, and in fp32.  Quantised pools and
+        other widths are read sooner row by row (64 rows in groups of 8 behind 4096 tokens in int8: 340 us against 869)."""
+        if (self.shared is None or self.row_ids is not None or q.shape[0] != self.rows or q.shape[-1] > 256 or (q.requires_grad and torch.is_grad_enabled())
+                or (self.kind == 0 and q.dtype != self.dtype)):
+            return False
+        if not L.use_cuda(q):
+            return q.dtype in (torch.bfloat16, torch.float32)
+        return q.dtype == torch.float32 or prefix.on_tensor_cores(q, self.k[layer], self.v[layer], self.page_table.shape[1], self.rows)
 
     def fork_rows(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Give rows ``children`` what rows ``parents`` keep beside their pages (recurrent states, latents): the same list of parents may name a row several times."""
@@ -579,7 +584,7 @@ class KVStore:
         L.check(lib.dewb_rope_append(at(qkv), at(cos), at(sin), at(pos32), R, Hq, self.kv_heads, D, cos.shape[0] if cos is not None else 0, at(self.k[layer]),
                                      at(self.v[layer]), at(self.page_table), self.page_size, self.max_pages, L.stream()), "rope_append")
         sinks32 = None if sinks is None else sinks.detach().float().contiguous()      # referenced until the launch is enqueued
-        if self._shares(qkv):
+        if self._shares(qkv, layer):
             L.count_launches(1)
             return prefix.shared_decode(qkv[:, :Hq], self.k[layer], self.v[layer], self.page_table, lens32, self.shared, 1.0 / math.sqrt(D), window=window, sinks=sinks32)
         out = torch.empty((R, Hq, D), dtype=qkv.dtype, device=qkv.device)
@@ -608,7 +613,7 @@ class KVStore:
         """``q [R, Hq, D]`` against each row's first ``lengths[r]`` cached tokens -> ``[R, Hq, D]``."""
         R, Hq, D = q.shape
         scale = scale if scale is not None else 1.0 / math.sqrt(D)
-        if self._shares(q):
+        if self._shares(q, layer):
             return prefix.shared_decode(q, self.k[layer], self.v[layer], self.page_table, lengths.to(torch.int32).contiguous(), self.shared, scale, window=window, softcap=softcap,
                                         sinks=None if sinks is None else sinks.detach().float().contiguous(), k_scale=self.k_scale[layer] if self.kind else None,
                                         v_scale=self.v_scale[layer] if self.kind else None)
@@ -683,8 +688,10 @@ class KVStore:
         if total is None:
             total = int(positions.max()) + 1
         kc, vc = self.gather(layer, total, dtype=q.dtype)
-        # bottom-right aligned causal attention of the chunk against everything cached so far (rows share `start`)
-        return ops.attention_reference(q, kc, vc, causal=causal, window=window, softcap=softcap, sinks=sinks)
+        # bottom-right aligned causal attention of the chunk against everything cached so far (rows share `start`): without the padding that all rows end with
+        n = min(S, total - start)
+        out = ops.attention_reference(q[:, :n], kc, vc, causal=causal, window=window, softcap=softcap, sinks=sinks)
+        return out if n == S else torch.cat([out, out.new_zeros(R, S - n, *out.shape[2:])], 1)
 
 
 class PackedRows:

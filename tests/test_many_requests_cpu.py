@@ -172,3 +172,21 @@ def test_samples_with_adapters_over_shared_prefixes(monkeypatch):
         server.step()
         server.compact()
     assert [t.result() for t in got] == [t.result() for t in want] and len(other.result()) == 5
+
+
+def test_a_later_chunk_may_end_in_padding():
+    """A chunk behind a cached prefix, padded as a server pads it: its tokens see what they see without the padding."""
+    g = torch.Generator().manual_seed(0)
+    k, v, q = (torch.randn(2, 30, n, 16, generator=g) for n in (2, 2, 4))
+
+    def chunks(pad):
+        store = KVStore(KVCache(page_size=8), 1, 2, 64, 2, 16, dtype=torch.float32)
+        out = []
+        for a, b in ((0, 17), (17, 30)):
+            x = [torch.cat([t[:, a:b], torch.randn(2, pad, *t.shape[2:], generator=g)], 1) for t in (q, k, v)]
+            pos = torch.cat([torch.arange(a, b), torch.full((pad,), -1)])[None].expand(2, -1)
+            store.chunk_span = (a, b)
+            out.append(store.attend(0, *x, pos)[:, :b - a])
+        return torch.cat(out, 1)
+    want = chunks(0)
+    assert torch.allclose(chunks(5), want, atol=1e-6) and torch.allclose(chunks(40), want, atol=1e-6)
