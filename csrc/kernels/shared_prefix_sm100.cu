@@ -89,7 +89,8 @@ struct Item {
 struct alignas(16) Bars {
   uint64_t list_full[2], list_empty[2];           // what a list is about (wide: and its queries)
   uint64_t full[8], empty[8];                     // slots of the ring: [0, 4) keys, [4, 8) values
-  uint64_t q_full, s_full[2], p_full[2], done;
+  uint64_t q_full, s_full[2], p_full[2];
+  uint64_t done[2];                               // of even and odd tiles' products: whoever waits for tile t's knows that tile t - 2's are done, not that t - 1's are
   int abort_flag;
 };
 
@@ -507,7 +508,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, const Lists& lists, con
 #pragma unroll
         for (int q = 0; q < NC; ++q) l[q] *= by[q];
         // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
-        ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
+        ok = wait(&bars->done[(t - 1) & 1], ((t - 1) >> 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < C::HALVES * WN; c += 4) {
@@ -531,6 +532,8 @@ __device__ __forceinline__ bool wide_list(const Wide& x, const Lists& lists, con
     }
     if (__ballot_sync(FULL, !seen) != 0) {        // values that nobody sees, to zero (each thread its key's)
       const int slot = t % C::W_SLOTS;
+      // (the tile before may still wait for its values in the same slot: its products first)
+      if (t > 0) ok = wait(&bars->done[(t - 1) & 1], ((t - 1) >> 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
       ok = wait(&bars->full[4 + slot], (t / C::W_SLOTS) & 1, x.abort_flag, a.err, ERR_WAIT_FULL, lane) && ok;
       if (!seen) {
 #pragma unroll 1
@@ -578,7 +581,7 @@ __device__ __forceinline__ bool wide_list(const Wide& x, const Lists& lists, con
     }
   }
   __syncwarp();
-  ok = wait(&bars->done, (t - 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
+  ok = wait(&bars->done[(t - 1) & 1], ((t - 1) >> 1) & 1, x.abort_flag, a.err, ERR_WAIT_OTHER, lane) && ok;
   tc_fence_after();
 #pragma unroll 1
   for (int c = 0; c < C::HALVES * WN; c += 4) {
@@ -623,11 +626,11 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->done[i], 1);
       mbar_init(&bars->list_full[i], 1);
       mbar_init(&bars->list_empty[i], 5);         // (the tensor cores' warp, and the softmax's four)
     }
     mbar_init(&bars->q_full, 4);
-    mbar_init(&bars->done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async();
@@ -736,7 +739,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
             umma_bf16_ts(tmem + C::TM_O, tmem + b * BN + kk * 8, make_sdesc_sw128(va + kk * 2048, BN * 128, 1024), idesc_pv, kk > 0 ? 1u : add);
-          umma_commit(&bars->done);
+          umma_commit(&bars->done[b]);
           umma_commit(&bars->empty[4 + slot]);
         }
         __syncwarp();
@@ -794,7 +797,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         if (lane == 0) mbar_arrive(&bars->q_full);
       }
       if (list > 0) {
-        ok = wait(&bars->done, (t - 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+        ok = wait(&bars->done[(t - 1) & 1], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
         if (!ok) break;
         tc_fence_after();
         if (active) {
@@ -859,7 +862,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
             if (need) { m = m_new; l *= by; }
             if (j > 0) {
               // (the scores of this tile were behind the products before the last ones: those are all that may still be under way)
-              ok = wait(&bars->done, (t - 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
+              ok = wait(&bars->done[(t - 1) & 1], ((t - 1) >> 1) & 1, abort_flag, a.err, ERR_WAIT_OTHER, lane);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll 1
@@ -1010,7 +1013,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
               for (int kk = 0; kk < WK / 16; ++kk)  // (a head of 64 fills half of the rows: the others are of whatever follows)
                 umma_bf16_ss(tmem + C::TM_WO + h * WN, make_sdesc_sw128(va + h * 2 * (WK * 128) + kk * 2048, D == 64 ? WK * 64 : WK * 128, 1024),
                              make_sdesc_sw128(pa + (kk >> 2) * (WN * 128) + (kk & 3) * 32, 16, 1024), idesc, kk > 0 ? 1u : add);
-            umma_commit(&bars->done);
+            umma_commit(&bars->done[b]);
             umma_commit(&bars->empty[4 + slot]);
           }
           __syncwarp();

@@ -124,3 +124,29 @@ def test_large_scores_and_values(dtype):
     check({**a, "scale": 0.0})
     check({**a, "k": a["k"] * 1e4, "q": a["q"] * 1e-4})
     check({**a, "v": a["v"] * 2.0 ** 60})
+
+
+# enough work for every SM, lists that begin in one place and end in another, values that come late (nothing of the pools is in the cache): rows of 50 to 400 own keys
+def _many(rows, *shared):
+    per = rows // len(shared)
+    return [(n, [50 + (i * 37 + 11 * g) % 350 for i in range(per)]) for g, n in enumerate(shared)]
+
+
+@pytest.mark.parametrize("groups, heads, kv, dim, page, window, softcap, sinks", [
+    (_many(96, 2500), 16, 4, 128, 64, None, 0.0, False),                       # queries of many rows
+    (_many(96, *[600 + 64 * i for i in range(12)]), 16, 4, 128, 16, None, 0.0, True),      # of eight
+    (_many(90, 1000, 64, 2100), 40, 8, 64, 16, None, 30.0, True),
+    (_many(80, *[320] * 40), 32, 8, 64, 64, 500, 0.0, False),                  # of two, keys that a window ends
+    (_many(64, 1500, 700), 8, 2, 256, 32, None, 0.0, False),
+    ([(0, [200 + 13 * i]) for i in range(70)], 32, 8, 128, 64, None, 0.0, False),
+    (_many(400, 100, 300), 8, 8, 64, 16, None, 0.0, False)])
+def test_all_engines_and_late_values(groups, heads, kv, dim, page, window, softcap, sinks):
+    a = batch(groups, heads, kv, dim, page, BF16, device=DEV)
+    sinks = torch.randn(heads, device=DEV) * 3 if sinks else None
+    want = check(a, window, softcap, sinks)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    for i in range(30):
+        if i % 3:
+            flush.zero_()
+        assert torch.equal(shared_decode(**a, window=window, softcap=softcap, sinks=sinks), want), i
+    L.check_status()
