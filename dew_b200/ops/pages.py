@@ -3,8 +3,7 @@ compaction of the pool does to the device.  The page numbers are the host's, who
 from __future__ import annotations
 
 import ctypes
-import struct
-from itertools import chain
+from array import array
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -55,6 +54,10 @@ def _pool(t: torch.Tensor, pages: int, device) -> _Pool:
     return _Pool(t.data_ptr(), strides[0] * by, shape[0], size * by)
 
 
+def _take(numbers: array, ps: Sequence[int]) -> None:
+    numbers.fromlist(ps) if type(ps) is list else numbers.extend(ps)
+
+
 def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], table: Optional[torch.Tensor] = None, tables: Sequence[Span] = ()) -> None:
     """``pool[:, dst[i]] = pool[:, src[i]]`` in every pool ``[layers, pages, ...]`` (any types; all of as many pages), and ``table[row, first:first + len(pages)] = pages`` for
     every ``(row, first, pages)`` of ``tables`` (``table`` int32 ``[rows, columns]``).
@@ -79,22 +82,29 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
             if len(ps):
                 table[row, first:first + len(ps)] = torch.tensor(list(ps), dtype=torch.int32, device=table.device)
         return
-    spans = [] if not tables else list(zip(*tables))
-    named = list(chain.from_iterable(spans[2])) if tables else []
-    lengths = list(map(len, spans[2])) if tables else []
+    if not L.device_is_current(pools[0]):
+        with L.on_device_of(pools[0]):
+            return move_pages(pools, src, dst, table, tables)
+    # (the quickest way from lists to integers; they are held until the call is over)
+    numbers = array("i")
     try:
-        # (the quickest way from lists to integers; the bytes are held until the call is over)
-        numbers = struct.pack(f"{2 * len(src) + 3 * len(tables) + len(named)}i", *src, *dst, *(spans[0] if tables else ()), *(spans[1] if tables else ()), *lengths, *named)
-    except struct.error as e:
+        for ps in (src, dst):
+            _take(numbers, ps)
+        if tables:
+            rows, firsts, named = zip(*tables)
+            numbers.extend(rows)
+            numbers.extend(firsts)
+            numbers.extend(map(len, named))
+            for ps in named:
+                _take(numbers, ps)
+    except OverflowError as e:
         raise ValueError(f"move_pages: {e}") from None
     n, spans_n = len(src), len(tables)
-    start = ctypes.cast(ctypes.c_char_p(numbers), ctypes.c_void_p).value
-    part = lambda i: start + 4 * i
+    start = numbers.buffer_info()[0]
+    spans = start + 8 * n
     launches = ctypes.c_int(0)
-    with L.on_device_of(pools[0]) as stream:
-        rc = L.load().dewb_move_pages(ctypes.addressof(made), len(pools), pages, part(0), part(n), n, L.at(table if tables else None), table.shape[0] if tables else 0,
-                                      table.shape[1] if tables else 0, part(2 * n), part(2 * n + spans_n), part(2 * n + 2 * spans_n), part(2 * n + 3 * spans_n), spans_n,
-                                      ctypes.addressof(launches), stream)
+    rc = L.load().dewb_move_pages(ctypes.addressof(made), len(made), pages, start, start + 4 * n, n, table.data_ptr() if tables else 0, table.shape[0] if tables else 0,
+                                  table.shape[1] if tables else 0, spans, spans + 4 * spans_n, spans + 8 * spans_n, spans + 12 * spans_n, spans_n, ctypes.addressof(launches), L.stream())
     _refuse(rc)
     L.check(rc, "move_pages")
     L.count_launches(launches.value)
