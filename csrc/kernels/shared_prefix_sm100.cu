@@ -1,9 +1,9 @@
 // A decode step of rows that share prefixes, on the tensor cores: bf16 queries and pools, heads of 64, 128 or 256, pages of a multiple of 16 tokens.
 //
 // The work is lists: up to some number of queries (row, head) against a range of keys of one key head.  A group's shared keys (shared_range.cuh) make a list for each key head,
-// a row's own keys another.  There are two kinds, each with CTAs of its own (as many as its share of the work, dealt over the SMs).  All lists of a kind stand behind one
-// another in one sequence that its CTAs share evenly, tile by tile: a list may begin in one CTA and end in another.  In front of each list there is room in the sequence for
-// what beginning and ending one costs, so that CTAs with many short lists get fewer tiles.
+// a row's own keys another.  There are two kinds, each with engines of its own (as many as its share of the work).  All lists of a kind stand behind one another in one sequence
+// that its engines share evenly, tile by tile: a list may begin in one engine and end in another.  In front of each list there is room in the sequence for what beginning and
+// ending one costs, so that engines with many short lists get fewer tiles.
 //
 // TALL lists (a group of more than 32 queries on a key head, 128 of them a list): queries are the rows of the products.  Per 64 keys  S = Q K^T  (one of two score buffers in
 // tensor memory),  a thread a query makes the weights P over its scores,  O += P V  with P read from tensor memory.
@@ -13,19 +13,22 @@
 // weights are relative to one maximum a query, which the threads agree on anew only where a score has passed it by 2^8 (one vote a tile); sums of weights stay with the
 // threads until the list ends.
 //
-//   warps 0..3  softmax, results;  tall lists' queries
-//   warp 4      TMA: keys and values; finds out what the next list is about, and fetches wide lists' queries
-//   warp 5      tensor cores
+// An engine is six warps, with rings, barriers and a part of tensor memory of its own:
+//   0..3  softmax, results;  tall lists' queries
+//   4     TMA: keys and values; finds out what the next list is about, and fetches wide lists' queries
+//   5     tensor cores
 //
-// Two CTAs an SM (one at heads of 256), whose chains lie beside one another: an SM's share of the memory rate brings 64 keys and values of a head of 128 in 1400 cycles.
+// A CTA an SM, of two engines of one kind (one at heads of 256) whose chains lie beside one another: an SM's share of the memory rate brings 64 keys and values of a head of 128
+// in 1400 cycles.  As two CTAs, of either kind as they came, a third of all instruction fetches missed: tall and wide lists' code is more than the SM's instruction cache holds
+// (128 rows behind 8192 shared tokens 88 us instead of 65, 61 rows with capped scores 62 instead of 42).
 // With four queries as rows of a 128-row product, a wide list's tile took one warp 2300 cycles of scores (four of its lanes had any) and a list of one tile 7100, mostly chain:
 // 128 rows in 16 groups of 1000 to 2048 shared tokens 181 us, 128 rows behind 8192 shared tokens 121.
 //
 // No score needs a mask but at the ends of a list's keys, where it is the same for all queries.  Values there are put to zero in shared memory, since a weight of zero does
 // not cancel what is not a number.
 //
-// A list that is a row's whole attention is finished here.  Otherwise (m, l, sum) of a list, or of the piece of it that a CTA had, goes to scratch, and a second kernel joins
-// a query's pieces:  o = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i.  Scratch is bounded by queries and CTAs, whatever the keys' number: of each kind a CTA holds at most
+// A list that is a row's whole attention is finished here.  Otherwise (m, l, sum) of a list, or of the piece of it that an engine had, goes to scratch, and a second kernel joins
+// a query's pieces:  o = sum_i 2^(m_i - M) a_i / sum_i 2^(m_i - M) l_i.  Scratch is bounded by queries and engines, whatever the keys' number: an engine holds at most
 // two lists in part (its first and its last), the others' queries have a place of their own.  Nothing is counted with atomics: the same call gives the same bits.
 #include <cstddef>
 #include <cstdint>
@@ -43,7 +46,7 @@ constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys o
 constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
 constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;              // of an engine
 constexpr int MOST_ROWS = 448;
-constexpr int TALL_GAP = 2, WIDE_GAP = 1;         // tiles that a list takes as long as beyond its own
+constexpr int TALL_GAP = 5, WIDE_GAP = 1;         // tiles that a list takes as long as beyond its own (with 2 for tall ones, 64 rows of 500 keys behind 64 take 68 us instead of 41)
 constexpr int TALL_COST = 1, CAPPED_COST = 2, WIDE_COST = 2;       // of a tile (a tall one, one with a cap, a wide one), where engines are dealt: with 1 : 1 for what has no cap
                                                   // 128 rows behind 8192 tokens take 85 us instead of 65, with 1 : 2 for what has one 97 instead of 84
 constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
@@ -75,13 +78,13 @@ struct Ranges {                                   // the keys of a list, [a0, a1
   __device__ __forceinline__ bool meets(int key, int n) const { return (key < a1 && key + n > a0 && a1 > a0) || (key < b1 && key + n > b0 && b1 > b0); }
 };
 
-// A list, or the piece of it that a CTA has.
+// A list, or the piece of it that an engine has.
 struct Item {
   Ranges keys;
   int index, list, lists;                         // group or place, and which of its lists
   bool shared;                                    // of a group
   int start, units;                               // the whole list's first tile, in the sequence, and its tiles
-  int from, tiles;                                // of its tiles (tiles 0: the CTA's lists are over)
+  int from, tiles;                                // of its tiles (tiles 0: the engine's lists are over)
   int place, each, hk, head0, n;                  // first query counted through the places, query heads a row, key head, first query head, queries
   int row;                                        // whose table
 };
@@ -165,7 +168,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 
 __device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * a.ratio; }
 
-// The CTA's first list, from unit u on, or (!begins) the one behind w's; up to `end`.  One thread.
+// The engine's first list, from unit u on, or (!begins) the one behind w's; up to `end`.  One thread.
 template <bool TALL>
 __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, int u, int end, bool begins) {
   constexpr int GAP = TALL ? TALL_GAP : WIDE_GAP;
@@ -242,28 +245,22 @@ __device__ __forceinline__ int query(const Lists& s, const Args& a, const Item& 
 }
 
 // A warp's up to 32 queries (lane i holds query()'s answer for number i) to rows of 128 bytes (128-byte swizzle), 64-column pieces `apart` bytes apart; `to`: the first's row,
-// on a 1024-byte boundary.  EACH: 16-byte loads of a lane that are on their way at a time.
-template <int D, int EACH>
+// on a 1024-byte boundary.  (A loop of copies: it runs once a list, and straight code of 16 loads
+// and stores takes 15000 cycles to come from L2 each time.)
+template <int D>
 __device__ __forceinline__ void fetch_queries(uint8_t* to, int apart, const Args& a, int mine, int n, int lane) {
   constexpr int PIECES = D / 8, ROWS = 32 / PIECES;
-  const int row = mine / a.heads;
+  const int row = mine / a.heads, c = lane % PIECES;
   const long long from = mine < 0 ? -1 : row * a.q_stride + static_cast<long long>(mine - row * a.heads) * D;
-  const int c = lane % PIECES;
 #pragma unroll 1
-  for (int x0 = 0; x0 < n; x0 += ROWS * EACH) {
-    uint4 v[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int x = x0 + e * ROWS + lane / PIECES;
-      const long long at = __shfl_sync(FULL, from, x & 31);
-      v[e] = x < n && at >= 0 ? __ldg(reinterpret_cast<const uint4*>(a.q + at) + c) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int x = x0 + e * ROWS + lane / PIECES;
-      if (x < n) *reinterpret_cast<uint4*>(to + (c >> 3) * apart + x * 128 + (((c & 7) ^ (x & 7)) << 4)) = v[e];
-    }
+  for (int x0 = 0; x0 < n; x0 += ROWS) {
+    const int x = x0 + lane / PIECES;
+    const long long at = __shfl_sync(FULL, from, x & 31);
+    const uint32_t place = smem_u32(to + (c >> 3) * apart + x * 128 + (((c & 7) ^ (x & 7)) << 4));
+    const __nv_bfloat16* p = a.q + max(at, 0ll) + c * 8;
+    if (x < n) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(place), "l"(p), "r"(at < 0 ? 0 : 16) : "memory");
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   fence_proxy_async();
   __syncwarp();
 }
@@ -793,7 +790,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       int one = -1;
       if (tiles > 0) {
         one = query(lists, a, w, tid);
-        fetch_queries<D, D / 8 < 16 ? D / 8 : 16>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
+        fetch_queries<D>(sQ + warp * 32 * 128, BM * 128, a, one, min(32, w.n - warp * 32), lane);
         if (lane == 0) mbar_arrive(&bars->q_full);
       }
       if (list > 0) {
@@ -944,7 +941,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         load(&tk, w_keys + slot * C::W_TILE, WK, &bars->full[slot], row, lanes, hk);
         if (begins) {
           const Item& w = own.item[list & 1];
-          fetch_queries<D, 8>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
+          fetch_queries<D>(sQ + (list & 1) * C::W_Q, WN * 128, a, query(lists, a, w, lane), w.n, lane);
           if (lane == 0) mbar_arrive(&bars->list_full[list & 1]);
         }
       }

@@ -86,7 +86,7 @@ def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: 
     R, H, D = q.shape
     pages, page, G, _ = k.shape
     return (q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
-            and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 2) < 1 << 30
+            and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 8) < 1 << 30
             and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
 
 
