@@ -213,6 +213,12 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
 template <typename TQ>
 __global__ void __launch_bounds__(64) join_parts_kernel(const __grid_constant__ Args a) {
   const int row = blockIdx.x, head = blockIdx.y;
+  if (head == 0) {                                       // (a row that `order` names twice, and another that it leaves out)
+    int times = 0;
+    for (int i = threadIdx.x; i < a.rows; i += blockDim.x) times += a.order[i] == row;
+    if (__syncthreads_count(times > 0) != 1 || __syncthreads_or(times > 1))
+      if (threadIdx.x == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+  }
   const long long one = static_cast<long long>(row) * a.heads + head, step = static_cast<long long>(a.rows) * a.heads;
   const float sink = a.sinks != nullptr ? a.sinks[head] * 1.4426950408889634f : -INFINITY;
   float top = sink;

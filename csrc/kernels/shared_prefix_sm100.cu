@@ -1079,6 +1079,9 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant_
   const bool there = row >= 0 && row < a.rows, rests = !there || a.lengths[row] <= 0;
   const long long all = static_cast<long long>(a.rows) * a.heads, wide0 = 2 * all + static_cast<long long>(engines) * 2 * BM;
   float sink = a.sinks != nullptr && warp < a.ratio ? a.sinks[hk * a.ratio + warp] * LOG2E : -INFINITY;
+  if (hk == 0)                                    // (a row that `order` names twice, and another that it leaves out)
+    for (int i = threadIdx.x; i < a.rows; i += blockDim.x)
+      if (i != place && a.order[i] == row) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
   griddep_wait();
   if (!there) return;
   const int4 lists = a.plan[2 * place], group = a.plan[2 * place + 1];

@@ -269,8 +269,9 @@ class AdaptedLinear(nn.Module):
         self.base = base
         self._of = (bank,)                                 # (not a module of this one)
         w = base.weight
-        self.register_buffer("a", torch.zeros(bank.slots, bank.rank, base.in_features, dtype=w.dtype, device=w.device), persistent=False)
-        self.register_buffer("b", torch.zeros(bank.slots, base.out_features, bank.rank, dtype=w.dtype, device=w.device), persistent=False)
+        rank = -(-bank.rank // 8) * 8 if w.dtype == torch.bfloat16 else bank.rank            # (rows of b that begin at 16 bytes are fetched as blocks)
+        self.register_buffer("a", torch.zeros(bank.slots, rank, base.in_features, dtype=w.dtype, device=w.device), persistent=False)
+        self.register_buffer("b", torch.zeros(bank.slots, base.out_features, rank, dtype=w.dtype, device=w.device), persistent=False)
         self.register_buffer("scale", torch.zeros(bank.slots, dtype=torch.float32, device=w.device), persistent=False)
 
     @property

@@ -62,6 +62,8 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
     _check(x, bank, ids, y.shape[-1] if y.dim() else 0, y.device)
     if y.dtype is not x.dtype or y.shape[:-1] != x.shape[:-1] or not y.is_contiguous():
         raise ValueError("add_adapters: the projection's result in one piece, of the tokens' type and count")
+    if y.data_ptr() == x.data_ptr() and y.numel():
+        raise ValueError("add_adapters: the projection's result and the tokens are two tensors")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, *bank)):
         raise NotImplementedError("add_adapters has no gradient: it serves adapters that were trained alone (nn.lora)")
     return _add(y, x, bank, ids)
@@ -79,7 +81,7 @@ def _add(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> tor
             return _add(y, x, bank, ids)
     x2 = x if x.dim() == 2 else x.reshape(-1, width)
     stride, step = x2.stride()
-    if step != 1:
+    if step != 1 or stride < width:                     # (rows that overlap, or are one)
         x2 = x2.contiguous()
         stride = width
     if not ids.is_contiguous():

@@ -43,3 +43,9 @@ def test_refusals():
     for bad in (y[:5], y.double(), torch.zeros(8, 6).T):
         with pytest.raises(ValueError):
             add_adapters(bad, x, bank, ids)
+
+
+def test_the_result_may_not_be_the_tokens():
+    a = batch(6, 3, 4, 16, 16, torch.float32)
+    with pytest.raises(ValueError):
+        add_adapters(a["x"], a["x"], a["bank"], a["ids"])

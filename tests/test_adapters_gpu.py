@@ -119,3 +119,33 @@ def test_the_same_bits_again():
     a = batch(200, 9, 24, 1024, 640, BF16, device=DEV)
     want = check(a)
     assert all(torch.equal(adapted_linear(**a), want) for _ in range(5))
+
+
+@pytest.mark.parametrize("tokens", [60, 900])
+@pytest.mark.parametrize("n, rank", [(3500, 8), (3501, 8), (4, 512), (3, 513)])
+def test_the_largest_banks_and_ranks(n, rank, tokens):
+    check(batch(tokens, n, rank, 64, 72, BF16, device=DEV, used=min(n, 200), seed=tokens))
+
+
+@pytest.mark.parametrize("tokens", [40, 600])
+def test_rows_that_overlap_or_are_one(tokens):
+    a = batch(tokens, 3, 8, 64, 40, BF16, device=DEV)
+    one = a["x"][:1]
+    want = adapted_linear(**{**a, "x": one.expand(tokens, -1).contiguous()})
+    assert torch.equal(adapted_linear(**{**a, "x": one.expand(tokens, -1)}), want)
+    flat = a["x"].flatten()[:tokens * 8 + 64]
+    windows = flat.as_strided((tokens, 64), (8, 1))
+    assert torch.equal(adapted_linear(**{**a, "x": windows}), adapted_linear(**{**a, "x": windows.contiguous()}))
+
+
+@pytest.mark.parametrize("runs", [False, True])
+@pytest.mark.parametrize("tokens, n, rank, width, out", [(8000, 12, 64, 1024, 2048), (500, 48, 32, 2048, 1536), (2000, 5, 24, 512, 1000)])
+def test_the_same_bits_from_memory(tokens, n, rank, width, out, runs):
+    """Operands that come late (nothing of them is in the cache), on all SMs."""
+    a = batch(tokens, n, rank, width, out, BF16, device=DEV, runs=runs)
+    want, flush = check(a), torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    for i in range(20):
+        if i % 3:
+            flush.zero_()
+        assert torch.equal(adapted_linear(**a), want), i
+    L.check_status()

@@ -150,3 +150,15 @@ def test_all_engines_and_late_values(groups, heads, kv, dim, page, window, softc
             flush.zero_()
         assert torch.equal(shared_decode(**a, window=window, softcap=softcap, sinks=sinks), want), i
     L.check_status()
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (FP32, 48)])
+def test_a_row_named_twice_is_reported(dtype, dim):
+    a = batch([(64, [3, 4, 5]), (0, [9])], 4, 2, dim, 16, dtype, device=DEV)
+    order = a["shared"].order.clone()
+    order[1] = order[0]
+    L.check_status()
+    shared_decode(**{**a, "shared": a["shared"]._replace(order=order)})
+    with pytest.raises(L.KernelError):
+        L.check_status()
+    check(a)
