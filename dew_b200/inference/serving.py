@@ -97,7 +97,8 @@ class Server:
         self.queue: Deque[Ticket] = deque()
         self.device = p.device
         self.clock = clock
-        self.shared_prefix, self._shared_rows = bool(shared_prefix), None
+        self.shared_prefix = bool(shared_prefix)
+        self._layout, self._shared_layout = 0, -1          # counts changes of which pages rows have; the one that the cache was last told of
         self.adapters = adapters
         self._row_adapters = None if adapters is None else torch.full((slots,), -1, dtype=torch.int32, device=self.device)
         self.last_tokens = torch.zeros(slots, dtype=torch.long, device=self.device)      # device-resident draws
@@ -174,6 +175,7 @@ class Server:
                 if r is not None and any(p in moved for p in r.pages):
                     r.pages = [moved.get(p, p) for p in r.pages]
                     tables.append((slot, 0, r.pages))
+            self._layout += 1
             self.store.move_pages(list(moved), list(moved.values()), tables)
         return len(moved)
 
@@ -208,6 +210,7 @@ class Server:
             t.waiting = []
         self.queue.clear()
         self.rows = [None] * self.slots
+        self._layout += 1
 
     def reload(self, variables) -> None:
         self.variables = variables
@@ -250,6 +253,7 @@ class Server:
             table = self.store.page_table[slot]
             table[: len(seat.pages)] = torch.tensor(seat.pages, dtype=torch.int32, device=self.device)
             self.rows[slot] = _Row(t, seat.pages, prefilled=seat.reused_tokens)
+            self._layout += 1
             if self._row_adapters is not None:
                 self._row_adapters[slot] = t.adapter_slot
 
@@ -334,6 +338,7 @@ class Server:
         self.queue.extendleft(reversed(waiting))
         if not children:
             return
+        self._layout += 1
         self.store.move_pages(src, dst, tables)
         self.store.fork_rows([slot] * len(children), children)
         for child in children:
@@ -445,11 +450,9 @@ class Server:
         """Tell the cache which rows begin with the same pages, where that has changed."""
         if not self.shared_prefix:
             return
-        tables = [None if r is None else r.pages for r in self.rows]
-        known = [None if t is None else tuple(t) for t in tables]
-        if known != self._shared_rows:
-            self._shared_rows = known
-            self.store.share(tables, SHARED_LEAST)
+        if self._layout != self._shared_layout:
+            self._shared_layout = self._layout
+            self.store.share([None if r is None else r.pages for r in self.rows], SHARED_LEAST)
 
     def _queue_settle(self, host, snapshot, ev) -> None:
         self._later = getattr(self, "_later", deque())
@@ -486,4 +489,5 @@ class Server:
                     if self.rows[s] is r:
                         self.ledger.release(r.pages)
                         self.rows[s] = None
+                        self._layout += 1
         self._pending = None if not later else later[-1]
