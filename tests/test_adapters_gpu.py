@@ -149,3 +149,24 @@ def test_the_same_bits_from_memory(tokens, n, rank, width, out, runs):
             flush.zero_()
         assert torch.equal(adapted_linear(**a), want), i
     L.check_status()
+
+
+@pytest.mark.parametrize("runs", [False, True])
+def test_layouts_of_prompts(runs):
+    a = batch(640, 5, 16, 256, 384, BF16, device=DEV, runs=runs)
+    want = check(a)
+    wide = torch.randn(640, 512, device=DEV).to(BF16)
+    wide[:, 128:384] = a["x"]
+    assert torch.equal(check({**a, "x": wide[:, 128:384]}), want)
+    odd = torch.randn(640, 259, device=DEV).to(BF16)                     # rows that do not begin at 16 bytes
+    odd[:, 3:] = a["x"]
+    check({**a, "x": odd[:, 3:]})
+    for name, shape in (("a", (5, 16, 256)), ("b", (5, 384, 16))):       # adapters that do not begin at 16 bytes
+        raw = torch.empty(a["bank"].a.numel() * 2 + 1, device=DEV, dtype=BF16)
+        part = getattr(a["bank"], name)
+        raw[1:1 + part.numel()] = part.reshape(-1)
+        check({**a, "bank": a["bank"]._replace(**{name: raw[1:1 + part.numel()].view(shape)})})
+    y = torch.empty(640 * 384 + 1, device=DEV, dtype=BF16)[1:].view(640, 384)
+    base = adapted_linear(a["x"], a["weight"], a["bank"], torch.full_like(a["ids"], -1))
+    assert torch.equal(add_adapters(y.copy_(base), a["x"], a["bank"], a["ids"]), add_adapters(base.clone(), a["x"], a["bank"], a["ids"]))
+    assert torch.equal(adapted_linear(a["x"].view(4, 160, 256), a["weight"], a["bank"], a["ids"].view(4, 160)).view(640, 384), want)
