@@ -46,7 +46,9 @@ constexpr int BM = 128, BN = 64;                  // tall lists: queries, keys o
 constexpr int WK = 128, WN = 32;                  // wide lists: keys of a tile, queries
 constexpr int THREADS = 192, TMA_WARP = 4, MMA_WARP = 5;              // of an engine
 constexpr int MOST_ROWS = 448;
-constexpr int TALL_GAP = 5, WIDE_GAP = 1;         // tiles that a list takes as long as beyond its own (with 2 for tall ones, 64 rows of 500 keys behind 64 take 68 us instead of 41)
+// tiles that a list takes as long as beyond its own: a tall one, a wide one of a group's, a row's own.  (With 2 for tall ones, 64 rows of 500 keys behind 64 shared ones take 68 us
+// instead of 41; with 1 for a group's, 128 rows in 16 groups 100 instead of 90, 256 rows of 256 keys in 32 groups behind 64 tokens 120 instead of 72.)
+constexpr int TALL_GAP = 5, SHARED_GAP = 3, WIDE_GAP = 1;
 constexpr int TALL_COST = 1, CAPPED_COST = 2, WIDE_COST = 2;       // of a tile (a tall one, one with a cap, a wide one), where engines are dealt: with 1 : 1 for what has no cap
                                                   // 128 rows behind 8192 tokens take 85 us instead of 65, with 1 : 2 for what has one 97 instead of 84
 constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
@@ -171,7 +173,6 @@ __device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int 
 // The engine's first list, from unit u on, or (!begins) the one behind w's; up to `end`.  One thread.
 template <bool TALL>
 __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, int u, int end, bool begins) {
-  constexpr int GAP = TALL ? TALL_GAP : WIDE_GAP;
   const int* at = TALL ? s.tall : s.wide;
   bool same = false;
   if (begins) {
@@ -182,10 +183,13 @@ __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, i
   } else {
     u = w.start + w.units;                         // (the room in front of the next list)
     w.tiles = 0;
-    if (u + GAP >= end) return;
+  }
+  const int gap = TALL ? TALL_GAP : u < s.wide_shared_units ? SHARED_GAP : WIDE_GAP;
+  if (!begins) {
+    if (u + gap >= end) return;
     if (++w.list < w.lists) {
       same = true;
-      w.start = u + GAP;
+      w.start = u + gap;
     } else {
       if (!TALL && w.shared && u >= s.wide_shared_units) {
         w.shared = false;
@@ -205,18 +209,18 @@ __device__ __noinline__ void next_list(Item& w, const Lists& s, const Args& a, i
       w.keys = ranges(s.lo[w.index], s.hi[w.index], 0, 0, a.box);
       w.lists = a.kv_heads * (TALL ? (group_queries(s, a, w.index) + BM - 1) / BM : 1);
       w.row = s.through[w.index];
-      w.start = at[w.index] + GAP;
+      w.start = at[w.index] + gap;
       w.units = w.keys.tiles<TALL ? BN : WK>();
     } else {
       const int g = s.group[w.index];
       w.keys = own_ranges(s.len[w.index], a.window, s.lo[g], s.hi[g], a.box);
       w.lists = a.kv_heads * a.chunks;
       w.row = s.row[w.index];
-      w.start = s.wide_shared_units + s.own[w.index] * w.lists + GAP;
-      w.units = s.own[w.index + 1] - s.own[w.index] - GAP;
+      w.start = s.wide_shared_units + s.own[w.index] * w.lists + gap;
+      w.units = s.own[w.index + 1] - s.own[w.index] - gap;
     }
-    w.list = begins ? (u + GAP - w.start) / (w.units + GAP) : 0;
-    w.start += w.list * (w.units + GAP);
+    w.list = begins ? (u + gap - w.start) / (w.units + gap) : 0;
+    w.start += w.list * (w.units + gap);
   }
   if (w.shared) {
     const int queries = group_queries(s, a, w.index), pieces = TALL ? (queries + BM - 1) / BM : 1;
@@ -365,7 +369,7 @@ __device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines)
     const int queries = group_queries(s, a, g);
     const Ranges both = ranges(s.lo[g], s.hi[g], 0, 0, a.box);
     s.tall[g + 1] = s.hi[g] == 0 || queries <= WN ? 0 : a.kv_heads * ((queries + BM - 1) / BM) * (both.tiles<BN>() + TALL_GAP);
-    s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * (both.tiles<WK>() + WIDE_GAP);
+    s.wide[g + 1] = s.hi[g] == 0 || queries > WN ? 0 : a.kv_heads * (both.tiles<WK>() + SHARED_GAP);
   }
   __syncthreads();
 #pragma unroll 1
@@ -1104,7 +1108,7 @@ __global__ void __launch_bounds__(128) join_pieces_kernel(const __grid_constant_
       long long at;
       if (k == 0) {
         const int x = (place - group.x) * a.ratio + h, pieces = (group.y + BM - 1) / BM;
-        start = lists.x + (tall ? (hk * pieces + x / BM) * (n + TALL_GAP) + TALL_GAP : hk * (n + WIDE_GAP) + WIDE_GAP);
+        start = lists.x + (tall ? (hk * pieces + x / BM) * (n + TALL_GAP) + TALL_GAP : hk * (n + SHARED_GAP) + SHARED_GAP);
         per = tall ? group.z : group.w;
         step = tall ? BM : WN;
         at = tall ? 2 * all + x % BM : wide0 + x;
