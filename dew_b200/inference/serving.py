@@ -23,8 +23,8 @@ from .pages import HostTier, OutOfPages, PageLedger
 
 
 # Fewest tokens that rows have to begin with together for a group of theirs.  A step's attention with 32 heads over 8 of 128, 256 tokens of each row's own, apart against shared: with
-# 256 shared tokens 28.5 against 31 us (64 rows in eights) and 77 against 85 (256 in twos), with 1024 of them 66 against 50 (64 in twos), 44 against 42 (in eights) and 195 against 106
-# (256 in eights).  (8 rows: 15 against 20 with 1024, 29 against 24 with 4096.)
+# 256 shared tokens 28.5 against 30 us (64 rows in eights), 77 against 90 (256 in twos) and 72 against 70 (in eights), with 1024 of them 66 against 50 (64 in twos), 44 against 38 (in
+# eights) and 194 against 95 (256 in eights).  (8 rows: 15 against 19 with 1024, 29 against 23 with 4096.)
 SHARED_LEAST = 512
 
 
