@@ -859,7 +859,8 @@ __global__ void __launch_bounds__(GROUP_WARPS * 32) group_tokens_kernel(const in
   each([&](int i, int id) {
     const bool there = id >= 0 && id < adapters;
     const unsigned same = __match_any_sync(FULL, there ? id : -1);
-    if (there) order[mine[id] + __popc(same & ((1u << lane) - 1))] = i;
+    const int place = there ? mine[id] + __popc(same & ((1u << lane) - 1)) : tokens;
+    if (place < tokens) order[place] = i;          // (past the end: never, unless someone writes the ids meanwhile)
     __syncwarp();
     if (there && lane == __ffs(same) - 1) mine[id] += __popc(same);
     __syncwarp();
