@@ -8,7 +8,8 @@
 //
 // grid = (place in `order`, key head x sixteens of its query heads, part): parts [0, splits) are of the shared keys, [splits, 2 splits) of the row's own.  A place that does
 // not start a tile of the shared queries leaves at once.  Per 32 keys: keys and values to shared memory as fp32, scores with a lane a key, values with a lane every 32nd
-// column.  Bound by shared memory reads (5 for 16 multiply-adds): this is the form for types and widths that the tensor cores' kernel does not take.
+// column; a warp whose queries do not exist only fetches.  This is the form for types and widths that the tensor cores' kernel does not take, bound by the chain of a tile's loads,
+// scores and values and by what goes through shared memory (128 fp32 rows of 700 to 1000 keys, 8 heads of 64: 350 us, 1.3 TB/s; 24 rows of 500 keys, 6 heads over 2 of 80: 30 us).
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -59,12 +60,12 @@ __device__ __forceinline__ int group_of(const int* __restrict__ first, int group
 
 template <typename TQ, typename TP, bool SCALED>
 __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_constant__ Args a) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   const int D = a.D, wide = D + 1;
   float* sq = smem;                                      // [QUERIES][D]
   float* sk = sq + QUERIES * D;                          // [KEYS][D + 1]
   float* sv = sk + KEYS * wide;                          // [KEYS][D]
-  float* sp = sv + KEYS * D;                             // [QUERIES][KEYS]
+  float* sp = sv + KEYS * D;                             // [KEYS][QUERIES]
   __shared__ long long stok[2][KEYS];                    // where keys stand in the pools (-1: nowhere), of this tile and the next one
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ratio = a.heads / a.kv_heads, chunks = (ratio + QUERIES - 1) / QUERIES;
@@ -147,12 +148,25 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
       }
     }
     __syncthreads();
+    if (warp * EACH >= n) continue;                      // (no queries for this warp)
     const bool seen = stok[b][lane] >= 0;
-    float s[EACH];
+    float s[EACH], weights[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) s[i] = 0.f;
     const float* mine = sq + warp * EACH * D;
-    for (int d = 0; d < D; ++d) {
+    int d = 0;
+    if (D % 4 == 0)                                      // (queries four columns at a time)
+      for (; d < D; d += 4) {
+        float kx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kx[e] = sk[lane * wide + d + e];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const float4 qx = *reinterpret_cast<const float4*>(mine + i * D + d);
+          s[i] = fmaf(qx.w, kx[3], fmaf(qx.z, kx[2], fmaf(qx.y, kx[1], fmaf(qx.x, kx[0], s[i]))));
+        }
+      }
+    for (; d < D; ++d) {
       const float kx = sk[lane * wide + d];
 #pragma unroll
       for (int i = 0; i < EACH; ++i) s[i] = fmaf(mine[i * D + d], kx, s[i]);
@@ -175,13 +189,14 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
       m[i] = m_new;
 #pragma unroll
       for (int c = 0; c < MOST_D / 32; ++c) acc[i][c] *= by;
-      sp[(warp * EACH + i) * KEYS + lane] = p;
+      weights[i] = p;
     }
+    static_assert(EACH == 4, "a key's weights are one 16-byte word a warp");
+    *reinterpret_cast<float4*>(sp + lane * QUERIES + warp * EACH) = make_float4(weights[0], weights[1], weights[2], weights[3]);
     __syncwarp();
     for (int j = 0; j < KEYS; ++j) {
-      float p[EACH];
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) p[i] = sp[(warp * EACH + i) * KEYS + j];
+      const float4 word = *reinterpret_cast<const float4*>(sp + j * QUERIES + warp * EACH);
+      const float p[EACH] = {word.x, word.y, word.z, word.w};
 #pragma unroll
       for (int c = 0; c < MOST_D / 32; ++c) {
         const int d = c * 32 + lane;
