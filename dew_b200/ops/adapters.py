@@ -45,7 +45,11 @@ def _check(x, bank: Bank, ids, out: int, device) -> None:
         raise TypeError(f"adapters: bf16 or fp32 tokens and adapters of one type, fp32 scales and int32 ids, got {x.dtype}, {a.dtype}, {b.dtype}, {scale.dtype}, {ids.dtype}")
     if not (a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()):
         raise ValueError("adapters: a, b and scale in one piece each")
-    if a.device != device or b.device != device or scale.device != device or ids.device != device or x.device != device:
+    if x.is_cuda and type(device) is int:                # (the quicker question)
+        apart = a.get_device() != device or b.get_device() != device or scale.get_device() != device or ids.get_device() != device or x.get_device() != device
+    else:
+        apart = a.device != device or b.device != device or scale.device != device or ids.device != device or x.device != device
+    if apart:
         raise ValueError("adapters: tensors of one device")
 
 
@@ -62,7 +66,7 @@ def add_adapters_reference(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: to
 def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> torch.Tensor:
     """``y [..., out] += scale[i] (x [..., in] a[i]^T) b[i]^T`` in place, ``i = ids [...]`` (int32; below 0: the token has none) -> ``y``.  Sums are fp32; in bf16 the rank's
     values, with their scale, are rounded once between the two products."""
-    _check(x, bank, ids, y.shape[-1] if y.dim() else 0, y.device)
+    _check(x, bank, ids, y.shape[-1] if y.dim() else 0, y.get_device() if y.is_cuda else y.device)
     if y.dtype is not x.dtype or y.shape[:-1] != x.shape[:-1] or not y.is_contiguous():
         raise ValueError("add_adapters: the projection's result in one piece, of the tokens' type and count")
     if y.data_ptr() == x.data_ptr() and y.numel():
@@ -115,7 +119,7 @@ def _add(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> tor
 
 def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bank: Bank, ids: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``ops.linear(x, weight, bias)`` plus each token's adapter (``add_adapters``): ``x [..., in]``, ``weight [out, in]``, ``ids [...]`` int32."""
-    _check(x, bank, ids, weight.shape[0], weight.device)
+    _check(x, bank, ids, weight.shape[0], weight.get_device() if weight.is_cuda else weight.device)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, *bank)):
         raise NotImplementedError("adapted_linear has no gradient: it serves adapters that were trained alone (nn.lora)")
     y = linear(x, weight, bias)

@@ -83,11 +83,14 @@ def _engines(lib, device, D: int) -> int:
 def on_tensor_cores(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, columns: int, groups: int) -> bool:
     """Whether the call is one of ``shared_prefix_sm100.cu``'s: bf16 throughout, heads of 64, 128 or 256, pages of whole sixteens of tokens, 16-byte rows, tables whose tiles
     can be counted in 32 bits."""
-    R, H, D = q.shape
-    pages, page, G, _ = k.shape
-    return (q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
-            and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 8) < 1 << 30
-            and q.data_ptr() % 16 == k.data_ptr() % 16 == v.data_ptr() % 16 == 0 and (R == 1 or q.stride(0) % 8 == 0))
+    (R, H, D), (pages, page, G, _) = q.shape, k.shape
+    return (q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and _counted(R, H, D, pages, page, G, columns, groups)
+            and (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 == 0 and (R == 1 or q.stride(0) % 8 == 0))
+
+
+def _counted(R: int, H: int, D: int, pages: int, page: int, G: int, columns: int, groups: int) -> bool:
+    return (D in (64, 128, 256) and page % 16 == 0 and R <= MOST_ROWS and groups <= MOST_ROWS and pages * page < 0x7fffff00
+            and (2 * R * -(-H // G // 32) + groups) * G * (columns * page // 64 + 8) < 1 << 30)
 
 
 def _splits(most: int, lists: int) -> int:
@@ -97,6 +100,10 @@ def _splits(most: int, lists: int) -> int:
 
 
 _POOLS = {torch.int8: 1, torch.float8_e4m3fn: 2}
+
+
+def _device(t: torch.Tensor) -> torch.device:
+    return t.device
 
 
 def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_scale, v_scale) -> None:
@@ -118,21 +125,22 @@ def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_sc
         raise ValueError(f"shared_decode: order [rows], first [groups + 1] and tokens [groups] for {R} rows, got {[tuple(t.shape) for t in shared]}")
     if table.dim() != 2 or len(table) != R or lengths.shape != (R,):
         raise ValueError(f"shared_decode: a table [rows, columns] and lengths [rows] for {R} rows, got {tuple(table.shape)}, {tuple(lengths.shape)}")
-    device = q.device
-    apart = k.device != device or v.device != device
+    where = torch.Tensor.get_device if q.is_cuda else _device          # (the quicker question)
+    device = where(q)
+    apart = where(k) != device or where(v) != device
     for t in (table, lengths, order, first, tokens):
         if t.dtype is not torch.int32 or not t.is_contiguous():
             raise TypeError("shared_decode: table, lengths, order, first and tokens are int32 in one piece")
-        apart = apart or t.device != device
+        apart = apart or where(t) != device
     if scaled:
         for t in (k_scale, v_scale):
             if t.shape != k_shape[:3] or t.dtype is not torch.float32 or not t.is_contiguous():
                 raise ValueError("shared_decode: fp32 scales [pages, page, kv heads]")
-            apart = apart or t.device != device
+            apart = apart or where(t) != device
     if sinks is not None:
         if sinks.shape != (H,) or sinks.dtype is not torch.float32 or not sinks.is_contiguous():
             raise ValueError("shared_decode: fp32 sinks, one a head")
-        apart = apart or sinks.device != device
+        apart = apart or where(sinks) != device
     if (window is not None and window < 1) or softcap < 0:
         raise ValueError(f"shared_decode: a window of 1 or more and a cap of 0 or more, got {window}, {softcap}")
     if not (k.is_contiguous() and v.is_contiguous()):
@@ -167,15 +175,17 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     out = torch.empty(R, H, D, dtype=q.dtype, device=q.device)
     pages, page, G, _ = k.shape
     columns, groups, fp32, lib = table.shape[1], len(shared.tokens), torch.float32, L.load()
+    at_q, at_k, at_v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     numbers = (table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks))
     err, stream = L.status(q.device).data_ptr(), L.stream()
-    if on_tensor_cores(q, k, v, columns, groups):
+    if (q.dtype is torch.bfloat16 and k.dtype is torch.bfloat16 and (at_q | at_k | at_v) & 15 == 0 and (R == 1 or strides[0] % 8 == 0)
+            and _counted(R, H, D, pages, page, G, columns, groups)):
         engines = _engines(lib, q.device, D)
         rows = 2 * R * H + 320 * engines
         # one piece of scratch a call: sums, maxima and sums of weights, the plan
         scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
         at = scratch.data_ptr()
-        L.check(lib.dewb_shared_decode_mma(q.data_ptr(), strides[0] if R > 1 else H * D, k.data_ptr(), v.data_ptr(), *numbers, at, at + 4 * rows * D, at + 4 * rows * (D + 2),
+        L.check(lib.dewb_shared_decode_mma(at_q, strides[0] if R > 1 else H * D, at_k, at_v, *numbers, at, at + 4 * rows * D, at + 4 * rows * (D + 2),
                                            out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, engines, scale, softcap, err, stream), "shared_decode_mma")
         L.count_launches(2)
         return out
@@ -183,7 +193,7 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     parts = torch.empty(2 * splits * R * H * (D + 2), dtype=fp32, device=q.device)
     at = parts.data_ptr()
     one = 2 * splits * R * H * 4
-    L.check(lib.dewb_shared_decode(q.data_ptr(), strides[0], k.data_ptr(), v.data_ptr(), L.at(k_scale), L.at(v_scale), *numbers, at, at + one, at + 2 * one, out.data_ptr(),
+    L.check(lib.dewb_shared_decode(at_q, strides[0], at_k, at_v, L.at(k_scale), L.at(v_scale), *numbers, at, at + one, at + 2 * one, out.data_ptr(),
                                    R, H, G, D, page, columns, pages, groups, splits, window or 0, scale, softcap, int(q.dtype is fp32), _POOLS.get(k.dtype, 0), err, stream),
             "shared_decode")
     L.count_launches(2)
