@@ -397,6 +397,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   return false;
 }
 
+// After a wait that ran out: what is on its way to shared memory gets 20 ms to land before that memory is another's.
+__device__ __noinline__ void let_copies_land(volatile int* abort_flag) {
+  if (*abort_flag == 0) return;
+  const unsigned long long from = globaltimer_ns();
+  while (globaltimer_ns() - from < 20000000ull) __nanosleep(1000);
+}
+
 // whether a tile's tokens are neighbours (all threads)
 __device__ __forceinline__ bool neighbours(const int* rows, int count, int tid) { return __syncthreads_and(tid >= count || rows[tid] == rows[0] + tid) != 0; }
 
@@ -501,6 +508,7 @@ __global__ void __launch_bounds__(192) make_low_kernel(const __grid_constant__ C
    }
     if (steps > 0) wait(&bars.acc_full[0], 0, abort_flag, m.err, ERR_WAIT_TMEM_FULL, lane);
     tc_fence_after();
+    let_copies_land(abort_flag);
     // this part's values to the CTA that adds up this thread's token, where its operands were (in room of their own, 106 KB a CTA and two instead of three an SM: 29 us instead of 24)
     cluster_arrive();
     cluster_wait();                              // (all are done with their operands)
@@ -784,6 +792,7 @@ __global__ void __launch_bounds__(320, 1) add_columns_kernel(const __grid_consta
     }
     piece += n;
   }
+  let_copies_land(abort_flag);
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {

@@ -168,6 +168,13 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   return false;
 }
 
+// After a wait that ran out: what is on its way to shared memory gets 20 ms to land before that memory is another's.
+__device__ __noinline__ void let_copies_land(volatile int* abort_flag) {
+  if (*abort_flag == 0) return;
+  const unsigned long long from = globaltimer_ns();
+  while (globaltimer_ns() - from < 20000000ull) __nanosleep(1000);
+}
+
 __device__ __forceinline__ int group_queries(const Lists& s, const Args& a, int g) { return (s.first[g + 1] - s.first[g]) * a.ratio; }
 
 // The engine's first list, from unit u on, or (!begins) the one behind w's; up to `end`.  One thread.
@@ -1065,6 +1072,7 @@ shared_mma_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
   }
   if (blockIdx.x == gridDim.x - 1) write_plan(lists, a);
+  let_copies_land(abort_flag);
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP && engine == 0) {
