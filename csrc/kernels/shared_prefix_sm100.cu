@@ -49,8 +49,9 @@ constexpr int MOST_ROWS = 448;
 // tiles that a list takes as long as beyond its own: a tall one, a wide one of a group's, a row's own.  (With 2 for tall ones, 64 rows of 500 keys behind 64 shared ones take 68 us
 // instead of 41; with 1 for a group's, 128 rows in 16 groups 100 instead of 90, 256 rows of 256 keys in 32 groups behind 64 tokens 120 instead of 72.)
 constexpr int TALL_GAP = 5, SHARED_GAP = 3, WIDE_GAP = 1;
-constexpr int TALL_COST = 1, CAPPED_COST = 2, WIDE_COST = 2;       // of a tile (a tall one, one with a cap, a wide one), where engines are dealt: with 1 : 1 for what has no cap
-                                                  // 128 rows behind 8192 tokens take 85 us instead of 65, with 1 : 2 for what has one 97 instead of 84
+// of a tile (a tall one, one with a cap, a wide one), where engines are dealt: 128 rows behind 8192 tokens take 64 us with 2 : 4 and 75 with 3 : 4, with a cap 82 with 3 : 4, 86
+// with 4 : 4 and 97 with 2 : 4
+constexpr int TALL_COST = 2, CAPPED_COST = 3, WIDE_COST = 4;
 constexpr float RESCALE = 8.f;                    // how far (log2) a query's scores may pass the maximum in use before O is rescaled
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t FULL = 0xffffffffu;
