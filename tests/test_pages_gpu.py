@@ -180,3 +180,20 @@ def test_a_served_group_and_compaction(graph, page):
     assert all(t.result() == got[0].result() for t in got)
     agree = sum(a == b for a, b in zip(got[0].result(), want[0]))
     assert got[0].result()[0] == want[0][0] and agree >= 1
+
+
+@pytest.mark.parametrize("runs", [[1], [2], [7], [5, 1, 1, 9], [1, 1, 1], [3] * 40, [1, 2] * 60, [4000], [3000, 1, 2500], [2, 1] * 900 + [5000]])
+@pytest.mark.parametrize("dtype, page", [(torch.bfloat16, 8), (torch.int8, 5), (torch.float32, 3)])
+def test_copies_of_one_page_that_follow_one_another(runs, dtype, page):
+    """A source's copies side by side are made from one load; the runs may be cut between two launches."""
+    n, copies = len(runs), sum(runs)
+    g = torch.Generator().manual_seed(copies)
+    order = torch.randperm(n + copies + 3, generator=g).tolist()
+    src = [s for s, k in zip(order, runs) for _ in range(k)]
+    dst = order[n:n + copies]
+    pools = [torch.randint(-100, 100, (2, len(order), page, 3), generator=g).to(dtype).to(DEV) for _ in range(2)]
+    table = torch.zeros(4, 9, dtype=torch.int32, device=DEV)
+    tables = [(1, 2, dst[:3]), (3, 0, src[:1])]
+    want = plain(pools, src, dst, table, tables)
+    move_pages(pools, src, dst, table, tables)
+    same(pools, table, want)
