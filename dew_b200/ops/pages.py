@@ -54,10 +54,6 @@ def _pool(t: torch.Tensor, pages: int, device) -> _Pool:
     return _Pool(t.data_ptr(), strides[0] * by, shape[0], size * by)
 
 
-def _take(numbers: array, ps: Sequence[int]) -> None:
-    numbers.fromlist(ps) if type(ps) is list else numbers.extend(ps)
-
-
 def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], table: Optional[torch.Tensor] = None, tables: Sequence[Span] = ()) -> None:
     """``pool[:, dst[i]] = pool[:, src[i]]`` in every pool ``[layers, pages, ...]`` (any types; all of as many pages), and ``table[row, first:first + len(pages)] = pages`` for
     every ``(row, first, pages)`` of ``tables`` (``table`` int32 ``[rows, columns]``).
@@ -87,16 +83,17 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
             return move_pages(pools, src, dst, table, tables)
     # (the quickest way from lists to integers; they are held until the call is over)
     numbers = array("i")
+    take = numbers.fromlist
     try:
         for ps in (src, dst):
-            _take(numbers, ps)
+            take(ps) if type(ps) is list else numbers.extend(ps)
         if tables:
             rows, firsts, named = zip(*tables)
             numbers.extend(rows)
             numbers.extend(firsts)
             numbers.extend(map(len, named))
             for ps in named:
-                _take(numbers, ps)
+                take(ps) if type(ps) is list else numbers.extend(ps)
     except OverflowError as e:
         raise ValueError(f"move_pages: {e}") from None
     n, spans_n = len(src), len(tables)
