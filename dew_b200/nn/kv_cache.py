@@ -369,7 +369,8 @@ class KVStore:
 
     def resize(self, pages: int) -> None:
         """Pools of another number of pages (a graph that was captured over the old ones has to be captured again).  What the first pages hold stays; what the table names past
-        the end, the caller has moved (``move_pages``) or does not need."""
+        the end, the caller has moved (``move_pages``) or does not need: those places name the first page from here on, so that whatever reads a row to the end of another
+        (``gather``) finds no name outside the pools."""
         if pages < 1:
             raise ValueError(f"a cache of {pages} pages")
         kept = min(pages, self.pages)
@@ -391,6 +392,7 @@ class KVStore:
                     continue
                 new = sized(old, 0)
                 self.k, self.v = ([new if t is old else t for t in pools] for pools in (self.k, self.v))
+        self.page_table.masked_fill_(self.page_table >= pages, 0)
         self.pages = pages
 
     def share(self, tables: Optional[Sequence[Optional[Sequence[int]]]], least: int = 1) -> None:
