@@ -14,7 +14,7 @@ import ctypes
 import math
 import os
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Any, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -373,27 +373,55 @@ class KVStore:
         (``gather``) finds no name outside the pools."""
         if pages < 1:
             raise ValueError(f"a cache of {pages} pages")
-        kept = min(pages, self.pages)
-
-        def sized(t: torch.Tensor, axis: int) -> torch.Tensor:
-            shape = list(t.shape)
-            shape[axis] = pages + 1
-            new = t.new_ones(shape) if t is self.k_scale or t is self.v_scale else t.new_zeros(shape)
-            new.narrow(axis, 0, kept).copy_(t.narrow(axis, 0, kept))
-            return new
-        if self.slots is None:
-            for name in ("k", "v", "k_scale", "v_scale"):
-                if getattr(self, name) is not None:
-                    setattr(self, name, sized(getattr(self, name), 1))
-        else:
-            # (layers that read another's keys and values, and latent rows, name one pool several times)
-            for old in [t for pools in (self.k, self.v) for t in pools if t is not None]:
-                if not any(old is t for pools in (self.k, self.v) for t in pools):
-                    continue
-                new = sized(old, 0)
-                self.k, self.v = ([new if t is old else t for t in pools] for pools in (self.k, self.v))
+        axis, was = (1, self.pages) if self.slots is None else (0, self.pages)
+        places = self._pool_places()
+        try:
+            for place in places:
+                self._resize_pool(place, axis, pages)
+        except torch.OutOfMemoryError:
+            for place in places:                     # (what has grown already: as long as it was)
+                old = place[0][0][place[0][1]].narrow(axis, 0, was + 1)
+                for pools, name in place:
+                    pools[name] = old
+            raise
         self.page_table.masked_fill_(self.page_table >= pages, 0)
         self.pages = pages
+
+    def _pool_places(self) -> List[List[Tuple[Any, Any]]]:
+        """Where the store names each of its pools, a list of (container, key) for each: layers that read another's keys and values, and latent rows, name one several times."""
+        if self.slots is None:
+            return [[(self.__dict__, n)] for n in ("k", "v", "k_scale", "v_scale") if getattr(self, n) is not None]
+        places: Dict[int, List[Tuple[Any, Any]]] = {}
+        for pools in (self.k, self.v):
+            for i, t in enumerate(pools):
+                if t is not None:
+                    places.setdefault(id(t), []).append((pools, i))
+        return list(places.values())
+
+    def _resize_pool(self, place: List[Tuple[Any, Any]], axis: int, pages: int) -> None:
+        """One pool, wherever it is named, with room for ``pages`` pages and the spare one.  Raises where there is no room for a larger one; a smaller one goes by way of the host
+        where there is none for both."""
+        pools, name = place[0]
+        t = pools[name]
+        kept = min(pages, t.shape[axis] - 1)
+        shape, make, like = [*t.shape[:axis], pages + 1, *t.shape[axis + 1:]], torch.ones if t is self.k_scale or t is self.v_scale else torch.zeros, dict(dtype=t.dtype, device=t.device)
+        try:
+            new = make(shape, **like)
+        except torch.OutOfMemoryError:
+            if pages + 1 > t.shape[axis]:
+                raise
+            new = None
+        held = t.narrow(axis, 0, kept)
+        if new is None:
+            held = held.cpu()
+            for pools, name in place:
+                pools[name] = None
+            del t
+            torch.cuda.empty_cache()                 # (a piece of the old one would keep all of it)
+            new = make(shape, **like)
+        new.narrow(axis, 0, kept).copy_(held)
+        for pools, name in place:
+            pools[name] = new
 
     def share(self, tables: Optional[Sequence[Optional[Sequence[int]]]], least: int = 1) -> None:
         """Rows whose pages (``tables``, one list a row, None for an empty one) begin with the same ones read those once in the decode steps to come (``ops.prefix``), from

@@ -1,10 +1,11 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
 import pytest
 import torch
+from torch.overrides import TorchFunctionMode
 
 from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
-from dew_b200.nn.kv_cache import KVCache, KVStore
+from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore
 
 CONFIG = dict(vocab_size=64, emb_features=32, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, mlp_features=48, max_seq_len=160)
 
@@ -53,3 +54,59 @@ def test_a_store_takes_names_past_its_end_out_of_the_table():
     store.resize(10)
     assert store.page_table.tolist() == [[4, 5, 6, 7, 8, 9, 0, 0], [0] * 8]
     store.gather(0, 64)
+
+
+def _stores():
+    slots = [CacheSlot(1, 8, 8), CacheSlot(2, 16, 16), CacheSlot(1, 8, 8, source=0)]
+    return [KVStore(KVCache(page_size=4, pages=12), 2, 2, 24, 1, 8, dtype=torch.float32), KVStore(KVCache("int8", 4, 12), 2, 2, 24, 1, 8, dtype=torch.float32),
+            KVStore(KVCache(page_size=4, pages=12), 3, 2, 24, 1, 8, dtype=torch.float32, slots=slots)]
+
+
+def _filled(store):
+    for i, t in enumerate(store.pools()):
+        t.copy_((torch.arange(t.numel(), dtype=torch.float32) * (i + 1) % 100).view(t.shape))
+    return [t.clone() for t in store.pools()]
+
+
+class ShortOfMemory(TorchFunctionMode):
+    """The device has no room for a pool from the ``after``-th one asked for on, ``times`` times."""
+
+    def __init__(self, after, times=100):
+        super().__init__()
+        self.made, self.after, self.times = 0, after, times
+
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        if func in (torch.zeros, torch.ones, torch.empty, torch.full, torch.Tensor.new_zeros, torch.Tensor.new_ones, torch.Tensor.new_empty, torch.Tensor.new_full):
+            self.made += 1
+            if self.after < self.made <= self.after + self.times:
+                raise torch.OutOfMemoryError("no room")
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("after", [0, 1])
+def test_a_pool_that_cannot_grow_stays_as_it_is(which, after):
+    store = _stores()[which]
+    held = _filled(store)
+    with pytest.raises(torch.OutOfMemoryError), ShortOfMemory(after):
+        store.resize(30)
+    assert store.pages == 12 and all(torch.equal(a, b) for a, b in zip(store.pools(), held)) and len(store.pools()) == len(held)
+    assert {t.shape[1 if store.slots is None else 0] for t in _all(store)} == {13}
+    store.resize(30)
+    assert store.pages == 30 and all(torch.equal(a[:, :12], b) for a, b in zip(store.pools(), held)) and len(store.pools()) == len(held)
+
+
+def _all(store):
+    return [t for t in ([store.k, store.v, store.k_scale, store.v_scale] if store.slots is None else [*store.k, *store.v]) if t is not None]
+
+
+@pytest.mark.parametrize("which", range(3))
+@pytest.mark.parametrize("after", [0, 1])
+def test_a_pool_shrinks_where_there_is_no_room_for_both(which, after):
+    store = _stores()[which]
+    held = _filled(store)
+    with ShortOfMemory(after, 1):                             # (there is room once the old one is gone)
+        store.resize(5)
+    assert store.pages == 5 and all(torch.equal(a, b[:, :5]) for a, b in zip(store.pools(), held))
+    if store.slots is not None:
+        assert store.k[2] is store.k[0] and store.v[2] is store.v[0]
