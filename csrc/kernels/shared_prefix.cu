@@ -75,7 +75,19 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
   const int split = shared ? blockIdx.z : blockIdx.z - a.splits;
   const int g = group_of(a.first, a.groups, at);
   const int begin = max(0, a.first[g]), end = min(a.rows, a.first[g + 1]);
-  if (at < begin || at >= end) return;                   // (places that no group holds)
+  if (tid == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+    for (int i = at; i < a.groups; i += a.rows)
+      if (a.first[i] > a.first[i + 1]) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+  if (at < begin || at >= end) {                         // (a place that no group holds: its row is reported, and sees nothing)
+    if (tid == 0) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
+    const int row = a.order[at];
+    if (tid < heads && row >= 0 && row < a.rows) {
+      const long long to_part = (static_cast<long long>(blockIdx.z) * a.rows + row) * a.heads + head0 + tid;
+      a.part_m[to_part] = -INFINITY;
+      a.part_l[to_part] = 0.f;
+    }
+    return;
+  }
   const int together = shared ? max(1, QUERIES / heads) : 1;
   if (shared && (at - begin) % together != 0) return;
   const int n_rows = min(together, end - at), n = n_rows * heads;

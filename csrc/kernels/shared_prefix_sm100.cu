@@ -278,10 +278,15 @@ __device__ __forceinline__ void fetch_queries(uint8_t* to, int apart, const Args
 }
 
 // What the second kernel needs of a place: its group's first unit and tiles (of either kind), its own; its group's first place and queries a key head (0: wide), units a CTA.
+// (Nothing for a place that no group holds: group 0's lists, counted from there, would end past the scratch.)
 __device__ __forceinline__ void write_plan(const Lists& s, const Args& a) {
   const int lists = a.kv_heads * a.chunks;
 #pragma unroll 1
   for (int i = threadIdx.x; i < a.rows; i += blockDim.x) {
+    if (s.row[i] < 0) {
+      a.plan[2 * i] = a.plan[2 * i + 1] = make_int4(0, 0, 0, 0);
+      continue;
+    }
     const int g = s.group[i], queries = group_queries(s, a, g);
     const Ranges both = ranges(s.lo[g], s.hi[g], 0, 0, a.box);
     const bool tall = queries > WN;
@@ -324,6 +329,7 @@ __device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines)
   for (int g = tid; g <= a.groups; g += THREADS) {
     s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
     if (g == a.groups) break;
+    if (blockIdx.x == 0 && a.first[g] > a.first[g + 1]) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
     s.lo[g] = 0;
     s.hi[g] = min(max(a.tokens[g], 0), most);
     live[g] = 0;

@@ -158,7 +158,8 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     dim]``; rows of length 0 give zeros.  Pools ``[pages, page, kv heads, dim]``, ``table [rows, columns]``.  A ``window`` leaves a row its last keys, ``softcap`` and ``sinks`` are
     those of ``ops.attention``.  ``shared`` says what is read once for several rows; it does not change what is computed.
 
-    Page numbers, lengths and rows that lie outside their tensors, and rows that ``order`` names twice, are reported by the status word (``library.check_status``) and read nothing."""
+    Page numbers, lengths and rows that lie outside their tensors, rows that ``order`` names twice, places that no group holds and groups that begin behind their end are
+    reported by the status word (``library.check_status``) and read nothing."""
     _check(q, k, v, table, lengths, shared, window, softcap, sinks, k_scale, v_scale)
     R, H, D = q.shape
     if R == 0:
