@@ -63,6 +63,17 @@ class _Row:
     pending_first: bool = False
 
 
+class _Methods(torch.nn.Module):
+    """A method of ``model`` as a module's call."""
+
+    def __init__(self, model):
+        super().__init__()
+        self.model = model
+
+    def forward(self, method: str, hidden: torch.Tensor) -> torch.Tensor:
+        return getattr(self.model, method)(hidden)
+
+
 class Server:
     def __init__(self, model, variables=None, *, slots: int, capacity: int, kv_cache: Optional[KVCache] = None,
                  chunk: Optional[int] = None, prefix_cache: bool = True, decode_steps: int = 1, sampling: Optional[Sampling] = None,
@@ -108,12 +119,7 @@ class Server:
         self.steps = 0
         self.wait_s = 0.0
         self.decoded_tokens = 0
-        if variables is None:
-            self._call = lambda t, **kw: model(t, **kw)
-        else:
-            from ..utils.trees import variables_for_call
-            named = variables_for_call(model, variables)
-            self._call = lambda t, **kw: torch.func.functional_call(model, named, (t,), kw)
+        self._bind(variables)
 
     # ------------------------------------------------------------------ construction / API
     @classmethod
@@ -214,10 +220,20 @@ class Server:
 
     def reload(self, variables) -> None:
         self.variables = variables
+        self._bind(variables)
+        self._graph = None
+
+    def _bind(self, variables) -> None:
+        """``_call``: the model with these variables (None: its own weights); ``_head``: one of its methods on hidden states, with the same."""
+        if variables is None:
+            self._call = lambda t, **kw: self.model(t, **kw)
+            self._head = lambda method, hidden: getattr(self.model, method)(hidden)
+            return
         from ..utils.trees import variables_for_call
         named = variables_for_call(self.model, variables)
+        methods, of_methods = _Methods(self.model), {f"model.{n}": t for n, t in named.items()}
         self._call = lambda t, **kw: torch.func.functional_call(self.model, named, (t,), kw)
-        self._graph = None
+        self._head = lambda method, hidden: torch.func.functional_call(methods, of_methods, (method, hidden))
 
     def __call__(self, prompts: Sequence[Any], max_new_tokens: int = 32) -> List[List[int]]:
         tickets = [self.submit(p, max_new_tokens) for p in prompts]
@@ -299,7 +315,7 @@ class Server:
                 if hasattr(self.model, "logits"):
                     hidden = self._call(ids, positions=pos, cache=self.store.select(slots), return_hidden=True)
                     picked = hidden[torch.arange(len(members), device=self.device), torch.tensor(last, device=self.device)]
-                    last_logits = self.model.logits(picked)
+                    last_logits = self._head("logits", picked)
                 else:
                     full = self._call(ids, positions=pos, cache=self.store.select(slots))
                     last_logits = full[torch.arange(len(members), device=self.device), torch.tensor(last, device=self.device)]
@@ -369,9 +385,9 @@ class Server:
             hidden = self._call(self.last_tokens[:, None], positions=self._in_pos[:, None], cache=self.store.select(None),
                                 return_hidden=True)[:, 0]
             if greedy:
-                nxt = self.model.next_tokens_greedy(hidden)
+                nxt = self._head("next_tokens_greedy", hidden)
             else:
-                self._logits = self.model.logits(hidden)
+                self._logits = self._head("logits", hidden)
                 nxt = self._logits.argmax(-1)
         self.last_tokens.copy_(torch.where(self._in_pos >= 0, nxt, self.last_tokens))
 

@@ -6,8 +6,10 @@ from torch.overrides import TorchFunctionMode
 from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
 from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore
+from dew_b200.sampling.text import Sampling
+from dew_b200.utils.trees import module_variables, tree_map
 
-CONFIG = dict(vocab_size=64, emb_features=32, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, mlp_features=48, max_seq_len=160)
+CONFIG = dict(vocab_size=64, emb_features=32, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, mlp_features=48, max_seq_len=160, tie_embeddings=False)
 
 
 def model(seed=0, **kw):
@@ -110,3 +112,32 @@ def test_a_pool_shrinks_where_there_is_no_room_for_both(which, after):
     assert store.pages == 5 and all(torch.equal(a, b[:, :5]) for a, b in zip(store.pools(), held))
     if store.slots is not None:
         assert store.k[2] is store.k[0] and store.v[2] is store.v[0]
+
+
+# ---------------------------------------------------------------------------------------------------------- weights given as variables
+PROMPTS = [list(range(3, 25)), [9, 8, 7]]
+
+
+def variables_of(m):
+    return tree_map(lambda t: t.detach().clone(), module_variables(m))
+
+
+def alone(m, prompt, variables=None, new=8):
+    return Server(m, variables, slots=1, capacity=160, kv_cache=KVCache(page_size=8), prefix_cache=False)([prompt], new)[0]
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("temperature", [0.0, 0.02])
+def test_variables_reach_the_head(tied, temperature):
+    def tokens(m, variables=None, reloaded=None):
+        server = Server(m, variables, slots=2, capacity=160, kv_cache=KVCache(page_size=8), prefix_cache=False, sampling=Sampling(temperature=temperature))
+        if reloaded is not None:
+            server.reload(reloaded)
+        return server(PROMPTS, 8)
+    ours, theirs = model(0, tie_embeddings=tied), model(7, tie_embeddings=tied)
+    for m in (ours, theirs):
+        m.embed.weight.data.mul_(0.05)                        # (a tied head repeats its input otherwise)
+    want = tokens(theirs)
+    assert want != tokens(ours)
+    assert tokens(ours, variables_of(theirs)) == want
+    assert tokens(ours, None, variables_of(theirs)) == want
