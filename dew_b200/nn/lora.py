@@ -73,7 +73,7 @@ def apply_lora(model: nn.Module, targets: Iterable[str] = ("qkv_proj", "o_proj")
             p.requires_grad_(False)
     for path, module in list(model.named_modules()):
         for name, child in list(module.named_children()):
-            if isinstance(child, Linear) and any(p.search(name) for p in pats):
+            if isinstance(child, Linear) and not isinstance(child, AdaptedLinear) and any(p.search(name) for p in pats):
                 setattr(module, name, LoRALinear(child, rank, alpha, dropout))
                 wrapped.append(f"{path}.{name}" if path else name)
     return wrapped
@@ -187,7 +187,7 @@ def apply_lora_config(model: nn.Module, cfg: LoRAConfig) -> List[str]:
             p.requires_grad_(False)
     for path, module in list(model.named_modules()):
         for name, child in list(module.named_children()):
-            if not (isinstance(child, Linear) and any(p.search(name) for p in pats)):
+            if not isinstance(child, Linear) or isinstance(child, AdaptedLinear) or not any(p.search(name) for p in pats):
                 continue
             full = f"{path}.{name}" if path else name
             rank = next((r for pat, r in cfg.rank_pattern.items() if re.search(pat, full)), cfg.rank)
@@ -261,37 +261,45 @@ def from_peft_state(state: Mapping[str, torch.Tensor]) -> Dict[str, torch.Tensor
 # Serving: adapters of many requests beside one copy of the weights
 
 
-class AdaptedLinear(nn.Module):
-    """A ``Linear`` beside which every token may have an adapter of its own, as ``bank.using`` says; without it, the ``Linear``."""
+class AdaptedLinear(Linear):
+    """A ``Linear`` beside which every token may have an adapter of its own, as ``bank.using`` says; without it, the ``Linear``.  It stands in for ``base`` with the same
+    parameters under the same names (and the same hooks): variables, checkpoints and optimisers of the model without a bank are those of the model with one."""
 
     def __init__(self, base: Linear, bank: "AdapterBank"):
-        super().__init__()
-        self.base = base
+        if "forward" in base.__dict__:
+            raise ValueError("a Linear whose forward has been replaced cannot have adapters beside it")
+        self.__dict__.update(base.__dict__)
         self._of = (bank,)                                 # (not a module of this one)
-        w = base.weight
+        w = self.weight
         rank = -(-bank.rank // 8) * 8 if w.dtype == torch.bfloat16 else bank.rank            # (rows of b that begin at 16 bytes are fetched as blocks)
-        self.register_buffer("a", torch.zeros(bank.slots, rank, base.in_features, dtype=w.dtype, device=w.device), persistent=False)
-        self.register_buffer("b", torch.zeros(bank.slots, base.out_features, rank, dtype=w.dtype, device=w.device), persistent=False)
+        self.register_buffer("a", torch.zeros(bank.slots, rank, self.in_features, dtype=w.dtype, device=w.device), persistent=False)
+        self.register_buffer("b", torch.zeros(bank.slots, self.out_features, rank, dtype=w.dtype, device=w.device), persistent=False)
         self.register_buffer("scale", torch.zeros(bank.slots, dtype=torch.float32, device=w.device), persistent=False)
 
-    @property
-    def weight(self):
-        return self.base.weight
+    def opened(self) -> Tuple[nn.Module, str, Linear]:
+        """``(module, name, layer)`` of a ``Linear`` of its own that holds the parameters from here on, for what replaces layers by others (``nn.quantization``)."""
+        if "base" not in self._modules:
+            base = Linear.__new__(Linear)
+            nn.Module.__init__(base)
+            base.in_features, base.out_features, base.init_std, base.zero_init = self.in_features, self.out_features, self.init_std, self.zero_init
+            base._parameters, self._parameters = self._parameters, {}
+            if "bias" in self.__dict__:                    # (None: not among the parameters)
+                base.bias = self.__dict__.pop("bias")
+            base.training = self.training
+            self.base = base
+        return self, "base", self.base
 
-    @property
-    def bias(self):
-        return self.base.bias
+    def __getattr__(self, name):
+        if name in ("weight", "bias") and "base" in self.__dict__["_modules"]:
+            return getattr(self.base, name)
+        return super().__getattr__(name)
 
-    @property
-    def in_features(self):
-        return self.base.in_features
-
-    @property
-    def out_features(self):
-        return self.base.out_features
+    def reset_parameters(self, generator: Optional[torch.Generator] = None):
+        if "base" not in self._modules:
+            super().reset_parameters(generator)
 
     def forward(self, x):
-        y = self.base(x)
+        y = self.base(x) if "base" in self._modules else super().forward(x)
         ids = self._of[0].ids_for(x.shape[:-1])
         return y if ids is None else adapters.add_adapters(y, x, adapters.Bank(self.a, self.b, self.scale), ids)
 

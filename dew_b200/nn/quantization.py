@@ -133,6 +133,11 @@ class QuantizedLinear(nn.Module):
         return ops.linear(x, self.weight.to(x.dtype), self.bias)
 
 
+def _place(module: nn.Module, name: str, child):
+    """``(module, name, layer)`` of what is to be replaced: a layer that adapters stand beside (``nn.lora.AdaptedLinear``) keeps them, and the ``Linear`` inside it goes."""
+    return child.opened() if hasattr(child, "opened") else (module, name, child)
+
+
 def quantize_model(model: nn.Module, q: Quantization) -> Dict[str, int]:
     """Replace every eligible ``Linear`` of ``model`` in place by a ``QuantizedLinear``; returns bytes before / after."""
     from .layers import Linear
@@ -141,10 +146,11 @@ def quantize_model(model: nn.Module, q: Quantization) -> Dict[str, int]:
         for name, child in list(module.named_children()):
             full = f"{path}.{name}" if path else name
             if isinstance(child, Linear) and child.weight.numel() >= q.min_size and not any(s in full for s in q.skip):
+                where, at, child = _place(module, name, child)
                 ql = QuantizedLinear.from_linear(child, q.kind)
                 before += child.weight.numel() * child.weight.element_size()
                 after += ql.bytes()
-                setattr(module, name, ql)
+                setattr(where, at, ql)
     return {"bytes_before": before, "bytes_after": after}
 
 
@@ -172,7 +178,8 @@ def prepare_qat(model: nn.Module, q: Quantization) -> int:
         for name, child in list(module.named_children()):
             full = f"{path}.{name}" if path else name
             if isinstance(child, Linear) and child.weight.numel() >= q.min_size and not any(s in full for s in q.skip):
-                setattr(module, name, QATLinear(child, q.kind))
+                where, at, child = _place(module, name, child)
+                setattr(where, at, QATLinear(child, q.kind))
                 n += 1
     return n
 

@@ -4,8 +4,12 @@ import torch
 from torch.overrides import TorchFunctionMode
 
 from dew_b200.inference.serving import Server
+from dew_b200.inference.tasks import TextGeneration
 from dew_b200.models import CausalTransformer
 from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore
+from dew_b200.nn.layers import reset_all
+from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
+from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
 from dew_b200.sampling.text import Sampling
 from dew_b200.utils.trees import module_variables, tree_map
 
@@ -141,3 +145,82 @@ def test_variables_reach_the_head(tied, temperature):
     assert want != tokens(ours)
     assert tokens(ours, variables_of(theirs)) == want
     assert tokens(ours, None, variables_of(theirs)) == want
+
+
+# ---------------------------------------------------------------------------------------------------------- a bank of adapters and the model's weights
+TARGETS = ("qkv_proj", "o_proj", "down_proj")
+
+
+def adapter(seed, rank=4, base=0):
+    """An adapter as training leaves it on ``model(base)``, and the model that has it merged into its weights."""
+    m = model(base)
+    apply_lora(m, TARGETS, rank=rank, alpha=2.0 * rank)
+    g = torch.Generator().manual_seed(seed)
+    for n, p in m.named_parameters():
+        if ".lora_b" in n:
+            p.data.normal_(0.0, 0.2, generator=g)
+    state = lora_state(m)
+    merge_all(m)
+    return state, m
+
+
+def test_variables_reach_the_layers_of_a_bank():
+    want = [alone(model(7), p) for p in PROMPTS]
+    assert want != [alone(model(0), p) for p in PROMPTS]
+    state, merged = adapter(1, base=7)
+    m = model(0)
+    bank = AdapterBank(m, TARGETS, slots=2, rank=4)
+    bank.load("one", state, alpha=8.0)
+    make = dict(slots=3, capacity=160, kv_cache=KVCache(page_size=8), adapters=bank)
+    for server in (Server(m, variables_of(model(7)), **make), Server.from_task(TextGeneration(m, variables_of(model(7))), **make)):
+        plain, adapted = [server.submit(p, 8) for p in PROMPTS], server.submit(PROMPTS[0], 8, adapter="one")
+        server.run()
+        assert [t.result() for t in plain] == want and adapted.result() == alone(merged, PROMPTS[0])
+    server = Server(m, **make)
+    assert server(PROMPTS, 8) == [alone(model(0), p) for p in PROMPTS]
+    server = Server(m, prefix_cache=False, **make)
+    server.reload(variables_of(model(7)))
+    assert server(PROMPTS, 8) == want
+
+
+def test_a_bank_changes_no_name_of_the_model():
+    m, plain = model(), model()
+    AdapterBank(m, TARGETS, slots=2, rank=4)
+    assert [n for n, _ in m.named_parameters()] == [n for n, _ in plain.named_parameters()] and list(m.state_dict()) == list(plain.state_dict())
+    m.load_state_dict(model(7).state_dict())
+    assert alone(m, PROMPTS[0]) == alone(model(7), PROMPTS[0])
+    other = model(3)
+    AdapterBank(other, TARGETS, slots=1, rank=2)
+    reset_all(other, 5), reset_all(plain, 5)
+    assert all(torch.equal(a, b) for a, b in zip(other.parameters(), plain.parameters()))
+
+
+def test_layers_of_a_bank_can_still_be_quantised_and_watched():
+    state, merged = adapter(1)
+    m, plain = model(), model()
+    seen = []
+    m.layers[0].mixer.qkv_proj.register_forward_hook(lambda mod, args, out: seen.append(out.shape))
+    bank = AdapterBank(m, TARGETS, slots=2, rank=4)
+    bank.load("one", state, alpha=8.0)
+    q = Quantization("int8", min_size=0, skip=("embed",))
+    assert quantize_model(m, q) == quantize_model(plain, q)
+    ids = torch.tensor([[1, 2, 3, 4]])
+    with torch.no_grad():
+        want = plain(ids)
+        assert torch.equal(m(ids), want) and seen
+        with bank.using(torch.tensor([0], dtype=torch.int32)):
+            got = m(ids)
+    assert not torch.allclose(got, want, atol=1e-2) and torch.allclose(got, merged(ids), atol=0.2)
+    assert m.layers[0].mixer.qkv_proj.weight.shape == plain.layers[0].mixer.qkv_proj.weight.shape
+    m = model()
+    AdapterBank(m, TARGETS, slots=2, rank=4)
+    assert prepare_qat(m, q) == prepare_qat(model(), q)
+    with torch.no_grad():
+        m(ids)
+    assert convert_qat(m) == convert_qat(_qat(q))
+
+
+def _qat(q):
+    m = model()
+    prepare_qat(m, q)
+    return m
