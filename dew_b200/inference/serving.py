@@ -61,6 +61,7 @@ class _Row:
     prefilled: int = 0          # prompt tokens already in the cache
     generated: int = 0
     pending_first: bool = False
+    salt: bytes = b""           # what beside the tokens its pages depend on
 
 
 class _Methods(torch.nn.Module):
@@ -119,6 +120,7 @@ class Server:
         self.steps = 0
         self.wait_s = 0.0
         self.decoded_tokens = 0
+        self._reloads, self._weights = 0, b""              # what the pages' names begin with
         self._bind(variables)
 
     # ------------------------------------------------------------------ construction / API
@@ -222,6 +224,8 @@ class Server:
         self.variables = variables
         self._bind(variables)
         self._graph = None
+        self._reloads += 1
+        self._weights = f"weights {self._reloads}/".encode()       # (pages of the old ones, or begun with them, are nobody's prefix from here on)
 
     def _bind(self, variables) -> None:
         """``_call``: the model with these variables (None: its own weights); ``_head``: one of its methods on hidden states, with the same."""
@@ -262,13 +266,14 @@ class Server:
                 continue
             t = self.queue[0]
             try:
-                seat = self.ledger.seat(t.prompt, len(t.prompt) + t.max_new_tokens, t.salt)
+                salt = self._weights + t.salt
+                seat = self.ledger.seat(t.prompt, len(t.prompt) + t.max_new_tokens, salt)
             except OutOfPages:
                 break
             self.queue.popleft()
             table = self.store.page_table[slot]
             table[: len(seat.pages)] = torch.tensor(seat.pages, dtype=torch.int32, device=self.device)
-            self.rows[slot] = _Row(t, seat.pages, prefilled=seat.reused_tokens)
+            self.rows[slot] = _Row(t, seat.pages, prefilled=seat.reused_tokens, salt=salt)
             self._layout += 1
             if self._row_adapters is not None:
                 self._row_adapters[slot] = t.adapter_slot
@@ -324,7 +329,7 @@ class Server:
             for i, (s, r) in enumerate(members):
                 r.prefilled += last[i] + 1
                 if r.prefilled >= len(r.ticket.prompt):
-                    self.ledger.publish(r.ticket.prompt, r.pages, r.ticket.salt)
+                    self.ledger.publish(r.ticket.prompt, r.pages, r.salt)
                     tok = self._draw(last_logits[i][None], r, 0)
                     self.last_tokens[s] = tok
                     r.pending_first = True

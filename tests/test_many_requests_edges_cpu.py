@@ -224,3 +224,18 @@ def _qat(q):
     m = model()
     prepare_qat(m, q)
     return m
+
+
+@pytest.mark.parametrize("host_pages", [0, 8])
+def test_pages_of_other_weights_are_no_prefix(host_pages):
+    prompts = [list(range(3, 25)), list(range(3, 45)), list(range(3, 25))]
+    want = [alone(model(7), p) for p in prompts]
+    server = Server(model(0), slots=2, capacity=160, kv_cache=KVCache(page_size=8, pages=9 if host_pages else None), chunk=16, host_pages=host_pages)
+    server(prompts[:1], 8)
+    late = server.submit(prompts[1], 8)
+    server.step()                                             # a prompt half way through when the weights change: its pages are of both
+    server.reload(variables_of(model(7)))
+    server.run()
+    hits = server.ledger.hits
+    assert [server([p], 8)[0] for p in prompts] == want and len(late.result()) == 8
+    assert server.ledger.hits == hits + 2 + 2                 # the two whole pages that all three begin with, of the new weights
