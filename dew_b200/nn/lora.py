@@ -272,9 +272,16 @@ class AdaptedLinear(Linear):
         self._of = (bank,)                                 # (not a module of this one)
         w = self.weight
         rank = -(-bank.rank // 8) * 8 if w.dtype == torch.bfloat16 else bank.rank            # (rows of b that begin at 16 bytes are fetched as blocks)
-        self.register_buffer("a", torch.zeros(bank.slots, rank, self.in_features, dtype=w.dtype, device=w.device), persistent=False)
-        self.register_buffer("b", torch.zeros(bank.slots, self.out_features, rank, dtype=w.dtype, device=w.device), persistent=False)
-        self.register_buffer("scale", torch.zeros(bank.slots, dtype=torch.float32, device=w.device), persistent=False)
+        # (the bank's, not the model's: no buffers, which variables would take along)
+        self.a = torch.zeros(bank.slots, rank, self.in_features, dtype=w.dtype, device=w.device)
+        self.b = torch.zeros(bank.slots, self.out_features, rank, dtype=w.dtype, device=w.device)
+        self.scale = torch.zeros(bank.slots, dtype=torch.float32, device=w.device)
+
+    def _apply(self, fn, recurse=True):
+        """``to`` and its like: the scales stay as they are, in fp32."""
+        super()._apply(fn, recurse)
+        self.a, self.b, self.scale = fn(self.a), fn(self.b), self.scale.to(fn(self.scale).device)
+        return self
 
     def opened(self) -> Tuple[nn.Module, str, Linear]:
         """``(module, name, layer)`` of a ``Linear`` of its own that holds the parameters from here on, for what replaces layers by others (``nn.quantization``)."""

@@ -11,7 +11,7 @@ from dew_b200.nn.layers import reset_all
 from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
 from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
 from dew_b200.sampling.text import Sampling
-from dew_b200.utils.trees import module_variables, tree_map
+from dew_b200.utils.trees import flatten, module_variables, tree_map
 
 CONFIG = dict(vocab_size=64, emb_features=32, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=16, mlp_features=48, max_seq_len=160, tie_embeddings=False)
 
@@ -239,3 +239,32 @@ def test_pages_of_other_weights_are_no_prefix(host_pages):
     hits = server.ledger.hits
     assert [server([p], 8)[0] for p in prompts] == want and len(late.result()) == 8
     assert server.ledger.hits == hits + 2 + 2                 # the two whole pages that all three begin with, of the new weights
+
+
+def test_variables_bring_no_adapters_along():
+    """What stands in a bank is the bank's: a copy of the model's variables, taken earlier, says nothing about it."""
+    state, merged = adapter(1)
+    m = model()
+    bank = AdapterBank(m, TARGETS, slots=2, rank=4)
+    early = variables_of(m)
+    bank.load("one", state, alpha=8.0)
+    server = Server(m, early, slots=1, capacity=160, kv_cache=KVCache(page_size=8), adapters=bank)
+    ticket = server.submit(PROMPTS[0], 8, adapter="one")
+    server.run()
+    assert ticket.result() == alone(merged, PROMPTS[0])
+    assert set(flatten(early)) == set(flatten(variables_of(model())))
+
+
+def test_a_bank_moves_with_its_model():
+    state, _ = adapter(1)
+    m = model()
+    bank = AdapterBank(m, TARGETS, slots=2, rank=4)
+    bank.load("one", state, alpha=8.1)
+    layer = bank.layers["layers.0.mixer.qkv_proj"]
+    scale = layer.scale
+    m.to(torch.bfloat16)
+    assert layer.a.dtype == layer.b.dtype == torch.bfloat16 and torch.equal(layer.scale, scale) and layer.scale.dtype == torch.float32 and layer.a.any()
+    with torch.no_grad(), bank.using(torch.tensor([0], dtype=torch.int32)):
+        m(torch.tensor([[1, 2, 3]]))
+    m.to("meta")
+    assert layer.a.device.type == layer.b.device.type == layer.scale.device.type == "meta"
