@@ -750,11 +750,12 @@ class PackedRows:
 
     @staticmethod
     def suits(store: KVStore, model) -> bool:
-        """Whether the model's layers are attention over this store alone and nothing in them looks at a token's neighbours by index or at other ranks, the kernels take
-        its heads, and no hook may see that its calls are given one row of tokens."""
+        """Whether the model's layers are attention over this store alone and nothing in them looks at a token's neighbours by index, at its row (as rows' adapters do) or at other
+        ranks, the kernels take its heads, and no hook may see that its calls are given one row of tokens."""
         from ..models.causal_transformer import CausalTransformer
         from ..utils.hooks import watched
         from .attention import SelfAttention
+        from .lora import AdaptedLinear
         if not (store.slots is None and store.kind == 0 and store.dtype == torch.bfloat16 and store.device.type == "cuda" and store.row_ids is None and store.head_dim in (64, 128)
                 and type(model) is CausalTransformer and L.env("DEWB_FORCE_REFERENCE") != "1" and L.env("DEWB_KERNEL_ATTENTION") is None
                 and hasattr(L.load(), "dewb_flash_fwd_rows")):
@@ -770,7 +771,7 @@ class PackedRows:
             if type(m) is not SelfAttention or layer.cross is not None or layer.streams is not None or m.num_heads % m.num_kv_heads or m.num_kv_heads != store.kv_heads \
                     or m.head_dim != store.head_dim or (layer.sparse and getattr(layer.mlp, "mix", None) is not None and layer.mlp.mix.capacity_factor is not None):
                 return False
-        return not watched(model)
+        return not watched(model) and not any(type(m) is AdaptedLinear and m.in_use for m in model.modules())
 
     @staticmethod
     def pays(store: KVStore, lengths: Sequence[int], width: int) -> bool:

@@ -283,6 +283,11 @@ class AdaptedLinear(Linear):
         self.a, self.b, self.scale = fn(self.a), fn(self.b), self.scale.to(fn(self.scale).device)
         return self
 
+    @property
+    def in_use(self) -> bool:
+        """Whether the calls of now have adapters (``AdapterBank.using``)."""
+        return self._of[0]._ids is not None
+
     def opened(self) -> Tuple[nn.Module, str, Linear]:
         """``(module, name, layer)`` of a ``Linear`` of its own that holds the parameters from here on, for what replaces layers by others (``nn.quantization``)."""
         if "base" not in self._modules:

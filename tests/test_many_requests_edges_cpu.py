@@ -1,4 +1,6 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 from torch.overrides import TorchFunctionMode
@@ -6,7 +8,7 @@ from torch.overrides import TorchFunctionMode
 from dew_b200.inference.serving import Server
 from dew_b200.inference.tasks import TextGeneration
 from dew_b200.models import CausalTransformer
-from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore
+from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore, PackedRows
 from dew_b200.nn.layers import reset_all
 from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
 from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
@@ -268,3 +270,15 @@ def test_a_bank_moves_with_its_model():
         m(torch.tensor([[1, 2, 3]]))
     m.to("meta")
     assert layer.a.device.type == layer.b.device.type == layer.scale.device.type == "meta"
+
+
+def test_prompts_behind_one_another_are_not_for_rows_with_adapters():
+    store = SimpleNamespace(slots=None, kind=0, dtype=torch.bfloat16, device=torch.device("cuda"), row_ids=None, head_dim=16 * 4, kv_heads=2)
+    m = model(head_dim=64)
+    assert PackedRows.suits(store, m)
+    bank = AdapterBank(m, TARGETS, slots=2, rank=4)
+    assert PackedRows.suits(store, m)
+    with bank.using(torch.tensor([0, -1, 1], dtype=torch.int32)):
+        assert not PackedRows.suits(store, m)
+        with bank.using(None):
+            assert PackedRows.suits(store, m)

@@ -4,8 +4,12 @@ import math
 import pytest
 import torch
 
+from dew_b200.models import CausalTransformer
+from dew_b200.nn.kv_cache import PackedRows
+from dew_b200.nn.lora import AdapterBank
 from dew_b200.ops import library as L
 from dew_b200.ops.prefix import Shared, shared_decode
+from dew_b200.sampling.text import RowBatch, generate
 from prefix_cases import allowed, batch, truth
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +49,35 @@ def test_rows_that_no_group_holds_are_reported_and_give_zeros(dtype, heads, kv, 
 def test_groups_that_begin_behind_their_end_are_reported(dtype, dim, first):
     a = batch([(64, [3, 4, 5, 6, 7, 8])], 4, 2, dim, 16, dtype, device=DEV)
     reported({**a, "shared": Shared(a["shared"].order, ints(first), ints([64, 64, 64]))})
+
+
+# ---------------------------------------------------------------------------------------------------------- adapters
+CONFIG = dict(vocab_size=96, emb_features=128, num_layers=2, num_heads=4, num_kv_heads=2, head_dim=64, mlp_features=256, max_seq_len=512, tie_embeddings=False)
+TARGETS = ("qkv_proj", "o_proj", "gate_up_proj", "down_proj")
+
+
+def banked(dtype=BF16, seed=0):
+    torch.manual_seed(seed)
+    m = CausalTransformer(**CONFIG).eval().to(DEV, dtype)
+    bank = AdapterBank(m, TARGETS, slots=3, rank=8)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    for layer in bank.layers.values():
+        for t in (layer.a, layer.b):
+            t.copy_(torch.randn(t.shape, generator=g, device=DEV) * 0.1)
+        layer.scale.fill_(1.0)
+    return m, bank
+
+
+def test_rows_of_prompts_behind_one_another_keep_their_adapters(monkeypatch):
+    m, bank = banked()
+    prompts = [[1 + (i * 7 + j) % 90 for j in range(n)] for i, n in enumerate((300, 20, 150, 9))]
+    packed, plain = [], RowBatch._prefill_packed
+    monkeypatch.setattr(RowBatch, "_prefill_packed", lambda *a: packed.append(1) or plain(*a))
+    generate(m, None, prompts, 2)
+    assert packed                                             # (what such prompts take without adapters)
+    with bank.using(ints([0, -1, 2, 1])):
+        got = generate(m, None, prompts, 4)
+        monkeypatch.setattr(PackedRows, "pays", staticmethod(lambda *a: False))
+        want = generate(m, None, prompts, 4)
+    assert len(packed) == 1 and torch.equal(got.tokens, want.tokens)
+    L.check_status()
