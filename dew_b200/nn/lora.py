@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import math
 import re
+import threading
 from typing import Dict, Iterable, List, Optional
 
 import torch
@@ -286,7 +287,7 @@ class AdaptedLinear(Linear):
     @property
     def in_use(self) -> bool:
         """Whether the calls of now have adapters (``AdapterBank.using``)."""
-        return self._of[0]._ids is not None
+        return self._of[0]._now()[0] is not None
 
     def opened(self) -> Tuple[nn.Module, str, Linear]:
         """``(module, name, layer)`` of a ``Linear`` of its own that holds the parameters from here on, for what replaces layers by others (``nn.quantization``)."""
@@ -338,8 +339,10 @@ class AdapterBank:
         self.names: Dict[str, int] = {}                    # adapter -> slot
         self.version: Dict[str, int] = {}                  # how often something was loaded under that name
         self.holds: Dict[str, int] = {}                    # requests in flight
-        self._ids: Optional[torch.Tensor] = None
-        self._wide: Dict[Tuple[int, ...], torch.Tensor] = {}
+        self._calls: Dict[int, Tuple[Optional[torch.Tensor], Dict]] = {}      # thread -> the ids of its calls, and those spread over tokens
+
+    def _now(self) -> Tuple[Optional[torch.Tensor], Dict]:
+        return self._calls.get(threading.get_ident(), (None, {}))
 
     def load(self, name: str, state: Mapping[str, torch.Tensor], alpha: float, rs: bool = False) -> int:
         """Put an adapter under ``name`` (in place of one that is not in use); returns its slot.  Its scale is ``alpha / rank``, or ``alpha / sqrt(rank)`` with ``rs``, by each
@@ -396,23 +399,29 @@ class AdapterBank:
 
     @contextmanager
     def using(self, ids: Optional[torch.Tensor]):
-        """Rows' adapters (int32 ``[rows]`` on the model's device, below 0: none) for the calls inside.  The tensor is read when they run: a captured call follows its values."""
+        """Rows' adapters (int32 ``[rows]`` on the model's device, below 0: none) for this thread's calls inside.  The tensor is read when they run: a captured call follows its
+        values."""
         if ids is not None and (ids.dtype != torch.int32 or ids.dim() != 1):
             raise TypeError(f"one int32 id a row, got {ids.dtype} {tuple(ids.shape)}")
-        before = self._ids, self._wide
-        self._ids, self._wide = ids, {}
+        thread = threading.get_ident()
+        before = self._calls.get(thread)
+        self._calls[thread] = (ids, {})
         try:
             yield self
         finally:
-            self._ids, self._wide = before
+            if before is None:
+                del self._calls[thread]
+            else:
+                self._calls[thread] = before
 
     def ids_for(self, shape) -> Optional[torch.Tensor]:
         """The ids of tokens ``[rows, ...]``."""
-        if self._ids is None:
+        ids, wide = self._now()
+        if ids is None:
             return None
         shape = tuple(shape)
-        if shape not in self._wide:
-            if not shape or shape[0] != self._ids.shape[0]:
-                raise ValueError(f"adapters of {self._ids.shape[0]} rows in a call of {shape}")
-            self._wide[shape] = self._ids.view(-1, *(1,) * (len(shape) - 1)).expand(shape).contiguous()
-        return self._wide[shape]
+        if shape not in wide:
+            if not shape or shape[0] != ids.shape[0]:
+                raise ValueError(f"adapters of {ids.shape[0]} rows in a call of {shape}")
+            wide[shape] = ids.view(-1, *(1,) * (len(shape) - 1)).expand(shape).contiguous()
+        return wide[shape]

@@ -1,4 +1,7 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
+import copy
+import threading
+from contextlib import nullcontext
 from types import SimpleNamespace
 
 import pytest
@@ -282,3 +285,49 @@ def test_prompts_behind_one_another_are_not_for_rows_with_adapters():
         assert not PackedRows.suits(store, m)
         with bank.using(None):
             assert PackedRows.suits(store, m)
+
+
+def random_bank(m, slots=2):
+    bank, g = AdapterBank(m, TARGETS, slots=slots, rank=4), torch.Generator().manual_seed(2)
+    for layer in bank.layers.values():
+        for t in (layer.a, layer.b):
+            t.copy_(torch.randn(t.shape, generator=g) * 0.2)
+        layer.scale.fill_(1.0)
+    return bank
+
+
+def test_every_thread_has_its_own_rows():
+    m = model()
+    bank = random_bank(m)
+    calls = [(torch.tensor(ids, dtype=torch.int32), torch.randint(60, (len(ids), 5), generator=torch.Generator().manual_seed(i))) for i, ids in enumerate(([0, 1], [1, 0], [-1, 1, 0]))]
+
+    def one(ids, tokens):
+        with torch.no_grad(), bank.using(ids):
+            return m(tokens)
+    want = [one(*c) for c in calls]
+    with torch.no_grad():
+        plain = m(calls[2][1])
+    together, got = threading.Barrier(4, timeout=20), [None] * 4
+
+    def work(i):
+        with torch.no_grad(), bank.using(calls[i][0]) if i < 3 else nullcontext():
+            together.wait()                                   # all are inside
+            got[i] = m(calls[min(i, 2)][1])
+            together.wait()
+    threads = [threading.Thread(target=work, args=(i,), daemon=True) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert all(x is not None and torch.equal(x, w) for x, w in zip(got, want + [plain]))
+
+
+def test_a_model_with_a_bank_is_copied_with_it():
+    m = model()
+    random_bank(m)
+    other = copy.deepcopy(m)
+    theirs = other.layers[0].mixer.qkv_proj._of[0]
+    assert theirs.layers["layers.0.mixer.qkv_proj"] is other.layers[0].mixer.qkv_proj
+    ids = torch.tensor([0], dtype=torch.int32)
+    with torch.no_grad(), theirs.using(ids), m.layers[0].mixer.qkv_proj._of[0].using(ids):
+        assert torch.equal(other(torch.tensor([[1, 2, 3]])), m(torch.tensor([[1, 2, 3]])))
