@@ -317,6 +317,9 @@ class AdaptedLinear(Linear):
         return y if ids is None else adapters.add_adapters(y, x, adapters.Bank(self.a, self.b, self.scale), ids)
 
 
+_BANKS = threading.RLock()       # what stands in banks, and who holds it, changes by one thread at a time
+
+
 class AdapterBank:
     """Room for ``slots`` adapters of rank up to ``rank`` beside the ``targets`` of ``model`` (regexes over the attribute names of its ``Linear`` layers, which are replaced).
     ``load`` takes what ``lora_state`` (or ``from_peft_state``) gives; ``using`` says which adapter each row of the calls inside it has.  For generation: the adapters take no
@@ -357,31 +360,33 @@ class AdapterBank:
             layer, a, b = self.layers[path], parts.get("lora_a"), parts.get("lora_b")
             if a is None or b is None or a.dim() != 2 or b.shape != (layer.out_features, a.shape[0]) or a.shape[1] != layer.in_features or not 0 < a.shape[0] <= self.rank:
                 raise ValueError(f"adapter {name!r}, {path}: lora_a [rank, {layer.in_features}] and lora_b [{layer.out_features}, rank] of rank up to {self.rank}")
-        self._free(name)
-        slot = self.names.get(name)
-        if slot is None:
-            taken = set(self.names.values())
-            slot = next((i for i in range(self.slots) if i not in taken), None)
+        with _BANKS:
+            self._free(name)
+            slot = self.names.get(name)
             if slot is None:
-                raise RuntimeError(f"the bank's {self.slots} slots are taken: {sorted(self.names)}")
-        with torch.no_grad():
-            for path, layer in self.layers.items():
-                parts = found.get(path)
-                layer.a[slot].zero_()
-                layer.b[slot].zero_()
-                layer.scale[slot] = 0.0
-                if parts is not None:
-                    r = parts["lora_a"].shape[0]
-                    layer.a[slot, :r] = parts["lora_a"].to(layer.a)
-                    layer.b[slot, :, :r] = parts["lora_b"].to(layer.b)
-                    layer.scale[slot] = alpha / (math.sqrt(r) if rs else r)
-        self.names[name] = slot
-        self.version[name] = self.version.get(name, 0) + 1
-        return slot
+                taken = set(self.names.values())
+                slot = next((i for i in range(self.slots) if i not in taken), None)
+                if slot is None:
+                    raise RuntimeError(f"the bank's {self.slots} slots are taken: {sorted(self.names)}")
+            with torch.no_grad():
+                for path, layer in self.layers.items():
+                    parts = found.get(path)
+                    layer.a[slot].zero_()
+                    layer.b[slot].zero_()
+                    layer.scale[slot] = 0.0
+                    if parts is not None:
+                        r = parts["lora_a"].shape[0]
+                        layer.a[slot, :r] = parts["lora_a"].to(layer.a)
+                        layer.b[slot, :, :r] = parts["lora_b"].to(layer.b)
+                        layer.scale[slot] = alpha / (math.sqrt(r) if rs else r)
+            self.names[name] = slot
+            self.version[name] = self.version.get(name, 0) + 1
+            return slot
 
     def remove(self, name: str) -> None:
-        self._free(name)
-        del self.names[name]
+        with _BANKS:
+            self._free(name)
+            del self.names[name]
 
     def _free(self, name: str) -> None:
         if self.holds.get(name):
@@ -389,13 +394,15 @@ class AdapterBank:
 
     def acquire(self, name: str) -> int:
         """The adapter's slot, held for a request until ``release``."""
-        if name not in self.names:
-            raise KeyError(f"no adapter {name!r}; loaded: {sorted(self.names)}")
-        self.holds[name] = self.holds.get(name, 0) + 1
-        return self.names[name]
+        with _BANKS:
+            if name not in self.names:
+                raise KeyError(f"no adapter {name!r}; loaded: {sorted(self.names)}")
+            self.holds[name] = self.holds.get(name, 0) + 1
+            return self.names[name]
 
     def release(self, name: str) -> None:
-        self.holds[name] -= 1
+        with _BANKS:
+            self.holds[name] -= 1
 
     @contextmanager
     def using(self, ids: Optional[torch.Tensor]):

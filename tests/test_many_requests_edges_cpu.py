@@ -1,5 +1,6 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
 import copy
+import sys
 import threading
 from contextlib import nullcontext
 from types import SimpleNamespace
@@ -320,6 +321,26 @@ def test_every_thread_has_its_own_rows():
     for t in threads:
         t.join(60)
     assert all(x is not None and torch.equal(x, w) for x, w in zip(got, want + [plain]))
+
+
+def test_holds_of_many_threads_are_counted():
+    bank = AdapterBank(model(), TARGETS, slots=2, rank=4)
+    bank.load("x", adapter(1)[0], alpha=8.0)
+    was = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        def work():
+            for _ in range(20000):
+                bank.acquire("x")
+                bank.release("x")
+        threads = [threading.Thread(target=work, daemon=True) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(60)
+    finally:
+        sys.setswitchinterval(was)
+    assert bank.holds["x"] == 0
 
 
 def test_a_model_with_a_bank_is_copied_with_it():
