@@ -427,8 +427,16 @@ class AdapterBank:
         if ids is None:
             return None
         shape = tuple(shape)
-        if shape not in wide:
-            if not shape or shape[0] != ids.shape[0]:
-                raise ValueError(f"adapters of {ids.shape[0]} rows in a call of {shape}")
-            wide[shape] = ids.view(-1, *(1,) * (len(shape) - 1)).expand(shape).contiguous()
-        return wide[shape]
+        if not shape or shape[0] != ids.shape[0]:
+            raise ValueError(f"adapters of {ids.shape[0]} rows in a call of {shape}")
+        spread = ids.view(-1, *(1,) * (len(shape) - 1)).expand(shape)
+        if spread.numel() == ids.numel():
+            return ids.view(shape)
+        # what the layers of one call share: not once the ids have changed, not across streams, and a captured call makes its own
+        if ids.is_inference() or (ids.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return spread.contiguous()
+        key = (shape, ids._version, torch.cuda.current_stream(ids.device).cuda_stream if ids.is_cuda else 0)
+        if key not in wide:
+            wide.clear()
+            wide[key] = spread.contiguous()
+        return wide[key]

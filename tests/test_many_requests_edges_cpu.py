@@ -352,3 +352,22 @@ def test_a_model_with_a_bank_is_copied_with_it():
     ids = torch.tensor([0], dtype=torch.int32)
     with torch.no_grad(), theirs.using(ids), m.layers[0].mixer.qkv_proj._of[0].using(ids):
         assert torch.equal(other(torch.tensor([[1, 2, 3]])), m(torch.tensor([[1, 2, 3]])))
+
+
+def test_ids_are_read_when_the_calls_run():
+    m = model()
+    bank, ids, tokens = random_bank(m), torch.tensor([0, -1], dtype=torch.int32), torch.tensor([[1, 2, 3], [4, 5, 6]])
+    other = torch.tensor([1, 0], dtype=torch.int32)
+    with torch.no_grad():
+        with bank.using(other):
+            want = m(tokens)
+        with bank.using(ids):
+            first = m(tokens)
+            ids.copy_(other)
+            assert torch.equal(m(tokens), want) and not torch.equal(first, want)
+    with torch.inference_mode():
+        ids = torch.tensor([0, -1], dtype=torch.int32)        # (which counts no versions)
+        with bank.using(ids):
+            m(tokens)
+            ids.copy_(other)
+            assert torch.equal(m(tokens), want)

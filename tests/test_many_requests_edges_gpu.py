@@ -81,3 +81,26 @@ def test_rows_of_prompts_behind_one_another_keep_their_adapters(monkeypatch):
         want = generate(m, None, prompts, 4)
     assert len(packed) == 1 and torch.equal(got.tokens, want.tokens)
     L.check_status()
+
+
+def test_captured_calls_of_several_tokens_follow_their_ids():
+    m, bank = banked()
+    tokens = torch.randint(96, (3, 7), device=DEV)
+    ids, later = ints([0, -1, 1]), ints([2, 0, -1])
+    with torch.no_grad():
+        with bank.using(later):
+            want = m(tokens)
+        with bank.using(ids):
+            eager = m(tokens)                                 # (a warm-up, and calls between and behind captures)
+            graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+            outs = []
+            for g in graphs:
+                with torch.cuda.graph(g):
+                    outs.append(m(tokens))
+                assert torch.equal(m(tokens), eager)
+            ids.copy_(later)
+            graphs[1].replay()
+            assert torch.equal(outs[1], want) and torch.equal(m(tokens), want)
+            graphs[0].replay()
+            assert torch.equal(outs[0], want)
+    L.check_status()
