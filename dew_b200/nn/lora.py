@@ -271,7 +271,7 @@ class AdaptedLinear(Linear):
             raise ValueError("a Linear whose forward has been replaced cannot have adapters beside it")
         self.__dict__.update(base.__dict__)
         self._of = (bank,)                                 # (not a module of this one)
-        w = self.weight
+        w = base.weight
         rank = -(-bank.rank // 8) * 8 if w.dtype == torch.bfloat16 else bank.rank            # (rows of b that begin at 16 bytes are fetched as blocks)
         # (the bank's, not the model's: no buffers, which variables would take along)
         self.a = torch.zeros(bank.slots, rank, self.in_features, dtype=w.dtype, device=w.device)
@@ -303,6 +303,8 @@ class AdaptedLinear(Linear):
         return self, "base", self.base
 
     def __getattr__(self, name):
+        if name == "weight" and self.in_use:
+            raise RuntimeError("the model multiplies with this layer's weight itself: adapters beside it would be passed over, so it cannot be a target of theirs")
         if name in ("weight", "bias") and "base" in self.__dict__["_modules"]:
             return getattr(self.base, name)
         return super().__getattr__(name)
@@ -312,7 +314,7 @@ class AdaptedLinear(Linear):
             super().reset_parameters(generator)
 
     def forward(self, x):
-        y = self.base(x) if "base" in self._modules else super().forward(x)
+        y = self.base(x) if "base" in self._modules else ops.linear(x, self._parameters["weight"], self.bias)
         ids = self._of[0].ids_for(x.shape[:-1])
         return y if ids is None else adapters.add_adapters(y, x, adapters.Bank(self.a, self.b, self.scale), ids)
 

@@ -371,3 +371,18 @@ def test_ids_are_read_when_the_calls_run():
             m(tokens)
             ids.copy_(other)
             assert torch.equal(m(tokens), want)
+
+
+def test_layers_whose_weight_the_model_takes_itself_are_refused():
+    """The head's weight, the latent attention's up-projection: what stands beside such a layer would be passed over."""
+    ids, tokens = torch.tensor([0], dtype=torch.int32), torch.tensor([[1, 2, 3]])
+    for m, targets in ((model(), ("head",)), (model(layer_types=("mla", "mla"), mixer_options=dict(kv_latent=16, nope_dim=8, rope_dim=8, v_dim=8)), ("kv_up", "o_proj"))):
+        plain = m(tokens)
+        bank = AdapterBank(m, targets, slots=1, rank=4)
+        server = Server(m, slots=1, capacity=160, kv_cache=KVCache(page_size=8), adapters=bank)
+        layer = next(iter(bank.layers.values()))
+        bank.load("x", {f"{path}.lora_{n}": torch.ones(*s) for path, x in bank.layers.items() for n, s in (("a", (1, x.in_features)), ("b", (x.out_features, 1)))}, alpha=1.0)
+        server.submit([1, 2, 3], 4, adapter="x")
+        with pytest.raises(RuntimeError, match="itself"):
+            server.run()
+        assert layer.weight.shape == (layer.out_features, layer.in_features) and torch.equal(m(tokens), plain)
