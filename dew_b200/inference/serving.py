@@ -111,6 +111,8 @@ class Server:
         self.clock = clock
         self.shared_prefix = bool(shared_prefix)
         self._layout, self._shared_layout = 0, -1          # counts changes of which pages rows have; the one that the cache was last told of
+        if adapters is not None and not {id(layer) for layer in adapters.layers.values()} <= {id(m) for m in model.modules()}:
+            raise ValueError("the bank of adapters stands beside the layers of another model")
         self.adapters = adapters
         self._row_adapters = None if adapters is None else torch.full((slots,), -1, dtype=torch.int32, device=self.device)
         self.last_tokens = torch.zeros(slots, dtype=torch.long, device=self.device)      # device-resident draws

@@ -386,3 +386,11 @@ def test_layers_whose_weight_the_model_takes_itself_are_refused():
         with pytest.raises(RuntimeError, match="itself"):
             server.run()
         assert layer.weight.shape == (layer.out_features, layer.in_features) and torch.equal(m(tokens), plain)
+
+
+def test_a_bank_of_another_model_is_refused():
+    m, other = model(), model()
+    bank = AdapterBank(other, TARGETS, slots=1, rank=4)
+    with pytest.raises(ValueError, match="bank"):
+        Server(m, slots=1, capacity=32, adapters=bank)
+    Server(other, slots=1, capacity=32, adapters=bank)
