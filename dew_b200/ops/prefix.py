@@ -19,25 +19,83 @@ class Shared(NamedTuple):
     tokens: torch.Tensor       # [groups]
 
 
+def _common(a: Sequence[int], b: Sequence[int]) -> int:
+    """Pages that both begin with (halving: comparing pieces of lists is quick)."""
+    lo, hi = 0, min(len(a), len(b))
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        if a[lo:mid] == b[lo:mid]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
+
+
+def _families(rows: Sequence[int], tables: Sequence[Optional[Sequence[int]]], least: int) -> List[Tuple[List[int], int]]:
+    """``rows``, which begin with the same page, in groups of (rows, pages that all of them begin with and that are read once for them): those that save the most pages,
+    (rows of a group - 1) x its pages, over all groups; no group of fewer than ``least`` pages.
+
+    The tables form a tree that branches where they part.  A row counts the pages of the group that it is in, and a group costs its pages once.  So what is saved below a node, if
+    the group around it has d pages, is the larger of: the sum over its branches with that d (a row: d), or the sum with the node's own depth, less that depth."""
+    tables = {r: list(tables[r]) for r in rows}
+    at = sorted(rows, key=tables.get)
+    # nodes [depth, branches], a branch a row's number or a node: those open from the root on, in the order of the tables
+    open_, last = [], at[0]
+    for before, row in zip(at, at[1:]):
+        depth = _common(tables[before], tables[row])
+        while open_ and open_[-1][0] > depth:
+            open_[-1][1].append(last)
+            last = open_.pop()
+        if open_ and open_[-1][0] == depth:
+            open_[-1][1].append(last)
+        else:
+            open_.append([depth, [last]])
+        last = row
+    while open_:
+        open_[-1][1].append(last)
+        last = open_.pop()
+    # every node with the depths of the groups that may be around it (0: none), its own last where it may be one
+    nodes, todo = [], [(last, (0,))]
+    while todo:
+        node, around = todo.pop()
+        inside = around + (node[0],) if node[0] >= max(1, least) else around
+        nodes.append((node, around, inside))
+        todo += [(branch, inside) for branch in node[1] if type(branch) is list]
+    sums, saved = {}, {}
+    for node, around, inside in reversed(nodes):
+        lists, n = [saved[id(x)] for x in node[1] if type(x) is list], sum(type(x) is int for x in node[1])
+        total = [n * d + sum(x[i] for x in lists) for i, d in enumerate(inside)]
+        sums[id(node)] = total
+        saved[id(node)] = [max(x, total[-1] - inside[-1]) for x in total[:len(around)]] if len(inside) > len(around) else total
+    groups, alone, todo = [], [], [(last, 0, None)]
+    place = {id(node): (around, inside) for node, around, inside in nodes}
+    while todo:
+        branch, i, group = todo.pop()
+        if type(branch) is int:
+            alone.append(([branch], 0)) if group is None else group.append(branch)
+            continue
+        (around, inside), total = place[id(branch)], sums[id(branch)]
+        if len(inside) > len(around) and total[-1] - inside[-1] > total[i]:
+            i, group = len(around), []
+            groups.append((group, branch[0]))
+        todo += [(x, i, group) for x in branch[1]]
+    return [(sorted(group), pages) for group, pages in groups] + alone
+
+
 def group_rows(tables: Sequence[Optional[Sequence[int]]], page_size: int, least: int = 1) -> Tuple[List[int], List[int], List[int]]:
-    """``order, first, tokens`` of ``Shared`` for rows of these pages (None: an empty row), as lists of as many groups as rows: rows whose first pages are the same make a group,
-    which shares the pages that all of it begins with.  Fewer than ``least`` tokens are not worth a group."""
-    families: Dict[object, List[int]] = {}
+    """``order, first, tokens`` of ``Shared`` for rows of these pages (None: an empty row), as lists of as many groups as rows: rows that begin with the same pages, in the groups
+    that leave the fewest tokens to read.  Fewer than ``least`` tokens are not worth a group."""
+    starts: Dict[object, List[int]] = {}
     for r, pages in enumerate(tables):
-        families.setdefault(pages[0] if pages else ("alone", r), []).append(r)
+        starts.setdefault(pages[0] if pages else ("alone", r), []).append(r)
+    groups: List[Tuple[List[int], int]] = []
+    for rows in starts.values():
+        groups += [(rows, 0)] if len(rows) == 1 else _families(rows, tables, -(-least // page_size))
     order, first, tokens = [], [0], []
-    for rows in families.values():
-        common = 0
-        if len(rows) > 1:
-            for column in zip(*(tables[r] for r in rows)):
-                if any(p != column[0] for p in column):
-                    break
-                common += 1
-        pieces = [rows] if common * page_size >= max(1, least) else [[r] for r in rows]
-        for piece in pieces:
-            order += piece
-            first.append(len(order))
-            tokens.append(common * page_size if len(piece) > 1 else 0)
+    for rows, pages in sorted(groups):
+        order += rows
+        first.append(len(order))
+        tokens.append(pages * page_size)
     empty = len(order) - len(tokens)
     return order, first + [len(order)] * empty, tokens + [0] * empty
 

@@ -1,7 +1,10 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
 import copy
+import itertools
+import random
 import sys
 import threading
+import time
 from contextlib import nullcontext
 from types import SimpleNamespace
 
@@ -16,6 +19,7 @@ from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore, PackedRows
 from dew_b200.nn.layers import reset_all
 from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
 from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
+from dew_b200.ops.prefix import group_rows
 from dew_b200.sampling.text import Sampling
 from dew_b200.utils.trees import flatten, module_variables, tree_map
 
@@ -394,3 +398,91 @@ def test_a_bank_of_another_model_is_refused():
     with pytest.raises(ValueError, match="bank"):
         Server(m, slots=1, capacity=32, adapters=bank)
     Server(other, slots=1, capacity=32, adapters=bank)
+
+
+# ---------------------------------------------------------------------------------------------------------- which rows share what
+def groups_of(tables, page=16, least=1):
+    order, first, tokens = group_rows(tables, page, least)
+    R = len(tables)
+    assert sorted(order) == list(range(R)) and len(first) == R + 1 and len(tokens) == R and first[0] == 0 and first[-1] == R and first == sorted(first)
+    found = {tuple(order[a:b]): n for a, b, n in zip(first, first[1:], tokens) if a < b}
+    for rows, n in found.items():
+        assert n % page == 0 and (n == 0 if len(rows) == 1 else n >= max(1, least))
+        assert len({tuple(tables[r][:n // page]) if n else r for r in rows}) == (1 if n else len(rows)) and all(len(tables[r] or ()) * page >= n for r in rows)
+    return found
+
+
+def saved(found):
+    return sum((len(rows) - 1) * n for rows, n in found.items())
+
+
+def best(tables, page, least):
+    """Most tokens that any grouping saves, by trying all of them."""
+    def part(rows):
+        if not rows:
+            return 0
+        head, rest = rows[0], rows[1:]
+        most = 0
+        for mask in range(1 << len(rest)):
+            group = [head] + [r for i, r in enumerate(rest) if mask >> i & 1]
+            common = 0
+            for column in zip(*(tables[r] or () for r in group)):
+                if len(set(column)) > 1:
+                    break
+                common += 1
+            n = common * page if len(group) > 1 and common * page >= max(1, least) else 0
+            if n or len(group) == 1:
+                most = max(most, (len(group) - 1) * n + part([r for r in rest if r not in group]))
+        return most
+    return part(list(range(len(tables))))
+
+
+def test_groups_behind_a_common_start_share_their_own_prefixes():
+    # prompts behind one template of a page: four groups of eight that share 64 pages each
+    tables = [[1] + [100 * g + i for i in range(63)] + [10000 + 8 * g + r] for g in range(4) for r in range(8)]
+    assert groups_of(tables, least=512) == {tuple(range(8 * g, 8 * g + 8)): 1024 for g in range(4)}
+    # one row that leaves early does not end what the others share
+    assert groups_of(tables[:8] + [[1, 7, 8]], least=512) == {tuple(range(8)): 1024, (8,): 0}
+    assert groups_of([[1, 2, 3, 4], [1, 2, 3, 5], [1, 9, 8, 7], [1, 9, 8, 6]], least=32) == {(0, 1): 48, (2, 3): 48}
+    # a long start that many rows have is worth more than what two of them have beyond it, and less than what most of them have
+    start = list(range(40))
+    assert groups_of([start + [50 + i] for i in range(6)] + [start + [99, 7], start + [99, 8]]) == {tuple(range(8)): 640}
+    deep = start + list(range(200, 300))
+    assert groups_of([start + [50], start + [51]] + [deep + [60 + i] for i in range(6)]) == {(0, 1): 640, tuple(range(2, 8)): 2240}
+    assert groups_of([[1, 2], (1, 2), [1, 2, 3]]) == {(0, 1, 2): 32}
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_no_grouping_saves_more(seed):
+    rng = random.Random(seed)
+    names, tables = itertools.count(), []
+    for _ in range(rng.randint(1, 7)):
+        kind = rng.random()
+        if kind < 0.1:
+            tables.append(rng.choice((None, [])))
+            continue
+        t = list(rng.choice(tables) or ()) if tables and kind < 0.85 else []
+        t = t[:rng.randint(0, len(t))]
+        tables.append(t + [next(names) for _ in range(rng.randint(0 if t else 1, 4))])
+    for least in (1, 17, 33):
+        assert saved(groups_of(tables, 16, least)) == best(tables, 16, least)
+
+
+def test_many_rows_are_grouped_quickly():
+    tables = [list(range(i + 1)) + [1000 + i] for i in range(448)]                # each leaves the others one page later
+    start = time.perf_counter()
+    groups_of(tables)
+    assert time.perf_counter() - start < 5.0
+
+
+def test_a_server_shares_what_groups_behind_a_template_have(monkeypatch):
+    from dew_b200.inference import serving
+    monkeypatch.setattr(serving, "SHARED_LEAST", 32)
+    template, told = list(range(1, 9)), []
+    plain = KVStore.share
+    monkeypatch.setattr(KVStore, "share", lambda self, *a: plain(self, *a) or told.append(sorted(self.shared.tokens.tolist())[-2:]))
+    server = Server(model(), slots=8, capacity=160, kv_cache=KVCache(page_size=8), shared_prefix=True)
+    got = [server.submit_group(template + [10 + 20 * g + i % 20 for i in range(41)], 3, 6) for g in range(2)]
+    server.run()
+    want = [alone(model(), template + [10 + 20 * g + i % 20 for i in range(41)], new=6) for g in range(2)]
+    assert [t.result() for ts in got for t in ts] == [w for w in want for _ in range(3)] and [48, 48] in told
