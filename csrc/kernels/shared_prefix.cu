@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(THREADS) shared_prefix_kernel(const __grid_con
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
       const float m_new = fmaxf(m[i], top);
       const float by = m[i] == -INFINITY ? 0.f : exp2f(m[i] - m_new);
-      const float p = m_new == -INFINITY ? 0.f : exp2f(x - m_new);
+      const float p = exp2f(x - (m_new == -INFINITY ? 0.f : m_new));       // (a score that is no number is no maximum, and shows in the sum)
       float sum = p;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);

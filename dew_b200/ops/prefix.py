@@ -122,7 +122,9 @@ def shared_decode_reference(q, k, v, table, lengths, scale, window=None, softcap
     s = s.masked_fill(~seen[:, None, None], -math.inf)
     if sinks is not None:
         s = torch.cat([s, sinks.float().view(1, G, H // G, 1).expand(R, -1, -1, 1)], -1)
-    p = torch.nan_to_num(torch.softmax(s, -1)) if sinks is None else torch.softmax(s, -1)[..., :-1]
+    p = torch.softmax(s, -1)
+    p = torch.where((s == -math.inf).all(-1, keepdim=True), torch.zeros_like(p), p)          # (nothing to see; a score that is no number shows)
+    p = p if sinks is None else p[..., :-1]
     return torch.einsum("rghn,rngd->rghd", p, vr).reshape(R, H, D).to(q.dtype)
 
 

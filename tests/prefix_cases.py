@@ -92,3 +92,37 @@ def allowed(a, found):
     dim, half = a["q"].shape[-1], torch.finfo(a["q"].dtype).eps / 2
     weights = half if a["q"].dtype == torch.bfloat16 else 0.0
     return half * o.abs() + size * (weights * 1.01 + 2 * ((dim + 4) * 2.0 ** -24 * most + 2.0 ** -21) + (longest + 64) * 2.0 ** -24) + 1e-30
+
+
+def numbers_that_are_none(a, row, other):
+    """``a`` with queries that no score of is a number (one head of ``row``; all of a resting row's), one whose every key scores minus infinity (a head of ``other``), and one
+    that meets infinity: ``(arguments, rows x heads that are to be NaN, to be zero, as they were)``."""
+    q, k = a["q"].clone(), a["k"].clone()
+    R, H, _ = q.shape
+    page, G = k.shape[1:3]
+    q[row, 0] = math.nan
+    q[a["lengths"] == 0] = math.nan
+    nan, zero = torch.zeros(R, H, dtype=torch.bool), torch.zeros(R, H, dtype=torch.bool)
+    nan[row, 0] = True
+    # the last key head's first column: what one query multiplies with minus infinity, another with zero
+    stored = torch.zeros(k.shape[:2], dtype=torch.bool)
+    held = a["table"][other].tolist()
+    n = int(a["lengths"][other])
+    for x in range(n):
+        stored[held[x // page], x % page] = True
+    k[..., -1, 0] = 0
+    k[..., -1, 0][stored.to(k.device)] = -math.inf
+    q[:, (G - 1) * H // G:, 0] = 0                            # (0 times infinity: no number)
+    q[other, H - 1, 0] = 1.0
+    meets = torch.zeros(R, dtype=torch.bool)
+    for r, length in enumerate(a["lengths"].tolist()):
+        t = a["table"][r].tolist()
+        meets[r] = any(bool(stored[t[x // page], x % page]) for x in range(length))
+    nan[meets, (G - 1) * H // G:] = True
+    nan[other, H - 1] = False
+    zero[other, H - 1] = True
+    zero[(a["lengths"] == 0).cpu()] = True
+    nan &= ~zero
+    same = ~nan & ~zero
+    same[:, (G - 1) * H // G:] = False                        # (their queries and keys are others now)
+    return {**a, "q": q, "k": k}, nan, zero, same

@@ -12,6 +12,7 @@ import pytest
 import torch
 from torch.overrides import TorchFunctionMode
 
+import prefix_cases
 from dew_b200.inference.serving import Server
 from dew_b200.inference.tasks import TextGeneration
 from dew_b200.models import CausalTransformer
@@ -19,7 +20,7 @@ from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore, PackedRows
 from dew_b200.nn.layers import reset_all
 from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
 from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
-from dew_b200.ops.prefix import group_rows
+from dew_b200.ops.prefix import group_rows, shared_decode
 from dew_b200.sampling.text import Sampling
 from dew_b200.utils.trees import flatten, module_variables, tree_map
 
@@ -486,3 +487,14 @@ def test_a_server_shares_what_groups_behind_a_template_have(monkeypatch):
     server.run()
     want = [alone(model(), template + [10 + 20 * g + i % 20 for i in range(41)], new=6) for g in range(2)]
     assert [t.result() for ts in got for t in ts] == [w for w in want for _ in range(3)] and [48, 48] in told
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_scores_that_are_no_numbers_show(dtype, sinks):
+    a = prefix_cases.batch([(32, [1, 9, 17]), (0, [5]), (50, [3, 3])], 6, 2, 24, 16, dtype, resting=(1,))
+    s = torch.randn(6, generator=torch.Generator().manual_seed(1)) if sinks else None
+    live = [r for r, n in enumerate(a["lengths"].tolist()) if n]
+    b, nan, zero, same = prefix_cases.numbers_that_are_none(a, live[0], live[1])
+    got, was = shared_decode(**b, sinks=s), shared_decode(**a, sinks=s)
+    assert bool(got[nan].isnan().all()) and not got[zero].any() and torch.equal(got[same], was[same])

@@ -10,7 +10,7 @@ from dew_b200.nn.lora import AdapterBank
 from dew_b200.ops import library as L
 from dew_b200.ops.prefix import Shared, shared_decode
 from dew_b200.sampling.text import RowBatch, generate
-from prefix_cases import allowed, batch, truth
+from prefix_cases import allowed, batch, numbers_that_are_none, truth
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -104,3 +104,20 @@ def test_captured_calls_of_several_tokens_follow_their_ids():
             graphs[0].replay()
             assert torch.equal(outs[0], want)
     L.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------- scores that are no numbers
+@pytest.mark.parametrize("groups", [[(130, [1, 64, 65, 200]), (0, [33]), (512, [1, 1])], [(257, [1 + i % 7 for i in range(40)]), (300, [5] * 9)], [(0, [300])] * 2])
+@pytest.mark.parametrize("heads, kv, dim, page, dtype", [(8, 2, 128, 64, BF16), (16, 2, 64, 16, BF16), (4, 2, 256, 16, BF16), (6, 2, 80, 16, BF16), (8, 2, 48, 16, FP32)])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_scores_that_are_no_numbers_show(groups, heads, kv, dim, page, dtype, sinks):
+    a = batch(groups, heads, kv, dim, page, dtype, device=DEV, resting=(len(groups[0][1]),) if len(groups) > 2 else ())
+    s = torch.randn(heads, device=DEV) if sinks else None
+    live = [r for r, n in enumerate(a["lengths"].tolist()) if n]
+    b, nan, zero, same = numbers_that_are_none(a, live[0], live[1])
+    L.check_status()
+    got = shared_decode(**b, sinks=s).cpu()
+    L.check_status()
+    found = truth(a, None, 0.0, s)
+    assert bool(got[nan].isnan().all()) and not got[zero].any()
+    assert bool(((got.double() - found[0]).abs() <= allowed(a, found))[same].all())
