@@ -443,7 +443,7 @@ class KVStore:
         """Whether a decode step with queries ``[rows, heads, dim]`` goes by what the rows share: where the tensor cores' kernel takes it, and in fp32.  Quantised pools and
         other widths are read sooner row by row (64 rows in groups of 8 behind 4096 tokens in int8: 340 us against 869)."""
         if (self.shared is None or self.row_ids is not None or q.shape[0] != self.rows or q.shape[-1] > 256 or (q.requires_grad and torch.is_grad_enabled())
-                or (self.kind == 0 and q.dtype != self.dtype)):
+                or L.transformed(q) or (self.kind == 0 and q.dtype != self.dtype)):
             return False
         if not L.use_cuda(q):
             return q.dtype in (torch.bfloat16, torch.float32)

@@ -69,10 +69,10 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
     _check(x, bank, ids, y.shape[-1] if y.dim() else 0, y.get_device() if y.is_cuda else y.device)
     if y.dtype is not x.dtype or y.shape[:-1] != x.shape[:-1] or not y.is_contiguous():
         raise ValueError("add_adapters: the projection's result in one piece, of the tokens' type and count")
+    if L.transformed(y, x, *bank) or (torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, *bank))):
+        raise NotImplementedError("add_adapters has no gradient: it serves adapters that were trained alone (nn.lora)")
     if y.data_ptr() == x.data_ptr() and y.numel():
         raise ValueError("add_adapters: the projection's result and the tokens are two tensors")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, *bank)):
-        raise NotImplementedError("add_adapters has no gradient: it serves adapters that were trained alone (nn.lora)")
     return _add(y, x, bank, ids)
 
 
@@ -120,7 +120,7 @@ def _add(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> tor
 def adapted_linear(x: torch.Tensor, weight: torch.Tensor, bank: Bank, ids: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``ops.linear(x, weight, bias)`` plus each token's adapter (``add_adapters``): ``x [..., in]``, ``weight [out, in]``, ``ids [...]`` int32."""
     _check(x, bank, ids, weight.shape[0], weight.get_device() if weight.is_cuda else weight.device)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, *bank)):
+    if L.transformed(x, weight, bias, *bank) or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, *bank))):
         raise NotImplementedError("adapted_linear has no gradient: it serves adapters that were trained alone (nn.lora)")
     y = linear(x, weight, bias)
     return _add(y if y.is_contiguous() else y.contiguous(), x, bank, ids)

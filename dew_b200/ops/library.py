@@ -155,6 +155,15 @@ def plain_autograd() -> bool:
     return torch.autograd.forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
 
 
+def transformed(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of these has a tangent or belongs to a functorch transform, or a trace is under way: what launches on their memory would lose without a word."""
+    if plain_autograd():
+        return False
+    dual = torch.autograd.forward_ad._current_level >= 0
+    return torch._C._get_tracing_state() is not None or any(
+        t is not None and (torch._C._functorch.is_functorch_wrapped_tensor(t) or (dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None)) for t in tensors)
+
+
 _TLS = threading.local()
 
 

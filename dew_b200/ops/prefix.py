@@ -207,7 +207,8 @@ def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_sc
         raise ValueError("shared_decode: pools in one piece")
     if apart:
         raise ValueError("shared_decode: tensors of one device")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (sinks is not None and sinks.requires_grad)):
+    if L.transformed(q, k, v, sinks, k_scale, v_scale) or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                                                                        or (sinks is not None and sinks.requires_grad))):
         raise NotImplementedError("shared_decode has no gradient: it is a step of generation")
 
 

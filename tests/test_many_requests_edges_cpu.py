@@ -10,6 +10,7 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.overrides import TorchFunctionMode
 
 import prefix_cases
@@ -20,6 +21,8 @@ from dew_b200.nn.kv_cache import CacheSlot, KVCache, KVStore, PackedRows
 from dew_b200.nn.layers import reset_all
 from dew_b200.nn.lora import AdapterBank, apply_lora, lora_state, merge_all
 from dew_b200.nn.quantization import Quantization, convert_qat, prepare_qat, quantize_model
+from dew_b200.ops.adapters import Bank, adapted_linear, add_adapters
+from dew_b200.ops.pages import move_pages
 from dew_b200.ops.prefix import group_rows, shared_decode
 from dew_b200.sampling.text import Sampling
 from dew_b200.utils.trees import flatten, module_variables, tree_map
@@ -498,3 +501,40 @@ def test_scores_that_are_no_numbers_show(dtype, sinks):
     b, nan, zero, same = prefix_cases.numbers_that_are_none(a, live[0], live[1])
     got, was = shared_decode(**b, sinks=s), shared_decode(**a, sinks=s)
     assert bool(got[nan].isnan().all()) and not got[zero].any() and torch.equal(got[same], was[same])
+
+
+# ---------------------------------------------------------------------------------------------------------- what the operators refuse
+def adapter_call():
+    g = torch.Generator().manual_seed(0)
+    make = lambda *s: torch.randn(*s, generator=g)
+    return make(5, 8), make(6, 8), Bank(make(2, 3, 8), make(2, 6, 3), torch.ones(2)), torch.tensor([0, -1, 1, 0, 1], dtype=torch.int32)
+
+
+def test_tangents_and_transforms_are_refused():
+    x, w, bank, ids = adapter_call()
+    a = prefix_cases.batch([(16, [1, 2])], 4, 2, 16, 16, torch.float32)
+    calls = [lambda t: adapted_linear(t(x), w, bank, ids), lambda t: adapted_linear(x, t(w), bank, ids), lambda t: adapted_linear(x, w, bank._replace(b=t(bank.b)), ids),
+             lambda t: add_adapters(t(torch.zeros(5, 6)), x, bank, ids), lambda t: add_adapters(torch.zeros(5, 6), t(x), bank, ids),
+             lambda t: shared_decode(**{**a, "q": t(a["q"])}), lambda t: shared_decode(**{**a, "v": t(a["v"])}), lambda t: shared_decode(**a, sinks=t(torch.zeros(4))),
+             lambda t: move_pages([t(torch.zeros(2, 4, 3))], [0], [1])]
+    for call in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+            call(lambda t: t)                                 # (nothing here has a tangent)
+        with pytest.raises(NotImplementedError):
+            torch.func.vmap(lambda by: call(lambda t: t * by))(torch.ones(2))
+        with pytest.raises(NotImplementedError):
+            torch.func.grad(lambda by: torch.as_tensor(call(lambda t: t * by)).sum())(torch.ones(()))
+    with pytest.raises(NotImplementedError):
+        move_pages([torch.zeros(2, 4, 3, requires_grad=True)], [0], [1])
+    with torch.no_grad():
+        move_pages([torch.zeros(2, 4, 3, requires_grad=True)], [0], [1])
+
+
+def test_a_store_reads_rows_apart_under_a_tangent():
+    store = KVStore(KVCache(page_size=8, pages=8), 1, 2, 32, 1, 16, dtype=torch.float32)
+    store.share([[0, 1], [0, 2]])
+    q, lengths = torch.randn(2, 2, 16), torch.tensor([9, 10], dtype=torch.int32)
+    with torch.no_grad(), forward_ad.dual_level():
+        assert store.decode_attention(0, forward_ad.make_dual(q, torch.ones_like(q)), lengths).shape == q.shape
