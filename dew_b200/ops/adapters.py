@@ -73,7 +73,10 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
         raise NotImplementedError("add_adapters has no gradient: it serves adapters that were trained alone (nn.lora)")
     if y.data_ptr() == x.data_ptr() and y.numel():
         raise ValueError("add_adapters: the projection's result and the tokens are two tensors")
-    return _add(y, x, bank, ids)
+    _add(y, x, bank, ids)
+    if y.is_cuda:                                       # (autograd is to know, as it does of what torch writes)
+        torch.autograd.graph.increment_version(y)
+    return y
 
 
 def _add(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> torch.Tensor:

@@ -107,3 +107,4 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     _refuse(rc)
     L.check(rc, "move_pages")
     L.count_launches(launches.value)
+    torch.autograd.graph.increment_version((*pools, table) if tables else pools)         # (autograd is to know, as it does of what torch writes)

@@ -8,6 +8,8 @@ from dew_b200.models import CausalTransformer
 from dew_b200.nn.kv_cache import PackedRows
 from dew_b200.nn.lora import AdapterBank
 from dew_b200.ops import library as L
+from dew_b200.ops.adapters import Bank, add_adapters
+from dew_b200.ops.pages import move_pages
 from dew_b200.ops.prefix import Shared, shared_decode
 from dew_b200.sampling.text import RowBatch, generate
 from prefix_cases import allowed, batch, numbers_that_are_none, truth
@@ -121,3 +123,23 @@ def test_scores_that_are_no_numbers_show(groups, heads, kv, dim, page, dtype, si
     found = truth(a, None, 0.0, s)
     assert bool(got[nan].isnan().all()) and not got[zero].any()
     assert bool(((got.double() - found[0]).abs() <= allowed(a, found))[same].all())
+
+
+# ---------------------------------------------------------------------------------------------------------- what is written in place
+def test_autograd_knows_what_was_written_in_place():
+    x, ids = torch.randn(5, 64, device=DEV), ints([0, -1, 1, 0, 1])
+    bank = Bank(torch.randn(2, 8, 64, device=DEV), torch.randn(2, 48, 8, device=DEV), torch.ones(2, device=DEV))
+    for by in (x, x.bfloat16()):
+        y, p = torch.randn(5, 48, device=DEV).to(by.dtype), torch.ones(48, device=DEV, dtype=by.dtype, requires_grad=True)
+        z = (y * p).sum()                                     # (keeps y)
+        add_adapters(y, by, Bank(bank.a.to(by.dtype), bank.b.to(by.dtype), bank.scale), ids)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+    pools, table = [torch.randn(2, 6, 4, device=DEV), torch.randn(1, 6, 9, device=DEV)], ints([[0, 1], [2, 3]])
+    before = [t._version for t in (*pools, table)]
+    move_pages(pools, [0], [1], table, [(0, 0, [5])])
+    assert all(t._version > v for t, v in zip((*pools, table), before))
+    with torch.inference_mode():
+        y = torch.randn(5, 48, device=DEV)
+        add_adapters(y, x, bank, ids)
+        move_pages([torch.zeros(2, 6, 4, device=DEV)], [0], [1])
