@@ -53,6 +53,11 @@ def _check(x, bank: Bank, ids, out: int, device) -> None:
         raise ValueError("adapters: tensors of one device")
 
 
+def _end(t: torch.Tensor, at: int) -> int:
+    """The address behind a tensor's last element."""
+    return at + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else at
+
+
 def add_adapters_reference(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> torch.Tensor:
     flat, x2, out = ids.reshape(-1), x.reshape(-1, x.shape[-1]).float(), y.view(-1, y.shape[-1])
     for i in sorted(set(flat.tolist())):
@@ -71,8 +76,13 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor
         raise ValueError("add_adapters: the projection's result in one piece, of the tokens' type and count")
     if L.transformed(y, x, *bank) or (torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, *bank))):
         raise NotImplementedError("add_adapters has no gradient: it serves adapters that were trained alone (nn.lora)")
-    if y.data_ptr() == x.data_ptr() and y.numel():
-        raise ValueError("add_adapters: the projection's result and the tokens are two tensors")
+    if y.numel():                                       # (tokens are read and results written in no order)
+        first = y.data_ptr()
+        end = first + y.numel() * y.element_size()
+        for t in (x, *bank, ids):
+            at = t.data_ptr()
+            if at < end and _end(t, at) > first:
+                raise ValueError("add_adapters: the projection's result lies over what is read")
     _add(y, x, bank, ids)
     if y.is_cuda:                                       # (autograd is to know, as it does of what torch writes)
         torch.autograd.graph.increment_version(y)

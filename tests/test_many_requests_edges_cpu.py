@@ -1,6 +1,7 @@
 """Where a server of many requests meets the rest of the framework: pools that change their size, weights given as variables, threads, layouts that nobody has in mind."""
 import copy
 import itertools
+import math
 import random
 import sys
 import threading
@@ -538,3 +539,24 @@ def test_a_store_reads_rows_apart_under_a_tangent():
     q, lengths = torch.randn(2, 2, 16), torch.tensor([9, 10], dtype=torch.int32)
     with torch.no_grad(), forward_ad.dual_level():
         assert store.decode_attention(0, forward_ad.make_dual(q, torch.ones_like(q)), lengths).shape == q.shape
+
+
+def test_a_result_that_lies_over_what_is_read_is_refused():
+    x, w, bank, ids = adapter_call()
+    room = torch.zeros(200)
+
+    def at(offset, *shape):
+        return room[offset:offset + math.prod(shape)].view(shape)
+    for y, mine in ((at(0, 5, 6), at(0, 5, 8)), (at(20, 5, 6), at(0, 5, 8)), (at(0, 5, 6), at(29, 5, 8)), (at(39, 5, 6), at(0, 5, 8)),
+                    (at(0, 5, 6), torch.as_strided(room, (5, 8), (20, 1), 10))):
+        with pytest.raises(ValueError, match="over"):
+            add_adapters(y, mine, bank, ids)
+    for y, mine in ((at(40, 5, 6), at(0, 5, 8)), (at(0, 5, 6), at(30, 5, 8)), (at(0, 5, 6), torch.as_strided(room, (5, 8), (20, 1), 30)), (at(0, 5, 6), at(30, 1, 8).expand(5, 8)),
+                    (at(0, 0, 6), at(0, 0, 8))):
+        add_adapters(y, mine, bank, ids[:len(y)])
+    y = torch.zeros(5, 6)
+    for i, shape in enumerate(((2, 3, 8), (2, 6, 3), (2,))):
+        with pytest.raises(ValueError, match="over"):
+            add_adapters(at(10, 5, 6), x, bank._replace(**{bank._fields[i]: at(39, *shape)}), ids)
+    with pytest.raises(ValueError, match="over"):
+        add_adapters(y, x, bank, y.view(torch.int32)[0, :5])
