@@ -185,6 +185,8 @@ def _check(q, k, v, table, lengths, shared: Shared, window, softcap, sinks, k_sc
         raise ValueError(f"shared_decode: order [rows], first [groups + 1] and tokens [groups] for {R} rows, got {[tuple(t.shape) for t in shared]}")
     if table.dim() != 2 or len(table) != R or lengths.shape != (R,):
         raise ValueError(f"shared_decode: a table [rows, columns] and lengths [rows] for {R} rows, got {tuple(table.shape)}, {tuple(lengths.shape)}")
+    if R and (k_shape[0] == 0 or k_shape[1] == 0 or table.shape[1] == 0):
+        raise ValueError(f"shared_decode: pools and tables of a page or more, got {tuple(k_shape)}, {tuple(table.shape)}")
     where = torch.Tensor.get_device if q.is_cuda else _device          # (the quicker question)
     device = where(q)
     apart = where(k) != device or where(v) != device

@@ -560,3 +560,12 @@ def test_a_result_that_lies_over_what_is_read_is_refused():
             add_adapters(at(10, 5, 6), x, bank._replace(**{bank._fields[i]: at(39, *shape)}), ids)
     with pytest.raises(ValueError, match="over"):
         add_adapters(y, x, bank, y.view(torch.int32)[0, :5])
+
+
+def test_pools_and_tables_without_a_page_are_refused():
+    a = prefix_cases.batch([(16, [1, 2])], 4, 2, 16, 16, torch.float32)
+    for changed in (dict(table=a["table"][:, :0].contiguous()), dict(k=a["k"][:0], v=a["v"][:0]), dict(k=a["k"][:, :0].contiguous(), v=a["v"][:, :0].contiguous())):
+        with pytest.raises(ValueError, match="page"):
+            shared_decode(**{**a, **changed})
+        with pytest.raises(ValueError, match="page"):
+            shared_decode(**{**a, **changed, "lengths": torch.zeros_like(a["lengths"])})
