@@ -219,6 +219,9 @@ class Server:
                 self._let_go(each)
             t.waiting = []
         self.queue.clear()
+        for r in self.rows:
+            if r is not None:
+                self.ledger.release(r.pages)
         self.rows = [None] * self.slots
         self._layout += 1
 

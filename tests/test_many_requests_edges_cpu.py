@@ -569,3 +569,13 @@ def test_pools_and_tables_without_a_page_are_refused():
             shared_decode(**{**a, **changed})
         with pytest.raises(ValueError, match="page"):
             shared_decode(**{**a, **changed, "lengths": torch.zeros_like(a["lengths"])})
+
+
+def test_requests_that_fail_give_their_pages_back():
+    server = Server(model(), slots=4, capacity=48, kv_cache=KVCache(page_size=8))
+    for _ in range(3):
+        server.submit_group(PROMPTS[0], 3, 8), server.submit(PROMPTS[1], 8)
+        server.step()
+        server.fail(RuntimeError("stopped"))
+        assert not server.ledger.refs and server.ledger.available() == server.ledger.pages
+    assert server([PROMPTS[0]], 8) == [alone(model(), PROMPTS[0])]
