@@ -329,7 +329,6 @@ __device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines)
   for (int g = tid; g <= a.groups; g += THREADS) {
     s.first[g] = static_cast<short>(min(max(a.first[g], 0), a.rows));
     if (g == a.groups) break;
-    if (blockIdx.x == 0 && a.first[g] > a.first[g + 1]) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
     s.lo[g] = 0;
     s.hi[g] = min(max(a.tokens[g], 0), most);
     live[g] = 0;
@@ -379,6 +378,7 @@ __device__ __forceinline__ bool make_lists(Lists& s, const Args& a, int engines)
   __syncthreads();
 #pragma unroll 1
   for (int g = tid; g < a.groups; g += THREADS) {
+    if (blockIdx.x == 0 && s.first[g] > s.first[g + 1]) atomicCAS(a.err, 0, static_cast<int>(ERR_BAD_ARG));
     if (live[g] < 2 || s.lo[g] >= s.hi[g]) s.lo[g] = s.hi[g] = 0;
     const int queries = group_queries(s, a, g);
     const Ranges both = ranges(s.lo[g], s.hi[g], 0, 0, a.box);

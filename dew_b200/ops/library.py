@@ -152,16 +152,19 @@ def unrecorded(*tensors: Optional[torch.Tensor]) -> bool:
 
 def plain_autograd() -> bool:
     """Neither forward-mode differentiation, nor a functorch transform, nor a trace is under way."""
-    return torch.autograd.forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
+    return _FORWARD._current_level < 0 and not _transforms() and _trace() is None
+
+
+_FORWARD, _transforms, _trace = torch.autograd.forward_ad, torch._C._are_functorch_transforms_active, torch._C._get_tracing_state      # (asked by every call)
 
 
 def transformed(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether one of these has a tangent or belongs to a functorch transform, or a trace is under way: what launches on their memory would lose without a word."""
     if plain_autograd():
         return False
-    dual = torch.autograd.forward_ad._current_level >= 0
-    return torch._C._get_tracing_state() is not None or any(
-        t is not None and (torch._C._functorch.is_functorch_wrapped_tensor(t) or (dual and torch.autograd.forward_ad.unpack_dual(t).tangent is not None)) for t in tensors)
+    dual = _FORWARD._current_level >= 0
+    return _trace() is not None or any(t is not None and (torch._C._functorch.is_functorch_wrapped_tensor(t) or (dual and _FORWARD.unpack_dual(t).tangent is not None))
+                                       for t in tensors)
 
 
 _TLS = threading.local()

@@ -40,7 +40,13 @@ def _check(src: Sequence[int], dst: Sequence[int], pages: int, table: Optional[t
         _refuse(-16)
 
 
+def _no_gradient() -> None:
+    raise NotImplementedError("move_pages has no gradient: pages of a cache are moved between steps of generation")
+
+
 def _pool(t: torch.Tensor, pages: int, device) -> _Pool:
+    if t.requires_grad and torch.is_grad_enabled():
+        _no_gradient()
     if t.dim() < 2 or t.shape[1] != pages or t.device != device:
         raise ValueError(f"move_pages: pools of one device and [layers, {pages}, ...], got {tuple(t.shape)} on {t.device}")
     shape, strides, size, by = t.shape, t.stride(), 1, t.element_size()
@@ -66,8 +72,8 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
         raise ValueError("move_pages: no pools")
     if tables and (table is None or table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.device != pools[0].device):
         raise ValueError("move_pages: the table is int32 [rows, columns] in one piece on the pools' device")
-    if L.transformed(*pools) or (torch.is_grad_enabled() and any(t.requires_grad for t in pools)):
-        raise NotImplementedError("move_pages has no gradient: pages of a cache are moved between steps of generation")
+    if L.transformed(*pools):
+        _no_gradient()
     pages = pools[0].shape[1] if pools[0].dim() > 1 else 0
     made = (_Pool * len(pools))(*(_pool(t, pages, pools[0].device) for t in pools))
     if not L.use_cuda(pools[0]):
