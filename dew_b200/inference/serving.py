@@ -64,15 +64,15 @@ class _Row:
     salt: bytes = b""           # what beside the tokens its pages depend on
 
 
-class _Methods(torch.nn.Module):
-    """A method of ``model`` as a module's call."""
+class _WithHead(torch.nn.Module):
+    """A model and one of its methods on what it makes of some places, as one module's call."""
 
     def __init__(self, model):
         super().__init__()
         self.model = model
 
-    def forward(self, method: str, hidden: torch.Tensor) -> torch.Tensor:
-        return getattr(self.model, method)(hidden)
+    def forward(self, method: str, places, tokens, **kw) -> torch.Tensor:
+        return getattr(self.model, method)(self.model(tokens, return_hidden=True, **kw)[places])
 
 
 class Server:
@@ -233,16 +233,16 @@ class Server:
         self._weights = f"weights {self._reloads}/".encode()       # (pages of the old ones, or begun with them, are nobody's prefix from here on)
 
     def _bind(self, variables) -> None:
-        """``_call``: the model with these variables (None: its own weights); ``_head``: one of its methods on hidden states, with the same."""
+        """``_call``: the model with these variables (None: its own weights); ``_head``: one of its methods on the hidden states of some places, with the same."""
+        with_head = _WithHead(self.model)
         if variables is None:
-            self._call = lambda t, **kw: self.model(t, **kw)
-            self._head = lambda method, hidden: getattr(self.model, method)(hidden)
+            self._call, self._head = lambda t, **kw: self.model(t, **kw), with_head.forward
             return
         from ..utils.trees import variables_for_call
         named = variables_for_call(self.model, variables)
-        methods, of_methods = _Methods(self.model), {f"model.{n}": t for n, t in named.items()}
+        of_both = {f"model.{n}": t for n, t in named.items()}
         self._call = lambda t, **kw: torch.func.functional_call(self.model, named, (t,), kw)
-        self._head = lambda method, hidden: torch.func.functional_call(methods, of_methods, (method, hidden))
+        self._head = lambda *args, **kw: torch.func.functional_call(with_head, of_both, args, kw)
 
     def __call__(self, prompts: Sequence[Any], max_new_tokens: int = 32) -> List[List[int]]:
         tickets = [self.submit(p, max_new_tokens) for p in prompts]
@@ -322,13 +322,11 @@ class Server:
             self.store.chunk_span = (start, start + longest)
             with torch.no_grad(), self._with_adapters(None if self.adapters is None else self._row_adapters[slots]):
                 # the head runs only on each row's last position (the only logits a prefill chunk can need)
+                places = (torch.arange(len(members), device=self.device), torch.tensor(last, device=self.device))
                 if hasattr(self.model, "logits"):
-                    hidden = self._call(ids, positions=pos, cache=self.store.select(slots), return_hidden=True)
-                    picked = hidden[torch.arange(len(members), device=self.device), torch.tensor(last, device=self.device)]
-                    last_logits = self._head("logits", picked)
+                    last_logits = self._head("logits", places, ids, positions=pos, cache=self.store.select(slots))
                 else:
-                    full = self._call(ids, positions=pos, cache=self.store.select(slots))
-                    last_logits = full[torch.arange(len(members), device=self.device), torch.tensor(last, device=self.device)]
+                    last_logits = self._call(ids, positions=pos, cache=self.store.select(slots))[places]
             self.store.select(None)
             self.store.chunk_span = None
             for i, (s, r) in enumerate(members):
@@ -392,12 +390,10 @@ class Server:
         captured once into a CUDA graph and replayed."""
         self._prev.copy_(self.last_tokens)
         with torch.no_grad(), self._with_adapters(self._row_adapters):
-            hidden = self._call(self.last_tokens[:, None], positions=self._in_pos[:, None], cache=self.store.select(None),
-                                return_hidden=True)[:, 0]
-            if greedy:
-                nxt = self._head("next_tokens_greedy", hidden)
-            else:
-                self._logits = self._head("logits", hidden)
+            nxt = self._head("next_tokens_greedy" if greedy else "logits", (slice(None), 0), self.last_tokens[:, None], positions=self._in_pos[:, None],
+                             cache=self.store.select(None))
+            if not greedy:
+                self._logits = nxt
                 nxt = self._logits.argmax(-1)
         self.last_tokens.copy_(torch.where(self._in_pos >= 0, nxt, self.last_tokens))
 
