@@ -81,6 +81,7 @@ def move_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
         if len(src):
             s, d = (torch.tensor(list(x), dtype=torch.long, device=pools[0].device) for x in (src, dst))
             for t in pools:
+                t = t.view(torch.uint8) if t.element_size() == 1 else t          # (8-bit floats have no indexing of their own)
                 t.index_copy_(1, d, t.index_select(1, s))
         for row, first, ps in tables:
             if len(ps):

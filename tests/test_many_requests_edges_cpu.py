@@ -579,3 +579,23 @@ def test_requests_that_fail_give_their_pages_back():
         server.fail(RuntimeError("stopped"))
         assert not server.ledger.refs and server.ledger.available() == server.ledger.pages
     assert server([PROMPTS[0]], 8) == [alone(model(), PROMPTS[0])]
+
+
+# ---------------------------------------------------------------------------------------------------------- pages of every type
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.float8_e5m2, torch.int8, torch.uint8, torch.bool, torch.float16, torch.bfloat16, torch.float64, torch.int64])
+def test_pages_of_any_type_move(dtype):
+    pool = (torch.arange(2 * 6 * 5).view(2, 6, 5) % 7).to(dtype)
+    want = [pool[:, p].clone() for p in (0, 0, 4, 3, 4, 5)]
+    move_pages([pool], [0, 4], [1, 2])
+    assert all(torch.equal(pool[:, i].float(), w.float()) for i, w in enumerate(want))
+
+
+def test_samples_fork_in_caches_of_every_kind():
+    for kind in (None, "int8", "float8_e4m3fn"):
+        server = Server(model(), slots=3, capacity=48, kv_cache=KVCache(kind, 8))
+        got = server.submit_group(PROMPTS[0], 3, 6)
+        while server.busy:
+            server.step()
+            server.compact()
+        assert len({tuple(t.result()) for t in got}) == 1
+        assert got[0].result() == Server(model(), slots=1, capacity=48, kv_cache=KVCache(kind, 8))([PROMPTS[0]], 6)[0]
