@@ -346,6 +346,9 @@ class AdapterBank:
         self.holds: Dict[str, int] = {}                    # requests in flight
         self._calls: Dict[int, Tuple[Optional[torch.Tensor], Dict]] = {}      # thread -> the ids of its calls, and those spread over tokens
 
+    def __getstate__(self):
+        return {**self.__dict__, "_calls": {}}             # (a copy is in nobody's use)
+
     def _now(self) -> Tuple[Optional[torch.Tensor], Dict]:
         return self._calls.get(threading.get_ident(), (None, {}))
 

@@ -599,3 +599,13 @@ def test_samples_fork_in_caches_of_every_kind():
             server.compact()
         assert len({tuple(t.result()) for t in got}) == 1
         assert got[0].result() == Server(model(), slots=1, capacity=48, kv_cache=KVCache(kind, 8))([PROMPTS[0]], 6)[0]
+
+
+def test_a_copy_made_inside_using_is_not_in_use():
+    m = model()
+    bank = random_bank(m)
+    with bank.using(torch.tensor([0], dtype=torch.int32)):
+        other = copy.deepcopy(m)
+    assert not other.layers[0].mixer.qkv_proj.in_use
+    with torch.no_grad():
+        assert torch.equal(other(torch.tensor([[1, 2], [3, 4]])), m(torch.tensor([[1, 2], [3, 4]])))
