@@ -238,6 +238,7 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
         strides = q.stride()
     out = torch.empty(R, H, D, dtype=q.dtype, device=q.device)
     pages, page, G, _ = k.shape
+    seen = window if window is not None and window < 1 << 30 else 0         # (a row's keys are counted in 30 bits: a wider window leaves it all)
     columns, groups, fp32, lib = table.shape[1], len(shared.tokens), torch.float32, L.load()
     at_q, at_k, at_v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     numbers = (table.data_ptr(), lengths.data_ptr(), shared.order.data_ptr(), shared.first.data_ptr(), shared.tokens.data_ptr(), L.at(sinks))
@@ -250,7 +251,7 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
         scratch = torch.empty(rows * (D + 2) + 8 * R, dtype=fp32, device=q.device)
         at = scratch.data_ptr()
         L.check(lib.dewb_shared_decode_mma(at_q, strides[0] if R > 1 else H * D, at_k, at_v, *numbers, at, at + 4 * rows * D, at + 4 * rows * (D + 2),
-                                           out.data_ptr(), R, H, G, D, page, columns, pages, groups, window or 0, LEAST_TILES, engines, scale, softcap, err, stream), "shared_decode_mma")
+                                           out.data_ptr(), R, H, G, D, page, columns, pages, groups, seen, LEAST_TILES, engines, scale, softcap, err, stream), "shared_decode_mma")
         L.count_launches(2)
         return out
     splits = _splits(columns * page, R * G)
@@ -258,7 +259,7 @@ def shared_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torc
     at = parts.data_ptr()
     one = 2 * splits * R * H * 4
     L.check(lib.dewb_shared_decode(at_q, strides[0], at_k, at_v, L.at(k_scale), L.at(v_scale), *numbers, at, at + one, at + 2 * one, out.data_ptr(),
-                                   R, H, G, D, page, columns, pages, groups, splits, window or 0, scale, softcap, int(q.dtype is fp32), _POOLS.get(k.dtype, 0), err, stream),
+                                   R, H, G, D, page, columns, pages, groups, splits, seen, scale, softcap, int(q.dtype is fp32), _POOLS.get(k.dtype, 0), err, stream),
             "shared_decode")
     L.count_launches(2)
     return out

@@ -143,3 +143,12 @@ def test_autograd_knows_what_was_written_in_place():
         y = torch.randn(5, 48, device=DEV)
         add_adapters(y, x, bank, ids)
         move_pages([torch.zeros(2, 6, 4, device=DEV)], [0], [1])
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (FP32, 48)])
+def test_a_window_past_32_bits_is_none(dtype, dim):
+    a = batch([(130, [1, 64, 65, 200]), (64, [3, 4, 5])], 4, 2, dim, 16, dtype, device=DEV)
+    want = shared_decode(**a)
+    for window in ((1 << 31) - 1, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(shared_decode(**a, window=window), want)
+    L.check_status()
