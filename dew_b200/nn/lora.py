@@ -314,9 +314,13 @@ class AdaptedLinear(Linear):
             super().reset_parameters(generator)
 
     def forward(self, x):
-        y = self.base(x) if "base" in self._modules else ops.linear(x, self._parameters["weight"], self.bias)
-        ids = self._of[0].ids_for(x.shape[:-1])
-        return y if ids is None else adapters.add_adapters(y, x, adapters.Bank(self.a, self.b, self.scale), ids)
+        ids, base = self._of[0].ids_for(x.shape[:-1]), self._modules.get("base")
+        bank = adapters.Bank(self.a, self.b, self.scale)
+        if base is None:
+            w = self._parameters["weight"]
+            return ops.linear(x, w, self.bias) if ids is None else adapters.adapted_linear(x, w, bank, ids, self.bias)
+        y = base(x)
+        return y if ids is None else adapters.add_adapters(y, x, bank, ids)
 
 
 _BANKS = threading.RLock()       # what stands in banks, and who holds it, changes by one thread at a time

@@ -1,17 +1,17 @@
 """The kernels of a server of many requests at their edges: groups that leave rows out, numbers that are none, packed prompts, captured calls."""
-import math
-
 import pytest
 import torch
 
+from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
-from dew_b200.nn.kv_cache import PackedRows
+from dew_b200.nn.kv_cache import KVCache, PackedRows
 from dew_b200.nn.lora import AdapterBank
 from dew_b200.ops import library as L
 from dew_b200.ops.adapters import Bank, add_adapters
 from dew_b200.ops.pages import move_pages
 from dew_b200.ops.prefix import Shared, shared_decode
 from dew_b200.sampling.text import RowBatch, generate
+from dew_b200.utils.trees import module_variables, tree_map
 from prefix_cases import allowed, batch, numbers_that_are_none, truth
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +152,53 @@ def test_a_window_past_32_bits_is_none(dtype, dim):
     for window in ((1 << 31) - 1, 1 << 31, (1 << 32) + 5):
         assert torch.equal(shared_decode(**a, window=window), want)
     L.check_status()
+
+
+# ---------------------------------------------------------------------------------------------------------- servers
+def small(seed, dtype=FP32):
+    torch.manual_seed(seed)
+    return CausalTransformer(**CONFIG).eval().to(DEV, dtype)
+
+
+def alone(m, prompts, new=8):
+    return [Server(m, slots=1, capacity=256, kv_cache=KVCache(page_size=16), prefix_cache=False)([p], new)[0] for p in prompts]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_variables_and_reloads_beside_a_bank(graph):
+    prompts = [[1 + i % 90 for i in range(70)], [5, 4, 3], [1 + i % 90 for i in range(70)]]
+    want, old = alone(small(7), prompts), alone(small(0), prompts)
+    assert want != old
+    m = small(0)
+    bank = AdapterBank(m, TARGETS, slots=2, rank=8)
+    theirs = tree_map(lambda t: t.detach().clone(), module_variables(small(7)))
+    server = Server(m, theirs, slots=3, capacity=256, kv_cache=KVCache(page_size=16), cuda_graph=graph, shared_prefix=True, adapters=bank)
+    assert server(prompts, 8) == want
+    server.reload(tree_map(lambda t: t.detach().clone(), module_variables(small(0))))
+    assert server(prompts, 8) == old
+    server.reload(theirs)
+    assert server(prompts, 8) == want
+    L.check_status()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_pools_of_other_sizes_between_requests(graph, dtype):
+    m = small(3, dtype)
+    long, prompts = [1 + i % 90 for i in range(200)], [[1 + i % 60 for i in range(70)], [2 + i % 50 for i in range(33)]]
+
+    def run(resize):
+        server = Server(m, slots=2, capacity=256, kv_cache=KVCache(page_size=16), chunk=32, cuda_graph=graph, shared_prefix=True)
+        server([long, long[3:]], 6)
+        out = []
+        for pages in (12, 9, 40):
+            if resize:
+                server.resize(pages)
+                assert int(server.store.page_table.max()) < pages and server.store.k.shape[1] == pages + 1
+            out.append(server(prompts, 6))                    # unequal prompts in chunks
+            row = server.submit(prompts[1], 6)                # a step beside an idle row
+            server.run()
+            out.append(row.result())
+        L.check_status()
+        return out
+    assert run(True) == run(False)
