@@ -80,8 +80,8 @@ class Server:
                  chunk: Optional[int] = None, prefix_cache: bool = True, decode_steps: int = 1, sampling: Optional[Sampling] = None,
                  tokenizer=None, prefill_budget: Optional[int] = None, cuda_graph: bool = False, clock: Callable[[], float] = time.perf_counter,
                  host_pages: int = 0, shared_prefix: bool = False, adapters=None):
-        """``shared_prefix``: decode steps read the pages that several rows begin with once for all of them.  ``adapters``: an ``nn.lora.AdapterBank`` over ``model``, whose
-        adapters requests name."""
+        """``shared_prefix``: decode steps read the pages that several rows begin with once for all of them (up to ``ops.prefix.MOST_ROWS`` rows in bf16).  ``adapters``: an
+        ``nn.lora.AdapterBank`` over ``model``, whose adapters requests name."""
         self.model, self.variables, self.tokenizer = model, variables, tokenizer
         self.slots, self.capacity = slots, capacity
         limit = getattr(getattr(model, "config", None), "max_seq_len", None)

@@ -70,7 +70,7 @@ def add_adapters_reference(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: to
 
 def add_adapters(y: torch.Tensor, x: torch.Tensor, bank: Bank, ids: torch.Tensor) -> torch.Tensor:
     """``y [..., out] += scale[i] (x [..., in] a[i]^T) b[i]^T`` in place, ``i = ids [...]`` (int32; below 0: the token has none) -> ``y``.  Sums are fp32; in bf16 the rank's
-    values, with their scale, are rounded once between the two products."""
+    values, with their scale, are rounded once between the two products.  ``y`` lies over nothing that is read."""
     _check(x, bank, ids, y.shape[-1] if y.dim() else 0, y.get_device() if y.is_cuda else y.device)
     if y.dtype is not x.dtype or y.shape[:-1] != x.shape[:-1] or not y.is_contiguous():
         raise ValueError("add_adapters: the projection's result in one piece, of the tokens' type and count")
