@@ -1,0 +1,172 @@
+// What the kernels of the selective state space scan share: their arguments, how a warp lies over channels and states, and how a tile of tokens comes in.
+//
+//   s = softplus(dt) (or dt);   h_t[n] = exp(s a[c, n]) h_{t-1}[n] + s x_t B_t[n];   y_t = (sum_n C_t[n] h_t[n] + D x_t) silu(z_t)
+//
+// A lane owns four channels and NS states of each; LN lanes share the states, 32 / LN groups of lanes the channels.  So what is summed over states crosses LN lanes and what is summed
+// over channels crosses 32 / LN, and neither takes a shuffle per product (a channel a lane with 16 states: 31 shuffles a token to sum 32 numbers over the lanes; here 7 for the
+// channels' sums and 3 for each number of the four channels).
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+// x, dt, z, b, c: row r, token t starts at r * row + t * token (elements).  Null where a call has none: z, d, initial, last, checkpoints, starts, sums, positions, lengths, row_ids.
+// With `heads` > 0 a channel is one of heads * dim, and the decay (a, dt, dt_bias, d) is a head's.
+extern "C" struct dewb_selective_args {
+  const void *x, *dt, *z, *b, *c;
+  long long x_row, x_token, dt_row, dt_token, z_row, z_token, b_row, b_token, c_row, c_token;
+  const float *a, *dt_bias, *d;        // [C, N] or [heads]; [heads]; [C] or [heads]
+  const float* initial;                // [rows, C, N]; with positions, [store rows, C, N], and `last` is the same tensor
+  float* last;
+  void* y;                             // [R, T, C]
+  float* checkpoints;                  // [R, ceil(T / EVERY), padded C, padded N]: the state in front of every EVERY tokens
+  float *starts, *sums;                // [R, segments, padded C, padded N], [R, segments, padded C]: see scan_kernel
+  const int *positions, *lengths, *row_ids;
+  int R, T, C, N, groups, heads, segments, segment;
+  int softplus, log_a, dt_fp32, stored;      // `stored`: rows of the store, where row_ids or positions name them
+  int* status;                         // told of a row outside the store, which then has no tokens
+};
+
+namespace dewb {
+namespace selective {
+
+using bf16 = __nv_bfloat16;
+using Args = dewb_selective_args;
+
+constexpr int THREADS = 128, WARPS = 4;
+constexpr int TT = 16;                 // tokens of a tile
+constexpr int OUTSIDE = 6;             // the status of a row that the store does not have
+constexpr int EVERY = 16;              // tokens between two kept states
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+template <int LN, int NS>
+struct Lay {
+  static constexpr int CG = 32 / LN;             // groups of lanes: four channels each
+  static constexpr int CW = 4 * CG;              // channels of a warp
+  static constexpr int CB = WARPS * CW;          // ... of a block
+  static constexpr int NP = LN * NS;             // states, padded
+  static constexpr int PASSES = TT >= LN ? TT / LN : 1;      // a lane's pieces of four channels in a tile: token lane / CG + pass * LN
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
+
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const bf16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st(bf16* p, float v) { *p = __float2bfloat16(v); }
+
+// Four neighbouring values as they lie in memory, on their way.
+template <typename T> struct Raw;
+template <> struct Raw<bf16> {
+  uint2 v;
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+};
+template <> struct Raw<float> {
+  uint4 v;
+  __device__ __forceinline__ void get(float (&f)[4]) const {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+};
+__device__ __forceinline__ uint32_t bits(const bf16* p) { return *reinterpret_cast<const unsigned short*>(p); }
+
+// `whole`: a vector load; else `n` (0 to 4) of the values, zeros behind.
+__device__ __forceinline__ Raw<bf16> fetch(const bf16* p, bool whole, int n) {
+  Raw<bf16> r{make_uint2(0u, 0u)};
+  if (whole) { r.v = *reinterpret_cast<const uint2*>(p); return r; }
+  if (n > 0) r.v.x = bits(p);
+  if (n > 1) r.v.x |= bits(p + 1) << 16;
+  if (n > 2) r.v.y = bits(p + 2);
+  if (n > 3) r.v.y |= bits(p + 3) << 16;
+  return r;
+}
+__device__ __forceinline__ Raw<float> fetch(const float* p, bool whole, int n) {
+  Raw<float> r{make_uint4(0u, 0u, 0u, 0u)};
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+  if (whole) { r.v = *reinterpret_cast<const uint4*>(p); return r; }
+  if (n > 0) r.v.x = q[0];
+  if (n > 1) r.v.y = q[1];
+  if (n > 2) r.v.z = q[2];
+  if (n > 3) r.v.w = q[3];
+  return r;
+}
+__device__ __forceinline__ void put(float* p, const float (&f)[4], bool whole, int n) {
+  if (whole) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); return; }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) if (j < n) p[j] = f[j];
+}
+__device__ __forceinline__ void put(bf16* p, const float (&f)[4], bool whole, int n) {
+  if (whole) {
+    __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) if (j < n) p[j] = __float2bfloat16(f[j]);
+}
+
+// Whether four values at multiples of four columns can be read as one piece.
+template <typename T>
+__device__ __forceinline__ bool fours(const void* p, long long row, long long token) {
+  return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && ((row | token) & 3) == 0;
+}
+
+// The steps' logits of four channels, bf16 or fp32.
+struct RawStep {
+  uint4 v;
+  __device__ __forceinline__ void get(float (&f)[4], bool fp32) const {
+    if (fp32) Raw<float>{v}.get(f);
+    else Raw<bf16>{make_uint2(v.x, v.y)}.get(f);
+  }
+};
+__device__ __forceinline__ RawStep fetch_step(const void* p, long long at, bool fp32, bool whole, int n) {
+  if (fp32) return {fetch(static_cast<const float*>(p) + at, whole, n).v};
+  const uint2 v = fetch(static_cast<const bf16*>(p) + at, whole, n).v;
+  return {make_uint4(v.x, v.y, 0u, 0u)};
+}
+
+// Sums of four channels' numbers over the LN lanes that share their states: the lane's result is that of channel `own_channel(lane)` (lanes with sl >= 4 hold copies).
+template <int LN>
+__device__ __forceinline__ float over_states(const float (&y)[4], int sl) {
+  const bool b0 = sl & 1, b1 = sl & 2;
+  const float p0 = (b0 ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, b0 ? y[0] : y[2], 1);
+  const float p1 = (b0 ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, b0 ? y[1] : y[3], 1);
+  float q = (b1 ? p1 : p0) + __shfl_xor_sync(0xffffffffu, b1 ? p0 : p1, 2);
+#pragma unroll
+  for (int o = 4; o < LN; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+  return q;
+}
+__device__ __forceinline__ int own_channel(int sl) { return (sl & 1) * 2 + ((sl >> 1) & 1); }
+
+// Which tokens of row `row` a call has, and where its state lies.
+struct Row {
+  int len;             // live tokens
+  bool held;           // a state to begin with
+  long long at;        // row of `initial` and `last`
+};
+__device__ __forceinline__ Row row_of(const Args& p, int row) {
+  if (p.positions == nullptr) return {p.T, p.initial != nullptr, row};
+  const int first = p.positions[static_cast<long long>(row) * p.T], at = p.row_ids == nullptr ? row : p.row_ids[row];
+  const bool inside = p.initial == nullptr || (at >= 0 && at < p.stored);
+  if (!inside && p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, OUTSIDE);
+  return {first < 0 || !inside ? 0 : max(0, min(p.lengths[row] - first, p.T)), p.initial != nullptr && first > 0, at};
+}
+
+// The rate of channel c's state n times log2 e, 0 outside.
+template <bool HEADS>
+__device__ __forceinline__ float rate(const Args& p, int c, int n, int dim) {
+  if (c >= p.C || n >= p.N) return 0.f;
+  const float a = p.a[HEADS ? c / dim : static_cast<long long>(c) * p.N + n];
+  return (p.log_a ? -expf(a) : a) * LOG2E;
+}
+
+}  // namespace selective
+}  // namespace dewb

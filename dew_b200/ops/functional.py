@@ -589,8 +589,11 @@ def stream_rms_norm(x: torch.Tensor, branch: torch.Tensor, w: torch.Tensor, eps:
     return rms_norm_reference(h, w, eps), h
 
 
-def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
-    """``norm(x) * w * silu(z)`` (the output gate of gated-delta-net / Mamba-2 blocks)."""
+def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float = 1e-6, gate_first: bool = False) -> torch.Tensor:
+    """``norm(x) * w * silu(z)`` (the output gate of gated-delta-net blocks); with ``gate_first``, ``norm(x * silu(z)) * w`` (Mamba-2's; ``ops/gate_norm.py``)."""
+    if gate_first:
+        from .gate_norm import gate_norm
+        return gate_norm(x, z, w, eps)
     if L.use_cuda(x) and _norm_cuda_ok(x, w):
         x, z = x.contiguous(), z.contiguous()
         return _rms_norm(x, z, w, eps, 2)[0] if L.unrecorded(x, z, w) else _RMSNorm.apply(x, z, w, eps, 2)

@@ -1,0 +1,75 @@
+"""The norm behind a gate, ``norm(x silu(z)) w`` (``csrc/kernels/gate_norm.cu``), forward and backward: launchers and autograd node."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+
+from . import library as L
+
+BLOCKS = 148 * 4         # that walk the rows of a backward, at most
+
+
+def plain(x, z, w, eps: float) -> torch.Tensor:
+    f = torch.float64 if x.dtype is torch.float64 else torch.float32
+    u = x.to(f) * F.silu(z.to(f))
+    return (u * torch.rsqrt(u.pow(2).mean(-1, keepdim=True) + eps) * w.to(f)).to(x.dtype)
+
+
+def kernel_available(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor) -> bool:
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and z.dtype is x.dtype and w.dtype in (x.dtype, torch.float32) and w.dim() == 1 and x.dim() > 0 and x.numel() > 0
+            and z.shape == x.shape and w.shape[0] == x.shape[-1] and z.device == w.device == x.device and not L.transformed(x, z, w) and L.use_cuda(x))
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t [..., d]`` as rows, each in one piece (a view of a wider tensor is one already)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _forward(x, z, w, eps: float) -> torch.Tensor:
+    x2, z2, w = _rows(x), _rows(z), w.contiguous()
+    rows, d = x2.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with L.on_device_of(x) as stream:
+        L.check(L.load().dewb_gate_norm_fwd(x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), y.data_ptr(), rows, d, eps, int(x.dtype is torch.float32),
+                                            int(w.dtype is torch.float32), stream), "gate_norm_fwd")
+    L.count_launches()
+    return y
+
+
+def _backward(x, z, w, eps: float, dy):
+    x2, z2, w, dy2 = _rows(x), _rows(z), w.contiguous(), _rows(dy.to(x.dtype))
+    rows, d = x2.shape
+    dx, dz, dw = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, z, w))
+    blocks = min(BLOCKS, rows)
+    parts = torch.empty(blocks, d, dtype=torch.float32, device=x.device)
+    with L.on_device_of(x) as stream:
+        L.check(L.load().dewb_gate_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), dx.data_ptr(), dz.data_ptr(),
+                                            dw.data_ptr(), parts.data_ptr(), blocks, rows, d, eps, int(x.dtype is torch.float32), int(w.dtype is torch.float32), stream), "gate_norm_bwd")
+    L.count_launches(2)
+    return dx, dz, dw
+
+
+class _GateNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, z, w, eps):
+        ctx.save_for_backward(x, z, w)
+        ctx.eps = eps
+        return _forward(x, z, w, eps)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, z, w = ctx.saved_tensors
+        if torch.is_grad_enabled():                          # (create_graph: the kernel's results would have no history)
+            at = [i for i, t in enumerate((x, z, w)) if ctx.needs_input_grad[i]]
+            grads = torch.autograd.grad(plain(x, z, w, ctx.eps), [(x, z, w)[i] for i in at], dy, create_graph=True)
+            return (*(grads[at.index(i)] if i in at else None for i in range(3)), None)
+        return (*_backward(x, z, w, ctx.eps, dy), None)
+
+
+def gate_norm(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
+    if not kernel_available(x, z, w):
+        return plain(x, z, w, eps)
+    return _forward(x, z, w, eps) if L.unrecorded(x, z, w) else _GateNorm.apply(x, z, w, eps)

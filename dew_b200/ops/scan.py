@@ -330,11 +330,22 @@ def selective_scan_reference(x, dt, A, Bm, Cm, D=None, z=None, initial_state=Non
     return y.to(x.dtype), h
 
 
-def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, chunk: int = 64):
+def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, chunk: int = 64, softplus: bool = False):
+    """Public entry: ``x, dt [B,T,C]`` (with ``softplus``, the steps' logits), ``A [C,N]``, ``Bm, Cm [B,T,N]``, ``D [C]``, ``z [B,T,C]``, ``initial_state [B,C,N]`` -> (y ``[B,T,C]``, state
+    ``[B,C,N]`` fp32).  CUDA tensors with up to 128 states run the sm_100a kernels (``ops/selective.py``), in either direction; everything else the chunked form below."""
+    if x.is_cuda and A.dim() == 2 and A.shape[1] <= 128:
+        from . import selective as K
+        if K.kernel_available(x, dt, A, Bm, Cm, D, z, initial_state):
+            return K.selective_scan(x, dt, A, Bm, Cm, D, z, initial_state, softplus)
+    return selective_scan_chunked(x, dt, A, Bm, Cm, D, z, initial_state, chunk, softplus)
+
+
+def selective_scan_chunked(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, chunk: int = 64, softplus: bool = False):
     """Chunked selective scan: a log-depth (Hillis-Steele) prefix combine of ``(decay, increment)`` pairs inside each chunk,
     state carried across chunks - O(T log chunk) parallel work instead of T sequential steps."""
     Bsz, T, C = x.shape
     N = A.shape[1]
+    dt = F.softplus(dt.float()) if softplus else dt
     pad = (-T) % chunk
     xf, dtf = x.float(), dt.float()
     Bf, Cf = Bm.float(), Cm.float()

@@ -1,0 +1,277 @@
+"""The selective state space scan (``csrc/kernels/selective_scan.cu``, ``selective_grad.cu``; the equations stand in ``csrc/common/selective.cuh``): a rate per channel and state
+(Mamba-1) over whole rows with every gradient, and over a call's ``Rows`` with the states that a store keeps; and the same with a decay per head (Mamba-2) for such a call.  The plain
+forms go token by token (``selective_tokens_reference``, ``ssd_tokens_reference``) or in chunks (``ops.scan.selective_scan_chunked``).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+
+from . import library as L
+from .token_mix import Rows, kernel_ok, whole
+
+MOST_STATES, MOST_HEAD_STATES = 128, 256
+EVERY = 16               # tokens between two states that the forward keeps for the backward
+
+_FIELDS = (("x dt z b c", ctypes.c_void_p), ("x_row x_token dt_row dt_token z_row z_token b_row b_token c_row c_token", ctypes.c_longlong),
+           ("a dt_bias d initial last y checkpoints starts sums positions lengths row_ids", ctypes.c_void_p),
+           ("R T C N groups heads segments segment softplus log_a dt_fp32 stored", ctypes.c_int), ("status", ctypes.c_void_p))
+
+
+class _Args(ctypes.Structure):
+    """``dewb_selective_args`` of ``csrc/common/selective.cuh``."""
+    _fields_ = [(name, kind) for names, kind in _FIELDS for name in names.split()]
+
+
+class _Grad(ctypes.Structure):
+    """``dewb_selective_grad_args`` of ``csrc/kernels/selective_grad.cu``."""
+    _fields_ = [("f", _Args), ("dy", ctypes.c_void_p), ("dy_row", ctypes.c_longlong), ("dy_token", ctypes.c_longlong)] + \
+               [(name, ctypes.c_void_p) for name in "dlast dx ddt dz db dc da dd dinitial bc_parts a_parts d_parts".split()]
+
+
+def _padded(C: int, N: int, groups: int = 1):
+    """Channels and states as the workspaces pad them, and the warps that a row's channels take."""
+    lanes = 4 if N <= 16 else 8 if N <= 32 else 16 if N <= 64 else 32
+    block = 512 // lanes
+    blocks = -(-(C // groups) // block) * groups
+    return blocks * block, lanes * 4 if N <= 128 else 256, blocks * 4
+
+
+WARPS = 148 * 8           # what the GPU is filled with
+
+
+def _segments(R: int, T: int, warps: int) -> int:
+    """How many pieces of a row run side by side, and tokens of a piece."""
+    pieces = max(1, min(-(-T // 64), WARPS // max(1, R * warps)))
+    length = -(-(-(-T // pieces)) // EVERY) * EVERY
+    return length
+
+
+def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """``t [R, T, n]`` with its last axis in one piece."""
+    return t if t is None or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def _rows(t: Optional[torch.Tensor]):
+    """Address, and row and token strides (0 where there is one of them)."""
+    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0):
+    """The arguments of a launch, and what has to live until it is issued."""
+    R, T, C = x.shape
+    channels, states, warps = _padded(C, N, groups)
+    segment = _segments(R, T, warps)
+    segments = -(-T // segment)
+    work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device) if segments > 1 else None
+    starts = L.at(work)
+    (px, *sx), (pd, *sd), (pz, *sz), (pb, *sb), (pc, *sc) = (_rows(t) for t in (x, dt, z, b, c))
+    at = (0, 0, 0) if rows is None else (rows.positions.data_ptr(), rows.lengths.data_ptr(), L.at(rows.row_ids))
+    args = _Args(px, pd, pz, pb, pc, *sx, *sd, *sz, *sb, *sc, a.data_ptr(), L.at(dt_bias), L.at(d), L.at(initial), L.at(last), L.at(y), L.at(checkpoints), starts,
+                 starts + 4 * R * segments * channels * states if work is not None else 0, *at, R, T, C, N, groups, heads, segments, segment, int(softplus), int(log_a),
+                 int(dt.dtype is torch.float32), stored, L.status(x.device).data_ptr())
+    return args, work
+
+
+def _launch(args: _Args, fp32: bool, token: bool, stream: int) -> None:
+    lib = L.load()
+    launch = lib.dewb_selective_token if token else lib.dewb_selective_scan
+    L.check(launch(ctypes.byref(args), ctypes.c_int(int(fp32)), ctypes.c_void_p(stream)), "selective_token" if token else "selective_scan")
+    L.count_launches(1 if args.segments == 1 else 2)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# whole rows, with gradients
+
+
+def _forward(x, dt, a, b, c, d, z, initial, softplus: bool, keep: bool):
+    R, T, C = x.shape
+    N = a.shape[1]
+    y = torch.empty(R, T, C, dtype=x.dtype, device=x.device)
+    last = torch.empty(R, C, N, dtype=torch.float32, device=x.device)
+    channels, states, _ = _padded(C, N)
+    kept = torch.empty(R, -(-T // EVERY), channels, states, dtype=torch.float32, device=x.device) if keep else None
+    with L.on_device_of(x) as stream:
+        args, work = _args(x, dt, z, b, c, a, None, d, initial, last, y, kept, None, N, 1, 0, softplus, False)
+        _launch(args, x.dtype is torch.float32, False, stream)
+    return y, last, kept
+
+
+def _backward(x, dt, a, b, c, d, z, initial, kept, softplus: bool, dy, dlast):
+    """-> dx, ddt, da, db, dc, dd, dz, dinitial."""
+    R, T, C = x.shape
+    N, dev = a.shape[1], x.device
+    channels, states, warps = _padded(C, N)
+    f32 = dict(dtype=torch.float32, device=dev)
+    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+    dx, ddt, dz, db, dc, da, dd, dinitial = like(x), like(dt), like(z), like(b), like(c), like(a), like(d), like(initial)
+    with L.on_device_of(x) as stream:
+        args, work = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False)
+        bc = torch.empty(warps // 4, R * T, 2, states, **f32)
+        parts = torch.empty(R * args.segments, channels, states + 1, **f32)
+        at, row, token = _rows(dy)
+        grad = _Grad(args, at, row, token, *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial, bc, parts)),
+                     parts.data_ptr() + 4 * R * args.segments * channels * states)
+        L.check(L.load().dewb_selective_grad(ctypes.byref(grad), ctypes.c_int(int(x.dtype is torch.float32)), ctypes.c_void_p(stream)), "selective_grad")
+        L.count_launches(2 if args.segments == 1 else 3)
+    return dx, ddt, da, db, dc, dd, dz, dinitial
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, a, b, c, d, z, initial, softplus):
+        ctx.set_materialize_grads(False)
+        ctx.softplus = softplus
+        y, last, kept = _forward(x, dt, a, b, c, d, z, initial, softplus, True)
+        ctx.save_for_backward(x, dt, a, b, c, d, z, initial, kept)
+        return y, last
+
+    @staticmethod
+    def backward(ctx, dy, dlast):
+        *ins, kept = ctx.saved_tensors
+        x = ins[0]
+        if torch.is_grad_enabled():                          # (create_graph: the kernel's results would have no history)
+            return (*_plain_gradients(ins, ctx.softplus, dy, dlast, ctx.needs_input_grad), None)
+        dy = torch.zeros_like(x) if dy is None else _dense(dy.to(x.dtype))
+        dx, ddt, da, db, dc, dd, dz, dinitial = _backward(*ins, kept, ctx.softplus, dy, None if dlast is None else dlast.float().contiguous())
+        return dx, ddt, da, db, dc, dd, dz, dinitial, None
+
+
+def _plain_gradients(ins, softplus, dy, dlast, needed):
+    from .scan import selective_scan_chunked
+    out = selective_scan_chunked(*ins, softplus=softplus)
+    pairs = [(o, g) for o, g in zip(out, (dy, dlast)) if g is not None]
+    at = [i for i, t in enumerate(ins) if t is not None and needed[i]]
+    grads = torch.autograd.grad([o for o, _ in pairs], [ins[i] for i in at], [g for _, g in pairs], create_graph=True, allow_unused=True)
+    return [grads[at.index(i)] if i in at else None for i in range(len(ins))]
+
+
+def kernel_available(x: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """Whether the scan of whole rows runs on the kernels: a GPU's tensors of up to 32 bits, nothing that has to be seen through."""
+    given = [t for t in (x, *others) if t is not None]
+    return (x.is_cuda and x.dim() == 3 and all(t.dtype in (torch.bfloat16, torch.float16, torch.float32) for t in given) and not L.transformed(*given)
+            and L.use_cuda(x))
+
+
+def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplus: bool = False):
+    """``ops.scan.selective_scan`` on the kernels."""
+    R, T, C = x.shape
+    N = A.shape[-1]
+    given = [t for t in (dt, A, Bm, Cm, D, z, initial_state) if t is not None]
+    if any(t.device != x.device for t in given):
+        raise ValueError("selective_scan: tensors of one device")
+    out_type = x.dtype
+    # one type for what is per token: where they differ (or are fp16) in fp32, which holds every value of each
+    one = out_type is not torch.float16 and all(t is None or t.dtype is out_type for t in (Bm, Cm, z)) and dt.dtype in (out_type, torch.float32)
+    fit = lambda t, *size: None if t is None else _dense((t if one else t.float()).expand(size))
+    fp32 = lambda t, *size: None if t is None else t.float().expand(size).contiguous()
+    ins = (fit(x, R, T, C), fit(dt, R, T, C), fp32(A, C, N), fit(Bm, R, T, N), fit(Cm, R, T, N), fp32(D, C), fit(z, R, T, C), fp32(initial_state, R, C, N))
+    if 0 in (R, T, C, N):
+        from .scan import selective_scan_chunked
+        return selective_scan_chunked(x, dt, A, Bm, Cm, D, z, initial_state, softplus=softplus)
+    y, last = _forward(*ins, softplus, False)[:2] if L.unrecorded(*ins) else _SelectiveScan.apply(*ins, softplus)
+    return y.to(out_type), last
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# a call's rows, with the states of a store
+
+
+def _check(what: str, x, dt, b, c, z, state, rows: Optional[Rows], state_shape, per_token, widths) -> None:
+    if x.dim() != 3:
+        raise ValueError(f"{what}: x [rows, tokens, channels], got {tuple(x.shape)}")
+    R, S = x.shape[:2]
+    if x.dtype not in (torch.bfloat16, torch.float32) or any(t is not None and t.dtype is not x.dtype for t in per_token) or dt.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{what}: bf16 or fp32 tokens of one type and steps of that type or fp32, got {[t.dtype for t in (x, dt, *per_token) if t is not None]}")
+    for t, n in widths:
+        if t is not None and t.shape != (R, S, n):
+            raise ValueError(f"{what}: [{R}, {S}, {n}] beside x {tuple(x.shape)}, got {tuple(t.shape)}")
+    tensors = [dt, b, c, z, state]
+    if rows is not None:
+        tensors += [rows.positions, rows.lengths, rows.row_ids]
+        if rows.positions.shape != (R, S) or rows.lengths.shape != (R,) or (rows.row_ids is not None and rows.row_ids.shape != (R,)):
+            raise ValueError(f"{what}: positions [rows, tokens], lengths and row ids [rows] of {R} rows of {S} tokens")
+        if any(t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()) for t in (rows.positions, rows.lengths, rows.row_ids)):
+            raise TypeError(f"{what}: positions, lengths and row ids are int32 in one piece")
+    if state is not None:
+        if state.shape[1:] != state_shape or state.dtype is not torch.float32 or not state.is_contiguous():
+            raise ValueError(f"{what}: an fp32 state [store rows, {', '.join(map(str, state_shape))}] in one piece, got {tuple(state.shape)}, {state.dtype}")
+        if (rows is None or rows.row_ids is None) and state.shape[0] < R:
+            raise ValueError(f"{what}: {R} rows against a store of {state.shape[0]}")
+    if any(t is not None and t.device != x.device for t in tensors):
+        raise ValueError(f"{what}: tensors of one device")
+
+
+def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: int, heads: int) -> torch.Tensor:
+    x, dt, z, b, c = (_dense(t) for t in (x, dt, z, b, c))
+    f32 = lambda t: None if t is None else t.detach().float().contiguous()
+    a, dt_bias, d = f32(a), f32(dt_bias), f32(d)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with L.on_device_of(x) as stream:
+        args, work = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0])
+        _launch(args, x.dtype is torch.float32, x.shape[1] == 1 and state is not None, stream)
+    return y
+
+
+def selective_tokens_reference(x, dt, A_log, Bm, Cm, D=None, z=None, rows: Optional[Rows] = None, state=None):
+    from .recurrence import _tokens as walk
+    R, S, C = x.shape
+    rows = whole(R, S, x.device) if rows is None else rows
+    step, A = F.softplus(dt.float(), threshold=60.0), -torch.exp(A_log.float())
+    xf, Bf, Cf = x.float(), Bm.float(), Cm.float()
+
+    def body(t, now):
+        h = torch.exp(step[:, t].unsqueeze(-1) * A) * now[0] + (step[:, t] * xf[:, t]).unsqueeze(-1) * Bf[:, t].unsqueeze(1)
+        y = torch.einsum("rcn,rn->rc", h, Cf[:, t])
+        y = y if D is None else y + xf[:, t] * D.float()
+        return [h], y if z is None else y * F.silu(z[:, t].float())
+    return walk(rows, [state], [xf.new_zeros(R, *A.shape)], body, (R, S, C), x.dtype)
+
+
+def selective_tokens(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                     rows: Optional[Rows] = None, state: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A call's tokens ``x [R, S, C]`` through the selective scan: the steps' logits ``dt [R, S, C]``, ``A_log [C, N]`` (rates ``-exp(A_log)``), ``Bm, Cm [R, S, N]``, ``D [C]``, the gate's
+    input ``z [R, S, C]`` (columns of wider rows will do) -> ``[R, S, C]``.  ``state [store rows, C, N]`` goes on in place (none: whole rows from nothing, nothing kept); a store row
+    belongs to one row of a call.  Rows outside the store are reported by the status word (``library.check_status``) and give zeros."""
+    N = A_log.shape[-1]
+    C = x.shape[-1]
+    _check("selective_tokens", x, dt, Bm, Cm, z, state, rows, (C, N), (Bm, Cm, z), ((dt, C), (z, C), (Bm, N), (Cm, N)))
+    if A_log.shape != (C, N) or (D is not None and D.shape != (C,)):
+        raise ValueError(f"selective_tokens: A_log [{C}, states] and D [{C}], got {tuple(A_log.shape)}, {None if D is None else tuple(D.shape)}")
+    if N > MOST_STATES or 0 in x.shape or not kernel_ok(x, dt, A_log, Bm, Cm, D, z) or L.transformed(x, dt, A_log, Bm, Cm, D, z):
+        return selective_tokens_reference(x, dt, A_log, Bm, Cm, D, z, rows, state) if 0 not in x.shape else torch.zeros_like(x)
+    return _tokens(x, dt, z, Bm, Cm, A_log, None, D, whole(*x.shape[:2], x.device) if rows is None else rows, state, N, 1, 0)
+
+
+def ssd_tokens_reference(x, dt, dt_bias, A_log, Bm, Cm, D, H: int, G: int, rows: Optional[Rows] = None, state=None):
+    from .recurrence import _tokens as walk
+    R, S, _ = x.shape
+    rows = whole(R, S, x.device) if rows is None else rows
+    xf = x.float().view(R, S, H, -1)
+    Bf, Cf = (t.float().reshape(R, S, G, -1).repeat_interleave(H // G, 2) for t in (Bm, Cm))
+    step = F.softplus(dt.float() if dt_bias is None else dt.float() + dt_bias.float(), threshold=60.0)
+    decay = torch.exp(-step * torch.exp(A_log.float()))
+
+    def body(t, now):
+        h = decay[:, t, :, None, None] * now[0] + (step[:, t, :, None] * xf[:, t]).unsqueeze(-1) * Bf[:, t].unsqueeze(2)
+        y = torch.einsum("rhpn,rhn->rhp", h, Cf[:, t])
+        return [h], y if D is None else y + xf[:, t] * D.float()[:, None]
+    return walk(rows, [state], [xf.new_zeros(R, H, xf.shape[-1], Bf.shape[-1])], body, x.shape, x.dtype)
+
+
+def ssd_tokens(x: torch.Tensor, dt: torch.Tensor, dt_bias: Optional[torch.Tensor], A_log: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, D: Optional[torch.Tensor], H: int, G: int,
+               rows: Optional[Rows] = None, state: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A call's tokens through the state space scan with a decay per head: ``x [R, S, H P]``, the steps' logits ``dt [R, S, H]`` and their bias ``[H]``, ``A_log [H]``, ``Bm, Cm [R, S, G N]``
+    (head h uses those of group ``h // (H // G)``), ``D [H]`` -> ``[R, S, H P]``.  ``state [store rows, H, P, N]`` as in ``selective_tokens``."""
+    if H < 1 or G < 1 or H % G or x.shape[-1] % H or Bm.shape[-1] % G or x.shape[-1] == 0:
+        raise ValueError(f"ssd_tokens: {H} heads in {G} groups of x {tuple(x.shape)}, B {tuple(Bm.shape)}")
+    P, N = x.shape[-1] // H, Bm.shape[-1] // G
+    _check("ssd_tokens", x, dt, Bm, Cm, None, state, rows, (H, P, N), (Bm, Cm), ((dt, H), (Bm, G * N), (Cm, G * N)))
+    if any(t is not None and t.shape != (H,) for t in (dt_bias, A_log, D)):
+        raise ValueError(f"ssd_tokens: a number per head, {H}, for A_log, the steps' bias and D")
+    if N > MOST_HEAD_STATES or 0 in x.shape or N == 0 or not kernel_ok(x, dt, dt_bias, A_log, Bm, Cm, D) or L.transformed(x, dt, dt_bias, A_log, Bm, Cm, D):
+        return ssd_tokens_reference(x, dt, dt_bias, A_log, Bm, Cm, D, H, G, rows, state) if 0 not in x.shape else torch.zeros_like(x)
+    return _tokens(x, dt, None, Bm, Cm, A_log, dt_bias, D, whole(*x.shape[:2], x.device) if rows is None else rows, state, N, G, H)

@@ -1,0 +1,166 @@
+"""The selective scan's kernels against the scan token by token in 64 bits: whole rows with every gradient, and a call's rows with the states of a store."""
+import pytest
+import torch
+
+from dew_b200.ops import library as L
+from dew_b200.ops import scan, selective
+from selective_cases import NAMES, check, companion, inputs, rows
+from selective_cases import scan as oracle
+from selective_cases import softplus
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+DEV = "cuda"
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def most(t, steps=True):
+    s = softplus(t["dt"].double()) if steps else t["dt"].double()
+    return float(s.amax() * t["a"].abs().amax())
+
+
+# one token, a tile and its neighbours, segments; channels of a warp, of a block and odd ones; every width of the lanes over the states; rows of a wider tensor
+SCANS = [(1, 1, 1, 1, FP32, {}), (2, 15, 3, 4, FP32, dict(gate=False)), (1, 16, 32, 16, BF16, {}), (3, 17, 129, 16, BF16, dict(initial=True)), (2, 130, 31, 17, FP32, dict(strided=True)),
+         (1, 300, 64, 24, BF16, dict(strided=True, skip=False)), (2, 70, 20, 33, FP32, dict(initial=True)), (1, 33, 24, 64, BF16, dict(gate=False, skip=False)),
+         (2, 40, 12, 100, FP32, dict(initial=True)), (1, 150, 17, 128, BF16, dict(initial=True)), (2, 200, 520, 16, FP32, dict(steps=False, initial=True)),
+         (1, 96, 64, 16, BF16, dict(dt_type=FP32, steps=False))]
+
+
+@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("B,T,C,N,dtype,more", SCANS)
+def test_scan_and_gradients(B, T, C, N, dtype, more, pieces, monkeypatch):
+    if pieces == "one":
+        monkeypatch.setattr(selective, "WARPS", 1)
+    steps = more.get("steps", True)
+    t = inputs(B, T, C, N, dtype, DEV, T + C, **more)
+    with torch.no_grad():
+        y, last = scan.selective_scan(*t.values(), softplus=steps)
+    leaves = {n: None if v is None else v.detach().requires_grad_() for n, v in t.items()}
+    out = scan.selective_scan(*leaves.values(), softplus=steps)
+    assert torch.equal(out[0], y) and torch.equal(out[1], last)
+    g = torch.Generator(DEV).manual_seed(5)
+    dy, dlast = torch.randn(B, T, C, generator=g, device=DEV).to(dtype), torch.randn(B, C, N, generator=g, device=DEV)
+    given = [n for n in NAMES if t[n] is not None]
+    grads = torch.autograd.grad(out, [leaves[n] for n in given], (dy, dlast))
+    L.check_status()
+    got = dict(y=y, last=last, **{f"d{n}": v for n, v in zip(given, grads)})
+    assert all(got[f"d{n}"].dtype is t[n].dtype for n in given)
+    check(got, oracle(**t, steps=steps, dy=dy, dlast=dlast), companion(**t, steps=steps, dy=dy, dlast=dlast), T, C, N, most(t, steps))
+
+
+def test_gradients_that_are_missing():
+    """A gradient of one result alone; leaves that need none."""
+    t = inputs(2, 50, 24, 16, FP32, DEV, 3, initial=True)
+    for which in ("y", "last"):
+        leaves = {n: v.detach().requires_grad_(n in ("x", "a", "initial")) for n, v in t.items()}
+        y, last = scan.selective_scan(*leaves.values(), softplus=True)
+        w = torch.randn_like(y if which == "y" else last)
+        grads = torch.autograd.grad(y if which == "y" else last, [leaves[n] for n in ("x", "a", "initial")], w)
+        given = dict(dy=w) if which == "y" else dict(dy=torch.zeros_like(y), dlast=w)
+        want, size = oracle(**t, steps=True, **given), companion(**t, steps=True, **given)
+        got = {f"d{n}": g for n, g in zip(("x", "a", "initial"), grads)}
+        check(got, {n: want[n] for n in got}, size, 50, 24, 16, most(t))
+
+
+def call(R, S, C, N, dtype, seed, first, lengths, ids, strided=False):
+    t = inputs(R, S, C, N, dtype, DEV, seed, strided=strided)
+    g = torch.Generator(DEV).manual_seed(seed + 1)
+    store = (R if ids is None else max(ids) + 1) + 2
+    return t, rows(first, lengths, S, ids, DEV), torch.randn(store, C, N, generator=g, device=DEV)
+
+
+TOKENS = [(1, 1, 64, 16, BF16, [9], [1], None), (4, 1, 130, 16, BF16, [3, 0, -1, 70], [1] * 4, [5, 1, 0, 2]), (3, 1, 7, 5, FP32, [0, 2, 9], [1] * 3, None),
+          (2, 1, 33, 24, FP32, [4, 4], [1, 1], [1, 0]), (5, 1, 40, 128, BF16, [1] * 5, [1] * 5, None), (3, 1, 100, 10, BF16, [8, 0, 3], [1] * 3, [4, 2, 0]),
+          (4, 40, 72, 16, BF16, [0, 5, -1, 30], [40, 1, 0, 17], [3, 0, 1, 6]), (2, 300, 33, 16, FP32, [0, 64], [131, 300], None), (3, 150, 20, 100, FP32, [7, 0, 1], [150, 3, 64], [2, 1, 0]),
+          (1, 256, 512, 16, BF16, [512], [256], [1])]
+
+
+@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("R,S,C,N,dtype,first,lengths,ids", TOKENS)
+def test_tokens_with_states(R, S, C, N, dtype, first, lengths, ids, pieces, monkeypatch):
+    if pieces == "one":
+        monkeypatch.setattr(selective, "WARPS", 1)
+    t, r, state = call(R, S, C, N, dtype, S + C, first, lengths, ids, strided=C % 2 == 0)
+    before = state.clone()
+    a_log = torch.log(-t["a"])
+    y = selective.selective_tokens(t["x"], t["dt"], a_log, t["b"], t["c"], t["d"], t["z"], r, state)
+    L.check_status()
+    untouched = torch.ones(len(state), dtype=torch.bool)
+    for i, (f, n) in enumerate(zip(first, lengths)):
+        at = i if ids is None else ids[i]
+        if f < 0:
+            assert not y[i].any()
+            continue
+        untouched[at] = False
+        assert not y[i, n:].any()
+        one = {k: None if v is None else v[i:i + 1, :n] if v.dim() == 3 else v for k, v in t.items()}
+        one["initial"] = before[at:at + 1] if f > 0 else None
+        check(dict(y=y[i:i + 1, :n], last=state[at:at + 1]), oracle(**one, steps=True), companion(**one, steps=True), n, C, N, 2 * most(t))
+    assert torch.equal(state[untouched], before[untouched])
+
+
+def test_whole_rows_and_rows_in_two_calls():
+    """Rows without a store are whole rows; a row's tokens in two calls and one by one are its tokens in one."""
+    t, r, state = call(2, 96, 48, 16, FP32, 4, [0, 0], [96, 96], None)
+    a_log, per = torch.log(-t["a"]), ("x", "dt", "b", "c", "z")
+    run = lambda lo, hi, r, s: selective.selective_tokens(*(t[n][:, lo:hi] if n in per else a_log if n == "a" else t[n] for n in ("x", "dt", "a", "b", "c", "d", "z")), r, s)
+    want = run(0, 96, None, None)
+    assert torch.equal(want, run(0, 96, r, state))
+    again = torch.full_like(state, float("nan"))
+    parts = [run(0, 64, rows([0, 0], [64, 64], 64, None, DEV), again)] + [run(i, i + 1, rows([i, i], [1, 1], 1, None, DEV), again) for i in range(64, 96)]
+    got = torch.cat(parts, 1)
+    one = dict(t, initial=None)
+    check(dict(y=got, last=again[:2]), oracle(**one, steps=True), companion(**one, steps=True), 96, 48, 16, most(t))
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+
+
+def heads(R, S, H, G, P, N, dtype, seed, first, lengths, ids):
+    g = torch.Generator(DEV).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    wide = r(R, S, H * P + 2 * G * N + 1).to(dtype)
+    t = dict(x=wide[..., 1:1 + H * P], dt=(r(R, S, H) - 3).to(dtype), dt_bias=r(H), a_log=r(H), b=wide[..., 1 + H * P:1 + H * P + G * N], c=wide[..., 1 + H * P + G * N:], d=r(H))
+    store = (R if ids is None else max(ids) + 1) + 1
+    return t, rows(first, lengths, S, ids, DEV), r(store, H, P, N)
+
+
+HEADS = [(1, 1, 4, 1, 64, 128, BF16, [5], [1], None), (3, 1, 6, 2, 48, 80, BF16, [0, 7, -1], [1] * 3, [2, 0, 3]), (2, 1, 3, 1, 5, 7, FP32, [1, 2], [1, 1], None),
+         (2, 1, 2, 1, 16, 256, BF16, [3, 0], [1, 1], [1, 0]), (2, 1, 4, 4, 100, 16, FP32, [3, 9], [1, 1], None), (1, 1, 2, 1, 33, 30, BF16, [6], [1], None),
+         (3, 50, 4, 2, 32, 16, BF16, [0, 9, -1], [50, 13, 0], [1, 0, 3]), (2, 140, 2, 1, 64, 128, BF16, [0, 3], [140, 70], None), (2, 33, 3, 3, 20, 33, FP32, [0, 4], [1, 33], [2, 1]),
+         (1, 200, 2, 1, 48, 200, FP32, [2], [200], None)]
+
+
+@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("R,S,H,G,P,N,dtype,first,lengths,ids", HEADS)
+def test_heads_with_states(R, S, H, G, P, N, dtype, first, lengths, ids, pieces, monkeypatch):
+    """A decay per head is a rate per channel and state that is one number in each head."""
+    if pieces == "one":
+        monkeypatch.setattr(selective, "WARPS", 1)
+    t, r, state = heads(R, S, H, G, P, N, dtype, S + H, first, lengths, ids)
+    before = state.clone()
+    y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], H, G, r, state)
+    L.check_status()
+    untouched = torch.ones(len(state), dtype=torch.bool)
+    for i, (f, n) in enumerate(zip(first, lengths)):
+        at = i if ids is None else ids[i]
+        if f < 0:
+            assert not y[i].any()
+            continue
+        untouched[at] = False
+        assert not y[i, n:].any()
+        for h in range(H):
+            g, cols = h // (H // G), slice(h * P, (h + 1) * P)
+            one = dict(x=t["x"][i:i + 1, :n, cols], dt=(t["dt"][i:i + 1, :n, h:h + 1].double() + t["dt_bias"][h].double()).expand(-1, -1, P), a=-t["a_log"][h].double().exp().expand(P, N),
+                       b=t["b"][i:i + 1, :n, g * N:(g + 1) * N], c=t["c"][i:i + 1, :n, g * N:(g + 1) * N], d=t["d"][h].expand(P), initial=before[at:at + 1, h] if f > 0 else None)
+            check(dict(y=y[i:i + 1, :n, cols], last=state[at:at + 1, h]), oracle(**one, steps=True), companion(**one, steps=True), n, P, N, 2 * most(one))
+    assert torch.equal(state[untouched], before[untouched])
+
+
+def test_rows_outside_the_store_are_reported():
+    t, r, state = call(3, 1, 16, 16, BF16, 1, [1, 1, 1], [1] * 3, [0, 1, 2])
+    before = state.clone()
+    for S, bad in ((1, 5), (1, -1), (40, 5)):
+        t, _, _ = call(3, S, 16, 16, BF16, 1, [1, 1, 1], [S] * 3, [0, 1, 2])
+        r = rows([1, 1, 1], [S] * 3, S, [0, bad, 2], DEV)
+        y = selective.selective_tokens(t["x"], t["dt"], torch.log(-t["a"]), t["b"], t["c"], t["d"], t["z"], r, state)
+        with pytest.raises(L.KernelError, match="bad argument"):
+            L.check_status()
+        assert not y[1].any() and y[0].any() and torch.equal(state[3:], before[3:])
