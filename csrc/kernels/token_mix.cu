@@ -1,6 +1,6 @@
 // What a token takes from its neighbours, and the small products and norms around a recurrence, for sm_100a.
 //
-//   conv_tokens     a short causal convolution per channel over a call's tokens, behind the bias of the projection it follows, with or without silu;
+//   conv_tokens     a short causal convolution per channel over a call's tokens, behind the bias of the projection it follows, with or without an offset of its own and silu;
 //                   the inputs in front of the call's first token come from the row's state, zeros at a sequence's start
 //   conv_tail       the row's state after the call: its last taps - 1 inputs (taps 2: the previous token itself)
 //   conv_step       both for one token per row
@@ -36,8 +36,8 @@ constexpr int MAX_TAPS = 64;
 // TAPS 0: any number of taps, re-read from memory; else the inputs slide through registers.
 template <typename T, int V, int TAPS>
 __global__ void __launch_bounds__(128)
-conv_tokens_kernel(const T* __restrict__ x, long long row_stride, const T* __restrict__ bias, const T* __restrict__ w, const float* __restrict__ state,
-                   const int* __restrict__ positions, const int* __restrict__ row_ids, int S, int C, int taps_rt, int act, T* __restrict__ y) {
+conv_tokens_kernel(const T* __restrict__ x, long long row_stride, const T* __restrict__ bias, const T* __restrict__ w, const T* __restrict__ offset,
+                   const float* __restrict__ state, const int* __restrict__ positions, const int* __restrict__ row_ids, int S, int C, int taps_rt, int act, T* __restrict__ y) {
   const int taps = TAPS ? TAPS : taps_rt;
   const int c = (blockIdx.x * 128 + threadIdx.x) * V, row = blockIdx.z, t0 = blockIdx.y * RUN;
   if (c >= C) return;
@@ -46,10 +46,11 @@ conv_tokens_kernel(const T* __restrict__ x, long long row_stride, const T* __res
   T* yr = y + static_cast<long long>(row) * S * C + c;
   const int r = row_ids == nullptr ? row : row_ids[row];
   const float* st_row = state != nullptr && pos[0] > 0 ? state + (static_cast<long long>(r) * C + c) * (taps - 1) : nullptr;
-  float b[V];
+  float b[V], add[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) b[j] = 0.f;
+  for (int j = 0; j < V; ++j) b[j] = add[j] = 0.f;
   if (bias != nullptr) load_v<V>(bias + c, b);
+  if (offset != nullptr) load_v<V>(offset + c, add);
   auto input = [&](int t, float (&u)[V]) {
     if (t >= 0) {
       load_v<V>(xr + t * row_stride, u);
@@ -92,7 +93,7 @@ conv_tokens_kernel(const T* __restrict__ x, long long row_stride, const T* __res
         const bool live = pos[t + s] >= 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          o[j] = 0.f;
+          o[j] = add[j];
 #pragma unroll
           for (int q = 0; q < TAPS; ++q) o[j] += wt[j][q] * u[q + s][j];
           if (!live) o[j] = 0.f;
@@ -106,6 +107,8 @@ conv_tokens_kernel(const T* __restrict__ x, long long row_stride, const T* __res
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = 0.f;
       if (pos[t] >= 0) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = add[j];
         for (int q = 0; q < taps; ++q) {
           float u[V];
           input(t - taps + 1 + q, u);
@@ -139,8 +142,8 @@ conv_tail_kernel(const T* __restrict__ x, long long row_stride, const T* __restr
 // One token per row: y [R, C], and the state moves on.
 template <typename T>
 __global__ void __launch_bounds__(128)
-conv_step_kernel(const T* __restrict__ x, long long row_stride, const T* __restrict__ bias, const T* __restrict__ w, float* __restrict__ state,
-                 const int* __restrict__ positions, const int* __restrict__ row_ids, int C, int taps, int act, T* __restrict__ y) {
+conv_step_kernel(const T* __restrict__ x, long long row_stride, const T* __restrict__ bias, const T* __restrict__ w, const T* __restrict__ offset,
+                 float* __restrict__ state, const int* __restrict__ positions, const int* __restrict__ row_ids, int C, int taps, int act, T* __restrict__ y) {
   const int c = blockIdx.x * 128 + threadIdx.x, row = blockIdx.y;
   if (c >= C) return;
   const int p = positions[row], keep = taps - 1;
@@ -149,7 +152,7 @@ conv_step_kernel(const T* __restrict__ x, long long row_stride, const T* __restr
   const float u = ld(x + row * row_stride + c) + (bias == nullptr ? 0.f : ld(bias + c));
   const T* wc = w + static_cast<long long>(c) * taps;
   float* s = state + (static_cast<long long>(row_ids == nullptr ? row : row_ids[row]) * C + c) * keep;
-  float o = ld(wc + keep) * u;
+  float o = ld(wc + keep) * u + (offset == nullptr ? 0.f : ld(offset + c));
   for (int j = 0; j < keep; ++j) {
     const float v = p > 0 ? s[j] : 0.f;
     o += ld(wc + j) * v;
@@ -331,18 +334,18 @@ head_gated_norm_kernel(const T* __restrict__ x, const T* __restrict__ gate, long
 }
 
 template <typename T>
-int conv_any(const T* x, long long rs, const T* bias, const T* w, float* state, const int* positions, const int* lengths, const int* row_ids, int R, int S,
-             int C, int taps, int act, T* y, cudaStream_t stream) {
+int conv_any(const T* x, long long rs, const T* bias, const T* w, const T* offset, float* state, const int* positions, const int* lengths, const int* row_ids,
+             int R, int S, int C, int taps, int act, T* y, cudaStream_t stream) {
   if (S == 1 && state != nullptr) {
-    conv_step_kernel<T><<<dim3((C + 127) / 128, R), 128, 0, stream>>>(x, rs, bias, w, state, positions, row_ids, C, taps, act, y);
+    conv_step_kernel<T><<<dim3((C + 127) / 128, R), 128, 0, stream>>>(x, rs, bias, w, offset, state, positions, row_ids, C, taps, act, y);
     return static_cast<int>(cudaGetLastError());
   }
   constexpr int W = sizeof(T) == 2 ? 8 : 4;
-  const bool vec = C % W == 0 && rs % W == 0 && aligned(x, 16) && aligned(bias, 16) && aligned(y, 16);
+  const bool vec = C % W == 0 && rs % W == 0 && aligned(x, 16) && aligned(bias, 16) && aligned(offset, 16) && aligned(y, 16);
   const int per = 128 * (vec ? W : 1);
   const dim3 grid((C + per - 1) / per, (S + RUN - 1) / RUN, R);
   if (grid.y > 65535u) return -3;
-#define DEWB_CONV(VV, KK) conv_tokens_kernel<T, VV, KK><<<grid, 128, 0, stream>>>(x, rs, bias, w, state, positions, row_ids, S, C, taps, act, y)
+#define DEWB_CONV(VV, KK) conv_tokens_kernel<T, VV, KK><<<grid, 128, 0, stream>>>(x, rs, bias, w, offset, state, positions, row_ids, S, C, taps, act, y)
   if (vec) { if (taps == 4) DEWB_CONV(W, 4); else if (taps == 3) DEWB_CONV(W, 3); else if (taps == 2) DEWB_CONV(W, 2); else DEWB_CONV(W, 0); }
   else DEWB_CONV(1, 0);
 #undef DEWB_CONV
@@ -370,18 +373,18 @@ int shift_any(const T* x, const T* mu, float* state, const int* positions, const
 
 using namespace dewb::tokenmix;
 
-// x [R * S, row_stride >= C] -> y [R, S, C]; bias [C] (null: none), w [C, taps], state [store rows, C, taps - 1] (null: nothing before, nothing kept);
+// x [R * S, row_stride >= C] -> y [R, S, C]; bias [C] (null: none), w [C, taps], offset [C] (null: none), state [store rows, C, taps - 1] (null: nothing before, nothing kept);
 // lengths [R]: the position after a row's last token.  `act`: silu.
-extern "C" int dewb_conv_tokens(const void* x, long long row_stride, const void* bias, const void* w, float* state, const int* positions, const int* lengths,
+extern "C" int dewb_conv_tokens(const void* x, long long row_stride, const void* bias, const void* w, const void* offset, float* state, const int* positions, const int* lengths,
                                 const int* row_ids, int R, int S, int C, int taps, int act, void* y, int fp32, void* stream_ptr) {
   if (R <= 0 || S <= 0) return 0;
   if (C < 1 || taps < 1 || taps > MAX_TAPS || row_stride < C || R > 65535 || (state != nullptr && lengths == nullptr)) return -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  if (fp32) return conv_any<float>(static_cast<const float*>(x), row_stride, static_cast<const float*>(bias), static_cast<const float*>(w), state, positions,
-                                   lengths, row_ids, R, S, C, taps, act, static_cast<float*>(y), stream);
+  if (fp32) return conv_any<float>(static_cast<const float*>(x), row_stride, static_cast<const float*>(bias), static_cast<const float*>(w),
+                                   static_cast<const float*>(offset), state, positions, lengths, row_ids, R, S, C, taps, act, static_cast<float*>(y), stream);
   return conv_any<dewb::rows::bf16>(static_cast<const dewb::rows::bf16*>(x), row_stride, static_cast<const dewb::rows::bf16*>(bias),
-                                    static_cast<const dewb::rows::bf16*>(w), state, positions, lengths, row_ids, R, S, C, taps, act,
-                                    static_cast<dewb::rows::bf16*>(y), stream);
+                                    static_cast<const dewb::rows::bf16*>(w), static_cast<const dewb::rows::bf16*>(offset), state, positions, lengths, row_ids, R, S, C,
+                                    taps, act, static_cast<dewb::rows::bf16*>(y), stream);
 }
 
 // x [R, S, d], mu [n, d] -> out [n, R, S, d]; state [store rows, d] (null: zeros before every row, nothing kept)

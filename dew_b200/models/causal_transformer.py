@@ -580,12 +580,14 @@ class CausalTransformer(nn.Module):
         """One entry per layer run where the layers differ in what they keep (heads of their own widths, recurrent states); None where one
         shape of keys and values serves them all."""
         cfg, kinds = self.config, self.config.kinds()
-        if not (cfg.fp32_stack or cfg.layer_options is not None or cfg.query_temperature is not None or cfg.value_dim is not None or cfg.attn_chunk is not None
+        # a stack of state space layers keeps their states and no keys
+        recurrent = set(kinds) <= {"mamba", "mamba2", "none"} and set(kinds) != {"none"} and not cfg.depth_residual_block
+        if not (recurrent or cfg.fp32_stack or cfg.layer_options is not None or cfg.query_temperature is not None or cfg.value_dim is not None or cfg.attn_chunk is not None
                 or cfg.attn_head_gate or cfg.rotation is not None or cfg.keep_first or cfg.qk_unit_norm):
             return None
         if any(self._wants_tables(i) or not (k in ("mla", "lightning", "none") or hasattr(self.layers[i].mixer, "cache_slot")) for i, k in enumerate(kinds)):
             raise NotImplementedError("per-layer caches are built for attention without rotation ('nope') or with one of its own, 'mla' with one of its own, "
-                                      f"'lightning', 'gdn', 'mlstm', 'rwkv6' and 'pair' layers, not {sorted(set(kinds))}")
+                                      f"'lightning', 'gdn', 'mlstm', 'rwkv6', 'mamba', 'mamba2' and 'pair' layers, not {sorted(set(kinds))}")
         out, latest = [], {}
         for i, slot in self.runs():
             m = self.layers[i].mixer
@@ -757,6 +759,8 @@ class CausalTransformer(nn.Module):
             h = h * (cfg.emb_features ** 0.5)
         if cfg.embed_multiplier is not None:
             h = h * cfg.embed_multiplier
+        if positions is None and getattr(cache, "slots", None) is not None:
+            positions = torch.arange(h.shape[1], device=h.device)[None].expand(h.shape[0], -1)
         cos, sin = self.rope_tables(h.device)
         n_streams = max(cfg.hyper_connections, cfg.altup)
         if n_streams > 1:

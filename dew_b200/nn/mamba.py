@@ -1,14 +1,13 @@
 """Mamba-1 block: input projection to (x, z), short causal conv + SiLU, input-dependent (dt, B, C), selective scan, gate,
-output projection.  Reference: src/dew/nn/mixers/mamba.py (450 lines)."""
+output projection; a row of a cache keeps the convolution's last inputs and the scan's state.  Reference: src/dew/nn/mixers/mamba.py (450 lines)."""
 from __future__ import annotations
 
 import math
 
 import torch
 import torch.nn as nn
-import torch.nn.functional as F
 
-from ..ops import scan
+from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
 from .linear_attention import ShortConv
 
@@ -28,13 +27,39 @@ class Mamba(nn.Module):
         self.D = declare(nn.Parameter(torch.ones(inner, dtype=torch.float32, device=device)), ("mlp",), "scale")
         self.out_proj = Linear(inner, features, **kw)
 
-    def forward(self, x, segment_ids=None, cache=None, layer: int = 0, chunked: bool = True):
+    def fresh_state(self, batch: int) -> dict:
+        p = self.out_proj.weight
+        return {"conv": torch.zeros(batch, self.conv.kernel_size - 1, self.inner, dtype=p.dtype, device=p.device),
+                "S": torch.zeros(batch, self.inner, self.n, dtype=torch.float32, device=p.device)}
+
+    def cache_slot(self):
+        from .kv_cache import CacheSlot
+        conv = (("conv", (self.inner, self.conv.kernel_size - 1)),) if self.conv.kernel_size > 1 else ()
+        return CacheSlot(state=(self.inner, self.n), more=conv)
+
+    def _narrow(self, xi):
+        """The step's logits, B and C of every token."""
+        p = self.x_proj(xi)
+        return self.dt_proj(p[..., :self.dt_rank]), p[..., self.dt_rank:self.dt_rank + self.n], p[..., self.dt_rank + self.n:]
+
+    def _in_slot(self, x, cache, slot: int, positions):
+        """A call's tokens with the state in the cache's slot."""
+        rows, state, more = cache.call(positions).rows, cache.states[slot], cache.more[slot]
+        xz = self.in_proj(x)
+        xi = token_mix.conv_tokens(xz[..., :self.inner], self.conv.weight, None, self.conv.activation, rows, more.get("conv"), self.conv.bias)
+        dt, Bm, Cm = self._narrow(xi)
+        return self.out_proj(selective.selective_tokens(xi, dt, self.A_log, Bm, Cm, self.D, xz[..., self.inner:], rows, state))
+
+    def forward(self, x, segment_ids=None, cache=None, layer: int = 0, chunked: bool = True, positions=None):
+        if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+            return self._in_slot(x, cache, layer, positions)
         xz = self.in_proj(x)
         xi, z = xz[..., :self.inner], xz[..., self.inner:]
-        xi = self.conv(xi, segment_ids)
-        p = self.x_proj(xi)
-        dt = F.softplus(self.dt_proj(p[..., :self.dt_rank]).float())
-        Bm, Cm = p[..., self.dt_rank:self.dt_rank + self.n], p[..., self.dt_rank + self.n:]
+        state = cache.recurrent(layer, x.shape[0], self) if cache is not None and hasattr(cache, "recurrent") else None
+        xi = self.conv(xi, segment_ids, state["conv"] if state is not None else None)
+        dt, Bm, Cm = self._narrow(xi)
         fn = scan.selective_scan if chunked else scan.selective_scan_reference
-        y, _ = fn(xi, dt, -torch.exp(self.A_log.float()), Bm, Cm, self.D, z)
+        y, S = fn(xi, dt, -torch.exp(self.A_log.float()), Bm, Cm, self.D, z, initial_state=None if state is None else state["S"], softplus=True)
+        if state is not None:
+            state["S"].copy_(S)
         return self.out_proj(y.to(x.dtype))

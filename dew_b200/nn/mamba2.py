@@ -1,5 +1,5 @@
 """Mamba-2 mixer: input projection to ``[z | x | B | C | dt]``, short causal conv over ``[x | B | C]``, chunked SSD scan,
-gated RMSNorm, output projection.
+gated RMSNorm, output projection; a row of a cache keeps the convolution's last inputs and the scan's state.
 
 Parity: src/dew/nn/mixers/mamba2.py:101-587 (``chunk_ssd`` :101, ``recurrent_ssd`` :139, ``MambaRMSNormGated`` :194,
 ``Mamba2`` :233), numerics src/dew/nn/kernels/mamba_ssd.py:9-22.
@@ -13,7 +13,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from ..ops import scan
+from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
 from .linear_attention import ShortConv
 
@@ -52,7 +52,23 @@ class Mamba2(nn.Module):
         return {"conv": torch.zeros(batch, self.conv1d.kernel_size - 1, C, dtype=p.dtype, device=p.device),
                 "S": torch.zeros(batch, self.H, self.P, self.N, dtype=torch.float32, device=p.device)}
 
-    def forward(self, x, segment_ids=None, cache=None, layer: int = 0):
+    def cache_slot(self):
+        from .kv_cache import CacheSlot
+        conv = (("conv", (self.inner + 2 * self.G * self.N, self.conv1d.kernel_size - 1)),) if self.conv1d.kernel_size > 1 else ()
+        return CacheSlot(state=(self.H, self.P, self.N), more=conv)
+
+    def _in_slot(self, x, cache, slot: int, positions):
+        """A call's tokens with the state in the cache's slot."""
+        rows, state, more = cache.call(positions).rows, cache.states[slot], cache.more[slot]
+        z, xbc, dt = self.in_proj(x).split([self.inner, self.inner + 2 * self.G * self.N, self.H], -1)
+        xbc = token_mix.conv_tokens(xbc, self.conv1d.weight, None, self.conv1d.activation, rows, more.get("conv"), self.conv1d.bias)
+        xs, Bm, Cm = xbc.split([self.inner, self.G * self.N, self.G * self.N], -1)
+        y = selective.ssd_tokens(xs, dt, self.dt_bias, self.A_log, Bm, Cm, self.D, self.H, self.G, rows, state)
+        return self.out_proj(ops.gated_rms_norm(y, z, self.norm_weight, self.norm_eps, gate_first=not self.gate_after))
+
+    def forward(self, x, segment_ids=None, cache=None, layer: int = 0, positions=None):
+        if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+            return self._in_slot(x, cache, layer, positions)
         B, T, _ = x.shape
         zxbcdt = self.in_proj(x)
         z, xbc, dt = zxbcdt.split([self.inner, self.inner + 2 * self.G * self.N, self.H], -1)
@@ -70,9 +86,5 @@ class Mamba2(nn.Module):
             if state is not None:
                 state["S"].copy_(S)
         y = y.to(x.dtype).reshape(B, T, self.inner)
-        if self.gate_after:
-            y = ops.gated_rms_norm(y, z, self.norm_weight, self.norm_eps)              # norm, then gate (Falcon-H1's order)
-        else:
-            # Mamba-2's own order: the gate first, the norm over the whole width after (modeling_mamba2.py MambaRMSNormGated)
-            y = ops.rms_norm((y.float() * F.silu(z.float())).to(x.dtype), self.norm_weight, self.norm_eps)
-        return self.out_proj(y)
+        # Mamba-2's own order: the gate first, the norm over the whole width after (modeling_mamba2.py MambaRMSNormGated); gate_after: norm, then gate (Falcon-H1's)
+        return self.out_proj(ops.gated_rms_norm(y, z, self.norm_weight, self.norm_eps, gate_first=not self.gate_after))

@@ -311,9 +311,10 @@ def kda_chunked(q, k, v, g, beta, initial_state=None, scale: Optional[float] = N
 
 # ---------------------------------------------------------------------------------------------------------------
 # Mamba-1 selective scan.  Reference: src/dew/nn/kernels/templates/recurrence/selective.py, src/dew/nn/mixers/mamba.py.
-def selective_scan_reference(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None):
-    """``x, dt [B,T,C]``, ``A [C,N]`` (negative), ``Bm, Cm [B,T,N]``: ``h_t = exp(dt A) h_{t-1} + dt B x``; ``y = C h + D x``,
+def selective_scan_reference(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplus: bool = False):
+    """``x, dt [B,T,C]`` (with ``softplus``, the steps' logits), ``A [C,N]`` (negative), ``Bm, Cm [B,T,N]``: ``h_t = exp(dt A) h_{t-1} + dt B x``; ``y = C h + D x``,
     optionally gated by ``silu(z)``.  Sequential over T, fp32 state ``[B,C,N]``."""
+    dt = F.softplus(dt.float()) if softplus else dt
     Bsz, T, C = x.shape
     h = torch.zeros(Bsz, C, A.shape[1], dtype=torch.float32, device=x.device) if initial_state is None else initial_state.float().clone()
     xf, dtf, Af, Bf, Cf = x.float(), dt.float(), A.float(), Bm.float(), Cm.float()

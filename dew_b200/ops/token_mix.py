@@ -51,7 +51,7 @@ def same(t: Optional[torch.Tensor], dtype) -> Optional[torch.Tensor]:
     return None if t is None else t.detach().to(dtype).contiguous()
 
 
-def conv_tokens_reference(x, w, bias=None, silu: bool = False, rows: Optional[Rows] = None, state: Optional[torch.Tensor] = None):
+def conv_tokens_reference(x, w, bias=None, silu: bool = False, rows: Optional[Rows] = None, state: Optional[torch.Tensor] = None, offset=None):
     R, S, C = x.shape
     taps = w.shape[1]
     rows = whole(R, S, x.device) if rows is None else rows
@@ -63,6 +63,8 @@ def conv_tokens_reference(x, w, bias=None, silu: bool = False, rows: Optional[Ro
         before = torch.where((first > 0).view(R, 1, 1), state[at].transpose(1, 2), before)
     u = torch.cat([before, u], 1)
     y = sum(u[:, j:j + S] * w[:, j].float() for j in range(taps))
+    if offset is not None:
+        y = y + offset.float()
     if silu:
         y = F.silu(y)
     if state is not None and taps > 1:
@@ -74,16 +76,16 @@ def conv_tokens_reference(x, w, bias=None, silu: bool = False, rows: Optional[Ro
 
 
 def conv_tokens(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, silu: bool = False, rows: Optional[Rows] = None,
-                state: Optional[torch.Tensor] = None) -> torch.Tensor:
+                state: Optional[torch.Tensor] = None, offset: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [R, S, C]`` (columns of a wider row will do) through a causal convolution per channel, ``w [C, taps]`` with the token's own weight last, behind
-    ``bias [C]``; ``state [store rows, C, taps - 1]`` holds a row's last inputs."""
-    if not kernel_ok(x, w, bias):
-        return conv_tokens_reference(x, w, bias, silu, rows, state)
+    ``bias [C]`` and in front of ``offset [C]``; ``state [store rows, C, taps - 1]`` holds a row's last inputs."""
+    if not kernel_ok(x, w, bias, offset):
+        return conv_tokens_reference(x, w, bias, silu, rows, state, offset)
     R, S, C = x.shape
     rows = whole(R, S, x.device) if rows is None else rows
-    x, wk, b = rows_of(x), same(w, x.dtype), same(bias, x.dtype)
+    x, wk, b, add = rows_of(x), same(w, x.dtype), same(bias, x.dtype), same(offset, x.dtype)
     y = torch.empty(R, S, C, dtype=x.dtype, device=x.device)
-    L.check(L.load().dewb_conv_tokens(L.ptr(x), c_ll(x.stride(1)), L.ptr(b), L.ptr(wk), L.ptr(state), L.ptr(rows.positions), L.ptr(rows.lengths),
+    L.check(L.load().dewb_conv_tokens(L.ptr(x), c_ll(x.stride(1)), L.ptr(b), L.ptr(wk), L.ptr(add), L.ptr(state), L.ptr(rows.positions), L.ptr(rows.lengths),
                                       L.ptr(rows.row_ids), c_int(R), c_int(S), c_int(C), c_int(w.shape[1]), c_int(int(silu)), L.ptr(y),
                                       c_int(int(x.dtype == torch.float32)), L.stream_ptr()), "conv_tokens")
     L.count_launches(1 if S == 1 or state is None else 2)
