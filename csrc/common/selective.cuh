@@ -34,10 +34,12 @@ using bf16 = __nv_bfloat16;
 using Args = dewb_selective_args;
 
 constexpr int THREADS = 128, WARPS = 4;
-constexpr int TT = 16;                 // tokens of a tile
 constexpr int OUTSIDE = 6;             // the status of a row that the store does not have
 constexpr int EVERY = 16;              // tokens between two kept states
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
 
 template <int LN, int NS>
 struct Lay {
@@ -45,6 +47,7 @@ struct Lay {
   static constexpr int CW = 4 * CG;              // channels of a warp
   static constexpr int CB = WARPS * CW;          // ... of a block
   static constexpr int NP = LN * NS;             // states, padded
+  static constexpr int TT = NS > 4 ? 8 : 16;     // tokens of a tile
   static constexpr int PASSES = TT >= LN ? TT / LN : 1;      // a lane's pieces of four channels in a tile: token lane / CG + pass * LN
 };
 
@@ -53,8 +56,45 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// ln(1 + e^x) = max(x, 0) + ln(1 + t), t = e^-|x|: with q = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh q = 2 (q + q^3 / 3 + ... + q^13 / 13), the next term below 2e-8 of the sum
+__device__ __forceinline__ float softplus(float x) {
+  const float t = ex2(-LOG2E * fabsf(x)), q = t * rcp(2.f + t), r = q * q;
+  float p = fmaf(r, 1.f / 13.f, 1.f / 11.f);
+  p = fmaf(p, r, 1.f / 9.f);
+  p = fmaf(p, r, 1.f / 7.f);
+  p = fmaf(p, r, 1.f / 5.f);
+  p = fmaf(p, r, 1.f / 3.f);
+  p = fmaf(p, r, 1.f);
+  return fmaf(2.f * q, p, fmaxf(x, 0.f));
+}
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
+
+// Two fp32 numbers side by side, of two neighbouring channels: one instruction for both.
+struct f2 {
+  unsigned long long v;
+  __device__ __forceinline__ f2() {}
+  __device__ __forceinline__ f2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ float2 get() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ f2 mul(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+__device__ __forceinline__ f2 ex2(f2 x) {
+  const float2 t = x.get();
+  return f2(ex2(t.x), ex2(t.y));
+}
+__device__ __forceinline__ void pair(const float* p, f2& a, f2& b) {         // four numbers, 16 bytes
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  a.v = v.x; b.v = v.y;
+}
 
 __device__ __forceinline__ float ld(const float* p) { return *p; }
 __device__ __forceinline__ float ld(const bf16* p) { return __bfloat162float(*p); }
@@ -76,6 +116,11 @@ template <> struct Raw<float> {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   }
 };
+// A number as it lies in memory, and as fp32.
+__device__ __forceinline__ uint32_t word(const float* p) { return __float_as_uint(*p); }
+__device__ __forceinline__ uint32_t word(const bf16* p) { return *reinterpret_cast<const unsigned short*>(p); }
+template <typename T>
+__device__ __forceinline__ float value(uint32_t w) { return __uint_as_float(sizeof(T) == 2 ? w << 16 : w); }
 __device__ __forceinline__ uint32_t bits(const bf16* p) { return *reinterpret_cast<const unsigned short*>(p); }
 
 // `whole`: a vector load; else `n` (0 to 4) of the values, zeros behind.
@@ -119,20 +164,6 @@ __device__ __forceinline__ bool fours(const void* p, long long row, long long to
   return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && ((row | token) & 3) == 0;
 }
 
-// The steps' logits of four channels, bf16 or fp32.
-struct RawStep {
-  uint4 v;
-  __device__ __forceinline__ void get(float (&f)[4], bool fp32) const {
-    if (fp32) Raw<float>{v}.get(f);
-    else Raw<bf16>{make_uint2(v.x, v.y)}.get(f);
-  }
-};
-__device__ __forceinline__ RawStep fetch_step(const void* p, long long at, bool fp32, bool whole, int n) {
-  if (fp32) return {fetch(static_cast<const float*>(p) + at, whole, n).v};
-  const uint2 v = fetch(static_cast<const bf16*>(p) + at, whole, n).v;
-  return {make_uint4(v.x, v.y, 0u, 0u)};
-}
-
 // Sums of four channels' numbers over the LN lanes that share their states: the lane's result is that of channel `own_channel(lane)` (lanes with sl >= 4 hold copies).
 template <int LN>
 __device__ __forceinline__ float over_states(const float (&y)[4], int sl) {
@@ -145,6 +176,17 @@ __device__ __forceinline__ float over_states(const float (&y)[4], int sl) {
   return q;
 }
 __device__ __forceinline__ int own_channel(int sl) { return (sl & 1) * 2 + ((sl >> 1) & 1); }
+
+// The sum of `n` pieces of four, `stride` apart, from the `first` on and round (so that neighbouring lanes read from different banks).
+__device__ __forceinline__ float4 sum4(const float4* p, int n, int stride, int first) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const float4 v = p[((i + first) & (n - 1)) * stride];
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  return s;
+}
 
 // Which tokens of row `row` a call has, and where its state lies.
 struct Row {

@@ -4,8 +4,9 @@
 //   dx = s sum_n g B + D w       ds = x sum_n g B + sum_n A q,  q = g a h_{t-1}     dA = sum_t s q               dD = sum_t w x       dz = dy (sum_n C h + D x) silu'(z)
 //
 //   back_ends_kernel  with several segments: what each makes of a gradient of zeros at its end
-//   grad_kernel       sixteen tokens at a time, from the last on: the states again from the one that the forward kept in front of them (they stand in shared memory, eight tokens'
-//                     at a time), then the tokens backwards with g in registers.  Sums over channels leave a block as parts, so the result has one order whatever runs first
+//   grad_kernel       sixteen tokens at a time, from the last on: the states in front of every four of them, from the one that the forward kept; then four tokens forwards, with their
+//                     decays and decayed states kept in registers, and the same four backwards.  Sums over channels leave a block as parts, so the result has one order whatever
+//                     runs first
 //   grad_sum_kernel   adds up the parts
 //
 // All in fp32; inputs and gradients are bf16 or fp32 (template T; the steps' logits either).  Compiled without fast math.
@@ -27,105 +28,164 @@ namespace dewb {
 namespace selective {
 
 using Grad = dewb_selective_grad_args;
-constexpr int HALF = 8;                // tokens whose states stand in shared memory together
+constexpr int TT = Lay<4, 4>::TT;
+constexpr int FOUR = 4;                // tokens whose decays and states a lane has in registers
 
 template <int LN>
 struct Shared {
   using L = Lay<LN, 4>;
-  float step[WARPS][TT][L::CW], w[WARPS][TT][L::CW], c[TT][L::NP];               // s, w, C: what back_ends_kernel has
-  float in[WARPS][TT][L::CW], b[TT][L::NP];                                      // u, B
-  float sums[WARPS][HALF][3][L::CW];                                             // sum g B, sum A q, sum C h
-  float bc[WARPS][TT][2][L::NP];
-  float4 h[WARPS][HALF][4][32];                                                  // h_{t-1}: token, channel of the lane's four, lane
+  float step[WARPS][TT][L::CW], w[WARPS][TT][L::CW];      // s, w
+  float2 c[TT][L::NP];                                    // C, each number twice; up to here, what back_ends_kernel has
+  float in[WARPS][TT][L::CW];                             // u
+  float2 b[TT][L::NP];
+  float bc[WARPS][TT][2][L::NP];                          // dB and dC of the warp's channels
+  float4 h[WARPS][TT / FOUR][4][32];                      // a lane's states in front of every four tokens: channels 0 and 1 of two states in each of the first two pieces, 2 and 3 in the others
+  float4 shares[WARPS][FOUR][5][32];                      // a lane's shares of sum g B, sum A q, sum C h (four channels), of dB and dC (four states)
 };
 
-// Where a lane loads and stores: four channels of token lt + pass * LN.
-template <typename T, int LN>
+// Where a lane loads and stores: four channels of token lt + pass * LN; and what it has of a tile's tokens.
+template <typename T, typename TD, int LN, bool STATES>
 struct Place {
   using L = Lay<LN, 4>;
-  int lt, lc, left;
-  bool x_whole, dt_whole, z_whole, dy_whole, y_whole;
+  int lt, lq, lc, left;
+  bool whole;                          // ... all over the block, in pieces of four
   const T *x, *z, *dy;
-  long long dt_row;
-  __device__ __forceinline__ Place(const Grad& g, int row, int c0, int lane) {
+  const TD* dt;
+  Raw<T> rx[L::PASSES], rz[L::PASSES], ry[L::PASSES];
+  Raw<TD> rd[L::PASSES];
+  __device__ __forceinline__ Place(const Grad& g, int row, int c_block, int c0, int lane) {
     const Args& p = g.f;
     lt = lane / L::CG;
-    lc = c0 + lane % L::CG * 4;
+    lq = lane % L::CG * 4;
+    lc = c0 + lq;
     left = max(0, min(4, p.C - lc));
     x = static_cast<const T*>(p.x) + row * p.x_row + lc;
     z = p.z == nullptr ? nullptr : static_cast<const T*>(p.z) + row * p.z_row + lc;
     dy = static_cast<const T*>(g.dy) + row * g.dy_row + lc;
-    dt_row = row * p.dt_row + lc;
-    const bool even = left == 4;
-    x_whole = even && fours<T>(p.x, p.x_row, p.x_token);
-    z_whole = even && fours<T>(p.z, p.z_row, p.z_token);
-    dy_whole = even && fours<T>(g.dy, g.dy_row, g.dy_token);
-    dt_whole = even && (p.dt_fp32 ? fours<float>(p.dt, p.dt_row, p.dt_token) : fours<bf16>(p.dt, p.dt_row, p.dt_token));
-    y_whole = even && (p.C & 3) == 0;
+    dt = static_cast<const TD*>(p.dt) + row * p.dt_row + lc;
+    whole = c_block + L::CB <= p.C && (p.C & 3) == 0 && fours<T>(p.x, p.x_row, p.x_token) && fours<TD>(p.dt, p.dt_row, p.dt_token) && fours<T>(g.dy, g.dy_row, g.dy_token) &&
+            (z == nullptr || fours<T>(p.z, p.z_row, p.z_token));
+  }
+  // ahead of their turn, as far as L2
+  __device__ __forceinline__ void call(const Grad& g, int t0, int t_end) const {
+#pragma unroll
+    for (int i = 0; i < L::PASSES; ++i) {
+      const int t = t0 + lt + i * LN;
+      if (lt < TT && t < t_end && left > 0 && t >= 0) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(x + t * g.f.x_token));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(dt + t * g.f.dt_token));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(dy + t * g.dy_token));
+        if (z != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(z + t * g.f.z_token));
+      }
+    }
+  }
+  template <bool FAST>
+  __device__ __forceinline__ void bring(const Grad& g, int t0, int t_end) {
+#pragma unroll
+    for (int i = 0; i < L::PASSES; ++i) {
+      const int t = t0 + lt + i * LN, n = lt < TT && t < t_end ? left : 0;
+      if (!FAST || LN <= TT || lt < TT) {
+        if (STATES) rx[i] = fetch(x + t * g.f.x_token, FAST, n);
+        rd[i] = fetch(dt + t * g.f.dt_token, FAST, n);
+        ry[i] = fetch(dy + t * g.dy_token, FAST, n);
+        if (z != nullptr) rz[i] = fetch(z + t * g.f.z_token, FAST, n);
+      }
+    }
+  }
+  __device__ __forceinline__ void bring(const Grad& g, int t0, int t_end) {
+    if (whole && t0 + TT <= t_end) bring<true>(g, t0, t_end);
+    else bring<false>(g, t0, t_end);
   }
 };
 
-// Sixteen tokens from t0 on: s, u and w of the warp's channels, B and C of the block.
+// What a block has of a tile's B and C.
 template <typename T, int LN, bool STATES>
-__device__ __forceinline__ void stage(Shared<LN>& sm, const Grad& g, const Place<T, LN>& at, int row, int t0, int t_end, int warp, int lane, float (&total)[4]) {
+struct Narrow {
   using L = Lay<LN, 4>;
-  const Args& p = g.f;
+  static constexpr int EACH = (TT * L::NP + THREADS - 1) / THREADS;
+  uint32_t b[STATES ? EACH : 1], c[EACH];
+  __device__ __forceinline__ void bring(const Args& p, int row, int t0, int t_end) {
+    const T *pb = static_cast<const T*>(p.b) + row * p.b_row, *pc = static_cast<const T*>(p.c) + row * p.c_row;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int at = threadIdx.x + i * THREADS, t = t0 + at / L::NP, n = at % L::NP;
+      const bool on = t < t_end && n < p.N;
+      if (STATES) b[i] = on ? word(pb + t * p.b_token + n) : 0u;
+      c[i] = on ? word(pc + t * p.c_token + n) : 0u;
+    }
+  }
+  __device__ __forceinline__ void put(Shared<LN>& sm) const {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int at = threadIdx.x + i * THREADS;
+      const float cf = value<T>(c[i]), bf = STATES ? value<T>(b[i]) : 0.f;
+      if (STATES) sm.b[at / L::NP][at % L::NP] = make_float2(bf, bf);
+      sm.c[at / L::NP][at % L::NP] = make_float2(cf, cf);
+    }
+  }
+};
+
+// s, u and w of the warp's channels from what the lanes have brought; behind t_end and the last channel, zeros.
+template <typename T, typename TD, int LN, bool STATES>
+__device__ __forceinline__ void stage(Shared<LN>& sm, const Place<T, TD, LN, STATES>& at, bool steps, int t0, int t_end, int warp, float (&total)[4]) {
+  using L = Lay<LN, 4>;
+  const bool all = t0 + TT <= t_end && at.left == 4;
 #pragma unroll
   for (int i = 0; i < L::PASSES; ++i) {
     const int t = at.lt + i * LN;
-    const bool on = t < TT && t0 + t < t_end;
-    const int n = on ? at.left : 0;
-    const long long tok = t0 + t;
+    if (LN > TT && t >= TT) continue;
     float x[4], s[4], w[4], z[4];
-    if (STATES) fetch(at.x + tok * p.x_token, on && at.x_whole, n).get(x);
-    fetch_step(p.dt, at.dt_row + tok * p.dt_token, p.dt_fp32, on && at.dt_whole, n).get(s, p.dt_fp32);
-    fetch(at.dy + tok * g.dy_token, on && at.dy_whole, n).get(w);
-    if (at.z != nullptr) fetch(at.z + tok * p.z_token, on && at.z_whole, n).get(z);
+    if (STATES) at.rx[i].get(x);
+    at.rd[i].get(s);
+    at.ry[i].get(w);
+    if (at.z != nullptr) at.rz[i].get(z);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      s[j] = j < n ? (p.softplus ? softplus(s[j]) : s[j]) : 0.f;
+      if (steps) s[j] = softplus(s[j]);
       if (at.z != nullptr) w[j] *= z[j] * sigmoid(z[j]);
+      if (!all && (j >= at.left || t0 + t >= t_end)) s[j] = w[j] = 0.f;
+      if (STATES) x[j] = !all && (j >= at.left || t0 + t >= t_end) ? 0.f : s[j] * x[j];
       total[j] += s[j];
     }
-    if (t < TT) {
-      const int c = lane % L::CG * 4;
-      *reinterpret_cast<float4*>(&sm.step[warp][t][c]) = make_float4(s[0], s[1], s[2], s[3]);
-      *reinterpret_cast<float4*>(&sm.w[warp][t][c]) = make_float4(w[0], w[1], w[2], w[3]);
-      if (STATES) *reinterpret_cast<float4*>(&sm.in[warp][t][c]) = make_float4(s[0] * x[0], s[1] * x[1], s[2] * x[2], s[3] * x[3]);
+    *reinterpret_cast<float4*>(&sm.step[warp][t][at.lq]) = make_float4(s[0], s[1], s[2], s[3]);
+    *reinterpret_cast<float4*>(&sm.w[warp][t][at.lq]) = make_float4(w[0], w[1], w[2], w[3]);
+    if (STATES) *reinterpret_cast<float4*>(&sm.in[warp][t][at.lq]) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// Numbers of four channels (from c on) and four states (from n on), channels in pairs.
+struct Block {
+  f2 v[2][4];
+  template <typename F>
+  __device__ __forceinline__ static Block make(F f) {
+    Block r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r.v[i][k] = f2(f(2 * i, k), f(2 * i + 1, k));
+    return r;
+  }
+  __device__ __forceinline__ static Block load(const float* p, int stride) {
+    return make([&](int j, int k) { return p[j * stride + k]; });
+  }
+  __device__ __forceinline__ void store(float* p, int stride) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 e0 = v[i][0].get(), e1 = v[i][1].get(), e2 = v[i][2].get(), e3 = v[i][3].get();
+      *reinterpret_cast<float4*>(p + 2 * i * stride) = make_float4(e0.x, e1.x, e2.x, e3.x);
+      *reinterpret_cast<float4*>(p + (2 * i + 1) * stride) = make_float4(e0.y, e1.y, e2.y, e3.y);
     }
   }
-  const T *b = static_cast<const T*>(p.b) + row * p.b_row, *c = static_cast<const T*>(p.c) + row * p.c_row;
-  for (int i = threadIdx.x; i < TT * L::NP; i += THREADS) {
-    const int t = i / L::NP, n = i % L::NP;
-    const bool on = t0 + t < t_end && n < p.N;
-    if (STATES) sm.b[t][n] = on ? ld(b + (t0 + t) * p.b_token + n) : 0.f;
-    sm.c[t][n] = on ? ld(c + (t0 + t) * p.c_token + n) : 0.f;
-  }
-}
+};
 
-template <int LN>
-__device__ __forceinline__ void load_rates(const Args& p, int c, int n, float (&a)[4][4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) a[j][k] = rate<false>(p, c + j, n + k, 1);
-}
-
-__device__ __forceinline__ void load4x4(const float* p, int stride, float (&h)[4][4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float4 v = *reinterpret_cast<const float4*>(p + static_cast<long long>(j) * stride);
-    h[j][0] = v.x; h[j][1] = v.y; h[j][2] = v.z; h[j][3] = v.w;
-  }
-}
-__device__ __forceinline__ void store4x4(float* p, int stride, const float (&h)[4][4]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(p + static_cast<long long>(j) * stride) = make_float4(h[j][0], h[j][1], h[j][2], h[j][3]);
+__device__ __forceinline__ Block last_of(const Grad& g, int row, int c, int n, bool there) {
+  const Args& p = g.f;
+  return Block::make([&](int j, int k) { return there && g.dlast != nullptr && c + j < p.C && n + k < p.N ? g.dlast[(static_cast<long long>(row) * p.C + c + j) * p.N + n + k] : 0.f; });
 }
 
 // grid R * (segments - 1) * channel blocks, of segments 1, 2, ...: starts[r, j] is the gradient of the state in front of segment j that the segment itself makes (the last one: with dlast).
-template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, typename TD, int LN>
+__global__ void __launch_bounds__(THREADS, 4)
 back_ends_kernel(const Grad g) {
   using L = Lay<LN, 4>;
   __shared__ __align__(16) char raw[offsetof(Shared<LN>, in)];
@@ -135,65 +195,52 @@ back_ends_kernel(const Grad g) {
   const int blocks = (p.C + L::CB - 1) / L::CB, padded = blocks * L::CB;
   const int cb = blockIdx.x % blocks, seg = 1 + blockIdx.x / blocks % (p.segments - 1), row = blockIdx.x / blocks / (p.segments - 1);
   const int c0 = cb * L::CB + warp * L::CW, t_begin = seg * p.segment, t_end = min(p.T, t_begin + p.segment);
-  const Place<T, LN> at(g, row, c0, lane);
-  float a[4][4], d[4][4], total[4] = {0.f, 0.f, 0.f, 0.f};
-  load_rates<LN>(p, c0 + cg * 4, sl * 4, a);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = c0 + cg * 4 + j, n = sl * 4 + k;
-      d[j][k] = seg == p.segments - 1 && g.dlast != nullptr && c < p.C && n < p.N ? g.dlast[(static_cast<long long>(row) * p.C + c) * p.N + n] : 0.f;
+  Place<T, TD, LN, false> at(g, row, cb * L::CB, c0, lane);
+  Narrow<T, LN, false> narrow;
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
+  const Block a = Block::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * 4 + k, 1); });
+  Block d = last_of(g, row, c0 + cg * 4, sl * 4, seg == p.segments - 1);
+  int t0 = t_begin + (t_end - t_begin - 1) / TT * TT;
+  at.bring(g, t0, t_end);
+  narrow.bring(p, row, t0, t_end);
+  for (; t0 >= t_begin; t0 -= TT) {
+    __syncthreads();
+    stage<T, TD, LN, false>(sm, at, p.softplus, t0, t_end, warp, total);
+    narrow.put(sm);
+    __syncthreads();
+    if (t0 > t_begin) {
+      at.bring(g, t0 - TT, t_end);
+      narrow.bring(p, row, t0 - TT, t_end);
     }
-  for (int t0 = t_begin + (t_end - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
-    __syncthreads();
-    stage<T, LN, false>(sm, g, at, row, t0, t_end, warp, lane, total);
-    __syncthreads();
+    const int count = min(TT, t_end - t0);
 #pragma unroll 4
-    for (int t = min(TT, t_end - t0) - 1; t >= 0; --t) {
-      const float4 s4 = *reinterpret_cast<const float4*>(&sm.step[warp][t][cg * 4]), w4 = *reinterpret_cast<const float4*>(&sm.w[warp][t][cg * 4]);
-      const float4 c4 = *reinterpret_cast<const float4*>(&sm.c[t][sl * 4]);
-      const float s[4] = {s4.x, s4.y, s4.z, s4.w}, w[4] = {w4.x, w4.y, w4.z, w4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+    for (int t = (count + 3) / 4 * 4 - 1; t >= 0; --t) {
+      f2 s[2], w[2], c[4];
+      pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
+      pair(&sm.w[warp][t][cg * 4], w[0], w[1]);
+      pair(&sm.c[t][sl * 4].x, c[0], c[1]);
+      pair(&sm.c[t][sl * 4 + 2].x, c[2], c[3]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[j][k] = ex2(s[j] * a[j][k]) * fmaf(w[j], c[k], d[j][k]);
+        for (int k = 0; k < 4; ++k) d.v[i][k] = mul(ex2(mul(s[i], a.v[i][k])), fma(w[i], c[k], d.v[i][k]));
     }
   }
   const long long out = (static_cast<long long>(row) * p.segments + seg) * padded + c0;
-  store4x4(p.starts + (out + cg * 4) * L::NP + sl * 4, L::NP, d);
+  d.store(p.starts + (out + cg * 4) * L::NP + sl * 4, L::NP);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int o = L::CG; o < 32; o <<= 1) total[j] += __shfl_xor_sync(0xffffffffu, total[j], o);
-    if (at.lt == 0) p.sums[out + lane % L::CG * 4 + j] = total[j];
+    if (at.lt == 0) p.sums[out + at.lq + j] = total[j];
   }
 }
 
-// Eight numbers of a lane (dB and dC of its four states) summed over the 32 / LN groups of lanes: lane keeps COUNT = 8 / groups of them, from `base` on.
-template <int LN>
-__device__ __forceinline__ int over_channels(float (&v)[8], int lane) {
-  int base = 0;
-#pragma unroll
-  for (int o = LN, half = 4; o < 32; o <<= 1, half >>= 1) {
-    const bool upper = lane & o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i < half) {
-        const float give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
-    }
-    base += upper ? half : 0;
-  }
-  return base;
-}
-
-template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, typename TD, int LN>
+__global__ void __launch_bounds__(THREADS, 2)
 grad_kernel(const Grad g) {
   using L = Lay<LN, 4>;
-  constexpr int CG = L::CG, NP = L::NP, COUNT = 8 / CG;
+  constexpr int CG = L::CG, NP = L::NP;
   extern __shared__ __align__(16) char raw[];
   Shared<LN>& sm = *reinterpret_cast<Shared<LN>*>(raw);
   const Args& p = g.f;
@@ -201,26 +248,19 @@ grad_kernel(const Grad g) {
   const int blocks = (p.C + L::CB - 1) / L::CB, padded = blocks * L::CB;
   const int cb = blockIdx.x % blocks, seg = blockIdx.x / blocks % p.segments, row = blockIdx.x / blocks / p.segments;
   const int c0 = cb * L::CB + warp * L::CW, t_begin = seg * p.segment, t_end = min(p.T, t_begin + p.segment);
-  const Place<T, LN> at(g, row, c0, lane);
+  Place<T, TD, LN, true> at(g, row, cb * L::CB, c0, lane);
+  int t0 = t_begin + (t_end - t_begin - 1) / TT * TT;
   const long long pad_row = static_cast<long long>(row) * p.segments * padded + c0 + cg * 4;
-  float a[4][4], d[4][4], da[4][4];
-  load_rates<LN>(p, c0 + cg * 4, sl * 4, a);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = c0 + cg * 4 + j, n = sl * 4 + k;
-      da[j][k] = 0.f;
-      d[j][k] = seg == p.segments - 1 && g.dlast != nullptr && c < p.C && n < p.N ? g.dlast[(static_cast<long long>(row) * p.C + c) * p.N + n] : 0.f;
-    }
+  const Block a = Block::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * 4 + k, 1); });
+  Block d = last_of(g, row, c0 + cg * 4, sl * 4, seg == p.segments - 1), da = Block::make([](int, int) { return 0.f; });
   for (int q = p.segments - 1; q > seg; --q) {    // what comes from behind the segment
-    float e[4][4];
-    load4x4(p.starts + (pad_row + static_cast<long long>(q) * padded) * NP + sl * 4, NP, e);
+    const long long there = pad_row + static_cast<long long>(q) * padded;
+    const Block e = Block::load(p.starts + there * NP + sl * 4, NP);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float sum = q < p.segments - 1 ? p.sums[pad_row + static_cast<long long>(q) * padded + j] : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const f2 sum = q < p.segments - 1 ? f2(p.sums[there + 2 * i], p.sums[there + 2 * i + 1]) : f2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[j][k] = ex2(sum * a[j][k]) * d[j][k] + e[j][k];
+      for (int k = 0; k < 4; ++k) d.v[i][k] = fma(ex2(mul(sum, a.v[i][k])), d.v[i][k], e.v[i][k]);
     }
   }
   float skip[4], dd[4] = {0.f, 0.f, 0.f, 0.f}, unused[4] = {0.f, 0.f, 0.f, 0.f};
@@ -228,126 +268,174 @@ grad_kernel(const Grad g) {
   for (int j = 0; j < 4; ++j) skip[j] = p.d != nullptr && j < at.left ? p.d[at.lc + j] : 0.f;
   const int kept = (p.T + EVERY - 1) / EVERY;
   const long long here = static_cast<long long>(row) * p.T * p.C + at.lc;
-  for (int t0 = t_begin + (t_end - t_begin - 1) / TT * TT; t0 >= t_begin; t0 -= TT) {
-    stage<T, LN, true>(sm, g, at, row, t0, t_end, warp, lane, unused);
+  const bool y_whole = at.left == 4 && (p.C & 3) == 0;
+  auto piece = [&](const float4* q, f2& x, f2& y) { pair(&q->x, x, y); };
+  auto leave = [](float4* q, f2 x, f2 y) { *reinterpret_cast<ulonglong2*>(q) = make_ulonglong2(x.v, y.v); };
+  for (; t0 >= t_begin; t0 -= TT) {
+    Narrow<T, LN, true> narrow;
+    at.bring(g, t0, t_end);
+    narrow.bring(p, row, t0, t_end);
+    Block h = Block::load(p.checkpoints + ((static_cast<long long>(row) * kept + t0 / EVERY) * padded + c0 + cg * 4) * NP + sl * 4, NP);
+    if (t0 > t_begin) at.call(g, t0 - TT, t_end);
+    stage<T, TD, LN, true>(sm, at, p.softplus, t0, t_end, warp, unused);
+    narrow.put(sm);
     __syncthreads();
-    const float* before = p.checkpoints + ((static_cast<long long>(row) * kept + t0 / EVERY) * padded + c0 + cg * 4) * NP + sl * 4;
-    const int count = min(TT, t_end - t0);
-    for (int half = count > HALF ? 1 : 0; half >= 0; --half) {
-      const int from = half * HALF, n_here = min(HALF, count - from);
-      float h[4][4];
-      load4x4(before, NP, h);
-      auto forth = [&](int t) {
-        const float4 s4 = *reinterpret_cast<const float4*>(&sm.step[warp][t][cg * 4]), u4 = *reinterpret_cast<const float4*>(&sm.in[warp][t][cg * 4]);
-        const float4 b4 = *reinterpret_cast<const float4*>(&sm.b[t][sl * 4]);
-        const float s[4] = {s4.x, s4.y, s4.z, s4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) h[j][k] = fmaf(ex2(s[j] * a[j][k]), h[j][k], u[j] * b[k]);
-      };
-#pragma unroll 2
-      for (int t = 0; t < from; ++t) forth(t);
-#pragma unroll 2
-      for (int t = 0; t < n_here; ++t) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sm.h[warp][t][j][lane] = make_float4(h[j][0], h[j][1], h[j][2], h[j][3]);
-        if (t + 1 < n_here) forth(from + t);
-      }
+    const int count = min(TT, t_end - t0), groups = (count + FOUR - 1) / FOUR;
+    // (behind the last token steps, u and w are zero: decays of one, and nothing added to any sum)
 #pragma unroll 1
-      for (int i = n_here - 1; i >= 0; --i) {
-        const int t = from + i;
-        const float4 s4 = *reinterpret_cast<const float4*>(&sm.step[warp][t][cg * 4]), u4 = *reinterpret_cast<const float4*>(&sm.in[warp][t][cg * 4]);
-        const float4 w4 = *reinterpret_cast<const float4*>(&sm.w[warp][t][cg * 4]);
-        const float4 b4 = *reinterpret_cast<const float4*>(&sm.b[t][sl * 4]), c4 = *reinterpret_cast<const float4*>(&sm.c[t][sl * 4]);
-        const float s[4] = {s4.x, s4.y, s4.z, s4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, w[4] = {w4.x, w4.y, w4.z, w4.w};
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
-        float bc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, s1[4], s2[4], s3[4];
+    for (int q = 0; q < groups; ++q) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float4 v = sm.h[warp][i][j][lane];
-          const float hp[4] = {v.x, v.y, v.z, v.w};
-          s1[j] = s2[j] = s3[j] = 0.f;
+      for (int i = 0; i < 4; ++i) leave(&sm.h[warp][q][i][lane], h.v[i / 2][i % 2 * 2], h.v[i / 2][i % 2 * 2 + 1]);
+      if (q + 1 < groups) {
+#pragma unroll
+        for (int i = 0; i < FOUR; ++i) {
+          const int t = q * FOUR + i;
+          f2 s[2], u[2], b[4];
+          pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
+          pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
+          pair(&sm.b[t][sl * 4].x, b[0], b[1]);
+          pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h.v[j][k] = fma(ex2(mul(s[j], a.v[j][k])), h.v[j][k], mul(u[j], b[k]));
+        }
+      }
+    }
+#pragma unroll 1
+    for (int q = groups - 1; q >= 0; --q) {
+      const int from = q * FOUR, mine = from + at.lt;
+      const long long tok = t0 + mine;
+      const bool ends = at.lt < FOUR && mine < count;          // this lane forms gradients of four channels of a token
+      const int n = ends ? at.left : 0;
+      const bool fast = at.whole && ends;
+      const Raw<T> rx = fetch(at.x + tok * p.x_token, fast, n), ry = fetch(at.dy + tok * g.dy_token, fast, n);
+      const Raw<TD> rd = fetch(at.dt + tok * p.dt_token, fast, n);
+      Raw<T> rz;
+      if (at.z != nullptr) rz = fetch(at.z + tok * p.z_token, fast, n);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        piece(&sm.h[warp][q][2 * i][lane], h.v[i][0], h.v[i][1]);
+        piece(&sm.h[warp][q][2 * i + 1][lane], h.v[i][2], h.v[i][3]);
+      }
+      Block e[FOUR], ah[FOUR];
+#pragma unroll
+      for (int i = 0; i < FOUR; ++i) {
+        const int t = from + i;
+        f2 s[2], u[2], b[4];
+        pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
+        pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
+        pair(&sm.b[t][sl * 4].x, b[0], b[1]);
+        pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float e = ex2(s[j] * a[j][k]), ah = e * hp[k], now = fmaf(u[j], b[k], ah);
-            d[j][k] = fmaf(w[j], c[k], d[j][k]);
-            bc[k] = fmaf(u[j], d[j][k], bc[k]);
-            bc[4 + k] = fmaf(w[j], now, bc[4 + k]);
-            s1[j] = fmaf(d[j][k], b[k], s1[j]);
-            s3[j] = fmaf(now, c[k], s3[j]);
-            const float q = d[j][k] * ah;
-            s2[j] = fmaf(q, a[j][k], s2[j]);
-            da[j][k] = fmaf(q, s[j], da[j][k]);
-            d[j][k] *= e;
+            e[i].v[j][k] = ex2(mul(s[j], a.v[j][k]));
+            ah[i].v[j][k] = mul(e[i].v[j][k], h.v[j][k]);
+            if (i + 1 < FOUR) h.v[j][k] = fma(u[j], b[k], ah[i].v[j][k]);
           }
-        }
-        const int own = cg * 4 + own_channel(sl);
-        const float r1 = over_states<LN>(s1, sl), r2 = over_states<LN>(s2, sl), r3 = at.z != nullptr ? over_states<LN>(s3, sl) : 0.f;
-        if (sl < 4) {
-          sm.sums[warp][i][0][own] = r1;
-          sm.sums[warp][i][1][own] = r2;
-          sm.sums[warp][i][2][own] = r3;
-        }
-        const int base = over_channels<LN>(bc, lane);
+      }
 #pragma unroll
-        for (int q = 0; q < COUNT; ++q) sm.bc[warp][t][(base + q) / 4][sl * 4 + (base + q) % 4] = bc[q];
+      for (int i = FOUR - 1; i >= 0; --i) {
+        const int t = from + i;
+        f2 s[2], u[2], w[2], b[4], c[4], db[4], dc[4], s1[2], s2[2], s3[2];
+        pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
+        pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
+        pair(&sm.w[warp][t][cg * 4], w[0], w[1]);
+        pair(&sm.b[t][sl * 4].x, b[0], b[1]);
+        pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
+        pair(&sm.c[t][sl * 4].x, c[0], c[1]);
+        pair(&sm.c[t][sl * 4 + 2].x, c[2], c[3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const f2 now = fma(u[j], b[k], ah[i].v[j][k]), gt = fma(w[j], c[k], d.v[j][k]), through = mul(gt, ah[i].v[j][k]);
+            db[k] = j == 0 ? mul(u[j], gt) : fma(u[j], gt, db[k]);
+            dc[k] = j == 0 ? mul(w[j], now) : fma(w[j], now, dc[k]);
+            s1[j] = k == 0 ? mul(gt, b[k]) : fma(gt, b[k], s1[j]);
+            s2[j] = k == 0 ? mul(through, a.v[j][k]) : fma(through, a.v[j][k], s2[j]);
+            s3[j] = k == 0 ? mul(now, c[k]) : fma(now, c[k], s3[j]);
+            da.v[j][k] = fma(through, s[j], da.v[j][k]);
+            d.v[j][k] = mul(gt, e[i].v[j][k]);
+          }
+        float vb[4], vc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 x = db[k].get(), y = dc[k].get();
+          vb[k] = x.x + x.y;
+          vc[k] = y.x + y.y;
+        }
+        leave(&sm.shares[warp][i][0][lane], s1[0], s1[1]);
+        leave(&sm.shares[warp][i][1][lane], s2[0], s2[1]);
+        leave(&sm.shares[warp][i][2][lane], s3[0], s3[1]);
+        sm.shares[warp][i][3][lane] = make_float4(vb[0], vb[1], vb[2], vb[3]);
+        sm.shares[warp][i][4][lane] = make_float4(vc[0], vc[1], vc[2], vc[3]);
       }
       __syncwarp();
+      // dB and dC of the warp's channels: a lane takes four states of a token
 #pragma unroll
-      for (int pass = 0; pass < (HALF + LN - 1) / LN; ++pass) {
-        const int i = at.lt + pass * LN, t = from + i;
-        if (i >= n_here) continue;
-        const long long tok = t0 + t;
-        float x[4], raw_step[4], dx[4], ds[4], dy[4], z[4];
-        fetch(at.x + tok * p.x_token, at.x_whole, at.left).get(x);
-        if (p.softplus) fetch_step(p.dt, at.dt_row + tok * p.dt_token, p.dt_fp32, at.dt_whole, at.left).get(raw_step, p.dt_fp32);
-        const int c = lane % CG * 4;
+      for (int o = lane; o < FOUR * 2 * LN; o += 32) {
+        const int state = o % LN, which = o / LN % 2, i = o / LN / 2;
+        *reinterpret_cast<float4*>(&sm.bc[warp][from + i][which][state * 4]) = sum4(&sm.shares[warp][i][3 + which][state], CG, LN, which);
+      }
+      if (ends) {
+        const int turn = LN == 4 ? lane % CG >> 1 : 0, first = lane % CG * LN;
+        const float4 v1 = sum4(&sm.shares[warp][at.lt][0][first], LN, 1, turn), v2 = sum4(&sm.shares[warp][at.lt][1][first], LN, 1, turn);
+        const float4 s4 = *reinterpret_cast<const float4*>(&sm.step[warp][mine][at.lq]), w4 = *reinterpret_cast<const float4*>(&sm.w[warp][mine][at.lq]);
+        const float r1[4] = {v1.x, v1.y, v1.z, v1.w}, r2[4] = {v2.x, v2.y, v2.z, v2.w}, s[4] = {s4.x, s4.y, s4.z, s4.w}, w[4] = {w4.x, w4.y, w4.z, w4.w};
+        float x[4], raw_step[4], dx[4], ds[4];
+        rx.get(x);
+        rd.get(raw_step);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float r1 = sm.sums[warp][i][0][c + j], w = sm.w[warp][t][c + j];
-          dx[j] = fmaf(sm.step[warp][t][c + j], r1, skip[j] * w);
-          ds[j] = fmaf(x[j], r1, LN2 * sm.sums[warp][i][1][c + j]);
+          dx[j] = fmaf(s[j], r1[j], skip[j] * w[j]);
+          ds[j] = fmaf(x[j], r1[j], LN2 * r2[j]);
           if (p.softplus) ds[j] *= sigmoid(raw_step[j]);
-          dd[j] = fmaf(w, x[j], dd[j]);
+          dd[j] = fmaf(w[j], x[j], dd[j]);
         }
-        put(static_cast<T*>(g.dx) + here + tok * p.C, dx, at.y_whole, at.left);
-        if (p.dt_fp32) put(static_cast<float*>(g.ddt) + here + tok * p.C, ds, at.y_whole, at.left);
-        else put(static_cast<bf16*>(g.ddt) + here + tok * p.C, ds, at.y_whole, at.left);
+        put(static_cast<T*>(g.dx) + here + tok * p.C, dx, y_whole, at.left);
+        put(static_cast<TD*>(g.ddt) + here + tok * p.C, ds, y_whole, at.left);
         if (at.z != nullptr) {
-          fetch(at.dy + tok * g.dy_token, at.dy_whole, at.left).get(dy);
-          fetch(at.z + tok * p.z_token, at.z_whole, at.left).get(z);
+          const float4 v3 = sum4(&sm.shares[warp][at.lt][2][first], LN, 1, turn);
+          const float r3[4] = {v3.x, v3.y, v3.z, v3.w};
+          float dy[4], z[4];
+          ry.get(dy);
+          rz.get(z);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float sig = sigmoid(z[j]);
-            z[j] = dy[j] * fmaf(skip[j], x[j], sm.sums[warp][i][2][c + j]) * sig * fmaf(z[j], 1.f - sig, 1.f);
+            z[j] = dy[j] * fmaf(skip[j], x[j], r3[j]) * sig * fmaf(z[j], 1.f - sig, 1.f);
           }
-          put(static_cast<T*>(g.dz) + here + tok * p.C, z, at.y_whole, at.left);
+          put(static_cast<T*>(g.dz) + here + tok * p.C, z, y_whole, at.left);
         }
       }
-      __syncwarp();                               // (the sums and states have been read)
+      __syncwarp();                               // (the shares have been read)
     }
     __syncthreads();
-    for (int i = tid; i < count * 2 * NP; i += THREADS) {
-      const int t = i / (2 * NP), q = i % (2 * NP);
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < WARPS; ++k) v += sm.bc[k][t][q / NP][q % NP];
-      g.bc_parts[((static_cast<long long>(cb) * p.R + row) * p.T + t0 + t) * (2 * NP) + q] = v;
-    }
+    for (int o = tid; o < count * 2 * LN; o += THREADS)
+      *reinterpret_cast<float4*>(g.bc_parts + ((static_cast<long long>(cb) * p.R + row) * p.T + t0) * (2 * NP) + o * 4) =
+          sum4(reinterpret_cast<const float4*>(&sm.bc[0][0][0][0]) + o, WARPS, TT * 2 * LN, 0);
   }
   const long long part = (static_cast<long long>(row) * p.segments + seg) * padded + c0;
-  store4x4(g.a_parts + (part + cg * 4) * NP + sl * 4, NP, da);
+  da.store(g.a_parts + (part + cg * 4) * NP + sl * 4, NP);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
     for (int o = CG; o < 32; o <<= 1) dd[j] += __shfl_xor_sync(0xffffffffu, dd[j], o);
-    if (at.lt == 0) g.d_parts[part + lane % CG * 4 + j] = dd[j];
+    if (at.lt == 0) g.d_parts[part + at.lq + j] = dd[j];
+  }
+  if (seg == 0 && g.dinitial != nullptr) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = c0 + cg * 4 + j, n = sl * 4 + k;
-      if (seg == 0 && g.dinitial != nullptr && c < p.C && n < p.N) g.dinitial[(static_cast<long long>(row) * p.C + c) * p.N + n] = d[j][k];
-    }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + cg * 4 + 2 * i, n = sl * 4 + k;
+        const float2 v = d.v[i][k].get();
+        if (c < p.C && n < p.N) g.dinitial[(static_cast<long long>(row) * p.C + c) * p.N + n] = v.x;
+        if (c + 1 < p.C && n < p.N) g.dinitial[(static_cast<long long>(row) * p.C + c + 1) * p.N + n] = v.y;
+      }
   }
 }
 
@@ -385,7 +473,7 @@ grad_sum_kernel(const Grad g, int blocks, int padded, int np) {
   }
 }
 
-template <typename T, int LN>
+template <typename T, typename TD, int LN>
 int grad_go(const Grad& g, cudaStream_t stream) {
   using L = Lay<LN, 4>;
   const Args& p = g.f;
@@ -393,20 +481,20 @@ int grad_go(const Grad& g, cudaStream_t stream) {
   const long long sums = (static_cast<long long>(p.R) * p.T * 2 * p.N + static_cast<long long>(p.C) * (p.N + 1) + 255) / 256;
   if (blocks * p.segments * p.R > 0x7fffffffLL || sums > 0x7fffffffLL) return -3;
   constexpr int smem = static_cast<int>(sizeof(Shared<LN>));
-  cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, TD, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return static_cast<int>(e);
-  if (p.segments > 1) back_ends_kernel<T, LN><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, 0, stream>>>(g);
-  grad_kernel<T, LN><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, smem, stream>>>(g);
+  if (p.segments > 1) back_ends_kernel<T, TD, LN><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, 0, stream>>>(g);
+  grad_kernel<T, TD, LN><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, smem, stream>>>(g);
   grad_sum_kernel<T><<<static_cast<unsigned>(sums), 256, 0, stream>>>(g, static_cast<int>(blocks), static_cast<int>(blocks) * L::CB, L::NP);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T>
+template <typename T, typename TD>
 int grad_any(const Grad& g, cudaStream_t stream) {
-  if (g.f.N <= 16) return grad_go<T, 4>(g, stream);
-  if (g.f.N <= 32) return grad_go<T, 8>(g, stream);
-  if (g.f.N <= 64) return grad_go<T, 16>(g, stream);
-  if (g.f.N <= 128) return grad_go<T, 32>(g, stream);
+  if (g.f.N <= 16) return grad_go<T, TD, 4>(g, stream);
+  if (g.f.N <= 32) return grad_go<T, TD, 8>(g, stream);
+  if (g.f.N <= 64) return grad_go<T, TD, 16>(g, stream);
+  if (g.f.N <= 128) return grad_go<T, TD, 32>(g, stream);
   return -3;
 }
 
@@ -427,5 +515,6 @@ extern "C" int dewb_selective_grad(const dewb_selective_grad_args* a, int fp32, 
     return -3;
   if ((p.z != nullptr) != (a->dz != nullptr)) return -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  return fp32 ? grad_any<float>(*a, stream) : grad_any<bf16>(*a, stream);
+  if (fp32) return p.dt_fp32 ? grad_any<float, float>(*a, stream) : -3;
+  return p.dt_fp32 ? grad_any<bf16, float>(*a, stream) : grad_any<bf16, bf16>(*a, stream);
 }

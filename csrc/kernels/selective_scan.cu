@@ -12,16 +12,26 @@
 namespace dewb {
 namespace selective {
 
+template <int LN, int NS, bool ENDS>
+struct Tile {
+  using L = Lay<LN, NS>;
+  float step[WARPS][L::TT][L::CW], in[WARPS][L::TT][L::CW];                  // s (heads: the decay), s x
+  float2 b[L::TT][L::NP], c[ENDS ? 1 : L::TT][L::NP];                        // each number twice: beside two channels
+  float4 out[ENDS ? 1 : WARPS][ENDS ? 1 : L::TT][32];                        // a lane's share of sum C h, four channels
+};
+
 // grid R * segments * channel blocks.  With heads, a channel block lies within one group (that shares B and C).
 //   starts[r, 0]       the state that row r begins with          starts[r, j]   what segment j - 1 ends with: from there on for j = 1, from zeros for the others
 //   sums[r, j]         the sum of segment j's steps, per channel
-template <typename T, int LN, int NS, bool HEADS, bool ENDS>
-__global__ void __launch_bounds__(THREADS)
+// A tile's x and steps come a tile ahead, in registers; what the end of a tile needs (x again, z) is asked for at its beginning (L2) and read then.  The sums over states are formed at
+// the end of a tile from what every lane leaves in shared memory: with shuffles after every token (or two, or four) a warp alone took 620 cycles a token, so: DEWB_ALONE.
+template <typename T, typename TD, int LN, int NS, bool HEADS, bool ENDS>
+__global__ void __launch_bounds__(THREADS, NS > 4 ? 2 : 4)
 scan_kernel(const Args p) {
   using L = Lay<LN, NS>;
-  constexpr int CG = L::CG, CW = L::CW, CB = L::CB, NP = L::NP;
-  __shared__ __align__(16) float s_step[WARPS][TT][CW], s_in[WARPS][TT][CW], s_out[ENDS ? 1 : WARPS][TT][CW];      // s (heads: the decay), s x, the sums over the states
-  __shared__ __align__(16) float s_b[TT][NP], s_c[ENDS ? 1 : TT][NP];
+  constexpr int CG = L::CG, CW = L::CW, CB = L::CB, NP = L::NP, TT = L::TT, PASSES = L::PASSES, BC = (TT * NP + THREADS - 1) / THREADS;
+  extern __shared__ __align__(16) char raw[];
+  Tile<LN, NS, ENDS>& sm = *reinterpret_cast<Tile<LN, NS, ENDS>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sl = lane % LN, cg = lane / LN;
   const int per = p.C / p.groups, blocks = (per + CB - 1) / CB * p.groups, padded = blocks * CB;
   const int segments = ENDS ? p.segments - 1 : p.segments;
@@ -32,7 +42,7 @@ scan_kernel(const Args p) {
   const Row r = row_of(p, row);
   const int t_begin = seg * p.segment, t_end = min(r.len, t_begin + p.segment), t_stop = min(p.T, t_begin + p.segment);
   // where this lane loads and stores: four channels of token lane / CG + pass * LN
-  const int lt = lane / CG, lc = c0 + lane % CG * 4, left = max(0, min(4, c_end - lc));
+  const int lt = lane / CG, lq = lane % CG * 4, lc = c0 + lq, left = max(0, min(4, c_end - lc));
   T* y = static_cast<T*>(p.y) + static_cast<long long>(row) * p.T * p.C + lc;
   const bool y_whole = left == 4 && ((c_block | p.C) & 3) == 0;
   const int last_seg = r.len > 0 ? (r.len - 1) / p.segment : -1;
@@ -42,38 +52,40 @@ scan_kernel(const Args p) {
   }
   if (seg > last_seg) return;
 
-  float a[4][NS], h[4][NS];
+  f2 a[2][NS], h[2][NS];                          // of channels 2 i and 2 i + 1
   const long long pad_row = (static_cast<long long>(row) * p.segments) * padded + static_cast<long long>(cb) * CB + warp * CW + cg * 4;      // of segment 0, this lane's first channel
+  auto held = [&](int c, int n) { return (ENDS || p.segments == 1) && seg == 0 && r.held && c < c_end && n < p.N ? p.initial[(r.at * p.C + c) * p.N + n] : 0.f; };
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = c0 + cg * 4 + j;
+  for (int i = 0; i < 2; ++i) {
+    const int c = c0 + cg * 4 + 2 * i;
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
       const int n = sl * NS + k;
-      a[j][k] = rate<HEADS>(p, c < c_end ? c : p.C, n, dim);
-      h[j][k] = (ENDS || p.segments == 1) && seg == 0 && r.held && c < c_end && n < p.N ? p.initial[(r.at * p.C + c) * p.N + n] : 0.f;
+      a[i][k] = HEADS && ENDS ? f2(0.f, 0.f) : f2(rate<HEADS>(p, c < c_end ? c : p.C, n, dim), rate<HEADS>(p, c + 1 < c_end ? c + 1 : p.C, n, dim));
+      h[i][k] = f2(held(c, n), held(c + 1, n));
     }
   }
-  if (ENDS && seg == 0) {
+  // the states of this lane's channels at `to`, rows of NP
+  auto keep = [&](float* to) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int k = 0; k < NS; k += 4)
-        *reinterpret_cast<float4*>(p.starts + (pad_row + j) * NP + sl * NS + k) = make_float4(h[j][k], h[j][k + 1], h[j][k + 2], h[j][k + 3]);
-  }
+      for (int k = 0; k < NS; k += 4) {
+        const float2 e0 = h[i][k].get(), e1 = h[i][k + 1].get(), e2 = h[i][k + 2].get(), e3 = h[i][k + 3].get();
+        *reinterpret_cast<float4*>(to + 2 * i * NP + k) = make_float4(e0.x, e1.x, e2.x, e3.x);
+        *reinterpret_cast<float4*>(to + (2 * i + 1) * NP + k) = make_float4(e0.y, e1.y, e2.y, e3.y);
+      }
+  };
+  if (ENDS && seg == 0) keep(p.starts + pad_row * NP + sl * NS);
   if (!ENDS && p.segments > 1) {                  // what stands in front of the segment
     for (int q = min(seg, 1); q <= seg; ++q) {
+      const long long at = pad_row + static_cast<long long>(q) * padded;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const long long at = pad_row + static_cast<long long>(q) * padded + j;
-        const float sum = q > 1 ? p.sums[at - padded] : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const f2 sum = q > 1 ? f2(p.sums[at - padded + 2 * i], p.sums[at - padded + 2 * i + 1]) : f2(0.f, 0.f);
+        const float* e = p.starts + (at + 2 * i) * NP + sl * NS;
 #pragma unroll
-        for (int k = 0; k < NS; k += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.starts + at * NP + sl * NS + k);
-          const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) h[j][k + i] = ex2(sum * a[j][k + i]) * h[j][k + i] + e[i];
-        }
+        for (int k = 0; k < NS; ++k) h[i][k] = fma(ex2(mul(sum, a[i][k])), h[i][k], f2(e[k], e[NP + k]));
       }
     }
   }
@@ -90,151 +102,173 @@ scan_kernel(const Args p) {
     skip[j] = p.d != nullptr && !ENDS ? p.d[HEADS ? head[j] : c] : 0.f;
   }
   const T* x = static_cast<const T*>(p.x) + row * p.x_row + lc;
+  const TD* dt = static_cast<const TD*>(p.dt) + row * p.dt_row + (HEADS ? 0 : lc);
   const T* z = p.z == nullptr || ENDS ? nullptr : static_cast<const T*>(p.z) + row * p.z_row + lc;
   const T* b = static_cast<const T*>(p.b) + row * p.b_row + group * p.N;
   const T* cc = static_cast<const T*>(p.c) + row * p.c_row + group * p.N;
-  const bool even = left == 4 && (c_block & 3) == 0;
-  const bool x_whole = even && fours<T>(p.x, p.x_row, p.x_token), z_whole = even && fours<T>(p.z, p.z_row, p.z_token);
-  const bool dt_whole = even && (p.dt_fp32 ? fours<float>(p.dt, p.dt_row, p.dt_token) : fours<bf16>(p.dt, p.dt_row, p.dt_token));
+  // whole pieces of four wherever the block loads and stores
+  const bool whole = c_block + CB <= c_end && ((c_block | p.C) & 3) == 0 && fours<T>(p.x, p.x_row, p.x_token) && (z == nullptr || fours<T>(p.z, p.z_row, p.z_token)) &&
+                     (HEADS || fours<TD>(p.dt, p.dt_row, p.dt_token));
 
-  Raw<T> rx[L::PASSES], rz[L::PASSES];
-  RawStep rd[L::PASSES];
-  float rb[(TT * NP + THREADS - 1) / THREADS], rc[ENDS ? 1 : (TT * NP + THREADS - 1) / THREADS];
-  auto bring = [&](int t0) {
+  Raw<T> rx[PASSES];
+  Raw<TD> rd[PASSES];
+  uint32_t rh[HEADS ? PASSES : 1][4], rb[BC], rc[ENDS ? 1 : BC];
+  auto bring = [&](int t0, auto fast) {
+    constexpr bool FAST = decltype(fast)::value;
 #pragma unroll
-    for (int i = 0; i < L::PASSES; ++i) {
+    for (int i = 0; i < PASSES; ++i) {
       const int t = t0 + lt + i * LN;
-      const bool on = lt < TT && t < t_end;
+      const bool on = FAST ? LN <= TT || lt < TT : lt < TT && t < t_end;
       const int n = on ? left : 0;
-      rx[i] = fetch(x + t * p.x_token, on && x_whole, n);
+      if (FAST) { if (on) rx[i] = fetch(x + t * p.x_token, true, 4); }
+      else rx[i] = fetch(x + t * p.x_token, false, n);
       if (HEADS) {
-        const long long at = row * p.dt_row + t * p.dt_token;
-        float f[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = j < n ? (p.dt_fp32 ? static_cast<const float*>(p.dt)[at + head[j]] : ld(static_cast<const bf16*>(p.dt) + at + head[j])) : 0.f;
-        rd[i].v = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        for (int j = 0; j < 4; ++j) rh[i][j] = j < n ? word(dt + t * p.dt_token + head[j]) : 0u;
       } else {
-        rd[i] = fetch_step(p.dt, row * p.dt_row + t * p.dt_token + lc, p.dt_fp32, on && dt_whole, n);
+        if (FAST) { if (on) rd[i] = fetch(dt + t * p.dt_token, true, 4); }
+        else rd[i] = fetch(dt + t * p.dt_token, false, n);
       }
-      if (z != nullptr) rz[i] = fetch(z + t * p.z_token, on && z_whole, n);
+      if (z != nullptr && n > 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(z + t * p.z_token));
     }
 #pragma unroll
-    for (int i = 0; i < (TT * NP + THREADS - 1) / THREADS; ++i) {
+    for (int i = 0; i < BC; ++i) {
       const int at = tid + i * THREADS, t = t0 + at / NP, n = at % NP;
       const bool on = at < TT * NP && t < t_end && n < p.N;
-      rb[i] = on ? ld(b + t * p.b_token + n) : 0.f;
-      if (!ENDS) rc[i] = on ? ld(cc + t * p.c_token + n) : 0.f;
+      rb[i] = on ? word(b + t * p.b_token + n) : 0u;
+      if (!ENDS) rc[i] = on ? word(cc + t * p.c_token + n) : 0u;
     }
   };
-  bring(t_begin);
+  auto next = [&](int t0) {
+    if (whole && t0 + TT <= t_end) bring(t0, Yes());
+    else bring(t0, No());
+  };
+  next(t_begin);
   for (int t0 = t_begin; t0 < t_end; t0 += TT) {
-    float xs[L::PASSES][4];
-    Raw<T> gate[L::PASSES];
     __syncthreads();                              // (the tile before has been read)
+    auto stage = [&](auto fast) {
+      constexpr bool FAST = decltype(fast)::value;
 #pragma unroll
-    for (int i = 0; i < L::PASSES; ++i) {
-      const int t = lt + i * LN;
-      float s[4], u[4];
-      rx[i].get(xs[i]);
-      rd[i].get(s, HEADS || p.dt_fp32);
-      if (z != nullptr) gate[i] = rz[i];
-      const bool on = t < TT && t0 + t < t_end;
+      for (int i = 0; i < PASSES; ++i) {
+        const int t = lt + i * LN;
+        float xs[4], s[4];
+        rx[i].get(xs);
+        if (HEADS) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] = on && j < left ? (p.softplus ? softplus(s[j] + bias[j]) : s[j] + bias[j]) : 0.f;
-        u[j] = s[j] * xs[i][j];
-        if (ENDS) total[j] += s[j];
-        if (HEADS) s[j] = ex2(s[j] * rate_of[j]);
+          for (int j = 0; j < 4; ++j) s[j] = value<TD>(rh[i][j]);
+        } else {
+          rd[i].get(s);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[j] = p.softplus ? softplus(s[j] + bias[j]) : s[j] + bias[j];
+          if (!FAST && (j >= left || t0 + t >= t_end)) s[j] = xs[j] = 0.f;
+          if (ENDS && (LN <= TT || t < TT)) total[j] += s[j];
+          xs[j] *= s[j];
+          if (HEADS) s[j] = ex2(s[j] * rate_of[j]);
+        }
+        if (LN <= TT || t < TT) {
+          *reinterpret_cast<float4*>(&sm.step[warp][t][lq]) = make_float4(s[0], s[1], s[2], s[3]);
+          *reinterpret_cast<float4*>(&sm.in[warp][t][lq]) = make_float4(xs[0], xs[1], xs[2], xs[3]);
+        }
       }
-      if (t < TT) {
-        *reinterpret_cast<float4*>(&s_step[warp][t][lane % CG * 4]) = make_float4(s[0], s[1], s[2], s[3]);
-        *reinterpret_cast<float4*>(&s_in[warp][t][lane % CG * 4]) = make_float4(u[0], u[1], u[2], u[3]);
-      }
-    }
+    };
+    if (t0 + TT <= t_end && c_block + CB <= c_end) stage(Yes());
+    else stage(No());
 #pragma unroll
-    for (int i = 0; i < (TT * NP + THREADS - 1) / THREADS; ++i) {
+    for (int i = 0; i < BC; ++i) {
       const int at = tid + i * THREADS;
-      if (at < TT * NP) {
-        s_b[at / NP][at % NP] = rb[i];
-        if (!ENDS) s_c[at / NP][at % NP] = rc[i];
+      if (TT * NP % THREADS == 0 || at < TT * NP) {
+        const float bf = value<T>(rb[i]);
+        sm.b[at / NP][at % NP] = make_float2(bf, bf);
+        if (!ENDS) {
+          const float cf = value<T>(rc[i]);
+          sm.c[at / NP][at % NP] = make_float2(cf, cf);
+        }
       }
     }
     __syncthreads();
-    if (t0 + TT < t_end) bring(t0 + TT);
+    if (t0 + TT < t_end) next(t0 + TT);
     if (!ENDS && p.checkpoints != nullptr) {
-      static_assert(EVERY == TT, "a kept state a tile");
-      float* keep = p.checkpoints + ((static_cast<long long>(row) * ((p.T + EVERY - 1) / EVERY) + t0 / EVERY) * padded + static_cast<long long>(cb) * CB + warp * CW + cg * 4) * NP + sl * NS;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < NS; k += 4) *reinterpret_cast<float4*>(keep + j * NP + k) = make_float4(h[j][k], h[j][k + 1], h[j][k + 2], h[j][k + 3]);
+      static_assert(EVERY == TT || NS > 4, "a kept state a tile");
+      keep(p.checkpoints + ((static_cast<long long>(row) * ((p.T + EVERY - 1) / EVERY) + t0 / EVERY) * padded + static_cast<long long>(cb) * CB + warp * CW + cg * 4) * NP + sl * NS);
     }
-    const int count = min(TT, t_end - t0);
-#pragma unroll 4
-    for (int t = 0; t < count; ++t) {
-      const float4 s4 = *reinterpret_cast<const float4*>(&s_step[warp][t][cg * 4]), u4 = *reinterpret_cast<const float4*>(&s_in[warp][t][cg * 4]);
-      const float s[4] = {s4.x, s4.y, s4.z, s4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-      float bb[NS], cv[NS], out[4] = {0.f, 0.f, 0.f, 0.f};
+    const int count = min(TT, t_end - t0);        // (four at a time; behind the last one steps and inputs are zero and change nothing)
+#pragma unroll 1
+    for (int f = 0; f < count; f += 4) {
 #pragma unroll
-      for (int k = 0; k < NS; k += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(&s_b[t][sl * NS + k]);
-        bb[k] = v.x; bb[k + 1] = v.y; bb[k + 2] = v.z; bb[k + 3] = v.w;
-        if (!ENDS) {
-          const float4 w = *reinterpret_cast<const float4*>(&s_c[t][sl * NS + k]);
-          cv[k] = w.x; cv[k + 1] = w.y; cv[k + 2] = w.z; cv[k + 3] = w.w;
+      for (int i = 0; i < 4; ++i) {
+        const int t = f + i;
+        f2 step[2], in[2], bb[NS], cv[NS], out[2];
+        pair(&sm.step[warp][t][cg * 4], step[0], step[1]);
+        pair(&sm.in[warp][t][cg * 4], in[0], in[1]);
+#pragma unroll
+        for (int k = 0; k < NS; k += 2) {
+          pair(&sm.b[t][sl * NS + k].x, bb[k], bb[k + 1]);
+          if (!ENDS) pair(&sm.c[t][sl * NS + k].x, cv[k], cv[k + 1]);
         }
-      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int k = 0; k < NS; ++k) {
-          h[j][k] = fmaf(HEADS ? s[j] : ex2(s[j] * a[j][k]), h[j][k], u[j] * bb[k]);
-          if (!ENDS) out[j] = fmaf(h[j][k], cv[k], out[j]);
-        }
-      if (!ENDS) {
-        const float sum = over_states<LN>(out, sl);
-        if (sl < 4) s_out[warp][t][cg * 4 + own_channel(sl)] = sum;
+          for (int k = 0; k < NS; ++k) {
+            h[j][k] = fma(HEADS ? step[j] : ex2(mul(step[j], a[j][k])), h[j][k], mul(in[j], bb[k]));
+            if (!ENDS) out[j] = k == 0 ? mul(h[j][k], cv[k]) : fma(h[j][k], cv[k], out[j]);
+          }
+        if (!ENDS) *reinterpret_cast<ulonglong2*>(&sm.out[warp][t][lane]) = make_ulonglong2(out[0].v, out[1].v);
       }
     }
     if (!ENDS) {
       __syncwarp();
+      auto finish = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+        Raw<T> ex[PASSES], ez[PASSES];
 #pragma unroll
-      for (int i = 0; i < L::PASSES; ++i) {
-        const int t = lt + i * LN;
-        if (t >= TT || t0 + t >= t_end) continue;
-        const float4 o4 = *reinterpret_cast<const float4*>(&s_out[warp][t][lane % CG * 4]);
-        float o[4] = {o4.x, o4.y, o4.z, o4.w}, g[4];
-        if (z != nullptr) gate[i].get(g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j] += skip[j] * xs[i][j];
-          if (z != nullptr) o[j] *= g[j] * sigmoid(g[j]);
+        for (int i = 0; i < PASSES; ++i) {
+          const int t = t0 + lt + i * LN;
+          const int n = lt < TT && t < t_end ? left : 0;
+          ex[i] = fetch(x + t * p.x_token, FAST && n > 0, n);
+          if (z != nullptr) ez[i] = fetch(z + t * p.z_token, FAST && n > 0, n);
         }
-        put(y + static_cast<long long>(t0 + t) * p.C, o, y_whole, left);
-      }
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int t = lt + i * LN;
+          if (t >= TT || t0 + t >= t_end) continue;
+          const float4 o4 = sum4(&sm.out[warp][t][lane % CG * LN], LN, 1, LN == 4 ? lane % CG >> 1 : 0);
+          float o[4] = {o4.x, o4.y, o4.z, o4.w}, xs[4], g[4];
+          ex[i].get(xs);
+          if (z != nullptr) ez[i].get(g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[j] = fmaf(skip[j], xs[j], o[j]);
+            if (z != nullptr) o[j] *= g[j] * sigmoid(g[j]);
+          }
+          put(y + static_cast<long long>(t0 + t) * p.C, o, FAST || y_whole, left);
+        }
+      };
+      if (whole) finish(Yes());
+      else finish(No());
       __syncwarp();                               // (read before the next tile writes them)
     }
   }
   if (ENDS) {
-    const long long at = pad_row + static_cast<long long>(seg + 1) * padded;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int k = 0; k < NS; k += 4)
-        *reinterpret_cast<float4*>(p.starts + (at + j) * NP + sl * NS + k) = make_float4(h[j][k], h[j][k + 1], h[j][k + 2], h[j][k + 3]);
+    keep(p.starts + (pad_row + static_cast<long long>(seg + 1) * padded) * NP + sl * NS);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {                 // over the tokens' lanes
 #pragma unroll
       for (int o = CG; o < 32; o <<= 1) total[j] += __shfl_xor_sync(0xffffffffu, total[j], o);
-      if (lt == 0) p.sums[(static_cast<long long>(row) * p.segments + seg) * padded + static_cast<long long>(cb) * CB + warp * CW + lane % CG * 4 + j] = total[j];
+      if (lt == 0) p.sums[(static_cast<long long>(row) * p.segments + seg) * padded + static_cast<long long>(cb) * CB + warp * CW + lq + j] = total[j];
     }
   } else if (p.last != nullptr && seg == last_seg) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = c0 + cg * 4 + j;
+    for (int i = 0; i < 2; ++i) {
+      const int c = c0 + cg * 4 + 2 * i;
 #pragma unroll
-      for (int k = 0; k < NS; ++k)
-        if (c < c_end && sl * NS + k < p.N) p.last[(r.at * p.C + c) * p.N + sl * NS + k] = h[j][k];
+      for (int k = 0; k < NS; ++k) {
+        const int n = sl * NS + k;
+        const float2 v = h[i][k].get();
+        if (c < c_end && n < p.N) p.last[(r.at * p.C + c) * p.N + n] = v.x;
+        if (c + 1 < c_end && n < p.N) p.last[(r.at * p.C + c + 1) * p.N + n] = v.y;
+      }
     }
   }
 }
@@ -374,30 +408,34 @@ head_token_kernel(const Args p) {
   }
 }
 
-template <typename T, int LN, int NS, bool HEADS>
+template <typename T, typename TD, int LN, int NS, bool HEADS>
 int scan_go(const Args& p, cudaStream_t stream) {
   using L = Lay<LN, NS>;
   const long long blocks = static_cast<long long>((p.C / p.groups + L::CB - 1) / L::CB) * p.groups;
   if (blocks * p.segments * p.R > 0x7fffffffLL) return -3;
-  if (p.segments > 1) scan_kernel<T, LN, NS, HEADS, true><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, 0, stream>>>(p);
-  scan_kernel<T, LN, NS, HEADS, false><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, 0, stream>>>(p);
+  constexpr int ends = static_cast<int>(sizeof(Tile<LN, NS, true>)), whole = static_cast<int>(sizeof(Tile<LN, NS, false>));
+  static_assert(ends <= 48 * 1024, "within what a launch has without asking");
+  cudaError_t e = cudaFuncSetAttribute(scan_kernel<T, TD, LN, NS, HEADS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, whole);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (p.segments > 1) scan_kernel<T, TD, LN, NS, HEADS, true><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, ends, stream>>>(p);
+  scan_kernel<T, TD, LN, NS, HEADS, false><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, whole, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T>
+template <typename T, typename TD>
 int scan_any(const Args& p, cudaStream_t stream) {
   if (p.heads > 0) {
-    if (p.N <= 16) return scan_go<T, 4, 4, true>(p, stream);
-    if (p.N <= 32) return scan_go<T, 8, 4, true>(p, stream);
-    if (p.N <= 64) return scan_go<T, 16, 4, true>(p, stream);
-    if (p.N <= 128) return scan_go<T, 32, 4, true>(p, stream);
-    if (p.N <= 256) return scan_go<T, 32, 8, true>(p, stream);
+    if (p.N <= 16) return scan_go<T, TD, 4, 4, true>(p, stream);
+    if (p.N <= 32) return scan_go<T, TD, 8, 4, true>(p, stream);
+    if (p.N <= 64) return scan_go<T, TD, 16, 4, true>(p, stream);
+    if (p.N <= 128) return scan_go<T, TD, 32, 4, true>(p, stream);
+    if (p.N <= 256) return scan_go<T, TD, 32, 8, true>(p, stream);
     return -3;
   }
-  if (p.N <= 16) return scan_go<T, 4, 4, false>(p, stream);
-  if (p.N <= 32) return scan_go<T, 8, 4, false>(p, stream);
-  if (p.N <= 64) return scan_go<T, 16, 4, false>(p, stream);
-  if (p.N <= 128) return scan_go<T, 32, 4, false>(p, stream);
+  if (p.N <= 16) return scan_go<T, TD, 4, 4, false>(p, stream);
+  if (p.N <= 32) return scan_go<T, TD, 8, 4, false>(p, stream);
+  if (p.N <= 64) return scan_go<T, TD, 16, 4, false>(p, stream);
+  if (p.N <= 128) return scan_go<T, TD, 32, 4, false>(p, stream);
   return -3;
 }
 
@@ -447,7 +485,8 @@ extern "C" int dewb_selective_padding(int C, int N, int groups, int* padded) {
 extern "C" int dewb_selective_scan(const dewb_selective_args* a, int fp32, void* stream_ptr) {
   if (a == nullptr || !args_ok(*a)) return -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
-  return fp32 ? scan_any<float>(*a, stream) : scan_any<bf16>(*a, stream);
+  if (fp32) return a->dt_fp32 ? scan_any<float, float>(*a, stream) : -3;
+  return a->dt_fp32 ? scan_any<bf16, float>(*a, stream) : scan_any<bf16, bf16>(*a, stream);
 }
 
 // One token per row, with positions and a state.
