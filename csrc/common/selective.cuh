@@ -2,9 +2,8 @@
 //
 //   s = softplus(dt) (or dt);   h_t[n] = exp(s a[c, n]) h_{t-1}[n] + s x_t B_t[n];   y_t = (sum_n C_t[n] h_t[n] + D x_t) silu(z_t)
 //
-// A lane owns four channels and NS states of each; LN lanes share the states, 32 / LN groups of lanes the channels.  So what is summed over states crosses LN lanes and what is summed
-// over channels crosses 32 / LN, and neither takes a shuffle per product (a channel a lane with 16 states: 31 shuffles a token to sum 32 numbers over the lanes; here 7 for the
-// channels' sums and 3 for each number of the four channels).
+// A lane owns four channels and NS states of each; LN lanes share the states, 32 / LN groups of lanes the channels.  So a number of B or C serves four channels and a step NS states,
+// and what is summed over states or over channels is added up in the lane before it crosses lanes.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -19,10 +18,12 @@ extern "C" struct dewb_selective_args {
   const float* initial;                // [rows, C, N]; with positions, [store rows, C, N], and `last` is the same tensor
   float* last;
   void* y;                             // [R, T, C]
-  float* checkpoints;                  // [R, ceil(T / EVERY), padded C, padded N]: the state in front of every EVERY tokens
-  float *starts, *sums;                // [R, segments, padded C, padded N], [R, segments, padded C]: see scan_kernel
+  float* checkpoints;                  // [R, ceil(T / EVERY), groups * padded, padded N]: the state in front of every EVERY tokens
+  float *starts, *sums;                // [R, segments, groups * padded, padded N], [R, segments, groups * padded]: see scan_kernel
   const int *positions, *lengths, *row_ids;
-  int R, T, C, N, groups, heads, segments, segment;
+  int R, T, C, N, groups, heads, segments, segment, padded, states_each;      // `padded`: channels of a group in checkpoints, starts and sums, a multiple of 128 (with heads, of 256);
+                                       // `states_each`:
+                                       // states of a lane where there are up to 16 (1, 2 or 4)
   int softplus, log_a, dt_fp32, stored;      // `stored`: rows of the store, where row_ids or positions name them
   int* status;                         // told of a row outside the store, which then has no tokens
 };
@@ -47,7 +48,7 @@ struct Lay {
   static constexpr int CW = 4 * CG;              // channels of a warp
   static constexpr int CB = WARPS * CW;          // ... of a block
   static constexpr int NP = LN * NS;             // states, padded
-  static constexpr int TT = NS > 4 ? 8 : 16;     // tokens of a tile
+  static constexpr int TT = 16;                  // tokens of a tile
   static constexpr int PASSES = TT >= LN ? TT / LN : 1;      // a lane's pieces of four channels in a tile: token lane / CG + pass * LN
 };
 
@@ -90,6 +91,19 @@ __device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0
 __device__ __forceinline__ f2 ex2(f2 x) {
   const float2 t = x.get();
   return f2(ex2(t.x), ex2(t.y));
+}
+// n pairs that lie together
+template <int N>
+__device__ __forceinline__ void pairs(const float2* p, f2 (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0].v = *reinterpret_cast<const unsigned long long*>(p);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(p + k);
+      v[k].v = t.x; v[k + 1].v = t.y;
+    }
+  }
 }
 __device__ __forceinline__ void pair(const float* p, f2& a, f2& b) {         // four numbers, 16 bytes
   const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
@@ -158,6 +172,15 @@ __device__ __forceinline__ void put(bf16* p, const float (&f)[4], bool whole, in
   for (int j = 0; j < 4; ++j) if (j < n) p[j] = __float2bfloat16(f[j]);
 }
 
+// Four values, each twice.
+template <typename T>
+__device__ __forceinline__ void twice(float2* to, const Raw<T>& r) {
+  float f[4];
+  r.get(f);
+  reinterpret_cast<float4*>(to)[0] = make_float4(f[0], f[0], f[1], f[1]);
+  reinterpret_cast<float4*>(to)[1] = make_float4(f[2], f[2], f[3], f[3]);
+}
+
 // Whether four values at multiples of four columns can be read as one piece.
 template <typename T>
 __device__ __forceinline__ bool fours(const void* p, long long row, long long token) {
@@ -188,6 +211,9 @@ __device__ __forceinline__ float4 sum4(const float4* p, int n, int stride, int f
   return s;
 }
 
+template <int LN>
+__device__ __forceinline__ int turn_of(int lane) { return LN == 4 ? lane % 8 >> 1 : lane & 7; }
+
 // Which tokens of row `row` a call has, and where its state lies.
 struct Row {
   int len;             // live tokens
@@ -200,6 +226,14 @@ __device__ __forceinline__ Row row_of(const Args& p, int row) {
   const bool inside = p.initial == nullptr || (at >= 0 && at < p.stored);
   if (!inside && p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, OUTSIDE);
   return {first < 0 || !inside ? 0 : max(0, min(p.lengths[row] - first, p.T)), p.initial != nullptr && first > 0, at};
+}
+
+inline bool args_ok(const Args& p) {
+  if (p.R < 1 || p.T < 1 || p.C < 1 || p.N < 1 || p.groups < 1 || p.segments < 1 || p.segment < 1) return false;
+  if (p.heads > 0 ? p.C % p.heads || p.heads % p.groups : p.groups != 1) return false;
+  if (p.x == nullptr || p.dt == nullptr || p.b == nullptr || p.c == nullptr || p.a == nullptr || p.y == nullptr) return false;
+  if (p.padded % (p.heads > 0 ? 256 : 128) || p.padded < p.C / p.groups || p.segment % EVERY || static_cast<long long>(p.segments) * p.segment < p.T || (p.segments > 1 && (p.starts == nullptr || p.sums == nullptr))) return false;
+  return p.positions == nullptr || (p.lengths != nullptr && p.initial == p.last);
 }
 
 // The rate of channel c's state n times log2 e, 0 outside.

@@ -21,7 +21,7 @@ extern "C" struct dewb_selective_grad_args {
   void *dx, *ddt, *dz;                 // [R, T, C]; dz null where the call has no gate
   void *db, *dc;                       // [R, T, N]
   float *da, *dd, *dinitial;           // [C, N], [C], [R, C, N]; dd and dinitial may be null
-  float *bc_parts, *a_parts, *d_parts; // [channel blocks, R * T, 2, padded N], [R * segments, padded C, padded N], [R * segments, padded C]
+  float *bc_parts, *a_parts, *d_parts; // [channel blocks, R * T, 2, padded N], [R * segments, padded, padded N], [R * segments, padded]
 };
 
 namespace dewb {
@@ -31,22 +31,23 @@ using Grad = dewb_selective_grad_args;
 constexpr int TT = Lay<4, 4>::TT;
 constexpr int FOUR = 4;                // tokens whose decays and states a lane has in registers
 
-template <int LN>
+template <int LN, int NS>
 struct Shared {
-  using L = Lay<LN, 4>;
+  using L = Lay<LN, NS>;
   float step[WARPS][TT][L::CW], w[WARPS][TT][L::CW];      // s, w
   float2 c[TT][L::NP];                                    // C, each number twice; up to here, what back_ends_kernel has
   float in[WARPS][TT][L::CW];                             // u
   float2 b[TT][L::NP];
   float bc[WARPS][TT][2][L::NP];                          // dB and dC of the warp's channels
-  float4 h[WARPS][TT / FOUR][4][32];                      // a lane's states in front of every four tokens: channels 0 and 1 of two states in each of the first two pieces, 2 and 3 in the others
-  float4 shares[WARPS][FOUR][5][32];                      // a lane's shares of sum g B, sum A q, sum C h (four channels), of dB and dC (four states)
+  float4 h[WARPS][TT / FOUR][NS][32];                     // a lane's states in front of every four tokens, in pairs of channels as they are
+  float4 shares[WARPS][FOUR][3][32];                      // a lane's shares of sum g B, sum A q and sum C h, four channels each
+  float4 both[WARPS][FOUR][NS / 2][32];                   // ... and of dB and dC, NS states each
 };
 
 // Where a lane loads and stores: four channels of token lt + pass * LN; and what it has of a tile's tokens.
-template <typename T, typename TD, int LN, bool STATES>
+template <typename T, typename TD, int LN, int NS, bool STATES>
 struct Place {
-  using L = Lay<LN, 4>;
+  using L = Lay<LN, NS>;
   int lt, lq, lc, left;
   bool whole;                          // ... all over the block, in pieces of four
   const T *x, *z, *dy;
@@ -99,9 +100,9 @@ struct Place {
 };
 
 // What a block has of a tile's B and C.
-template <typename T, int LN, bool STATES>
+template <typename T, int LN, int NS, bool STATES>
 struct Narrow {
-  using L = Lay<LN, 4>;
+  using L = Lay<LN, NS>;
   static constexpr int EACH = (TT * L::NP + THREADS - 1) / THREADS;
   uint32_t b[STATES ? EACH : 1], c[EACH];
   __device__ __forceinline__ void bring(const Args& p, int row, int t0, int t_end) {
@@ -114,7 +115,7 @@ struct Narrow {
       c[i] = on ? word(pc + t * p.c_token + n) : 0u;
     }
   }
-  __device__ __forceinline__ void put(Shared<LN>& sm) const {
+  __device__ __forceinline__ void put(Shared<LN, NS>& sm) const {
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int at = threadIdx.x + i * THREADS;
@@ -126,9 +127,9 @@ struct Narrow {
 };
 
 // s, u and w of the warp's channels from what the lanes have brought; behind t_end and the last channel, zeros.
-template <typename T, typename TD, int LN, bool STATES>
-__device__ __forceinline__ void stage(Shared<LN>& sm, const Place<T, TD, LN, STATES>& at, bool steps, int t0, int t_end, int warp, float (&total)[4]) {
-  using L = Lay<LN, 4>;
+template <typename T, typename TD, int LN, int NS, bool STATES>
+__device__ __forceinline__ void stage(Shared<LN, NS>& sm, const Place<T, TD, LN, NS, STATES>& at, bool steps, int t0, int t_end, int warp, float (&total)[4]) {
+  using L = Lay<LN, NS>;
   const bool all = t0 + TT <= t_end && at.left == 4;
 #pragma unroll
   for (int i = 0; i < L::PASSES; ++i) {
@@ -153,59 +154,78 @@ __device__ __forceinline__ void stage(Shared<LN>& sm, const Place<T, TD, LN, STA
   }
 }
 
-// Numbers of four channels (from c on) and four states (from n on), channels in pairs.
+// Numbers of four channels and NS states, channels in pairs.
+template <int NS>
 struct Block {
-  f2 v[2][4];
+  f2 v[2][NS];
   template <typename F>
   __device__ __forceinline__ static Block make(F f) {
     Block r;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r.v[i][k] = f2(f(2 * i, k), f(2 * i + 1, k));
+      for (int k = 0; k < NS; ++k) r.v[i][k] = f2(f(2 * i, k), f(2 * i + 1, k));
     return r;
   }
-  __device__ __forceinline__ static Block load(const float* p, int stride) {
-    return make([&](int j, int k) { return p[j * stride + k]; });
+  // `channels` of them (0 to 4), zeros in place of the others
+  __device__ __forceinline__ static Block load(const float* p, int stride, int channels = 4) {
+    float2 e[4][NS / 2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < NS / 2; ++k) e[j][k] = j < channels ? *reinterpret_cast<const float2*>(p + j * stride + 2 * k) : make_float2(0.f, 0.f);
+    Block r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < NS / 2; ++k) {
+        r.v[i][2 * k] = f2(e[2 * i][k].x, e[2 * i + 1][k].x);
+        r.v[i][2 * k + 1] = f2(e[2 * i][k].y, e[2 * i + 1][k].y);
+      }
+    return r;
   }
   __device__ __forceinline__ void store(float* p, int stride) const {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 e0 = v[i][0].get(), e1 = v[i][1].get(), e2 = v[i][2].get(), e3 = v[i][3].get();
-      *reinterpret_cast<float4*>(p + 2 * i * stride) = make_float4(e0.x, e1.x, e2.x, e3.x);
-      *reinterpret_cast<float4*>(p + (2 * i + 1) * stride) = make_float4(e0.y, e1.y, e2.y, e3.y);
-    }
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < NS; k += 2) {
+        const float2 e0 = v[i][k].get(), e1 = v[i][k + 1].get();
+        *reinterpret_cast<float2*>(p + 2 * i * stride + k) = make_float2(e0.x, e1.x);
+        *reinterpret_cast<float2*>(p + (2 * i + 1) * stride + k) = make_float2(e0.y, e1.y);
+      }
   }
 };
 
-__device__ __forceinline__ Block last_of(const Grad& g, int row, int c, int n, bool there) {
+template <int NS>
+__device__ __forceinline__ Block<NS> last_of(const Grad& g, int row, int c, int n, bool there) {
   const Args& p = g.f;
-  return Block::make([&](int j, int k) { return there && g.dlast != nullptr && c + j < p.C && n + k < p.N ? g.dlast[(static_cast<long long>(row) * p.C + c + j) * p.N + n + k] : 0.f; });
+  return Block<NS>::make([&](int j, int k) { return there && g.dlast != nullptr && c + j < p.C && n + k < p.N ? g.dlast[(static_cast<long long>(row) * p.C + c + j) * p.N + n + k] : 0.f; });
 }
 
 // grid R * (segments - 1) * channel blocks, of segments 1, 2, ...: starts[r, j] is the gradient of the state in front of segment j that the segment itself makes (the last one: with dlast).
-template <typename T, typename TD, int LN>
+template <typename T, typename TD, int LN, int NS>
 __global__ void __launch_bounds__(THREADS, 4)
 back_ends_kernel(const Grad g) {
-  using L = Lay<LN, 4>;
-  __shared__ __align__(16) char raw[offsetof(Shared<LN>, in)];
-  Shared<LN>& sm = *reinterpret_cast<Shared<LN>*>(raw);
+  using L = Lay<LN, NS>;
+  using S = Shared<LN, NS>;
+  __shared__ __align__(16) char raw[offsetof(S, in)];
+  S& sm = *reinterpret_cast<S*>(raw);
   const Args& p = g.f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sl = lane % LN, cg = lane / LN;
-  const int blocks = (p.C + L::CB - 1) / L::CB, padded = blocks * L::CB;
+  const int blocks = (p.C + L::CB - 1) / L::CB, padded = p.padded;
   const int cb = blockIdx.x % blocks, seg = 1 + blockIdx.x / blocks % (p.segments - 1), row = blockIdx.x / blocks / (p.segments - 1);
   const int c0 = cb * L::CB + warp * L::CW, t_begin = seg * p.segment, t_end = min(p.T, t_begin + p.segment);
-  Place<T, TD, LN, false> at(g, row, cb * L::CB, c0, lane);
-  Narrow<T, LN, false> narrow;
+  Place<T, TD, LN, NS, false> at(g, row, cb * L::CB, c0, lane);
+  Narrow<T, LN, NS, false> narrow;
   float total[4] = {0.f, 0.f, 0.f, 0.f};
-  const Block a = Block::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * 4 + k, 1); });
-  Block d = last_of(g, row, c0 + cg * 4, sl * 4, seg == p.segments - 1);
+  const Block<NS> a = Block<NS>::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * NS + k, 1); });
+  Block<NS> d = last_of<NS>(g, row, c0 + cg * 4, sl * NS, seg == p.segments - 1);
   int t0 = t_begin + (t_end - t_begin - 1) / TT * TT;
   at.bring(g, t0, t_end);
   narrow.bring(p, row, t0, t_end);
   for (; t0 >= t_begin; t0 -= TT) {
     __syncthreads();
-    stage<T, TD, LN, false>(sm, at, p.softplus, t0, t_end, warp, total);
+    stage<T, TD, LN, NS, false>(sm, at, p.softplus, t0, t_end, warp, total);
     narrow.put(sm);
     __syncthreads();
     if (t0 > t_begin) {
@@ -215,19 +235,18 @@ back_ends_kernel(const Grad g) {
     const int count = min(TT, t_end - t0);
 #pragma unroll 4
     for (int t = (count + 3) / 4 * 4 - 1; t >= 0; --t) {
-      f2 s[2], w[2], c[4];
+      f2 s[2], w[2], c[NS];
       pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
       pair(&sm.w[warp][t][cg * 4], w[0], w[1]);
-      pair(&sm.c[t][sl * 4].x, c[0], c[1]);
-      pair(&sm.c[t][sl * 4 + 2].x, c[2], c[3]);
+      pairs(&sm.c[t][sl * NS], c);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d.v[i][k] = mul(ex2(mul(s[i], a.v[i][k])), fma(w[i], c[k], d.v[i][k]));
+        for (int k = 0; k < NS; ++k) d.v[i][k] = mul(ex2(mul(s[i], a.v[i][k])), fma(w[i], c[k], d.v[i][k]));
     }
   }
   const long long out = (static_cast<long long>(row) * p.segments + seg) * padded + c0;
-  d.store(p.starts + (out + cg * 4) * L::NP + sl * 4, L::NP);
+  d.store(p.starts + (out + cg * 4) * L::NP + sl * NS, L::NP);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -236,31 +255,31 @@ back_ends_kernel(const Grad g) {
   }
 }
 
-template <typename T, typename TD, int LN>
-__global__ void __launch_bounds__(THREADS, 2)
+template <typename T, typename TD, int LN, int NS>
+__global__ void __launch_bounds__(THREADS, NS == 2 ? 3 : 2)
 grad_kernel(const Grad g) {
-  using L = Lay<LN, 4>;
+  using L = Lay<LN, NS>;
   constexpr int CG = L::CG, NP = L::NP;
   extern __shared__ __align__(16) char raw[];
-  Shared<LN>& sm = *reinterpret_cast<Shared<LN>*>(raw);
+  Shared<LN, NS>& sm = *reinterpret_cast<Shared<LN, NS>*>(raw);
   const Args& p = g.f;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sl = lane % LN, cg = lane / LN;
-  const int blocks = (p.C + L::CB - 1) / L::CB, padded = blocks * L::CB;
+  const int blocks = (p.C + L::CB - 1) / L::CB, padded = p.padded;
   const int cb = blockIdx.x % blocks, seg = blockIdx.x / blocks % p.segments, row = blockIdx.x / blocks / p.segments;
   const int c0 = cb * L::CB + warp * L::CW, t_begin = seg * p.segment, t_end = min(p.T, t_begin + p.segment);
-  Place<T, TD, LN, true> at(g, row, cb * L::CB, c0, lane);
+  Place<T, TD, LN, NS, true> at(g, row, cb * L::CB, c0, lane);
   int t0 = t_begin + (t_end - t_begin - 1) / TT * TT;
   const long long pad_row = static_cast<long long>(row) * p.segments * padded + c0 + cg * 4;
-  const Block a = Block::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * 4 + k, 1); });
-  Block d = last_of(g, row, c0 + cg * 4, sl * 4, seg == p.segments - 1), da = Block::make([](int, int) { return 0.f; });
+  const Block<NS> a = Block<NS>::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * NS + k, 1); });
+  Block<NS> d = last_of<NS>(g, row, c0 + cg * 4, sl * NS, seg == p.segments - 1), da = Block<NS>::make([](int, int) { return 0.f; });
   for (int q = p.segments - 1; q > seg; --q) {    // what comes from behind the segment
     const long long there = pad_row + static_cast<long long>(q) * padded;
-    const Block e = Block::load(p.starts + there * NP + sl * 4, NP);
+    const Block<NS> e = Block<NS>::load(p.starts + there * NP + sl * NS, NP);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const f2 sum = q < p.segments - 1 ? f2(p.sums[there + 2 * i], p.sums[there + 2 * i + 1]) : f2(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d.v[i][k] = fma(ex2(mul(sum, a.v[i][k])), d.v[i][k], e.v[i][k]);
+      for (int k = 0; k < NS; ++k) d.v[i][k] = fma(ex2(mul(sum, a.v[i][k])), d.v[i][k], e.v[i][k]);
     }
   }
   float skip[4], dd[4] = {0.f, 0.f, 0.f, 0.f}, unused[4] = {0.f, 0.f, 0.f, 0.f};
@@ -272,33 +291,35 @@ grad_kernel(const Grad g) {
   auto piece = [&](const float4* q, f2& x, f2& y) { pair(&q->x, x, y); };
   auto leave = [](float4* q, f2 x, f2 y) { *reinterpret_cast<ulonglong2*>(q) = make_ulonglong2(x.v, y.v); };
   for (; t0 >= t_begin; t0 -= TT) {
-    Narrow<T, LN, true> narrow;
+    Narrow<T, LN, NS, true> narrow;
     at.bring(g, t0, t_end);
     narrow.bring(p, row, t0, t_end);
-    Block h = Block::load(p.checkpoints + ((static_cast<long long>(row) * kept + t0 / EVERY) * padded + c0 + cg * 4) * NP + sl * 4, NP);
     if (t0 > t_begin) at.call(g, t0 - TT, t_end);
-    stage<T, TD, LN, true>(sm, at, p.softplus, t0, t_end, warp, unused);
+    stage<T, TD, LN, NS, true>(sm, at, p.softplus, t0, t_end, warp, unused);
     narrow.put(sm);
+    // (channels behind the last one have no kept states: the forward's blocks may be narrower)
+    const float* before = p.checkpoints + ((static_cast<long long>(row) * kept + t0 / EVERY) * padded + c0 + cg * 4) * NP + sl * NS;
+    Block<NS> h = Block<NS>::load(before, NP, p.C - c0 - cg * 4);
+    if (t0 > t_begin && c0 + cg * 4 < p.C) asm volatile("prefetch.global.L2 [%0];" ::"l"(before - static_cast<long long>(padded) * NP));
     __syncthreads();
     const int count = min(TT, t_end - t0), groups = (count + FOUR - 1) / FOUR;
     // (behind the last token steps, u and w are zero: decays of one, and nothing added to any sum)
 #pragma unroll 1
     for (int q = 0; q < groups; ++q) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) leave(&sm.h[warp][q][i][lane], h.v[i / 2][i % 2 * 2], h.v[i / 2][i % 2 * 2 + 1]);
+      for (int i = 0; i < NS; ++i) leave(&sm.h[warp][q][i][lane], h.v[i / (NS / 2)][i % (NS / 2) * 2], h.v[i / (NS / 2)][i % (NS / 2) * 2 + 1]);
       if (q + 1 < groups) {
 #pragma unroll
         for (int i = 0; i < FOUR; ++i) {
           const int t = q * FOUR + i;
-          f2 s[2], u[2], b[4];
+          f2 s[2], u[2], b[NS];
           pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
           pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
-          pair(&sm.b[t][sl * 4].x, b[0], b[1]);
-          pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
+          pairs(&sm.b[t][sl * NS], b);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) h.v[j][k] = fma(ex2(mul(s[j], a.v[j][k])), h.v[j][k], mul(u[j], b[k]));
+            for (int k = 0; k < NS; ++k) h.v[j][k] = fma(ex2(mul(s[j], a.v[j][k])), h.v[j][k], mul(u[j], b[k]));
         }
       }
     }
@@ -314,23 +335,19 @@ grad_kernel(const Grad g) {
       Raw<T> rz;
       if (at.z != nullptr) rz = fetch(at.z + tok * p.z_token, fast, n);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        piece(&sm.h[warp][q][2 * i][lane], h.v[i][0], h.v[i][1]);
-        piece(&sm.h[warp][q][2 * i + 1][lane], h.v[i][2], h.v[i][3]);
-      }
-      Block e[FOUR], ah[FOUR];
+      for (int i = 0; i < NS; ++i) piece(&sm.h[warp][q][i][lane], h.v[i / (NS / 2)][i % (NS / 2) * 2], h.v[i / (NS / 2)][i % (NS / 2) * 2 + 1]);
+      Block<NS> e[FOUR], ah[FOUR];
 #pragma unroll
       for (int i = 0; i < FOUR; ++i) {
         const int t = from + i;
-        f2 s[2], u[2], b[4];
+        f2 s[2], u[2], b[NS];
         pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
         pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
-        pair(&sm.b[t][sl * 4].x, b[0], b[1]);
-        pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
+        pairs(&sm.b[t][sl * NS], b);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < NS; ++k) {
             e[i].v[j][k] = ex2(mul(s[j], a.v[j][k]));
             ah[i].v[j][k] = mul(e[i].v[j][k], h.v[j][k]);
             if (i + 1 < FOUR) h.v[j][k] = fma(u[j], b[k], ah[i].v[j][k]);
@@ -339,18 +356,16 @@ grad_kernel(const Grad g) {
 #pragma unroll
       for (int i = FOUR - 1; i >= 0; --i) {
         const int t = from + i;
-        f2 s[2], u[2], w[2], b[4], c[4], db[4], dc[4], s1[2], s2[2], s3[2];
+        f2 s[2], u[2], w[2], b[NS], c[NS], db[NS], dc[NS], s1[2], s2[2], s3[2];
         pair(&sm.step[warp][t][cg * 4], s[0], s[1]);
         pair(&sm.in[warp][t][cg * 4], u[0], u[1]);
         pair(&sm.w[warp][t][cg * 4], w[0], w[1]);
-        pair(&sm.b[t][sl * 4].x, b[0], b[1]);
-        pair(&sm.b[t][sl * 4 + 2].x, b[2], b[3]);
-        pair(&sm.c[t][sl * 4].x, c[0], c[1]);
-        pair(&sm.c[t][sl * 4 + 2].x, c[2], c[3]);
+        pairs(&sm.b[t][sl * NS], b);
+        pairs(&sm.c[t][sl * NS], c);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < NS; ++k) {
             const f2 now = fma(u[j], b[k], ah[i].v[j][k]), gt = fma(w[j], c[k], d.v[j][k]), through = mul(gt, ah[i].v[j][k]);
             db[k] = j == 0 ? mul(u[j], gt) : fma(u[j], gt, db[k]);
             dc[k] = j == 0 ? mul(w[j], now) : fma(w[j], now, dc[k]);
@@ -360,28 +375,34 @@ grad_kernel(const Grad g) {
             da.v[j][k] = fma(through, s[j], da.v[j][k]);
             d.v[j][k] = mul(gt, e[i].v[j][k]);
           }
-        float vb[4], vc[4];
+        float v[2 * NS];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < NS; ++k) {
           const float2 x = db[k].get(), y = dc[k].get();
-          vb[k] = x.x + x.y;
-          vc[k] = y.x + y.y;
+          v[k] = x.x + x.y;
+          v[NS + k] = y.x + y.y;
         }
         leave(&sm.shares[warp][i][0][lane], s1[0], s1[1]);
         leave(&sm.shares[warp][i][1][lane], s2[0], s2[1]);
         leave(&sm.shares[warp][i][2][lane], s3[0], s3[1]);
-        sm.shares[warp][i][3][lane] = make_float4(vb[0], vb[1], vb[2], vb[3]);
-        sm.shares[warp][i][4][lane] = make_float4(vc[0], vc[1], vc[2], vc[3]);
+#pragma unroll
+        for (int k = 0; k < NS / 2; ++k) sm.both[warp][i][k][lane] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
       }
       __syncwarp();
-      // dB and dC of the warp's channels: a lane takes four states of a token
+      // dB and dC of the warp's channels: a lane takes four of a token's numbers
 #pragma unroll
-      for (int o = lane; o < FOUR * 2 * LN; o += 32) {
-        const int state = o % LN, which = o / LN % 2, i = o / LN / 2;
-        *reinterpret_cast<float4*>(&sm.bc[warp][from + i][which][state * 4]) = sum4(&sm.shares[warp][i][3 + which][state], CG, LN, which);
+      for (int o = lane; o < FOUR * NS / 2 * LN; o += 32) {
+        const int state = o % LN, k = o / LN % (NS / 2), i = o / LN / (NS / 2);
+        const float4 v = sum4(&sm.both[warp][i][k][state], CG, LN, k);
+        if constexpr (NS == 4) {
+          *reinterpret_cast<float4*>(&sm.bc[warp][from + i][k][state * 4]) = v;
+        } else {
+          *reinterpret_cast<float2*>(&sm.bc[warp][from + i][0][state * 2]) = make_float2(v.x, v.y);
+          *reinterpret_cast<float2*>(&sm.bc[warp][from + i][1][state * 2]) = make_float2(v.z, v.w);
+        }
       }
       if (ends) {
-        const int turn = LN == 4 ? lane % CG >> 1 : 0, first = lane % CG * LN;
+        const int turn = turn_of<LN>(lane), first = lane % CG * LN;
         const float4 v1 = sum4(&sm.shares[warp][at.lt][0][first], LN, 1, turn), v2 = sum4(&sm.shares[warp][at.lt][1][first], LN, 1, turn);
         const float4 s4 = *reinterpret_cast<const float4*>(&sm.step[warp][mine][at.lq]), w4 = *reinterpret_cast<const float4*>(&sm.w[warp][mine][at.lq]);
         const float r1[4] = {v1.x, v1.y, v1.z, v1.w}, r2[4] = {v2.x, v2.y, v2.z, v2.w}, s[4] = {s4.x, s4.y, s4.z, s4.w}, w[4] = {w4.x, w4.y, w4.z, w4.w};
@@ -414,12 +435,12 @@ grad_kernel(const Grad g) {
       __syncwarp();                               // (the shares have been read)
     }
     __syncthreads();
-    for (int o = tid; o < count * 2 * LN; o += THREADS)
+    for (int o = tid; o < count * NP / 2; o += THREADS)
       *reinterpret_cast<float4*>(g.bc_parts + ((static_cast<long long>(cb) * p.R + row) * p.T + t0) * (2 * NP) + o * 4) =
-          sum4(reinterpret_cast<const float4*>(&sm.bc[0][0][0][0]) + o, WARPS, TT * 2 * LN, 0);
+          sum4(reinterpret_cast<const float4*>(&sm.bc[0][0][0][0]) + o, WARPS, TT * NP / 2, 0);
   }
   const long long part = (static_cast<long long>(row) * p.segments + seg) * padded + c0;
-  da.store(g.a_parts + (part + cg * 4) * NP + sl * 4, NP);
+  da.store(g.a_parts + (part + cg * 4) * NP + sl * NS, NP);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -430,8 +451,8 @@ grad_kernel(const Grad g) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = c0 + cg * 4 + 2 * i, n = sl * 4 + k;
+      for (int k = 0; k < NS; ++k) {
+        const int c = c0 + cg * 4 + 2 * i, n = sl * NS + k;
         const float2 v = d.v[i][k].get();
         if (c < p.C && n < p.N) g.dinitial[(static_cast<long long>(row) * p.C + c) * p.N + n] = v.x;
         if (c + 1 < p.C && n < p.N) g.dinitial[(static_cast<long long>(row) * p.C + c + 1) * p.N + n] = v.y;
@@ -473,25 +494,25 @@ grad_sum_kernel(const Grad g, int blocks, int padded, int np) {
   }
 }
 
-template <typename T, typename TD, int LN>
+template <typename T, typename TD, int LN, int NS = 4>
 int grad_go(const Grad& g, cudaStream_t stream) {
-  using L = Lay<LN, 4>;
+  using L = Lay<LN, NS>;
   const Args& p = g.f;
   const long long blocks = (p.C + L::CB - 1) / L::CB;
   const long long sums = (static_cast<long long>(p.R) * p.T * 2 * p.N + static_cast<long long>(p.C) * (p.N + 1) + 255) / 256;
   if (blocks * p.segments * p.R > 0x7fffffffLL || sums > 0x7fffffffLL) return -3;
-  constexpr int smem = static_cast<int>(sizeof(Shared<LN>));
-  cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, TD, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr int smem = static_cast<int>(sizeof(Shared<LN, NS>));
+  cudaError_t e = cudaFuncSetAttribute(grad_kernel<T, TD, LN, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return static_cast<int>(e);
-  if (p.segments > 1) back_ends_kernel<T, TD, LN><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, 0, stream>>>(g);
-  grad_kernel<T, TD, LN><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, smem, stream>>>(g);
-  grad_sum_kernel<T><<<static_cast<unsigned>(sums), 256, 0, stream>>>(g, static_cast<int>(blocks), static_cast<int>(blocks) * L::CB, L::NP);
+  if (p.segments > 1) back_ends_kernel<T, TD, LN, NS><<<static_cast<unsigned>(blocks * (p.segments - 1) * p.R), THREADS, 0, stream>>>(g);
+  grad_kernel<T, TD, LN, NS><<<static_cast<unsigned>(blocks * p.segments * p.R), THREADS, smem, stream>>>(g);
+  grad_sum_kernel<T><<<static_cast<unsigned>(sums), 256, 0, stream>>>(g, static_cast<int>(blocks), p.padded, L::NP);
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, typename TD>
 int grad_any(const Grad& g, cudaStream_t stream) {
-  if (g.f.N <= 16) return grad_go<T, TD, 4>(g, stream);
+  if (g.f.N <= 16) return g.f.states_each == 2 ? grad_go<T, TD, 8, 2>(g, stream) : grad_go<T, TD, 4>(g, stream);
   if (g.f.N <= 32) return grad_go<T, TD, 8>(g, stream);
   if (g.f.N <= 64) return grad_go<T, TD, 16>(g, stream);
   if (g.f.N <= 128) return grad_go<T, TD, 32>(g, stream);
@@ -506,7 +527,8 @@ using namespace dewb::selective;
 extern "C" int dewb_selective_grad(const dewb_selective_grad_args* a, int fp32, void* stream_ptr) {
   if (a == nullptr) return -3;
   const Args& p = a->f;
-  if (p.R < 1 || p.T < 1 || p.C < 1 || p.N < 1 || p.heads > 0 || p.groups != 1 || p.positions != nullptr || p.checkpoints == nullptr || p.segments < 1 || p.segment < 1 || p.segment % EVERY)
+  if (p.R < 1 || p.T < 1 || p.C < 1 || p.N < 1 || p.heads > 0 || p.groups != 1 || p.positions != nullptr || p.checkpoints == nullptr || p.segments < 1 || p.segment < 1 || p.segment % EVERY ||
+      p.padded % 128 || p.padded < p.C)
     return -3;
   // every segment has a token, and every token a segment
   if (static_cast<long long>(p.segments) * p.segment < p.T || static_cast<long long>(p.segments - 1) * p.segment >= p.T) return -3;

@@ -27,7 +27,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--use_fast_math", "-Xcompiler",
 
 # Files whose 32-bit arithmetic has to hold up on its own (decoders that run in fp32): compiled without fast math.
 EXACT_MATH = ("residual_streams", "paged_attention", "latent_attention", "decayed_recurrence", "gated_recurrence", "gated_chunks", "token_mix", "moe_serve",
-              "shared_prefix", "selective_scan", "gate_norm")
+              "shared_prefix", "selective_scan", "selective_heads", "gate_norm")
 
 # The same for kernels of training, which a program that only decodes does not build: gradients that are kept in fp32.
 EXACT_TRAINING = ("ssd_sm100", "ada_norm", "selective_grad")

@@ -86,6 +86,10 @@ _SIGNATURES = {
     "dewb_shared_decode_mma": "pl" + "pp" + "ppppp" + "p" + "pppp" + "iiiiiiiiiii" + "ff" + "pp",
     "dewb_add_adapters_mma": "pl" + "pppp" + "pppp" + "iiiiii" + "pp",
     "dewb_add_adapters": "pl" + "pppp" + "pp" + "iiiiiii" + "pp",
+    "dewb_selective_scan": "pip",
+    "dewb_selective_token": "pip",
+    "dewb_selective_grad": "pip",
+    "dewb_head_scan": "piip",
     "dewb_gate_norm_fwd": "plplpp" + "li" + "f" + "ii" + "p",
     "dewb_gate_norm_bwd": "plplpl" + "ppppp" + "ili" + "f" + "ii" + "p",
     "dewb_rope_append": "pppp" + "iiiii" + "ppp" + "ii" + "p",

@@ -1,4 +1,4 @@
-"""The selective state space scan (``csrc/kernels/selective_scan.cu``, ``selective_grad.cu``; the equations stand in ``csrc/common/selective.cuh``): a rate per channel and state
+"""The selective state space scan (``csrc/kernels/selective_scan.cu``, ``selective_grad.cu``, ``selective_heads.cu``; the equations stand in ``csrc/common/selective.cuh``): a rate per channel and state
 (Mamba-1) over whole rows with every gradient, and over a call's ``Rows`` with the states that a store keeps; and the same with a decay per head (Mamba-2) for such a call.  The plain
 forms go token by token (``selective_tokens_reference``, ``ssd_tokens_reference``) or in chunks (``ops.scan.selective_scan_chunked``).
 """
@@ -18,7 +18,7 @@ EVERY = 16               # tokens between two states that the forward keeps for 
 
 _FIELDS = (("x dt z b c", ctypes.c_void_p), ("x_row x_token dt_row dt_token z_row z_token b_row b_token c_row c_token", ctypes.c_longlong),
            ("a dt_bias d initial last y checkpoints starts sums positions lengths row_ids", ctypes.c_void_p),
-           ("R T C N groups heads segments segment softplus log_a dt_fp32 stored", ctypes.c_int), ("status", ctypes.c_void_p))
+           ("R T C N groups heads segments segment padded states_each softplus log_a dt_fp32 stored", ctypes.c_int), ("status", ctypes.c_void_p))
 
 
 class _Args(ctypes.Structure):
@@ -32,22 +32,28 @@ class _Grad(ctypes.Structure):
                [(name, ctypes.c_void_p) for name in "dlast dx ddt dz db dc da dd dinitial bc_parts a_parts d_parts".split()]
 
 
-def _padded(C: int, N: int, groups: int = 1):
-    """Channels and states as the workspaces pad them, and the warps that a row's channels take."""
+def _padded(C: int, N: int, groups: int = 1, heads: int = 0):
+    """Channels (of all groups) and states as the workspaces pad them, and the channels that a warp takes with four states a lane."""
     lanes = 4 if N <= 16 else 8 if N <= 32 else 16 if N <= 64 else 32
-    block = 512 // lanes
-    blocks = -(-(C // groups) // block) * groups
-    return blocks * block, lanes * 4 if N <= 128 else 256, blocks * 4
+    block = 256 if heads else 128
+    return -(-(C // groups) // block) * block * groups, lanes * 4 if N <= 128 else 256, block // lanes
 
 
-WARPS = 148 * 8           # what the GPU is filled with
+WARPS = 148 * 28          # what the GPU is filled with
 
 
-def _segments(R: int, T: int, warps: int) -> int:
-    """How many pieces of a row run side by side, and tokens of a piece."""
-    pieces = max(1, min(-(-T // 64), WARPS // max(1, R * warps)))
-    length = -(-(-(-T // pieces)) // EVERY) * EVERY
-    return length
+def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward: bool = False):
+    """Tokens of a piece of a row (the pieces run side by side), and states of a lane (of up to 16)."""
+    warps = max(1, R * groups * -(-(C // groups) // _padded(C, N, groups, heads)[2]))
+    most = -(-T // 32)
+    if heads:
+        pieces, each = (1 if warps >= 2368 else min(most, -(-WARPS // warps))), 4
+    elif N <= 16 and not backward and 448 <= warps < 1536:
+        pieces, each = 1, 2
+    else:
+        pieces = min(most, -(-WARPS // warps)) if warps < 1536 else 1
+        each = 4 if N > 16 or warps * most >= WARPS // 2 else 2 if backward or warps * most >= WARPS // 4 else 1
+    return -(-(-(-T // pieces)) // EVERY) * EVERY, each
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -60,26 +66,30 @@ def _rows(t: Optional[torch.Tensor]):
     return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
 
 
-def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0):
+def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0, backward: bool = False):
     """The arguments of a launch, and what has to live until it is issued."""
     R, T, C = x.shape
-    channels, states, warps = _padded(C, N, groups)
-    segment = _segments(R, T, warps)
+    channels, states, _ = _padded(C, N, groups, heads)
+    segment, each = _split(R, T, C, N, groups, heads, backward)
     segments = -(-T // segment)
     work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device) if segments > 1 else None
     starts = L.at(work)
     (px, *sx), (pd, *sd), (pz, *sz), (pb, *sb), (pc, *sc) = (_rows(t) for t in (x, dt, z, b, c))
     at = (0, 0, 0) if rows is None else (rows.positions.data_ptr(), rows.lengths.data_ptr(), L.at(rows.row_ids))
     args = _Args(px, pd, pz, pb, pc, *sx, *sd, *sz, *sb, *sc, a.data_ptr(), L.at(dt_bias), L.at(d), L.at(initial), L.at(last), L.at(y), L.at(checkpoints), starts,
-                 starts + 4 * R * segments * channels * states if work is not None else 0, *at, R, T, C, N, groups, heads, segments, segment, int(softplus), int(log_a),
+                 starts + 4 * R * segments * channels * states if work is not None else 0, *at, R, T, C, N, groups, heads, segments, segment, channels // groups, each, int(softplus), int(log_a),
                  int(dt.dtype is torch.float32), stored, L.status(x.device).data_ptr())
     return args, work
 
 
 def _launch(args: _Args, fp32: bool, token: bool, stream: int) -> None:
-    lib = L.load()
-    launch = lib.dewb_selective_token if token else lib.dewb_selective_scan
-    L.check(launch(ctypes.byref(args), ctypes.c_int(int(fp32)), ctypes.c_void_p(stream)), "selective_token" if token else "selective_scan")
+    lib, at = L.load(), ctypes.addressof(args)
+    if args.heads:
+        L.check(lib.dewb_head_scan(at, fp32, token, stream), "head_scan")
+    elif token:
+        L.check(lib.dewb_selective_token(at, fp32, stream), "selective_token")
+    else:
+        L.check(lib.dewb_selective_scan(at, fp32, stream), "selective_scan")
     L.count_launches(1 if args.segments == 1 else 2)
 
 
@@ -104,18 +114,18 @@ def _backward(x, dt, a, b, c, d, z, initial, kept, softplus: bool, dy, dlast):
     """-> dx, ddt, da, db, dc, dd, dz, dinitial."""
     R, T, C = x.shape
     N, dev = a.shape[1], x.device
-    channels, states, warps = _padded(C, N)
+    channels, states, wide = _padded(C, N)
     f32 = dict(dtype=torch.float32, device=dev)
     like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
     dx, ddt, dz, db, dc, da, dd, dinitial = like(x), like(dt), like(z), like(b), like(c), like(a), like(d), like(initial)
     with L.on_device_of(x) as stream:
-        args, work = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False)
-        bc = torch.empty(warps // 4, R * T, 2, states, **f32)
+        args, work = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False, backward=True)
+        bc = torch.empty(-(-C // (wide * args.states_each)), R * T, 2, states, **f32)
         parts = torch.empty(R * args.segments, channels, states + 1, **f32)
         at, row, token = _rows(dy)
         grad = _Grad(args, at, row, token, *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial, bc, parts)),
                      parts.data_ptr() + 4 * R * args.segments * channels * states)
-        L.check(L.load().dewb_selective_grad(ctypes.byref(grad), ctypes.c_int(int(x.dtype is torch.float32)), ctypes.c_void_p(stream)), "selective_grad")
+        L.check(L.load().dewb_selective_grad(ctypes.addressof(grad), x.dtype is torch.float32, stream), "selective_grad")
         L.count_launches(2 if args.segments == 1 else 3)
     return dx, ddt, da, db, dc, dd, dz, dinitial
 

@@ -29,7 +29,7 @@ SCANS = [(1, 1, 1, 1, FP32, {}), (2, 15, 3, 4, FP32, dict(gate=False)), (1, 16, 
 @pytest.mark.parametrize("B,T,C,N,dtype,more", SCANS)
 def test_scan_and_gradients(B, T, C, N, dtype, more, pieces, monkeypatch):
     if pieces == "one":
-        monkeypatch.setattr(selective, "WARPS", 1)
+        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
     steps = more.get("steps", True)
     t = inputs(B, T, C, N, dtype, DEV, T + C, **more)
     with torch.no_grad():
@@ -78,7 +78,7 @@ TOKENS = [(1, 1, 64, 16, BF16, [9], [1], None), (4, 1, 130, 16, BF16, [3, 0, -1,
 @pytest.mark.parametrize("R,S,C,N,dtype,first,lengths,ids", TOKENS)
 def test_tokens_with_states(R, S, C, N, dtype, first, lengths, ids, pieces, monkeypatch):
     if pieces == "one":
-        monkeypatch.setattr(selective, "WARPS", 1)
+        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
     t, r, state = call(R, S, C, N, dtype, S + C, first, lengths, ids, strided=C % 2 == 0)
     before = state.clone()
     a_log = torch.log(-t["a"])
@@ -133,7 +133,7 @@ HEADS = [(1, 1, 4, 1, 64, 128, BF16, [5], [1], None), (3, 1, 6, 2, 48, 80, BF16,
 def test_heads_with_states(R, S, H, G, P, N, dtype, first, lengths, ids, pieces, monkeypatch):
     """A decay per head is a rate per channel and state that is one number in each head."""
     if pieces == "one":
-        monkeypatch.setattr(selective, "WARPS", 1)
+        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
     t, r, state = heads(R, S, H, G, P, N, dtype, S + H, first, lengths, ids)
     before = state.clone()
     y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], H, G, r, state)
