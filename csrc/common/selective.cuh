@@ -9,6 +9,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "special.cuh"
+
 // x, dt, z, b, c: row r, token t starts at r * row + t * token (elements).  Null where a call has none: z, d, initial, last, checkpoints, starts, sums, positions, lengths, row_ids.
 // With `heads` > 0 a channel is one of heads * dim, and the decay (a, dt, dt_bias, d) is a head's.
 extern "C" struct dewb_selective_args {
@@ -23,7 +25,7 @@ extern "C" struct dewb_selective_args {
   const int *positions, *lengths, *row_ids;
   int R, T, C, N, groups, heads, segments, segment, padded, states_each;      // `padded`: channels of a group in checkpoints, starts and sums, a multiple of 128 (with heads, of 256);
                                        // `states_each`:
-                                       // states of a lane where there are up to 16 (1, 2 or 4)
+                                       // states of a lane where there are up to 16 (1, 2 or 4); of token_kernel, rows of a block
   int softplus, log_a, dt_fp32, stored;      // `stored`: rows of the store, where row_ids or positions name them
   int* status;                         // told of a row outside the store, which then has no tokens
 };
@@ -37,7 +39,11 @@ using Args = dewb_selective_args;
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int OUTSIDE = 6;             // the status of a row that the store does not have
 constexpr int EVERY = 16;              // tokens between two kept states
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LN2 = 0.6931471805599453f;
+using special::ex2;
+using special::LOG2E;
+using special::rcp;
+using special::sigmoid;
 
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
@@ -52,16 +58,6 @@ struct Lay {
   static constexpr int PASSES = TT >= LN ? TT / LN : 1;      // a lane's pieces of four channels in a tile: token lane / CG + pass * LN
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // ln(1 + e^x) = max(x, 0) + ln(1 + t), t = e^-|x|: with q = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh q = 2 (q + q^3 / 3 + ... + q^13 / 13), the next term below 2e-8 of the sum
 __device__ __forceinline__ float softplus(float x) {
   const float t = ex2(-LOG2E * fabsf(x)), q = t * rcp(2.f + t), r = q * q;
@@ -73,7 +69,6 @@ __device__ __forceinline__ float softplus(float x) {
   p = fmaf(p, r, 1.f);
   return fmaf(2.f * q, p, fmaxf(x, 0.f));
 }
-__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-LOG2E * x)); }
 
 // Two fp32 numbers side by side, of two neighbouring channels: one instruction for both.
 struct f2 {

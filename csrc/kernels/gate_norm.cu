@@ -4,24 +4,26 @@
 //
 // Bound by memory: a row's values are read once and stay in registers between the sums and the results (`ITEMS` pieces of V values a thread; ITEMS 0, for rows that are longer or lie
 // askew, reads them again).  The backward forms r anew from what it reads anyway, in the same reduction as mean(g u), so the forward keeps nothing.  A row belongs to a warp (up to
-// 32 V ITEMS values) or to a block; in the backward a block walks rows with its columns' dw in registers, and its sums leave as one part, added up in one order by weight_sum_kernel.
+// 32 V ITEMS values) or to a block of NT threads; in the backward a block walks rows with its columns' dw in registers, and its sums leave as one part, added up in one order by
+// weight_sum_kernel.  There values stay as they lie in memory (half the registers in bf16) and the next row is on its way while one is summed: 8192 rows of 8192 DEWB_NORM.
 // Values are bf16 or fp32 (template T; w either), sums fp32.  Compiled without fast math.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include "../common/rows.cuh"
+#include "../common/special.cuh"
 
 namespace dewb {
 namespace gatenorm {
 
 using namespace rows;
+using special::sigmoid;
 
-constexpr int THREADS = 256, WARPS = 8;
+constexpr int THREADS = 256, WARPS = 8;       // of rows that belong to a warp, and of what is read twice
 
 __device__ __forceinline__ void st(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st(bf16* p, float v) { *p = __float2bfloat16(v); }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
 
 struct Args {
   const void *x, *z, *w, *dy;          // [rows, d]; x, z and dy at strides of their own
@@ -52,7 +54,7 @@ __device__ __forceinline__ void load_w(const Args& p, int c, float (&f)[V], cons
 }
 
 // The sums of two numbers over a row's threads.
-template <bool WARP>
+template <bool WARP, int NT>
 __device__ __forceinline__ float2 row_sum(float a, float b, float2* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
@@ -62,15 +64,15 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2* red) {
   __syncthreads();
   float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i) { s.x += red[i].x; s.y += red[i].y; }
+  for (int i = 0; i < NT / 32; ++i) { s.x += red[i].x; s.y += red[i].y; }
   return s;
 }
 
-template <typename T, int V, int ITEMS, bool WARP>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int V, int ITEMS, bool WARP, int NT>
+__global__ void __launch_bounds__(NT)
 gate_norm_kernel(const Args p) {
-  __shared__ float2 red[WARPS];
-  constexpr int N = WARP ? 32 : THREADS;
+  __shared__ float2 red[NT / 32];
+  constexpr int N = WARP ? 32 : NT;
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x;
   const long long row = WARP ? static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP && row >= p.rows) return;
@@ -102,7 +104,7 @@ gate_norm_kernel(const Args p) {
       for (int j = 0; j < V; ++j) ss += kept[0][j] * kept[0][j];
     }
   }
-  const float r = 1.f / sqrtf(row_sum<WARP>(ss, 0.f, red).x / p.d + p.eps);
+  const float r = 1.f / sqrtf(row_sum<WARP, NT>(ss, 0.f, red).x / p.d + p.eps);
   auto finish = [&](int c, float (&u)[V]) {
     float w[V];
     load_w<V>(p, c, w, static_cast<const T*>(nullptr));
@@ -124,91 +126,87 @@ gate_norm_kernel(const Args p) {
   }
 }
 
-// grid: blocks that walk the rows.  dw stays in registers; with ITEMS 0, in the block's own part.
-template <typename T, int V, int ITEMS, bool WARP>
-__global__ void __launch_bounds__(THREADS)
+// V values as they lie in memory.
+template <typename T, int V>
+struct Raw {
+  static constexpr int WORDS = V * sizeof(T) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+    static_assert(WORDS == 4, "pieces of 16 bytes");
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  }
+  __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0u; }
+  __device__ __forceinline__ float operator[](int j) const {
+    return sizeof(T) == 4 ? __uint_as_float(w[j]) : __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+};
+
+// grid: blocks that walk the rows, with dw in registers.
+template <typename T, int V, int ITEMS, bool WARP, int NT>
+__global__ void __launch_bounds__(NT)
 gate_norm_grad_kernel(const Args p) {
-  __shared__ float2 red[WARPS];
-  __shared__ float add[WARP ? WARPS : 1][WARP ? 32 * V * (ITEMS > 0 ? ITEMS : 1) : 1];
-  constexpr int N = WARP ? 32 : THREADS;
+  __shared__ float2 red[NT / 32];
+  __shared__ float add[WARP ? WARPS : 1][WARP ? 32 * V * ITEMS : 1];
+  constexpr int N = WARP ? 32 : NT;
   const int lane = WARP ? threadIdx.x & 31 : threadIdx.x;
   const long long step = static_cast<long long>(gridDim.x) * (WARP ? WARPS : 1);
   float* part = p.parts + static_cast<long long>(blockIdx.x) * p.d;
-  float dw[ITEMS > 0 ? ITEMS : 1][V], w[ITEMS > 0 ? ITEMS : 1][V];
+  float dw[ITEMS][V];
 #pragma unroll
-  for (int i = 0; i < (ITEMS > 0 ? ITEMS : 1); ++i)
+  for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = w[i][j] = 0.f;
-  if constexpr (ITEMS > 0) {
+    for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
+  struct Row { Raw<T, V> x, z, dy; } now[ITEMS], next[ITEMS];
+  auto bring = [&](Row (&r)[ITEMS], long long row) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
-      if ((i * N + lane) * V < p.d) load_w<V>(p, (i * N + lane) * V, w[i], static_cast<const T*>(nullptr));
-  } else {
-    for (int c = lane * V; c < p.d; c += N * V)
-#pragma unroll
-      for (int j = 0; j < V; ++j) part[c + j] = 0.f;
-  }
-  for (long long row = WARP ? static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5) : blockIdx.x; row < p.rows; row += step) {
-    const T *x = static_cast<const T*>(p.x) + row * p.x_row, *z = static_cast<const T*>(p.z) + row * p.z_row, *dy = static_cast<const T*>(p.dy) + row * p.dy_row;
-    T *dx = static_cast<T*>(p.dx) + row * p.d, *dz = static_cast<T*>(p.dz) + row * p.d;
-    float xs[ITEMS > 0 ? ITEMS : 1][V], zs[ITEMS > 0 ? ITEMS : 1][V], gs[ITEMS > 0 ? ITEMS : 1][V];
-    float ss = 0.f, gu = 0.f;
-    auto bring = [&](int c, float (&a)[V], float (&b)[V], float (&e)[V]) { load_v<V>(x + c, a); load_v<V>(z + c, b); load_v<V>(dy + c, e); };
-    auto sums = [&](const float (&a)[V], const float (&b)[V], const float (&e)[V], const float (&m)[V]) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float u = a[j] * b[j] * sigmoid(b[j]);
-        ss += u * u;
-        gu += e[j] * m[j] * u;
-      }
-    };
-    if constexpr (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const int c = (i * N + lane) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) xs[i][j] = zs[i][j] = gs[i][j] = 0.f;
-        if (c < p.d) bring(c, xs[i], zs[i], gs[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) sums(xs[i], zs[i], gs[i], w[i]);
-    } else {
-      for (int c = lane * V; c < p.d; c += N * V) {
-        bring(c, xs[0], zs[0], gs[0]);
-        load_w<V>(p, c, w[0], static_cast<const T*>(nullptr));
-        sums(xs[0], zs[0], gs[0], w[0]);
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * N + lane) * V;
+      if (c < p.d && row < p.rows) {
+        r[i].x.load(static_cast<const T*>(p.x) + row * p.x_row + c);
+        r[i].z.load(static_cast<const T*>(p.z) + row * p.z_row + c);
+        r[i].dy.load(static_cast<const T*>(p.dy) + row * p.dy_row + c);
+      } else {
+        r[i].x.zero(); r[i].z.zero(); r[i].dy.zero();
       }
     }
-    const float2 s = row_sum<WARP>(ss, gu, red);
-    const float r = 1.f / sqrtf(s.x / p.d + p.eps), back = r * r * r * (s.y / p.d);
-    auto finish = [&](int c, const float (&a)[V], const float (&b)[V], const float (&e)[V], const float (&m)[V], float (&sum)[V]) {
-      float ox[V], oz[V];
+  };
+  long long row = WARP ? static_cast<long long>(blockIdx.x) * WARPS + (threadIdx.x >> 5) : blockIdx.x;
+  bring(next, row);
+  for (; row < p.rows; row += step) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) now[i] = next[i];
+    bring(next, row + step);
+    float ss = 0.f, gu = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * N + lane) * V;
+      float w[V];
+      if (c < p.d) load_w<V>(p, c, w, static_cast<const T*>(nullptr));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float sig = sigmoid(b[j]), gate = b[j] * sig, u = a[j] * gate, du = r * e[j] * m[j] - u * back;
-        sum[j] += e[j] * u * r;
+        const float z = now[i].z[j], u = now[i].x[j] * z * sigmoid(z);
+        ss = fmaf(u, u, ss);
+        if (c < p.d) gu = fmaf(now[i].dy[j] * w[j], u, gu);
+      }
+    }
+    const float2 s = row_sum<WARP, NT>(ss, gu, red);
+    const float r = 1.f / sqrtf(s.x / p.d + p.eps), back = r * r * r * (s.y / p.d);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = (i * N + lane) * V;
+      if (c >= p.d) continue;
+      float w[V], ox[V], oz[V];
+      load_w<V>(p, c, w, static_cast<const T*>(nullptr));
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = now[i].x[j], z = now[i].z[j], e = now[i].dy[j] * r, sig = sigmoid(z), gate = z * sig, u = x * gate, du = e * w[j] - u * back;
+        dw[i][j] = fmaf(e, u, dw[i][j]);
         ox[j] = du * gate;
-        oz[j] = du * a[j] * sig * fmaf(b[j], 1.f - sig, 1.f);
+        oz[j] = du * x * sig * fmaf(z, 1.f - sig, 1.f);
       }
-      store_v<V>(dx + c, ox);
-      store_v<V>(dz + c, oz);
-    };
-    if constexpr (ITEMS > 0) {
-#pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const int c = (i * N + lane) * V;
-        if (c < p.d) finish(c, xs[i], zs[i], gs[i], w[i], dw[i]);
-      }
-    } else {
-      for (int c = lane * V; c < p.d; c += N * V) {
-        bring(c, xs[0], zs[0], gs[0]);
-        load_w<V>(p, c, w[0], static_cast<const T*>(nullptr));
-#pragma unroll
-        for (int j = 0; j < V; ++j) dw[0][j] = part[c + j];
-        finish(c, xs[0], zs[0], gs[0], w[0], dw[0]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) part[c + j] = dw[0][j];
-      }
+      store_v<V>(static_cast<T*>(p.dx) + row * p.d + c, ox);
+      store_v<V>(static_cast<T*>(p.dz) + row * p.d + c, oz);
     }
   }
   if constexpr (WARP) {
@@ -217,16 +215,61 @@ gate_norm_grad_kernel(const Args p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) add[threadIdx.x >> 5][(i * 32 + lane) * V + j] = dw[i][j];
     __syncthreads();
-    for (int c = threadIdx.x; c < p.d; c += THREADS) {
+    for (int c = threadIdx.x; c < p.d; c += NT) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < WARPS; ++i) s += add[i][c];
       part[c] = s;
     }
-  } else if constexpr (ITEMS > 0) {
+  } else {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
       if ((i * N + lane) * V < p.d) store_v<V>(part + (i * N + lane) * V, dw[i]);
+  }
+}
+
+// The same for rows of any length and place, read twice; dw in the block's own part.
+template <typename T, int V>
+__global__ void __launch_bounds__(THREADS)
+gate_norm_grad_twice_kernel(const Args p) {
+  __shared__ float2 red[WARPS];
+  float* part = p.parts + static_cast<long long>(blockIdx.x) * p.d;
+  for (int c = threadIdx.x * V; c < p.d; c += THREADS * V)
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[c + j] = 0.f;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T *x = static_cast<const T*>(p.x) + row * p.x_row, *z = static_cast<const T*>(p.z) + row * p.z_row, *dy = static_cast<const T*>(p.dy) + row * p.dy_row;
+    float ss = 0.f, gu = 0.f, a[V], b[V], e[V], w[V];
+    auto bring = [&](int c) {
+      load_v<V>(x + c, a);
+      load_v<V>(z + c, b);
+      load_v<V>(dy + c, e);
+      load_w<V>(p, c, w, static_cast<const T*>(nullptr));
+    };
+    for (int c = threadIdx.x * V; c < p.d; c += THREADS * V) {
+      bring(c);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float u = a[j] * b[j] * sigmoid(b[j]);
+        ss = fmaf(u, u, ss);
+        gu = fmaf(e[j] * w[j], u, gu);
+      }
+    }
+    const float2 s = row_sum<false, THREADS>(ss, gu, red);
+    const float r = 1.f / sqrtf(s.x / p.d + p.eps), back = r * r * r * (s.y / p.d);
+    for (int c = threadIdx.x * V; c < p.d; c += THREADS * V) {
+      float ox[V], oz[V];
+      bring(c);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float sig = sigmoid(b[j]), gate = b[j] * sig, u = a[j] * gate, du = r * e[j] * w[j] - u * back;
+        part[c + j] += e[j] * u * r;
+        ox[j] = du * gate;
+        oz[j] = du * a[j] * sig * fmaf(b[j], 1.f - sig, 1.f);
+      }
+      store_v<V>(static_cast<T*>(p.dx) + row * p.d + c, ox);
+      store_v<V>(static_cast<T*>(p.dz) + row * p.d + c, oz);
+    }
   }
 }
 
@@ -248,14 +291,16 @@ weight_sum_kernel(const float* __restrict__ parts, int n, int d, W* __restrict__
   }
 }
 
-template <typename T, int V, int ITEMS, bool WARP>
+template <typename T, int V, int ITEMS, bool WARP, int NT>
 int go(const Args& p, int blocks, cudaStream_t stream) {
   if (p.dy == nullptr) {
     const long long grid = WARP ? (p.rows + WARPS - 1) / WARPS : p.rows;
     if (grid > 0x7fffffffLL) return -3;
-    gate_norm_kernel<T, V, ITEMS, WARP><<<static_cast<unsigned>(grid), THREADS, 0, stream>>>(p);
+    gate_norm_kernel<T, V, ITEMS, WARP, NT><<<static_cast<unsigned>(grid), NT, 0, stream>>>(p);
+  } else if constexpr (ITEMS > 0) {
+    gate_norm_grad_kernel<T, V, ITEMS, WARP, NT><<<blocks, NT, 0, stream>>>(p);
   } else {
-    gate_norm_grad_kernel<T, V, ITEMS, WARP><<<blocks, THREADS, 0, stream>>>(p);
+    gate_norm_grad_twice_kernel<T, V><<<blocks, THREADS, 0, stream>>>(p);
   }
   return static_cast<int>(cudaGetLastError());
 }
@@ -264,13 +309,14 @@ template <typename T>
 int any(const Args& p, int blocks, cudaStream_t stream) {
   constexpr int V = sizeof(T) == 2 ? 8 : 4;
   const bool whole = p.d % V == 0 && (p.x_row | p.z_row | p.dy_row) % V == 0 && aligned(p.x, 16) && aligned(p.z, 16) && aligned(p.dy, 16) && aligned(p.w, 16);
-  if (!whole) return go<T, 1, 0, false>(p, blocks, stream);
-  if (p.d <= 32 * V) return go<T, V, 1, true>(p, blocks, stream);
-  if (p.d <= 64 * V) return go<T, V, 2, true>(p, blocks, stream);
-  if (p.d <= THREADS * V) return go<T, V, 1, false>(p, blocks, stream);
-  if (p.d <= 2 * THREADS * V) return go<T, V, 2, false>(p, blocks, stream);
-  if (p.d <= 4 * THREADS * V) return go<T, V, 4, false>(p, blocks, stream);
-  return go<T, V, 0, false>(p, blocks, stream);
+  if (!whole) return go<T, 1, 0, false, THREADS>(p, blocks, stream);
+  if (p.d <= 32 * V) return go<T, V, 1, true, THREADS>(p, blocks, stream);
+  if (p.d <= 64 * V) return go<T, V, 2, true, THREADS>(p, blocks, stream);
+  if (p.d <= 128 * V) return go<T, V, 1, false, 128>(p, blocks, stream);
+  if (p.d <= 256 * V) return go<T, V, 2, false, 128>(p, blocks, stream);
+  if (p.d <= 512 * V) return go<T, V, 2, false, 256>(p, blocks, stream);
+  if (p.d <= 1024 * V) return go<T, V, 2, false, 512>(p, blocks, stream);
+  return go<T, V, 0, false, THREADS>(p, blocks, stream);
 }
 
 inline bool ok(const void* x, const void* z, const void* w, long long rows, int d) { return x != nullptr && z != nullptr && w != nullptr && rows > 0 && d > 0; }

@@ -81,77 +81,86 @@ struct Place {
     }
   }
   template <bool FAST>
-  __device__ __forceinline__ void bring(const Grad& g, int t0, int t_end) {
-#pragma unroll
-    for (int i = 0; i < L::PASSES; ++i) {
-      const int t = t0 + lt + i * LN, n = lt < TT && t < t_end ? left : 0;
-      if (!FAST || LN <= TT || lt < TT) {
-        if (STATES) rx[i] = fetch(x + t * g.f.x_token, FAST, n);
-        rd[i] = fetch(dt + t * g.f.dt_token, FAST, n);
-        ry[i] = fetch(dy + t * g.dy_token, FAST, n);
-        if (z != nullptr) rz[i] = fetch(z + t * g.f.z_token, FAST, n);
-      }
+  __device__ __forceinline__ void bring(const Grad& g, int i, int t0, int t_end) {
+    const int t = t0 + lt + i * LN, n = lt < TT && t < t_end ? left : 0;
+    const bool four = FAST || (whole && n == 4);
+    if (!FAST || LN <= TT || lt < TT) {
+      if (STATES) rx[i] = fetch(x + t * g.f.x_token, four, n);
+      rd[i] = fetch(dt + t * g.f.dt_token, four, n);
+      ry[i] = fetch(dy + t * g.dy_token, four, n);
+      if (z != nullptr) rz[i] = fetch(z + t * g.f.z_token, four, n);
     }
   }
   __device__ __forceinline__ void bring(const Grad& g, int t0, int t_end) {
-    if (whole && t0 + TT <= t_end) bring<true>(g, t0, t_end);
-    else bring<false>(g, t0, t_end);
+    if (whole && t0 + TT <= t_end) {
+#pragma unroll
+      for (int i = 0; i < L::PASSES; ++i) bring<true>(g, i, t0, t_end);
+    } else {
+#pragma unroll
+      for (int i = 0; i < L::PASSES; ++i) bring<false>(g, i, t0, t_end);
+    }
   }
 };
 
-// What a block has of a tile's B and C.
+// What a block has of a tile's B and C, four states of a token a piece.
 template <typename T, int LN, int NS, bool STATES>
 struct Narrow {
   using L = Lay<LN, NS>;
-  static constexpr int EACH = (TT * L::NP + THREADS - 1) / THREADS;
-  uint32_t b[STATES ? EACH : 1], c[EACH];
-  __device__ __forceinline__ void bring(const Args& p, int row, int t0, int t_end) {
-    const T *pb = static_cast<const T*>(p.b) + row * p.b_row, *pc = static_cast<const T*>(p.c) + row * p.c_row;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int at = threadIdx.x + i * THREADS, t = t0 + at / L::NP, n = at % L::NP;
-      const bool on = t < t_end && n < p.N;
-      if (STATES) b[i] = on ? word(pb + t * p.b_token + n) : 0u;
-      c[i] = on ? word(pc + t * p.c_token + n) : 0u;
+  static constexpr int ALL = TT * L::NP / 4, EACH = (ALL + THREADS - 1) / THREADS;
+  Raw<T> b[STATES ? EACH : 1], c[EACH];
+  const T *pb, *pc;
+  bool b_whole, c_whole;
+  __device__ __forceinline__ Narrow(const Args& p, int row) {
+    pb = static_cast<const T*>(p.b) + row * p.b_row;
+    pc = static_cast<const T*>(p.c) + row * p.c_row;
+    b_whole = fours<T>(pb, p.b_row, p.b_token);
+    c_whole = fours<T>(pc, p.c_row, p.c_token);
+  }
+  __device__ __forceinline__ void bring(const Args& p, int i, int t0, int t_end) {
+    const int at = threadIdx.x + i * THREADS, t = t0 + at / (L::NP / 4), n = at % (L::NP / 4) * 4;
+    const int there = at < ALL && t < t_end ? max(0, min(4, p.N - n)) : 0;
+    if (STATES) b[i] = fetch(pb + t * p.b_token + n, b_whole && there == 4, there);
+    c[i] = fetch(pc + t * p.c_token + n, c_whole && there == 4, there);
+  }
+  __device__ __forceinline__ void put(Shared<LN, NS>& sm, int i) const {
+    const int at = threadIdx.x + i * THREADS, t = at / (L::NP / 4), n = at % (L::NP / 4) * 4;
+    if (ALL % THREADS == 0 || at < ALL) {
+      if (STATES) twice(&sm.b[t][n], b[i]);
+      twice(&sm.c[t][n], c[i]);
     }
+  }
+  __device__ __forceinline__ void bring(const Args& p, int t0, int t_end) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) bring(p, i, t0, t_end);
   }
   __device__ __forceinline__ void put(Shared<LN, NS>& sm) const {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      const int at = threadIdx.x + i * THREADS;
-      const float cf = value<T>(c[i]), bf = STATES ? value<T>(b[i]) : 0.f;
-      if (STATES) sm.b[at / L::NP][at % L::NP] = make_float2(bf, bf);
-      sm.c[at / L::NP][at % L::NP] = make_float2(cf, cf);
-    }
+    for (int i = 0; i < EACH; ++i) put(sm, i);
   }
 };
 
-// s, u and w of the warp's channels from what the lanes have brought; behind t_end and the last channel, zeros.
+// s, u and w of the warp's channels from what the lanes have brought, pass i; behind t_end and the last channel, zeros.
 template <typename T, typename TD, int LN, int NS, bool STATES>
-__device__ __forceinline__ void stage(Shared<LN, NS>& sm, const Place<T, TD, LN, NS, STATES>& at, bool steps, int t0, int t_end, int warp, float (&total)[4]) {
-  using L = Lay<LN, NS>;
+__device__ __forceinline__ void stage(Shared<LN, NS>& sm, const Place<T, TD, LN, NS, STATES>& at, bool steps, int i, int t0, int t_end, int warp, float (&total)[4]) {
   const bool all = t0 + TT <= t_end && at.left == 4;
+  const int t = at.lt + i * LN;
+  if (LN > TT && t >= TT) return;
+  float x[4], s[4], w[4], z[4];
+  if (STATES) at.rx[i].get(x);
+  at.rd[i].get(s);
+  at.ry[i].get(w);
+  if (at.z != nullptr) at.rz[i].get(z);
 #pragma unroll
-  for (int i = 0; i < L::PASSES; ++i) {
-    const int t = at.lt + i * LN;
-    if (LN > TT && t >= TT) continue;
-    float x[4], s[4], w[4], z[4];
-    if (STATES) at.rx[i].get(x);
-    at.rd[i].get(s);
-    at.ry[i].get(w);
-    if (at.z != nullptr) at.rz[i].get(z);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (steps) s[j] = softplus(s[j]);
-      if (at.z != nullptr) w[j] *= z[j] * sigmoid(z[j]);
-      if (!all && (j >= at.left || t0 + t >= t_end)) s[j] = w[j] = 0.f;
-      if (STATES) x[j] = !all && (j >= at.left || t0 + t >= t_end) ? 0.f : s[j] * x[j];
-      total[j] += s[j];
-    }
-    *reinterpret_cast<float4*>(&sm.step[warp][t][at.lq]) = make_float4(s[0], s[1], s[2], s[3]);
-    *reinterpret_cast<float4*>(&sm.w[warp][t][at.lq]) = make_float4(w[0], w[1], w[2], w[3]);
-    if (STATES) *reinterpret_cast<float4*>(&sm.in[warp][t][at.lq]) = make_float4(x[0], x[1], x[2], x[3]);
+  for (int j = 0; j < 4; ++j) {
+    if (steps) s[j] = softplus(s[j]);
+    if (at.z != nullptr) w[j] *= z[j] * sigmoid(z[j]);
+    if (!all && (j >= at.left || t0 + t >= t_end)) s[j] = w[j] = 0.f;
+    if (STATES) x[j] = !all && (j >= at.left || t0 + t >= t_end) ? 0.f : s[j] * x[j];
+    total[j] += s[j];
   }
+  *reinterpret_cast<float4*>(&sm.step[warp][t][at.lq]) = make_float4(s[0], s[1], s[2], s[3]);
+  *reinterpret_cast<float4*>(&sm.w[warp][t][at.lq]) = make_float4(w[0], w[1], w[2], w[3]);
+  if (STATES) *reinterpret_cast<float4*>(&sm.in[warp][t][at.lq]) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
 // Numbers of four channels and NS states, channels in pairs.
@@ -204,7 +213,7 @@ __device__ __forceinline__ Block<NS> last_of(const Grad& g, int row, int c, int 
 
 // grid R * (segments - 1) * channel blocks, of segments 1, 2, ...: starts[r, j] is the gradient of the state in front of segment j that the segment itself makes (the last one: with dlast).
 template <typename T, typename TD, int LN, int NS>
-__global__ void __launch_bounds__(THREADS, 4)
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 2 : 4)
 back_ends_kernel(const Grad g) {
   using L = Lay<LN, NS>;
   using S = Shared<LN, NS>;
@@ -216,21 +225,22 @@ back_ends_kernel(const Grad g) {
   const int cb = blockIdx.x % blocks, seg = 1 + blockIdx.x / blocks % (p.segments - 1), row = blockIdx.x / blocks / (p.segments - 1);
   const int c0 = cb * L::CB + warp * L::CW, t_begin = seg * p.segment, t_end = min(p.T, t_begin + p.segment);
   Place<T, TD, LN, NS, false> at(g, row, cb * L::CB, c0, lane);
-  Narrow<T, LN, NS, false> narrow;
+  Narrow<T, LN, NS, false> narrow(p, row);
   float total[4] = {0.f, 0.f, 0.f, 0.f};
   const Block<NS> a = Block<NS>::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * NS + k, 1); });
   Block<NS> d = last_of<NS>(g, row, c0 + cg * 4, sl * NS, seg == p.segments - 1);
   int t0 = t_begin + (t_end - t_begin - 1) / TT * TT;
   at.bring(g, t0, t_end);
-  narrow.bring(p, row, t0, t_end);
+  narrow.bring(p, t0, t_end);
   for (; t0 >= t_begin; t0 -= TT) {
     __syncthreads();
-    stage<T, TD, LN, NS, false>(sm, at, p.softplus, t0, t_end, warp, total);
+#pragma unroll
+    for (int i = 0; i < L::PASSES; ++i) stage<T, TD, LN, NS, false>(sm, at, p.softplus, i, t0, t_end, warp, total);
     narrow.put(sm);
     __syncthreads();
     if (t0 > t_begin) {
       at.bring(g, t0 - TT, t_end);
-      narrow.bring(p, row, t0 - TT, t_end);
+      narrow.bring(p, t0 - TT, t_end);
     }
     const int count = min(TT, t_end - t0);
 #pragma unroll 4
@@ -291,12 +301,28 @@ grad_kernel(const Grad g) {
   auto piece = [&](const float4* q, f2& x, f2& y) { pair(&q->x, x, y); };
   auto leave = [](float4* q, f2 x, f2 y) { *reinterpret_cast<ulonglong2*>(q) = make_ulonglong2(x.v, y.v); };
   for (; t0 >= t_begin; t0 -= TT) {
-    Narrow<T, LN, NS, true> narrow;
-    at.bring(g, t0, t_end);
-    narrow.bring(p, row, t0, t_end);
     if (t0 > t_begin) at.call(g, t0 - TT, t_end);
-    stage<T, TD, LN, NS, true>(sm, at, p.softplus, t0, t_end, warp, unused);
-    narrow.put(sm);
+    Narrow<T, LN, NS, true> narrow(p, row);
+    if constexpr (sizeof(T) == 2) {               // all loads of the tile on their way together
+      at.bring(g, t0, t_end);
+      narrow.bring(p, t0, t_end);
+#pragma unroll
+      for (int i = 0; i < L::PASSES; ++i) stage<T, TD, LN, NS, true>(sm, at, p.softplus, i, t0, t_end, warp, unused);
+      narrow.put(sm);
+    } else {                                      // one after another: fp32 takes twice the registers
+#pragma unroll
+      for (int i = 0; i < L::PASSES; ++i) {
+        at.template bring<false>(g, i, t0, t_end);
+        stage<T, TD, LN, NS, true>(sm, at, p.softplus, i, t0, t_end, warp, unused);
+        asm volatile("" ::: "memory");
+      }
+#pragma unroll
+      for (int i = 0; i < narrow.EACH; ++i) {
+        narrow.bring(p, i, t0, t_end);
+        narrow.put(sm, i);
+        asm volatile("" ::: "memory");
+      }
+    }
     // (channels behind the last one have no kept states: the forward's blocks may be narrower)
     const float* before = p.checkpoints + ((static_cast<long long>(row) * kept + t0 / EVERY) * padded + c0 + cg * 4) * NP + sl * NS;
     Block<NS> h = Block<NS>::load(before, NP, p.C - c0 - cg * 4);
@@ -472,6 +498,7 @@ grad_sum_kernel(const Grad g, int blocks, int padded, int np) {
     const int q = static_cast<int>(i - tok * 2 * p.N), which = q / p.N, n = q % p.N;
     const float* v = g.bc_parts + tok * 2 * np + which * np + n;
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < blocks; ++k) s += v[k * tokens * 2 * np];
     st(static_cast<T*>(which ? g.dc : g.db) + tok * p.N + n, s);
     return;
@@ -482,6 +509,7 @@ grad_sum_kernel(const Grad g, int blocks, int padded, int np) {
     const long long c = i / p.N;
     const float* v = g.a_parts + c * np + i % p.N;
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) s += v[static_cast<long long>(k) * padded * np];
     g.da[i] = s;
     return;
@@ -489,6 +517,7 @@ grad_sum_kernel(const Grad g, int blocks, int padded, int np) {
   i -= na;
   if (i < p.C && g.dd != nullptr) {
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) s += g.d_parts[static_cast<long long>(k) * padded + i];
     g.dd[i] = s;
   }

@@ -8,10 +8,6 @@
 // Inputs and outputs are bf16 or fp32 (template T; the steps' logits either), everything else fp32.  Compiled without fast math.
 #include "../common/selective.cuh"
 
-#ifndef DEWB_EACH
-#define DEWB_EACH 8
-#define DEWB_BLOCKS 1184
-#endif
 namespace dewb {
 namespace selective {
 
@@ -260,15 +256,16 @@ scan_kernel(const Args p) {
   }
 }
 
-// One token per row; a warp owns 32 channels of `rows_each` rows, whose rates it reads once.  A lane forms the step, gate and output of channel 4 (lane / 4) + own_channel(lane % 4), and
-// holds four states of each of its group's four channels; more than 16 states go by in sixteens.  The next row's states are on their way while one is worked on.
+// One token per row; a warp owns 32 channels of `rows_each` rows, whose rates it reads once.  A lane holds four states of
+// each of channels lane / 4 + 8 j (so that a load of all lanes is 512 bytes in a row), and forms the step, gate and output of that of j = own_channel(lane % 4); more than 16 states go by
+// in sixteens.  The next row's states are on their way while one is worked on.
 // grid (ceil(C / 128), ceil(R / rows_each)).
 template <typename T, bool ONE>
 __global__ void __launch_bounds__(THREADS)
 token_kernel(const Args p, int rows_each) {
-  const int lane = threadIdx.x & 31, sl = lane & 3, c4 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 32 + (lane >> 2) * 4, c = c4 + own_channel(sl);
+  const int lane = threadIdx.x & 31, sl = lane & 3, c4 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 32 + (lane >> 2), c = c4 + 8 * own_channel(sl);
   const bool on = c < p.C, whole = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.initial) & 15) == 0;
-  if (c4 - (lane >> 2) * 4 >= p.C) return;
+  if (c4 - (lane >> 2) >= p.C) return;
   const float skip = p.d != nullptr && on ? p.d[c] : 0.f;
   float a[4][4];
   auto rates = [&](int n0) {
@@ -276,53 +273,54 @@ token_kernel(const Args p, int rows_each) {
     const bool all = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && n < p.N;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int there = c4 + j < p.C ? max(0, min(4, p.N - n)) : 0;
-      fetch(p.a + static_cast<long long>(c4 + j) * p.N + n, all && there == 4, there).get(a[j]);
+      const int there = c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
+      fetch(p.a + static_cast<long long>(c4 + 8 * j) * p.N + n, all && there == 4, there).get(a[j]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) a[j][k] = k < there ? (p.log_a ? -expf(a[j][k]) : a[j][k]) * LOG2E : 0.f;
     }
   };
+  const bool b_whole = (p.N & 3) == 0 && fours<T>(p.b, p.b_row, 0), c_whole = (p.N & 3) == 0 && fours<T>(p.c, p.c_row, 0);
+  const int first = blockIdx.y * rows_each, rows = min(rows_each, p.R - first);
+  // the rows' places, a lane each: what a row's loads begin with is there before its turn
+  const Row mine = lane < rows ? row_of(p, first + lane) : Row{0, false, 0};
   struct Item {
-    Row r;
+    int len;
     bool held;
     float* state;
     Raw<float> h[4];
-    float x, s, g, b[4], c[4];
+    Raw<T> b, c;
+    float x, s, g;
   };
   auto states = [&](Item& it, int n0) {
     const int n = n0 + sl * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int there = it.held && c4 + j < p.C ? max(0, min(4, p.N - n)) : 0;
-      it.h[j] = fetch(it.state + static_cast<long long>(j) * p.N + n, whole && there == 4, there);
+      const int there = it.held && c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
+      it.h[j] = fetch(it.state + static_cast<long long>(8 * j) * p.N + n, whole && there == 4, there);
     }
   };
-  auto bring = [&](Item& it, int row) {
-    it.r = row_of(p, row);
-    it.held = it.r.len > 0 && it.r.held;
-    it.state = p.last + (it.r.at * p.C + c4) * p.N;
+  auto narrow = [&](Item& it, int row, int n0) {
+    const int n = n0 + sl * 4, there = max(0, min(4, p.N - n));
+    it.b = fetch(static_cast<const T*>(p.b) + row * p.b_row + n, b_whole && there == 4, there);
+    it.c = fetch(static_cast<const T*>(p.c) + row * p.c_row + n, c_whole && there == 4, there);
+  };
+  auto bring = [&](Item& it, int i) {
+    const int row = first + i;
+    it.len = __shfl_sync(0xffffffffu, mine.len, i);
+    it.held = __shfl_sync(0xffffffffu, mine.held, i) && it.len > 0;
+    it.state = p.last + (static_cast<long long>(__shfl_sync(0xffffffffu, static_cast<int>(mine.at), i)) * p.C + c4) * p.N;
     it.x = it.s = it.g = 0.f;
-    if (it.r.len > 0 && on) {
+    if (it.len > 0 && on) {
       it.x = ld(static_cast<const T*>(p.x) + row * p.x_row + c);
       it.s = p.dt_fp32 ? static_cast<const float*>(p.dt)[row * p.dt_row + c] : ld(static_cast<const bf16*>(p.dt) + row * p.dt_row + c);
       if (p.z != nullptr) it.g = ld(static_cast<const T*>(p.z) + row * p.z_row + c);
     }
     states(it, 0);
+    if (ONE) narrow(it, row, 0);
   };
-  auto narrow = [&](Item& it, int row, int n0) {
-    const T *b = static_cast<const T*>(p.b) + row * p.b_row, *cc = static_cast<const T*>(p.c) + row * p.c_row;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = n0 + sl * 4 + k;
-      it.b[k] = n < p.N ? ld(b + n) : 0.f;
-      it.c[k] = n < p.N ? ld(cc + n) : 0.f;
-    }
-  };
-  if (ONE) rates(0);
-  const int first = blockIdx.y * rows_each, end = min(p.R, first + rows_each);
   auto work = [&](Item& it, int row) {
     T* y = static_cast<T*>(p.y) + static_cast<long long>(row) * p.C + c;
-    if (it.r.len == 0) {
+    if (it.len == 0) {
       if (on) st(y, 0.f);
       return;
     }
@@ -333,8 +331,11 @@ token_kernel(const Args p, int rows_each) {
       if (!ONE) {
         rates(n0);
         if (n0 > 0) states(it, n0);
+        narrow(it, row, n0);
       }
-      if (!ONE) narrow(it, row, n0);
+      float b[4], cv[4];
+      it.b.get(b);
+      it.c.get(cv);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int from = (lane & ~3) + (j >> 1) + (j & 1) * 2;                     // the lane whose own channel j is
@@ -343,10 +344,10 @@ token_kernel(const Args p, int rows_each) {
         it.h[j].get(h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          h[k] = fmaf(ex2(sj * a[j][k]), h[k], uj * it.b[k]);
-          out[j] = fmaf(h[k], it.c[k], out[j]);
+          h[k] = fmaf(ex2(sj * a[j][k]), h[k], uj * b[k]);
+          out[j] = fmaf(h[k], cv[k], out[j]);
         }
-        if (c4 + j < p.C) put(it.state + static_cast<long long>(j) * p.N + n, h, whole && n < p.N, p.N - n);
+        if (c4 + 8 * j < p.C) put(it.state + static_cast<long long>(8 * j) * p.N + n, h, whole && n < p.N, p.N - n);
       }
       if (ONE) break;
     }
@@ -355,15 +356,12 @@ token_kernel(const Args p, int rows_each) {
     if (on) st(y, o);
   };
   Item now, next;
-  bring(now, first);
-  if (ONE) narrow(now, first, 0);
-  for (int row = first; row < end; ++row) {
-    if (row + 1 < end) {
-      bring(next, row + 1);
-      if (ONE) narrow(next, row + 1, 0);
-    }
-    work(now, row);
+  bring(next, 0);
+  if (ONE) rates(0);
+  for (int i = 0; i < rows; ++i) {
     now = next;
+    if (i + 1 < rows) bring(next, i + 1);
+    work(now, first + i);
   }
 }
 
@@ -396,10 +394,7 @@ int scan_any(const Args& p, cudaStream_t stream) {
 
 template <typename T>
 int token_any(const Args& p, cudaStream_t stream) {
-  const int across = (p.C + THREADS - 1) / THREADS;
-  // rows that share a block's rates, as long as there are blocks for every SM (128 rows of 8192 channels, 1, 2, 4, 8, 16 rows: DEWB_ROWS us)
-  const long long most = static_cast<long long>(across) * p.R / DEWB_BLOCKS;
-  const int rows_each = static_cast<int>(most < 1 ? 1 : most > DEWB_EACH ? DEWB_EACH : most);
+  const int across = (p.C + THREADS - 1) / THREADS, rows_each = p.states_each;
   const dim3 grid(across, (p.R + rows_each - 1) / rows_each);
   if (grid.y > 65535) return -3;
   if (p.N <= 16) token_kernel<T, true><<<grid, THREADS, 0, stream>>>(p, rows_each);
@@ -421,7 +416,7 @@ extern "C" int dewb_selective_scan(const dewb_selective_args* a, int fp32, void*
 
 // One token per row, with positions and a state.
 extern "C" int dewb_selective_token(const dewb_selective_args* a, int fp32, void* stream_ptr) {
-  if (a == nullptr || a->heads != 0 || !args_ok(*a) || a->T != 1 || a->positions == nullptr || a->last == nullptr) return -3;
+  if (a == nullptr || a->heads != 0 || !args_ok(*a) || a->T != 1 || a->positions == nullptr || a->last == nullptr || a->states_each < 1 || a->states_each > 32) return -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   return fp32 ? token_any<float>(*a, stream) : token_any<bf16>(*a, stream);
 }

@@ -8,7 +8,13 @@ import torch.nn.functional as F
 
 from . import library as L
 
-BLOCKS = 148 * 4         # that walk the rows of a backward, at most
+
+
+def _blocks(rows: int, row_bytes: int) -> int:
+    """Blocks that walk the rows of a backward: as many as an SM holds of them (8192 rows of 1024 bf16 values: 148, 296, 592, 1184 blocks 64, 39, 29, 34 us with the sum of their parts)."""
+    if row_bytes <= 1024:                  # a row a warp
+        return max(1, min(148, -(-rows // 8)))
+    return min(rows, 148 * (4 if row_bytes <= 4096 or row_bytes > 16384 else 2 if row_bytes <= 8192 else 1))
 
 
 def plain(x, z, w, eps: float) -> torch.Tensor:
@@ -24,7 +30,7 @@ def kernel_available(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor) -> bool:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t [..., d]`` as rows, each in one piece (a view of a wider tensor is one already)."""
-    t = t.reshape(-1, t.shape[-1])
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -43,7 +49,7 @@ def _backward(x, z, w, eps: float, dy):
     x2, z2, w, dy2 = _rows(x), _rows(z), w.contiguous(), _rows(dy.to(x.dtype))
     rows, d = x2.shape
     dx, dz, dw = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, z, w))
-    blocks = min(BLOCKS, rows)
+    blocks = _blocks(rows, d * x.element_size())
     parts = torch.empty(blocks, d, dtype=torch.float32, device=x.device)
     with L.on_device_of(x) as stream:
         L.check(L.load().dewb_gate_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), dx.data_ptr(), dz.data_ptr(),

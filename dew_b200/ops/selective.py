@@ -56,29 +56,39 @@ def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward
     return -(-(-(-T // pieces)) // EVERY) * EVERY, each
 
 
+def _rows_each(R: int, C: int) -> int:
+    """Rows of a step whose rates a block of 128 channels reads once: so many that all blocks are on the GPU together, five an SM (128 rows of 8192 channels, 1, 4, 8, 12, 16 rows: 54, 36,
+    38, 32, 36 us; 32 rows of 4096, 1, 2, 4 rows: 10.8, 8.7, 11.2)."""
+    return max(1, min(32, -(-R * -(-C // 128) // 740)))
+
+
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """``t [R, T, n]`` with its last axis in one piece."""
     return t if t is None or t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _rows(t: Optional[torch.Tensor]):
-    """Address, and row and token strides (0 where there is one of them)."""
-    return (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+def _strides(t: torch.Tensor):
+    """Row and token strides (0 where there is one of them)."""
+    shape, (row, token, _) = t.shape, t.stride()
+    return row if shape[0] > 1 else 0, token if shape[1] > 1 else 0
 
 
-def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0, backward: bool = False):
+def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0,
+          token: bool = False, backward: bool = False):
     """The arguments of a launch, and what has to live until it is issued."""
     R, T, C = x.shape
     channels, states, _ = _padded(C, N, groups, heads)
-    segment, each = _split(R, T, C, N, groups, heads, backward)
+    segment, each = (EVERY, _rows_each(R, C)) if token else _split(R, T, C, N, groups, heads, backward)
     segments = -(-T // segment)
     work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device) if segments > 1 else None
-    starts = L.at(work)
-    (px, *sx), (pd, *sd), (pz, *sz), (pb, *sb), (pc, *sc) = (_rows(t) for t in (x, dt, z, b, c))
-    at = (0, 0, 0) if rows is None else (rows.positions.data_ptr(), rows.lengths.data_ptr(), L.at(rows.row_ids))
-    args = _Args(px, pd, pz, pb, pc, *sx, *sd, *sz, *sb, *sc, a.data_ptr(), L.at(dt_bias), L.at(d), L.at(initial), L.at(last), L.at(y), L.at(checkpoints), starts,
-                 starts + 4 * R * segments * channels * states if work is not None else 0, *at, R, T, C, N, groups, heads, segments, segment, channels // groups, each, int(softplus), int(log_a),
-                 int(dt.dtype is torch.float32), stored, L.status(x.device).data_ptr())
+    starts, sums = (work.data_ptr(), work.data_ptr() + 4 * R * segments * channels * states) if segments > 1 else (0, 0)
+    at, positions, lengths, ids = L.at, 0, 0, 0
+    if rows is not None:
+        positions, lengths, ids = rows.positions.data_ptr(), rows.lengths.data_ptr(), at(rows.row_ids)
+    z_row, z_token = (0, 0) if z is None else _strides(z)
+    args = _Args(x.data_ptr(), dt.data_ptr(), at(z), b.data_ptr(), c.data_ptr(), *_strides(x), *_strides(dt), z_row, z_token, *_strides(b), *_strides(c), a.data_ptr(), at(dt_bias), at(d),
+                 at(initial), at(last), at(y), at(checkpoints), starts, sums, positions, lengths, ids, R, T, C, N, groups, heads, segments, segment, channels // groups, each, softplus, log_a,
+                 dt.dtype is torch.float32, stored, L.status(x.device).data_ptr())
     return args, work
 
 
@@ -115,16 +125,15 @@ def _backward(x, dt, a, b, c, d, z, initial, kept, softplus: bool, dy, dlast):
     R, T, C = x.shape
     N, dev = a.shape[1], x.device
     channels, states, wide = _padded(C, N)
-    f32 = dict(dtype=torch.float32, device=dev)
     like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
     dx, ddt, dz, db, dc, da, dd, dinitial = like(x), like(dt), like(z), like(b), like(c), like(a), like(d), like(initial)
     with L.on_device_of(x) as stream:
         args, work = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False, backward=True)
-        bc = torch.empty(-(-C // (wide * args.states_each)), R * T, 2, states, **f32)
-        parts = torch.empty(R * args.segments, channels, states + 1, **f32)
-        at, row, token = _rows(dy)
-        grad = _Grad(args, at, row, token, *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial, bc, parts)),
-                     parts.data_ptr() + 4 * R * args.segments * channels * states)
+        # one piece of scratch: parts of dB and dC per channel block, of dA and of dD per row and piece
+        of_bc, of_a = -(-C // (wide * args.states_each)) * R * T * 2 * states, R * args.segments * channels * states
+        scratch = torch.empty(of_bc + of_a + R * args.segments * channels, dtype=torch.float32, device=dev)
+        parts = scratch.data_ptr()
+        grad = _Grad(args, dy.data_ptr(), *_strides(dy), *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial)), parts, parts + 4 * of_bc, parts + 4 * (of_bc + of_a))
         L.check(L.load().dewb_selective_grad(ctypes.addressof(grad), x.dtype is torch.float32, stream), "selective_grad")
         L.count_launches(2 if args.segments == 1 else 3)
     return dx, ddt, da, db, dc, dd, dz, dinitial
@@ -176,8 +185,17 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
     out_type = x.dtype
     # one type for what is per token: where they differ (or are fp16) in fp32, which holds every value of each
     one = out_type is not torch.float16 and all(t is None or t.dtype is out_type for t in (Bm, Cm, z)) and dt.dtype in (out_type, torch.float32)
-    fit = lambda t, *size: None if t is None else _dense((t if one else t.float()).expand(size))
-    fp32 = lambda t, *size: None if t is None else t.float().expand(size).contiguous()
+
+    def fit(t, *size):
+        if t is None:
+            return None
+        t = t if one else t.float()
+        return _dense(t if t.shape == size else t.expand(size))
+
+    def fp32(t, *size):
+        if t is None or (t.dtype is torch.float32 and t.shape == size and t.is_contiguous()):
+            return t
+        return t.float().expand(size).contiguous()
     ins = (fit(x, R, T, C), fit(dt, R, T, C), fp32(A, C, N), fit(Bm, R, T, N), fit(Cm, R, T, N), fp32(D, C), fit(z, R, T, C), fp32(initial_state, R, C, N))
     if 0 in (R, T, C, N):
         from .scan import selective_scan_chunked
@@ -190,39 +208,55 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
 # a call's rows, with the states of a store
 
 
-def _check(what: str, x, dt, b, c, z, state, rows: Optional[Rows], state_shape, per_token, widths) -> None:
+def _check(what: str, x, dt, b, c, z, state, rows: Optional[Rows], state_shape, wide, steps, narrow) -> None:
     if x.dim() != 3:
         raise ValueError(f"{what}: x [rows, tokens, channels], got {tuple(x.shape)}")
-    R, S = x.shape[:2]
-    if x.dtype not in (torch.bfloat16, torch.float32) or any(t is not None and t.dtype is not x.dtype for t in per_token) or dt.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"{what}: bf16 or fp32 tokens of one type and steps of that type or fp32, got {[t.dtype for t in (x, dt, *per_token) if t is not None]}")
-    for t, n in widths:
-        if t is not None and t.shape != (R, S, n):
-            raise ValueError(f"{what}: [{R}, {S}, {n}] beside x {tuple(x.shape)}, got {tuple(t.shape)}")
-    tensors = [dt, b, c, z, state]
+    R, S, _ = shape = x.shape
+    own, where = x.dtype, torch.Tensor.get_device if x.is_cuda else _device          # (the quicker question)
+    if (own is not torch.bfloat16 and own is not torch.float32) or b.dtype is not own or c.dtype is not own or (z is not None and z.dtype is not own) or \
+            (dt.dtype is not own and dt.dtype is not torch.float32):
+        raise TypeError(f"{what}: bf16 or fp32 tokens of one type and steps of that type or fp32, got {[t.dtype for t in (x, dt, b, c, z) if t is not None]}")
+    if dt.shape != (R, S, steps) or b.shape != (R, S, narrow) or c.shape != b.shape or (z is not None and z.shape != shape):
+        raise ValueError(f"{what}: steps [.., {steps}], B and C [.., {narrow}] and z [.., {wide}] beside x {tuple(shape)}, got {[tuple(t.shape) for t in (dt, b, c, z) if t is not None]}")
+    device = where(x)
+    apart = where(dt) != device or where(b) != device or where(c) != device or (z is not None and where(z) != device)
     if rows is not None:
-        tensors += [rows.positions, rows.lengths, rows.row_ids]
-        if rows.positions.shape != (R, S) or rows.lengths.shape != (R,) or (rows.row_ids is not None and rows.row_ids.shape != (R,)):
+        positions, lengths, ids = rows
+        if positions.shape != (R, S) or lengths.shape != (R,) or (ids is not None and ids.shape != (R,)):
             raise ValueError(f"{what}: positions [rows, tokens], lengths and row ids [rows] of {R} rows of {S} tokens")
-        if any(t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()) for t in (rows.positions, rows.lengths, rows.row_ids)):
-            raise TypeError(f"{what}: positions, lengths and row ids are int32 in one piece")
+        for t in rows:
+            if t is not None:
+                if t.dtype is not torch.int32 or not t.is_contiguous():
+                    raise TypeError(f"{what}: positions, lengths and row ids are int32 in one piece")
+                apart = apart or where(t) != device
     if state is not None:
         if state.shape[1:] != state_shape or state.dtype is not torch.float32 or not state.is_contiguous():
             raise ValueError(f"{what}: an fp32 state [store rows, {', '.join(map(str, state_shape))}] in one piece, got {tuple(state.shape)}, {state.dtype}")
         if (rows is None or rows.row_ids is None) and state.shape[0] < R:
             raise ValueError(f"{what}: {R} rows against a store of {state.shape[0]}")
-    if any(t is not None and t.device != x.device for t in tensors):
+        apart = apart or where(state) != device
+    if apart:
         raise ValueError(f"{what}: tensors of one device")
 
 
+def _device(t: torch.Tensor) -> torch.device:
+    return t.device
+
+
+def _fp32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
+
+
 def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: int, heads: int) -> torch.Tensor:
-    x, dt, z, b, c = (_dense(t) for t in (x, dt, z, b, c))
-    f32 = lambda t: None if t is None else t.detach().float().contiguous()
-    a, dt_bias, d = f32(a), f32(dt_bias), f32(d)
+    if not L.device_is_current(x):
+        with L.on_device_of(x):
+            return _tokens(x, dt, z, b, c, a, dt_bias, d, rows, state, N, groups, heads)
+    x, dt, z, b, c = _dense(x), _dense(dt), _dense(z), _dense(b), _dense(c)
+    a, dt_bias, d = _fp32(a), _fp32(dt_bias), _fp32(d)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with L.on_device_of(x) as stream:
-        args, work = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0])
-        _launch(args, x.dtype is torch.float32, x.shape[1] == 1 and state is not None, stream)
+    token = x.shape[1] == 1 and state is not None
+    args, work = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0], token)
+    _launch(args, x.dtype is torch.float32, token, L.stream())
     return y
 
 
@@ -248,7 +282,7 @@ def selective_tokens(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, Bm:
     belongs to one row of a call.  Rows outside the store are reported by the status word (``library.check_status``) and give zeros."""
     N = A_log.shape[-1]
     C = x.shape[-1]
-    _check("selective_tokens", x, dt, Bm, Cm, z, state, rows, (C, N), (Bm, Cm, z), ((dt, C), (z, C), (Bm, N), (Cm, N)))
+    _check("selective_tokens", x, dt, Bm, Cm, z, state, rows, (C, N), C, C, N)
     if A_log.shape != (C, N) or (D is not None and D.shape != (C,)):
         raise ValueError(f"selective_tokens: A_log [{C}, states] and D [{C}], got {tuple(A_log.shape)}, {None if D is None else tuple(D.shape)}")
     if N > MOST_STATES or 0 in x.shape or not kernel_ok(x, dt, A_log, Bm, Cm, D, z) or L.transformed(x, dt, A_log, Bm, Cm, D, z):
@@ -279,7 +313,7 @@ def ssd_tokens(x: torch.Tensor, dt: torch.Tensor, dt_bias: Optional[torch.Tensor
     if H < 1 or G < 1 or H % G or x.shape[-1] % H or Bm.shape[-1] % G or x.shape[-1] == 0:
         raise ValueError(f"ssd_tokens: {H} heads in {G} groups of x {tuple(x.shape)}, B {tuple(Bm.shape)}")
     P, N = x.shape[-1] // H, Bm.shape[-1] // G
-    _check("ssd_tokens", x, dt, Bm, Cm, None, state, rows, (H, P, N), (Bm, Cm), ((dt, H), (Bm, G * N), (Cm, G * N)))
+    _check("ssd_tokens", x, dt, Bm, Cm, None, state, rows, (H, P, N), H * P, H, G * N)
     if any(t is not None and t.shape != (H,) for t in (dt_bias, A_log, D)):
         raise ValueError(f"ssd_tokens: a number per head, {H}, for A_log, the steps' bias and D")
     if N > MOST_HEAD_STATES or 0 in x.shape or N == 0 or not kernel_ok(x, dt, dt_bias, A_log, Bm, Cm, D) or L.transformed(x, dt, dt_bias, A_log, Bm, Cm, D):
