@@ -83,12 +83,11 @@ struct Place {
   template <bool FAST>
   __device__ __forceinline__ void bring(const Grad& g, int i, int t0, int t_end) {
     const int t = t0 + lt + i * LN, n = lt < TT && t < t_end ? left : 0;
-    const bool four = FAST || (whole && n == 4);
     if (!FAST || LN <= TT || lt < TT) {
-      if (STATES) rx[i] = fetch(x + t * g.f.x_token, four, n);
-      rd[i] = fetch(dt + t * g.f.dt_token, four, n);
-      ry[i] = fetch(dy + t * g.dy_token, four, n);
-      if (z != nullptr) rz[i] = fetch(z + t * g.f.z_token, four, n);
+      if (STATES) rx[i] = fetch(x + t * g.f.x_token, FAST, n);
+      rd[i] = fetch(dt + t * g.f.dt_token, FAST, n);
+      ry[i] = fetch(dy + t * g.dy_token, FAST, n);
+      if (z != nullptr) rz[i] = fetch(z + t * g.f.z_token, FAST, n);
     }
   }
   __device__ __forceinline__ void bring(const Grad& g, int t0, int t_end) {
@@ -282,6 +281,7 @@ grad_kernel(const Grad g) {
   const long long pad_row = static_cast<long long>(row) * p.segments * padded + c0 + cg * 4;
   const Block<NS> a = Block<NS>::make([&](int j, int k) { return rate<false>(p, c0 + cg * 4 + j, sl * NS + k, 1); });
   Block<NS> d = last_of<NS>(g, row, c0 + cg * 4, sl * NS, seg == p.segments - 1), da = Block<NS>::make([](int, int) { return 0.f; });
+#pragma unroll 2
   for (int q = p.segments - 1; q > seg; --q) {    // what comes from behind the segment
     const long long there = pad_row + static_cast<long long>(q) * padded;
     const Block<NS> e = Block<NS>::load(p.starts + there * NP + sl * NS, NP);
@@ -312,7 +312,8 @@ grad_kernel(const Grad g) {
     } else {                                      // one after another: fp32 takes twice the registers
 #pragma unroll
       for (int i = 0; i < L::PASSES; ++i) {
-        at.template bring<false>(g, i, t0, t_end);
+        if (at.whole && t0 + TT <= t_end) at.template bring<true>(g, i, t0, t_end);
+        else at.template bring<false>(g, i, t0, t_end);
         stage<T, TD, LN, NS, true>(sm, at, p.softplus, i, t0, t_end, warp, unused);
         asm volatile("" ::: "memory");
       }
@@ -541,7 +542,11 @@ int grad_go(const Grad& g, cudaStream_t stream) {
 
 template <typename T, typename TD>
 int grad_any(const Grad& g, cudaStream_t stream) {
-  if (g.f.N <= 16) return g.f.states_each == 2 ? grad_go<T, TD, 8, 2>(g, stream) : grad_go<T, TD, 4>(g, stream);
+  if (g.f.N <= 16) {
+    if (g.f.states_each == 2) return grad_go<T, TD, 8, 2>(g, stream);
+    if constexpr (sizeof(T) == 2) return grad_go<T, TD, 4>(g, stream);
+    return -3;                                    // (four states a lane: more registers than there are)
+  }
   if (g.f.N <= 32) return grad_go<T, TD, 8>(g, stream);
   if (g.f.N <= 64) return grad_go<T, TD, 16>(g, stream);
   if (g.f.N <= 128) return grad_go<T, TD, 32>(g, stream);

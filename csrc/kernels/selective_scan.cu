@@ -85,6 +85,7 @@ scan_kernel(const Args p) {
   };
   if (ENDS && seg == 0) keep(p.starts + pad_row * NP + sl * NS);
   if (!ENDS && p.segments > 1) {                  // what stands in front of the segment
+#pragma unroll 2
     for (int q = min(seg, 1); q <= seg; ++q) {
       const long long at = pad_row + static_cast<long long>(q) * padded;
 #pragma unroll

@@ -39,20 +39,26 @@ def _padded(C: int, N: int, groups: int = 1, heads: int = 0):
     return -(-(C // groups) // block) * block * groups, lanes * 4 if N <= 128 else 256, block // lanes
 
 
-WARPS = 148 * 28          # what the GPU is filled with
-
-
-def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward: bool = False):
-    """Tokens of a piece of a row (the pieces run side by side), and states of a lane (of up to 16)."""
+def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward: bool = False, fp32: bool = False):
+    """Tokens of a piece of a row (the pieces run side by side), and states of a lane (of up to 16).  Pieces cost a pass of their own over the tokens (about half of the other) and are put
+    together one after another, so there are no more than fill the GPU, or than the square root of half the tokens; fewer states a lane fill it without them, at the price of more sums over lanes.
+    (16 states, in us, forwards: 4 rows of 2048 tokens of 4096 channels whole with 4, 2, 1 states a lane 566, 390, 425, in 8 pieces 409, 421, 559; one of 2048 of 2048 channels in 16, 24
+    pieces of 2 states 74, 78; one of 16384 in 32, 64 pieces 457, 459; one of 512 of 1024 channels in 16 pieces of 2, 11 of 1 19, 20.  Backwards: 8 of 512 of 4096 channels whole,
+    in 5 pieces 457, 497; one of 2048 of 2048 channels in 16 pieces of 4, 22 of 2 154, 177.)"""
     warps = max(1, R * groups * -(-(C // groups) // _padded(C, N, groups, heads)[2]))
-    most = -(-T // 32)
-    if heads:
-        pieces, each = (1 if warps >= 2368 else min(most, -(-WARPS // warps))), 4
-    elif N <= 16 and not backward and 448 <= warps < 1536:
-        pieces, each = 1, 2
+    most = max(1, min(-(-T // EVERY), int((T / 2) ** 0.5)))
+    narrow = N <= 16 and not heads
+    if warps >= 1024 or (narrow and not backward and warps >= 448):
+        pieces = 1
+    elif narrow:
+        # all blocks on the GPU at once (two an SM backwards, four with two states a lane forwards) where that leaves eight pieces or more
+        pieces = 1184 // warps if backward else 592 // -(-warps // 2)
+        pieces = min(most, pieces if pieces >= 8 else -(-(4096 if backward else 1536) // warps))
     else:
-        pieces = min(most, -(-WARPS // warps)) if warps < 1536 else 1
-        each = 4 if N > 16 or warps * most >= WARPS // 2 else 2 if backward or warps * most >= WARPS // 4 else 1
+        pieces = min(most, -(-4096 // warps))
+    each = 4
+    if narrow:
+        each = (4 if warps * pieces >= 1024 and not fp32 else 2) if backward else 4 if warps >= 1536 else 2 if warps * pieces >= 384 else 1
     return -(-(-(-T // pieces)) // EVERY) * EVERY, each
 
 
@@ -78,7 +84,7 @@ def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Op
     """The arguments of a launch, and what has to live until it is issued."""
     R, T, C = x.shape
     channels, states, _ = _padded(C, N, groups, heads)
-    segment, each = (EVERY, _rows_each(R, C)) if token else _split(R, T, C, N, groups, heads, backward)
+    segment, each = (EVERY, _rows_each(R, C)) if token else _split(R, T, C, N, groups, heads, backward, x.dtype is torch.float32)
     segments = -(-T // segment)
     work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device) if segments > 1 else None
     starts, sums = (work.data_ptr(), work.data_ptr() + 4 * R * segments * channels * states) if segments > 1 else (0, 0)

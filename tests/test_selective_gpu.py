@@ -18,6 +18,14 @@ def most(t, steps=True):
     return float(s.amax() * t["a"].abs().amax())
 
 
+def split(pieces, monkeypatch):
+    """How rows are cut and states dealt: by the rule, or as given."""
+    if pieces != "rule":
+        n, each = pieces
+        monkeypatch.setattr(selective, "_split", lambda R, T, C, N, groups, heads=0, backward=False, fp32=False: (
+            max(16, T // n // 16 * 16), (max(2, each) if not fp32 else 2) if backward and N <= 16 else each if N <= 16 and not heads else 4))
+
+
 # one token, a tile and its neighbours, segments; channels of a warp, of a block and odd ones; every width of the lanes over the states; rows of a wider tensor
 SCANS = [(1, 1, 1, 1, FP32, {}), (2, 15, 3, 4, FP32, dict(gate=False)), (1, 16, 32, 16, BF16, {}), (3, 17, 129, 16, BF16, dict(initial=True)), (2, 130, 31, 17, FP32, dict(strided=True)),
          (1, 300, 64, 24, BF16, dict(strided=True, skip=False)), (2, 70, 20, 33, FP32, dict(initial=True)), (1, 33, 24, 64, BF16, dict(gate=False, skip=False)),
@@ -25,11 +33,10 @@ SCANS = [(1, 1, 1, 1, FP32, {}), (2, 15, 3, 4, FP32, dict(gate=False)), (1, 16, 
          (1, 96, 64, 16, BF16, dict(dt_type=FP32, steps=False))]
 
 
-@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("pieces", ["rule", (1, 4), (3, 2), (5, 1)])
 @pytest.mark.parametrize("B,T,C,N,dtype,more", SCANS)
 def test_scan_and_gradients(B, T, C, N, dtype, more, pieces, monkeypatch):
-    if pieces == "one":
-        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
+    split(pieces, monkeypatch)
     steps = more.get("steps", True)
     t = inputs(B, T, C, N, dtype, DEV, T + C, **more)
     with torch.no_grad():
@@ -74,11 +81,10 @@ TOKENS = [(1, 1, 64, 16, BF16, [9], [1], None), (4, 1, 130, 16, BF16, [3, 0, -1,
           (1, 256, 512, 16, BF16, [512], [256], [1])]
 
 
-@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("pieces", ["rule", (1, 4), (3, 2), (5, 1)])
 @pytest.mark.parametrize("R,S,C,N,dtype,first,lengths,ids", TOKENS)
 def test_tokens_with_states(R, S, C, N, dtype, first, lengths, ids, pieces, monkeypatch):
-    if pieces == "one":
-        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
+    split(pieces, monkeypatch)
     t, r, state = call(R, S, C, N, dtype, S + C, first, lengths, ids, strided=C % 2 == 0)
     before = state.clone()
     a_log = torch.log(-t["a"])
@@ -128,12 +134,11 @@ HEADS = [(1, 1, 4, 1, 64, 128, BF16, [5], [1], None), (3, 1, 6, 2, 48, 80, BF16,
          (1, 200, 2, 1, 48, 200, FP32, [2], [200], None)]
 
 
-@pytest.mark.parametrize("pieces", ["rule", "one"])
+@pytest.mark.parametrize("pieces", ["rule", (1, 4), (3, 2), (5, 1)])
 @pytest.mark.parametrize("R,S,H,G,P,N,dtype,first,lengths,ids", HEADS)
 def test_heads_with_states(R, S, H, G, P, N, dtype, first, lengths, ids, pieces, monkeypatch):
     """A decay per head is a rate per channel and state that is one number in each head."""
-    if pieces == "one":
-        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (-(-T // 16) * 16, 4))
+    split(pieces, monkeypatch)
     t, r, state = heads(R, S, H, G, P, N, dtype, S + H, first, lengths, ids)
     before = state.clone()
     y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], H, G, r, state)
