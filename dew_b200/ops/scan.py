@@ -334,7 +334,7 @@ def selective_scan_reference(x, dt, A, Bm, Cm, D=None, z=None, initial_state=Non
 def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, chunk: int = 64, softplus: bool = False):
     """Public entry: ``x, dt [B,T,C]`` (with ``softplus``, the steps' logits), ``A [C,N]``, ``Bm, Cm [B,T,N]``, ``D [C]``, ``z [B,T,C]``, ``initial_state [B,C,N]`` -> (y ``[B,T,C]``, state
     ``[B,C,N]`` fp32).  CUDA tensors with up to 128 states run the sm_100a kernels (``ops/selective.py``), in either direction; everything else the chunked form below."""
-    if x.is_cuda and A.dim() == 2 and A.shape[1] <= 128:
+    if x.is_cuda and A.dim() == 2 and 0 < A.shape[1] <= 128:
         from . import selective as K
         if K.kernel_available(x, dt, A, Bm, Cm, D, z, initial_state):
             return K.selective_scan(x, dt, A, Bm, Cm, D, z, initial_state, softplus)

@@ -188,6 +188,9 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
     given = [t for t in (dt, A, Bm, Cm, D, z, initial_state) if t is not None]
     if any(t.device != x.device for t in given):
         raise ValueError("selective_scan: tensors of one device")
+    if 0 in (R, T, C):
+        last = torch.zeros(R, C, N, device=x.device) if initial_state is None else initial_state.float().expand(R, C, N)
+        return torch.empty_like(x), last.clone()
     out_type = x.dtype
     # one type for what is per token: where they differ (or are fp16) in fp32, which holds every value of each
     one = out_type is not torch.float16 and all(t is None or t.dtype is out_type for t in (Bm, Cm, z)) and dt.dtype in (out_type, torch.float32)
@@ -203,9 +206,6 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
             return t
         return t.float().expand(size).contiguous()
     ins = (fit(x, R, T, C), fit(dt, R, T, C), fp32(A, C, N), fit(Bm, R, T, N), fit(Cm, R, T, N), fp32(D, C), fit(z, R, T, C), fp32(initial_state, R, C, N))
-    if 0 in (R, T, C, N):
-        from .scan import selective_scan_chunked
-        return selective_scan_chunked(x, dt, A, Bm, Cm, D, z, initial_state, softplus=softplus)
     y, last = _forward(*ins, softplus, False)[:2] if L.unrecorded(*ins) else _SelectiveScan.apply(*ins, softplus)
     return y.to(out_type), last
 
