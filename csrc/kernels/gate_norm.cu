@@ -5,7 +5,9 @@
 // Bound by memory: a row's values are read once and stay in registers between the sums and the results (`ITEMS` pieces of V values a thread; ITEMS 0, for rows that are longer or lie
 // askew, reads them again).  The backward forms r anew from what it reads anyway, in the same reduction as mean(g u), so the forward keeps nothing.  A row belongs to a warp (up to
 // 32 V ITEMS values) or to a block of NT threads; in the backward a block walks rows with its columns' dw in registers, and its sums leave as one part, added up in one order by
-// weight_sum_kernel.  There values stay as they lie in memory (half the registers in bf16) and the next row is on its way while one is summed: 8192 rows of 8192 DEWB_NORM.
+// weight_sum_kernel.  There values stay as they lie in memory (half the registers in bf16) and the next row is on its way while one is summed.
+// 8192 rows of 8192 bf16 values: forward 69 us (5.8 TB/s; with expf and a division, 91: issuing), backward 136 (4.9 TB/s; as fp32 values without the next row ahead, 272).  Two pieces
+// a thread: with one (rows of 4096 and 512 threads) the barriers take their share, backward 120 us instead of 83.
 // Values are bf16 or fp32 (template T; w either), sums fp32.  Compiled without fast math.
 #include <cstdint>
 #include <cuda_bf16.h>

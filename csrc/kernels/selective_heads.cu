@@ -4,7 +4,9 @@
 //   head_token_kernel  one token per row: the state is read and written once
 //
 // A lane owns eight channels (rows p of the state) and NS states of each, in pairs; LN lanes share the states.  A decay is one exponential a head, so what counts are three
-// multiply-adds a state, and how often a number is fetched for them: B and C serve eight channels, a step all states.  Compiled without fast math.
+// multiply-adds a state, and how often a number is fetched for them: B and C serve eight channels, a step all states (four channels a lane in pairs of channels, B and C twice in shared
+// memory: 104 us for 5 rows of up to 300 tokens, 24 heads of 48 over 80 states, fp32; so, and in segments, 60).  head_token_kernel: 128 rows of 64 heads of 64 x 128 85 us, 6.1 TB/s.
+// Compiled without fast math.
 #include "../common/selective.cuh"
 
 namespace dewb {

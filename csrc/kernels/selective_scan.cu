@@ -6,6 +6,11 @@
 //
 // A call row whose first position is 0 starts from zero; positions below 0 are padding at a row's end: they change no state and give zeros.
 // Inputs and outputs are bf16 or fp32 (template T; the steps' logits either), everything else fp32.  Compiled without fast math.
+//
+// What bounds scan_kernel is the exponential of every token, channel and state: the special-function unit takes eight cycles for a warp's, so 4 rows of 2048 tokens of 4096 channels of 16
+// states cannot take less than 119 us (149 with those of steps and gates; the bytes, 41).  The ENDS pass comes to 75 % of that rate; the other reaches 56 to 70 %, where a SM has 16
+// warps: 247 us in eight segments and 162 for their ends, or 399 for whole rows with two states a lane and 7 warps an SM, whose chains are then what takes the time (a warp waits 1.8
+// of 5 cycles for the instruction before, 1.1 for an exponential or shared memory).  token_kernel is bound by memory: 128 rows of 8192 channels 32 us, 4.3 TB/s.
 #include "../common/selective.cuh"
 
 namespace dewb {
@@ -22,8 +27,10 @@ struct Tile {
 // grid R * segments * channel blocks.
 //   starts[r, 0]       the state that row r begins with          starts[r, j]   what segment j - 1 ends with: from there on for j = 1, from zeros for the others
 //   sums[r, j]         the sum of segment j's steps, per channel
-// A tile's x and steps come a tile ahead, in registers; what the end of a tile needs (x again, z) is asked for at its beginning (L2) and read then.  The sums over states are formed at
-// the end of a tile from what every lane leaves in shared memory: with shuffles after every token (or two, or four) a warp alone took 620 cycles a token, so: DEWB_ALONE.
+// A tile's x and steps come a tile ahead, in registers as they lie in memory (converted on arrival, every tile waited for them: 10 to 25 % of the time); what the end of a tile needs (x
+// again, z) is asked for at its beginning (L2) and read then.  Channels go in pairs, two to an instruction: no more of them a second, but half as many to issue (one at a time: 3 %
+// slower here, 13 % in the gradients).  The sums over states are formed at the end of a tile from what every lane leaves in shared memory: with shuffles after every two or four tokens
+// the whole rows above took 665 and 528 us with four states a lane, so 555.  NS 4, 2, 1: what _split in ops/selective.py says of each.
 template <typename T, typename TD, int LN, int NS, bool ENDS>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4)
 scan_kernel(const Args p) {

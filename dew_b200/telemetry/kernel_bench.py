@@ -250,6 +250,30 @@ def bench_ssd(out, peaks, flush, iters=10, shapes=None):
         _row(out, kernel="ssd", B=B, T=T, H=H, G=G, fwd_ms=t_k.median_ms, fwd_bwd_ms=t_b.median_ms, torch_chunked_ms=t_t.median_ms)
 
 
+def bench_selective(out, peaks, flush, iters=10, shapes=None):
+    """The selective scan forward and backward, and a decode step of its states: the kernels against the chunked form in PyTorch (forward)."""
+    from ..ops import scan, selective, token_mix
+    for B, T, C, N in shapes or [(4, 2048, 4096, 16), (1, 4096, 2048, 16)]:
+        make = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+        x, dt, z, Bm, Cm, D = make(B, T, C), make(B, T, C) - 4, make(B, T, C), make(B, T, N), make(B, T, N), torch.ones(C, device="cuda")
+        A_log = torch.log(torch.arange(1, N + 1, device="cuda", dtype=torch.float32)).repeat(C, 1)
+        A = -torch.exp(A_log)
+        with torch.no_grad():
+            t_k = device_time(lambda: scan.selective_scan(x, dt, A, Bm, Cm, D, z, softplus=True), iters=iters, flush=flush)
+            t_t = device_time(lambda: scan.selective_scan_chunked(x[:1, :512], dt[:1, :512], A, Bm[:1, :512], Cm[:1, :512], D, z[:1, :512], softplus=True), iters=max(2, iters // 3),
+                              flush=flush)
+        leaves = [t.requires_grad_() for t in (x, dt, A, Bm, Cm, D, z)]
+        dy = torch.randn_like(x)
+        t_b = device_time(lambda: torch.autograd.grad(scan.selective_scan(*leaves, softplus=True)[0], leaves, dy), iters=iters, flush=flush)
+        rows = token_mix.Rows(torch.full((128, 1), 5, device="cuda", dtype=torch.int32), torch.full((128,), 6, device="cuda", dtype=torch.int32))
+        step, state = [make(128, 1, n) for n in (C, C, N, N, C)], torch.zeros(128, C, N, device="cuda")
+        with torch.no_grad():
+            t_s = device_time(lambda: selective.selective_tokens(step[0], step[1], A_log, step[2], step[3], D.detach(), step[4], rows, state), iters=iters, flush=flush)
+        L.check_status()
+        _row(out, kernel="selective", B=B, T=T, C=C, N=N, fwd_ms=t_k.median_ms, fwd_bwd_ms=t_b.median_ms, step_128_rows_ms=t_s.median_ms,
+             torch_chunked_512_tokens_ms=t_t.median_ms)
+
+
 def bench_sampling(out, peaks, flush, iters=10):
     """Token draws over a 128256-entry vocabulary, 128 rows: the kernels against the PyTorch transforms + multinomial."""
     from ..ops import sample as S
@@ -434,6 +458,8 @@ def main(argv=None):
         bench_attention_variants(out, peaks, flush, iters=args.iters)
     if "gdn" in only:
         bench_gdn(out, peaks, flush, iters=args.iters)
+    if "selective" in only:
+        bench_selective(out, peaks, flush, iters=args.iters)
     if "ssd" in only:
         bench_ssd(out, peaks, flush, iters=args.iters)
     if "sampling" in only:
