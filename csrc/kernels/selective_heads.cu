@@ -2,6 +2,7 @@
 //
 //   head_scan_kernel   tokens one after another with the states in registers, in fp32; segments of a row side by side as in selective_scan.cu
 //   head_token_kernel  one token per row: the state is read and written once
+//   head_steps_kernel  what the scan in chunks on the tensor cores (ssd_sm100.cu) wants of a call's rows: their steps, rates and places
 //
 // A lane owns eight channels (rows p of the state) and NS states of each, in pairs; LN lanes share the states.  A decay is one exponential a head, so what counts are three
 // multiply-adds a state, and how often a number is fetched for them: B and C serve eight channels, a step all states (four channels a lane in pairs of channels, B and C twice in shared
@@ -303,6 +304,33 @@ head_token_kernel(const Args p) {
   }
 }
 
+// steps [R, T, heads], rates [heads] (negative), places [3, R]: tokens that count, the store's row that a row begins with (-1: with zeros) and the one that it ends in (-1: none).
+template <typename TD>
+__global__ void __launch_bounds__(256)
+head_steps_kernel(const Args p, float* __restrict__ steps, float* __restrict__ rates, int* __restrict__ places) {
+  const int row = blockIdx.y;
+  const Row r = row_of(p, row);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) {
+      places[row] = r.len;
+      places[p.R + row] = r.len > 0 && r.held ? static_cast<int>(r.at) : -1;
+      places[2 * p.R + row] = r.len > 0 && p.last != nullptr ? static_cast<int>(r.at) : -1;
+    }
+    if (row == 0)
+      for (int h = threadIdx.x; h < p.heads; h += 256) rates[h] = p.log_a ? -expf(p.a[h]) : p.a[h];
+  }
+  const long long all = static_cast<long long>(p.T) * p.heads;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+    const int t = static_cast<int>(i / p.heads), h = static_cast<int>(i - static_cast<long long>(t) * p.heads);
+    float s = 0.f;
+    if (t < r.len) {
+      s = ld(static_cast<const TD*>(p.dt) + row * p.dt_row + t * p.dt_token + h) + (p.dt_bias == nullptr ? 0.f : p.dt_bias[h]);
+      s = p.softplus ? softplus(s) : s;
+    }
+    steps[row * all + i] = s;
+  }
+}
+
 template <typename T, typename TD, int LN, int NS>
 int head_go(const Args& p, cudaStream_t stream) {
   using L = HeadLay<LN, NS>;
@@ -356,4 +384,14 @@ extern "C" int dewb_head_scan(const dewb_selective_args* a, int fp32, int token,
   if (token) return fp32 ? head_token_any<float>(*a, stream) : head_token_any<bf16>(*a, stream);
   if (fp32) return heads_any<float, float>(*a, stream);
   return a->dt_fp32 ? heads_any<bf16, float>(*a, stream) : heads_any<bf16, bf16>(*a, stream);
+}
+
+extern "C" int dewb_head_steps(const dewb_selective_args* a, float* steps, float* rates, int* places, void* stream_ptr) {
+  if (a == nullptr || a->heads < 1 || a->R > 65535 || !args_ok(*a) || steps == nullptr || rates == nullptr || places == nullptr) return -3;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
+  const long long all = static_cast<long long>(a->T) * a->heads, blocks = (all + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(blocks < 512 ? blocks : 512), a->R);
+  if (a->dt_fp32) head_steps_kernel<float><<<grid, 256, 0, stream>>>(*a, steps, rates, places);
+  else head_steps_kernel<bf16><<<grid, 256, 0, stream>>>(*a, steps, rates, places);
+  return static_cast<int>(cudaGetLastError());
 }

@@ -39,6 +39,10 @@ struct Call {
   const float *dt, *A, *D;
   long long xb, xt, bb, bt, cb, ct;      // dy is contiguous
   int B, T, H, G, chunks;
+  // Of a call's rows with the states of a store (forward alone; null: every token counts, and batch row b's states are row b of `initial` and `last`): tokens of a row that count (what lies
+  // behind them is not read and gives zeros), the store's row that it begins with (below 0: with zeros) and the one that it leaves its state in (below 0: none).
+  const int *live, *from, *to;
+  __device__ __forceinline__ int tokens(int b) const { return live == nullptr ? T : live[b]; }
 };
 
 __device__ __forceinline__ void cp16(void* dst, const void* src, bool real) {
@@ -133,6 +137,7 @@ ssd_states(Call k, const float* __restrict__ initial, Out* __restrict__ states, 
   if (rev) { initial = rev_initial; states = rev_states; last = rev_last; }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, r = lane >> 2;
   const int b = blockIdx.x / k.H, h = blockIdx.x % k.H, grp = h / (k.H / k.G), col0 = blockIdx.y * NT * 8;
+  const int tokens = k.tokens(b);
   auto chunk = [&](int it) { return rev ? k.chunks - 1 - it : it; };
   if (warp == 4) {
     const __nv_bfloat16* u = rev ? k.dy + static_cast<long long>(b) * k.T * k.H * P + h * P : k.x + b * k.xb + h * P;
@@ -140,17 +145,17 @@ ssd_states(Call k, const float* __restrict__ initial, Out* __restrict__ states, 
     const long long us = rev ? static_cast<long long>(k.H) * P : k.xt, vs = rev ? k.ct : k.bt;
     auto fetch = [&](int it) {
       if (it < k.chunks) {
-        const int t0 = chunk(it) * L, real = min(L, k.T - t0);
+        const int t0 = chunk(it) * L, real = min(L, tokens - t0);
         uint8_t* st = smem + (it % WALK_STAGES) * (U_BYTES + V_BYTES);
 #pragma unroll 4
         for (int i = 0; i < L * 8 / 32; ++i) {
           const int row = i * 4 + (lane >> 3), c = lane & 7;
-          cp16(st + piece<8>(row, c), u + (t0 + (row < real ? row : 0)) * us + c * 8, row < real);
+          cp16(st + piece<8>(row, c), u + (row < real ? t0 + row : 0) * us + c * 8, row < real);
         }
 #pragma unroll 4
         for (int i = 0; i < L * CV / 32; ++i) {
           const int row = (i * 32 + lane) / CV, c = (i * 32 + lane) % CV;
-          cp16(st + U_BYTES + piece<CV>(row, c), v + (t0 + (row < real ? row : 0)) * vs + c * 8, row < real);
+          cp16(st + U_BYTES + piece<CV>(row, c), v + (row < real ? t0 + row : 0) * vs + c * 8, row < real);
         }
       }
       cp_commit();                                     // (a group for every chunk, empty behind the last)
@@ -169,9 +174,9 @@ ssd_states(Call k, const float* __restrict__ initial, Out* __restrict__ states, 
     const float* dt = k.dt + static_cast<long long>(b) * k.T * k.H + h;
     float next0, next1;
     auto fetch = [&](int it) {
-      const int t = it < k.chunks ? chunk(it) * L + 2 * lane : k.T;
-      next0 = t < k.T ? dt[static_cast<long long>(t) * k.H] : 0.f;
-      next1 = t + 1 < k.T ? dt[static_cast<long long>(t + 1) * k.H] : 0.f;
+      const int t = it < k.chunks ? chunk(it) * L + 2 * lane : tokens;
+      next0 = t < tokens ? dt[static_cast<long long>(t) * k.H] : 0.f;
+      next1 = t + 1 < tokens ? dt[static_cast<long long>(t + 1) * k.H] : 0.f;
     };
     auto weigh = [&](int it) {                         // e^{g_i}, or dt_j e^{g_L - g_j}
       const float dt0 = next0, dt1 = next1;
@@ -193,7 +198,8 @@ ssd_states(Call k, const float* __restrict__ initial, Out* __restrict__ states, 
   }
   const long long cell = static_cast<long long>(P) * N, at = (warp * 16 + r) * N + col0 + 2 * q;      // this thread's first value of a state
   float S[NT][4];
-  const float* from = initial == nullptr ? nullptr : initial + blockIdx.x * cell + at;
+  const int begins = k.from == nullptr ? b : k.from[b], ends = k.to == nullptr ? b : k.to[b];
+  const float* from = initial == nullptr || begins < 0 ? nullptr : initial + (static_cast<long long>(begins) * k.H + h) * cell + at;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float2 a = from == nullptr ? make_float2(0.f, 0.f) : *reinterpret_cast<const float2*>(from + n * 8);
@@ -243,8 +249,8 @@ ssd_states(Call k, const float* __restrict__ initial, Out* __restrict__ states, 
       for (int i = 0; i < 4; ++i) { S[n][i] = fmaf(S[n][i], decay, c0[i]); S[n + 1][i] = fmaf(S[n + 1][i], decay, c1[i]); }
     }
   }
-  if (last != nullptr) {
-    float* to = last + blockIdx.x * cell + at;
+  if (last != nullptr && ends >= 0) {
+    float* to = last + (static_cast<long long>(ends) * k.H + h) * cell + at;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       *reinterpret_cast<float2*>(to + n * 8) = make_float2(S[n][0], S[n][1]);
@@ -265,24 +271,24 @@ ssd_output(Call k, const __nv_bfloat16* __restrict__ states, __nv_bfloat16* __re
   uint8_t *tC = smem, *tB = tC + L * N * 2, *stages = tB + L * N * 2, *tY = stages + 2 * OUT_STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane & 3, r = lane >> 2;
   const int b = blockIdx.x / k.chunks, n = blockIdx.x % k.chunks, grp = blockIdx.y, h0 = grp * (k.H / k.G) + blockIdx.z * per;
-  const int t0 = n * L, real = min(L, k.T - t0), row = warp * 16;
+  const int tokens = k.tokens(b), t0 = n * L, real = min(L, k.T - t0), there = min(L, tokens - t0), row = warp * 16;      // tokens that are stored, and that are read
   auto fetch = [&](int i) {
     uint8_t* st = stages + (i & 1) * OUT_STAGE;
-    load_tile<8, 128>(st, k.x + b * k.xb + t0 * k.xt + (h0 + i) * P, k.xt, real);
+    load_tile<8, 128>(st, k.x + b * k.xb + t0 * k.xt + (h0 + i) * P, k.xt, there);
     load_tile<16, 128>(st + L * P * 2, states + ((static_cast<long long>(b) * k.H + h0 + i) * k.chunks + n) * P * N, N, P);
     cp_commit();
   };
   auto decays = [&](int i) {                           // warp 0
     const int t = t0 + 2 * lane;
     const float* dt = k.dt + static_cast<long long>(b) * k.T * k.H + h0 + i;
-    const float a = t < k.T ? dt[static_cast<long long>(t) * k.H] : 0.f, c = t + 1 < k.T ? dt[static_cast<long long>(t + 1) * k.H] : 0.f;
+    const float a = t < tokens ? dt[static_cast<long long>(t) * k.H] : 0.f, c = t + 1 < tokens ? dt[static_cast<long long>(t + 1) * k.H] : 0.f;
     float g0, g1;
     running(a, c, k.A[h0 + i], g0, g1);
     *reinterpret_cast<float2*>(&sg[i & 1][2 * lane]) = make_float2(g0, g1);
     *reinterpret_cast<float2*>(&sdt[i & 1][2 * lane]) = make_float2(a, c);
   };
-  load_tile<16, 128>(tC, k.Cm + b * k.cb + t0 * k.ct + grp * N, k.ct, real);
-  load_tile<16, 128>(tB, k.Bm + b * k.bb + t0 * k.bt + grp * N, k.bt, real);
+  load_tile<16, 128>(tC, k.Cm + b * k.cb + t0 * k.ct + grp * N, k.ct, there);
+  load_tile<16, 128>(tB, k.Bm + b * k.bb + t0 * k.bt + grp * N, k.bt, there);
   cp_commit();
   fetch(0);
   if (warp == 0) decays(0);
@@ -793,6 +799,15 @@ static int walk(const Call& k, const Walk<Out>& forward, const Walk<Out>* revers
   return run_states<8, TERMS, Out>(k, forward, reverse, stream);
 }
 
+static int run_output(const Call& k, const __nv_bfloat16* states, __nv_bfloat16* y, cudaStream_t stream) {
+  int splits = 1;                                      // two CTAs an SM
+  while ((k.H / k.G) % (splits * 2) == 0 && static_cast<long long>(k.B) * k.chunks * k.G * splits < 2 * SMS) splits *= 2;
+  cudaError_t c = cudaFuncSetAttribute(ssd_output, cudaFuncAttributeMaxDynamicSharedMemorySize, OUT_SMEM);
+  if (c != cudaSuccess) return static_cast<int>(c);
+  ssd_output<<<dim3(k.B * k.chunks, k.G, splits), 128, OUT_SMEM, stream>>>(k, states, y, k.H / k.G / splits);
+  return static_cast<int>(cudaGetLastError());
+}
+
 static int check(const Call& k) {
   if (k.B <= 0 || k.T <= 0 || k.H <= 0 || k.G <= 0 || k.H % k.G != 0 || k.G > 65535) return -3;
   // (batch rows by chunks, and by heads, lie along the grid's first dimension)
@@ -833,12 +848,24 @@ extern "C" int dewb_ssd_fwd(const void* x, const float* dt, const float* A, cons
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const Walk<__nv_bfloat16> forward{initial, static_cast<__nv_bfloat16*>(states), last};
   if ((e = walk<1, __nv_bfloat16>(k, forward, nullptr, stream))) return e;
-  int splits = 1;                                      // two CTAs an SM
-  while ((H / G) % (splits * 2) == 0 && static_cast<long long>(B) * k.chunks * G * splits < 2 * SMS) splits *= 2;
-  cudaError_t c = cudaFuncSetAttribute(ssd_output, cudaFuncAttributeMaxDynamicSharedMemorySize, OUT_SMEM);
-  if (c != cudaSuccess) return static_cast<int>(c);
-  ssd_output<<<dim3(B * k.chunks, G, splits), 128, OUT_SMEM, stream>>>(k, static_cast<in>(states), static_cast<__nv_bfloat16*>(y), H / G / splits);
-  return static_cast<int>(cudaGetLastError());
+  return run_output(k, static_cast<in>(states), static_cast<__nv_bfloat16*>(y), stream);
+}
+
+// The same for a call's rows, with the states of a store: state fp32 [store rows, H, 64, 128] goes on in place, live / from / to [B] as in `Call`; dt fp32 [B, T, H], zeros where nothing
+// counts.  Every state is fp32 through and through: the decayed x enters its products as three bf16 terms, so that a row that comes in many calls is the row in one.  y is formed as
+// above, of states rounded to bf16 once.
+extern "C" int dewb_ssd_rows(const void* x, const float* dt, const float* A, const void* Bm, const void* Cm, const float* D, float* state, void* states, void* y, const int* live,
+                             const int* from, const int* to, int B, int T, int H, int G, const long long* strides, void* stream_ptr) {
+  using namespace dewb::ssd;
+  typedef const __nv_bfloat16* in;
+  const Call k{static_cast<in>(x), static_cast<in>(Bm), static_cast<in>(Cm), nullptr, dt, A, D, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
+               B, T, H, G, (T + L - 1) / L, live, from, to};
+  int e = check(k);
+  if (e || live == nullptr || from == nullptr || to == nullptr) return e ? e : -3;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
+  const Walk<__nv_bfloat16> forward{state, static_cast<__nv_bfloat16*>(states), state};
+  if ((e = walk<3, __nv_bfloat16>(k, forward, nullptr, stream))) return e;
+  return run_output(k, static_cast<in>(states), static_cast<__nv_bfloat16*>(y), stream);
 }
 
 // The gradients of dewb_ssd_fwd's inputs for dy (bf16 [B, T, H, 64], contiguous) and dlast (fp32, gradient of `last`, may be null).  Scratch: states and dstates

@@ -90,6 +90,8 @@ _SIGNATURES = {
     "dewb_selective_token": "pip",
     "dewb_selective_grad": "pip",
     "dewb_head_scan": "piip",
+    "dewb_head_steps": "ppppp",
+    "dewb_ssd_rows": "pppppppppppp" + "iiii" + "pp",
     "dewb_gate_norm_fwd": "plplpp" + "li" + "f" + "ii" + "p",
     "dewb_gate_norm_bwd": "plplpl" + "ppppp" + "ili" + "f" + "ii" + "p",
     "dewb_rope_append": "pppp" + "iiiii" + "ppp" + "ii" + "p",

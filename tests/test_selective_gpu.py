@@ -137,7 +137,8 @@ HEADS = [(1, 1, 4, 1, 64, 128, BF16, [5], [1], None), (3, 1, 6, 2, 48, 80, BF16,
 @pytest.mark.parametrize("pieces", ["rule", (1, 4), (3, 2), (5, 1)])
 @pytest.mark.parametrize("R,S,H,G,P,N,dtype,first,lengths,ids", HEADS)
 def test_heads_with_states(R, S, H, G, P, N, dtype, first, lengths, ids, pieces, monkeypatch):
-    """A decay per head is a rate per channel and state that is one number in each head."""
+    """A decay per head is a rate per channel and state that is one number in each head.  Token by token (chunks: below)."""
+    monkeypatch.setattr(selective, "CHUNKED_TOKENS", 1 << 30)
     split(pieces, monkeypatch)
     t, r, state = heads(R, S, H, G, P, N, dtype, S + H, first, lengths, ids)
     before = state.clone()
@@ -157,6 +158,53 @@ def test_heads_with_states(R, S, H, G, P, N, dtype, first, lengths, ids, pieces,
                        b=t["b"][i:i + 1, :n, g * N:(g + 1) * N], c=t["c"][i:i + 1, :n, g * N:(g + 1) * N], d=t["d"][h].expand(P), initial=before[at:at + 1, h] if f > 0 else None)
             check(dict(y=y[i:i + 1, :n, cols], last=state[at:at + 1, h]), oracle(**one, steps=True), companion(**one, steps=True), n, P, N, 2 * most(one))
     assert torch.equal(state[untouched], before[untouched])
+
+
+CHUNKS = [(1, 32, 2, 1, [0], [32], None), (3, 65, 4, 2, [0, 9, -1], [65, 13, 0], [1, 0, 3]), (2, 200, 8, 1, [5, 0], [200, 64], [3, 0]), (4, 100, 2, 1, [1, 0, 700, 3], [1, 2, 100, 63], None)]
+
+
+@pytest.mark.parametrize("R,S,H,G,first,lengths,ids", CHUNKS)
+def test_heads_in_chunks(R, S, H, G, first, lengths, ids):
+    """Heads of 64 over 128 states in bf16: the states as exact as token by token; y of states and weights that were rounded to bf16 once."""
+    P, N = 64, 128
+    t, r, state = heads(R, S, H, G, P, N, BF16, S + H, first, lengths, ids)
+    assert selective._suits_chunks(t["x"], H, G, N)
+    for n in ("x", "b", "c", "dt"):                   # (nothing behind a row's end is read)
+        t[n] = t[n].clone()
+        for i, m in enumerate(lengths):
+            t[n][i, m:] = float("nan")
+    before = state.clone()
+    y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], H, G, r, state)
+    L.check_status()
+    untouched = torch.ones(len(state), dtype=torch.bool)
+    for i, (f, n) in enumerate(zip(first, lengths)):
+        at = i if ids is None else ids[i]
+        assert not y[i, max(n, 0):].any()
+        if f < 0:
+            continue
+        untouched[at] = False
+        for h in range(H):
+            g, cols = h // (H // G), slice(h * P, (h + 1) * P)
+            one = dict(x=t["x"][i:i + 1, :n, cols], dt=(t["dt"][i:i + 1, :n, h:h + 1].double() + t["dt_bias"][h].double()).expand(-1, -1, P), a=-t["a_log"][h].double().exp().expand(P, N),
+                       b=t["b"][i:i + 1, :n, g * N:(g + 1) * N], c=t["c"][i:i + 1, :n, g * N:(g + 1) * N], d=t["d"][h].expand(P), initial=before[at:at + 1, h] if f > 0 else None)
+            want, size = oracle(**one, steps=True), companion(**one, steps=True)
+            check(dict(last=state[at:at + 1, h]), {"last": want["last"]}, size, n, P, N, 2 * most(one))
+            # a term of y is off by half a step of bf16 for its state or weight, and the sum by half a step of its own
+            off = (y[i:i + 1, :n, cols].double() - want["y"]).abs()
+            assert bool((off <= 2.0 ** -8 * 1.05 * (size["y"] + want["y"].abs())).all())
+    assert torch.equal(state[untouched], before[untouched])
+
+
+def test_a_long_row_in_many_calls():
+    """Chunks, tokens one after another and single tokens go on from one another's states."""
+    t, r, state = heads(1, 300, 2, 1, 64, 128, BF16, 3, [0], [300], None)
+    run = lambda lo, hi, s: selective.ssd_tokens(t["x"][:, lo:hi], t["dt"][:, lo:hi], t["dt_bias"], t["a_log"], t["b"][:, lo:hi], t["c"][:, lo:hi], t["d"], 2, 1,
+                                                 rows([lo], [hi - lo], hi - lo, None, DEV), s)
+    whole = state.clone()
+    want = run(0, 300, whole)
+    parts = torch.cat([run(lo, hi, state) for lo, hi in ((0, 130), (130, 131), (131, 150), (150, 299), (299, 300))], 1)
+    far = lambda a, b: float((a.double() - b.double()).norm() / b.double().norm())
+    assert far(state[0], whole[0]) < 1e-5 and far(parts, want) < 2.0 ** -7      # (the states' roundings to bf16 fall elsewhere)
 
 
 def test_rows_outside_the_store_are_reported():
