@@ -1,7 +1,16 @@
 """The selective state space scan token by token in 64 bits, forward and backward, and what 32 bits may lose of it."""
+import pytest
 import torch
 
 STEP = 2.0 ** -21        # of one token: the step (softplus, four units of 2^-24), its product with the rate and log2 e (three roundings), the exponential (2^-22), two multiply-adds
+
+
+@pytest.fixture(autouse=True)
+def draws_of_its_own():
+    """What a test draws without a generator depends on no other test, nor does what another draws on it."""
+    with torch.random.fork_rng(devices=list(range(torch.cuda.device_count()))):
+        torch.manual_seed(0)
+        yield
 
 
 def softplus(x):

@@ -5,6 +5,7 @@ import torch
 from dew_b200 import ops
 from dew_b200.ops import gate_norm as K
 from dew_b200.ops import library as L
+from selective_cases import draws_of_its_own  # noqa: F401
 
 EPS = 1e-5
 

@@ -4,7 +4,7 @@ import torch
 
 from dew_b200.ops import library as L
 from dew_b200.ops import scan, selective
-from selective_cases import NAMES, check, companion, inputs, rows
+from selective_cases import NAMES, check, companion, draws_of_its_own, inputs, rows  # noqa: F401
 from selective_cases import scan as oracle
 from selective_cases import softplus
 

@@ -8,6 +8,7 @@ from dew_b200.nn.kv_cache import KVCache
 from dew_b200.nn.linear_attention import RecurrentCache
 from dew_b200.ops import token_mix
 from dew_b200.sampling.text import RowBatch, Sampling, generate, make_cache
+from selective_cases import draws_of_its_own  # noqa: F401
 
 OPTIONS = {"mamba": dict(state_dim=16), "mamba2": dict(state_dim=16, head_dim=16, groups=2)}
 
