@@ -214,7 +214,7 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
 # a call's rows, with the states of a store
 
 
-def _check(what: str, x, dt, b, c, z, state, rows: Optional[Rows], state_shape, wide, steps, narrow) -> None:
+def _check(what: str, x, dt, b, c, z, weights, state, rows: Optional[Rows], state_shape, wide, steps, narrow) -> None:
     if x.dim() != 3:
         raise ValueError(f"{what}: x [rows, tokens, channels], got {tuple(x.shape)}")
     R, S, _ = shape = x.shape
@@ -226,6 +226,8 @@ def _check(what: str, x, dt, b, c, z, state, rows: Optional[Rows], state_shape, 
         raise ValueError(f"{what}: steps [.., {steps}], B and C [.., {narrow}] and z [.., {wide}] beside x {tuple(shape)}, got {[tuple(t.shape) for t in (dt, b, c, z) if t is not None]}")
     device = where(x)
     apart = where(dt) != device or where(b) != device or where(c) != device or (z is not None and where(z) != device)
+    for t in weights:
+        apart = apart or (t is not None and where(t) != device)
     if rows is not None:
         positions, lengths, ids = rows
         if positions.shape != (R, S) or lengths.shape != (R,) or (ids is not None and ids.shape != (R,)):
@@ -322,7 +324,7 @@ def selective_tokens(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, Bm:
     belongs to one row of a call.  Rows outside the store are reported by the status word (``library.check_status``) and give zeros."""
     N = A_log.shape[-1]
     C = x.shape[-1]
-    _check("selective_tokens", x, dt, Bm, Cm, z, state, rows, (C, N), C, C, N)
+    _check("selective_tokens", x, dt, Bm, Cm, z, (A_log, D), state, rows, (C, N), C, C, N)
     if A_log.shape != (C, N) or (D is not None and D.shape != (C,)):
         raise ValueError(f"selective_tokens: A_log [{C}, states] and D [{C}], got {tuple(A_log.shape)}, {None if D is None else tuple(D.shape)}")
     if N > MOST_STATES or 0 in x.shape or not kernel_ok(x, dt, A_log, Bm, Cm, D, z) or L.transformed(x, dt, A_log, Bm, Cm, D, z):
@@ -353,7 +355,7 @@ def ssd_tokens(x: torch.Tensor, dt: torch.Tensor, dt_bias: Optional[torch.Tensor
     if H < 1 or G < 1 or H % G or x.shape[-1] % H or Bm.shape[-1] % G or x.shape[-1] == 0:
         raise ValueError(f"ssd_tokens: {H} heads in {G} groups of x {tuple(x.shape)}, B {tuple(Bm.shape)}")
     P, N = x.shape[-1] // H, Bm.shape[-1] // G
-    _check("ssd_tokens", x, dt, Bm, Cm, None, state, rows, (H, P, N), H * P, H, G * N)
+    _check("ssd_tokens", x, dt, Bm, Cm, None, (A_log, dt_bias, D), state, rows, (H, P, N), H * P, H, G * N)
     if any(t is not None and t.shape != (H,) for t in (dt_bias, A_log, D)):
         raise ValueError(f"ssd_tokens: a number per head, {H}, for A_log, the steps' bias and D")
     if N > MOST_HEAD_STATES or 0 in x.shape or N == 0 or not kernel_ok(x, dt, dt_bias, A_log, Bm, Cm, D) or L.transformed(x, dt, dt_bias, A_log, Bm, Cm, D):

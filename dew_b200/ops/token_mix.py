@@ -79,6 +79,8 @@ def conv_tokens(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
                 state: Optional[torch.Tensor] = None, offset: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [R, S, C]`` (columns of a wider row will do) through a causal convolution per channel, ``w [C, taps]`` with the token's own weight last, behind
     ``bias [C]`` and in front of ``offset [C]``; ``state [store rows, C, taps - 1]`` holds a row's last inputs."""
+    if offset is not None and (offset.shape != x.shape[2:] or offset.device != x.device):
+        raise ValueError(f"conv_tokens: an offset per channel on the tokens' device, {x.shape[-1]}, got {tuple(offset.shape)} on {offset.device}")
     if not kernel_ok(x, w, bias, offset):
         return conv_tokens_reference(x, w, bias, silu, rows, state, offset)
     R, S, C = x.shape

@@ -105,6 +105,10 @@ REFUSALS = [("tokens", ValueError, lambda c: dict(x=c["x"][0])), ("tokens", Valu
             ("heads", ValueError, lambda c: dict(H=3)), ("heads", ValueError, lambda c: dict(G=4)), ("heads", ValueError, lambda c: dict(A_log=torch.zeros(3))),
             ("heads", ValueError, lambda c: dict(dt_bias=torch.zeros(1))), ("heads", ValueError, lambda c: dict(dt=c["dt"][..., :1])), ("heads", ValueError, lambda c: dict(state=c["state"][:, :1])),
             ("heads", TypeError, lambda c: dict(Bm=c["Bm"].bfloat16()))]
+# what lies elsewhere
+REFUSALS += [("tokens", ValueError, lambda c, n=n: {n: c[n].to("meta")}) for n in ("dt", "Cm", "z", "A_log", "D", "state")]
+REFUSALS += [("heads", ValueError, lambda c, n=n: {n: c[n].to("meta")}) for n in ("Bm", "A_log", "dt_bias", "D", "state")]
+REFUSALS += [("tokens", ValueError, lambda c: dict(rows=c["rows"]._replace(row_ids=c["rows"].row_ids.to("meta"))))]
 
 
 @pytest.mark.parametrize("kind,what,change", REFUSALS)

@@ -137,6 +137,12 @@ def test_convolution_with_an_offset_gpu(dtype):
 @pytest.mark.parametrize("graph", [False, True])
 @pytest.mark.parametrize("kind", sorted(OPTIONS))
 def test_server_on_a_gpu(kind, graph):
+@pytest.mark.parametrize("add", [torch.zeros(7), torch.zeros(1, 8), torch.zeros(8, device="meta")])
+def test_offsets_that_a_convolution_refuses(add):
+    with pytest.raises(ValueError, match="offset"):
+        token_mix.conv_tokens(torch.zeros(2, 9, 8), torch.zeros(8, 4), None, False, None, None, add)
+
+
     """fp32 weights: the same tokens as the whole row on the CPU, through prompts in chunks, forks and (captured) steps."""
     m = model(kind)
     asked = prompts()
