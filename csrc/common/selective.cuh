@@ -219,7 +219,7 @@ __device__ __forceinline__ Row row_of(const Args& p, int row) {
   if (p.positions == nullptr) return {p.T, p.initial != nullptr, row};
   const int first = p.positions[static_cast<long long>(row) * p.T], at = p.row_ids == nullptr ? row : p.row_ids[row];
   const bool inside = p.initial == nullptr || (at >= 0 && at < p.stored);
-  if (!inside && p.status != nullptr && threadIdx.x == 0) atomicExch(p.status, OUTSIDE);
+  if (!inside && p.status != nullptr) atomicExch(p.status, OUTSIDE);
   return {first < 0 || !inside ? 0 : max(0, min(p.lengths[row] - first, p.T)), p.initial != nullptr && first > 0, at};
 }
 

@@ -217,3 +217,19 @@ def test_rows_outside_the_store_are_reported():
         with pytest.raises(L.KernelError, match="bad argument"):
             L.check_status()
         assert not y[1].any() and y[0].any() and torch.equal(state[3:], before[3:])
+    # a step of so many rows that a block has several, and one that is cut into chunks
+    t, _, _ = call(1600, 1, 16, 16, BF16, 1, [1] * 1600, [1] * 1600, None)
+    state, ids = torch.randn(1600, 16, 16, device=DEV), list(range(1600))
+    ids[801] = 1600
+    r = rows([1] * 1600, [1] * 1600, 1, ids, DEV)
+    y = selective.selective_tokens(t["x"], t["dt"], torch.log(-t["a"]), t["b"], t["c"], t["d"], t["z"], r, state)
+    with pytest.raises(L.KernelError, match="bad argument"):
+        L.check_status()
+    assert not y[801].any() and y[800].any() and y[802].any()
+    t, r, state = heads(2, 40, 2, 1, 64, 128, BF16, 1, [1, 1], [40, 40], [0, 1])
+    r.row_ids[1] = 7
+    before = state.clone()
+    y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], 2, 1, r, state)
+    with pytest.raises(L.KernelError, match="bad argument"):
+        L.check_status()
+    assert not y[1].any() and y[0].any() and torch.equal(state[1:], before[1:])
