@@ -372,7 +372,8 @@ ssd_output(Call k, const __nv_bfloat16* __restrict__ states, __nv_bfloat16* __re
     for (int s = 0; s < 4; ++s) {
       const int at = row + s * 4 + (lane >> 3), c = lane & 7;
       if (at < real)
-        *reinterpret_cast<uint4*>(y + ((static_cast<long long>(b) * k.T + t0 + at) * k.H + h0 + i) * P + c * 8) = *reinterpret_cast<const uint4*>(tY + piece<8>(at, c));
+        *reinterpret_cast<uint4*>(y + ((static_cast<long long>(b) * k.T + t0 + at) * k.H + h0 + i) * P + c * 8) =
+            at < there ? *reinterpret_cast<const uint4*>(tY + piece<8>(at, c)) : make_uint4(0u, 0u, 0u, 0u);      // (behind the last one a state that overflowed would show)
     }
     __syncthreads();                                   // the stage is free for the head after the next
   }

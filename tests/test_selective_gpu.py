@@ -207,6 +207,14 @@ def test_a_long_row_in_many_calls():
     assert far(state[0], whole[0]) < 1e-5 and far(parts, want) < 2.0 ** -7      # (the states' roundings to bf16 fall elsewhere)
 
 
+@pytest.mark.parametrize("S,dtype", [(20, BF16), (100, BF16), (100, FP32)])
+def test_padding_behind_a_state_that_overflowed(S, dtype):
+    t, r, state = heads(2, S, 2, 1, 64, 128, dtype, 3, [4, 0], [S - 5, S], None)
+    state[0] = float("inf")
+    y = selective.ssd_tokens(t["x"], t["dt"], t["dt_bias"], t["a_log"], t["b"], t["c"], t["d"], 2, 1, r, state)
+    assert not y[0, S - 5:].any() and not y[0, :S - 5].isfinite().all() and y[1].isfinite().all() and state[1].isfinite().all()
+
+
 def test_rows_outside_the_store_are_reported():
     t, r, state = call(3, 1, 16, 16, BF16, 1, [1, 1, 1], [1] * 3, [0, 1, 2])
     before = state.clone()
