@@ -186,7 +186,7 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
     R, T, C = x.shape
     N = A.shape[-1]
     given = [t for t in (dt, A, Bm, Cm, D, z, initial_state) if t is not None]
-    if any(t.device != x.device for t in given):
+    if any(t.dim() and t.device != x.device for t in given):
         raise ValueError("selective_scan: tensors of one device")
     if 0 in (R, T, C):
         last = torch.zeros(R, C, N, device=x.device) if initial_state is None else initial_state.float().expand(R, C, N)
@@ -198,13 +198,13 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
     def fit(t, *size):
         if t is None:
             return None
-        t = t if one else t.float()
+        t = (t if one else t.float()).to(x.device)                                       # (a number may lie elsewhere)
         return _dense(t if t.shape == size else t.expand(size))
 
     def fp32(t, *size):
         if t is None or (t.dtype is torch.float32 and t.shape == size and t.is_contiguous()):
             return t
-        return t.float().expand(size).contiguous()
+        return t.to(x.device).float().expand(size).contiguous()
     ins = (fit(x, R, T, C), fit(dt, R, T, C), fp32(A, C, N), fit(Bm, R, T, N), fit(Cm, R, T, N), fp32(D, C), fit(z, R, T, C), fp32(initial_state, R, C, N))
     y, last = _forward(*ins, softplus, False)[:2] if L.unrecorded(*ins) else _SelectiveScan.apply(*ins, softplus)
     return y.to(out_type), last

@@ -166,6 +166,20 @@ def test_types_that_differ_and_what_broadcasts():
     check(got, fit(want), fit(size), 37, 24, 24 * 8, most(whole))                # (sums of 24 more terms)
 
 
+def test_a_number_of_the_cpu_among_the_tensors():
+    """A tensor of no dimensions broadcasts from wherever it lies, as in the plain operators; it has its gradient there."""
+    t = inputs(2, 20, 16, 8, FP32, DEV, 6, initial=True)
+    number = torch.tensor(0.75, requires_grad=True)
+    y, _ = scan.selective_scan(t["x"], t["dt"], t["a"], t["b"], t["c"], number, t["z"], softplus=True)
+    same = number.detach().to(DEV).expand(16).contiguous().requires_grad_()
+    want, _ = scan.selective_scan(t["x"], t["dt"], t["a"], t["b"], t["c"], same, t["z"], softplus=True)
+    y.sum().backward(), want.sum().backward()
+    assert torch.equal(y, want) and number.grad.device == number.device
+    assert torch.allclose(number.grad, same.grad.sum().cpu(), rtol=16 * 2.0 ** -24, atol=16 * 2.0 ** -24 * float(same.grad.abs().sum()))
+    bare = scan.selective_scan(t["x"], torch.tensor(0.5), t["a"], t["b"], t["c"])[0]
+    assert torch.equal(bare, scan.selective_scan(t["x"], torch.full_like(t["dt"], 0.5), t["a"], t["b"], t["c"])[0])
+
+
 def test_layouts():
     """Columns of wider rows, tokens in front of rows, a batch of one at any stride: the same bits."""
     t = inputs(3, 50, 36, 16, BF16, DEV, 7)
