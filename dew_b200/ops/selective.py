@@ -327,7 +327,7 @@ def selective_tokens(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, Bm:
     _check("selective_tokens", x, dt, Bm, Cm, z, (A_log, D), state, rows, (C, N), C, C, N)
     if A_log.shape != (C, N) or (D is not None and D.shape != (C,)):
         raise ValueError(f"selective_tokens: A_log [{C}, states] and D [{C}], got {tuple(A_log.shape)}, {None if D is None else tuple(D.shape)}")
-    if N > MOST_STATES or 0 in x.shape or not kernel_ok(x, dt, A_log, Bm, Cm, D, z) or L.transformed(x, dt, A_log, Bm, Cm, D, z):
+    if N > MOST_STATES or N == 0 or 0 in x.shape or not kernel_ok(x, dt, A_log, Bm, Cm, D, z) or L.transformed(x, dt, A_log, Bm, Cm, D, z):
         return selective_tokens_reference(x, dt, A_log, Bm, Cm, D, z, rows, state) if 0 not in x.shape else torch.zeros_like(x)
     return _tokens(x, dt, z, Bm, Cm, A_log, None, D, whole(*x.shape[:2], x.device) if rows is None else rows, state, N, 1, 0)
 

@@ -120,3 +120,5 @@ def test_empty_calls():
     t = inputs(2, 3, 8, 4, torch.float32, "cpu", 7)
     y = selective.selective_tokens(t["x"][:0], t["dt"][:0], torch.log(-t["a"]), t["b"][:0], t["c"][:0], t["d"], t["z"][:0])
     assert y.shape == (0, 3, 8)
+    none = selective.selective_tokens(t["x"], t["dt"], torch.zeros(8, 0), t["b"][..., :0], t["c"][..., :0], t["d"])
+    assert torch.equal(none, t["x"] * t["d"])
