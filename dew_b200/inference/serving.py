@@ -97,7 +97,7 @@ class Server:
         self.store = make_cache(model, slots, capacity, self.spec)
         if self.store.keeps_state:
             prefix_cache = False          # a recurrent state stands for a whole row: no page of another row brings it along
-        if self.store.slots is not None and host_pages > 0:
+        if self.store.slots is not None and host_pages > 0 and self.store.pools():
             raise NotImplementedError("the host tier copies pages of caches whose layers all keep the same heads")
         self.host_tier = HostTier(self.store, host_pages) if host_pages > 0 and prefix_cache else None
         self.ledger = PageLedger(pool, self.spec.page_size, prefix_cache, self.host_tier)

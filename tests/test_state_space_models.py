@@ -77,6 +77,17 @@ def test_generation_and_server(kind):
     assert [t.result() for t in group] == [want[0], want[0]]
 
 
+def test_options_that_concern_pages_alone():
+    """A server of states has no pages to quantise, share or keep on the host; it is asked for them all the same, as one of keys would be."""
+    m = model("mamba")
+    asked = prompts(2)
+    server = Server(m, slots=2, capacity=256, kv_cache=KVCache(quantized="int8", page_size=16), host_pages=8, shared_prefix=True, sampling=Sampling(temperature=0.0))
+    assert server(asked, 4) == [greedy(m, p, 4) for p in asked]
+    server.compact()
+    server.resize(40)
+    assert server(asked, 4) == [greedy(m, p, 4) for p in asked]
+
+
 @pytest.mark.parametrize("kind", sorted(OPTIONS))
 def test_the_plain_cache_of_recurrent_layers(kind):
     m = model(kind)
@@ -126,6 +137,12 @@ def test_convolution_with_an_offset(silu, device="cpu", dtype=torch.float32):
     assert torch.allclose(got.double(), want, **close) and torch.allclose(torch.cat(parts, 1).double(), want, **close)
 
 
+@pytest.mark.parametrize("add", [torch.zeros(7), torch.zeros(1, 8), torch.zeros(8, device="meta")])
+def test_offsets_that_a_convolution_refuses(add):
+    with pytest.raises(ValueError, match="offset"):
+        token_mix.conv_tokens(torch.zeros(2, 9, 8), torch.zeros(8, 4), None, False, None, None, add)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_convolution_with_an_offset_gpu(dtype):
@@ -137,12 +154,6 @@ def test_convolution_with_an_offset_gpu(dtype):
 @pytest.mark.parametrize("graph", [False, True])
 @pytest.mark.parametrize("kind", sorted(OPTIONS))
 def test_server_on_a_gpu(kind, graph):
-@pytest.mark.parametrize("add", [torch.zeros(7), torch.zeros(1, 8), torch.zeros(8, device="meta")])
-def test_offsets_that_a_convolution_refuses(add):
-    with pytest.raises(ValueError, match="offset"):
-        token_mix.conv_tokens(torch.zeros(2, 9, 8), torch.zeros(8, 4), None, False, None, None, add)
-
-
     """fp32 weights: the same tokens as the whole row on the CPU, through prompts in chunks, forks and (captured) steps."""
     m = model(kind)
     asked = prompts()
