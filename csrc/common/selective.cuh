@@ -178,7 +178,7 @@ __device__ __forceinline__ void twice(float2* to, const Raw<T>& r) {
 
 // Whether four values at multiples of four columns can be read as one piece.
 template <typename T>
-__device__ __forceinline__ bool fours(const void* p, long long row, long long token) {
+__host__ __device__ __forceinline__ bool fours(const void* p, long long row, long long token) {
   return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0 && ((row | token) & 3) == 0;
 }
 

@@ -10,7 +10,8 @@
 // What bounds scan_kernel is the exponential of every token, channel and state: the special-function unit takes eight cycles for a warp's, so 4 rows of 2048 tokens of 4096 channels of 16
 // states cannot take less than 119 us (149 with those of steps and gates; the bytes, 41).  The ENDS pass comes to 75 % of that rate; the other reaches 56 to 70 %, where a SM has 16
 // warps: 247 us in eight segments and 162 for their ends, or 399 for whole rows with two states a lane and 7 warps an SM, whose chains are then what takes the time (a warp waits 1.8
-// of 5 cycles for the instruction before, 1.1 for an exponential or shared memory).  token_kernel is bound by memory: 128 rows of 8192 channels 32 us, 4.3 TB/s.
+// of 5 cycles for the instruction before, 1.1 for an exponential or shared memory).  token_kernel is bound by memory: 128 rows of 8192 channels 27 us, 4.9 TB/s (32 where
+// every load asks whether its channel and states are there: 450 instructions a row of 32 channels; states three rows ahead in shared memory instead of one in registers: 27).
 #include "../common/selective.cuh"
 
 namespace dewb {
@@ -266,28 +267,28 @@ scan_kernel(const Args p) {
 
 // One token per row; a warp owns 32 channels of `rows_each` rows, whose rates it reads once.  A lane holds four states of
 // each of channels lane / 4 + 8 j (so that a load of all lanes is 512 bytes in a row), and forms the step, gate and output of that of j = own_channel(lane % 4); more than 16 states go by
-// in sixteens.  The next row's states are on their way while one is worked on.
+// in sixteens.  ALL: a warp's channels and a lane's states are all there, from boundaries of four.  The next row's states are on their way while one is worked on.
 // grid (ceil(C / 128), ceil(R / rows_each)).
-template <typename T, bool ONE>
+template <typename T, bool ONE, bool ALL>
 __global__ void __launch_bounds__(THREADS)
 token_kernel(const Args p, int rows_each) {
   const int lane = threadIdx.x & 31, sl = lane & 3, c4 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 32 + (lane >> 2), c = c4 + 8 * own_channel(sl);
-  const bool on = c < p.C, whole = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.initial) & 15) == 0;
+  const bool on = ALL || c < p.C, whole = ALL || ((p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.initial) & 15) == 0);
   if (c4 - (lane >> 2) >= p.C) return;
   const float skip = p.d != nullptr && on ? p.d[c] : 0.f;
   float a[4][4];
   auto rates = [&](int n0) {
     const int n = n0 + sl * 4;
-    const bool all = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && n < p.N;
+    const bool all = ALL || ((p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && n < p.N);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int there = c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
+      const int there = ALL ? 4 : c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
       fetch(p.a + static_cast<long long>(c4 + 8 * j) * p.N + n, all && there == 4, there).get(a[j]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) a[j][k] = k < there ? (p.log_a ? -expf(a[j][k]) : a[j][k]) * LOG2E : 0.f;
     }
   };
-  const bool b_whole = (p.N & 3) == 0 && fours<T>(p.b, p.b_row, 0), c_whole = (p.N & 3) == 0 && fours<T>(p.c, p.c_row, 0);
+  const bool b_whole = ALL || ((p.N & 3) == 0 && fours<T>(p.b, p.b_row, 0)), c_whole = ALL || ((p.N & 3) == 0 && fours<T>(p.c, p.c_row, 0));
   const int first = blockIdx.y * rows_each, rows = min(rows_each, p.R - first);
   // the rows' places, a lane each: what a row's loads begin with is there before its turn
   const Row mine = lane < rows ? row_of(p, first + lane) : Row{0, false, 0};
@@ -303,12 +304,12 @@ token_kernel(const Args p, int rows_each) {
     const int n = n0 + sl * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int there = it.held && c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
-      it.h[j] = fetch(it.state + static_cast<long long>(8 * j) * p.N + n, whole && there == 4, there);
+      const int there = it.held && (ALL || c4 + 8 * j < p.C) ? ALL ? 4 : max(0, min(4, p.N - n)) : 0;
+      it.h[j] = fetch(it.state + static_cast<long long>(8 * j) * p.N + n, whole && there == 4, ALL ? 0 : there);
     }
   };
   auto narrow = [&](Item& it, int row, int n0) {
-    const int n = n0 + sl * 4, there = max(0, min(4, p.N - n));
+    const int n = n0 + sl * 4, there = ALL ? 4 : max(0, min(4, p.N - n));
     it.b = fetch(static_cast<const T*>(p.b) + row * p.b_row + n, b_whole && there == 4, there);
     it.c = fetch(static_cast<const T*>(p.c) + row * p.c_row + n, c_whole && there == 4, there);
   };
@@ -355,7 +356,7 @@ token_kernel(const Args p, int rows_each) {
           h[k] = fmaf(ex2(sj * a[j][k]), h[k], uj * b[k]);
           out[j] = fmaf(h[k], cv[k], out[j]);
         }
-        if (c4 + 8 * j < p.C) put(it.state + static_cast<long long>(8 * j) * p.N + n, h, whole && n < p.N, p.N - n);
+        if (ALL || c4 + 8 * j < p.C) put(it.state + static_cast<long long>(8 * j) * p.N + n, h, ALL || (whole && n < p.N), p.N - n);
       }
       if (ONE) break;
     }
@@ -405,8 +406,16 @@ int token_any(const Args& p, cudaStream_t stream) {
   const int across = (p.C + THREADS - 1) / THREADS, rows_each = p.states_each;
   const dim3 grid(across, (p.R + rows_each - 1) / rows_each);
   if (grid.y > 65535) return -3;
-  if (p.N <= 16) token_kernel<T, true><<<grid, THREADS, 0, stream>>>(p, rows_each);
-  else token_kernel<T, false><<<grid, THREADS, 0, stream>>>(p, rows_each);
+  const bool all = (p.N & 15) == 0 && (p.C & 31) == 0 && ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.last)) & 15) == 0 && fours<T>(p.b, p.b_row, 0) &&
+                   fours<T>(p.c, p.c_row, 0);
+  if (p.N <= 16) {
+    if (all) token_kernel<T, true, true><<<grid, THREADS, 0, stream>>>(p, rows_each);
+    else token_kernel<T, true, false><<<grid, THREADS, 0, stream>>>(p, rows_each);
+  } else if (all) {
+    token_kernel<T, false, true><<<grid, THREADS, 0, stream>>>(p, rows_each);
+  } else {
+    token_kernel<T, false, false><<<grid, THREADS, 0, stream>>>(p, rows_each);
+  }
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -63,8 +63,8 @@ def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward
 
 
 def _rows_each(R: int, C: int) -> int:
-    """Rows of a step whose rates a block of 128 channels reads once: so many that all blocks are on the GPU together, five an SM (128 rows of 8192 channels, 1, 4, 8, 12, 16 rows: 54, 36,
-    38, 32, 36 us; 32 rows of 4096, 1, 2, 4 rows: 10.8, 8.7, 11.2)."""
+    """Rows of a step whose rates a block of 128 channels reads once: so many that all blocks are on the GPU together, five an SM (128 rows of 8192 channels, 1, 4, 8, 12, 16 rows: 37, 28,
+    30, 27, 30 us; 32 rows of 4096, 1, 2, 4 rows: 8.0, 6.8, 8.3; 256 of 2048, 2, 6, 8 rows: 18, 16, 17)."""
     return max(1, min(32, -(-R * -(-C // 128) // 740)))
 
 
