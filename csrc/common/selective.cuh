@@ -29,6 +29,7 @@ extern "C" struct dewb_selective_args {
   int softplus, log_a, dt_fp32, stored;      // `stored`: rows of the store, where row_ids or positions name them
   int* status;                         // told of a row outside the store, which then has no tokens
 };
+static_assert(sizeof(dewb_selective_args) == 280, "packed by ops/selective.py");
 
 namespace dewb {
 namespace selective {

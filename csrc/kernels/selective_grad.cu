@@ -29,6 +29,7 @@ extern "C" struct dewb_selective_grad_args {
   float *da, *dd, *dinitial;           // [C, N], [C], [R, C, N]; dd and dinitial may be null
   float *bc_parts, *a_parts, *d_parts; // [channel blocks, R * T, 2, padded N], [R * segments, padded, padded N], [R * segments, padded]
 };
+static_assert(sizeof(dewb_selective_grad_args) == 280 + 120, "packed by ops/selective.py");
 
 namespace dewb {
 namespace selective {

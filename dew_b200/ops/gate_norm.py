@@ -9,7 +9,6 @@ import torch.nn.functional as F
 from . import library as L
 
 
-
 def _blocks(rows: int, row_bytes: int) -> int:
     """Blocks that walk the rows of a backward: as many as an SM holds of them (8192 rows of 1024 bf16 values: 148, 296, 592, 1184 blocks 64, 39, 29, 34 us with the sum of their parts)."""
     if row_bytes <= 1024:                  # a row a warp
@@ -35,25 +34,30 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(x, z, w, eps: float) -> torch.Tensor:
+    if not L.device_is_current(x):
+        with L.on_device_of(x):
+            return _forward(x, z, w, eps)
     x2, z2, w = _rows(x), _rows(z), w.contiguous()
     rows, d = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with L.on_device_of(x) as stream:
-        L.check(L.load().dewb_gate_norm_fwd(x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), y.data_ptr(), rows, d, eps, int(x.dtype is torch.float32),
-                                            int(w.dtype is torch.float32), stream), "gate_norm_fwd")
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    L.check(L.load().dewb_gate_norm_fwd(x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), y.data_ptr(), rows, d, eps, int(x.dtype is torch.float32),
+                                        int(w.dtype is torch.float32), L.stream()), "gate_norm_fwd")
     L.count_launches()
     return y
 
 
 def _backward(x, z, w, eps: float, dy):
+    if not L.device_is_current(x):
+        with L.on_device_of(x):
+            return _backward(x, z, w, eps, dy)
+    L.ensure_device(x)                                       # (a thread of autograd's may come here first)
     x2, z2, w, dy2 = _rows(x), _rows(z), w.contiguous(), _rows(dy.to(x.dtype))
     rows, d = x2.shape
-    dx, dz, dw = (torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, z, w))
+    dx, dz, dw = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, z, w))
     blocks = _blocks(rows, d * x.element_size())
     parts = torch.empty(blocks, d, dtype=torch.float32, device=x.device)
-    with L.on_device_of(x) as stream:
-        L.check(L.load().dewb_gate_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), dx.data_ptr(), dz.data_ptr(),
-                                            dw.data_ptr(), parts.data_ptr(), blocks, rows, d, eps, int(x.dtype is torch.float32), int(w.dtype is torch.float32), stream), "gate_norm_bwd")
+    L.check(L.load().dewb_gate_norm_bwd(dy2.data_ptr(), dy2.stride(0), x2.data_ptr(), x2.stride(0), z2.data_ptr(), z2.stride(0), w.data_ptr(), dx.data_ptr(), dz.data_ptr(),
+                                        dw.data_ptr(), parts.data_ptr(), blocks, rows, d, eps, int(x.dtype is torch.float32), int(w.dtype is torch.float32), L.stream()), "gate_norm_bwd")
     L.count_launches(2)
     return dx, dz, dw
 

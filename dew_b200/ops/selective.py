@@ -5,7 +5,8 @@ forms go token by token (``selective_tokens_reference``, ``ssd_tokens_reference`
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+import struct
+from typing import NamedTuple, Optional
 
 import torch
 import torch.nn.functional as F
@@ -16,20 +17,9 @@ from .token_mix import Rows, kernel_ok, whole
 MOST_STATES, MOST_HEAD_STATES = 128, 256
 EVERY = 16               # tokens between two states that the forward keeps for the backward
 
-_FIELDS = (("x dt z b c", ctypes.c_void_p), ("x_row x_token dt_row dt_token z_row z_token b_row b_token c_row c_token", ctypes.c_longlong),
-           ("a dt_bias d initial last y checkpoints starts sums positions lengths row_ids", ctypes.c_void_p),
-           ("R T C N groups heads segments segment padded states_each softplus log_a dt_fp32 stored", ctypes.c_int), ("status", ctypes.c_void_p))
-
-
-class _Args(ctypes.Structure):
-    """``dewb_selective_args`` of ``csrc/common/selective.cuh``."""
-    _fields_ = [(name, kind) for names, kind in _FIELDS for name in names.split()]
-
-
-class _Grad(ctypes.Structure):
-    """``dewb_selective_grad_args`` of ``csrc/kernels/selective_grad.cu``."""
-    _fields_ = [("f", _Args), ("dy", ctypes.c_void_p), ("dy_row", ctypes.c_longlong), ("dy_token", ctypes.c_longlong)] + \
-               [(name, ctypes.c_void_p) for name in "dlast dx ddt dz db dc da dd dinitial bc_parts a_parts d_parts".split()]
+# ``dewb_selective_args`` of ``csrc/common/selective.cuh`` and ``dewb_selective_grad_args`` of ``csrc/kernels/selective_grad.cu``, packed in one call (a ctypes structure of 42 fields takes five
+# microseconds to fill, a step's call of one token all in all 20)
+_ARGS, _GRAD = struct.Struct("@5P10q12P14iP"), struct.Struct("@P2q12P")
 
 
 def _padded(C: int, N: int, groups: int = 1, heads: int = 0):
@@ -79,34 +69,48 @@ def _strides(t: torch.Tensor):
     return row if shape[0] > 1 else 0, token if shape[1] > 1 else 0
 
 
+class _Call(NamedTuple):
+    """A launch's arguments, how it cuts rows and deals states, and the workspace that has to live until it is issued."""
+    packed: bytes
+    segments: int
+    each: int
+    work: Optional[torch.Tensor]
+
+
 def _args(x, dt, z, b, c, a, dt_bias, d, initial, last, y, checkpoints, rows: Optional[Rows], N: int, groups: int, heads: int, softplus: bool, log_a: bool, stored: int = 0,
-          token: bool = False, backward: bool = False, whole: bool = False):
-    """The arguments of a launch, and what has to live until it is issued."""
+          token: bool = False, backward: bool = False, whole: bool = False) -> _Call:
     R, T, C = x.shape
+    at, starts, sums, segments, work = L.at, 0, 0, 1, None
     channels, states, _ = _padded(C, N, groups, heads)
-    segment, each = (EVERY, _rows_each(R, C)) if token else (-(-T // EVERY) * EVERY, 4) if whole else _split(R, T, C, N, groups, heads, backward, x.dtype is torch.float32)
-    segments = -(-T // segment)
-    work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device) if segments > 1 else None
-    starts, sums = (work.data_ptr(), work.data_ptr() + 4 * R * segments * channels * states) if segments > 1 else (0, 0)
-    at, positions, lengths, ids = L.at, 0, 0, 0
-    if rows is not None:
-        positions, lengths, ids = rows.positions.data_ptr(), rows.lengths.data_ptr(), at(rows.row_ids)
-    z_row, z_token = (0, 0) if z is None else _strides(z)
-    args = _Args(x.data_ptr(), dt.data_ptr(), at(z), b.data_ptr(), c.data_ptr(), *_strides(x), *_strides(dt), z_row, z_token, *_strides(b), *_strides(c), a.data_ptr(), at(dt_bias), at(d),
-                 at(initial), at(last), at(y), at(checkpoints), starts, sums, positions, lengths, ids, R, T, C, N, groups, heads, segments, segment, channels // groups, each, softplus, log_a,
-                 dt.dtype is torch.float32, stored, L.status(x.device).data_ptr())
-    return args, work
-
-
-def _launch(args: _Args, fp32: bool, token: bool, stream: int) -> None:
-    lib, at = L.load(), ctypes.addressof(args)
-    if args.heads:
-        L.check(lib.dewb_head_scan(at, fp32, token, stream), "head_scan")
-    elif token:
-        L.check(lib.dewb_selective_token(at, fp32, stream), "selective_token")
+    if token:
+        segment, each = EVERY, _rows_each(R, C)
+        strides = [0] * 10
+        if R > 1:
+            strides[::2] = x.stride(0), dt.stride(0), 0 if z is None else z.stride(0), b.stride(0), c.stride(0)
     else:
-        L.check(lib.dewb_selective_scan(at, fp32, stream), "selective_scan")
-    L.count_launches(1 if args.segments == 1 else 2)
+        segment, each = (-(-T // EVERY) * EVERY, 4) if whole else _split(R, T, C, N, groups, heads, backward, x.dtype is torch.float32)
+        segments = -(-T // segment)
+        if segments > 1:
+            work = torch.empty(R * segments * channels * (states + 1), dtype=torch.float32, device=x.device)
+            starts = work.data_ptr()
+            sums = starts + 4 * R * segments * channels * states
+        strides = *_strides(x), *_strides(dt), *((0, 0) if z is None else _strides(z)), *_strides(b), *_strides(c)
+    positions, lengths, ids = (0, 0, 0) if rows is None else (rows.positions.data_ptr(), rows.lengths.data_ptr(), at(rows.row_ids))
+    packed = _ARGS.pack(x.data_ptr(), dt.data_ptr(), at(z), b.data_ptr(), c.data_ptr(), *strides, a.data_ptr(), at(dt_bias), at(d), at(initial), at(last), at(y), at(checkpoints), starts, sums,
+                        positions, lengths, ids, R, T, C, N, groups, heads, segments, segment, channels // groups, each, softplus, log_a, dt.dtype is torch.float32, stored,
+                        L.status(x.device).data_ptr())
+    return _Call(packed, segments, each, work)
+
+
+def _launch(call: _Call, heads: bool, fp32: bool, token: bool, stream: int) -> None:
+    lib = L.load()
+    if heads:
+        L.check(lib.dewb_head_scan(call.packed, fp32, token, stream), "head_scan")
+    elif token:
+        L.check(lib.dewb_selective_token(call.packed, fp32, stream), "selective_token")
+    else:
+        L.check(lib.dewb_selective_scan(call.packed, fp32, stream), "selective_scan")
+    L.count_launches(1 if call.segments == 1 else 2)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -114,34 +118,38 @@ def _launch(args: _Args, fp32: bool, token: bool, stream: int) -> None:
 
 
 def _forward(x, dt, a, b, c, d, z, initial, softplus: bool, keep: bool):
+    if not L.device_is_current(x):
+        with L.on_device_of(x):
+            return _forward(x, dt, a, b, c, d, z, initial, softplus, keep)
     R, T, C = x.shape
     N = a.shape[1]
-    y = torch.empty(R, T, C, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     last = torch.empty(R, C, N, dtype=torch.float32, device=x.device)
     channels, states, _ = _padded(C, N)
     kept = torch.empty(R, -(-T // EVERY), channels, states, dtype=torch.float32, device=x.device) if keep else None
-    with L.on_device_of(x) as stream:
-        args, work = _args(x, dt, z, b, c, a, None, d, initial, last, y, kept, None, N, 1, 0, softplus, False)
-        _launch(args, x.dtype is torch.float32, False, stream)
+    _launch(_args(x, dt, z, b, c, a, None, d, initial, last, y, kept, None, N, 1, 0, softplus, False), False, x.dtype is torch.float32, False, L.stream())
     return y, last, kept
 
 
 def _backward(x, dt, a, b, c, d, z, initial, kept, softplus: bool, dy, dlast):
     """-> dx, ddt, da, db, dc, dd, dz, dinitial."""
+    if not L.device_is_current(x):
+        with L.on_device_of(x):
+            return _backward(x, dt, a, b, c, d, z, initial, kept, softplus, dy, dlast)
+    L.ensure_device(x)                                       # (a thread of autograd's may come here first)
     R, T, C = x.shape
     N, dev = a.shape[1], x.device
     channels, states, wide = _padded(C, N)
-    like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)
+    like = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
     dx, ddt, dz, db, dc, da, dd, dinitial = like(x), like(dt), like(z), like(b), like(c), like(a), like(d), like(initial)
-    with L.on_device_of(x) as stream:
-        args, work = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False, backward=True)
-        # one piece of scratch: parts of dB and dC per channel block, of dA and of dD per row and piece
-        of_bc, of_a = -(-C // (wide * args.states_each)) * R * T * 2 * states, R * args.segments * channels * states
-        scratch = torch.empty(of_bc + of_a + R * args.segments * channels, dtype=torch.float32, device=dev)
-        parts = scratch.data_ptr()
-        grad = _Grad(args, dy.data_ptr(), *_strides(dy), *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial)), parts, parts + 4 * of_bc, parts + 4 * (of_bc + of_a))
-        L.check(L.load().dewb_selective_grad(ctypes.addressof(grad), x.dtype is torch.float32, stream), "selective_grad")
-        L.count_launches(2 if args.segments == 1 else 3)
+    call = _args(x, dt, z, b, c, a, None, d, initial, None, None, kept, None, N, 1, 0, softplus, False, backward=True)
+    # one piece of scratch: parts of dB and dC per channel block, of dA and of dD per row and piece
+    of_bc, of_a = -(-C // (wide * call.each)) * R * T * 2 * states, R * call.segments * channels * states
+    scratch = torch.empty(of_bc + of_a + R * call.segments * channels, dtype=torch.float32, device=dev)
+    parts = scratch.data_ptr()
+    grad = _GRAD.pack(dy.data_ptr(), *_strides(dy), *(L.at(t) for t in (dlast, dx, ddt, dz, db, dc, da, dd, dinitial)), parts, parts + 4 * of_bc, parts + 4 * (of_bc + of_a))
+    L.check(L.load().dewb_selective_grad(call.packed + grad, x.dtype is torch.float32, L.stream()), "selective_grad")
+    L.count_launches(2 if call.segments == 1 else 3)
     return dx, ddt, da, db, dc, dd, dz, dinitial
 
 
@@ -261,10 +269,10 @@ def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: in
             return _tokens(x, dt, z, b, c, a, dt_bias, d, rows, state, N, groups, heads)
     x, dt, z, b, c = _dense(x), _dense(dt), _dense(z), _dense(b), _dense(c)
     a, dt_bias, d = _fp32(a), _fp32(dt_bias), _fp32(d)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     token = x.shape[1] == 1 and state is not None
-    args, work = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0], token)
-    _launch(args, x.dtype is torch.float32, token, L.stream())
+    call = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0], token)
+    _launch(call, heads > 0, x.dtype is torch.float32, token, L.stream())
     return y
 
 
@@ -293,8 +301,8 @@ def _chunks(x, dt, b, c, a, dt_bias, d, rows: Rows, state, heads: int, groups: i
     states = torch.empty(R * heads * -(-T // 64) * 64 * 128, dtype=torch.bfloat16, device=dev)
     steps = scratch.data_ptr()
     rates, places = steps + 4 * R * T * heads, steps + 4 * (R * T * heads + heads)
-    args, _ = _args(x, dt, None, b, c, a, dt_bias, d, state, state, y, None, rows, 128, groups, heads, True, True, 0 if state is None else state.shape[0], whole=True)
-    L.check(lib.dewb_head_steps(ctypes.addressof(args), steps, rates, places, stream), "head_steps")
+    call = _args(x, dt, None, b, c, a, dt_bias, d, state, state, y, None, rows, 128, groups, heads, True, True, 0 if state is None else state.shape[0], whole=True)
+    L.check(lib.dewb_head_steps(call.packed, steps, rates, places, stream), "head_steps")
     strides = (ctypes.c_longlong * 6)(*_strides(x), *_strides(b), *_strides(c))
     L.check(lib.dewb_ssd_rows(x.data_ptr(), steps, rates, b.data_ptr(), c.data_ptr(), L.at(d), L.at(state), states.data_ptr(), y.data_ptr(), places, places + 4 * R, places + 8 * R,
                               R, T, heads, groups, ctypes.addressof(strides), stream), "ssd_rows")
@@ -356,7 +364,7 @@ def ssd_tokens(x: torch.Tensor, dt: torch.Tensor, dt_bias: Optional[torch.Tensor
         raise ValueError(f"ssd_tokens: {H} heads in {G} groups of x {tuple(x.shape)}, B {tuple(Bm.shape)}")
     P, N = x.shape[-1] // H, Bm.shape[-1] // G
     _check("ssd_tokens", x, dt, Bm, Cm, None, (A_log, dt_bias, D), state, rows, (H, P, N), H * P, H, G * N)
-    if any(t is not None and t.shape != (H,) for t in (dt_bias, A_log, D)):
+    if A_log.shape != (H,) or (dt_bias is not None and dt_bias.shape != (H,)) or (D is not None and D.shape != (H,)):
         raise ValueError(f"ssd_tokens: a number per head, {H}, for A_log, the steps' bias and D")
     if N > MOST_HEAD_STATES or 0 in x.shape or N == 0 or not kernel_ok(x, dt, dt_bias, A_log, Bm, Cm, D) or L.transformed(x, dt, dt_bias, A_log, Bm, Cm, D):
         return ssd_tokens_reference(x, dt, dt_bias, A_log, Bm, Cm, D, H, G, rows, state) if 0 not in x.shape else torch.zeros_like(x)

@@ -116,6 +116,11 @@ def test_refusals(kind, what, change):
     refused(kind, what, change)
 
 
+def test_the_size_of_what_the_launchers_are_given():
+    """What the kernels' sources assert of their structures."""
+    assert selective._ARGS.size == 280 and selective._GRAD.size == 120
+
+
 def test_empty_calls():
     t = inputs(2, 3, 8, 4, torch.float32, "cpu", 7)
     y = selective.selective_tokens(t["x"][:0], t["dt"][:0], torch.log(-t["a"]), t["b"][:0], t["c"][:0], t["d"], t["z"][:0])
