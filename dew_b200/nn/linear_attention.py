@@ -36,13 +36,17 @@ class ShortConv(nn.Module):
             self.weight.uniform_(-bound, bound, generator=generator)
 
     def forward(self, x, segment_ids=None, cache=None):
-        if cache is not None and x.shape[1] == 1:
+        """``cache [B, K-1, C]``: the row's inputs in front of ``x`` (zeros: none), which move on in place."""
+        if cache is None:
+            return scan.short_conv(x, self.weight, self.bias, self.activation, segment_ids)
+        if x.shape[1] == 1:
             return scan.short_conv_step(x[:, 0], self.weight, self.bias, cache, self.activation)[:, None]
-        y = scan.short_conv(x, self.weight, self.bias, self.activation, segment_ids)
-        if cache is not None:
-            K = self.kernel_size
-            tail = x[:, -(K - 1):]
-            cache[:, -tail.shape[1]:] = tail.to(cache.dtype)
+        kept, tokens = self.kernel_size - 1, x.shape[1]
+        window = torch.cat([cache.to(x.dtype), x], 1)
+        if segment_ids is not None:            # (what was kept belongs to the first token's document)
+            segment_ids = torch.cat([segment_ids[:, :1].expand(-1, kept), segment_ids], 1)
+        y = scan.short_conv(window, self.weight, self.bias, self.activation, segment_ids)[:, kept:]
+        cache.copy_(window[:, tokens:])
         return y
 
 

@@ -1,0 +1,56 @@
+"""Decoders of state space layers where a call is unusual: caches in pieces, caches without a place for a state, packed documents, other types, options of a store."""
+import pytest
+import torch
+
+from dew_b200.nn.linear_attention import RecurrentCache, ShortConv
+from dew_b200.sampling.text import make_cache
+from selective_cases import draws_of_its_own  # noqa: F401
+from test_state_space_models import OPTIONS, model
+
+
+# a piece in front and behind, pieces shorter than the three inputs that a convolution of four taps keeps, single tokens between them
+@pytest.mark.parametrize("pieces", [(20, 20), (6, 6, 28), (1, 2, 2, 1, 34), (2, 1, 3, 4, 30), (39, 1)])
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_the_plain_cache_in_pieces(kind, pieces):
+    m = model(kind)
+    tokens = torch.randint(1, 97, (2, 40))
+    cache, got, at = RecurrentCache(make_cache(m, 2, 64)), [], 0
+    with torch.no_grad():
+        want = m(tokens)
+        for n in pieces:
+            got.append(m(tokens[:, at:at + n], positions=torch.arange(at, at + n)[None].expand(2, n), cache=cache))
+            at += n
+    assert torch.allclose(torch.cat(got, 1), want, atol=1e-4)
+
+
+@pytest.mark.parametrize("taps", [1, 2, 4, 7])
+def test_a_convolution_goes_on_from_its_last_inputs(taps):
+    conv, x = ShortConv(6, taps, bias=True), torch.randn(2, 30, 6)
+    with torch.no_grad():
+        want, kept, got = conv(x), torch.zeros(2, taps - 1, 6), []
+        for lo, hi in ((0, 9), (9, 10), (10, 12), (12, 15), (15, 30)):
+            got.append(conv(x[:, lo:hi], cache=kept))
+            assert torch.equal(kept, torch.cat([torch.zeros(2, taps, 6), x[:, :hi]], 1)[:, taps + hi - (taps - 1):])
+        assert torch.allclose(torch.cat(got, 1), want, atol=1e-6)
+        # documents packed into a row: what was kept belongs to the first of them
+        segments = torch.tensor([[0] * 5 + [1] * 10] * 2)
+        again = conv(x[:, 15:], segments, x[:, 15 - (taps - 1):15].clone())
+        assert torch.allclose(again, torch.cat([conv(x[:, :20])[:, 15:], conv(x[:, 20:])], 1), atol=1e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_the_plain_cache_in_pieces_in_bf16(kind):
+    """As near to fp32 as the whole row in bf16 is."""
+    more = dict(mixer_options=dict(state_dim=128, head_dim=64, groups=1)) if kind == "mamba2" else {}
+    m32, m = model(kind, "cuda", **more), model(kind, "cuda", **more).to(torch.bfloat16)
+    m32.load_state_dict({k: v.float() for k, v in m.state_dict().items()})
+    tokens = torch.randint(1, 97, (3, 160), device="cuda")
+    cache, got, at = RecurrentCache(make_cache(m, 3, 256)), [], 0
+    with torch.no_grad():
+        exact, whole = m32(tokens), m(tokens).float()
+        for n in (70, 2, 1, 67, 20):
+            got.append(m(tokens[:, at:at + n], positions=torch.arange(at, at + n, device="cuda")[None].expand(3, n), cache=cache).float())
+            at += n
+    far = lambda a: float((a - exact).norm() / exact.norm())
+    assert far(torch.cat(got, 1)) < 2 * far(whole) + 1e-3 and far(whole) < 0.1
