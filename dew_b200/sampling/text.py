@@ -143,7 +143,7 @@ def make_cache(model, rows: int, max_len: int, spec: Optional[KVCache] = None, d
     slots = model.cache_slots() if hasattr(model, "cache_slots") else None
     if slots is not None and (spec is None or spec.page_size is None):
         spec = replace(spec or KVCache(), page_size=64)                                     # the paged decode kernels walk tiles of 64 keys
-    if slots is not None and spec.quantized and all(s.state is not None for s in slots):
+    if slots is not None and spec.quantized and all(s.state is not None for slot in slots for s in (slot, slot.beside) if s is not None):
         spec = replace(spec, quantized=None)                                                # (nothing but states: no keys to store in fewer bits)
     layers = len(model.runs()) if hasattr(model, "runs") else cfg.num_layers                # a looped block keeps a cache per pass
     return KVStore(spec or KVCache(), layers, rows, max_len, kvh, hd, dtype or p.dtype, device or p.device, slots=slots)

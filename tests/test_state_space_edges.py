@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from dew_b200.models import CausalTransformer
+from dew_b200.nn.kv_cache import KVCache
 from dew_b200.nn.linear_attention import RecurrentCache, ShortConv
 from dew_b200.sampling.text import make_cache
 from selective_cases import draws_of_its_own  # noqa: F401
@@ -36,6 +38,26 @@ def test_a_convolution_goes_on_from_its_last_inputs(taps):
         segments = torch.tensor([[0] * 5 + [1] * 10] * 2)
         again = conv(x[:, 15:], segments, x[:, 15 - (taps - 1):15].clone())
         assert torch.allclose(again, torch.cat([conv(x[:, :20])[:, 15:], conv(x[:, 20:])], 1), atol=1e-6)
+
+
+def beside(left, right):
+    """Two mixers in every layer."""
+    sides = {"mamba2": ("mamba2", dict(mixer_options=OPTIONS["mamba2"])), "mamba": ("mamba", dict(mixer_options=OPTIONS["mamba"])), "nope": ("nope", {})}
+    return CausalTransformer(vocab_size=97, emb_features=64, num_layers=2, num_heads=4, num_kv_heads=2, max_seq_len=512, mlp_features=96, layer_types=("pair",), fp32_residual=True,
+                             mixer_options=dict(left=sides[left], right=sides[right]), dtype=torch.float32).eval()
+
+
+@pytest.mark.parametrize("left,right", [("mamba2", "nope"), ("nope", "mamba2"), ("mamba2", "mamba"), ("nope", "nope")])
+def test_keys_beside_states_are_asked_for_in_the_type_that_they_are_kept_in(left, right):
+    """Keys in fewer bits are refused wherever there are keys, on either side of a layer; where there are none, nobody misses them."""
+    m = beside(left, right)
+    assert make_cache(m, 2, 64).pools() or "nope" not in (left, right)
+    for kind in ("int8", "float8_e4m3fn"):
+        if "nope" in (left, right):
+            with pytest.raises(NotImplementedError, match="quantised"):
+                make_cache(m, 2, 64, KVCache(quantized=kind))
+        else:
+            assert not make_cache(m, 2, 64, KVCache(quantized=kind)).pools()
 
 
 @pytest.mark.gpu
