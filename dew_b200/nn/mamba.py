@@ -52,6 +52,8 @@ class Mamba(nn.Module):
 
     def forward(self, x, segment_ids=None, cache=None, layer: int = 0, chunked: bool = True, positions=None):
         if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+            if segment_ids is not None:
+                raise NotImplementedError("a state in a cache's slot runs over rows without packed segments")
             return self._in_slot(x, cache, layer, positions)
         xz = self.in_proj(x)
         xi, z = xz[..., :self.inner], xz[..., self.inner:]

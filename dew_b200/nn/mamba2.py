@@ -68,6 +68,8 @@ class Mamba2(nn.Module):
 
     def forward(self, x, segment_ids=None, cache=None, layer: int = 0, positions=None):
         if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+            if segment_ids is not None:
+                raise NotImplementedError("a state in a cache's slot runs over rows without packed segments")
             return self._in_slot(x, cache, layer, positions)
         B, T, _ = x.shape
         zxbcdt = self.in_proj(x)

@@ -60,6 +60,20 @@ def test_keys_beside_states_are_asked_for_in_the_type_that_they_are_kept_in(left
             assert not make_cache(m, 2, 64, KVCache(quantized=kind)).pools()
 
 
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_packed_documents_and_a_state_are_refused(kind):
+    """A slot's state stands for one row: it would run from a document into the next."""
+    m = model(kind)
+    layer, store, x = m.layers[0].mixer, make_cache(m, 2, 64), torch.randn(2, 9, 64)
+    at, segments = torch.arange(9)[None].expand(2, 9), torch.tensor([[0] * 4 + [1] * 5] * 2)
+    before = [t.clone() for t in store.kept_states()]
+    with pytest.raises(NotImplementedError, match="packed"):
+        layer(x, segments, store, 0, positions=at)
+    assert all(torch.equal(a, b) for a, b in zip(before, store.kept_states()))
+    with torch.no_grad():
+        assert torch.allclose(layer(x, None, store, 0, positions=at), layer(x), atol=1e-5)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", sorted(OPTIONS))
 def test_the_plain_cache_in_pieces_in_bf16(kind):
