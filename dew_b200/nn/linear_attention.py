@@ -138,6 +138,15 @@ class GatedDeltaNet(nn.Module):
         return self.out_proj(o.reshape(B, T, self.value_dim))
 
 
+def kept_state(cache, layer: int, batch: int, mixer: nn.Module):
+    """What ``cache`` keeps of ``mixer``, None without a cache; a cache of keys alone is refused, since every call would start from nothing."""
+    if cache is None:
+        return None
+    if not hasattr(cache, "recurrent"):
+        raise NotImplementedError(f"{type(mixer).__name__}: the cache has no place for its state (a RecurrentCache around it has)")
+    return cache.recurrent(layer, batch, mixer)
+
+
 class RecurrentCache:
     """Per-layer decode state of recurrent mixers: the conv window ``[B, K-1, C]`` and the fp32 state ``[B, H, Dk, Dv]``.
     Attention layers of a hybrid stack delegate to the wrapped ``KVStore``."""

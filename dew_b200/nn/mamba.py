@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
-from .linear_attention import ShortConv
+from .linear_attention import ShortConv, kept_state
 
 
 class Mamba(nn.Module):
@@ -57,7 +57,7 @@ class Mamba(nn.Module):
             return self._in_slot(x, cache, layer, positions)
         xz = self.in_proj(x)
         xi, z = xz[..., :self.inner], xz[..., self.inner:]
-        state = cache.recurrent(layer, x.shape[0], self) if cache is not None and hasattr(cache, "recurrent") else None
+        state = kept_state(cache, layer, x.shape[0], self)
         xi = self.conv(xi, segment_ids, state["conv"] if state is not None else None)
         dt, Bm, Cm = self._narrow(xi)
         fn = scan.selective_scan if chunked else scan.selective_scan_reference

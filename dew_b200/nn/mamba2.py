@@ -15,7 +15,7 @@ import torch.nn.functional as F
 from .. import ops
 from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
-from .linear_attention import ShortConv
+from .linear_attention import ShortConv, kept_state
 
 
 class Mamba2(nn.Module):
@@ -74,7 +74,7 @@ class Mamba2(nn.Module):
         B, T, _ = x.shape
         zxbcdt = self.in_proj(x)
         z, xbc, dt = zxbcdt.split([self.inner, self.inner + 2 * self.G * self.N, self.H], -1)
-        state = cache.recurrent(layer, B, self) if cache is not None and hasattr(cache, "recurrent") else None
+        state = kept_state(cache, layer, B, self)
         xbc = self.conv1d(xbc, segment_ids, state["conv"] if state is not None else None)
         xs, Bm, Cm = xbc.split([self.inner, self.G * self.N, self.G * self.N], -1)
         dt = F.softplus(dt.float() + self.dt_bias.float())

@@ -2,10 +2,11 @@
 import pytest
 import torch
 
+from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
 from dew_b200.nn.kv_cache import KVCache
 from dew_b200.nn.linear_attention import RecurrentCache, ShortConv
-from dew_b200.sampling.text import make_cache
+from dew_b200.sampling.text import Sampling, generate, make_cache
 from selective_cases import draws_of_its_own  # noqa: F401
 from test_state_space_models import OPTIONS, model
 
@@ -72,6 +73,23 @@ def test_packed_documents_and_a_state_are_refused(kind):
     assert all(torch.equal(a, b) for a, b in zip(before, store.kept_states()))
     with torch.no_grad():
         assert torch.allclose(layer(x, None, store, 0, positions=at), layer(x), atol=1e-5)
+
+
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_a_cache_without_a_place_for_a_state_is_refused(kind):
+    """State space layers between attention layers that turn by the model's tables: their store has keys alone.  A cache of states around it serves them."""
+    m = model(kind, num_heads=4, layer_types=(kind, "attention"), layer_mlp=None, mlp_features=96, num_layers=2)
+    assert m.cache_slots() is None
+    with pytest.raises(NotImplementedError, match="no place for its state"):
+        generate(m, None, [[3, 4, 5]], 4, sampling=Sampling(temperature=0.0))
+    with pytest.raises(NotImplementedError, match="no place for its state"):
+        Server(m, slots=2, capacity=64, sampling=Sampling(temperature=0.0))([[3, 4, 5]], 4)
+    tokens = torch.randint(1, 97, (2, 20))
+    cache, got = RecurrentCache(make_cache(m, 2, 64)), []
+    with torch.no_grad():
+        for lo, hi in ((0, 9), (9, 16), (16, 17), (17, 20)):
+            got.append(m(tokens[:, lo:hi], positions=torch.arange(lo, hi)[None].expand(2, hi - lo), cache=cache))
+        assert torch.allclose(torch.cat(got, 1), m(tokens), atol=1e-4)
 
 
 @pytest.mark.gpu
