@@ -852,7 +852,7 @@ extern "C" int dewb_ssd_fwd(const void* x, const float* dt, const float* A, cons
   return run_output(k, static_cast<in>(states), static_cast<__nv_bfloat16*>(y), stream);
 }
 
-// The same for a call's rows, with the states of a store: state fp32 [store rows, H, 64, 128] goes on in place, live / from / to [B] as in `Call`; dt fp32 [B, T, H], zeros where nothing
+// The same for a call's rows, with the states of a store: state fp32 [store rows, H, 64, 128] (on a boundary of 8 bytes, as it is read in pairs) goes on in place, live / from / to [B] as in `Call`; dt fp32 [B, T, H], zeros where nothing
 // counts.  Every state is fp32 through and through: the decayed x enters its products as three bf16 terms, so that a row that comes in many calls is the row in one.  y is formed as
 // above, of states rounded to bf16 once.
 extern "C" int dewb_ssd_rows(const void* x, const float* dt, const float* A, const void* Bm, const void* Cm, const float* D, float* state, void* states, void* y, const int* live,
@@ -862,7 +862,7 @@ extern "C" int dewb_ssd_rows(const void* x, const float* dt, const float* A, con
   const Call k{static_cast<in>(x), static_cast<in>(Bm), static_cast<in>(Cm), nullptr, dt, A, D, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
                B, T, H, G, (T + L - 1) / L, live, from, to};
   int e = check(k);
-  if (e || live == nullptr || from == nullptr || to == nullptr) return e ? e : -3;
+  if (e || live == nullptr || from == nullptr || to == nullptr || (reinterpret_cast<uintptr_t>(state) & 7)) return e ? e : -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const Walk<__nv_bfloat16> forward{state, static_cast<__nv_bfloat16*>(states), state};
   if ((e = walk<3, __nv_bfloat16>(k, forward, nullptr, stream))) return e;

@@ -281,8 +281,9 @@ def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: in
 CHUNKED_TOKENS = 32
 
 
-def _suits_chunks(x, heads: int, groups: int, N: int) -> bool:
-    return (x.dtype is torch.bfloat16 and x.shape[1] >= CHUNKED_TOKENS and x.shape[2] == 64 * heads and N == 128 and heads % 2 == 0 and heads // groups % 2 == 0
+def _suits_chunks(x, heads: int, groups: int, N: int, state: Optional[torch.Tensor] = None) -> bool:
+    """(The chunks read and write states in pairs of floats; the kernels of tokens take them from any float on.)"""
+    return ((state is None or state.data_ptr() % 8 == 0) and x.dtype is torch.bfloat16 and x.shape[1] >= CHUNKED_TOKENS and x.shape[2] == 64 * heads and N == 128 and heads % 2 == 0 and heads // groups % 2 == 0
             and x.shape[0] <= 65535 and hasattr(L.load(), "dewb_ssd_rows"))
 
 
@@ -369,6 +370,6 @@ def ssd_tokens(x: torch.Tensor, dt: torch.Tensor, dt_bias: Optional[torch.Tensor
     if N > MOST_HEAD_STATES or 0 in x.shape or N == 0 or not kernel_ok(x, dt, dt_bias, A_log, Bm, Cm, D) or L.transformed(x, dt, dt_bias, A_log, Bm, Cm, D):
         return ssd_tokens_reference(x, dt, dt_bias, A_log, Bm, Cm, D, H, G, rows, state) if 0 not in x.shape else torch.zeros_like(x)
     rows = whole(*x.shape[:2], x.device) if rows is None else rows
-    if _suits_chunks(x, H, G, N):
+    if _suits_chunks(x, H, G, N, state):
         return _chunks(x, dt, Bm, Cm, A_log, dt_bias, D, rows, state, H, G)
     return _tokens(x, dt, None, Bm, Cm, A_log, dt_bias, D, rows, state, N, G, H)

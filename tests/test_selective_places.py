@@ -1,0 +1,54 @@
+"""States of the scans with a decay per head that begin on odd floats: the chunks read and write them in pairs, so they go token by token there or lie elsewhere first."""
+import ctypes
+
+import pytest
+import torch
+
+from dew_b200.ops import library as L
+from dew_b200.ops import selective
+from selective_cases import draws_of_its_own, rows  # noqa: F401
+
+
+def odd(t):
+    """The same numbers from an odd float on, in one piece."""
+    room = t.new_empty(t.numel() + 1)[1:].view(t.shape).copy_(t)
+    assert room.is_contiguous() and room.data_ptr() % 8 == 4
+    return room
+
+
+class Library:
+    dewb_ssd_rows = None
+
+
+def test_which_states_the_chunks_take(monkeypatch):
+    monkeypatch.setattr(L, "load", lambda: Library)
+    x, state = torch.zeros(2, 32, 256, dtype=torch.bfloat16), torch.zeros(2, 4, 64, 128)
+    assert selective._suits_chunks(x, 4, 2, 128, state) and selective._suits_chunks(x, 4, 2, 128, None)
+    assert not selective._suits_chunks(x, 4, 2, 128, odd(state)) and not selective._suits_chunks(x[:, :31], 4, 2, 128, state)
+
+
+@pytest.mark.skipif(not L.exists(), reason="the library is not built")
+def test_the_launcher_looks():
+    """(Refused before anything is launched: the addresses are the host's.)"""
+    room = torch.zeros(64, dtype=torch.float64)
+    at, strides = room.data_ptr() + (-room.data_ptr()) % 16, (ctypes.c_longlong * 6)()
+    for off in (1, 2, 4, 12):
+        assert L.load().dewb_ssd_rows(at, at, at, at, at, at, at + off, at, at, at, at, at, 1, 64, 2, 1, ctypes.addressof(strides), 0) == -3
+    assert L.load().dewb_ssd_rows(at, at, at, at, at, at, 0, at, at, 0, at, at, 1, 64, 2, 1, ctypes.addressof(strides), 0) == -3      # (no lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 31, 32, 100])
+def test_states_from_an_odd_float_on(S, monkeypatch):
+    """The same bits as from an even one, token by token."""
+    g = torch.Generator("cuda").manual_seed(S)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    call = dict(x=r(2, S, 256).bfloat16(), dt=(r(2, S, 4) - 3).bfloat16(), dt_bias=r(4), A_log=r(4), Bm=r(2, S, 256).bfloat16(), Cm=r(2, S, 256).bfloat16(), D=r(4), H=4, G=2,
+                rows=rows([3, 0], [S, max(1, S - 5)], S, [2, 0], "cuda"))
+    start = r(3, 4, 64, 128)
+    state, beside = odd(start), start.clone()
+    y = selective.ssd_tokens(**call, state=state)
+    monkeypatch.setattr(selective, "CHUNKED_TOKENS", 1 << 30)
+    want = selective.ssd_tokens(**call, state=beside)
+    L.check_status()
+    assert torch.equal(y, want) and torch.equal(state, beside)
