@@ -20,6 +20,7 @@
 //
 // Replaces the reference's ported SSD kernels ChunkState / StatePassing / ChunkScan (src/dew/nn/kernels/mamba_ssd.py:421-660).
 #include <cstdint>
+#include <initializer_list>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include "../common/mma_bf16.cuh"
@@ -809,6 +810,13 @@ static int run_output(const Call& k, const __nv_bfloat16* states, __nv_bfloat16*
   return static_cast<int>(cudaGetLastError());
 }
 
+// (states are read and written in pairs of floats)
+static bool even(std::initializer_list<const float*> states) {
+  for (const float* s : states)
+    if (reinterpret_cast<uintptr_t>(s) & 7) return false;
+  return true;
+}
+
 static int check(const Call& k) {
   if (k.B <= 0 || k.T <= 0 || k.H <= 0 || k.G <= 0 || k.H % k.G != 0 || k.G > 65535) return -3;
   // (batch rows by chunks, and by heads, lie along the grid's first dimension)
@@ -845,7 +853,7 @@ extern "C" int dewb_ssd_fwd(const void* x, const float* dt, const float* A, cons
   const Call k{static_cast<in>(x), static_cast<in>(Bm), static_cast<in>(Cm), nullptr, dt, A, D, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
                B, T, H, G, (T + L - 1) / L};
   int e = check(k);
-  if (e) return e;
+  if (e || !even({initial, last})) return e ? e : -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const Walk<__nv_bfloat16> forward{initial, static_cast<__nv_bfloat16*>(states), last};
   if ((e = walk<1, __nv_bfloat16>(k, forward, nullptr, stream))) return e;
@@ -862,7 +870,7 @@ extern "C" int dewb_ssd_rows(const void* x, const float* dt, const float* A, con
   const Call k{static_cast<in>(x), static_cast<in>(Bm), static_cast<in>(Cm), nullptr, dt, A, D, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
                B, T, H, G, (T + L - 1) / L, live, from, to};
   int e = check(k);
-  if (e || live == nullptr || from == nullptr || to == nullptr || (reinterpret_cast<uintptr_t>(state) & 7)) return e ? e : -3;
+  if (e || live == nullptr || from == nullptr || to == nullptr || !even({state})) return e ? e : -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const Walk<__nv_bfloat16> forward{state, static_cast<__nv_bfloat16*>(states), state};
   if ((e = walk<3, __nv_bfloat16>(k, forward, nullptr, stream))) return e;
@@ -881,7 +889,7 @@ extern "C" int dewb_ssd_bwd(const void* x, const float* dt, const float* A, cons
   const Call k{static_cast<in>(x), static_cast<in>(Bm), static_cast<in>(Cm), static_cast<in>(dy), dt, A, D, strides[0], strides[1], strides[2], strides[3], strides[4],
                strides[5], B, T, H, G, (T + L - 1) / L};
   int e = check(k);
-  if (e) return e;
+  if (e || !even({initial, dlast, states, dstates, dinitial})) return e ? e : -3;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_ptr);
   const Walk<float> forward{initial, states, nullptr}, reverse{dlast, dstates, dinitial};
   if ((e = walk<3, float>(k, forward, &reverse, stream))) return e;

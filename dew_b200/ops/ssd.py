@@ -48,7 +48,12 @@ def _sized(x, dt, A, Bm, Cm, D, initial):
         if t is not None and t.dim() and t.device != x.device:
             raise ValueError(f"ssd: operands on {t.device} and on {x.device}")
     fp32 = lambda t, *size: None if t is None else t.detach().to(x.device).float().expand(size).contiguous()
-    return fp32(dt, B, T, H), fp32(A, H), fp32(D, H), fp32(initial, B, H, HEAD, STATE)
+    return fp32(dt, B, T, H), fp32(A, H), fp32(D, H), _even(fp32(initial, B, H, HEAD, STATE))
+
+
+def _even(t):
+    """A state in one piece, on a boundary of 8 bytes: the kernels read it in pairs of floats."""
+    return t if t is None or t.data_ptr() % 8 == 0 else t.clone()
 
 
 def _forward(x, dt, A, Bm, Cm, D, initial):
@@ -127,7 +132,7 @@ class _SSD(torch.autograd.Function):
         dy = dy.to(torch.bfloat16).contiguous()
         if dy.data_ptr() % 16:
             dy = dy.clone()
-        dx, ddt, dA, dB, dC, dD, dinitial = _backward(*saved, dy, None if dlast is None else dlast.float().contiguous())
+        dx, ddt, dA, dB, dC, dD, dinitial = _backward(*saved, dy, None if dlast is None else _even(dlast.float().contiguous()))
         fit = lambda g, given: None if given is None else g.sum_to_size(given[1]).to(given[0])
         dt_, A_, D_, initial_ = ctx.given
         return dx, fit(ddt, dt_), fit(dA, A_), dB, dC, fit(dD, D_), fit(dinitial, initial_)

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from dew_b200.ops import library as L
-from dew_b200.ops import selective
+from dew_b200.ops import scan, selective
+from dew_b200.ops import ssd as chunks
 from selective_cases import draws_of_its_own, rows  # noqa: F401
 
 
@@ -52,3 +53,39 @@ def test_states_from_an_odd_float_on(S, monkeypatch):
     want = selective.ssd_tokens(**call, state=beside)
     L.check_status()
     assert torch.equal(y, want) and torch.equal(state, beside)
+
+
+@pytest.mark.skipif(not L.exists(), reason="the library is not built")
+def test_the_launchers_of_whole_rows_look():
+    room = torch.zeros(64, dtype=torch.float64)
+    at, strides = room.data_ptr() + (-room.data_ptr()) % 16, (ctypes.c_longlong * 6)()
+    p, i = ctypes.c_void_p, ctypes.c_int
+    sizes = (i(1), i(64), i(2), i(1), strides, p(0))
+    for initial, last in ((4, 0), (0, 12)):
+        assert L.load().dewb_ssd_fwd(*(p(at),) * 6, p(at + initial), p(at), p(at), p(at + last), *sizes) == -3
+    for initial, dlast, dinitial in ((4, 0, 0), (0, 4, 0), (0, 0, 4)):
+        assert L.load().dewb_ssd_bwd(*(p(at),) * 6, p(at + initial), p(at), p(at + dlast), *(p(at),) * 6, *(p(at),) * 6, p(at + dinitial), *sizes) == -3
+
+
+def test_what_the_kernels_are_given_of_states():
+    state = torch.randn(2, 2, 64, 128)
+    assert chunks._even(None) is None and chunks._even(state) is state
+    moved = chunks._even(odd(state))
+    assert torch.equal(moved, state) and moved.data_ptr() % 8 == 0
+
+
+@pytest.mark.gpu
+def test_whole_rows_from_states_and_gradients_on_odd_floats():
+    """The state that rows begin with, and the gradient of the one that they end with."""
+    g = torch.Generator("cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, b, c, dt, a = r(2, 70, 2, 64).bfloat16(), r(2, 70, 1, 128).bfloat16(), r(2, 70, 1, 128).bfloat16(), torch.nn.functional.softplus(r(2, 70, 2) - 3), -torch.exp(r(2))
+    initial, dy, dlast = r(2, 2, 64, 128), r(2, 70, 2, 64).bfloat16(), r(2, 2, 64, 128)
+
+    def run(initial, dlast):
+        leaves = [t.detach().requires_grad_() for t in (x, dt, a, b, c, initial)]
+        out = scan.ssd(*leaves[:5], None, leaves[5])
+        return [o.detach() for o in out] + list(torch.autograd.grad(out, leaves, (dy, dlast)))
+    want, got = run(initial, dlast), run(odd(initial), odd(dlast))
+    L.check_status()
+    assert all(torch.equal(u, v) for u, v in zip(want, got))
