@@ -237,15 +237,15 @@ head_scan_kernel(const Args p) {
   }
 }
 
-// One token per row, a decay per head.  A warp takes `ROWS` rows p of a head's [dim, N] state at a time, LN lanes a row.  grid (heads, parts, R).
+// One token per row, a decay per head.  A warp takes `ROWS` rows p of a head's [dim, N] state at a time, LN lanes a row.  grid R * heads, a row's heads side by side.
 template <typename T, int LN, int NS>
 __global__ void __launch_bounds__(THREADS)
 head_token_kernel(const Args p) {
   constexpr int CG = 32 / LN;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sl = lane % LN, cg = lane / LN;
-  const int head = blockIdx.x, row = blockIdx.z, dim = p.C / p.heads, pos = p.positions[row];
+  const int head = blockIdx.x % p.heads, row = blockIdx.x / p.heads, dim = p.C / p.heads, pos = p.positions[row];
   T* y = static_cast<T*>(p.y) + static_cast<long long>(row) * p.C + head * dim;
-  const int first = (blockIdx.y * WARPS + warp) * 4 * CG, stride = gridDim.y * WARPS * 4 * CG;
+  const int first = warp * 4 * CG, stride = WARPS * 4 * CG;
   const Row r = row_of(p, row);
   if (r.len == 0) {
     for (int q = first; q < dim; q += stride)
@@ -360,8 +360,8 @@ int heads_any(const Args& p, cudaStream_t stream) {
 
 template <typename T>
 int head_token_any(const Args& p, cudaStream_t stream) {
-  const dim3 grid(p.heads, 1, p.R);
-  if (p.R > 65535) return -3;
+  if (static_cast<long long>(p.R) * p.heads > 0x7fffffffLL) return -3;
+  const unsigned grid = static_cast<unsigned>(p.R) * p.heads;
   if (p.N <= 16) head_token_kernel<T, 4, 4><<<grid, THREADS, 0, stream>>>(p);
   else if (p.N <= 32) head_token_kernel<T, 8, 4><<<grid, THREADS, 0, stream>>>(p);
   else if (p.N <= 64) head_token_kernel<T, 16, 4><<<grid, THREADS, 0, stream>>>(p);

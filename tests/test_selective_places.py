@@ -1,4 +1,5 @@
-"""States of the scans with a decay per head that begin on odd floats: the chunks read and write them in pairs, so they go token by token there or lie elsewhere first."""
+"""Where states lie and how many rows a call has, of the scans with a decay per head.  The chunks read and write states in pairs of floats: those that begin on an odd one go token by token
+or lie elsewhere first."""
 import ctypes
 
 import pytest
@@ -89,3 +90,23 @@ def test_whole_rows_from_states_and_gradients_on_odd_floats():
     want, got = run(initial, dlast), run(odd(initial), odd(dlast))
     L.check_status()
     assert all(torch.equal(u, v) for u, v in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [65535, 65537, 200_001])
+def test_a_token_of_many_rows(R):
+    """The rows of one call are the rows of several."""
+    g = torch.Generator("cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    call = dict(x=r(R, 1, 6), dt=r(R, 1, 3) - 3, Bm=r(R, 1, 5), Cm=r(R, 1, 5))
+    heads = dict(dt_bias=r(3), A_log=r(3), D=r(3), H=3, G=1)
+    at = rows([4], [1], 1, None, "cuda")
+    many = at._replace(positions=at.positions.expand(R, 1).contiguous(), lengths=at.lengths.expand(R).contiguous())
+    start = r(R, 3, 2, 5)
+    state, parts = start.clone(), []
+    y = selective.ssd_tokens(**call, **heads, rows=many, state=state)
+    for lo in range(0, R, 30_000):
+        hi = min(R, lo + 30_000)
+        parts.append(selective.ssd_tokens(**{k: v[lo:hi] for k, v in call.items()}, **heads, rows=at._replace(positions=many.positions[lo:hi], lengths=many.lengths[lo:hi]), state=start[lo:hi]))
+    L.check_status()
+    assert torch.equal(y, torch.cat(parts)) and torch.equal(state, start)
