@@ -40,11 +40,12 @@ using Args = dewb_selective_args;
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int OUTSIDE = 6;             // the status of a row that the store does not have
 constexpr int EVERY = 16;              // tokens between two kept states
-constexpr float LN2 = 0.6931471805599453f;
 using special::ex2;
-using special::LOG2E;
+using special::exp_minus;
+using special::LN2;
 using special::rcp;
 using special::sigmoid;
+using special::times_log2e;
 
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
@@ -61,7 +62,7 @@ struct Lay {
 
 // ln(1 + e^x) = max(x, 0) + ln(1 + t), t = e^-|x|: with q = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh q = 2 (q + q^3 / 3 + ... + q^13 / 13), the next term below 2e-8 of the sum
 __device__ __forceinline__ float softplus(float x) {
-  const float t = ex2(-LOG2E * fabsf(x)), q = t * rcp(2.f + t), r = q * q;
+  const float t = exp_minus(x), q = t * rcp(2.f + t), r = q * q;
   float p = fmaf(r, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(p, r, 1.f / 9.f);
   p = fmaf(p, r, 1.f / 7.f);
@@ -237,7 +238,7 @@ template <bool HEADS>
 __device__ __forceinline__ float rate(const Args& p, int c, int n, int dim) {
   if (c >= p.C || n >= p.N) return 0.f;
   const float a = p.a[HEADS ? c / dim : static_cast<long long>(c) * p.N + n];
-  return (p.log_a ? -expf(a) : a) * LOG2E;
+  return times_log2e(p.log_a ? -expf(a) : a);
 }
 
 }  // namespace selective
