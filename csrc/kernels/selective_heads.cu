@@ -14,6 +14,7 @@ namespace dewb {
 namespace selective {
 
 constexpr int EIGHT = 8;               // channels of a lane
+constexpr int MOST_Z = 65535;          // blocks along a grid's third axis
 
 template <int LN, int NS>
 struct HeadLay {
@@ -237,15 +238,15 @@ head_scan_kernel(const Args p) {
   }
 }
 
-// One token per row, a decay per head.  A warp takes `ROWS` rows p of a head's [dim, N] state at a time, LN lanes a row.  grid R * heads, a row's heads side by side.
+// One token per row, a decay per head.  A warp takes `ROWS` rows p of a head's [dim, N] state at a time, LN lanes a row.  grid (heads, parts, rows from `row0` on).
 template <typename T, int LN, int NS>
 __global__ void __launch_bounds__(THREADS)
-head_token_kernel(const Args p) {
+head_token_kernel(const Args p, int row0) {
   constexpr int CG = 32 / LN;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sl = lane % LN, cg = lane / LN;
-  const int head = blockIdx.x % p.heads, row = blockIdx.x / p.heads, dim = p.C / p.heads, pos = p.positions[row];
+  const int head = blockIdx.x, row = row0 + blockIdx.z, dim = p.C / p.heads, pos = p.positions[row];
   T* y = static_cast<T*>(p.y) + static_cast<long long>(row) * p.C + head * dim;
-  const int first = warp * 4 * CG, stride = WARPS * 4 * CG;
+  const int first = (blockIdx.y * WARPS + warp) * 4 * CG, stride = gridDim.y * WARPS * 4 * CG;
   const Row r = row_of(p, row);
   if (r.len == 0) {
     for (int q = first; q < dim; q += stride)
@@ -360,14 +361,16 @@ int heads_any(const Args& p, cudaStream_t stream) {
 
 template <typename T>
 int head_token_any(const Args& p, cudaStream_t stream) {
-  if (static_cast<long long>(p.R) * p.heads > 0x7fffffffLL) return -3;
-  const unsigned grid = static_cast<unsigned>(p.R) * p.heads;
-  if (p.N <= 16) head_token_kernel<T, 4, 4><<<grid, THREADS, 0, stream>>>(p);
-  else if (p.N <= 32) head_token_kernel<T, 8, 4><<<grid, THREADS, 0, stream>>>(p);
-  else if (p.N <= 64) head_token_kernel<T, 16, 4><<<grid, THREADS, 0, stream>>>(p);
-  else if (p.N <= 128) head_token_kernel<T, 32, 4><<<grid, THREADS, 0, stream>>>(p);
-  else if (p.N <= 256) head_token_kernel<T, 32, 8><<<grid, THREADS, 0, stream>>>(p);
-  else return -3;
+  for (long long from = 0; from < p.R; from += MOST_Z) {
+    const int row0 = static_cast<int>(from);
+    const dim3 grid(p.heads, 1, p.R - row0 < MOST_Z ? p.R - row0 : MOST_Z);
+    if (p.N <= 16) head_token_kernel<T, 4, 4><<<grid, THREADS, 0, stream>>>(p, row0);
+    else if (p.N <= 32) head_token_kernel<T, 8, 4><<<grid, THREADS, 0, stream>>>(p, row0);
+    else if (p.N <= 64) head_token_kernel<T, 16, 4><<<grid, THREADS, 0, stream>>>(p, row0);
+    else if (p.N <= 128) head_token_kernel<T, 32, 4><<<grid, THREADS, 0, stream>>>(p, row0);
+    else if (p.N <= 256) head_token_kernel<T, 32, 8><<<grid, THREADS, 0, stream>>>(p, row0);
+    else return -3;
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
