@@ -41,7 +41,8 @@ constexpr int THREADS = 128, WARPS = 4;
 constexpr int OUTSIDE = 6;             // the status of a row that the store does not have
 constexpr int EVERY = 16;              // tokens between two kept states
 using special::ex2;
-using special::exp_minus;
+using special::exp_minus_abs;
+using special::gate;
 using special::LN2;
 using special::rcp;
 using special::sigmoid;
@@ -62,7 +63,7 @@ struct Lay {
 
 // ln(1 + e^x) = max(x, 0) + ln(1 + t), t = e^-|x|: with q = t / (2 + t) <= 1/3, ln(1 + t) = 2 artanh q = 2 (q + q^3 / 3 + ... + q^13 / 13), the next term below 2e-8 of the sum
 __device__ __forceinline__ float softplus(float x) {
-  const float t = exp_minus(x), q = t * rcp(2.f + t), r = q * q;
+  const float t = exp_minus_abs(x), q = t * rcp(2.f + t), r = q * q;
   float p = fmaf(r, 1.f / 13.f, 1.f / 11.f);
   p = fmaf(p, r, 1.f / 9.f);
   p = fmaf(p, r, 1.f / 7.f);

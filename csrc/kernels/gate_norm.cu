@@ -20,7 +20,7 @@ namespace dewb {
 namespace gatenorm {
 
 using namespace rows;
-using special::sigmoid;
+using special::gate;
 
 constexpr int THREADS = 256, WARPS = 8;       // of rows that belong to a warp, and of what is read twice
 
@@ -86,7 +86,7 @@ gate_norm_kernel(const Args p) {
     load_v<V>(x + c, u);
     load_v<V>(z + c, g);
 #pragma unroll
-    for (int j = 0; j < V; ++j) u[j] *= g[j] * sigmoid(g[j]);
+    for (int j = 0; j < V; ++j) u[j] *= g[j] * gate<T>(g[j]);
   };
   float ss = 0.f;
   if constexpr (ITEMS > 0) {
@@ -187,7 +187,7 @@ gate_norm_grad_kernel(const Args p) {
       if (c < p.d) load_w<V>(p, c, w, static_cast<const T*>(nullptr));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float z = now[i].z[j], u = now[i].x[j] * z * sigmoid(z);
+        const float z = now[i].z[j], u = now[i].x[j] * z * gate<T>(z);
         ss = fmaf(u, u, ss);
         if (c < p.d) gu = fmaf(now[i].dy[j] * w[j], u, gu);
       }
@@ -202,7 +202,7 @@ gate_norm_grad_kernel(const Args p) {
       load_w<V>(p, c, w, static_cast<const T*>(nullptr));
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float x = now[i].x[j], z = now[i].z[j], e = now[i].dy[j] * r, sig = sigmoid(z), gate = z * sig, u = x * gate, du = e * w[j] - u * back;
+        const float x = now[i].x[j], z = now[i].z[j], e = now[i].dy[j] * r, sig = gate<T>(z), gate = z * sig, u = x * gate, du = e * w[j] - u * back;
         dw[i][j] = fmaf(e, u, dw[i][j]);
         ox[j] = du * gate;
         oz[j] = du * x * sig * fmaf(z, 1.f - sig, 1.f);
@@ -252,7 +252,7 @@ gate_norm_grad_twice_kernel(const Args p) {
       bring(c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float u = a[j] * b[j] * sigmoid(b[j]);
+        const float u = a[j] * b[j] * gate<T>(b[j]);
         ss = fmaf(u, u, ss);
         gu = fmaf(e[j] * w[j], u, gu);
       }
@@ -264,7 +264,7 @@ gate_norm_grad_twice_kernel(const Args p) {
       bring(c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float sig = sigmoid(b[j]), gate = b[j] * sig, u = a[j] * gate, du = r * e[j] * w[j] - u * back;
+        const float sig = gate<T>(b[j]), gate = b[j] * sig, u = a[j] * gate, du = r * e[j] * w[j] - u * back;
         part[c + j] += e[j] * u * r;
         ox[j] = du * gate;
         oz[j] = du * a[j] * sig * fmaf(b[j], 1.f - sig, 1.f);

@@ -159,7 +159,7 @@ __device__ __forceinline__ void stage(Shared<LN, NS>& sm, const Place<T, TD, LN,
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (steps) s[j] = softplus(s[j]);
-    if (at.z != nullptr) w[j] *= z[j] * sigmoid(z[j]);
+    if (at.z != nullptr) w[j] *= z[j] * gate<T>(z[j]);
     if (!all && (j >= at.left || t0 + t >= t_end)) s[j] = w[j] = 0.f;
     if (STATES) x[j] = !all && (j >= at.left || t0 + t >= t_end) ? 0.f : s[j] * x[j];
     total[j] += s[j];
@@ -447,7 +447,7 @@ grad_kernel(const Grad g) {
         for (int j = 0; j < 4; ++j) {
           dx[j] = fmaf(s[j], r1[j], skip[j] * w[j]);
           ds[j] = fmaf(x[j], r1[j], LN2 * r2[j]);
-          if (p.softplus) ds[j] *= sigmoid(raw_step[j]);
+          if (p.softplus) ds[j] *= gate<TD>(raw_step[j]);
           dd[j] = fmaf(w[j], x[j], dd[j]);
         }
         put(static_cast<T*>(g.dx) + here + tok * p.C, dx, y_whole, at.left);
@@ -460,7 +460,7 @@ grad_kernel(const Grad g) {
           rz.get(z);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float sig = sigmoid(z[j]);
+            const float sig = gate<T>(z[j]);
             z[j] = dy[j] * fmaf(skip[j], x[j], r3[j]) * sig * fmaf(z[j], 1.f - sig, 1.f);
           }
           put(static_cast<T*>(g.dz) + here + tok * p.C, z, y_whole, at.left);

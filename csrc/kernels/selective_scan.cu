@@ -232,7 +232,7 @@ scan_kernel(const Args p) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             o[j] = fmaf(skip[j], xs[j], o[j]);
-            if (z != nullptr) o[j] *= g[j] * sigmoid(g[j]);
+            if (z != nullptr) o[j] *= g[j] * gate<T>(g[j]);
           }
           put(y + static_cast<long long>(t0 + t) * p.C, o, FAST || y_whole, left);
         }
@@ -361,7 +361,7 @@ token_kernel(const Args p, int rows_each) {
       if (ONE) break;
     }
     float o = over_states<4>(out, sl) + skip * it.x;
-    if (p.z != nullptr) o *= it.g * sigmoid(it.g);
+    if (p.z != nullptr) o *= it.g * gate<T>(it.g);
     if (on) st(y, o);
   };
   Item now, next;

@@ -283,8 +283,8 @@ CHUNKED_TOKENS = 32
 
 def _suits_chunks(x, heads: int, groups: int, N: int, state: Optional[torch.Tensor] = None) -> bool:
     """(The chunks read and write states in pairs of floats; the kernels of tokens take them from any float on.)"""
-    return ((state is None or state.data_ptr() % 8 == 0) and x.dtype is torch.bfloat16 and x.shape[1] >= CHUNKED_TOKENS and x.shape[2] == 64 * heads and N == 128 and heads % 2 == 0 and heads // groups % 2 == 0
-            and x.shape[0] <= 65535 and hasattr(L.load(), "dewb_ssd_rows"))
+    return (x.dtype is torch.bfloat16 and x.shape[1] >= CHUNKED_TOKENS and x.shape[2] == 64 * heads and N == 128 and heads % 2 == 0 and heads // groups % 2 == 0
+            and x.shape[0] <= 65535 and (state is None or state.data_ptr() % 8 == 0) and hasattr(L.load(), "dewb_ssd_rows"))
 
 
 def _chunks(x, dt, b, c, a, dt_bias, d, rows: Rows, state, heads: int, groups: int) -> torch.Tensor:
