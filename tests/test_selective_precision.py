@@ -129,3 +129,28 @@ def test_heads_in_32_bits(H, P, N, S):
         # (decays of e^-0.85 and less, 2.8 times as above with terms that differ by 3.7; steps from a softplus and rates from an exponential: FAR and 3 more of each exponent, up to 1.9)
         bound = 2.8 * (12 + 2 * (FAR + 3)) + TERM + FAR
         assert off(y[..., cols], want["y"], size["y"]) <= bound + N and off(state[:, h], want["last"], size["last"]) <= bound
+
+
+@pytest.mark.parametrize("logit,a_log", [(0.0, 0.0), (5.0, 2.77), (2.0, 5.0)])
+def test_states_of_chunks_in_32_bits(logit, a_log):
+    """Also behind decays that are many times what is left of a row: 64 tokens of 80 each, then ends of every length."""
+    g = torch.Generator(DEV).manual_seed(7)
+    r = lambda *s: torch.rand(*s, generator=g, device=DEV) / 2 + 0.75
+    S, H, P, N = 150, 2, 64, 128
+    lengths = [150, 129, 131, 137, 64, 65, 100, 33]
+    R = len(lengths)
+    x, dt, b, c, state = r(R, S, H * P).bfloat16(), (r(R, S, H) + logit - 1).bfloat16(), r(R, S, N).bfloat16(), r(R, S, N).bfloat16(), r(R, H, P, N)
+    rates, before = torch.full((H,), a_log, device=DEV), state.clone()
+    assert selective._suits_chunks(x, H, 1, N, state)
+    y = selective.ssd_tokens(x, dt, None, rates, b, c, None, H, 1, rows([1] * R, lengths, S, None, DEV), state)
+    for i, n in enumerate(lengths):
+        for h in range(H):
+            one = dict(x=x[i:i + 1, :n, h * P:h * P + P], dt=dt[i:i + 1, :n, h:h + 1].expand(1, n, P), a=-rates[h].double().exp().expand(P, N), b=b[i:i + 1, :n], c=c[i:i + 1, :n],
+                       initial=before[i:i + 1, h])
+            want, size = oracle(**one, steps=True), companion(**one, steps=True)
+            # A token's share: its step FAR, products 8, the decay behind it 4 and the roundings of its exponent (steps FAR, rates 4, a sum of 64 in 8 levels: 24 of each unit) where it is
+            # up to 12; smaller shares than e^-12 are off by less than the sum's own roundings, 3 terms of 64 tokens.
+            assert off(state[i:i + 1, h], want["last"], size["last"]) <= FAR + 8 + 4 + 24 * 12 + 3 * 64
+            # y: half a step of bf16 for a weight, a state and itself; weights are of differences of sums: up to 2^-24 of 64 decays, twice
+            most = 64 * float(softplus(dt.double()).max() * rates.double().exp().max())
+            assert off(y[i:i + 1, :n, h * P:h * P + P], want["y"], size["y"]) <= 2.1 * 2 ** 16 + 4 * most
