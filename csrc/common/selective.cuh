@@ -234,12 +234,16 @@ inline bool args_ok(const Args& p) {
   return p.positions == nullptr || (p.lengths != nullptr && p.initial == p.last);
 }
 
+// A rate of minus infinity (a state without memory; what e^A_log gives from 88.8 on) becomes one of -1e30: a step of 0 (a token behind the row's end) or a sum of none leaves a decay of one, where
+// 0 times infinity is no number, and every other step nothing, as the definition has it.
+__device__ __forceinline__ float finite_rate(float a) { return a < -1e30f ? -1e30f : a; }
+__device__ __forceinline__ float rate_of(const Args& p, float a) { return finite_rate(p.log_a ? -expf(a) : a); }
+
 // The rate of channel c's state n times log2 e, 0 outside.
 template <bool HEADS>
 __device__ __forceinline__ float rate(const Args& p, int c, int n, int dim) {
   if (c >= p.C || n >= p.N) return 0.f;
-  const float a = p.a[HEADS ? c / dim : static_cast<long long>(c) * p.N + n];
-  return times_log2e(p.log_a ? -expf(a) : a);
+  return times_log2e(rate_of(p, p.a[HEADS ? c / dim : static_cast<long long>(c) * p.N + n]));
 }
 
 }  // namespace selective

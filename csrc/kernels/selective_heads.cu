@@ -105,13 +105,13 @@ head_scan_kernel(const Args p) {
     }
   }
 
-  float rate_of[4], bias[4], skip[4], total[4] = {0.f, 0.f, 0.f, 0.f};
+  float rates[4], bias[4], skip[4], total[4] = {0.f, 0.f, 0.f, 0.f};
   int head[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int c = min(lc + j, p.C - 1);
     head[j] = c / dim;
-    rate_of[j] = rate<true>(p, c, 0, dim);
+    rates[j] = rate<true>(p, c, 0, dim);
     bias[j] = p.dt_bias != nullptr ? p.dt_bias[head[j]] : 0.f;
     skip[j] = p.d != nullptr && !ENDS ? p.d[head[j]] : 0.f;
   }
@@ -152,7 +152,7 @@ head_scan_kernel(const Args p) {
         const float s = value<TD>(rd[i][j]) + bias[j], step = j < n ? (p.softplus ? softplus(s) : s) : 0.f;
         u[j] = j < n ? step * xs[i][j] : 0.f;
         if (ENDS) total[j] += step;
-        e[j] = ex2(step * rate_of[j]);
+        e[j] = ex2(step * rates[j]);
       }
       reinterpret_cast<float4*>(&sm.step[warp][t][lq])[0] = make_float4(e[0], e[0], e[1], e[1]);
       reinterpret_cast<float4*>(&sm.step[warp][t][lq])[1] = make_float4(e[2], e[2], e[3], e[3]);
@@ -318,7 +318,7 @@ head_steps_kernel(const Args p, float* __restrict__ steps, float* __restrict__ r
       places[2 * p.R + row] = r.len > 0 && p.last != nullptr ? static_cast<int>(r.at) : -1;
     }
     if (row == 0)
-      for (int h = threadIdx.x; h < p.heads; h += 256) rates[h] = p.log_a ? -expf(p.a[h]) : p.a[h];
+      for (int h = threadIdx.x; h < p.heads; h += 256) rates[h] = rate_of(p, p.a[h]);
   }
   const long long all = static_cast<long long>(p.T) * p.heads;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {

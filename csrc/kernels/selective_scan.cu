@@ -285,7 +285,7 @@ token_kernel(const Args p, int rows_each) {
       const int there = ALL ? 4 : c4 + 8 * j < p.C ? max(0, min(4, p.N - n)) : 0;
       fetch(p.a + static_cast<long long>(c4 + 8 * j) * p.N + n, all && there == 4, there).get(a[j]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) a[j][k] = k < there ? times_log2e(p.log_a ? -expf(a[j][k]) : a[j][k]) : 0.f;
+      for (int k = 0; k < 4; ++k) a[j][k] = k < there ? times_log2e(rate_of(p, a[j][k])) : 0.f;
     }
   };
   const bool b_whole = ALL || ((p.N & 3) == 0 && fours<T>(p.b, p.b_row, 0)), c_whole = ALL || ((p.N & 3) == 0 && fours<T>(p.c, p.c_row, 0));

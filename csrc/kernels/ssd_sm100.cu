@@ -104,10 +104,14 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// The exponent of a token's decay.  A head without memory comes with a rate of -1e30 (selective.cuh), and one such exponent for each of its tokens: their sums tell tokens apart however small
+// a step is beside the others.
+__device__ __forceinline__ float exponent(float dt, float A) { return A <= -1e30f ? (dt > 0.f ? 1.f : dt) * -1e30f : dt * A; }
+
 // One warp: the running sums of dt A over a chunk, lane l the tokens 2l and 2l + 1.
 __device__ __forceinline__ void running(float dt0, float dt1, float A, float& g0, float& g1) {
   const int lane = threadIdx.x & 31;
-  const float v0 = dt0 * A, v1 = dt1 * A;
+  const float v0 = exponent(dt0, A), v1 = exponent(dt1, A);
   float incl = v0 + v1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -120,12 +124,15 @@ __device__ __forceinline__ void running(float dt0, float dt1, float A, float& g0
   g1 = before + (v0 + v1);
 }
 
+// Between two tokens, from their running sums; where rates are below zero (`most` 0), two that differ by less than their rounding are not a growth.
+__device__ __forceinline__ float decay(float gi, float gj, float most) { return expf(fminf(gi - gj, most)); }
+
 // ... and from a token's end to the chunk's: the decay that its share of the state has behind it.  (As the difference of two running sums it was off by 2^-24 of these: rates of 16 and steps of
 // 5, a state off by 1.2e-4 of itself, 2e-7 so.)
 __device__ __forceinline__ void remaining(float dt0, float dt1, float A, float& b0, float& b1, float& all) {
   const int lane = threadIdx.x & 31;
-  const float v1 = dt1 * A;
-  float incl = dt0 * A + v1;
+  const float v1 = exponent(dt1, A);
+  float incl = exponent(dt0, A) + v1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const float down = __shfl_down_sync(FULL, incl, o);
@@ -300,6 +307,7 @@ ssd_output(Call k, const __nv_bfloat16* __restrict__ states, __nv_bfloat16* __re
     load_tile<16, 128>(st + L * P * 2, states + ((static_cast<long long>(b) * k.H + h0 + i) * k.chunks + n) * P * N, N, P);
     cp_commit();
   };
+  const float most = k.live == nullptr ? INFINITY : 0.f;
   auto decays = [&](int i) {                           // warp 0
     const int t = t0 + 2 * lane;
     const float* dt = k.dt + static_cast<long long>(b) * k.T * k.H + h0 + i;
@@ -371,8 +379,8 @@ ssd_output(Call k, const __nv_bfloat16* __restrict__ states, __nv_bfloat16* __re
           const float2 gj = *reinterpret_cast<const float2*>(g + j), d = *reinterpret_cast<const float2*>(dt + j);
           const float* w = G[ks * 2 + t];
           const int i0 = row + r, i1 = i0 + 8;
-          a[2 * t] = pack2(j <= i0 ? w[0] * expf(gi0 - gj.x) * d.x : 0.f, j + 1 <= i0 ? w[1] * expf(gi0 - gj.y) * d.y : 0.f);
-          a[2 * t + 1] = pack2(j <= i1 ? w[2] * expf(gi1 - gj.x) * d.x : 0.f, j + 1 <= i1 ? w[3] * expf(gi1 - gj.y) * d.y : 0.f);
+          a[2 * t] = pack2(j <= i0 ? w[0] * decay(gi0, gj.x, most) * d.x : 0.f, j + 1 <= i0 ? w[1] * decay(gi0, gj.y, most) * d.y : 0.f);
+          a[2 * t + 1] = pack2(j <= i1 ? w[2] * decay(gi1, gj.x, most) * d.x : 0.f, j + 1 <= i1 ? w[3] * decay(gi1, gj.y, most) * d.y : 0.f);
         }
 #pragma unroll
         for (int p = 0; p < 8; p += 2) {

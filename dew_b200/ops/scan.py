@@ -354,7 +354,8 @@ def selective_scan_chunked(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None,
         p3 = lambda t: torch.nn.functional.pad(t, (0, 0, 0, pad))
         xf, dtf, Bf, Cf = p3(xf), p3(dtf), p3(Bf), p3(Cf)
     n = xf.shape[1] // chunk
-    a = torch.exp(dtf.unsqueeze(-1) * A.float()).reshape(Bsz, n, chunk, C, N)                      # decay per step
+    # (a rate of minus infinity times the steps of 0 behind a row's end would be no number)
+    a = torch.exp(dtf.unsqueeze(-1) * A.float().clamp_min(-1e30)).reshape(Bsz, n, chunk, C, N)                      # decay per step
     b = ((dtf * xf).unsqueeze(-1) * Bf.unsqueeze(2)).reshape(Bsz, n, chunk, C, N)                  # increment per step
     # inclusive scan of the affine maps h -> a h + b along the chunk axis
     step = 1

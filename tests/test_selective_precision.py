@@ -9,7 +9,7 @@ from selective_cases import NAMES, companion, draws_of_its_own, rows  # noqa: F4
 from selective_cases import scan as oracle
 from selective_cases import softplus
 
-pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a GPU")]
+pytestmark = pytest.mark.gpu
 DEV, UNIT = "cuda", 2.0 ** -24
 # The exponential 4 (2^-22) and its correction 1, 1 + t or 2 + t 1, the reciprocal 2, their product 1, the series 2, the last step 1: 12 for a softplus, 10 for a sigmoid; then
 # one for every product that follows.
@@ -154,3 +154,57 @@ def test_states_of_chunks_in_32_bits(logit, a_log):
             # y: half a step of bf16 for a weight, a state and itself; weights are of differences of sums: up to 2^-24 of 64 decays, twice
             most = 64 * float(softplus(dt.double()).max() * rates.double().exp().max())
             assert off(y[i:i + 1, :n, h * P:h * P + P], want["y"], size["y"]) <= 2.1 * 2 ** 16 + 4 * most
+
+
+def forgetting(t):
+    """Rates of minus infinity among the others, and what the definition makes of them: decays of 0."""
+    a = t["a"].clone()
+    a[::3, ::2] = -float("inf")
+    a[-1] = -float("inf")
+    return dict(t, a=a), dict(t, a=a.clamp_min(-1e30))
+
+
+@pytest.mark.parametrize("pieces", [1, 3])
+@pytest.mark.parametrize("B,T,C,N", [(1, 1, 7, 4), (2, 5, 7, 4), (1, 70, 40, 16), (2, 67, 20, 33), (1, 49, 9, 100)])
+def test_states_without_memory(B, T, C, N, pieces, monkeypatch):
+    whole = selective._split
+    if pieces > 1:
+        monkeypatch.setattr(selective, "_split", lambda R, T, *a, **k: (max(16, T // pieces // 16 * 16), whole(R, T, *a, **k)[1]))
+    t, dy, dlast = positive(B, T, C, N)
+    t, exact = forgetting(t)
+    leaves = {n: v.clone().requires_grad_() for n, v in t.items()}
+    out = scan.selective_scan(*leaves.values())
+    grads = torch.autograd.grad(out, list(leaves.values()), (dy, dlast))
+    want, size = oracle(**exact, dy=dy, dlast=dlast), companion(**exact, dy=dy, dlast=dlast)
+    terms = dict(y=N, last=0, dx=N, ddt=2 * N, dz=N, db=C, dc=C, da=B * T, dd=B * T, dinitial=0)
+    for n, v in dict(y=out[0], last=out[1], **{f"d{n}": v for n, v in zip(NAMES, grads)}).items():
+        assert v.isfinite().all() and off(v.detach(), want[n], size[n] + 1e-30) <= 2 * TERM + terms[n], n
+    at = rows([5] * B, [T] * B, T, None, DEV)
+    state = t["initial"].clone()
+    logits = torch.log(torch.expm1(t["dt"].double())).float()
+    y = selective.selective_tokens(t["x"], logits, torch.log(-t["a"]), t["b"], t["c"], t["d"], t["z"], at, state)
+    # (steps and rates through a logarithm and back: FAR and 3 more of each exponent, up to 2.5, 1.84 times over; and of the step itself)
+    more = TERM + 2 * 2.5 * (FAR + 3) + FAR
+    assert off(y, want["y"], size["y"]) <= more + N and off(state, want["last"], size["last"] + 1e-30) <= more
+
+
+@pytest.mark.parametrize("far", [95.0, float("inf")])
+@pytest.mark.parametrize("S,P,N,dtype", [(1, 24, 16, torch.float32), (21, 24, 16, torch.float32), (70, 64, 128, torch.float32), (70, 64, 128, torch.bfloat16), (128, 64, 128, torch.bfloat16)])
+def test_heads_without_memory(S, P, N, dtype, far):
+    g, H = torch.Generator(DEV).manual_seed(S), 4
+    r = lambda *s: torch.rand(*s, generator=g, device=DEV) / 2 + 0.75
+    x, dt, b, c, d, a_log, state = r(2, S, H * P).to(dtype), r(2, S, H).to(dtype), r(2, S, N).to(dtype), r(2, S, N).to(dtype), r(H), torch.zeros(H, device=DEV), r(2, H, P, N)
+    a_log[1::2] = far
+    before = state.clone()
+    y = selective.ssd_tokens(x, dt, None, a_log, b, c, d, H, 1, rows([3, 0], [S, max(1, S - 3)], S, None, DEV), state)
+    assert y.isfinite().all() and state.isfinite().all()
+    for i, (first, n) in enumerate(((3, S), (0, max(1, S - 3)))):
+        for h in range(H):
+            cols = slice(h * P, h * P + P)
+            one = dict(x=x[i:i + 1, :n, cols], dt=dt[i:i + 1, :n, h:h + 1].expand(1, n, P), a=torch.full((P, N), -1e30 if h % 2 else -1.0, device=DEV, dtype=torch.float64), b=b[i:i + 1, :n],
+                       c=c[i:i + 1, :n], d=d[h].expand(P), initial=before[i:i + 1, h] if first else None)
+            want, size = oracle(**one, steps=True), companion(**one, steps=True)
+            # (as above; in chunks a state's share is a sum of 64 tokens' three terms on the tensor cores, a rounding toward zero each; bf16: half a step of states, weights and y)
+            bound = 2.8 * (12 + 2 * (FAR + 3)) + TERM + FAR + (2 * 3 * 64 if dtype is torch.bfloat16 else 0)
+            assert off(state[i:i + 1, h], want["last"], size["last"]) <= bound
+            assert off(y[i:i + 1, :n, cols], want["y"], size["y"]) <= (2.1 * 2.0 ** 16 if dtype is torch.bfloat16 else bound + N)

@@ -6,6 +6,7 @@ from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
 from dew_b200.nn.kv_cache import KVCache
 from dew_b200.nn.linear_attention import RecurrentCache, ShortConv
+from dew_b200.ops import scan
 from dew_b200.sampling.text import Sampling, generate, make_cache
 from selective_cases import draws_of_its_own  # noqa: F401
 from test_state_space_models import OPTIONS, model
@@ -90,6 +91,17 @@ def test_a_cache_without_a_place_for_a_state_is_refused(kind):
         for lo, hi in ((0, 9), (9, 16), (16, 17), (17, 20)):
             got.append(m(tokens[:, lo:hi], positions=torch.arange(lo, hi)[None].expand(2, hi - lo), cache=cache))
         assert torch.allclose(torch.cat(got, 1), m(tokens), atol=1e-4)
+
+
+def test_states_without_memory_in_the_plain_form():
+    """Rates of minus infinity: what a token leaves is gone at the next."""
+    x, dt, b, c = torch.randn(2, 70, 5), torch.rand(2, 70, 5) + 0.1, torch.randn(2, 70, 3), torch.randn(2, 70, 3)
+    a, initial = torch.full((5, 3), -float("inf")), torch.randn(2, 5, 3)
+    leaves = [t.requires_grad_() for t in (x, dt, a, b, c)]
+    y, last = scan.selective_scan(*leaves, initial_state=initial)
+    state = (dt * x).unsqueeze(-1) * b.unsqueeze(2)
+    assert torch.allclose(y, (state * c.unsqueeze(2)).sum(-1), atol=1e-5) and torch.allclose(last, state[:, -1], atol=1e-6)
+    assert all(g.isfinite().all() for g in torch.autograd.grad(y.sum() + last.sum(), leaves))
 
 
 @pytest.mark.gpu
