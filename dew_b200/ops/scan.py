@@ -333,10 +333,16 @@ def selective_scan_reference(x, dt, A, Bm, Cm, D=None, z=None, initial_state=Non
 
 def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, chunk: int = 64, softplus: bool = False):
     """Public entry: ``x, dt [B,T,C]`` (with ``softplus``, the steps' logits), ``A [C,N]``, ``Bm, Cm [B,T,N]``, ``D [C]``, ``z [B,T,C]``, ``initial_state [B,C,N]`` -> (y ``[B,T,C]``, state
-    ``[B,C,N]`` fp32).  CUDA tensors with up to 128 states run the sm_100a kernels (``ops/selective.py``), in either direction; everything else the chunked form below."""
-    if x.is_cuda and A.dim() == 2 and 0 < A.shape[1] <= 128:
+    ``[B,C,N]`` fp32).  CUDA tensors with up to 128 states run the sm_100a kernels (``ops/selective.py``), in either direction, with what expands to these sizes; everything else the chunked
+    form below."""
+    if D is not None and D.dim() > 1 and D.numel() == D.shape[-1]:
+        D = D.reshape(-1)
+    if x.dim() == 3 and x.shape[1] == 0:
+        state = (x.shape[0], x.shape[2], A.shape[-1])
+        return x.clone(), torch.zeros(state, device=x.device) if initial_state is None else initial_state.float().expand(state).clone()
+    if x.is_cuda and A.dim() == 2 and 0 < A.shape[1] <= 128 and x.numel() > 0:
         from . import selective as K
-        if K.kernel_available(x, dt, A, Bm, Cm, D, z, initial_state):
+        if K.kernel_available(x, dt, A, Bm, Cm, D, z, initial_state) and K.fits(x, dt, A, Bm, Cm, D, z, initial_state):
             return K.selective_scan(x, dt, A, Bm, Cm, D, z, initial_state, softplus)
     return selective_scan_chunked(x, dt, A, Bm, Cm, D, z, initial_state, chunk, softplus)
 

@@ -189,6 +189,14 @@ def kernel_available(x: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
             and L.use_cuda(x))
 
 
+def fits(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None) -> bool:
+    """Whether everything expands to its size beside ``x [R, T, C]``."""
+    R, T, C = x.shape
+    tokens, narrow, rates = (R, T, C), (R, T, A.shape[-1]), (C, A.shape[-1])
+    return all(t is None or t.shape == size or (t.dim() <= len(size) and all(n == m or n == 1 for n, m in zip(reversed(t.shape), reversed(size))))
+               for t, size in ((dt, tokens), (A, rates), (Bm, narrow), (Cm, narrow), (D, (C,)), (z, tokens), (initial_state, (R, *rates))))
+
+
 def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplus: bool = False):
     """``ops.scan.selective_scan`` on the kernels."""
     R, T, C = x.shape
@@ -196,9 +204,6 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
     given = [t for t in (dt, A, Bm, Cm, D, z, initial_state) if t is not None]
     if any(t.dim() and t.device != x.device for t in given):
         raise ValueError("selective_scan: tensors of one device")
-    if 0 in (R, T, C):
-        last = torch.zeros(R, C, N, device=x.device) if initial_state is None else initial_state.float().expand(R, C, N)
-        return torch.empty_like(x), last.clone()
     out_type = x.dtype
     # one type for what is per token: where they differ (or are fp16) in fp32, which holds every value of each
     one = out_type is not torch.float16 and all(t is None or t.dtype is out_type for t in (Bm, Cm, z)) and dt.dtype in (out_type, torch.float32)
