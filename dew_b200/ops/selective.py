@@ -227,14 +227,16 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, initial_state=None, softplu
 # a call's rows, with the states of a store
 
 
+_TYPES = (torch.bfloat16, torch.float32, torch.float16, torch.float64)         # (the last two in the plain form)
+
+
 def _check(what: str, x, dt, b, c, z, weights, state, rows: Optional[Rows], state_shape, wide, steps, narrow) -> None:
     if x.dim() != 3:
         raise ValueError(f"{what}: x [rows, tokens, channels], got {tuple(x.shape)}")
     R, S, _ = shape = x.shape
     own, where = x.dtype, torch.Tensor.get_device if x.is_cuda else _device          # (the quicker question)
-    if (own is not torch.bfloat16 and own is not torch.float32) or b.dtype is not own or c.dtype is not own or (z is not None and z.dtype is not own) or \
-            (dt.dtype is not own and dt.dtype is not torch.float32):
-        raise TypeError(f"{what}: bf16 or fp32 tokens of one type and steps of that type or fp32, got {[t.dtype for t in (x, dt, b, c, z) if t is not None]}")
+    if own not in _TYPES or b.dtype is not own or c.dtype is not own or (z is not None and z.dtype is not own) or (dt.dtype is not own and dt.dtype is not torch.float32):
+        raise TypeError(f"{what}: floating-point tokens of one type and steps of that type or fp32, got {[t.dtype for t in (x, dt, b, c, z) if t is not None]}")
     if dt.shape != (R, S, steps) or b.shape != (R, S, narrow) or c.shape != b.shape or (z is not None and z.shape != shape):
         raise ValueError(f"{what}: steps [.., {steps}], B and C [.., {narrow}] and z [.., {wide}] beside x {tuple(shape)}, got {[tuple(t.shape) for t in (dt, b, c, z) if t is not None]}")
     device = where(x)

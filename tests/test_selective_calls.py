@@ -59,3 +59,56 @@ def test_empty_calls_have_gradients():
 @pytest.mark.gpu
 def test_empty_calls_have_gradients_on_a_gpu():
     empty_calls_have_gradients("cuda")
+
+
+FNS = {"channels": (selective.selective_tokens, lambda t: dict(x=t["x"], dt=t["dt"], A_log=torch.log(-t["a"]), Bm=t["b"], Cm=t["c"], D=t["d"], z=t["z"]), (8, 4)),
+       "heads": (selective.ssd_tokens, lambda t: dict(x=t["x"], dt=t["dt"][..., :2], dt_bias=t["d"][:2], A_log=t["d"][2:4], Bm=t["b"], Cm=t["c"], D=t["d"][4:6], H=2, G=2), (2, 4, 2))}
+
+
+def other_types(kind, dtype, device):
+    """fp16 and fp64 in one type take the plain form, as the other recurrences leave them to theirs; the state stays fp32."""
+    fn, make, shape = FNS[kind]
+    t = inputs(3, 6, 8, 4, torch.float32, device, 2)
+    one = make(t)
+    cast = {k: v.to(dtype) if torch.is_tensor(v) and k not in ("A_log", "D", "dt_bias") else v for k, v in one.items()}
+    wide = {k: v.float() if torch.is_tensor(v) else v for k, v in cast.items()}
+    at = rows([0, 5, -1], [6, 4, 0], 6, [2, 0, 1], device)
+    state = torch.randn(4, *shape, device=device)
+    want_state = state.clone()
+    y, want = fn(**cast, rows=at, state=state), fn(**wide, rows=at, state=want_state)
+    assert y.dtype is dtype and torch.allclose(state, want_state, atol=1e-5)
+    # (half a step of fp16, where the results are rounded to it)
+    assert torch.allclose(y.float(), want, rtol=1e-5 + (2.0 ** -11 if dtype is torch.float16 else 0), atol=1e-5)
+    with pytest.raises(TypeError):
+        fn(**dict(cast, Bm=cast["Bm"].float()), rows=at, state=state)
+    with pytest.raises(TypeError):
+        fn(**dict(cast, dt=cast["dt"].bfloat16()), rows=at, state=state)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_other_types(kind, dtype):
+    other_types(kind, dtype, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_other_types_on_a_gpu(kind, dtype):
+    other_types(kind, dtype, "cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+@pytest.mark.parametrize("kind", ["mamba", "mamba2"])
+def test_models_of_other_types_generate(kind, dtype):
+    from dew_b200.sampling.text import Sampling, generate
+    from test_state_space_models import model, prompts
+    m, asked = model(kind).to(dtype), prompts(2)
+    out = generate(m, None, asked, 4, sampling=Sampling(temperature=0.0))
+    for r, p in enumerate(asked):
+        row = out.tokens[r, :len(p) + 4]
+        with torch.no_grad():
+            logits = m(row[None])[0, len(p) - 1:-1].float()
+        # (near to the whole row's best: in fp16 two tokens may come as near as its roundings)
+        taken = logits.gather(1, row[len(p):, None])[:, 0]
+        assert bool((logits.amax(1) - taken <= (2.0 ** -5 if dtype is torch.float16 else 1e-4)).all())
