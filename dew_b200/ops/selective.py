@@ -15,6 +15,7 @@ from . import library as L
 from .token_mix import Rows, kernel_ok, whole
 
 MOST_STATES, MOST_HEAD_STATES = 128, 256
+OUTSIDE = 6              # the status word's code of a row outside the store
 EVERY = 16               # tokens between two states that the forward keeps for the backward
 
 # ``dewb_selective_args`` of ``csrc/common/selective.cuh`` and ``dewb_selective_grad_args`` of ``csrc/kernels/selective_grad.cu``, packed in one call (a ctypes structure of 42 fields takes five
@@ -318,10 +319,24 @@ def _chunks(x, dt, b, c, a, dt_bias, d, rows: Rows, state, heads: int, groups: i
     return y
 
 
+def _inside(rows: Rows, state: Optional[torch.Tensor]) -> Rows:
+    """The plain forms' rows, of which those outside the store rest: on a GPU the status word tells of them, as the kernels have it (there an index outside would end the process); on the
+    CPU they are an error."""
+    if state is None or rows.row_ids is None:
+        return rows
+    there = (rows.row_ids >= 0) & (rows.row_ids < state.shape[0])
+    if state.is_cuda:
+        word = L.status(state.device)
+        word.copy_(torch.where(there.all(), word, torch.full_like(word, OUTSIDE)))
+    elif not bool((there | (rows.positions[:, 0] < 0)).all()):
+        raise IndexError(f"rows {rows.row_ids.tolist()} of a store of {state.shape[0]}")
+    return Rows(torch.where(there[:, None], rows.positions, -1), rows.lengths, torch.where(there, rows.row_ids, 0))
+
+
 def selective_tokens_reference(x, dt, A_log, Bm, Cm, D=None, z=None, rows: Optional[Rows] = None, state=None):
     from .recurrence import _tokens as walk
     R, S, C = x.shape
-    rows = whole(R, S, x.device) if rows is None else rows
+    rows = whole(R, S, x.device) if rows is None else _inside(rows, state)
     step, A = F.softplus(dt.float(), threshold=60.0), -torch.exp(A_log.float())
     xf, Bf, Cf = x.float(), Bm.float(), Cm.float()
 
@@ -351,7 +366,7 @@ def selective_tokens(x: torch.Tensor, dt: torch.Tensor, A_log: torch.Tensor, Bm:
 def ssd_tokens_reference(x, dt, dt_bias, A_log, Bm, Cm, D, H: int, G: int, rows: Optional[Rows] = None, state=None):
     from .recurrence import _tokens as walk
     R, S, _ = x.shape
-    rows = whole(R, S, x.device) if rows is None else rows
+    rows = whole(R, S, x.device) if rows is None else _inside(rows, state)
     xf = x.float().view(R, S, H, -1)
     Bf, Cf = (t.float().reshape(R, S, G, -1).repeat_interleave(H // G, 2) for t in (Bm, Cm))
     step = F.softplus(dt.float() if dt_bias is None else dt.float() + dt_bias.float(), threshold=60.0)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from dew_b200.ops import library as L
 from dew_b200.ops import scan, selective
 from selective_cases import draws_of_its_own, inputs, rows  # noqa: F401
 
@@ -112,3 +113,39 @@ def test_models_of_other_types_generate(kind, dtype):
         # (near to the whole row's best: in fp16 two tokens may come as near as its roundings)
         taken = logits.gather(1, row[len(p):, None])[:, 0]
         assert bool((logits.amax(1) - taken <= (2.0 ** -5 if dtype is torch.float16 else 1e-4)).all())
+
+
+@pytest.mark.parametrize("bad", [-1, 4, 1 << 30])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_rows_outside_the_store_in_the_plain_form(kind, bad):
+    """Nothing is read or written there: an error on the CPU, but for a row that rests."""
+    fn, make, shape = FNS[kind]
+    t = inputs(3, 6, 8, 4, torch.float32, "cpu", 2)
+    state = torch.randn(4, *shape)
+    before = state.clone()
+    with pytest.raises(IndexError, match="store"):
+        fn(**make(t), rows=rows([2, 5, 1], [6, 4, 6], 6, [2, bad, 1], "cpu"), state=state)
+    assert torch.equal(state, before)
+    y = fn(**make(t), rows=rows([2, -1, 1], [6, 0, 6], 6, [2, bad, 1], "cpu"), state=state)
+    assert not y[1].any() and y[0].any() and torch.equal(state[[0, 3]], before[[0, 3]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["gradients", "fp16"])
+@pytest.mark.parametrize("bad", [-1, 4, 1 << 30])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_rows_outside_the_store_in_the_plain_form_on_a_gpu(kind, bad, how):
+    """Calls that the kernels leave to the plain form: such a row is reported and gives zeros there as well."""
+    fn, make, shape = FNS[kind]
+    one = make(inputs(3, 6, 8, 4, torch.float32, "cuda", 2))
+    if how == "fp16":
+        one = {k: v.half() if torch.is_tensor(v) and k not in ("A_log", "D", "dt_bias") else v for k, v in one.items()}
+    else:
+        one["D"].requires_grad_()
+    state = torch.randn(4, *shape, device="cuda")
+    before = state.clone()
+    y = fn(**one, rows=rows([2, 5, 1], [6, 4, 6], 6, [2, bad, 1], "cuda"), state=state)
+    with pytest.raises(L.KernelError, match="bad argument"):
+        L.check_status()
+    assert not y[1].any() and y[0].any() and torch.equal(state[[0, 3]], before[[0, 3]]) and not torch.equal(state[2], before[2])
+    L.check_status()
