@@ -271,6 +271,12 @@ def _fp32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.detach().float().contiguous()
 
 
+def _moved(state: Optional[torch.Tensor]) -> None:
+    """A state went on in place: autograd is to know, as it does of what torch writes (inference tensors have no version)."""
+    if state is not None and not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+
+
 def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: int, heads: int) -> torch.Tensor:
     if not L.device_is_current(x):
         with L.on_device_of(x):
@@ -281,6 +287,7 @@ def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: in
     token = x.shape[1] == 1 and state is not None
     call = _args(x, dt, z, b, c, a, dt_bias, d, state, state, y, None, rows, N, groups, heads, True, True, 0 if state is None else state.shape[0], token)
     _launch(call, heads > 0, x.dtype is torch.float32, token, L.stream())
+    _moved(state)
     return y
 
 
@@ -316,6 +323,7 @@ def _chunks(x, dt, b, c, a, dt_bias, d, rows: Rows, state, heads: int, groups: i
     L.check(lib.dewb_ssd_rows(x.data_ptr(), steps, rates, b.data_ptr(), c.data_ptr(), L.at(d), L.at(state), states.data_ptr(), y.data_ptr(), places, places + 4 * R, places + 8 * R,
                               R, T, heads, groups, ctypes.addressof(strides), stream), "ssd_rows")
     L.count_launches(3)
+    _moved(state)
     return y
 
 

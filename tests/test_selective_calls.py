@@ -37,7 +37,7 @@ def test_what_broadcasts(at, change):
     plain = [t.detach().cpu().clone().requires_grad_() for t in args]
     want = scan.selective_scan_chunked(*plain, softplus=True)
     grads = torch.autograd.grad(got[0].square().sum() + got[1].sum(), leaves)
-    for a, b in zip((*got, *grads), (*want, *torch.autograd.grad(want[0].square().sum() + want[1].sum(), plain))):
+    for a, b in zip((*(t.detach() for t in got), *grads), (*(t.detach() for t in want), *torch.autograd.grad(want[0].square().sum() + want[1].sum(), plain))):
         assert a.shape == b.shape and torch.allclose(a.cpu(), b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
 
 
@@ -149,3 +149,47 @@ def test_rows_outside_the_store_in_the_plain_form_on_a_gpu(kind, bad, how):
         L.check_status()
     assert not y[1].any() and y[0].any() and torch.equal(state[[0, 3]], before[[0, 3]]) and not torch.equal(state[2], before[2])
     L.check_status()
+
+
+def state_that_autograd_holds(kind, S, device, dtype=torch.float32):
+    """A state that a call moves on is another value to autograd."""
+    fn, make, shape = FNS[kind]
+    one = {k: v.to(dtype) if torch.is_tensor(v) and k not in ("A_log", "D", "dt_bias") else v for k, v in make(inputs(2, S, 8, 4, torch.float32, device, 3)).items()}
+    state, w = torch.randn(2, *shape, device=device), torch.ones((), device=device, requires_grad=True)
+    held, version = (w * state).sum(), state._version
+    with torch.no_grad():
+        fn(**one, rows=rows([1, 0], [S, S], S, None, device), state=state)
+    assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        held.backward()
+    with torch.inference_mode():
+        again = torch.zeros(2, *shape, device=device)
+        fn(**one, rows=rows([1, 0], [S, S], S, None, device), state=again)
+        fn(**one)
+    version = state._version
+    with torch.no_grad():
+        fn(**one)                                            # (no state: nothing moves)
+    assert state._version == version
+
+
+@pytest.mark.parametrize("S", [1, 5])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_autograd_sees_that_a_state_moved_on(kind, S):
+    state_that_autograd_holds(kind, S, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 5])
+@pytest.mark.parametrize("kind", sorted(FNS))
+def test_autograd_sees_that_a_state_moved_on_on_a_gpu(kind, S):
+    state_that_autograd_holds(kind, S, "cuda")
+
+
+@pytest.mark.gpu
+def test_autograd_sees_that_a_state_of_chunks_moved_on():
+    r = lambda *s: torch.randn(*s, device="cuda")
+    state = r(2, 2, 64, 128)
+    version = state._version
+    with torch.no_grad():
+        selective.ssd_tokens(r(2, 40, 128).bfloat16(), r(2, 40, 2).bfloat16(), None, r(2), r(2, 40, 128).bfloat16(), r(2, 40, 128).bfloat16(), None, 2, 1, rows([0, 3], [40, 7], 40, None, "cuda"), state)
+    assert state._version > version
