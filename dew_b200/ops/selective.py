@@ -177,7 +177,10 @@ class _SelectiveScan(torch.autograd.Function):
 def _plain_gradients(ins, softplus, dy, dlast, needed):
     from .scan import selective_scan_chunked
     out = selective_scan_chunked(*ins, softplus=softplus)
-    pairs = [(o, g) for o, g in zip(out, (dy, dlast)) if g is not None]
+    # (the last state depends neither on C, D nor the gate, and needs no gradient where nothing else does)
+    pairs = [(o, g) for o, g in zip(out, (dy, dlast)) if g is not None and o.requires_grad]
+    if not pairs:
+        return [None] * len(ins)
     at = [i for i, t in enumerate(ins) if t is not None and needed[i]]
     grads = torch.autograd.grad([o for o, _ in pairs], [ins[i] for i in at], [g for _, g in pairs], create_graph=True, allow_unused=True)
     return [grads[at.index(i)] if i in at else None for i in range(len(ins))]

@@ -193,3 +193,40 @@ def test_autograd_sees_that_a_state_of_chunks_moved_on():
     with torch.no_grad():
         selective.ssd_tokens(r(2, 40, 128).bfloat16(), r(2, 40, 2).bfloat16(), None, r(2), r(2, 40, 128).bfloat16(), r(2, 40, 128).bfloat16(), None, 2, 1, rows([0, 3], [40, 7], 40, None, "cuda"), state)
     assert state._version > version
+
+
+# leaves that one of the two results does not depend on, alone and together
+LEAVES = [("c",), ("d",), ("z",), ("c", "d", "z"), ("initial",), ("c", "x")]
+
+
+@pytest.mark.parametrize("which", ["y", "last", "both"])
+@pytest.mark.parametrize("names", LEAVES)
+def test_gradients_to_be_differentiated_of_some_leaves(names, which):
+    """What the node gives where its gradients keep a history, from the plain form."""
+    all_names = ("x", "dt", "a", "b", "c", "d", "z", "initial")
+    ins = [t.requires_grad_(n in names) for n, t in zip(all_names, call())]
+    y, last = scan.selective_scan_chunked(*ins, softplus=True)
+    dy, dlast = torch.randn_like(y) if which != "last" else None, torch.randn_like(last) if which != "y" else None
+    got = selective._plain_gradients(ins, True, dy, dlast, [n in names for n in all_names])
+    for n, t, g in zip(all_names, ins, got):
+        if n not in names:
+            assert g is None
+            continue
+        sees = [(o, d) for o, d in ((y, dy), (last, dlast)) if d is not None and o.requires_grad]
+        want = torch.autograd.grad([o for o, _ in sees], t, [d for _, d in sees], retain_graph=True, allow_unused=True)[0] if sees else None
+        # (with a history a gate's slope is formed of other products: sig (1 + z (1 - sig)), some six roundings either way, of terms up to 2 |dz|'s factors)
+        assert (want is None and g is None) or torch.allclose(g, want, rtol=2.0 ** -20, atol=2.0 ** -20 * float(want.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("names", LEAVES)
+def test_gradients_to_be_differentiated_of_some_leaves_on_a_gpu(names):
+    """Through the kernels' node: with a history and without one."""
+    all_names = ("x", "dt", "a", "b", "c", "d", "z", "initial")
+    ins = [t.requires_grad_(n in names) for n, t in zip(all_names, call("cuda"))]
+    y, last = scan.selective_scan(*ins, softplus=True)
+    leaves, loss = [t for t in ins if t.requires_grad], y.square().sum() + last.square().sum()
+    kept = torch.autograd.grad(loss, leaves, create_graph=True)
+    for a, b in zip(kept, torch.autograd.grad(loss, leaves)):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
+    assert all(g.isfinite().all() for g in torch.autograd.grad(sum(g.square().sum() for g in kept), leaves))
