@@ -9,7 +9,7 @@
 //
 // What bounds scan_kernel is the exponential of every token, channel and state: the special-function unit takes eight cycles for a warp's, so 4 rows of 2048 tokens of 4096 channels of 16
 // states cannot take less than 119 us (149 with those of steps and gates; the bytes, 41).  The ENDS pass comes to 75 % of that rate; the other reaches 56 to 70 %, where a SM has 16
-// warps: 247 us in eight segments and 162 for their ends, or 399 for whole rows with two states a lane and 7 warps an SM, whose chains are then what takes the time (a warp waits 1.8
+// warps: 247 us in eight segments and 162 for their ends, or 396 for whole rows with two states a lane and 7 warps an SM, whose chains are then what takes the time (a warp waits 1.8
 // of 5 cycles for the instruction before, 1.1 for an exponential or shared memory).  token_kernel is bound by memory: 128 rows of 8192 channels 27 us, 4.9 TB/s (32 where
 // every load asks whether its channel and states are there: 450 instructions a row of 32 channels; states three rows ahead in shared memory instead of one in registers: 27).
 #include "../common/selective.cuh"
@@ -30,8 +30,9 @@ struct Tile {
 //   sums[r, j]         the sum of segment j's steps, per channel
 // A tile's x and steps come a tile ahead, in registers as they lie in memory (converted on arrival, every tile waited for them: 10 to 25 % of the time); what the end of a tile needs (x
 // again, z) is asked for at its beginning (L2) and read then.  Channels go in pairs, two to an instruction: no more of them a second, but half as many to issue (one at a time: 3 %
-// slower here, 13 % in the gradients).  The sums over states are formed at the end of a tile from what every lane leaves in shared memory: with shuffles after every two or four tokens
-// the whole rows above took 665 and 528 us with four states a lane, so 555.  NS 4, 2, 1: what _split in ops/selective.py says of each.
+// slower here, 13 % in the gradients).  The sums over states are formed at the end of a tile from what every lane leaves in shared memory: 4 whole rows of 2048 tokens of 4096 channels take
+// 539 us with four states a lane and 396 with two, which have twice the sums to cross lanes (four states a lane with shuffles after every two tokens 665, after every four 528).  NS 4, 2, 1:
+// what _split in ops/selective.py says of each.
 template <typename T, typename TD, int LN, int NS, bool ENDS>
 __global__ void __launch_bounds__(THREADS, sizeof(T) == 4 ? 3 : 4)
 scan_kernel(const Args p) {

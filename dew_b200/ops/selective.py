@@ -33,9 +33,25 @@ def _padded(C: int, N: int, groups: int = 1, heads: int = 0):
 def _split(R: int, T: int, C: int, N: int, groups: int, heads: int = 0, backward: bool = False, fp32: bool = False):
     """Tokens of a piece of a row (the pieces run side by side), and states of a lane (of up to 16).  Pieces cost a pass of their own over the tokens (about half of the other) and are put
     together one after another, so there are no more than fill the GPU, or than the square root of half the tokens; fewer states a lane fill it without them, at the price of more sums over lanes.
-    (16 states, in us, forwards: 4 rows of 2048 tokens of 4096 channels whole with 4, 2, 1 states a lane 566, 390, 425, in 8 pieces 409, 421, 559; one of 2048 of 2048 channels in 16, 24
-    pieces of 2 states 74, 78; one of 16384 in 32, 64 pieces 457, 459; one of 512 of 1024 channels in 16 pieces of 2, 11 of 1 19, 20.  Backwards: 8 of 512 of 4096 channels whole,
-    in 5 pieces 457, 497; one of 2048 of 2048 channels in 16 pieces of 4, 22 of 2 154, 177.)"""
+
+    What it was measured on: rows of 2048 tokens of 16 states in bf16, gated, in us, by the warps that the channels of all rows make.  Forwards, whole with 1, 2, 4 states a lane, and in
+    pieces (their number, states a lane):
+
+        64     259  338  538   (16, 2) 80         448    426  398  538   (5, 4) 376, (4, 2) 400     1024   841  607  663   (2, 4) 732
+        128    254  340  538   (9, 2) 138         512    427  396  539   (8, 4) 404                 1280  1113  868  829   (5, 4) 899
+        256    294  342  537   (6, 2) 261         640    698  490  657   (8, 4) 495                 1536  1174  947  828   (3, 4) 1050
+        384    350  398  545   (4, 2) 352         768    711  492  664   (3, 4) 551
+
+    so pieces of two states a lane up to 448 warps (within a tenth of the best there, but for up to a quarter below 256 in other numbers of pieces), whole rows from there on, with four states a
+    lane from 1536 on.  Backwards, whole with 2, 4 states a lane, and in pieces of 4:
+
+        64    1099 1399   (16) 202     384   1367 1400   (11) 826     896   2566 1823   (5) 1763
+        256   1115 1398   (16) 577     512   1370 1418   (8) 1059     1024  2609 1832   (4) 1971
+        128   1089 1401   (9) 334      768   1668 1830   (6) 1500     1280  2905 3030   (6) 2396
+
+    so pieces up to 1024 warps; behind 1184, as many as two blocks an SM are, whole rows make a second wave, and pieces would be faster again for some way.  512 tokens: forwards 512 warps whole
+    106, in pieces 118; 384 whole with one state 93, in pieces 101; backwards 1024 whole 507, in pieces 547; 512 whole 390, in 5 and 8 pieces 318, 323.  One row of 512 of 1024 channels
+    in 16 pieces of 2, 11 of 1: 19, 20; one of 2048 of 2048 channels backwards in 16 pieces of 4, 22 of 2: 154, 177."""
     warps = max(1, R * groups * -(-(C // groups) // _padded(C, N, groups, heads)[2]))
     most = max(1, min(-(-T // EVERY), int((T / 2) ** 0.5)))
     narrow = N <= 16 and not heads
@@ -294,8 +310,10 @@ def _tokens(x, dt, z, b, c, a, dt_bias, d, rows: Rows, state, N: int, groups: in
     return y
 
 
-# From here on a call of heads of 64 over 128 states in bf16 goes through the tensor cores' scan in chunks (64 heads, one row of 16, 32, 64, 2048 tokens: 12, 13, 13, 83 us against 8, 15, 26,
-# 387 token by token; eight rows of 512 143 against 477).  Its states are as exact; y is formed of states and weights that were rounded to bf16 once (0.0022 of y instead of 0.0017).
+# From here on a call of heads of 64 over 128 states in bf16 goes through the tensor cores' scan in chunks.  64 heads, in us, chunks and token by token: one row of 16 tokens 32, 12; of 32 37, 23;
+# of 64 25, 33; of 2048 94, 395; eight of 32 40, 42; of 512 151, 485; eight of 37 to 512 149, 301; 32 of 32 98, 139; 24 heads, one row of 33 30, 25, of 64 28, 29, of 512 40, 100.  Chunks
+# are formed for a call's longest row and all others, so one long row beside single tokens is slower so: 64 tokens and seven rows of one 42, 33; 512 and 31 rows of one 497, 209.  The states
+# are as exact; y is formed of states and weights that were rounded to bf16 once (0.0022 of y instead of 0.0017), as scan.ssd forms it of whole rows.  Heads come in pairs, as ops/ssd.py has them.
 CHUNKED_TOKENS = 32
 
 
