@@ -227,6 +227,6 @@ def test_gradients_to_be_differentiated_of_some_leaves_on_a_gpu(names):
     y, last = scan.selective_scan(*ins, softplus=True)
     leaves, loss = [t for t in ins if t.requires_grad], y.square().sum() + last.square().sum()
     kept = torch.autograd.grad(loss, leaves, create_graph=True)
-    for a, b in zip(kept, torch.autograd.grad(loss, leaves)):
+    for a, b in zip(kept, torch.autograd.grad(loss, leaves, retain_graph=True)):
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-4 * float(b.abs().max()))
     assert all(g.isfinite().all() for g in torch.autograd.grad(sum(g.square().sum() for g in kept), leaves))
