@@ -375,7 +375,7 @@ class DecoderLayer(nn.Module):
             cache = None
         if self.kind in ROTARY_KINDS:
             return self.mixer(n, cos, sin, positions, segment_ids, cache, slot)
-        if getattr(cache, "slots", None) is not None:
+        if getattr(cache, "slots", None) is not None or (hasattr(cache, "holds") and cache.holds(slot)):
             return self.mixer(n, segment_ids=segment_ids, cache=cache, layer=slot, positions=positions)
         return self.mixer(n, segment_ids=segment_ids, cache=cache, layer=slot)
 
@@ -602,6 +602,11 @@ class CausalTransformer(nn.Module):
                 out.append(CacheSlot(state=(0,) if m is None else (m.h, m.d, m.dv)))
         return out
 
+    def state_slots(self) -> Dict[int, CacheSlot]:
+        """What state space layers keep per layer run where one shape of keys and values serves the others (``cache_slots`` None)."""
+        cfg, kinds = self.config, self.config.kinds()
+        return {} if cfg.depth_residual_block else {slot: self.layers[i].mixer.cache_slot() for i, slot in self.runs() if kinds[i] in ("mamba", "mamba2")}
+
     # ------------------------------------------------------------------ helpers
     def _wants_tables(self, i: int) -> bool:
         """Whether layer ``i`` turns by the model's rotary tables."""
@@ -759,7 +764,7 @@ class CausalTransformer(nn.Module):
             h = h * (cfg.emb_features ** 0.5)
         if cfg.embed_multiplier is not None:
             h = h * cfg.embed_multiplier
-        if positions is None and getattr(cache, "slots", None) is not None:
+        if positions is None and (getattr(cache, "slots", None) is not None or getattr(cache, "keeps_state", False)):
             positions = torch.arange(h.shape[1], device=h.device)[None].expand(h.shape[0], -1)
         cos, sin = self.rope_tables(h.device)
         n_streams = max(cfg.hyper_connections, cfg.altup)

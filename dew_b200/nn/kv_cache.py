@@ -138,7 +138,8 @@ def default_page_table(rows: int, pages_per_row: int, device=None) -> torch.Tens
 
 class KVStore:
     def __init__(self, spec: KVCache, layers: int, rows: int, max_len: int, kv_heads: int, head_dim: int,
-                 dtype=torch.bfloat16, device="cpu", slots: Optional[Sequence[CacheSlot]] = None):
+                 dtype=torch.bfloat16, device="cpu", slots: Optional[Sequence[CacheSlot]] = None, states: Optional[Dict[int, CacheSlot]] = None):
+        """``slots``: what each layer run keeps, where they differ; ``states``: of layer runs whose keys all have one shape, those that keep a state beside."""
         self.spec = spec
         self.slots = None if slots is None else list(slots)
         self.layer_runs = 0 if slots is None else len(self.slots)
@@ -173,13 +174,14 @@ class KVStore:
                     if s.source is not None:
                         pools[i] = pools[s.source]
             self.last_reader = {s.source: i for i, s in enumerate(self.slots) if s.source is not None}
-            self.states = [None if s.state is None else torch.zeros(rows, *s.state, dtype=torch.float32, device=device) for s in self.slots]
-            self.more = [{n: torch.zeros(rows, *shape, dtype=torch.float32, device=device) for n, shape in s.more} for s in self.slots]
+            self._keep_states(self.slots, rows, device)
             self.k_scale = self.v_scale = None
         else:
             shape = (layers, self.pages + 1, self.page_size, kv_heads, head_dim)
             self.k = torch.zeros(shape, dtype=store, device=device)
             self.v = torch.zeros(shape, dtype=store, device=device)
+            if states:
+                self._keep_states([states.get(i) for i in range(layers)], rows, device)
             self.k_scale = torch.ones(shape[:-1], dtype=torch.float32, device=device) if self.kind else None
             self.v_scale = torch.ones(shape[:-1], dtype=torch.float32, device=device) if self.kind else None
         self.page_table = default_page_table(rows, self.max_pages, device) if spec.pages is None else \
@@ -193,10 +195,19 @@ class KVStore:
         self.shared: Optional[prefix.Shared] = None            # rows that share a prefix, of decode steps over all rows
 
     # ------------------------------------------------------------------ layers that differ (CacheSlot)
+    def _keep_states(self, slots: Sequence[Optional[CacheSlot]], rows: int, device) -> None:
+        zeros = lambda shape: torch.zeros(rows, *shape, dtype=torch.float32, device=device)
+        self.states = [None if s is None or s.state is None else zeros(s.state) for s in slots]
+        self.more = [{n: zeros(shape) for n, shape in (() if s is None else s.more)} for s in slots]
+
+    def holds(self, slot: int) -> bool:
+        """Whether there is a state for this layer run."""
+        return slot < len(self.states) and self.states[slot] is not None
+
     @property
     def keeps_state(self) -> bool:
         """Whether some layer keeps a state (which no page holds: a prompt's prefix cannot be taken from another row's pages)."""
-        return any(s.stateful for s in self.slots or ())
+        return any(s.stateful for s in self.slots) if self.slots is not None else bool(self.kept_states())
 
     def kept_states(self) -> List[torch.Tensor]:
         """Every tensor of the store that a step moves on instead of adding to."""

@@ -138,12 +138,17 @@ class GatedDeltaNet(nn.Module):
         return self.out_proj(o.reshape(B, T, self.value_dim))
 
 
+def in_slot(cache, layer: int) -> bool:
+    """Whether a row's state lies in the cache's slot (a ``RecurrentCache`` has its own)."""
+    return cache is not None and not hasattr(cache, "recurrent") and hasattr(cache, "holds") and cache.holds(layer)
+
+
 def kept_state(cache, layer: int, batch: int, mixer: nn.Module):
     """What ``cache`` keeps of ``mixer``, None without a cache; a cache of keys alone is refused, since every call would start from nothing."""
     if cache is None:
         return None
     if not hasattr(cache, "recurrent"):
-        raise NotImplementedError(f"{type(mixer).__name__}: the cache has no place for its state (a RecurrentCache around it has)")
+        raise NotImplementedError(f"{type(mixer).__name__}: the cache has no place for its state (make_cache gives it one; a RecurrentCache around it has)")
     return cache.recurrent(layer, batch, mixer)
 
 

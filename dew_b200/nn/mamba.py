@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
-from .linear_attention import ShortConv, kept_state
+from .linear_attention import ShortConv, in_slot, kept_state
 
 
 class Mamba(nn.Module):
@@ -51,7 +51,7 @@ class Mamba(nn.Module):
         return self.out_proj(selective.selective_tokens(xi, dt, self.A_log, Bm, Cm, self.D, xz[..., self.inner:], rows, state))
 
     def forward(self, x, segment_ids=None, cache=None, layer: int = 0, chunked: bool = True, positions=None):
-        if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+        if in_slot(cache, layer):
             if segment_ids is not None:
                 raise NotImplementedError("a state in a cache's slot runs over rows without packed segments")
             return self._in_slot(x, cache, layer, positions)

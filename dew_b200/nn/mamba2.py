@@ -15,7 +15,7 @@ import torch.nn.functional as F
 from .. import ops
 from ..ops import scan, selective, token_mix
 from .layers import Linear, declare
-from .linear_attention import ShortConv, kept_state
+from .linear_attention import ShortConv, in_slot, kept_state
 
 
 class Mamba2(nn.Module):
@@ -67,7 +67,7 @@ class Mamba2(nn.Module):
         return self.out_proj(ops.gated_rms_norm(y, z, self.norm_weight, self.norm_eps, gate_first=not self.gate_after))
 
     def forward(self, x, segment_ids=None, cache=None, layer: int = 0, positions=None):
-        if getattr(cache, "slots", None) is not None and not hasattr(cache, "recurrent"):
+        if in_slot(cache, layer):
             if segment_ids is not None:
                 raise NotImplementedError("a state in a cache's slot runs over rows without packed segments")
             return self._in_slot(x, cache, layer, positions)

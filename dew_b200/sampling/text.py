@@ -146,7 +146,8 @@ def make_cache(model, rows: int, max_len: int, spec: Optional[KVCache] = None, d
     if slots is not None and spec.quantized and all(s.state is not None for slot in slots for s in (slot, slot.beside) if s is not None):
         spec = replace(spec, quantized=None)                                                # (nothing but states: no keys to store in fewer bits)
     layers = len(model.runs()) if hasattr(model, "runs") else cfg.num_layers                # a looped block keeps a cache per pass
-    return KVStore(spec or KVCache(), layers, rows, max_len, kvh, hd, dtype or p.dtype, device or p.device, slots=slots)
+    states = model.state_slots() if slots is None and hasattr(model, "state_slots") else None
+    return KVStore(spec or KVCache(), layers, rows, max_len, kvh, hd, dtype or p.dtype, device or p.device, slots=slots, states=states)
 
 
 class RowBatch:

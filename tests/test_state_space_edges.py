@@ -4,12 +4,12 @@ import torch
 
 from dew_b200.inference.serving import Server
 from dew_b200.models import CausalTransformer
-from dew_b200.nn.kv_cache import KVCache
+from dew_b200.nn.kv_cache import KVCache, KVStore
 from dew_b200.nn.linear_attention import RecurrentCache, ShortConv
 from dew_b200.ops import scan
-from dew_b200.sampling.text import Sampling, generate, make_cache
+from dew_b200.sampling.text import RowBatch, Sampling, generate, make_cache
 from selective_cases import draws_of_its_own  # noqa: F401
-from test_state_space_models import OPTIONS, model
+from test_state_space_models import OPTIONS, greedy, model, prompts
 
 
 # a piece in front and behind, pieces shorter than the three inputs that a convolution of four taps keeps, single tokens between them
@@ -76,17 +76,64 @@ def test_packed_documents_and_a_state_are_refused(kind):
         assert torch.allclose(layer(x, None, store, 0, positions=at), layer(x), atol=1e-5)
 
 
+def between_attention(kind, device="cpu", **more):
+    """State space layers between attention layers that turn by the model's tables: one shape of keys for all, states beside."""
+    return model(kind, device, **{**dict(num_heads=4, num_kv_heads=2, layer_types=(kind, "attention", kind), layer_mlp=None, mlp_features=96, num_layers=3), **more})
+
+
+def generates(m):
+    """As the whole row again for every token: in one batch, through a server's chunks, slots that are used again and forks."""
+    asked = prompts()
+    want = [greedy(m, p, 6) for p in asked]
+    assert m.cache_slots() is None
+    store = make_cache(m, 2, 64)
+    assert store.keeps_state and [store.holds(i) for i in range(4)] == [True, False, True, False] and len(store.kept_states()) == 4
+    out = generate(m, None, asked, 6, sampling=Sampling(temperature=0.0))
+    assert [out.tokens[r, len(p):len(p) + 6].tolist() for r, p in enumerate(asked)] == want
+    for spec in (None, KVCache(page_size=16)):
+        server = Server(m, slots=2, capacity=256, chunk=32, kv_cache=spec, sampling=Sampling(temperature=0.0))
+        assert server(asked, 6) == want and server(asked[::-1], 6) == want[::-1]
+        group = server.submit_group(asked[0], 2, 6)
+        server.run()
+        assert [t.result() for t in group] == [want[0], want[0]]
+
+
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_between_attention_layers(kind):
+    generates(between_attention(kind))
+
+
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_pieces_between_attention_layers(kind):
+    """Prompts of their own lengths, then a token at a time with rows that rest; chunks that begin together; from the first token on also without positions."""
+    m = between_attention(kind)
+    tokens = torch.randint(1, 97, (3, 24))
+    batch, at = RowBatch(m, 3, 64), [7, 12, 1]
+    with torch.no_grad():
+        want = m(tokens)
+        got = batch.prefill(tokens[:, :12], torch.tensor(at))
+        assert torch.allclose(got, want[[0, 1, 2], [6, 11, 0]], atol=1e-4)
+        for step in [(1, 0, 1), (1, 1, 1), (0, 1, 0), (1, 1, 1)]:
+            pos = torch.tensor([a if n else -1 for a, n in zip(at, step)])
+            out = batch.forward(tokens.gather(1, pos.clamp_min(0)[:, None]), pos[:, None])[:, 0]
+            for r, n in enumerate(step):
+                assert not n or torch.allclose(out[r], want[r, at[r]], atol=1e-4), (r, at[r])
+                at[r] += n
+        store = make_cache(m, 3, 64)
+        assert torch.allclose(m(tokens[:, :11], cache=store), want[:, :11], atol=1e-4)
+        for lo, hi in ((11, 18), (18, 20), (20, 21), (21, 24)):
+            assert torch.allclose(m(tokens[:, lo:hi], positions=torch.arange(lo, hi)[None].expand(3, hi - lo), cache=store), want[:, lo:hi], atol=1e-4)
+
+
 @pytest.mark.parametrize("kind", sorted(OPTIONS))
 def test_a_cache_without_a_place_for_a_state_is_refused(kind):
-    """State space layers between attention layers that turn by the model's tables: their store has keys alone.  A cache of states around it serves them."""
-    m = model(kind, num_heads=4, layer_types=(kind, "attention"), layer_mlp=None, mlp_features=96, num_layers=2)
-    assert m.cache_slots() is None
-    with pytest.raises(NotImplementedError, match="no place for its state"):
-        generate(m, None, [[3, 4, 5]], 4, sampling=Sampling(temperature=0.0))
-    with pytest.raises(NotImplementedError, match="no place for its state"):
-        Server(m, slots=2, capacity=64, sampling=Sampling(temperature=0.0))([[3, 4, 5]], 4)
+    """A store of keys alone.  A cache of states around it serves such a stack, in any pieces."""
+    m = between_attention(kind)
+    bare = KVStore(KVCache(), 3, 2, 64, 2, 16, torch.float32, "cpu")
     tokens = torch.randint(1, 97, (2, 20))
-    cache, got = RecurrentCache(make_cache(m, 2, 64)), []
+    with pytest.raises(NotImplementedError, match="no place for its state"):
+        m(tokens, positions=torch.arange(20)[None].expand(2, 20), cache=bare)
+    cache, got = RecurrentCache(bare), []
     with torch.no_grad():
         for lo, hi in ((0, 9), (9, 16), (16, 17), (17, 20)):
             got.append(m(tokens[:, lo:hi], positions=torch.arange(lo, hi)[None].expand(2, hi - lo), cache=cache))
@@ -102,6 +149,37 @@ def test_states_without_memory_in_the_plain_form():
     state = (dt * x).unsqueeze(-1) * b.unsqueeze(2)
     assert torch.allclose(y, (state * c.unsqueeze(2)).sum(-1), atol=1e-5) and torch.allclose(last, state[:, -1], atol=1e-6)
     assert all(g.isfinite().all() for g in torch.autograd.grad(y.sum() + last.sum(), leaves))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_between_attention_layers_on_a_gpu(kind):
+    """fp32 weights, the same tokens as on the CPU."""
+    m, asked = between_attention(kind), prompts()
+    want = [greedy(m, p, 8) for p in asked]
+    m = m.cuda()
+    out = generate(m, None, asked, 8, sampling=Sampling(temperature=0.0))
+    assert [out.tokens[r, len(p):len(p) + 8].tolist() for r, p in enumerate(asked)] == want
+    server = Server(m, slots=3, capacity=256, chunk=64, kv_cache=KVCache(page_size=64), sampling=Sampling(temperature=0.0))
+    assert server(asked, 8) == want and server(asked[::-1], 8) == want[::-1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(OPTIONS))
+def test_steps_between_attention_layers_in_bf16(kind):
+    """Widths that the kernels of attention and of chunks take: as near to fp32 as the whole row in bf16 is; a server's captured steps are its steps."""
+    more = dict(emb_features=256, num_heads=4, num_kv_heads=2, mixer_options=dict(state_dim=128, head_dim=64, groups=1) if kind == "mamba2" else {})
+    m32, m = between_attention(kind, "cuda", **more), between_attention(kind, "cuda", **more).to(torch.bfloat16)
+    m32.load_state_dict({k: v.float() for k, v in m.state_dict().items()})
+    rows = torch.randint(1, 97, (3, 160), device="cuda")
+    batch, pos = RowBatch(m, 3, 256), torch.arange(160, device="cuda")[None].expand(3, -1)
+    with torch.no_grad():
+        exact, whole = m32(rows), m(rows).float()
+        steps = torch.cat([batch.forward(rows[:, :128], pos[:, :128], (0, 128))] + [batch.forward(rows[:, t:t + 1], pos[:, t:t + 1]) for t in range(128, 160)], 1).float()
+    far = lambda a: float((a - exact).norm() / exact.norm())
+    assert far(steps) < 2 * far(whole) + 1e-3 and far(whole) < 0.1
+    plain, graph = (Server(m, slots=2, capacity=256, chunk=64, kv_cache=KVCache(page_size=64), sampling=Sampling(temperature=0.0), cuda_graph=g)(prompts(), 8) for g in (False, True))
+    assert plain == graph
 
 
 @pytest.mark.gpu
